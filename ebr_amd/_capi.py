@@ -131,6 +131,26 @@ SIGNATURES = {
     "ebr_block_swiglu_bwd_add": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int] + [_P] * 5),
     "ebr_block_swiglu_bwd2": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int] + [_P] * 6),
     "ebr_block_split_sum": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64, _F32P, _P, _P]),
+    "ebr_block_embed": (
+        ctypes.c_int,
+        [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [ctypes.c_int, ctypes.c_double] + [_P] * 4,
+    ),
+    "ebr_block_embed_bwd_scratch": (ctypes.c_int64, [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_int]),
+    "ebr_block_embed_bwd": (
+        ctypes.c_int,
+        [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [ctypes.c_int, ctypes.c_double] + [_P] * 5,
+    ),
+    "ebr_block_distill": (
+        ctypes.c_int,
+        [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_int]
+        + [_P] * 8,
+    ),
+    "ebr_block_distill_scratch": (ctypes.c_int64, [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_int]),
+    "ebr_block_distill_bwd": (
+        ctypes.c_int,
+        [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [ctypes.c_int, ctypes.c_int64, ctypes.c_double] + [_P] * 6
+        + [ctypes.c_int64] + [_P] * 2,
+    ),
     "ebr_attn_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ebr_attn_abi_version": (ctypes.c_int, []),
     "ebr_attn_arch": (ctypes.c_char_p, []),

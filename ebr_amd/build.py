@@ -25,7 +25,7 @@ HOST_NAME = "ebr_host.so"
 ARCH = "gfx950"
 
 SOURCES = [CSRC / "ebr_attn.hip", CSRC / "ebr_rope.hip", CSRC / "ebr_descent.hip", CSRC / "ebr_block.hip",
-           CSRC / "ebr_noalloc.hip"]
+           CSRC / "ebr_embed.hip", CSRC / "ebr_distill.hip", CSRC / "ebr_noalloc.hip"]
 HEADERS = [
     CSRC / "attn_tiles.hpp",
     CSRC / "attn_resident.hpp",
@@ -35,6 +35,7 @@ HEADERS = [
     ROOT / "include" / "ebr_descent.h",
     ROOT / "include" / "ebr_block.h",
     CSRC / "attn_f64.hpp",
+    CSRC / "rowwise.hpp",
 ]
 
 

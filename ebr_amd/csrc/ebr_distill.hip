@@ -1,0 +1,372 @@
+// Distillation from a teacher's top logits on gfx950, with its gradient (C ABI: include/ebr_block.h).
+//
+// A row has V logits x of the student and K entries (id, t) of the teacher; an entry counts where id is in [0, V).
+//   p = softmax of the counted t / T,  q = softmax of x / T
+//   loss = T^2 sum_k p_k (log p_k - log q_id_k),   dx_j = g T (q_j - sum over { k : id_k = j } of p_k)
+// A row without an entry of positive probability has loss 0 and gradient 0 and is not counted in the mean.
+//
+// Bound by memory: the forward reads the logits once (running maximum and sum), the backward reads them again and writes
+// the gradient; between them a row keeps four numbers. Exponents are taken of (x - max) (log2 e) / T: the difference of
+// raw logits is exact or nearly so, where x / T would be rounded at the size of x.
+#include <type_traits>
+
+#include "rowwise.hpp"
+
+namespace ebr_distill {
+
+using namespace ebr_row;
+
+constexpr int K_MAX = 1024;  // a row's entries, held in shared memory by the backward
+constexpr double LN2 = 0.6931471805599453, LOG2E = 1.4426950408889634;
+
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ double pow2(double x) { return exp2(x); }
+__device__ __forceinline__ float lg2(float x) { return log2f(x); }
+__device__ __forceinline__ double lg2(double x) { return log2(x); }
+template <typename A> __device__ __forceinline__ A larger(A a, A b) { return a > b ? a : b; }
+template <typename A> __device__ __forceinline__ A lowest() { return (A)-__builtin_inff(); }
+
+struct Args {
+    const void *x, *teacher, *ids;
+    int64_t N, row;  // row: elements from one row of x to the next
+    int V, K, teacher_type, wide;
+    double k;  // log2 e / T
+    double weight;  // forward: T^2 ln 2; backward: T
+    int reduction;
+    void *stats, *loss, *scale, *part;
+    const void* grad;
+    int64_t grad_step;
+    void* dx;
+};
+
+// What a row's softmaxes need: its largest logit and log2 of the sum above it, the teacher's alike. tm is -inf for a row
+// that is not counted.
+template <typename A> struct alignas(4 * sizeof(A)) Stats { A m, s2, tm, ts2; };
+template <typename A> struct Partial { double loss, rows; };
+
+template <typename A> __device__ __forceinline__ A teacher_at(const Args& a, int64_t i) {
+    switch (a.teacher_type) {
+        case EBR_DTYPE_F32: return (A)reinterpret_cast<const float*>(a.teacher)[i];
+        case EBR_DTYPE_BF16: return (A)(float)reinterpret_cast<const __bf16*>(a.teacher)[i];
+        case EBR_DTYPE_F16: return (A)(float)reinterpret_cast<const _Float16*>(a.teacher)[i];
+        default: return (A)reinterpret_cast<const double*>(a.teacher)[i];
+    }
+}
+
+// An entry's column, -1 for one that does not count.
+__device__ __forceinline__ int column(const Args& a, int64_t i) {
+    const int64_t v = a.wide ? reinterpret_cast<const int64_t*>(a.ids)[i] : reinterpret_cast<const int*>(a.ids)[i];
+    return v >= 0 && v < a.V ? (int)v : -1;
+}
+
+// A maximum and the sum of 2^((x - m) k) above it, of parts of a row.
+template <typename A> struct Soft {
+    A m, s;
+    __device__ __forceinline__ void add(A x, A k) {
+        if (x > m) {
+            s *= pow2((m - x) * k);  // 0 from nothing: s is 0 then
+            m = x;
+        }
+        s += m == lowest<A>() ? (x == m ? (A)0 : x) : pow2((x - m) * k);  // nothing but -inf so far: 0, or a NaN
+    }
+    __device__ __forceinline__ void merge(A om, A os, A k) {
+        const A top = larger(m, om);
+        const A base = top == lowest<A>() ? (A)0 : top;
+        s = s * pow2((m - base) * k) + os * pow2((om - base) * k);
+        m = top;
+    }
+};
+
+// Over the TEAM threads of a row: aligned lanes of a wave, or the whole workgroup.
+template <int TEAM, typename A> __device__ __forceinline__ void soft_all(Soft<A>& v, A k, A* lds) {
+    constexpr int W = TEAM < 64 ? TEAM : 64;
+#pragma unroll
+    for (int d = W / 2; d >= 1; d >>= 1) {
+        const A om = __shfl_xor(v.m, d, 64), os = __shfl_xor(v.s, d, 64);
+        v.merge(om, os, k);
+    }
+    if constexpr (TEAM > 64) {
+        constexpr int WAVES = TEAM / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            lds[threadIdx.x >> 6] = v.m;
+            lds[WAVES + (threadIdx.x >> 6)] = v.s;
+        }
+        __syncthreads();
+        v.m = lds[0];
+        v.s = lds[WAVES];
+        for (int w = 1; w < WAVES; ++w) v.merge(lds[w], lds[WAVES + w], k);
+    }
+}
+template <int TEAM, typename A> __device__ __forceinline__ A sum_all(A v, A* lds) {
+    v = lanes_sum<(TEAM < 64 ? TEAM : 64)>(v);
+    if constexpr (TEAM > 64) {
+        constexpr int WAVES = TEAM / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = lds[0];
+        for (int w = 1; w < WAVES; ++w) v += lds[w];
+    }
+    return v;
+}
+
+// The teacher's part of a row, once its student statistics are known: its statistics and the row's loss in units of
+// weight.
+template <typename T, int TEAM, typename A>
+__device__ __forceinline__ A teach(const Args& a, int64_t n, Stats<A>& st, int t, bool on, A* lds) {
+    const A k = (A)a.k;
+    Soft<A> v = {lowest<A>(), 0};
+    if (on)
+        for (int i = t; i < a.K; i += TEAM)
+            if (column(a, n * a.K + i) >= 0) v.add(teacher_at<A>(a, n * a.K + i), k);
+    soft_all<TEAM, A>(v, k, lds);
+    st.tm = v.m;
+    st.ts2 = lg2(v.s);
+    A sum = 0;
+    if (on && !(v.m == lowest<A>() && v.s == (A)0)) {
+        const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
+        for (int i = t; i < a.K; i += TEAM) {
+            const int c = column(a, n * a.K + i);
+            if (c < 0) continue;
+            const A lp = (teacher_at<A>(a, n * a.K + i) - v.m) * k - st.ts2, p = pow2(lp);
+            if (p == (A)0) continue;
+            sum += p * (lp - (((A)x[c] - st.m) * k - st.s2));
+        }
+    }
+    return sum_all<TEAM, A>(sum, lds);
+}
+
+template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_loss(Args a) {
+    using A = typename Acc<T>::type;
+    __shared__ A lds[16];
+    __shared__ double rows[256 / TEAM][2];
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + team;
+    const bool on = n < a.N;
+    const A k = (A)a.k;
+    Soft<A> v = {lowest<A>(), 0};
+    if (on) {
+        const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
+        for (int j = t; j < a.V; j += TEAM) v.add((A)x[j], k);
+    }
+    soft_all<TEAM, A>(v, k, lds);
+    Stats<A> st = {v.m, lg2(v.s), 0, 0};
+    const A sum = teach<T, TEAM, A>(a, n, st, t, on, lds);
+    if (t == 0) {
+        const bool counted = on && !(st.tm == lowest<A>() && st.ts2 == lowest<A>());
+        const A loss = counted ? (A)a.weight * sum : (A)0;
+        if (on) {
+            reinterpret_cast<Stats<A>*>(a.stats)[n] = st;
+            if (a.reduction == EBR_REDUCE_NONE) reinterpret_cast<A*>(a.loss)[n] = loss;
+        }
+        rows[team][0] = (double)loss;
+        rows[team][1] = counted;
+    }
+    if (a.reduction == EBR_REDUCE_NONE) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Partial<A> p = {0, 0};
+        for (int i = 0; i < 256 / TEAM; ++i) {
+            p.loss += rows[i][0];
+            p.rows += rows[i][1];
+        }
+        reinterpret_cast<Partial<A>*>(a.part)[blockIdx.x] = p;
+    }
+}
+
+// The workgroups' sums together, in a fixed order; the mean's factor stays for the backward.
+template <typename A> __global__ __launch_bounds__(256) void k_total(Args a, int64_t parts) {
+    __shared__ double lds[2][4];
+    double loss = 0, rows = 0;
+    const Partial<A>* p = reinterpret_cast<const Partial<A>*>(a.part);
+    for (int64_t i = threadIdx.x; i < parts; i += 256) {
+        loss += p[i].loss;
+        rows += p[i].rows;
+    }
+    loss = lanes_sum<64>(loss);
+    rows = lanes_sum<64>(rows);
+    if ((threadIdx.x & 63) == 0) {
+        lds[0][threadIdx.x >> 6] = loss;
+        lds[1][threadIdx.x >> 6] = rows;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        loss = lds[0][0] + lds[0][1] + lds[0][2] + lds[0][3];
+        rows = lds[1][0] + lds[1][1] + lds[1][2] + lds[1][3];
+        const double f = a.reduction == EBR_REDUCE_SUM ? 1.0 : 1.0 / (rows > 0 ? rows : 1.0);
+        *reinterpret_cast<A*>(a.loss) = (A)(loss * f);
+        *reinterpret_cast<A*>(a.scale) = (A)f;
+    }
+}
+
+// Rows of at most TEAM columns: a thread has a column and goes through the row's entries.
+template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_short(Args a) {
+    using A = typename Acc<T>::type;
+    const int t = threadIdx.x % TEAM;
+    const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    if (n >= a.N || t >= a.V) return;
+    const A k = (A)a.k;
+    const Stats<A> st = reinterpret_cast<const Stats<A>*>(a.stats)[n];
+    A d = 0;
+    if (!(st.tm == lowest<A>() && st.ts2 == lowest<A>())) {
+        A p = 0;
+        for (int i = 0; i < a.K; ++i)
+            if (column(a, n * a.K + i) == t) p += pow2((teacher_at<A>(a, n * a.K + i) - st.tm) * k - st.ts2);
+        A c = reinterpret_cast<const A*>(a.grad)[n * a.grad_step] * (A)a.weight;
+        if (a.scale) c *= *reinterpret_cast<const A*>(a.scale);
+        d = c * (pow2(((A)reinterpret_cast<const T*>(a.x)[n * a.row + t] - st.m) * k - st.s2) - p);
+    }
+    reinterpret_cast<T*>(a.dx)[n * a.V + t] = (T)d;
+}
+
+// A row's columns one after another, each from q alone; then the columns that the teacher names once more, each by the
+// first of its entries, which adds the others of the same column in their order.
+template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Args a) {
+    using A = typename Acc<T>::type;
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    A* prob = reinterpret_cast<A*>(shared) + (int64_t)team * a.K;
+    int* col = reinterpret_cast<int*>(reinterpret_cast<A*>(shared) + (int64_t)(256 / TEAM) * a.K) + (int64_t)team * a.K;
+    const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + team;
+    const bool on = n < a.N;
+    const A k = (A)a.k;
+    Stats<A> st = {};
+    A c = 0;
+    bool counted = false;
+    const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
+    T* dx = reinterpret_cast<T*>(a.dx) + n * a.V;
+    if (on) {
+        st = reinterpret_cast<const Stats<A>*>(a.stats)[n];
+        counted = !(st.tm == lowest<A>() && st.ts2 == lowest<A>());
+        c = reinterpret_cast<const A*>(a.grad)[n * a.grad_step] * (A)a.weight;
+        if (a.scale) c *= *reinterpret_cast<const A*>(a.scale);
+        for (int i = t; i < a.K; i += TEAM) {
+            const int j = column(a, n * a.K + i);
+            col[i] = j;
+            prob[i] = j < 0 ? (A)0 : pow2((teacher_at<A>(a, n * a.K + i) - st.tm) * k - st.ts2);
+        }
+        for (int j = t; j < a.V; j += TEAM)
+            dx[j] = counted ? (T)(c * pow2(((A)x[j] - st.m) * k - st.s2)) : (T)0.f;
+    }
+    __syncthreads();
+    if (!counted) return;
+    for (int i = t; i < a.K; i += TEAM) {
+        const int j = col[i];
+        if (j < 0) continue;
+        A p = 0;
+        bool first = true;
+        for (int o = 0; o < a.K; ++o)
+            if (col[o] == j) {
+                first = first && o >= i;
+                p += prob[o];
+            }
+        if (first) dx[j] = (T)(c * (pow2(((A)x[j] - st.m) * k - st.s2) - p));
+    }
+}
+
+// Threads of a row: as many lanes as it has columns, up to a wave, and a workgroup for long rows.
+static int team_of(int64_t V) {
+    if (V > 2048) return 256;
+    int t = 8;
+    while (t < 64 && t < V) t *= 2;
+    return t;
+}
+
+static int64_t groups(int64_t N, int team) { return (N + 256 / team - 1) / (256 / team); }
+
+static int check(int dtype, int tdtype, int64_t N, int64_t V, int K, int64_t row, double T) {
+    for (const int d : {dtype, tdtype})
+        if (d != EBR_DTYPE_F32 && d != EBR_DTYPE_BF16 && d != EBR_DTYPE_F16 && d != EBR_DTYPE_F64) return EBR_ERR_DTYPE;
+    if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V >= ((int64_t)1 << 30) || K < 1 || K > K_MAX || row < V ||
+        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T > 0) || T > 1e30 || T < 1e-30 || groups(N, team_of(V)) > MAX_BLOCKS)
+        return EBR_ERR_SHAPE;
+    return EBR_OK;
+}
+
+template <typename F> static int by_type(int dtype, F f) {
+    switch (dtype) {
+        case EBR_DTYPE_F32: return f(float());
+        case EBR_DTYPE_BF16: return f(__bf16());
+        case EBR_DTYPE_F16: return f(_Float16());
+        default: return f(double());
+    }
+}
+
+template <typename F> static void by_team(int team, F f) {
+    switch (team) {
+        case 8: f(std::integral_constant<int, 8>()); break;
+        case 16: f(std::integral_constant<int, 16>()); break;
+        case 32: f(std::integral_constant<int, 32>()); break;
+        case 64: f(std::integral_constant<int, 64>()); break;
+        default: f(std::integral_constant<int, 256>()); break;
+    }
+}
+
+}  // namespace ebr_distill
+
+using namespace ebr_distill;
+
+extern "C" {
+
+int64_t ebr_block_distill_scratch(int dtype, int64_t N, int64_t V, int K) {
+    if (check(dtype, dtype, N, V, K, V, 1.0)) return -1;
+    return groups(N, team_of(V)) * (int64_t)sizeof(Partial<float>);
+}
+
+int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride, double temperature,
+                      int reduction, const void* logits, const void* teacher, const void* ids, void* stats, void* loss,
+                      void* scale, void* scratch, void* stream) {
+    const int rc = check(dtype, tdtype, N, V, K, row_stride, temperature);
+    if (rc) return rc;
+    if (reduction != EBR_REDUCE_NONE && reduction != EBR_REDUCE_SUM && reduction != EBR_REDUCE_MEAN) return EBR_ERR_SHAPE;
+    const bool one = reduction != EBR_REDUCE_NONE;
+    if ((N > 0 && (!logits || !teacher || !ids || !stats)) || ((N > 0 || one) && !loss) || (one && !scale))
+        return EBR_ERR_NULL;
+    if (one && N > 0 && !scratch) return EBR_ERR_SCRATCH;
+    if (!aligned(stats, 16) || !aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature,
+              temperature * temperature * LN2, reduction, stats, loss, scale, scratch};
+    hipStream_t s = (hipStream_t)stream;
+    return by_type(dtype, [&](auto v) {
+        using T = decltype(v);
+        const int team = team_of(V);
+        if (N > 0)
+            by_team(team, [&](auto w) {
+                hipLaunchKernelGGL((k_loss<T, decltype(w)::value>), dim3((unsigned)groups(N, team)), dim3(256), 0, s, a);
+            });
+        if (one) hipLaunchKernelGGL((k_total<typename Acc<T>::type>), dim3(1), dim3(256), 0, s, a, groups(N, team));
+        return launched();
+    });
+}
+
+int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride,
+                          double temperature, const void* logits, const void* teacher, const void* ids, const void* stats,
+                          const void* scale, const void* grad, int64_t grad_stride, void* dx, void* stream) {
+    const int rc = check(dtype, tdtype, N, V, K, row_stride, temperature);
+    if (rc) return rc;
+    if (grad_stride != 0 && grad_stride != 1) return EBR_ERR_SHAPE;
+    if (N == 0) return EBR_OK;
+    if (!logits || !teacher || !ids || !stats || !grad || !dx) return EBR_ERR_NULL;
+    if (!aligned(stats, 16)) return EBR_ERR_ALIGN;
+    Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature, temperature,
+              EBR_REDUCE_NONE, const_cast<void*>(stats), nullptr, const_cast<void*>(scale), nullptr, grad, grad_stride, dx};
+    return by_type(dtype, [&](auto v) {
+        using T = decltype(v);
+        using A = typename Acc<T>::type;
+        const int team = team_of(V);
+        const size_t lds = (size_t)(256 / team) * K * (sizeof(A) + sizeof(int));
+        by_team(team, [&](auto w) {
+            constexpr int TEAM = decltype(w)::value;
+            if constexpr (TEAM < 64)
+                hipLaunchKernelGGL((k_grad_short<T, TEAM>), dim3((unsigned)groups(N, team)), dim3(256), 0,
+                                   (hipStream_t)stream, a);
+            else
+                hipLaunchKernelGGL((k_grad<T, TEAM>), dim3((unsigned)groups(N, team)), dim3(256), lds,
+                                   (hipStream_t)stream, a);
+        });
+        return launched();
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,465 @@
+// Embedding of tokens and its table's gradient on gfx950 (C ABI: include/ebr_block.h).
+//
+//   y[n, :]  = round(s w[id_n, :]), a row of zeros where id_n lies outside [0, V)
+//   dw[v, :] = round(s sum over { n : id_n = v } of dy[n, :]), every row of the table written
+//
+// Both are bound by memory. The lookup reads the tokens' rows and writes y. The gradient has to read dy once and to write
+// the whole table, most of it zeros for text; what costs is bringing a token's rows together. Atomic sums would do that in
+// an order that changes from run to run, so the positions are sorted by token instead (a stable radix sort: equal tokens
+// keep their order), and a sum always adds the same rows in the same order, in 32 bits.
+#include "rowwise.hpp"
+
+namespace ebr_embed {
+
+using namespace ebr_row;
+
+struct Ids {
+    const void* p;
+    int wide;  // 64-bit tokens
+    int V;
+};
+
+// A position's token, V for one outside the table.
+__device__ __forceinline__ uint32_t token(const Ids& ids, int64_t n) {
+    if (ids.wide) {
+        const int64_t v = reinterpret_cast<const int64_t*>(ids.p)[n];
+        return v >= 0 && v < ids.V ? (uint32_t)v : (uint32_t)ids.V;
+    }
+    const int v = reinterpret_cast<const int*>(ids.p)[n];
+    return v >= 0 && v < ids.V ? (uint32_t)v : (uint32_t)ids.V;
+}
+
+// -- lookup ------------------------------------------------------------------------------------------------------------
+
+template <typename TW, typename TY, int VEC>
+__global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, double scale, const TW* w, TY* y) {
+    using A = typename Acc<TW>::type;
+    const int64_t CV = C / VEC, total = N * CV;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t n = i / CV;
+        const int64_t c = (i - n * CV) * VEC;
+        const uint32_t v = token(ids, n);
+        Pack<TY, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.e[e] = (TY)0.f;
+        if (v < (uint32_t)ids.V) {
+            const TW* row = w + (int64_t)v * C + c;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o.e[e] = (TY)((A)row[e] * (A)scale);
+        }
+        stp<TY, VEC>(y + n * C + c, o);
+    }
+}
+
+// -- positions sorted by token -----------------------------------------------------------------------------------------
+
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_KEYS = 4;
+constexpr int SORT_TILE = SORT_THREADS * SORT_KEYS;  // positions that a workgroup ranks at a time
+constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS;
+constexpr int SORT_GROUPS = 256;  // workgroups of a sort at most: each reads all the others' counts
+
+struct SortArgs {
+    Ids ids;                     // read where kin is null
+    const uint32_t *kin, *pin;   // tokens and positions
+    uint32_t *kout, *pout;
+    uint32_t* counts;            // [groups][SORT_DIGITS]
+    int N, shift, bits, tiles;   // tiles: of each workgroup
+};
+
+// The lanes of this wave that hold the same digit.
+__device__ __forceinline__ uint64_t alike(uint32_t digit, int bits, bool valid) {
+    uint64_t m = __ballot(valid);
+    for (int b = 0; b < bits; ++b) {
+        const bool on = (digit >> b) & 1;
+        const uint64_t s = __ballot(on);
+        m &= on ? s : ~s;
+    }
+    return m;
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_count(SortArgs a) {
+    __shared__ uint32_t count[SORT_DIGITS];
+    for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) count[d] = 0;
+    __syncthreads();
+    const int64_t from = (int64_t)blockIdx.x * a.tiles * SORT_TILE;
+    const int64_t to = from + (int64_t)a.tiles * SORT_TILE < a.N ? from + (int64_t)a.tiles * SORT_TILE : a.N;
+    for (int64_t i = from + threadIdx.x; i < to; i += SORT_THREADS) {
+        const uint32_t k = a.kin ? a.kin[i] : token(a.ids, i);
+        atomicAdd(&count[(k >> a.shift) & ((1u << a.bits) - 1)], 1u);  // whole numbers: the order does not matter
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) a.counts[(int64_t)blockIdx.x * SORT_DIGITS + d] = count[d];
+}
+
+// Exclusive prefix sums of v over SORT_DIGITS threads (the first ones of the workgroup), by wave and then over the waves.
+__device__ __forceinline__ uint32_t digits_before(uint32_t v, uint32_t* waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t s = v;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t o = __shfl_up(s, m, 64);
+        if (lane >= m) s += o;
+    }
+    if (lane == 63) waves[wave] = s;
+    __syncthreads();
+    uint32_t base = 0;
+    for (int w = 0; w < wave && w < SORT_DIGITS / 64; ++w) base += waves[w];
+    return base + s - v;
+}
+
+// Ranks of a tile's keys among those with the same digit that come before them: count[wave][digit] ends as the number in
+// the waves before, rank[k] as the number before in the wave. Positions run by wave, then by k, then by lane.
+__device__ __forceinline__ void rank_tile(const uint32_t (&key)[SORT_KEYS], const bool (&valid)[SORT_KEYS], int shift,
+                                          int bits, uint32_t (*count)[SORT_DIGITS], uint32_t (&rank)[SORT_KEYS]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = lane; d < SORT_DIGITS; d += 64) count[wave][d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SORT_KEYS; ++k) {
+        const uint32_t digit = (key[k] >> shift) & ((1u << bits) - 1);
+        const uint64_t same = alike(digit, bits, valid[k]);
+        const int first = same ? __ffsll((unsigned long long)same) - 1 : 0;
+        uint32_t old = 0;
+        if (valid[k] && lane == first) old = atomicAdd(&count[wave][digit], (uint32_t)__popcll(same));
+        rank[k] = __shfl(old, first, 64) + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_place(SortArgs a) {
+    __shared__ uint32_t count[SORT_WAVES][SORT_DIGITS];
+    __shared__ uint32_t start[SORT_DIGITS], waves[SORT_WAVES];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint32_t before = 0, total = 0;
+    if (t < SORT_DIGITS) {
+        for (int g = 0; g < (int)gridDim.x; ++g) {
+            const uint32_t c = a.counts[(int64_t)g * SORT_DIGITS + t];
+            total += c;
+            if (g < (int)blockIdx.x) before += c;
+        }
+    }
+    const uint32_t base = digits_before(total, waves);
+    if (t < SORT_DIGITS) start[t] = base + before;
+    for (int tile = 0; tile < a.tiles; ++tile) {
+        const int64_t at = ((int64_t)blockIdx.x * a.tiles + tile) * SORT_TILE + wave * (SORT_KEYS * 64) + lane;
+        uint32_t key[SORT_KEYS], pos[SORT_KEYS], rank[SORT_KEYS];
+        bool valid[SORT_KEYS];
+#pragma unroll
+        for (int k = 0; k < SORT_KEYS; ++k) {
+            const int64_t i = at + k * 64;
+            valid[k] = i < a.N;
+            key[k] = valid[k] ? (a.kin ? a.kin[i] : token(a.ids, i)) : 0;
+            pos[k] = valid[k] ? (a.kin ? a.pin[i] : (uint32_t)i) : 0;
+        }
+        rank_tile(key, valid, a.shift, a.bits, count, rank);
+        uint32_t sum = 0, s0 = 0;
+        if (t < SORT_DIGITS) {
+            s0 = start[t];
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                const uint32_t c = count[w][t];
+                count[w][t] = s0 + sum;
+                sum += c;
+            }
+            start[t] = s0 + sum;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < SORT_KEYS; ++k) {
+            if (!valid[k]) continue;
+            const uint32_t to = count[wave][(key[k] >> a.shift) & ((1u << a.bits) - 1)] + rank[k];
+            a.kout[to] = key[k];
+            a.pout[to] = pos[k];
+        }
+        __syncthreads();
+    }
+}
+
+// Up to a tile of positions: every pass in one workgroup, the keys going round through shared memory.
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_tile(SortArgs a, int passes) {
+    __shared__ uint32_t count[SORT_WAVES][SORT_DIGITS];
+    __shared__ uint32_t keys[SORT_TILE], waves[SORT_WAVES];
+    __shared__ uint16_t places[SORT_TILE];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, at = wave * (SORT_KEYS * 64) + lane;
+    uint32_t key[SORT_KEYS], pos[SORT_KEYS], rank[SORT_KEYS];
+    bool valid[SORT_KEYS];
+#pragma unroll
+    for (int k = 0; k < SORT_KEYS; ++k) {
+        valid[k] = at + k * 64 < a.N;
+        key[k] = valid[k] ? token(a.ids, at + k * 64) : 0;
+        pos[k] = at + k * 64;
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * a.bits;
+        rank_tile(key, valid, shift, a.bits, count, rank);
+        uint32_t sum = 0;
+        if (t < SORT_DIGITS)
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                const uint32_t c = count[w][t];
+                count[w][t] = sum;
+                sum += c;
+            }
+        const uint32_t base = digits_before(sum, waves);
+        if (t < SORT_DIGITS)
+            for (int w = 0; w < SORT_WAVES; ++w) count[w][t] += base;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < SORT_KEYS; ++k) {
+            if (!valid[k]) continue;
+            const uint32_t to = count[wave][(key[k] >> shift) & ((1u << a.bits) - 1)] + rank[k];
+            keys[to] = key[k];
+            places[to] = (uint16_t)pos[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < SORT_KEYS; ++k) {
+            if (!valid[k]) continue;
+            key[k] = keys[at + k * 64];
+            pos[k] = places[at + k * 64];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < SORT_KEYS; ++k) {
+        if (!valid[k]) continue;
+        a.kout[at + k * 64] = key[k];
+        a.pout[at + k * 64] = pos[k];
+    }
+}
+
+// -- sums of equal tokens' rows ----------------------------------------------------------------------------------------
+
+struct SumArgs {
+    const uint32_t *key, *pos;  // sorted
+    const void* dy;
+    void* dw;
+    void* part;  // [chunks][2][C]: a chunk's share of a run from the chunk before (0), and of one that goes on (1)
+    int N, V, C, chunk, chunks, zero_rows;
+    unsigned sum_blocks;
+    double scale;
+};
+
+template <typename A, typename TW, int VEC>
+__device__ __forceinline__ void put_row(TW* p, const A (&acc)[VEC], double scale) {
+    Pack<TW, VEC> o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o.e[e] = (TW)(acc[e] * (A)scale);
+    stp<TW, VEC>(p, o);
+}
+
+// The first workgroups sum: a wave takes a chunk of the sorted positions and 64 VEC columns. A run of equal tokens inside
+// the chunk is written to the table at once; a run over its border goes to part. The others write zeros to the rows of
+// tokens that do not occur, found by bisection.
+template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_sum(SumArgs a) {
+    using A = typename Acc<TW>::type;
+    const int lane = threadIdx.x & 63;
+    TW* dw = reinterpret_cast<TW*>(a.dw);
+    if (blockIdx.x >= a.sum_blocks) {
+        __shared__ uint8_t absent[256];
+        const int64_t r0 = (int64_t)(blockIdx.x - a.sum_blocks) * a.zero_rows;
+        const int rows = (int)(a.V - r0 < a.zero_rows ? a.V - r0 : a.zero_rows);
+        if ((int)threadIdx.x < rows) {
+            const uint32_t v = (uint32_t)(r0 + threadIdx.x);
+            int lo = 0, hi = a.N;  // the first position whose token is v or more
+            while (lo < hi) {
+                const int mid = lo + (hi - lo) / 2;
+                if (a.key[mid] < v) lo = mid + 1;
+                else hi = mid;
+            }
+            absent[threadIdx.x] = !(lo < a.N && a.key[lo] == v);
+        }
+        __syncthreads();
+        const int CV = a.C / VEC;
+        const Pack<TW, VEC> zero = {};
+        for (int r = 0; r < rows; ++r) {
+            if (!absent[r]) continue;
+            for (int c = threadIdx.x; c < CV; c += 256) stp<TW, VEC>(dw + (r0 + r) * a.C + (int64_t)c * VEC, zero);
+        }
+        return;
+    }
+    const int tiles = (a.C + 64 * VEC - 1) / (64 * VEC);
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (int64_t)a.chunks * tiles) return;  // wave-uniform
+    const int chunk = (int)(item / tiles), c = (int)(item % tiles) * 64 * VEC + lane * VEC;
+    const int from = chunk * a.chunk, to = from + a.chunk < a.N ? from + a.chunk : a.N;
+    const bool on = c < a.C;
+    const TY* dy = reinterpret_cast<const TY*>(a.dy) + c;
+    A* part = reinterpret_cast<A*>(a.part) + (int64_t)chunk * 2 * a.C + c;
+    const uint32_t before = from > 0 ? a.key[from - 1] : (uint32_t)a.V, after = to < a.N ? a.key[to] : (uint32_t)a.V;
+    A acc[VEC];
+    uint32_t cur = a.key[from];
+    bool opened = cur == before;  // the run came from the chunk before
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0;
+    const auto close = [&](bool goes_on) {
+        if (!on || cur >= (uint32_t)a.V) return;
+        if (opened || goes_on) {
+            A* p = part + (opened ? 0 : a.C);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+        } else {
+            put_row<A, TW, VEC>(dw + (int64_t)cur * a.C + c, acc, a.scale);
+        }
+    };
+    for (int i = from; i < to; ++i) {
+        const uint32_t k = a.key[i];
+        if (k >= (uint32_t)a.V) break;  // positions without a token come last
+        if (k != cur) {
+            close(false);
+            cur = k;
+            opened = false;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] = 0;
+        }
+        if (on) {
+            const Pack<TY, VEC> v = ldp<TY, VEC>(dy + (int64_t)a.pos[i] * a.C);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += (A)v.e[e];
+        }
+    }
+    close(cur == after);
+}
+
+// Runs over chunks' borders: the wave of the chunk in which a run begins adds its parts in order.
+template <typename TW, int VEC> __global__ __launch_bounds__(256) void k_join(SumArgs a) {
+    using A = typename Acc<TW>::type;
+    const int lane = threadIdx.x & 63, tiles = (a.C + 64 * VEC - 1) / (64 * VEC);
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (int64_t)(a.chunks - 1) * tiles) return;  // wave-uniform; the last chunk opens nothing
+    const int chunk = (int)(item / tiles), c = (int)(item % tiles) * 64 * VEC + lane * VEC;
+    const int from = chunk * a.chunk, next = from + a.chunk;
+    const uint32_t k = a.key[next - 1];
+    if (k >= (uint32_t)a.V || a.key[next] != k) return;                 // nothing goes on
+    if (a.key[from] == k && from > 0 && a.key[from - 1] == k) return;   // it began before this chunk
+    if (c >= a.C) return;
+    const A* part = reinterpret_cast<const A*>(a.part) + c;
+    A acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = part[((int64_t)chunk * 2 + 1) * a.C + e];
+    for (int j = chunk + 1; j < a.chunks && a.key[j * a.chunk] == k; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += part[(int64_t)j * 2 * a.C + e];
+    put_row<A, TW, VEC>(reinterpret_cast<TW*>(a.dw) + (int64_t)k * a.C + c, acc, a.scale);
+}
+
+// -- launches ----------------------------------------------------------------------------------------------------------
+
+static bool types_ok(int wt, int yt) {
+    const bool known = wt == EBR_DTYPE_F32 || wt == EBR_DTYPE_BF16 || wt == EBR_DTYPE_F16 || wt == EBR_DTYPE_F64;
+    return known && (wt == yt || (wt == EBR_DTYPE_F32 && (yt == EBR_DTYPE_BF16 || yt == EBR_DTYPE_F16)));
+}
+
+static int check(int wt, int yt, int64_t N, int64_t V, int64_t C) {
+    if (!types_ok(wt, yt)) return EBR_ERR_DTYPE;
+    if (N < 0 || N >= ((int64_t)1 << 31) - SORT_TILE || V < 1 || V >= ((int64_t)1 << 31) - 1 || C < 1 ||
+        C >= (1 << 18) || N * C >= ((int64_t)1 << 40) || V * C >= ((int64_t)1 << 40))
+        return EBR_ERR_SHAPE;
+    return EBR_OK;
+}
+
+template <typename F> static int by_types(int wt, int yt, F f) {
+    if (wt == EBR_DTYPE_F32 && yt == EBR_DTYPE_F32) return f(float(), float());
+    if (wt == EBR_DTYPE_F32 && yt == EBR_DTYPE_BF16) return f(float(), __bf16());
+    if (wt == EBR_DTYPE_F32) return f(float(), _Float16());
+    if (wt == EBR_DTYPE_BF16) return f(__bf16(), __bf16());
+    if (wt == EBR_DTYPE_F16) return f(_Float16(), _Float16());
+    return f(double(), double());
+}
+
+constexpr int CHUNK = 64, MAX_CHUNKS = 4096;
+
+struct Plan {
+    int passes, bits, groups, tiles, chunk, chunks;
+    int64_t words, part;  // 32-bit words of keys and positions (both halves) and counts; elements of part
+    Plan(int64_t N, int64_t V, int64_t C) {
+        int width = 1;
+        while ((V >> width) != 0) ++width;  // the tokens 0 .. V
+        passes = (width + SORT_BITS - 1) / SORT_BITS;
+        bits = (width + passes - 1) / passes;
+        const int64_t all = (N + SORT_TILE - 1) / SORT_TILE;
+        tiles = (int)((all + SORT_GROUPS - 1) / SORT_GROUPS);
+        groups = tiles ? (int)((all + tiles - 1) / tiles) : 0;
+        chunk = CHUNK;
+        while ((N + chunk - 1) / chunk > MAX_CHUNKS) chunk *= 2;
+        chunks = (int)((N + chunk - 1) / chunk);
+        words = 4 * N + (int64_t)groups * SORT_DIGITS;
+        words = (words + 3) / 4 * 4;
+        part = (int64_t)chunks * 2 * C;
+    }
+};
+
+template <typename TW, typename TY, int VEC> static void launch_sums(hipStream_t s, const SumArgs& a, int64_t zeros) {
+    hipLaunchKernelGGL((k_sum<TW, TY, VEC>), dim3((unsigned)(a.sum_blocks + zeros)), dim3(256), 0, s, a);
+    if (a.chunks > 1) {
+        const int64_t tiles = (a.C + 64 * VEC - 1) / (64 * VEC);
+        hipLaunchKernelGGL((k_join<TW, VEC>), dim3((unsigned)(((a.chunks - 1) * tiles + 3) / 4)), dim3(256), 0, s, a);
+    }
+}
+
+}  // namespace ebr_embed
+
+using namespace ebr_embed;
+
+extern "C" {
+
+int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int C, double scale, const void* ids,
+                    const void* w, void* y, void* stream) {
+    const int rc = check(wdtype, ydtype, N, V, C);
+    if (rc) return rc;
+    if (!ids || !w || !y) return EBR_ERR_NULL;
+    if (N == 0) return EBR_OK;
+    const Ids i = {ids, ids64 != 0, (int)V};
+    return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
+        using TW = decltype(tw);
+        using TY = decltype(ty);
+        hipLaunchKernelGGL((k_lookup<TW, TY, 1>), dim3(blocks_for(N * C, 256)), dim3(256), 0, (hipStream_t)stream, i, N, C,
+                           scale, (const TW*)w, (TY*)y);
+        return launched();
+    });
+}
+
+int64_t ebr_block_embed_bwd_scratch(int wdtype, int64_t N, int64_t V, int C) {
+    if (check(wdtype, wdtype, N, V, C)) return -1;
+    const Plan p(N, V, C);
+    return p.words * 4 + p.part * (wdtype == EBR_DTYPE_F64 ? 8 : 4);
+}
+
+int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int C, double scale, const void* ids,
+                        const void* dy, void* dw, void* scratch, void* stream) {
+    const int rc = check(wdtype, ydtype, N, V, C);
+    if (rc) return rc;
+    if (!dw || (N > 0 && (!ids || !dy))) return EBR_ERR_NULL;
+    if (N > 0 && !scratch) return EBR_ERR_SCRATCH;
+    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    const Plan p(N, V, C);
+    uint32_t* w32 = reinterpret_cast<uint32_t*>(scratch);
+    uint32_t *k0 = w32, *p0 = w32 + N, *k1 = w32 + 2 * N, *p1 = w32 + 3 * N, *counts = w32 + 4 * N;
+    SortArgs so = {{ids, ids64 != 0, (int)V}, nullptr, nullptr, k0, p0, counts, (int)N, 0, p.bits, p.tiles};
+    if (N > 0 && N <= SORT_TILE) {
+        hipLaunchKernelGGL(k_sort_tile, dim3(1), dim3(SORT_THREADS), 0, s, so, p.passes);
+    } else if (N > 0) {
+        for (int i = 0; i < p.passes; ++i) {
+            so.shift = i * p.bits;
+            hipLaunchKernelGGL(k_sort_count, dim3(p.groups), dim3(SORT_THREADS), 0, s, so);
+            hipLaunchKernelGGL(k_sort_place, dim3(p.groups), dim3(SORT_THREADS), 0, s, so);
+            so.kin = so.kout;
+            so.pin = so.pout;
+            so.kout = so.kout == k0 ? k1 : k0;
+            so.pout = so.pout == p0 ? p1 : p0;
+        }
+    }
+    const bool swapped = N > SORT_TILE && p.passes % 2 == 0;
+    return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
+        using TW = decltype(tw);
+        using TY = decltype(ty);
+        SumArgs a = {swapped ? k1 : k0, swapped ? p1 : p0, dy, dw, w32 + p.words, (int)N, (int)V, C, p.chunk, p.chunks,
+                     0, 0, scale};
+        a.zero_rows = 64;
+        while (a.zero_rows < 256 && V / a.zero_rows > (1 << 22)) a.zero_rows *= 2;
+        const int64_t tiles = (C + 63) / 64;
+        a.sum_blocks = (unsigned)((p.chunks * tiles + 3) / 4);
+        launch_sums<TW, TY, 1>(s, a, (V + a.zero_rows - 1) / a.zero_rows);
+        return launched();
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,44 @@
+// What the row-wise kernels of the token ends and of the group norm share: accumulation types, 16-byte vectors, sums and
+// maxima over a wave or a part of one.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ebr_block.h"
+
+namespace ebr_row {
+
+template <typename T> struct Acc { using type = float; };
+template <> struct Acc<double> { using type = double; };
+
+// N consecutive elements, loaded and stored whole (N * sizeof(T) a power of two, at most 16 bytes, and so aligned).
+template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T e[N]; };
+
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> ldp(const T* p) {
+    return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <typename T, int N> __device__ __forceinline__ void stp(T* p, const Pack<T, N>& v) {
+    *reinterpret_cast<Pack<T, N>*>(p) = v;
+}
+
+// Over aligned parts of W lanes of a wave.
+template <int W, typename A> __device__ __forceinline__ A lanes_sum(A v) {
+#pragma unroll
+    for (int m = W / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+
+static inline int launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? EBR_OK : EBR_ERR_HIP_BASE + (int)e;
+}
+
+static inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+constexpr int64_t MAX_BLOCKS = ((int64_t)1 << 24) - 1;  // of 256 threads: a launch holds fewer than 2^32 threads
+static inline unsigned blocks_for(int64_t n, int64_t per) {
+    const int64_t want = (n + per - 1) / per;
+    return (unsigned)(want < MAX_BLOCKS ? want : MAX_BLOCKS);
+}
+
+}  // namespace ebr_row

@@ -1,6 +1,7 @@
 /* C ABI of the energy network's fused pointwise blocks in libebr_attn.so (gfx950): rms_norm over the last dimension
  * and the SwiGLU activation, each with its backward and the backward of that backward, as the graded latent descent
- * differentiates the energy twice.
+ * differentiates the energy twice; and the ends of a training step, the embedding of tokens with its table's gradient and
+ * the distillation loss with its gradient.
  *
  * Tensors are contiguous rows of one dtype (EBR_DTYPE_F32, _BF16, _F16 or _F64). Arithmetic is fp32 (fp64 for fp64);
  * outputs are rounded once to the dtype. Conventions otherwise as in ebr_attn.h (error codes, streams, ownership).
@@ -53,6 +54,42 @@ int ebr_block_swiglu_bwd2(int dtype, int64_t rows, int I, const void* gu, const 
 
 /* out[i] = round(sum over s of part[s][i]) of S (2, 4, 8 or 16) fp32 partial products [S, n]; out in bf16 or fp16. */
 int ebr_block_split_sum(int dtype, int S, int64_t n, const float* part, void* out, void* stream);
+
+/* y[n, :] = round(scale * w[ids[n], :]) for N tokens and a table w [V, C], contiguous; a row of zeros for a token outside
+ * [0, V). ids: int64 where ids64, else int32. wdtype and ydtype are equal, or fp32 and a 16-bit type. N below 2^31 - 4096,
+ * C below 2^18. */
+int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int C, double scale, const void* ids,
+                    const void* w, void* y, void* stream);
+
+/* Bytes of scratch that ebr_block_embed_bwd needs (16-byte aligned), -1 for sizes or types that it refuses. */
+int64_t ebr_block_embed_bwd_scratch(int wdtype, int64_t N, int64_t V, int C);
+
+/* dw[v, :] = round(scale * sum of dy[n, :] over the n with ids[n] = v): the whole [V, C], rows without a token as zeros.
+ * Sums are fp32 (fp64 for fp64), always in the same order. */
+int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int C, double scale, const void* ids,
+                        const void* dy, void* dw, void* scratch, void* stream);
+
+/* How rows' losses go together. */
+enum { EBR_REDUCE_NONE = 0, EBR_REDUCE_SUM = 1, EBR_REDUCE_MEAN = 2 };
+
+/* Distillation from the K (at most 1024) top logits of a teacher: with p the softmax of a row's teacher / T over the
+ * entries whose ids lie in [0, V), and q the softmax of its logits / T, loss = T^2 sum_k p_k (log p_k - log q_id_k). A row
+ * without an entry of positive probability has loss 0 and is not counted in the mean (0 if none is).
+ * logits: N rows of V, row_stride elements apart; teacher (of tdtype) and ids (int64 where ids64, else int32): contiguous
+ * [N, K]. loss: fp32 (fp64 for fp64 logits), [N] for EBR_REDUCE_NONE, else one. stats: [N, 4] of loss's type, 16-byte
+ * aligned, and scale: one of it (not for EBR_REDUCE_NONE), both for the backward. */
+int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride, double temperature,
+                      int reduction, const void* logits, const void* teacher, const void* ids, void* stats, void* loss,
+                      void* scale, void* scratch, void* stream);
+
+/* Bytes of scratch that ebr_block_distill needs (16-byte aligned), -1 for sizes or types that it refuses. */
+int64_t ebr_block_distill_scratch(int dtype, int64_t N, int64_t V, int K);
+
+/* dx [N, V], contiguous, of that loss given its gradient (of loss's type; grad_stride 0: one, 1: one a row). scale: as the
+ * forward left it, NULL for EBR_REDUCE_NONE. */
+int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride,
+                          double temperature, const void* logits, const void* teacher, const void* ids, const void* stats,
+                          const void* scale, const void* grad, int64_t grad_stride, void* dx, void* stream);
 
 #ifdef __cplusplus
 }
