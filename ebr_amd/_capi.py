@@ -151,6 +151,22 @@ SIGNATURES = {
         [ctypes.c_int] * 3 + [ctypes.c_int64] * 2 + [ctypes.c_int, ctypes.c_int64, ctypes.c_double] + [_P] * 6
         + [ctypes.c_int64] + [_P] * 2,
     ),
+    "ebr_block_groupnorm": (
+        ctypes.c_int,
+        [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 2 + [ctypes.c_double] + [_P] * 7,
+    ),
+    "ebr_block_groupnorm_bwd": (
+        ctypes.c_int,
+        [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 2 + [_P] * 10,
+    ),
+    "ebr_block_groupnorm_bwd2": (
+        ctypes.c_int,
+        [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 2 + [_P] * 14,
+    ),
+    "ebr_block_groupnorm_scratch": (
+        ctypes.c_int64,
+        [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 2,
+    ),
     "ebr_attn_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ebr_attn_abi_version": (ctypes.c_int, []),
     "ebr_attn_arch": (ctypes.c_char_p, []),

@@ -24,7 +24,16 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from ebr_amd.layers import RMS_NORM_EPS, CastedLinear, RopeFused, RotaryTable2D, SwiGLU, apply_rope, rms_norm
+from ebr_amd.layers import (
+    RMS_NORM_EPS,
+    CastedLinear,
+    RopeFused,
+    RotaryTable2D,
+    SwiGLU,
+    apply_rope,
+    group_norm,
+    rms_norm,
+)
 
 Tensor = torch.Tensor
 AttnFn = Callable[[Tensor, Tensor, Tensor], Tensor]
@@ -387,7 +396,10 @@ class EnergyAttention(nn.Module):
 
 
 class EnergyReasoningBlock(nn.Module):
-    """Post-norm block: h <- rms_norm(h + sublayer(h)) for the attention, then for the SwiGLU MLP."""
+    """Post-norm block: h <- rms_norm(h + sublayer(h)) for the attention, then for the SwiGLU MLP. ``norm="group"`` takes a
+    group norm over the board's cells (``norm_groups`` groups of channels) in rms_norm's place."""
+
+    norm = "rms"  # on the class: a whole module unpickled from before it existed has no such attribute
 
     def __init__(self, config: Any) -> None:
         super().__init__()
@@ -395,11 +407,22 @@ class EnergyReasoningBlock(nn.Module):
         if hidden % heads:
             raise ValueError(f"hidden_size {hidden} does not split into {heads} heads")
         self.block_impl = getattr(config, "block_impl", "eager")
+        self.norm, self.norm_groups = getattr(config, "norm", "rms"), getattr(config, "norm_groups", 1)
+        if self.norm not in ("rms", "group"):
+            raise ValueError(f"norm must be 'rms' or 'group', got {self.norm!r}")
+        if self.norm == "group" and (self.norm_groups < 1 or hidden % self.norm_groups):
+            raise ValueError(f"hidden_size {hidden} does not split into {self.norm_groups} norm groups")
         self.self_attn = EnergyAttention(hidden, hidden // heads, heads, backend=config.attn_backend,
                                          nograd_backend=config.attn_nograd_backend)
         self.mlp = SwiGLU(hidden_size=hidden, expansion=config.expansion, impl=self.block_impl)
 
     def _add_norm(self, h: Tensor, r: Tensor) -> Tensor:
+        if self.norm == "group":
+            if self.block_impl == "fused":
+                from ebr_amd import block
+
+                return block.group_norm(h + r, self.norm_groups, eps=RMS_NORM_EPS)
+            return group_norm(h + r, self.norm_groups, RMS_NORM_EPS)
         if self.block_impl == "fused":  # rms_norm with its first and second derivatives as HIP kernels
             from ebr_amd import block
 

@@ -25,7 +25,8 @@ HOST_NAME = "ebr_host.so"
 ARCH = "gfx950"
 
 SOURCES = [CSRC / "ebr_attn.hip", CSRC / "ebr_rope.hip", CSRC / "ebr_descent.hip", CSRC / "ebr_block.hip",
-           CSRC / "ebr_embed.hip", CSRC / "ebr_distill.hip", CSRC / "ebr_noalloc.hip"]
+           CSRC / "ebr_embed.hip", CSRC / "ebr_distill.hip", CSRC / "ebr_groupnorm.hip",
+           CSRC / "ebr_noalloc.hip"]
 HEADERS = [
     CSRC / "attn_tiles.hpp",
     CSRC / "attn_resident.hpp",

@@ -55,6 +55,9 @@ class EnergyConfig:
     rope_impl: str = "broadcast"  # "fused": the HIP RoPE split/merge (RotaryTable2D), reference rope_impl
     block_impl: str = "eager"  # "fused": rms_norm and the SwiGLU activation as HIP kernels (ebr_amd.block)
     linear_impl: str = "eager"  # "splitk": projection weight gradients as split-K GEMMs (ebr_amd.linear)
+    embed_impl: str = "eager"  # "fused": token lookup and table gradient as HIP kernels (ebr_amd.tokens)
+    norm: str = "rms"  # "group": the blocks' norms over the board's cells, in norm_groups groups of channels
+    norm_groups: int = 8
 
 
 class ScalarEnergy(nn.Module):
@@ -64,6 +67,8 @@ class ScalarEnergy(nn.Module):
         self.embed = nn.Parameter(trunc_normal_init_(torch.empty(cfg.vocab_size, cfg.hidden_size), std=1.0))
         self.layers = nn.ModuleList(EnergyReasoningBlock(cfg) for _ in range(cfg.num_layers))
         self.energy_head = CastedLinear(cfg.hidden_size, 1, bias=False)
+        if cfg.embed_impl not in ("eager", "fused"):
+            raise ValueError(f"embed_impl must be 'eager' or 'fused', got {cfg.embed_impl!r}")
         head_dim = cfg.hidden_size // cfg.num_heads
         if not cfg.rope:
             self.rope = None
@@ -75,6 +80,10 @@ class ScalarEnergy(nn.Module):
             raise ValueError(f"rope_impl must be 'broadcast' or 'fused', got {cfg.rope_impl!r}")
 
     def puzzle_embedding(self, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+        if getattr(self.cfg, "embed_impl", "eager") == "fused":
+            from ebr_amd import tokens
+
+            return tokens.embedding(x, self.embed, dtype=dtype)
         return F.embedding(x, self.embed.to(dtype))
 
     def forward(self, z: torch.Tensor, x_emb: torch.Tensor) -> torch.Tensor:
@@ -271,14 +280,33 @@ class Decoder(nn.Module):
         return self.lm_head(v).float()
 
 
+def teacher_logits(model, decoder, x, z0, k: int, steps: int = 64, alpha=0.1):
+    """What a descent of ``steps`` steps has to teach one of fewer: its decoder's ``k`` largest logits for each cell and
+    their tokens, (values, ids) [B, L, k]."""
+    with torch.no_grad():
+        x_emb = model.puzzle_embedding(x, z0.dtype)
+    v = descend(model, z0, x_emb, steps, alpha, create_graph=False)
+    with torch.no_grad():
+        return tuple(decoder(v).topk(k, dim=-1))
+
+
 def train_step(model, decoder, x, z0, targets, steps: int = 16, alpha=0.1, compiled=None,
-               wrapper: Optional[str] = None, sigma=None, noises=None, active=None) -> torch.Tensor:
+               wrapper: Optional[str] = None, sigma=None, noises=None, active=None, teacher=None,
+               temperature: float = 1.0) -> torch.Tensor:
     """One config-3 training step: graded descent (create_graph), CE to ``targets``, backward. Returns the loss.
-    ``wrapper`` and the rest select the reference microstep (``descend``)."""
+    ``wrapper`` and the rest select the reference microstep (``descend``). With ``teacher``, (values, ids) as
+    ``teacher_logits`` gives them, the loss is the distillation from them at ``temperature`` (``tokens.distill_loss``, GPU
+    only) in the cross entropy's place, and ``targets`` is not read."""
     x_emb = model.puzzle_embedding(x, z0.dtype)
     z = z0.detach().requires_grad_(True)
     v = descend(model, z, x_emb, steps, alpha, create_graph=True, compiled=compiled, wrapper=wrapper, sigma=sigma,
                 noises=noises, active=active)
+    if teacher is not None:
+        from ebr_amd import tokens
+
+        loss = tokens.distill_loss(decoder.lm_head(v), *teacher, temperature=temperature)
+        loss.backward()
+        return loss.detach()
     logits = decoder(v)
     loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
     loss.backward()
@@ -348,6 +376,7 @@ __all__ = [
     "infer",
     "microstep",
     "sphere",
+    "teacher_logits",
     "train_step",
     "verify_compiled_energy_grad",
 ]

@@ -45,6 +45,14 @@ def rms_norm(x: torch.Tensor, variance_epsilon: float) -> torch.Tensor:
     return (xf * torch.rsqrt(xf.pow(2).mean(dim=-1, keepdim=True) + variance_epsilon)).to(x.dtype)
 
 
+def group_norm(x: torch.Tensor, groups: int, eps: float) -> torch.Tensor:
+    """Zero mean and unit variance of each sample and group of channels over all cells of [B, ..., C], statistics in fp32,
+    result in the input dtype."""
+    xf = x.float().reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
+    c = xf - xf.mean(dim=(1, 3), keepdim=True)
+    return (c * torch.rsqrt(c.square().mean(dim=(1, 3), keepdim=True) + eps)).reshape(x.shape).to(x.dtype)
+
+
 class CastedLinear(nn.Module):
     """y = x W^T (+ b) with fp32 parameters cast to x.dtype at every call. ``impl="splitk"`` takes the weight
     gradients as split-K GEMMs with fp32 partials (``ebr_amd.linear``); the values are those of ``F.linear``."""
@@ -185,6 +193,7 @@ __all__ = [
     "SwiGLU",
     "apply_rope",
     "check_linear_impl",
+    "group_norm",
     "rms_norm",
     "rotate_half",
     "swiglu_intermediate",

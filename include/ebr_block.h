@@ -1,6 +1,6 @@
 /* C ABI of the energy network's fused pointwise blocks in libebr_attn.so (gfx950): rms_norm over the last dimension
  * and the SwiGLU activation, each with its backward and the backward of that backward, as the graded latent descent
- * differentiates the energy twice; and the ends of a training step, the embedding of tokens with its table's gradient and
+ * differentiates the energy twice; the group norm with an activation, likewise; and the ends of a training step, the embedding of tokens with its table's gradient and
  * the distillation loss with its gradient.
  *
  * Tensors are contiguous rows of one dtype (EBR_DTYPE_F32, _BF16, _F16 or _F64). Arithmetic is fp32 (fp64 for fp64);
@@ -90,6 +90,30 @@ int64_t ebr_block_distill_scratch(int dtype, int64_t N, int64_t V, int K);
 int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride,
                           double temperature, const void* logits, const void* teacher, const void* ids, const void* stats,
                           const void* scale, const void* grad, int64_t grad_stride, void* dx, void* stream);
+
+/* Activations of the group norm. */
+enum { EBR_ACT_NONE = 0, EBR_ACT_SILU = 1 };
+
+/* y = f(w h + b), h = (x - mean) / sqrt(variance + eps), for x [B, L, C] contiguous, channels last: the statistics of each
+ * sample and group are over its L cells and C / groups channels. w and b: fp32 (fp64 for fp64) [C], or NULL (1 and 0).
+ * stats: [B, groups, 2] of that type, the mean and the factor, for the derivatives. scratch: 16-byte aligned, of
+ * ebr_block_groupnorm_scratch's size for order 0. */
+int ebr_block_groupnorm(int dtype, int act, int64_t B, int64_t L, int C, int groups, double eps, const void* x, const void* w,
+                        const void* b, void* y, void* stats, void* scratch, void* stream);
+
+/* dx, and dw and db (of w's type; NULL where not wanted), of y given dy. Scratch of order 1. */
+int ebr_block_groupnorm_bwd(int dtype, int act, int64_t B, int64_t L, int C, int groups, const void* x, const void* w,
+                            const void* b, const void* stats, const void* dy, void* dx, void* dw, void* db, void* scratch,
+                            void* stream);
+
+/* Gradients of <u, dx> + <uw, dw> + <ub, db> (uw, ub: NULL for zero) with respect to x (gx), dy (gdy), w (gw) and b (gb;
+ * gw and gb NULL where not wanted). Scratch of order 2. */
+int ebr_block_groupnorm_bwd2(int dtype, int act, int64_t B, int64_t L, int C, int groups, const void* x, const void* w,
+                             const void* b, const void* stats, const void* dy, const void* u, const void* uw, const void* ub,
+                             void* gx, void* gdy, void* gw, void* gb, void* scratch, void* stream);
+
+/* Bytes of scratch of the group norm (order 0) and its derivatives (1, 2), -1 for sizes or types that they refuse. */
+int64_t ebr_block_groupnorm_scratch(int dtype, int order, int64_t B, int64_t L, int C, int groups);
 
 #ifdef __cplusplus
 }
