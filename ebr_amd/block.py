@@ -513,12 +513,29 @@ class _GroupNorm(torch.autograd.Function):
         return dx, dw, db, None, None, None
 
 
+@_host.gradient("group_norm")
+def _group_norm_grads(x, w, b, stats, groups, act, params, dy):
+    return _GroupNormBwd.apply(x, w, b, stats, dy, groups, act, params)
+
+
+@_host.gradient("group_norm_bwd")
+def _group_norm_bwd_grads(x, w, b, stats, dy, groups, act, params, u, uw, ub):
+    u = torch.zeros_like(x) if u is None else u
+    gx, gdy, gw, gb = _GroupNormBwd2.apply(x, w, b, stats, dy, u, uw, ub, groups, act, params)
+    return gx, gw, gb, None, gdy
+
+
 def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
                activation: Optional[str] = None) -> Tensor:
     """f(weight * h + bias) for a channels-last tensor [B, ..., C]: h is x less its mean and over the square root of its
     variance plus ``eps``, both taken for each sample and each group of C / groups neighbouring channels, over all cells.
     ``activation``: None, or "silu". ``weight`` and ``bias``: [C], or None (1 and 0). Statistics and sums are fp32 or wider,
     outputs rounded once to x's dtype; differentiable twice, for x, weight and bias, and a third derivative raises."""
+    host = _host.module()
+    y = None if host is None or activation not in ACTIVATIONS else host.group_norm(x, groups, weight, bias, eps,
+                                                                                   ACTIVATIONS[activation])
+    if y is not None:
+        return y
     if activation not in ACTIVATIONS:
         raise ValueError(f"fused block: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
     _code(x), _board(x, groups)

@@ -1,7 +1,7 @@
 // Native host path of the GPU ops: argument checks, output allocation, autograd nodes and the launches of
 // libebr_attn.so (include/ebr_*.h) in C++, for calls on plain GPU tensors.
 //
-// The Python layer (ebr_amd/fused_attn/ops.py, rope_split.py, block.py, descent.py, linear.py) defines the ops, their
+// The Python layer (ebr_amd/fused_attn/ops.py, rope_split.py, block.py, descent.py, linear.py, tokens.py) defines the ops, their
 // fakes and their autograd Functions, and stays the path of every call this file does not take: tensor subclasses and
 // fake tensors, torch.func transforms, dispatch and function modes, tracing, forward-mode duals, saved-tensor hooks,
 // tensors off the GPU, and every argument the Python layer would refuse or pad. Each entry point below returns None for
@@ -1108,6 +1108,344 @@ py::object linear(const py::handle& hx, const py::handle& hw) {
     return py::cast(Linear::apply(x, w)[0]);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Group norm, differentiable twice (ebr_amd/block.py)
+// ---------------------------------------------------------------------------------------------------------------------
+
+at::ScalarType acc_type(const Tensor& x) { return x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
+
+// A weight, a bias or a cotangent of one as the kernels read it.
+Tensor as_param(const Tensor& p, const Tensor& x) { return p.defined() ? dense(p.to(acc_type(x))) : Tensor(); }
+
+struct NormShape {
+    int code, act, C, groups;
+    int64_t B, L;
+    NormShape(const Tensor& x, int64_t groups_, int64_t act_)
+        : code(dtype_code(x.scalar_type())), act((int)act_), C((int)x.size(-1)), groups((int)groups_), B(x.size(0)),
+          L(x.numel() / (x.size(0) * x.size(-1))) {}
+    Tensor scratch(const Tensor& x, int order) const {
+        const int64_t n = ebr_block_groupnorm_scratch(code, order, B, L, C, groups);
+        TORCH_CHECK_VALUE(n >= 0, "ebr_block_groupnorm: sizes out of range");
+        return at::empty({n}, x.options().dtype(at::kByte));
+    }
+};
+
+variable_list groupnorm(const Tensor& x_, const Tensor& w_, const Tensor& b_, int64_t groups, double eps, int64_t act) {
+    RECORD_FUNCTION("ebr_fused::block_groupnorm", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(x_.device());
+    const Tensor x = dense(x_), w = as_param(w_, x_), b = as_param(b_, x_), y = at::empty(x.sizes(), x.options());
+    const NormShape n(x, groups, act);
+    const Tensor stats = at::empty({n.B, groups, 2}, x.options().dtype(acc_type(x))), s = n.scratch(x, 0);
+    check(ebr_block_groupnorm(n.code, n.act, n.B, n.L, n.C, n.groups, eps, x.data_ptr(), vptr(w), vptr(b), y.data_ptr(),
+                              stats.data_ptr(), s.data_ptr(), stream_of(x)),
+          "ebr_block_groupnorm");
+    return {y, stats};
+}
+
+// {dx, dw, db}: the latter with want_w and want_b.
+variable_list groupnorm_bwd(const Tensor& x_, const Tensor& w_, const Tensor& b_, const Tensor& stats, const Tensor& dy_,
+                            int64_t groups, int64_t act, bool want_w, bool want_b) {
+    RECORD_FUNCTION("ebr_fused::block_groupnorm_bwd", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(x_.device());
+    const Tensor x = dense(x_), dy = dense(dy_.to(x_.scalar_type())), w = as_param(w_, x_), b = as_param(b_, x_);
+    const NormShape n(x, groups, act);
+    const auto p = x.options().dtype(acc_type(x));
+    const Tensor dx = at::empty(x.sizes(), x.options()), s = n.scratch(x, 1);
+    Tensor dw = want_w ? at::empty({n.C}, p) : Tensor(), db = want_b ? at::empty({n.C}, p) : Tensor();
+    check(ebr_block_groupnorm_bwd(n.code, n.act, n.B, n.L, n.C, n.groups, x.data_ptr(), vptr(w), vptr(b), stats.data_ptr(),
+                                  dy.data_ptr(), dx.data_ptr(), vptr(dw), vptr(db), s.data_ptr(), stream_of(x)),
+          "ebr_block_groupnorm_bwd");
+    if (want_w) dw = dw.to(w_.scalar_type());
+    if (want_b) db = db.to(b_.scalar_type());
+    return {dx, dw, db};
+}
+
+// Whether this pass uses the gradients of the weight and the bias, the inputs after x. (A node counts the tensors given.)
+std::pair<bool, bool> wanted(AutogradContext* ctx, const Tensor& w, const Tensor& b) {
+    return {w.defined() && ctx->needs_input_grad(1), b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)};
+}
+
+struct GroupNormBwd : Function<GroupNormBwd> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w_,
+                                 const std::optional<Tensor>& b_, const Tensor& stats, const Tensor& dy, int64_t groups,
+                                 int64_t act, bool want_w, bool want_b) {
+        const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
+        ctx->save_for_backward({x, w, b, stats, dy});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["want_w"] = want_w;
+        ctx->saved_data["want_b"] = want_b;
+        ctx->set_materialize_grads(false);
+        variable_list out;  // dx, and what is wanted of dw and db
+        for (const Tensor& t : groupnorm_bwd(x, w, b, stats, dy, groups, act, want_w, want_b))
+            if (t.defined()) out.push_back(t);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(9);
+        const bool had_w = ctx->saved_data["want_w"].toBool(), had_b = ctx->saved_data["want_b"].toBool();
+        const Tensor u_ = g[0], uw_ = had_w ? g[1] : Tensor(), ub_ = had_b ? g[1 + had_w] : Tensor();
+        if (!u_.defined() && !uw_.defined() && !ub_.defined()) return out;
+        const variable_list sv = ctx->get_saved_variables();
+        const Tensor &x_ = sv[0], &w_ = sv[1], &b_ = sv[2], &stats = sv[3], &dy_ = sv[4];
+        const int64_t groups = ctx->saved_data["groups"].toInt(), act = ctx->saved_data["act"].toInt();
+        const auto [want_w, want_b] = wanted(ctx, w_, b_);
+        if (!native(g))
+            return python_grads("group_norm_bwd", 9, x_, maybe(w_), maybe(b_), stats, dy_, groups, act, want_w || want_b,
+                                maybe(u_), maybe(uw_), maybe(ub_));
+        RECORD_FUNCTION("ebr_fused::block_groupnorm_bwd2", std::vector<c10::IValue>());
+        const c10::DeviceGuard on(x_.device());
+        const Tensor x = dense(x_), dy = dense(dy_.to(x_.scalar_type())), w = as_param(w_, x_), b = as_param(b_, x_);
+        const Tensor u = u_.defined() ? dense(u_.to(x_.scalar_type())) : at::zeros_like(x);
+        const Tensor uw = as_param(uw_, x_), ub = as_param(ub_, x_);
+        const NormShape n(x, groups, act);
+        const auto p = x.options().dtype(acc_type(x));
+        const Tensor gx = at::empty(x.sizes(), x.options()), gdy = at::empty(x.sizes(), x.options());
+        const Tensor gw = want_w ? at::empty({n.C}, p) : Tensor(), gb = want_b ? at::empty({n.C}, p) : Tensor();
+        const Tensor s = n.scratch(x, 2);
+        check(ebr_block_groupnorm_bwd2(n.code, n.act, n.B, n.L, n.C, n.groups, x.data_ptr(), vptr(w), vptr(b),
+                                       stats.data_ptr(), dy.data_ptr(), u.data_ptr(), vptr(uw), vptr(ub), gx.data_ptr(),
+                                       gdy.data_ptr(), vptr(gw), vptr(gb), s.data_ptr(), stream_of(x)),
+              "ebr_block_groupnorm_bwd2");
+        variable_list d = {gx, want_w ? gw.to(w_.scalar_type()) : Tensor(), want_b ? gb.to(b_.scalar_type()) : Tensor(),
+                           gdy.to(dy_.scalar_type())};
+        if (recorded({x_, w_, b_, dy_, u_, uw_, ub_})) d = last(std::move(d));
+        out[0] = d[0];
+        out[1] = d[1];
+        out[2] = d[2];
+        out[4] = d[3];
+        return out;
+    }
+};
+
+struct GroupNorm : Function<GroupNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w_,
+                                 const std::optional<Tensor>& b_, int64_t groups, double eps, int64_t act) {
+        const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
+        const variable_list out = groupnorm(x, w, b, groups, eps, act);
+        ctx->save_for_backward({x, w, b, out[1]});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        ctx->set_materialize_grads(false);
+        return {out[0]};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(6);
+        if (!g[0].defined()) return out;
+        const variable_list s = ctx->get_saved_variables();
+        const int64_t groups = ctx->saved_data["groups"].toInt(), act = ctx->saved_data["act"].toInt();
+        const auto [want_w, want_b] = wanted(ctx, s[1], s[2]);
+        if (!native(g))
+            return python_grads("group_norm", 6, s[0], maybe(s[1]), maybe(s[2]), s[3], groups, act, want_w || want_b, g[0]);
+        if (!at::GradMode::is_enabled()) {
+            const variable_list d = groupnorm_bwd(s[0], s[1], s[2], s[3], g[0], groups, act, want_w, want_b);
+            for (size_t i = 0; i < 3; ++i) out[i] = d[i];
+            return out;
+        }
+        const variable_list d =
+            GroupNormBwd::apply(s[0], maybe(s[1]), maybe(s[2]), s[3], g[0], groups, act, want_w, want_b);
+        out[0] = d[0];
+        if (want_w) out[1] = d[1];
+        if (want_b) out[2] = d[1 + want_w];
+        return out;
+    }
+};
+
+py::object group_norm(const py::handle& hx, int64_t groups, const py::handle& hw, const py::handle& hb, double eps,
+                      int64_t act) {
+    const Tensor x = plain(hx);
+    if (!x.defined() || !plain_context() || x.dim() < 2 || x.numel() == 0 || dtype_code(x.scalar_type()) < 0 || groups < 1 ||
+        x.size(-1) % groups || x.size(-1) > (1 << 20) || !(eps >= 0))
+        return py::none();
+    Tensor p[2];
+    const py::handle given[2] = {hw, hb};
+    for (int i = 0; i < 2; ++i) {
+        if (given[i].is_none()) continue;
+        p[i] = plain(given[i]);
+        if (!p[i].defined() || p[i].dim() != 1 || p[i].size(0) != x.size(-1) || p[i].device() != x.device() ||
+            dtype_code(p[i].scalar_type()) < 0)
+            return py::none();
+    }
+    if (ebr_block_groupnorm_scratch(dtype_code(x.scalar_type()), 2, x.size(0), x.numel() / (x.size(0) * x.size(-1)),
+                                    (int)x.size(-1), (int)groups) < 0)
+        return py::none();
+    return py::cast(GroupNorm::apply(x, maybe(p[0]), maybe(p[1]), groups, eps, act)[0]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Token ends of a training step (ebr_amd/tokens.py): the embedding, linear and differentiable to any order, and the
+// distillation loss, differentiable once
+// ---------------------------------------------------------------------------------------------------------------------
+
+at::ScalarType type_of(int64_t code) {
+    return code == EBR_DTYPE_F32 ? at::kFloat : code == EBR_DTYPE_BF16 ? at::kBFloat16
+         : code == EBR_DTYPE_F16 ? at::kHalf : at::kDouble;
+}
+
+bool token_type(const Tensor& ids) { return ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt; }
+int wide(const Tensor& ids) { return ids.scalar_type() == at::kLong; }
+
+Tensor embed(const Tensor& ids_, const Tensor& w_, double scale, int64_t ycode) {
+    RECORD_FUNCTION("ebr_fused::embed", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(w_.device());
+    const Tensor ids = dense(ids_), w = dense(w_);
+    std::vector<int64_t> shape = ids.sizes().vec();
+    shape.push_back(w.size(1));
+    const Tensor y = at::empty(shape, w.options().dtype(type_of(ycode)));
+    check(ebr_block_embed(dtype_code(w.scalar_type()), (int)ycode, wide(ids), ids.numel(), w.size(0), (int)w.size(1), scale,
+                          ids.data_ptr(), w.data_ptr(), y.data_ptr(), stream_of(w)),
+          "ebr_block_embed");
+    return y;
+}
+
+Tensor embed_bwd(const Tensor& ids_, const Tensor& dy_, int64_t V, double scale, int64_t wcode) {
+    RECORD_FUNCTION("ebr_fused::embed_bwd", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(dy_.device());
+    const Tensor ids = dense(ids_), dy = dense(dy_);
+    const int64_t C = dy.size(-1), N = ids.numel(), n = ebr_block_embed_bwd_scratch((int)wcode, N, V, (int)C);
+    TORCH_CHECK_VALUE(n >= 0, "ebr_block_embed_bwd: sizes out of range");
+    const Tensor dw = at::empty({V, C}, dy.options().dtype(type_of(wcode)));
+    const Tensor s = at::empty({n}, dy.options().dtype(at::kByte));
+    check(ebr_block_embed_bwd((int)wcode, dtype_code(dy.scalar_type()), wide(ids), N, V, (int)C, scale, ids.data_ptr(),
+                              dy.data_ptr(), dw.data_ptr(), s.data_ptr(), stream_of(dy)),
+          "ebr_block_embed_bwd");
+    return dw;
+}
+
+struct EmbedBwd;
+
+struct Embed : Function<Embed> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& ids, const Tensor& w, double scale, int64_t ycode) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["V"] = w.size(0);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["type"] = (int64_t)dtype_code(w.scalar_type());
+        ctx->set_materialize_grads(false);
+        return {embed(ids, w, scale, ycode)};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g);
+};
+
+struct EmbedBwd : Function<EmbedBwd> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& ids, const Tensor& dy, int64_t V, double scale,
+                                 int64_t wcode) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["type"] = (int64_t)dtype_code(dy.scalar_type());
+        ctx->set_materialize_grads(false);
+        return {embed_bwd(ids, dy, V, scale, wcode)};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(5);
+        if (!g[0].defined()) return out;
+        const Tensor ids = ctx->get_saved_variables()[0];
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const int64_t code = ctx->saved_data["type"].toInt();
+        if (!native(g)) return python_grads("embed_bwd", 5, ids, scale, code, g[0]);
+        out[1] = recorded({g[0]}) ? Embed::apply(ids, g[0], scale, code)[0] : embed(ids, g[0], scale, code);
+        return out;
+    }
+};
+
+variable_list Embed::backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(4);
+    if (!g[0].defined()) return out;
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const int64_t V = ctx->saved_data["V"].toInt(), code = ctx->saved_data["type"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    if (!native(g)) return python_grads("embed", 4, ids, V, scale, code, g[0]);
+    out[1] = recorded({g[0]}) ? EmbedBwd::apply(ids, g[0], V, scale, code)[0] : embed_bwd(ids, g[0], V, scale, code);
+    return out;
+}
+
+py::object embedding(const py::handle& hids, const py::handle& hw, double scale, int64_t ycode) {
+    const Tensor ids = plain(hids), w = plain(hw);
+    if (!ids.defined() || !w.defined() || !plain_context() || !token_type(ids) || w.dim() != 2 ||
+        ids.device() != w.device() || ids.numel() == 0 || w.numel() == 0 || !std::isfinite(scale))
+        return py::none();
+    const int wcode = dtype_code(w.scalar_type());
+    if (wcode < 0 || ycode < 0 || ycode > EBR_DTYPE_F64 ||
+        (ycode != wcode && !(wcode == EBR_DTYPE_F32 && (ycode == EBR_DTYPE_BF16 || ycode == EBR_DTYPE_F16))))
+        return py::none();
+    if (w.size(1) >= (1 << 18) || ebr_block_embed_bwd_scratch(wcode, ids.numel(), w.size(0), (int)w.size(1)) < 0)
+        return py::none();
+    return py::cast(Embed::apply(ids, w, scale, ycode)[0]);
+}
+
+// Rows of V columns with unit stride, and the stride from one to the next.
+Tensor logit_rows(const Tensor& logits, int64_t* stride) {
+    Tensor x = logits.reshape({-1, logits.size(-1)});
+    if ((x.size(1) > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < x.size(1))) x = x.contiguous();
+    *stride = std::max(x.stride(0), x.size(1));
+    return x;
+}
+
+struct Distill : Function<Distill> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_, const Tensor& ids_,
+                                 double temperature, int64_t reduction) {
+        RECORD_FUNCTION("ebr_fused::distill", std::vector<c10::IValue>());
+        const c10::DeviceGuard on(logits.device());
+        int64_t row;
+        const Tensor x = logit_rows(logits, &row), teacher = dense(teacher_), ids = dense(ids_);
+        const int64_t N = x.size(0), V = x.size(1), K = teacher.size(-1);
+        const int code = dtype_code(x.scalar_type());
+        const auto acc = x.options().dtype(acc_type(x));
+        const bool none = reduction == EBR_REDUCE_NONE;
+        const Tensor loss = at::empty(none ? logits.sizes().slice(0, logits.dim() - 1) : at::IntArrayRef(), acc);
+        const Tensor stats = at::empty({N, 4}, acc), scale = none ? Tensor() : at::empty({1}, acc);
+        const int64_t n = ebr_block_distill_scratch(code, N, V, (int)K);
+        TORCH_CHECK_VALUE(n >= 0, "ebr_block_distill: sizes out of range");
+        const Tensor s = at::empty({n}, x.options().dtype(at::kByte));
+        check(ebr_block_distill(code, dtype_code(teacher.scalar_type()), wide(ids), N, V, (int)K, row, temperature,
+                                (int)reduction, x.data_ptr(), teacher.data_ptr(), ids.data_ptr(), stats.data_ptr(),
+                                loss.data_ptr(), vptr(scale), s.data_ptr(), stream_of(x)),
+              "ebr_block_distill");
+        ctx->save_for_backward({logits, teacher_, ids_, stats, scale});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        return {loss};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(5);
+        if (!g[0].defined()) return out;
+        const variable_list sv = ctx->get_saved_variables();
+        const Tensor &logits = sv[0], &stats = sv[3], &scale = sv[4];
+        const double temperature = ctx->saved_data["temperature"].toDouble();
+        if (!native(g))
+            return python_grads("distill", 5, logits, sv[1], sv[2], stats,
+                                scale.defined() ? scale : at::empty({0}, stats.options()), temperature, g[0]);
+        RECORD_FUNCTION("ebr_fused::distill_bwd", std::vector<c10::IValue>());
+        const c10::DeviceGuard on(logits.device());
+        int64_t row;
+        const Tensor x = logit_rows(logits, &row), teacher = dense(sv[1]), ids = dense(sv[2]);
+        const Tensor grad = dense(g[0].to(stats.scalar_type())), dx = at::empty(logits.sizes(), logits.options());
+        check(ebr_block_distill_bwd(dtype_code(x.scalar_type()), dtype_code(teacher.scalar_type()), wide(ids), x.size(0),
+                                    x.size(1), (int)teacher.size(-1), row, temperature, x.data_ptr(), teacher.data_ptr(),
+                                    ids.data_ptr(), stats.data_ptr(), vptr(scale), grad.data_ptr(), !scale.defined(),
+                                    dx.data_ptr(), stream_of(x)),
+              "ebr_block_distill_bwd");
+        out[0] = dx;
+        if (recorded({logits, g[0]})) out[0] = last({dx})[0];
+        return out;
+    }
+};
+
+py::object distill_loss(const py::handle& hx, const py::handle& ht, const py::handle& hids, double temperature,
+                        int64_t reduction) {
+    const Tensor x = plain(hx), t = plain(ht), ids = plain(hids);
+    if (!x.defined() || !t.defined() || !ids.defined() || !plain_context() || x.dim() < 1 || t.dim() != x.dim() ||
+        t.sizes() != ids.sizes() || x.numel() == 0 || t.numel() == 0 || !token_type(ids) || dtype_code(x.scalar_type()) < 0 ||
+        dtype_code(t.scalar_type()) < 0 || t.device() != x.device() || ids.device() != x.device() || recorded({t}))
+        return py::none();
+    const int64_t lead = x.dim() - 1;
+    if (x.sizes().slice(0, lead) != t.sizes().slice(0, lead) || t.size(lead) > 1024 || !(temperature >= 1e-30) ||
+        temperature > 1e30)
+        return py::none();
+    if (ebr_block_distill_scratch(dtype_code(x.scalar_type()), x.numel() / x.size(lead), x.size(lead), (int)t.size(lead)) < 0)
+        return py::none();
+    return py::cast(Distill::apply(x, t, ids, temperature, reduction)[0]);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(ebr_host, m) {
@@ -1122,4 +1460,7 @@ PYBIND11_MODULE(ebr_host, m) {
     m.def("noisy_point", &noisy_point);
     m.def("step_and_project", &step_and_project);
     m.def("linear", &linear);
+    m.def("group_norm", &group_norm);
+    m.def("embedding", &embedding);
+    m.def("distill_loss", &distill_loss);
 }

@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ebr_amd import _capi
+from ebr_amd import _capi, _host
 from ebr_amd.fused_attn.loader import hip_library
 from ebr_amd.fused_attn.ops import _DTYPE_CODE, _stream
 
@@ -158,11 +158,28 @@ class _Embed(torch.autograd.Function):
         return None, _EmbedBwd.apply(ids, dy, ctx.V, ctx.scale, ctx.dtype), None, None
 
 
+_DTYPES = {code: dtype for dtype, code in _DTYPE_CODE.items()}
+
+
+@_host.gradient("embed")
+def _embed_grads(ids, V, scale, code, dy):
+    return None, _EmbedBwd.apply(ids, dy, V, scale, _DTYPES[code])
+
+
+@_host.gradient("embed_bwd")
+def _embed_bwd_grads(ids, scale, code, c):
+    return None, _Embed.apply(ids, c, scale, _DTYPES[code])
+
+
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> Tensor:
     """``scale * weight[ids]`` as [*ids.shape, C] in ``dtype`` (the table's, if not given; an fp32 table also gives
     bfloat16 and float16), taken in fp32 and rounded once. A token outside [0, V), such as a padding of -1, gives a row of
     zeros and no gradient. The table's gradient is dense, [V, C] in its dtype, summed in fp32 in a fixed order."""
     dtype = weight.dtype if dtype is None else dtype
+    host = _host.module()
+    y = None if host is None else host.embedding(ids, weight, scale, _DTYPE_CODE.get(dtype, -1))
+    if y is not None:
+        return y
     _check_embed(ids, weight.dtype, dtype)
     _check_table(ids, weight)
     if not math.isfinite(scale):
@@ -308,6 +325,11 @@ class _Distill(torch.autograd.Function):
         return dx, None, None, None, None
 
 
+@_host.gradient("distill")
+def _distill_grads(logits, teacher, ids, stats, scale, temperature, grad):
+    return (_DistillBwd.apply(logits, teacher, ids, stats, scale, grad, temperature),)
+
+
 def distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0,
                  reduction: str = "mean") -> Tensor:
     """Distillation of a student's ``logits`` [..., V] from a teacher's K largest logits, ``teacher_logits`` [..., K] at the
@@ -319,6 +341,11 @@ def distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, te
     A row without an entry of positive probability has loss 0 and gradient 0. ``reduction``: "mean" over the other rows (0
     if there is none), "sum", or "none" for [...]. The loss is fp32 (fp64 for fp64 logits) whatever the logits' dtype. K is
     at most 1024; a teacher entry of one token with any logit is the cross entropy to it. Only the logits get a gradient."""
+    host = _host.module()
+    y = None if host is None or reduction not in REDUCTIONS else host.distill_loss(
+        logits, teacher_logits, teacher_ids, temperature, REDUCTIONS[reduction])
+    if y is not None:
+        return y
     if reduction not in REDUCTIONS:
         raise ValueError(f"tokens: reduction must be one of {tuple(REDUCTIONS)}, got {reduction!r}")
     _check_distill(logits, teacher_logits, teacher_ids, temperature)
