@@ -7,6 +7,8 @@
 // the whole table, most of it zeros for text; what costs is bringing a token's rows together. Atomic sums would do that in
 // an order that changes from run to run, so the positions are sorted by token instead (a stable radix sort: equal tokens
 // keep their order), and a sum always adds the same rows in the same order, in 32 bits.
+#include <type_traits>
+
 #include "rowwise.hpp"
 
 namespace ebr_embed {
@@ -31,23 +33,27 @@ __device__ __forceinline__ uint32_t token(const Ids& ids, int64_t n) {
 
 // -- lookup ------------------------------------------------------------------------------------------------------------
 
+// A row's threads, at most a wave of them, go over its columns VEC at a time.
 template <typename TW, typename TY, int VEC>
-__global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, double scale, const TW* w, TY* y) {
+__global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int team, double scale, const TW* w, TY* y) {
     using A = typename Acc<TW>::type;
-    const int64_t CV = C / VEC, total = N * CV;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t n = i / CV;
-        const int64_t c = (i - n * CV) * VEC;
+    const int t = threadIdx.x & (team - 1);
+    const int per = 256 / team;
+    for (int64_t n = (int64_t)blockIdx.x * per + threadIdx.x / team; n < N; n += (int64_t)gridDim.x * per) {
         const uint32_t v = token(ids, n);
-        Pack<TY, VEC> o;
+        const bool there = v < (uint32_t)ids.V;
+        const TW* row = w + (int64_t)(there ? v : 0) * C;
+        TY* out = y + n * C;
+        for (int c = t * VEC; c < C; c += team * VEC) {
+            Pack<TY, VEC> o = {};
+            if (there) {
+                A x[VEC];
+                load_wide<TW, VEC>(row + c, x);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o.e[e] = (TY)0.f;
-        if (v < (uint32_t)ids.V) {
-            const TW* row = w + (int64_t)v * C + c;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) o.e[e] = (TY)((A)row[e] * (A)scale);
+                for (int e = 0; e < VEC; ++e) o.e[e] = (TY)(x[e] * (A)scale);
+            }
+            stp<TY, VEC>(out + c, o);
         }
-        stp<TY, VEC>(y + n * C + c, o);
     }
 }
 
@@ -232,25 +238,27 @@ struct SumArgs {
     const void* dy;
     void* dw;
     void* part;  // [chunks][2][C]: a chunk's share of a run from the chunk before (0), and of one that goes on (1)
-    int N, V, C, chunk, chunks, zero_rows;
+    int N, V, C, chunk, chunks, team, zero_rows;
     unsigned sum_blocks;
     double scale;
 };
 
 template <typename A, typename TW, int VEC>
 __device__ __forceinline__ void put_row(TW* p, const A (&acc)[VEC], double scale) {
-    Pack<TW, VEC> o;
+    TW o[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o.e[e] = (TW)(acc[e] * (A)scale);
-    stp<TW, VEC>(p, o);
+    for (int e = 0; e < VEC; ++e) o[e] = (TW)(acc[e] * (A)scale);
+    store_wide<TW, VEC>(p, o);
 }
 
-// The first workgroups sum: a wave takes a chunk of the sorted positions and 64 VEC columns. A run of equal tokens inside
-// the chunk is written to the table at once; a run over its border goes to part. The others write zeros to the rows of
-// tokens that do not occur, found by bisection.
+constexpr int AHEAD = 8;  // rows whose loads are under way together
+
+// The first workgroups sum: a team of lanes, as many as there are columns for and a wave at most, takes a chunk of the
+// sorted positions and VEC columns a lane. A run of equal tokens inside the chunk is written to the table at once; a run
+// over its border goes to part. The other workgroups write zeros to the rows of tokens that do not occur, found by
+// bisection: these are most of the table for text, and their stores fill the time that the sums wait for their rows.
 template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_sum(SumArgs a) {
     using A = typename Acc<TW>::type;
-    const int lane = threadIdx.x & 63;
     TW* dw = reinterpret_cast<TW*>(a.dw);
     if (blockIdx.x >= a.sum_blocks) {
         __shared__ uint8_t absent[256];
@@ -267,76 +275,121 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
             absent[threadIdx.x] = !(lo < a.N && a.key[lo] == v);
         }
         __syncthreads();
-        const int CV = a.C / VEC;
-        const Pack<TW, VEC> zero = {};
-        for (int r = 0; r < rows; ++r) {
+        const TW zero[VEC] = {};
+        const int per = 256 / a.team, t = threadIdx.x & (a.team - 1);
+        for (int r = threadIdx.x / a.team; r < rows; r += per) {
             if (!absent[r]) continue;
-            for (int c = threadIdx.x; c < CV; c += 256) stp<TW, VEC>(dw + (r0 + r) * a.C + (int64_t)c * VEC, zero);
+            for (int c = t * VEC; c < a.C; c += a.team * VEC) store_wide<TW, VEC>(dw + (r0 + r) * a.C + c, zero);
         }
         return;
     }
-    const int tiles = (a.C + 64 * VEC - 1) / (64 * VEC);
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (int64_t)a.chunks * tiles) return;  // wave-uniform
-    const int chunk = (int)(item / tiles), c = (int)(item % tiles) * 64 * VEC + lane * VEC;
+    const int per = a.team * VEC, tiles = (a.C + per - 1) / per;
+    const int64_t item = (int64_t)blockIdx.x * (256 / a.team) + threadIdx.x / a.team;
+    if (item >= (int64_t)a.chunks * tiles) return;
+    const int chunk = (int)(item / tiles), c = (int)(item % tiles) * per + (threadIdx.x & (a.team - 1)) * VEC;
+    if (c >= a.C) return;
+    const uint32_t V = (uint32_t)a.V;
     const int from = chunk * a.chunk, to = from + a.chunk < a.N ? from + a.chunk : a.N;
-    const bool on = c < a.C;
     const TY* dy = reinterpret_cast<const TY*>(a.dy) + c;
     A* part = reinterpret_cast<A*>(a.part) + (int64_t)chunk * 2 * a.C + c;
-    const uint32_t before = from > 0 ? a.key[from - 1] : (uint32_t)a.V, after = to < a.N ? a.key[to] : (uint32_t)a.V;
+    const uint32_t before = from > 0 ? a.key[from - 1] : V, after = to < a.N ? a.key[to] : V;
+    uint32_t key[AHEAD], pos[AHEAD];
+    const auto fetch = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            key[j] = i + j < to ? a.key[i + j] : V;
+            pos[j] = i + j < to ? a.pos[i + j] : 0;
+        }
+    };
+    fetch(from);
     A acc[VEC];
-    uint32_t cur = a.key[from];
+    uint32_t cur = key[0];
     bool opened = cur == before;  // the run came from the chunk before
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0;
     const auto close = [&](bool goes_on) {
-        if (!on || cur >= (uint32_t)a.V) return;
-        if (opened || goes_on) {
-            A* p = part + (opened ? 0 : a.C);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) p[e] = acc[e];
-        } else {
-            put_row<A, TW, VEC>(dw + (int64_t)cur * a.C + c, acc, a.scale);
-        }
+        if (cur >= V) return;  // positions without a token, which come last
+        if (opened || goes_on) store_wide<A, VEC>(part + (opened ? 0 : a.C), acc);
+        else put_row<A, TW, VEC>(dw + (int64_t)cur * a.C + c, acc, a.scale);
     };
-    for (int i = from; i < to; ++i) {
-        const uint32_t k = a.key[i];
-        if (k >= (uint32_t)a.V) break;  // positions without a token come last
-        if (k != cur) {
-            close(false);
-            cur = k;
-            opened = false;
+    for (int i = from; i < to; i += AHEAD) {
+        Pack<TY, VEC> row[AHEAD];
+        uint32_t k[AHEAD];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] = 0;
+        for (int j = 0; j < AHEAD; ++j) {
+            k[j] = key[j];
+            if (k[j] < V) row[j] = ldp<TY, VEC>(dy + (int64_t)pos[j] * a.C);
         }
-        if (on) {
-            const Pack<TY, VEC> v = ldp<TY, VEC>(dy + (int64_t)a.pos[i] * a.C);
+        if (i + AHEAD < to) fetch(i + AHEAD);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += (A)v.e[e];
+        for (int j = 0; j < AHEAD; ++j) {
+            if (i + j >= to) break;
+            if (k[j] != cur) {
+                close(false);
+                cur = k[j];
+                opened = false;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] = 0;
+            }
+            if (cur < V)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += (A)row[j].e[e];
         }
     }
     close(cur == after);
 }
 
-// Runs over chunks' borders: the wave of the chunk in which a run begins adds its parts in order.
-template <typename TW, int VEC> __global__ __launch_bounds__(256) void k_join(SumArgs a) {
+constexpr int JOIN_WAVES = 8;
+
+// Runs over chunks' borders: the workgroup of the chunk in which a run begins adds its parts, each wave every eighth, and
+// the waves' sums in order.
+template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_join(SumArgs a) {
     using A = typename Acc<TW>::type;
-    const int lane = threadIdx.x & 63, tiles = (a.C + 64 * VEC - 1) / (64 * VEC);
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (int64_t)(a.chunks - 1) * tiles) return;  // wave-uniform; the last chunk opens nothing
-    const int chunk = (int)(item / tiles), c = (int)(item % tiles) * 64 * VEC + lane * VEC;
+    __shared__ A sums[JOIN_WAVES][64 * VEC];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int chunk = (int)blockIdx.x, c = (int)blockIdx.y * 64 * VEC + lane * VEC;
     const int from = chunk * a.chunk, next = from + a.chunk;
     const uint32_t k = a.key[next - 1];
-    if (k >= (uint32_t)a.V || a.key[next] != k) return;                 // nothing goes on
-    if (a.key[from] == k && from > 0 && a.key[from - 1] == k) return;   // it began before this chunk
-    if (c >= a.C) return;
+    if (k >= (uint32_t)a.V || a.key[next] != k) return;                // nothing goes on (as for all that follow, of the
+    if (a.key[from] == k && from > 0 && a.key[from - 1] == k) return;  // whole workgroup); it began before this chunk
+    int end = chunk + 2;  // the first chunk that does not begin inside the run
+    for (bool more = true; more;) {
+        const int j = end + lane;
+        const uint64_t out = __ballot(j >= a.chunks || a.key[(int64_t)j * a.chunk] != k);
+        more = out == 0;
+        end += more ? 64 : __ffsll((unsigned long long)out) - 1;
+    }
     const A* part = reinterpret_cast<const A*>(a.part) + c;
     A acc[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = part[((int64_t)chunk * 2 + 1) * a.C + e];
-    for (int j = chunk + 1; j < a.chunks && a.key[j * a.chunk] == k; ++j)
+    for (int e = 0; e < VEC; ++e) acc[e] = 0;
+    if (c < a.C) {
+        if (wave == 0) load_wide<A, VEC>(part + ((int64_t)chunk * 2 + 1) * a.C, acc);
+        int j = chunk + 1 + wave;
+        for (; j + 3 * JOIN_WAVES < end; j += 4 * JOIN_WAVES) {
+            A x[4][VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += part[(int64_t)j * 2 * a.C + e];
+            for (int i = 0; i < 4; ++i) load_wide<A, VEC>(part + (int64_t)(j + i * JOIN_WAVES) * 2 * a.C, x[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += x[i][e];
+        }
+        for (; j < end; j += JOIN_WAVES) {
+            A x[VEC];
+            load_wide<A, VEC>(part + (int64_t)j * 2 * a.C, x);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += x[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sums[wave][lane * VEC + e] = acc[e];
+    __syncthreads();
+    if (wave || c >= a.C) return;
+#pragma unroll
+    for (int w = 1; w < JOIN_WAVES; ++w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += sums[w][lane * VEC + e];
     put_row<A, TW, VEC>(reinterpret_cast<TW*>(a.dw) + (int64_t)k * a.C + c, acc, a.scale);
 }
 
@@ -364,7 +417,9 @@ template <typename F> static int by_types(int wt, int yt, F f) {
     return f(double(), double());
 }
 
-constexpr int CHUNK = 64, MAX_CHUNKS = 4096;
+// Sorted positions that a team adds up: 64, or fewer (down to one round of loads) as far as that takes to have 768 waves,
+// three for each compute unit; more for very many positions, which bounds the parts that a run is in.
+constexpr int CHUNK = 64, MIN_CHUNK = AHEAD, MIN_WAVES = 768, MAX_CHUNKS = 4096;
 
 struct Plan {
     int passes, bits, groups, tiles, chunk, chunks;
@@ -378,6 +433,7 @@ struct Plan {
         tiles = (int)((all + SORT_GROUPS - 1) / SORT_GROUPS);
         groups = tiles ? (int)((all + tiles - 1) / tiles) : 0;
         chunk = CHUNK;
+        while (chunk > MIN_CHUNK && (N + chunk - 1) / chunk * ((C + 511) / 512) < MIN_WAVES) chunk /= 2;
         while ((N + chunk - 1) / chunk > MAX_CHUNKS) chunk *= 2;
         chunks = (int)((N + chunk - 1) / chunk);
         words = 4 * N + (int64_t)groups * SORT_DIGITS;
@@ -386,11 +442,27 @@ struct Plan {
     }
 };
 
-template <typename TW, typename TY, int VEC> static void launch_sums(hipStream_t s, const SumArgs& a, int64_t zeros) {
+// Lanes of a row of C / vec vectors: the next power of two, at most a wave.
+static int team_of(int C, int vec) {
+    int t = 1;
+    while (t < 64 && t * vec < C) t *= 2;
+    return t;
+}
+
+template <typename TW, typename TY, int VEC> static void launch_sums(hipStream_t s, SumArgs a) {
+    using A = typename Acc<TW>::type;
+    a.team = team_of(a.C, VEC);
+    const int64_t per = (int64_t)a.team * VEC, items = a.chunks * ((a.C + per - 1) / per), teams = 256 / a.team;
+    a.sum_blocks = (unsigned)((items + teams - 1) / teams);
+    // rows to a workgroup of zeros: about 64 KiB of them
+    a.zero_rows = 8;
+    while (a.zero_rows < 256 && (int64_t)a.zero_rows * a.C * (int64_t)sizeof(TW) < 65536) a.zero_rows *= 2;
+    const int64_t zeros = ((int64_t)a.V + a.zero_rows - 1) / a.zero_rows;
     hipLaunchKernelGGL((k_sum<TW, TY, VEC>), dim3((unsigned)(a.sum_blocks + zeros)), dim3(256), 0, s, a);
     if (a.chunks > 1) {
-        const int64_t tiles = (a.C + 64 * VEC - 1) / (64 * VEC);
-        hipLaunchKernelGGL((k_join<TW, VEC>), dim3((unsigned)(((a.chunks - 1) * tiles + 3) / 4)), dim3(256), 0, s, a);
+        constexpr int JV = VEC == 1 ? 1 : 16 / (int)sizeof(A);
+        const int64_t tiles = (a.C + 64 * JV - 1) / (64 * JV);
+        hipLaunchKernelGGL((k_join<TW, JV>), dim3(a.chunks - 1, (unsigned)tiles), dim3(64 * JOIN_WAVES), 0, s, a);
     }
 }
 
@@ -410,8 +482,15 @@ int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int
     return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
         using TW = decltype(tw);
         using TY = decltype(ty);
-        hipLaunchKernelGGL((k_lookup<TW, TY, 1>), dim3(blocks_for(N * C, 256)), dim3(256), 0, (hipStream_t)stream, i, N, C,
-                           scale, (const TW*)w, (TY*)y);
+        constexpr int VEC = 16 / (int)sizeof(TY);
+        const auto go = [&](auto vec) {
+            constexpr int VN = decltype(vec)::value;
+            const int team = team_of(C, VN);
+            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, 256 / team)), dim3(256), 0, (hipStream_t)stream, i,
+                               N, C, team, scale, (const TW*)w, (TY*)y);
+        };
+        if (C % VEC == 0 && aligned(w, 16) && aligned(y, 16)) go(std::integral_constant<int, VEC>());
+        else go(std::integral_constant<int, 1>());
         return launched();
     });
 }
@@ -452,12 +531,10 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
         using TW = decltype(tw);
         using TY = decltype(ty);
         SumArgs a = {swapped ? k1 : k0, swapped ? p1 : p0, dy, dw, w32 + p.words, (int)N, (int)V, C, p.chunk, p.chunks,
-                     0, 0, scale};
-        a.zero_rows = 64;
-        while (a.zero_rows < 256 && V / a.zero_rows > (1 << 22)) a.zero_rows *= 2;
-        const int64_t tiles = (C + 63) / 64;
-        a.sum_blocks = (unsigned)((p.chunks * tiles + 3) / 4);
-        launch_sums<TW, TY, 1>(s, a, (V + a.zero_rows - 1) / a.zero_rows);
+                     0, 0, 0, scale};
+        constexpr int VEC = 16 / (int)sizeof(TY);
+        if (C % VEC == 0 && aligned(dy, 16) && aligned(dw, 16)) launch_sums<TW, TY, VEC>(s, a);
+        else launch_sums<TW, TY, 1>(s, a);
         return launched();
     });
 }

@@ -21,6 +21,27 @@ template <typename T, int N> __device__ __forceinline__ void stp(T* p, const Pac
     *reinterpret_cast<Pack<T, N>*>(p) = v;
 }
 
+// N elements of T from or to memory of which 16 bytes (or all of them, where fewer) are aligned, as whole vectors.
+template <typename T, int N, typename A> __device__ __forceinline__ void load_wide(const T* p, A (&x)[N]) {
+    constexpr int V = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+        const Pack<T, V> v = ldp<T, V>(p + i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i + e] = (A)v.e[e];
+    }
+}
+template <typename A, int N> __device__ __forceinline__ void store_wide(A* p, const A (&x)[N]) {
+    constexpr int V = N * (int)sizeof(A) > 16 ? 16 / (int)sizeof(A) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+        Pack<A, V> v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v.e[e] = x[i + e];
+        stp<A, V>(p + i, v);
+    }
+}
+
 // Over aligned parts of W lanes of a wave.
 template <int W, typename A> __device__ __forceinline__ A lanes_sum(A v) {
 #pragma unroll
