@@ -33,36 +33,43 @@ __device__ __forceinline__ uint32_t token(const Ids& ids, int64_t n) {
 
 // -- lookup ------------------------------------------------------------------------------------------------------------
 
-// A row's threads, at most a wave of them, go over its columns VEC at a time.
+// A row's threads, at most a wave of them, go over its columns VEC at a time, ROWS rows side by side: a row's load waits
+// for its token's, and the next rows' fill that time.
+constexpr int ROWS = 4;
 template <typename TW, typename TY, int VEC>
 __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int team, double scale, const TW* w, TY* y) {
     using A = typename Acc<TW>::type;
-    const int t = threadIdx.x & (team - 1);
-    const int per = 256 / team;
-    for (int64_t n = (int64_t)blockIdx.x * per + threadIdx.x / team; n < N; n += (int64_t)gridDim.x * per) {
-        const uint32_t v = token(ids, n);
-        const bool there = v < (uint32_t)ids.V;
-        const TW* row = w + (int64_t)(there ? v : 0) * C;
-        TY* out = y + n * C;
-        for (int c = t * VEC; c < C; c += team * VEC) {
-            Pack<TY, VEC> o = {};
-            if (there) {
-                A x[VEC];
-                load_wide<TW, VEC>(row + c, x);
+    const int t = threadIdx.x & (team - 1), per = 256 / team;
+    for (int64_t n0 = (int64_t)blockIdx.x * per * ROWS + threadIdx.x / team; n0 < N; n0 += (int64_t)gridDim.x * per * ROWS) {
+        uint32_t v[ROWS];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o.e[e] = (TY)(x[e] * (A)scale);
+        for (int r = 0; r < ROWS; ++r) v[r] = n0 + r * per < N ? token(ids, n0 + r * per) : (uint32_t)ids.V;
+        for (int c = t * VEC; c < C; c += team * VEC) {
+            TW x[ROWS][VEC] = {};
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (v[r] < (uint32_t)ids.V) load_wide<TW, VEC>(w + (int64_t)v[r] * C + c, x[r]);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                if (n0 + r * per >= N) break;
+                Pack<TY, VEC> o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)  // a row of zeros stays one, whatever the scale's sign
+                    o.e[e] = v[r] < (uint32_t)ids.V ? (TY)((A)x[r][e] * (A)scale) : (TY)0.f;
+                stp<TY, VEC>(y + (n0 + r * per) * C + c, o);
             }
-            stp<TY, VEC>(out + c, o);
         }
     }
 }
 
 // -- positions sorted by token -----------------------------------------------------------------------------------------
 
-constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_KEYS = 4;
-constexpr int SORT_TILE = SORT_THREADS * SORT_KEYS;  // positions that a workgroup ranks at a time
+// A workgroup ranks a tile of 1,024 positions a round, as many rounds as leave at most 128 workgroups (each reads all the
+// others' counts); up to 4,096 positions are one workgroup's. A tile of 4,096 left most of the card idle: 16,384 positions
+// took 9.9 us a pass, 6.6 in tiles of 1,024.
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ONE = 4096;
 constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS;
-constexpr int SORT_GROUPS = 256;  // workgroups of a sort at most: each reads all the others' counts
+constexpr int SORT_GROUPS = 128;
 
 struct SortArgs {
     Ids ids;                     // read where kin is null
@@ -87,8 +94,8 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_count(SortArgs a) {
     __shared__ uint32_t count[SORT_DIGITS];
     for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) count[d] = 0;
     __syncthreads();
-    const int64_t from = (int64_t)blockIdx.x * a.tiles * SORT_TILE;
-    const int64_t to = from + (int64_t)a.tiles * SORT_TILE < a.N ? from + (int64_t)a.tiles * SORT_TILE : a.N;
+    const int64_t from = (int64_t)blockIdx.x * a.tiles * SORT_THREADS;
+    const int64_t to = from + (int64_t)a.tiles * SORT_THREADS < a.N ? from + (int64_t)a.tiles * SORT_THREADS : a.N;
     for (int64_t i = from + threadIdx.x; i < to; i += SORT_THREADS) {
         const uint32_t k = a.kin ? a.kin[i] : token(a.ids, i);
         atomicAdd(&count[(k >> a.shift) & ((1u << a.bits) - 1)], 1u);  // whole numbers: the order does not matter
@@ -115,13 +122,14 @@ __device__ __forceinline__ uint32_t digits_before(uint32_t v, uint32_t* waves) {
 
 // Ranks of a tile's keys among those with the same digit that come before them: count[wave][digit] ends as the number in
 // the waves before, rank[k] as the number before in the wave. Positions run by wave, then by k, then by lane.
-__device__ __forceinline__ void rank_tile(const uint32_t (&key)[SORT_KEYS], const bool (&valid)[SORT_KEYS], int shift,
-                                          int bits, uint32_t (*count)[SORT_DIGITS], uint32_t (&rank)[SORT_KEYS]) {
+template <int KEYS>
+__device__ __forceinline__ void rank_tile(const uint32_t (&key)[KEYS], const bool (&valid)[KEYS], int shift, int bits,
+                                          uint32_t (*count)[SORT_DIGITS], uint32_t (&rank)[KEYS]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = lane; d < SORT_DIGITS; d += 64) count[wave][d] = 0;
+    for (int d = lane; d < 1 << bits; d += 64) count[wave][d] = 0;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < SORT_KEYS; ++k) {
+    for (int k = 0; k < KEYS; ++k) {
         const uint32_t digit = (key[k] >> shift) & ((1u << bits) - 1);
         const uint64_t same = alike(digit, bits, valid[k]);
         const int first = same ? __ffsll((unsigned long long)same) - 1 : 0;
@@ -135,9 +143,10 @@ __device__ __forceinline__ void rank_tile(const uint32_t (&key)[SORT_KEYS], cons
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(SortArgs a) {
     __shared__ uint32_t count[SORT_WAVES][SORT_DIGITS];
     __shared__ uint32_t start[SORT_DIGITS], waves[SORT_WAVES];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x, wave = t >> 6, digits = 1 << a.bits;
     uint32_t before = 0, total = 0;
-    if (t < SORT_DIGITS) {
+    if (t < digits) {
+#pragma unroll 16
         for (int g = 0; g < (int)gridDim.x; ++g) {
             const uint32_t c = a.counts[(int64_t)g * SORT_DIGITS + t];
             total += c;
@@ -145,71 +154,65 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(SortArgs a) {
         }
     }
     const uint32_t base = digits_before(total, waves);
-    if (t < SORT_DIGITS) start[t] = base + before;
+    if (t < digits) start[t] = base + before;
     for (int tile = 0; tile < a.tiles; ++tile) {
-        const int64_t at = ((int64_t)blockIdx.x * a.tiles + tile) * SORT_TILE + wave * (SORT_KEYS * 64) + lane;
-        uint32_t key[SORT_KEYS], pos[SORT_KEYS], rank[SORT_KEYS];
-        bool valid[SORT_KEYS];
+        const int64_t i = ((int64_t)blockIdx.x * a.tiles + tile) * SORT_THREADS + t;
+        const bool valid[1] = {i < a.N};
+        const uint32_t key[1] = {valid[0] ? (a.kin ? a.kin[i] : token(a.ids, i)) : 0};
+        const uint32_t pos = valid[0] ? (a.kin ? a.pin[i] : (uint32_t)i) : 0;
+        uint32_t rank[1];
+        rank_tile<1>(key, valid, a.shift, a.bits, count, rank);
+        if (t < digits) {
+            uint32_t sum = start[t];
 #pragma unroll
-        for (int k = 0; k < SORT_KEYS; ++k) {
-            const int64_t i = at + k * 64;
-            valid[k] = i < a.N;
-            key[k] = valid[k] ? (a.kin ? a.kin[i] : token(a.ids, i)) : 0;
-            pos[k] = valid[k] ? (a.kin ? a.pin[i] : (uint32_t)i) : 0;
-        }
-        rank_tile(key, valid, a.shift, a.bits, count, rank);
-        uint32_t sum = 0, s0 = 0;
-        if (t < SORT_DIGITS) {
-            s0 = start[t];
             for (int w = 0; w < SORT_WAVES; ++w) {
                 const uint32_t c = count[w][t];
-                count[w][t] = s0 + sum;
+                count[w][t] = sum;
                 sum += c;
             }
-            start[t] = s0 + sum;
+            start[t] = sum;
         }
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < SORT_KEYS; ++k) {
-            if (!valid[k]) continue;
-            const uint32_t to = count[wave][(key[k] >> a.shift) & ((1u << a.bits) - 1)] + rank[k];
-            a.kout[to] = key[k];
-            a.pout[to] = pos[k];
+        if (valid[0]) {
+            const uint32_t to = count[wave][(key[0] >> a.shift) & (digits - 1)] + rank[0];
+            a.kout[to] = key[0];
+            a.pout[to] = pos;
         }
         __syncthreads();
     }
 }
 
-// Up to a tile of positions: every pass in one workgroup, the keys going round through shared memory.
+// Up to 4,096 positions: every pass in one workgroup, the keys going round through shared memory.
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_tile(SortArgs a, int passes) {
     __shared__ uint32_t count[SORT_WAVES][SORT_DIGITS];
-    __shared__ uint32_t keys[SORT_TILE], waves[SORT_WAVES];
-    __shared__ uint16_t places[SORT_TILE];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, at = wave * (SORT_KEYS * 64) + lane;
-    uint32_t key[SORT_KEYS], pos[SORT_KEYS], rank[SORT_KEYS];
-    bool valid[SORT_KEYS];
+    __shared__ uint32_t keys[SORT_ONE], waves[SORT_WAVES];
+    __shared__ uint16_t places[SORT_ONE];
+    constexpr int KEYS = SORT_ONE / SORT_THREADS;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, at = wave * (KEYS * 64) + lane;
+    uint32_t key[KEYS], pos[KEYS], rank[KEYS];
+    bool valid[KEYS];
 #pragma unroll
-    for (int k = 0; k < SORT_KEYS; ++k) {
+    for (int k = 0; k < KEYS; ++k) {
         valid[k] = at + k * 64 < a.N;
         key[k] = valid[k] ? token(a.ids, at + k * 64) : 0;
         pos[k] = at + k * 64;
     }
     for (int p = 0; p < passes; ++p) {
         const int shift = p * a.bits;
-        rank_tile(key, valid, shift, a.bits, count, rank);
+        rank_tile<KEYS>(key, valid, shift, a.bits, count, rank);
         uint32_t sum = 0;
-        if (t < SORT_DIGITS)
+        if (t < 1 << a.bits)
             for (int w = 0; w < SORT_WAVES; ++w) {
                 const uint32_t c = count[w][t];
                 count[w][t] = sum;
                 sum += c;
             }
         const uint32_t base = digits_before(sum, waves);
-        if (t < SORT_DIGITS)
+        if (t < 1 << a.bits)
             for (int w = 0; w < SORT_WAVES; ++w) count[w][t] += base;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < SORT_KEYS; ++k) {
+        for (int k = 0; k < KEYS; ++k) {
             if (!valid[k]) continue;
             const uint32_t to = count[wave][(key[k] >> shift) & ((1u << a.bits) - 1)] + rank[k];
             keys[to] = key[k];
@@ -217,14 +220,14 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_tile(SortArgs a, int pass
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < SORT_KEYS; ++k) {
+        for (int k = 0; k < KEYS; ++k) {
             if (!valid[k]) continue;
             key[k] = keys[at + k * 64];
             pos[k] = places[at + k * 64];
         }
     }
 #pragma unroll
-    for (int k = 0; k < SORT_KEYS; ++k) {
+    for (int k = 0; k < KEYS; ++k) {
         if (!valid[k]) continue;
         a.kout[at + k * 64] = key[k];
         a.pout[at + k * 64] = pos[k];
@@ -402,7 +405,7 @@ static bool types_ok(int wt, int yt) {
 
 static int check(int wt, int yt, int64_t N, int64_t V, int64_t C) {
     if (!types_ok(wt, yt)) return EBR_ERR_DTYPE;
-    if (N < 0 || N >= ((int64_t)1 << 31) - SORT_TILE || V < 1 || V >= ((int64_t)1 << 31) - 1 || C < 1 ||
+    if (N < 0 || N >= ((int64_t)1 << 31) - SORT_ONE || V < 1 || V >= ((int64_t)1 << 31) - 1 || C < 1 ||
         C >= (1 << 18) || N * C >= ((int64_t)1 << 40) || V * C >= ((int64_t)1 << 40))
         return EBR_ERR_SHAPE;
     return EBR_OK;
@@ -429,7 +432,7 @@ struct Plan {
         while ((V >> width) != 0) ++width;  // the tokens 0 .. V
         passes = (width + SORT_BITS - 1) / SORT_BITS;
         bits = (width + passes - 1) / passes;
-        const int64_t all = (N + SORT_TILE - 1) / SORT_TILE;
+        const int64_t all = (N + SORT_THREADS - 1) / SORT_THREADS;
         tiles = (int)((all + SORT_GROUPS - 1) / SORT_GROUPS);
         groups = tiles ? (int)((all + tiles - 1) / tiles) : 0;
         chunk = CHUNK;
@@ -486,7 +489,7 @@ int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int
         const auto go = [&](auto vec) {
             constexpr int VN = decltype(vec)::value;
             const int team = team_of(C, VN);
-            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, 256 / team)), dim3(256), 0, (hipStream_t)stream, i,
+            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, ROWS * (256 / team))), dim3(256), 0, (hipStream_t)stream, i,
                                N, C, team, scale, (const TW*)w, (TY*)y);
         };
         if (C % VEC == 0 && aligned(w, 16) && aligned(y, 16)) go(std::integral_constant<int, VEC>());
@@ -513,7 +516,7 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
     uint32_t* w32 = reinterpret_cast<uint32_t*>(scratch);
     uint32_t *k0 = w32, *p0 = w32 + N, *k1 = w32 + 2 * N, *p1 = w32 + 3 * N, *counts = w32 + 4 * N;
     SortArgs so = {{ids, ids64 != 0, (int)V}, nullptr, nullptr, k0, p0, counts, (int)N, 0, p.bits, p.tiles};
-    if (N > 0 && N <= SORT_TILE) {
+    if (N > 0 && N <= SORT_ONE) {
         hipLaunchKernelGGL(k_sort_tile, dim3(1), dim3(SORT_THREADS), 0, s, so, p.passes);
     } else if (N > 0) {
         for (int i = 0; i < p.passes; ++i) {
@@ -526,7 +529,7 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
             so.pout = so.pout == p0 ? p1 : p0;
         }
     }
-    const bool swapped = N > SORT_TILE && p.passes % 2 == 0;
+    const bool swapped = N > SORT_ONE && p.passes % 2 == 0;
     return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
         using TW = decltype(tw);
         using TY = decltype(ty);
