@@ -42,6 +42,22 @@ template <typename A, int N> __device__ __forceinline__ void store_wide(A* p, co
     }
 }
 
+// As store_wide, past the caches: for what nothing reads soon.
+template <typename A, int N> __device__ __forceinline__ void store_past(A* p, const A (&x)[N]) {
+    constexpr int V = N * (int)sizeof(A) > 16 ? 16 / (int)sizeof(A) : N;
+    if constexpr (V * sizeof(A) == 16) {
+        using W = uint32_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < N; i += V) {
+            W w;
+            __builtin_memcpy(&w, &x[i], 16);
+            __builtin_nontemporal_store(w, reinterpret_cast<W*>(p + i));
+        }
+    } else {
+        store_wide<A, N>(p, x);
+    }
+}
+
 // Over aligned parts of W lanes of a wave.
 template <int W, typename A> __device__ __forceinline__ A lanes_sum(A v) {
 #pragma unroll
