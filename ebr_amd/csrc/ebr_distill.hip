@@ -7,7 +7,11 @@
 //
 // Bound by memory: the forward reads the logits once (running maximum and sum), the backward reads them again and writes
 // the gradient; between them a row keeps four numbers. Exponents are taken of (x - max) (log2 e) / T: the difference of
-// raw logits is exact or nearly so, where x / T would be rounded at the size of x.
+// raw logits is exact or nearly so, where x / T would be rounded at the size of x, and x (log2 e) / T could pass the
+// largest float where a mask has left nothing but the type's lowest value.
+//
+// Rows of any width start at any element, so 16 bytes of them are loaded and stored at the type's own alignment, which
+// global memory takes on this card.
 #include <type_traits>
 
 #include "rowwise.hpp"
@@ -37,12 +41,14 @@ struct Args {
     const void* grad;
     int64_t grad_step;
     void* dx;
+    int splits, width;  // parts of a row where there are few, and their columns
+    void* soft;         // [N][splits]: a part's maximum and sum
 };
 
 // What a row's softmaxes need: its largest logit and log2 of the sum above it, the teacher's alike. tm is -inf for a row
 // that is not counted.
 template <typename A> struct alignas(4 * sizeof(A)) Stats { A m, s2, tm, ts2; };
-template <typename A> struct Partial { double loss, rows; };
+template <typename A> struct alignas(16) Partial { double loss, rows; };
 
 template <typename A> __device__ __forceinline__ A teacher_at(const Args& a, int64_t i) {
     switch (a.teacher_type) {
@@ -76,6 +82,46 @@ template <typename A> struct Soft {
         m = top;
     }
 };
+
+template <typename T, int VEC> struct __attribute__((packed, aligned(sizeof(T)))) Loose { T e[VEC]; };
+
+// Columns [from, to) of a row by TEAM threads, several vectors at a time: one step of the running maximum for all of them.
+template <typename T, int TEAM, typename A>
+__device__ __forceinline__ Soft<A> soft_row(const T* x, int from, int to, int t, A k) {
+    constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
+    using V = Loose<T, VEC>;
+    Soft<A> v = {lowest<A>(), 0};
+    int j = from + t * VEC;
+    const auto step = [&](const A* e, int n) {
+        A top = v.m;
+#pragma unroll
+        for (int i = 0; i < n; ++i) top = larger(e[i], top);
+        const A base = top == lowest<A>() ? (A)0 : top;
+        A sum = 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) sum += pow2((e[i] - base) * k);
+        v.s = v.s * pow2((v.m - base) * k) + sum;
+        v.m = top;
+    };
+    for (; j + (AT_ONCE - 1) * TEAM * VEC + VEC <= to; j += AT_ONCE * TEAM * VEC) {
+        V p[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) p[i] = *reinterpret_cast<const V*>(x + j + i * TEAM * VEC);
+        A e[AT_ONCE * VEC];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE * VEC; ++i) e[i] = (A)p[i / VEC].e[i % VEC];
+        step(e, AT_ONCE * VEC);
+    }
+    for (; j + VEC <= to; j += TEAM * VEC) {
+        const V p = *reinterpret_cast<const V*>(x + j);
+        A e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = (A)p.e[i];
+        step(e, VEC);
+    }
+    for (; j < to; ++j) v.add((A)x[j], k);  // the thread whose vector the row's end cuts
+    return v;
+}
 
 // Over the TEAM threads of a row: aligned lanes of a wave, or the whole workgroup.
 template <int TEAM, typename A> __device__ __forceinline__ void soft_all(Soft<A>& v, A k, A* lds) {
@@ -137,7 +183,19 @@ __device__ __forceinline__ A teach(const Args& a, int64_t n, Stats<A>& st, int t
     return sum_all<TEAM, A>(sum, lds);
 }
 
-template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_loss(Args a) {
+// A part of a row, where there are too few rows to fill the card.
+template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
+    using A = typename Acc<T>::type;
+    __shared__ A lds[16];
+    const int64_t n = blockIdx.x / a.splits;
+    const int part = (int)(blockIdx.x % a.splits), from = part * a.width, to = from + a.width < a.V ? from + a.width : a.V;
+    Soft<A> v = soft_row<T, 256, A>(reinterpret_cast<const T*>(a.x) + n * a.row, from, to, threadIdx.x, (A)a.k);
+    soft_all<256, A>(v, (A)a.k, lds);
+    if (threadIdx.x == 0) reinterpret_cast<Soft<A>*>(a.soft)[blockIdx.x] = v;
+}
+
+// Rows' losses, from the logits, or with JOIN from the rows' parts.
+template <typename T, int TEAM, bool JOIN> __global__ __launch_bounds__(256) void k_loss(Args a) {
     using A = typename Acc<T>::type;
     __shared__ A lds[16];
     __shared__ double rows[256 / TEAM][2];
@@ -148,7 +206,16 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_loss(Ar
     Soft<A> v = {lowest<A>(), 0};
     if (on) {
         const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
-        for (int j = t; j < a.V; j += TEAM) v.add((A)x[j], k);
+        if constexpr (JOIN) {
+            for (int i = t; i < a.splits; i += TEAM) {
+                const Soft<A> p = reinterpret_cast<const Soft<A>*>(a.soft)[n * a.splits + i];
+                v.merge(p.m, p.s, k);
+            }
+        } else if constexpr (TEAM < 64) {
+            if (t < a.V) v.add((A)x[t], k);  // a column a thread
+        } else {
+            v = soft_row<T, TEAM, A>(x, 0, a.V, t, k);
+        }
     }
     soft_all<TEAM, A>(v, k, lds);
     Stats<A> st = {v.m, lg2(v.s), 0, 0};
@@ -176,26 +243,27 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_loss(Ar
 }
 
 // The workgroups' sums together, in a fixed order; the mean's factor stays for the backward.
-template <typename A> __global__ __launch_bounds__(256) void k_total(Args a, int64_t parts) {
-    __shared__ double lds[2][4];
-    double loss = 0, rows = 0;
+template <typename A> __global__ __launch_bounds__(1024) void k_total(Args a, int64_t parts) {
+    __shared__ Partial<A> lds[16];
+    Partial<A> v = {0, 0};
     const Partial<A>* p = reinterpret_cast<const Partial<A>*>(a.part);
-    for (int64_t i = threadIdx.x; i < parts; i += 256) {
-        loss += p[i].loss;
-        rows += p[i].rows;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < parts; i += 1024) {
+        const Partial<A> o = p[i];
+        v.loss += o.loss;
+        v.rows += o.rows;
     }
-    loss = lanes_sum<64>(loss);
-    rows = lanes_sum<64>(rows);
-    if ((threadIdx.x & 63) == 0) {
-        lds[0][threadIdx.x >> 6] = loss;
-        lds[1][threadIdx.x >> 6] = rows;
-    }
+    v.loss = lanes_sum<64>(v.loss);
+    v.rows = lanes_sum<64>(v.rows);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     if (threadIdx.x == 0) {
-        loss = lds[0][0] + lds[0][1] + lds[0][2] + lds[0][3];
-        rows = lds[1][0] + lds[1][1] + lds[1][2] + lds[1][3];
-        const double f = a.reduction == EBR_REDUCE_SUM ? 1.0 : 1.0 / (rows > 0 ? rows : 1.0);
-        *reinterpret_cast<A*>(a.loss) = (A)(loss * f);
+        for (int w = 1; w < 16; ++w) {
+            v.loss += lds[w].loss;
+            v.rows += lds[w].rows;
+        }
+        const double f = a.reduction == EBR_REDUCE_SUM ? 1.0 : 1.0 / (v.rows > 0 ? v.rows : 1.0);
+        *reinterpret_cast<A*>(a.loss) = (A)(v.loss * f);
         *reinterpret_cast<A*>(a.scale) = (A)f;
     }
 }
@@ -220,15 +288,19 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_sh
     reinterpret_cast<T*>(a.dx)[n * a.V + t] = (T)d;
 }
 
-// A row's columns one after another, each from q alone; then the columns that the teacher names once more, each by the
-// first of its entries, which adds the others of the same column in their order.
+// A row's columns, or a part of them, each from q alone; then the columns among them that the teacher names once more, each
+// by the first of its entries, which adds the others of the same column in their order. The second write comes after a
+// barrier, from the same workgroup.
 template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Args a) {
     using A = typename Acc<T>::type;
+    constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
+    using V = Loose<T, VEC>;
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     A* prob = reinterpret_cast<A*>(shared) + (int64_t)team * a.K;
     int* col = reinterpret_cast<int*>(reinterpret_cast<A*>(shared) + (int64_t)(256 / TEAM) * a.K) + (int64_t)team * a.K;
-    const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + team;
+    const int64_t n = (int64_t)(blockIdx.x / a.splits) * (256 / TEAM) + team;
+    const int from = (int)(blockIdx.x % a.splits) * a.width, to = from + a.width < a.V ? from + a.width : a.V;
     const bool on = n < a.N;
     const A k = (A)a.k;
     Stats<A> st = {};
@@ -236,6 +308,7 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
     bool counted = false;
     const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
     T* dx = reinterpret_cast<T*>(a.dx) + n * a.V;
+    const auto q = [&](T v) { return pow2(((A)v - st.m) * k - st.s2); };
     if (on) {
         st = reinterpret_cast<const Stats<A>*>(a.stats)[n];
         counted = !(st.tm == lowest<A>() && st.ts2 == lowest<A>());
@@ -243,11 +316,37 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
         if (a.scale) c *= *reinterpret_cast<const A*>(a.scale);
         for (int i = t; i < a.K; i += TEAM) {
             const int j = column(a, n * a.K + i);
-            col[i] = j;
-            prob[i] = j < 0 ? (A)0 : pow2((teacher_at<A>(a, n * a.K + i) - st.tm) * k - st.ts2);
+            const bool mine = j >= from && j < to;
+            col[i] = mine ? j : -1;
+            prob[i] = mine ? pow2((teacher_at<A>(a, n * a.K + i) - st.tm) * k - st.ts2) : (A)0;
         }
-        for (int j = t; j < a.V; j += TEAM)
-            dx[j] = counted ? (T)(c * pow2(((A)x[j] - st.m) * k - st.s2)) : (T)0.f;
+        int j = from + t * VEC;
+        if (counted) {
+            for (; j + (AT_ONCE - 1) * TEAM * VEC + VEC <= to; j += AT_ONCE * TEAM * VEC) {
+                V p[AT_ONCE];
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) p[i] = *reinterpret_cast<const V*>(x + j + i * TEAM * VEC);
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    V o;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) o.e[e] = (T)(c * q(p[i].e[e]));
+                    *reinterpret_cast<V*>(dx + j + i * TEAM * VEC) = o;
+                }
+            }
+            for (; j + VEC <= to; j += TEAM * VEC) {
+                const V p = *reinterpret_cast<const V*>(x + j);
+                V o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o.e[e] = (T)(c * q(p.e[e]));
+                *reinterpret_cast<V*>(dx + j) = o;
+            }
+            for (; j < to; ++j) dx[j] = (T)(c * q(x[j]));
+        } else {
+            const V zero = {};
+            for (; j + VEC <= to; j += TEAM * VEC) *reinterpret_cast<V*>(dx + j) = zero;
+            for (; j < to; ++j) dx[j] = (T)0.f;
+        }
     }
     __syncthreads();
     if (!counted) return;
@@ -261,7 +360,7 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
                 first = first && o >= i;
                 p += prob[o];
             }
-        if (first) dx[j] = (T)(c * (pow2(((A)x[j] - st.m) * k - st.s2) - p));
+        if (first) dx[j] = (T)(c * (q(x[j]) - p));
     }
 }
 
@@ -272,6 +371,16 @@ static int team_of(int64_t V) {
     while (t < 64 && t < V) t *= 2;
     return t;
 }
+
+// Parts of a row: where rows of a workgroup each leave compute units without any, as many as give each of the 256 about
+// four, with at least 4,096 columns (a round of loads) and at most 64 parts.
+static int splits_of(int64_t N, int64_t V) {
+    if (team_of(V) < 256 || N >= 512) return 1;
+    int64_t s = 1024 / (N > 0 ? N : 1);
+    if (s > V / 4096) s = V / 4096;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+static int width_of(int64_t V, int splits) { return (int)(((V + splits - 1) / splits + 7) / 8 * 8); }
 
 static int64_t groups(int64_t N, int team) { return (N + 256 / team - 1) / (256 / team); }
 
@@ -311,7 +420,9 @@ extern "C" {
 
 int64_t ebr_block_distill_scratch(int dtype, int64_t N, int64_t V, int K) {
     if (check(dtype, dtype, N, V, K, V, 1.0)) return -1;
-    return groups(N, team_of(V)) * (int64_t)sizeof(Partial<float>);
+    const int splits = splits_of(N, V);
+    const int64_t soft = splits > 1 ? N * splits * 2 * (dtype == EBR_DTYPE_F64 ? 8 : 4) : 0;
+    return (soft + 15) / 16 * 16 + groups(N, splits > 1 ? 64 : team_of(V)) * (int64_t)sizeof(Partial<float>);
 }
 
 int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride, double temperature,
@@ -323,19 +434,30 @@ int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, in
     const bool one = reduction != EBR_REDUCE_NONE;
     if ((N > 0 && (!logits || !teacher || !ids || !stats)) || ((N > 0 || one) && !loss) || (one && !scale))
         return EBR_ERR_NULL;
-    if (one && N > 0 && !scratch) return EBR_ERR_SCRATCH;
+    if (N > 0 && !scratch && (one || splits_of(N, V) > 1)) return EBR_ERR_SCRATCH;
     if (!aligned(stats, 16) || !aligned(scratch, 16)) return EBR_ERR_ALIGN;
     Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature,
               temperature * temperature * LN2, reduction, stats, loss, scale, scratch};
     hipStream_t s = (hipStream_t)stream;
     return by_type(dtype, [&](auto v) {
         using T = decltype(v);
-        const int team = team_of(V);
-        if (N > 0)
+        using A = typename Acc<T>::type;
+        const int splits = splits_of(N, V), team = splits > 1 ? 64 : team_of(V);
+        a.splits = splits;
+        a.width = width_of(V, splits);
+        if (splits > 1) {
+            a.soft = scratch;
+            const int64_t soft = N * splits * (int64_t)sizeof(Soft<A>);
+            a.part = reinterpret_cast<char*>(scratch) + (soft + 15) / 16 * 16;
+            hipLaunchKernelGGL((k_part<T>), dim3((unsigned)(N * splits)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_loss<T, 64, true>), dim3((unsigned)groups(N, 64)), dim3(256), 0, s, a);
+        } else if (N > 0) {
             by_team(team, [&](auto w) {
-                hipLaunchKernelGGL((k_loss<T, decltype(w)::value>), dim3((unsigned)groups(N, team)), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((k_loss<T, decltype(w)::value, false>), dim3((unsigned)groups(N, team)), dim3(256), 0, s,
+                                   a);
             });
-        if (one) hipLaunchKernelGGL((k_total<typename Acc<T>::type>), dim3(1), dim3(256), 0, s, a, groups(N, team));
+        }
+        if (one) hipLaunchKernelGGL((k_total<A>), dim3(1), dim3(1024), 0, s, a, groups(N, team));
         return launched();
     });
 }
@@ -355,6 +477,8 @@ int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V
         using T = decltype(v);
         using A = typename Acc<T>::type;
         const int team = team_of(V);
+        a.splits = splits_of(N, V);
+        a.width = width_of(V, a.splits);
         const size_t lds = (size_t)(256 / team) * K * (sizeof(A) + sizeof(int));
         by_team(team, [&](auto w) {
             constexpr int TEAM = decltype(w)::value;
@@ -362,7 +486,7 @@ int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V
                 hipLaunchKernelGGL((k_grad_short<T, TEAM>), dim3((unsigned)groups(N, team)), dim3(256), 0,
                                    (hipStream_t)stream, a);
             else
-                hipLaunchKernelGGL((k_grad<T, TEAM>), dim3((unsigned)groups(N, team)), dim3(256), lds,
+                hipLaunchKernelGGL((k_grad<T, TEAM>), dim3((unsigned)(groups(N, team) * a.splits)), dim3(256), lds,
                                    (hipStream_t)stream, a);
         });
         return launched();
