@@ -39,6 +39,7 @@ struct Args {
     int64_t B, L;
     int C, G, cg;
     int tx, tiles, splits;  // threads across the channels, workgroups across them, parts of L
+    int tile;               // channels of a workgroup that holds whole groups
     int64_t rows;           // of a part
     double eps;
 };
@@ -47,6 +48,9 @@ __device__ __forceinline__ float pow_e(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ double pow_e(double x) { return exp(x); }
 __device__ __forceinline__ float inverse(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
+
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 // The activation's value, or its first two derivatives. ACT 0: none, 1: silu.
 template <int ACT, typename A> __device__ __forceinline__ A act(A a) {
@@ -81,20 +85,70 @@ template <typename A> __device__ __forceinline__ A param(const void* p, int c, A
     return p ? reinterpret_cast<const A*>(p)[c] : none;
 }
 
-// What a thread knows of its channels.
+template <typename A, int VEC> __device__ __forceinline__ void params(const void* p, int c, A none, A (&v)[VEC]) {
+    if (p)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = reinterpret_cast<const A*>(p)[c + e];
+    else
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = none;
+}
+
+// What a thread knows of its channels; h = x r + shift, shift = -mu r, rounded once (and shift no further than mu itself).
 template <typename A, int VEC> struct Channels {
-    A mu[VEC], r[VEC], w[VEC], b[VEC];
+    A shift[VEC], r[VEC], w[VEC], b[VEC];
     __device__ __forceinline__ void load(const Args& a, int64_t n, int c) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const A* s = reinterpret_cast<const A*>(a.stats) + (n * a.G + (c + e) / a.cg) * 2;
-            mu[e] = s[0];
             r[e] = s[1];
-            w[e] = param<A>(a.w, c + e, (A)1);
-            b[e] = param<A>(a.b, c + e, (A)0);
+            shift[e] = -s[0] * s[1];
         }
+        params<A, VEC>(a.w, c, (A)1, w);
+        params<A, VEC>(a.b, c, (A)0, b);
     }
 };
+
+// An element's part of the sums of modes 1 and 2.
+template <int ACT, int MODE, typename A, int NS, int VEC>
+__device__ __forceinline__ void add_sums(A (&s)[NS][VEC], int e, A x, A dy, A u, A r, A shift, A w, A b) {
+    const A h = fused(x, r, shift);
+    A f1, f2;
+    slopes<ACT, A>(w * h + b, f1, f2);
+    const A da = dy * f1;
+    if constexpr (MODE == 1) {
+        s[0][e] += da;
+        s[1][e] += da * h;
+    } else {
+        s[0][e] += u;
+        s[1][e] += u * h;
+        s[2][e] += da;
+        s[3][e] += da * h;
+        s[4][e] += da * u;
+        if constexpr (ACT != 0) {
+            const A t = dy * f2, th = t * h, tu = t * u;
+            s[5][e] += t;
+            s[6][e] += th;
+            s[7][e] += th * h;
+            s[8][e] += tu;
+            s[9][e] += tu * h;
+        }
+    }
+}
+
+// An element's gx and gdy, from its group's means.
+template <int ACT, typename A>
+__device__ __forceinline__ void second_out(A x, A dy, A u, A r, A shift, A w, A b, A uw, A ub, A u1, A u2, A k2, A v1, A v2,
+                                           A along, A& gx, A& gdy) {
+    const A h = fused(x, r, shift);
+    A f1, f2;
+    slopes<ACT, A>(w * h + b, f1, f2);
+    const A da = dy * f1, k = w * da;
+    const A q = w * r * (u - u1 - h * u2) + uw * h + ub;
+    const A v = w * dy * f2 * q + uw * da - r * (u * k2 + k * u2);
+    gx = r * (v - v1 - h * v2) - r * r * h * along;
+    gdy = f1 * q;
+}
 
 // A workgroup's place: sample, part of L, channels of this thread, and its first and last cell.
 struct Place {
@@ -171,31 +225,9 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
                 Pack<T, VEC> u;
                 if constexpr (MODE == 2) u = ldp<T, VEC>(reinterpret_cast<const T*>(a.u) + at);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const A h = ((A)x.e[e] - ch.mu[e]) * ch.r[e];
-                    A f1, f2;
-                    slopes<ACT, A>(ch.w[e] * h + ch.b[e], f1, f2);
-                    const A da = (A)dy.e[e] * f1;
-                    if constexpr (MODE == 1) {
-                        s[0][e] += da;
-                        s[1][e] += da * h;
-                    } else {
-                        const A uv = (A)u.e[e];
-                        s[0][e] += uv;
-                        s[1][e] += uv * h;
-                        s[2][e] += da;
-                        s[3][e] += da * h;
-                        s[4][e] += da * uv;
-                        if constexpr (ACT != 0) {
-                            const A t = (A)dy.e[e] * f2;
-                            s[5][e] += t;
-                            s[6][e] += t * h;
-                            s[7][e] += t * h * h;
-                            s[8][e] += t * uv;
-                            s[9][e] += t * uv * h;
-                        }
-                    }
-                }
+                for (int e = 0; e < VEC; ++e)
+                    add_sums<ACT, MODE, A>(s, e, (A)x.e[e], (A)dy.e[e], MODE == 2 ? (A)u.e[e] : (A)0, ch.r[e], ch.shift[e],
+                                           ch.w[e], ch.b[e]);
             }
         }
     }
@@ -254,131 +286,173 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
     }
 }
 
-// A sum over a workgroup of doubles, for everyone.
-__device__ __forceinline__ double all_sum(double v, double* lds) {
-    v = lanes_sum<64>(v);
+// A sum over a workgroup's threads of every sum, for everyone.
+template <int K> __device__ __forceinline__ void all_sums(double (&v)[K], double* lds) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = lanes_sum<64>(v[i]);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < K; ++i) lds[(threadIdx.x >> 6) * K + i] = v[i];
     __syncthreads();
-    v = lds[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v += lds[w];
-    return v;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        v[i] = lds[i];
+        for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v[i] += lds[w * K + i];
+    }
 }
 
-// One group of one sample: its means from the per-channel sums, and its channels' share of the parameters' gradients.
-// These few sums are taken in 64 bits: differences of means follow.
+// What follows from a channel's sums in a group of given means: a share of dw and db (gw, gb), and of the means of v and v h.
+struct Second {
+    double t, th, v1, v2, gw;
+};
+template <int ACT> __device__ __forceinline__ Second second(const double* s, double w, double uw, double ub, double r,
+                                                            double u1, double u2) {
+    Second o = {0, 0, 0, 0, 0};
+    if constexpr (ACT != 0) {  // q = cu u + ch h + cc
+        const double cu = w * r, ch = uw - cu * u2, cc = ub - cu * u1;
+        o.t = cu * s[8] + ch * s[6] + cc * s[5];
+        o.th = cu * s[9] + ch * s[7] + cc * s[6];
+    }
+    o.v1 = w * o.t + uw * s[2];
+    o.v2 = w * o.th + uw * s[3];
+    o.gw = r * (s[4] - u1 * s[2] - u2 * s[3]) + o.th;
+    return o;
+}
+
+// One group of one sample: its means from the per-channel sums of all parts, and its channels' share of the parameters'
+// gradients. Threads go over the channels and, as many as are left, over the parts. These few sums are taken in 64 bits:
+// differences of means follow.
 template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) void k_means(Args a) {
     constexpr int NS = MODE == 0 ? 2 : MODE == 1 ? 2 : ACT ? 10 : 5;
-    __shared__ double lds[WAVES];
+    __shared__ double lds[WAVES * 5];
+    __shared__ double tot[NS][THREADS];
     const int64_t n = blockIdx.x / a.G;
-    const int g = (int)(blockIdx.x % a.G), c0 = g * a.cg, c1 = c0 + a.cg;
+    const int g = (int)(blockIdx.x % a.G), c0 = g * a.cg;
     const double m = (double)a.L * a.cg;
+    int cols = 1;
+    while (cols < a.cg && cols < (int)blockDim.x) cols *= 2;
+    const int tc = threadIdx.x % cols, ts = threadIdx.x / cols, lanes = (int)blockDim.x / cols;
     const A* part = reinterpret_cast<const A*>(a.part) + n * a.splits * NS * a.C;
-    const auto total = [&](int i, int c) {
-        double v = 0;
-        for (int s = 0; s < a.splits; ++s) v += (double)part[((int64_t)s * NS + i) * a.C + c];
-        return v;
-    };
     const auto cells = [&](int s) { return (double)(s + 1 < a.splits ? a.rows : a.L - s * a.rows); };
     A* stats = reinterpret_cast<A*>(a.stats) + (n * a.G + g) * 2;
     if constexpr (MODE == 0) {
-        double v = 0;
-        for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x)
-            for (int s = 0; s < a.splits; ++s) v += cells(s) * (double)part[(int64_t)s * 2 * a.C + c];
-        const double mu = all_sum(v, lds) / m;
-        v = 0;
-        for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x)
-            for (int s = 0; s < a.splits; ++s) {
-                const double d = (double)part[(int64_t)s * 2 * a.C + c] - mu;
-                v += (double)part[((int64_t)s * 2 + 1) * a.C + c] + cells(s) * d * d;
+        double v[1] = {0};
+        for (int c = tc; c < a.cg; c += cols)
+            for (int s = ts; s < a.splits; s += lanes) v[0] += cells(s) * (double)part[(int64_t)s * 2 * a.C + c0 + c];
+        all_sums<1>(v, lds);
+        const double mu = v[0] / m;
+        v[0] = 0;
+        for (int c = tc; c < a.cg; c += cols)
+            for (int s = ts; s < a.splits; s += lanes) {
+                const double d = (double)part[(int64_t)s * 2 * a.C + c0 + c] - mu;
+                v[0] += (double)part[((int64_t)s * 2 + 1) * a.C + c0 + c] + cells(s) * d * d;
             }
-        const double var = all_sum(v, lds) / m;
+        all_sums<1>(v, lds);
         if (threadIdx.x == 0) {
             stats[0] = (A)mu;
-            stats[1] = (A)(1.0 / sqrt(var + a.eps));
+            stats[1] = (A)(1.0 / sqrt(v[0] / m + a.eps));
         }
         return;
     }
+    // a channel's sums over all parts, for its first thread
+    const auto channel = [&](int c, double (&s)[NS]) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s[i] = 0;
+        if (c < a.cg)
+#pragma unroll 4
+            for (int p = ts; p < a.splits; p += lanes)
+#pragma unroll
+                for (int i = 0; i < NS; ++i) s[i] += (double)part[((int64_t)p * NS + i) * a.C + c0 + c];
+        if (lanes == 1) return;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NS; ++i) tot[i][threadIdx.x] = s[i];
+        __syncthreads();
+        if (ts == 0)
+            for (int l = 1; l < lanes; ++l)
+#pragma unroll
+                for (int i = 0; i < NS; ++i) s[i] += tot[i][l * cols + tc];
+    };
     const double r = (double)stats[1];
     A* out = reinterpret_cast<A*>(a.means) + (n * a.G + g) * MEANS[MODE];
-    A* chan = reinterpret_cast<A*>(a.chan) + n * 2 * a.C;
+    A* chan = reinterpret_cast<A*>(a.chan) + n * 2 * a.C + c0;
     if constexpr (MODE == 1) {
-        double k1 = 0, k2 = 0;
-        for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) {
-            const double w = (double)param<A>(a.w, c, (A)1), da = total(0, c), dah = total(1, c);
-            k1 += w * da;
-            k2 += w * dah;
+        double k[2] = {0, 0};
+        for (int c = tc; c < (a.cg + cols - 1) / cols * cols; c += cols) {
+            double s[NS];
+            channel(c, s);
+            if (ts || c >= a.cg) continue;
+            const double w = (double)param<A>(a.w, c0 + c, (A)1);
+            k[0] += w * s[0];
+            k[1] += w * s[1];
             if (a.chan) {
-                chan[c] = (A)dah;
-                chan[a.C + c] = (A)da;
+                chan[c] = (A)s[1];
+                chan[a.C + c] = (A)s[0];
             }
         }
-        k1 = all_sum(k1, lds);
-        k2 = all_sum(k2, lds);
+        all_sums<2>(k, lds);
         if (threadIdx.x == 0) {
-            out[0] = (A)(k1 / m);
-            out[1] = (A)(k2 / m);
+            out[0] = (A)(k[0] / m);
+            out[1] = (A)(k[1] / m);
         }
     }
     if constexpr (MODE == 2) {
-        double u1 = 0, u2 = 0, k1 = 0, k2 = 0, ku = 0;
-        for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) {
-            const double w = (double)param<A>(a.w, c, (A)1);
-            u1 += total(0, c);
-            u2 += total(1, c);
-            k1 += w * total(2, c);
-            k2 += w * total(3, c);
-            ku += w * total(4, c);
+        const int rounds = (a.cg + cols - 1) / cols;
+        double k[5] = {0, 0, 0, 0, 0}, s[NS];
+        for (int i = 0; i < rounds; ++i) {
+            const int c = tc + i * cols;
+            channel(c, s);
+            if (ts || c >= a.cg) continue;
+            const double w = (double)param<A>(a.w, c0 + c, (A)1);
+            k[0] += s[0];
+            k[1] += s[1];
+            k[2] += w * s[2];
+            k[3] += w * s[3];
+            k[4] += w * s[4];
         }
-        u1 = all_sum(u1, lds) / m;
-        u2 = all_sum(u2, lds) / m;
-        k1 = all_sum(k1, lds) / m;
-        k2 = all_sum(k2, lds) / m;
-        ku = all_sum(ku, lds) / m;
-        double v1 = 0, v2 = 0;
-        for (int c = c0 + threadIdx.x; c < c1; c += blockDim.x) {
-            const double w = (double)param<A>(a.w, c, (A)1), uw = (double)param<A>(a.uw, c, (A)0);
-            const double da = total(2, c), dah = total(3, c);
-            double t = 0, th = 0;
-            if constexpr (ACT != 0) {  // q = cu u + ch h + cc
-                const double cu = w * r, ch = uw - cu * u2, cc = (double)param<A>(a.ub, c, (A)0) - cu * u1;
-                const double s0 = total(5, c), s1 = total(6, c);
-                t = cu * total(8, c) + ch * s1 + cc * s0;
-                th = cu * total(9, c) + ch * total(7, c) + cc * s1;
-            }
-            v1 += w * t + uw * da;
-            v2 += w * th + uw * dah;
+        all_sums<5>(k, lds);
+        const double u1 = k[0] / m, u2 = k[1] / m, k1 = k[2] / m, k2 = k[3] / m, ku = k[4] / m;
+        double v[2] = {0, 0};
+        for (int i = 0; i < rounds; ++i) {
+            const int c = tc + i * cols;
+            if (rounds > 1) channel(c, s);  // one round leaves them
+            if (ts || c >= a.cg) continue;
+            const Second o = second<ACT>(s, (double)param<A>(a.w, c0 + c, (A)1), (double)param<A>(a.uw, c0 + c, (A)0),
+                                         (double)param<A>(a.ub, c0 + c, (A)0), r, u1, u2);
+            v[0] += o.v1;
+            v[1] += o.v2;
             if (a.chan) {
-                chan[c] = (A)(r * (total(4, c) - u1 * da - u2 * dah) + th);
-                chan[a.C + c] = (A)t;
+                chan[c] = (A)o.gw;
+                chan[a.C + c] = (A)o.t;
             }
         }
-        v1 = all_sum(v1, lds) / m - r * (u1 * k2 + k1 * u2);
-        v2 = all_sum(v2, lds) / m - 2.0 * r * u2 * k2;
+        all_sums<2>(v, lds);
         if (threadIdx.x == 0) {
             out[0] = (A)u1;
             out[1] = (A)u2;
             out[2] = (A)k2;
-            out[3] = (A)v1;
-            out[4] = (A)v2;
+            out[3] = (A)(v[0] / m - r * (u1 * k2 + k1 * u2));
+            out[4] = (A)(v[1] / m - 2.0 * r * u2 * k2);
             out[5] = (A)(ku - k1 * u1 - u2 * k2);
         }
     }
 }
 
-// The samples' shares of the parameters' gradients together, in order.
+// The samples' shares of the parameters' gradients together, in a fixed order.
 template <typename A> __global__ __launch_bounds__(1024) void k_params(Args a) {
-    __shared__ double lds[16][64];
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + tx;
+    __shared__ double lds[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + tx;
     const A* chan = reinterpret_cast<const A*>(a.chan) + (int64_t)blockIdx.y * a.C + c;
     double v = 0;
     if (c < a.C)
-        for (int64_t n = ty; n < a.B; n += 16) v += (double)chan[n * 2 * a.C];
+#pragma unroll 8
+        for (int64_t n = ty; n < a.B; n += 32) v += (double)chan[n * 2 * a.C];
     lds[ty][tx] = v;
     __syncthreads();
     if (ty || c >= a.C) return;
-    for (int i = 1; i < 16; ++i) v += lds[i][tx];
+    for (int i = 1; i < 32; ++i) v += lds[i][tx];
     A* out = reinterpret_cast<A*>(blockIdx.y ? a.db : a.dw);
     if (out) out[c] = (A)v;
 }
@@ -392,14 +466,16 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
     Channels<A, VEC> ch;
     ch.load(a, p.n, p.c);
     A g[6][VEC], uw[VEC], ub[VEC];
+    if constexpr (MODE == 2) {
+        params<A, VEC>(a.uw, p.c, (A)0, uw);
+        params<A, VEC>(a.ub, p.c, (A)0, ub);
+    }
     if constexpr (MODE != 0)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const A* s = reinterpret_cast<const A*>(a.means) + (p.n * a.G + (p.c + e) / a.cg) * MEANS[MODE];
 #pragma unroll
             for (int i = 0; i < MEANS[MODE]; ++i) g[i][e] = s[i];
-            uw[e] = MODE == 2 ? param<A>(a.uw, p.c + e, (A)0) : (A)0;
-            ub[e] = MODE == 2 ? param<A>(a.ub, p.c + e, (A)0) : (A)0;
         }
     for (int64_t l = p.from + p.ty; l < p.to; l += p.step) {
         const int64_t at = base + l * a.C;
@@ -409,26 +485,267 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
         if constexpr (MODE == 2) u = ldp<T, VEC>(reinterpret_cast<const T*>(a.u) + at);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const A r = ch.r[e], w = ch.w[e], h = ((A)x.e[e] - ch.mu[e]) * r, av = w * h + ch.b[e];
-            if constexpr (MODE == 0) {
-                o.e[e] = (T)act<ACT, A>(av);
+            const A r = ch.r[e], w = ch.w[e];
+            if constexpr (MODE == 2) {
+                A gx, gdy;
+                second_out<ACT, A>((A)x.e[e], (A)dy.e[e], (A)u.e[e], r, ch.shift[e], w, ch.b[e], uw[e], ub[e], g[0][e], g[1][e],
+                                   g[2][e], g[3][e], g[4][e], g[5][e], gx, gdy);
+                o.e[e] = (T)gx;
+                o2.e[e] = (T)gdy;
             } else {
-                A f1, f2;
-                slopes<ACT, A>(av, f1, f2);
-                const A da = (A)dy.e[e] * f1, k = w * da;
-                if constexpr (MODE == 1) {
-                    o.e[e] = (T)(r * (k - g[0][e] - h * g[1][e]));
+                const A h = fused((A)x.e[e], r, ch.shift[e]), av = w * h + ch.b[e];
+                if constexpr (MODE == 0) {
+                    o.e[e] = (T)act<ACT, A>(av);
                 } else {
-                    const A uv = (A)u.e[e], u1 = g[0][e], u2 = g[1][e], k2 = g[2][e];
-                    const A q = w * r * (uv - u1 - h * u2) + uw[e] * h + ub[e];
-                    const A v = w * (A)dy.e[e] * f2 * q + uw[e] * da - r * (uv * k2 + k * u2);
-                    o.e[e] = (T)(r * (v - g[3][e] - h * g[4][e]) - r * r * h * g[5][e]);
-                    o2.e[e] = (T)(f1 * q);
+                    A f1, f2;
+                    slopes<ACT, A>(av, f1, f2);
+                    o.e[e] = (T)(r * (w * (A)dy.e[e] * f1 - g[0][e] - h * g[1][e]));
                 }
             }
         }
         stp<T, VEC>(reinterpret_cast<T*>(a.y) + at, o);
         if constexpr (MODE == 2) stp<T, VEC>(reinterpret_cast<T*>(a.gdy) + at, o2);
+    }
+}
+
+// -- groups that a workgroup holds ---------------------------------------------------------------------------------------
+
+// 16 bytes of elements as they lie in memory: held as elements, each of 16 bits would have a register of its own.
+template <typename T> __device__ __forceinline__ Pack<T, 16 / (int)sizeof(T)> unpacked(uint4 w) {
+    Pack<T, 16 / (int)sizeof(T)> v;
+    __builtin_memcpy(&v, &w, 16);
+    return v;
+}
+__device__ __forceinline__ void opaque(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+
+// The next cell's arithmetic after this one's: side by side they take registers that hold other waves' elements.
+__device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0); }
+
+// The elements of a sample's tile of whole groups stay in registers between the sums and the outputs: one launch, every
+// tensor read once. R cells a thread, W waves; a thread's VEC channels lie in one group. Sums go from lanes to a wave, from
+// waves to a channel, and from channels to a group, through shared memory: lds holds [W][NS][tc] of the waves, then [NS][tc]
+// of the channels, and the groups' sums as doubles.
+template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bounds__(64 * W) void k_whole(Args a) {
+    using A = typename Acc<T>::type;
+    constexpr int VEC = 16 / (int)sizeof(T), NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5, NG = MODE == 2 ? 5 : NS;
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tc = a.tx * VEC;
+    A* waves = reinterpret_cast<A*>(shared);
+    A* chan = waves + W * NS * tc;
+    double* group = reinterpret_cast<double*>(chan + (NS + 2) * tc);  // [NG + 2][groups of the tile]
+    const int tile = (int)(blockIdx.x % a.tiles), width = a.tile;
+    const int64_t n = blockIdx.x / a.tiles;
+    const int c0 = tile * width, have = a.C - c0 < width ? a.C - c0 : width, groups = have / a.cg;
+    const int at = (t % a.tx) * VEC, c = c0 + at, ty = t / a.tx, step = 64 * W / a.tx;
+    const bool on = at < have;
+    const int L = (int)a.L;
+    const int64_t base = n * a.L * a.C + c;
+    const double m = (double)a.L * a.cg;
+    const int g = on ? at / a.cg : 0;
+
+    // every load unconditional: a thread without channels reads the tile's first, a row past the end the last
+    uint4 x[R], dy[MODE >= 1 ? R : 1], u[MODE == 2 ? R : 1];
+    const int64_t from = n * a.L * a.C + (on ? c : c0);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int l = ty + i * step;
+        const int64_t off = from + (int64_t)(l < L ? l : L - 1) * a.C;
+        x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + off);
+        if constexpr (MODE >= 1) dy[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.dy) + off);
+        if constexpr (MODE == 2) u[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.u) + off);
+    }
+    A w[VEC], b[VEC], r = 0, shift = 0;
+    params<A, VEC>(a.w, on ? c : c0, (A)1, w);
+    params<A, VEC>(a.b, on ? c : c0, (A)0, b);
+    if (MODE >= 1 && on) {
+        const A* st = reinterpret_cast<const A*>(a.stats) + (n * a.G + c / a.cg) * 2;
+        r = st[1];
+        shift = -st[0] * st[1];
+    }
+
+    // The elements stay as they came, packed: without this the compiler keeps them widened from the sums to the outputs, in
+    // twice the registers (bf16), and half the waves fit.
+    const auto pack_again = [&]() {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            opaque(x[i]);
+            if constexpr (MODE >= 1) opaque(dy[i]);
+            if constexpr (MODE == 2) opaque(u[i]);
+        }
+    };
+    // sums of the channels over all threads
+    const auto reduce = [&](auto& s) {
+        constexpr int K = sizeof(s) / sizeof(s[0]);
+        for (int d = a.tx; d < 64; d <<= 1)
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[i][e] += __shfl_xor(s[i][e], d, 64);
+        if (lane < a.tx)
+#pragma unroll
+            for (int i = 0; i < K; ++i) store_wide<A, VEC>(waves + (wave * K + i) * tc + lane * VEC, s[i]);
+        __syncthreads();
+        for (int i = t; i < K * tc; i += 64 * W) {
+            A v = waves[i];
+#pragma unroll
+            for (int q = 1; q < W; ++q) v += waves[q * K * tc + i];
+            chan[i] = v;
+        }
+        __syncthreads();
+    };
+    const auto weight = [&](int ch) { return (double)param<A>(a.w, c0 + ch, (A)1); };
+
+    if constexpr (MODE == 0) {
+        const auto grouped = [&]() {  // group[g] = the mean over a group of what chan holds
+            if (t < groups) {
+                double v = 0;
+                for (int i = 0; i < a.cg; ++i) v += (double)chan[t * a.cg + i];
+                group[t] = v / m;
+            }
+            __syncthreads();
+        };
+        A s[1][VEC] = {};
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (on && ty + i * step < L) {
+                const Pack<T, VEC> xv = unpacked<T>(x[i]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[0][e] += (A)xv.e[e];
+            }
+        pack_again();
+        reduce(s);
+        grouped();
+        const A mu = (A)group[g];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[0][e] = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (one_by_one(); on && ty + i * step < L) {
+                const Pack<T, VEC> xv = unpacked<T>(x[i]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const A d = (A)xv.e[e] - mu;
+                    s[0][e] += d * d;
+                }
+            }
+        pack_again();
+        reduce(s);
+        grouped();
+        r = (A)(1.0 / sqrt(group[g] + a.eps));
+        shift = -mu * r;
+        if (on && at % a.cg == 0 && ty == 0) {
+            A* st = reinterpret_cast<A*>(a.stats) + (n * a.G + c / a.cg) * 2;
+            st[0] = mu;
+            st[1] = r;
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int l = ty + i * step;
+            one_by_one();
+            if (!on || l >= L) continue;
+            const Pack<T, VEC> xv = unpacked<T>(x[i]);
+            Pack<T, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o.e[e] = (T)act<ACT, A>(w[e] * fused((A)xv.e[e], r, shift) + b[e]);
+            stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
+        }
+    } else {
+        A s[NS][VEC] = {};
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            one_by_one();
+            if (!on || ty + i * step >= L) continue;
+            const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]), uv = unpacked<T>(u[MODE == 2 ? i : 0]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, r, shift, w[e], b[e]);
+        }
+        pack_again();
+        reduce(s);
+        for (int i = t; i < NG * groups; i += 64 * W) {
+            const int gi = i % groups, k = i / groups;
+            double v = 0;
+            for (int j = 0; j < a.cg; ++j) {
+                const int ch = gi * a.cg + j;
+                v += (double)chan[k * tc + ch] * (MODE == 1 || k >= 2 ? weight(ch) : 1.0);
+            }
+            group[i] = v / m;
+        }
+        __syncthreads();
+        A* share = reinterpret_cast<A*>(a.chan) + n * 2 * a.C + c0;
+        if constexpr (MODE == 1) {
+            if (a.chan)
+                for (int i = t; i < have; i += 64 * W) {
+                    share[i] = chan[tc + i];
+                    share[a.C + i] = chan[i];
+                }
+            const A k1 = (A)group[g], k2 = (A)group[groups + g];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int l = ty + i * step;
+                one_by_one();
+            if (!on || l >= L) continue;
+                const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]);
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const A h = fused((A)xv.e[e], r, shift);
+                    A f1, f2;
+                    slopes<ACT, A>(w[e] * h + b[e], f1, f2);
+                    o.e[e] = (T)(r * (w[e] * (A)dv.e[e] * f1 - k1 - h * k2));
+                }
+                stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
+            }
+        } else {
+            for (int i = t; i < have; i += 64 * W) {
+                const int gi = i / a.cg;
+                double v[10] = {};
+#pragma unroll
+                for (int k = 0; k < NS; ++k) v[k] = (double)chan[k * tc + i];
+                const double rg = (double)reinterpret_cast<const A*>(a.stats)[(n * a.G + c0 / a.cg + gi) * 2 + 1];
+                const Second o = second<ACT>(v, weight(i), (double)param<A>(a.uw, c0 + i, (A)0),
+                                             (double)param<A>(a.ub, c0 + i, (A)0), rg, group[gi], group[groups + gi]);
+                chan[NS * tc + i] = (A)o.v1;
+                chan[(NS + 1) * tc + i] = (A)o.v2;
+                if (a.chan) {
+                    share[i] = (A)o.gw;
+                    share[a.C + i] = (A)o.t;
+                }
+            }
+            __syncthreads();
+            for (int i = t; i < 2 * groups; i += 64 * W) {
+                const int gi = i % groups, k = i / groups;
+                double v = 0;
+                for (int j = 0; j < a.cg; ++j) v += (double)chan[(NS + k) * tc + gi * a.cg + j];
+                group[5 * groups + i] = v / m;
+            }
+            __syncthreads();
+            const auto of = [&](int k) { return group[k * groups + g]; };
+            const double u1d = of(0), u2d = of(1), k1d = of(2), k2d = of(3), rd = (double)r;
+            const A u1 = (A)u1d, u2 = (A)u2d, k2 = (A)k2d, along = (A)(of(4) - k1d * u1d - u2d * k2d);
+            const A v1 = (A)(of(5) - rd * (u1d * k2d + k1d * u2d)), v2 = (A)(of(6) - 2.0 * rd * u2d * k2d);
+            A uw[VEC], ub[VEC];
+            params<A, VEC>(a.uw, on ? c : c0, (A)0, uw);
+            params<A, VEC>(a.ub, on ? c : c0, (A)0, ub);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int l = ty + i * step;
+                one_by_one();
+            if (!on || l >= L) continue;
+                const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]), uv = unpacked<T>(u[i]);
+                Pack<T, VEC> o, o2;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    A gx, gdy;
+                    second_out<ACT, A>((A)xv.e[e], (A)dv.e[e], (A)uv.e[e], r, shift, w[e], b[e], uw[e], ub[e], u1, u2, k2,
+                                       v1, v2, along, gx, gdy);
+                    o.e[e] = (T)gx;
+                    o2.e[e] = (T)gdy;
+                }
+                stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
+                stp<T, VEC>(reinterpret_cast<T*>(a.gdy) + base + (int64_t)l * a.C, o2);
+            }
+        }
     }
 }
 
@@ -506,6 +823,49 @@ struct Scratch {
     int64_t all() const { return part + means + chan; }
 };
 
+// Whether a workgroup holds a sample's tile of groups, and how: W waves of R cells a thread, tx threads across the tile's
+// channels. A thread's vector has to lie in one group, and a tile of whole groups to fill three quarters of the threads
+// across; 8 threads are 128 bytes of a cell. The second derivative, with 80 sums and three tensors in registers, has 4 waves.
+// Above their cells (256 of the second derivative, 1,024 of the others at 8 threads across) k_sums and k_apply read twice.
+struct Whole {
+    int waves = 0, cells = 0, tx = 0, tile = 0, tiles = 0;
+    Whole(int mode, int dtype, int64_t L, int C, int groups, bool vector) {
+        const int vec = vector_of(dtype, C), cg = C / groups;
+        if (!vector || dtype == EBR_DTYPE_F64 || vec == 1 || cg % vec || L > 4096) return;
+        for (int x = 8; x <= (mode == 2 ? 32 : 64); x *= 2) {
+            const int t = x * vec / cg * cg;
+            if (t * 4 < x * vec * 3 && t < C) continue;
+            if (t == 0) continue;
+            for (const int w : {4, 16}) {
+                if (w == 16 && (mode == 2 || x > 32)) continue;  // (shared memory)
+                const int64_t step = 64 * w / x;
+                const int r = (int)((L + step - 1) / step);
+                if (r > 8 || (w == 4 && r > 4 && mode != 2)) continue;
+                waves = w;
+                cells = r <= 4 ? 4 : 8;
+                tx = x;
+                tile = t < C ? t : C;
+                tiles = (C + tile - 1) / tile;
+                return;
+            }
+        }
+    }
+};
+
+template <typename T, int MODE, int ACT> static void launch_whole(hipStream_t s, const Whole& h, const Args& a) {
+    using A = typename Acc<T>::type;
+    constexpr int VEC = 16 / (int)sizeof(T), NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5;
+    const int tc = h.tx * VEC;
+    const size_t lds = ((size_t)h.waves * NS + NS + 2) * tc * sizeof(A) + (size_t)(NS + 7) * (h.tile / a.cg) * sizeof(double);
+    const dim3 grid((unsigned)(a.B * h.tiles)), block(64 * h.waves);
+    if (h.waves == 4 && h.cells == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 4, 4>), grid, block, lds, s, a);
+    else if (h.waves == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 8, 4>), grid, block, lds, s, a);
+    else if constexpr (MODE != 2) {
+        if (h.cells == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 4, 16>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((k_whole<T, MODE, ACT, 8, 16>), grid, block, lds, s, a);
+    }
+}
+
 template <int MODE> static int run(int dtype, int act, Args a, void* scratch, void* stream) {
     const bool vector = vector_of(dtype, a.C) > 1 && all_aligned({a.x, a.dy, a.u, a.y, a.gdy});
     const Plan p(dtype, a.B, a.L, a.C, vector);
@@ -519,17 +879,29 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
     a.tiles = p.tiles;
     a.splits = p.splits;
     a.rows = p.rows;
-    const int64_t blocks = a.B * p.splits * p.tiles;
+    const Whole h(MODE, dtype, a.L, a.C, a.G, vector);
+    const int64_t blocks = h.waves ? a.B * h.tiles * (h.waves / 4) : a.B * p.splits * p.tiles;
     if (blocks > MAX_BLOCKS) return EBR_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     by_kind(dtype, vector, act, [&](auto v, auto n, auto f) {
         using T = decltype(v);
         using A = typename Acc<T>::type;
         constexpr int VEC = decltype(n)::value, ACT = decltype(f)::value;
+        if (h.waves) {
+            if constexpr (VEC > 1 && sizeof(T) < 8) {
+                a.tx = h.tx;
+                a.tile = h.tile;
+                a.tiles = h.tiles;
+                launch_whole<T, MODE, ACT>(s, h, a);
+            }
+            if (MODE != 0 && a.chan) hipLaunchKernelGGL((k_params<A>), dim3((a.C + 31) / 32, 2), dim3(1024), 0, s, a);
+            return;
+        }
         hipLaunchKernelGGL((k_sums<T, VEC, MODE, ACT>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a);
-        hipLaunchKernelGGL((k_means<A, MODE, ACT>), dim3((unsigned)(a.B * a.G)), dim3(a.cg > 64 ? THREADS : 64), 0, s, a);
+        hipLaunchKernelGGL((k_means<A, MODE, ACT>), dim3((unsigned)(a.B * a.G)), dim3(a.cg * (int64_t)a.splits > 64 ? THREADS : 64),
+                           0, s, a);
         hipLaunchKernelGGL((k_apply<T, VEC, MODE, ACT>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a);
-        if (MODE != 0 && a.chan) hipLaunchKernelGGL((k_params<A>), dim3((a.C + 63) / 64, 2), dim3(1024), 0, s, a);
+        if (MODE != 0 && a.chan) hipLaunchKernelGGL((k_params<A>), dim3((a.C + 31) / 32, 2), dim3(1024), 0, s, a);
     });
     return launched();
 }

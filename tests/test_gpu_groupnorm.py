@@ -132,6 +132,19 @@ def test_group_norm(cuda, dtype, act, shape, G):
     _check(ts["x"], G, ts["w"], ts["b"], act, ts["dy"], ts["u"], ts["uw"], ts["ub"])
 
 
+# groups that a workgroup holds: tiles of every width, an end of the channels and of the cells inside a tile, four and eight
+# cells a thread, 4 and 16 waves; and the sizes on either side of where it no longer does
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,G", [
+    ((2, 32, 64), 8), ((2, 33, 64), 4), ((3, 128, 96), 4), ((2, 129, 96), 4), ((2, 256, 64), 2), ((2, 257, 64), 2), ((2, 5, 512), 1),
+    ((2, 130, 256), 2), ((1, 1024, 64), 8), ((1, 1025, 64), 8), ((2, 500, 128), 2), ((3, 17, 144), 3), ((1, 60, 2048), 4), ((700, 4, 64), 4),
+])  # fmt: skip
+def test_held_groups(cuda, dtype, shape, G):
+    _say(f"group_norm held {shape} {G} {dtype}")
+    ts = _inputs(cuda, shape, dtype, seed=shape[-1] + G)
+    _check(ts["x"], G, ts["w"], ts["b"], "silu", ts["dy"], ts["u"], ts["uw"], ts["ub"])
+
+
 @pytest.mark.parametrize("act", [None, "silu"])
 @pytest.mark.parametrize("have", ["", "w", "b"])
 def test_parameters_left_out(cuda, act, have):
