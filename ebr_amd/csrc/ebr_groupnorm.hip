@@ -522,49 +522,48 @@ __device__ __forceinline__ void opaque(uint4& w) { asm volatile("" : "+v"(w.x), 
 __device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0); }
 
 // The elements of a sample's tile of whole groups stay in registers between the sums and the outputs: one launch, every
-// tensor read once. R cells a thread, W waves; a thread's VEC channels lie in one group. Sums go from lanes to a wave, from
-// waves to a channel, and from channels to a group, through shared memory: lds holds [W][NS][tc] of the waves, then [NS][tc]
-// of the channels, and the groups' sums as doubles.
+// tensor read once. R cells a thread, W waves; a thread's VEC channels lie in one group.
+//
+// A thread sums its own cells by channel. All that follows is linear in these sums, so a thread takes them to its group's
+// means by itself, and what goes through shared memory is one number a thread for each mean (five and then two of the second
+// derivative, in place of ten for each channel), and for the parameters' gradients, where they are wanted, two a channel.
+// With every channel's sums reduced, the second derivative of 768 boards of 81 x 512 took 224 us, most of it that reduction.
 template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bounds__(64 * W) void k_whole(Args a) {
     using A = typename Acc<T>::type;
     constexpr int VEC = 16 / (int)sizeof(T), NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5, NG = MODE == 2 ? 5 : NS;
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tc = a.tx * VEC;
-    A* waves = reinterpret_cast<A*>(shared);
-    A* chan = waves + W * NS * tc;
-    double* group = reinterpret_cast<double*>(chan + (NS + 2) * tc);  // [NG + 2][groups of the tile]
-    const int tile = (int)(blockIdx.x % a.tiles), width = a.tile;
+    A* waves = reinterpret_cast<A*>(shared);  // [W][NG][tx], and [W][2][tc]
+    A* cols = waves + W * 2 * tc;             // [NG][tx]
+    const int tile = (int)(blockIdx.x % a.tiles);
     const int64_t n = blockIdx.x / a.tiles;
-    const int c0 = tile * width, have = a.C - c0 < width ? a.C - c0 : width, groups = have / a.cg;
-    const int at = (t % a.tx) * VEC, c = c0 + at, ty = t / a.tx, step = 64 * W / a.tx;
+    const int c0 = tile * a.tile, have = a.C - c0 < a.tile ? a.C - c0 : a.tile;
+    const int at = (t % a.tx) * VEC, ty = t / a.tx, step = 64 * W / a.tx;
     const bool on = at < have;
+    const int c = on ? c0 + at : c0, g = c / a.cg, gcols = a.cg / VEC, gfrom = (c - c0) / a.cg * gcols;
     const int L = (int)a.L;
     const int64_t base = n * a.L * a.C + c;
     const double m = (double)a.L * a.cg;
-    const int g = on ? at / a.cg : 0;
 
     // every load unconditional: a thread without channels reads the tile's first, a row past the end the last
     uint4 x[R], dy[MODE >= 1 ? R : 1], u[MODE == 2 ? R : 1];
-    const int64_t from = n * a.L * a.C + (on ? c : c0);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int l = ty + i * step;
-        const int64_t off = from + (int64_t)(l < L ? l : L - 1) * a.C;
+        const int64_t off = base + (int64_t)(l < L ? l : L - 1) * a.C;
         x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + off);
         if constexpr (MODE >= 1) dy[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.dy) + off);
         if constexpr (MODE == 2) u[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.u) + off);
     }
     A w[VEC], b[VEC], r = 0, shift = 0;
-    params<A, VEC>(a.w, on ? c : c0, (A)1, w);
-    params<A, VEC>(a.b, on ? c : c0, (A)0, b);
-    if (MODE >= 1 && on) {
-        const A* st = reinterpret_cast<const A*>(a.stats) + (n * a.G + c / a.cg) * 2;
+    params<A, VEC>(a.w, c, (A)1, w);
+    params<A, VEC>(a.b, c, (A)0, b);
+    if constexpr (MODE >= 1) {
+        const A* st = reinterpret_cast<const A*>(a.stats) + (n * a.G + g) * 2;
         r = st[1];
         shift = -st[0] * st[1];
     }
-
-    // The elements stay as they came, packed: without this the compiler keeps them widened from the sums to the outputs, in
-    // twice the registers (bf16), and half the waves fit.
+    // Between the sums and the outputs the elements stay packed as they came, or they take twice the registers.
     const auto pack_again = [&]() {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -573,68 +572,83 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
             if constexpr (MODE == 2) opaque(u[i]);
         }
     };
-    // sums of the channels over all threads
-    const auto reduce = [&](auto& s) {
-        constexpr int K = sizeof(s) / sizeof(s[0]);
+    // p's means over this thread's group: over the wave's threads of the same channels, over the waves, over the channels
+    const auto means = [&](auto& p, double* out) {
+        constexpr int K = sizeof(p) / sizeof(p[0]);
         for (int d = a.tx; d < 64; d <<= 1)
 #pragma unroll
-            for (int i = 0; i < K; ++i)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) s[i][e] += __shfl_xor(s[i][e], d, 64);
+            for (int k = 0; k < K; ++k) p[k] += __shfl_xor(p[k], d, 64);
         if (lane < a.tx)
 #pragma unroll
-            for (int i = 0; i < K; ++i) store_wide<A, VEC>(waves + (wave * K + i) * tc + lane * VEC, s[i]);
+            for (int k = 0; k < K; ++k) waves[(wave * K + k) * a.tx + lane] = p[k];
         __syncthreads();
-        for (int i = t; i < K * tc; i += 64 * W) {
+        for (int i = t; i < K * a.tx; i += 64 * W) {
             A v = waves[i];
 #pragma unroll
-            for (int q = 1; q < W; ++q) v += waves[q * K * tc + i];
-            chan[i] = v;
+            for (int q = 1; q < W; ++q) v += waves[q * K * a.tx + i];
+            cols[i] = v;
         }
         __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            double v = 0;
+            for (int i = 0; i < gcols; ++i) v += (double)cols[k * a.tx + gfrom + i];
+            out[k] = v / m;
+        }
     };
-    const auto weight = [&](int ch) { return (double)param<A>(a.w, c0 + ch, (A)1); };
+    // the sample's share of the parameters' gradients
+    const auto shares = [&](A (&pw)[VEC], A (&pb)[VEC]) {
+        for (int d = a.tx; d < 64; d <<= 1)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                pw[e] += __shfl_xor(pw[e], d, 64);
+                pb[e] += __shfl_xor(pb[e], d, 64);
+            }
+        if (lane < a.tx) {
+            store_wide<A, VEC>(waves + wave * 2 * tc + lane * VEC, pw);
+            store_wide<A, VEC>(waves + (wave * 2 + 1) * tc + lane * VEC, pb);
+        }
+        __syncthreads();
+        A* share = reinterpret_cast<A*>(a.chan) + n * 2 * a.C + c0;
+        for (int i = t; i < 2 * tc; i += 64 * W) {
+            if (i % tc >= have) continue;
+            A v = waves[i];
+#pragma unroll
+            for (int q = 1; q < W; ++q) v += waves[q * 2 * tc + i];
+            share[i < tc ? i : a.C + i - tc] = v;
+        }
+    };
 
     if constexpr (MODE == 0) {
-        const auto grouped = [&]() {  // group[g] = the mean over a group of what chan holds
-            if (t < groups) {
-                double v = 0;
-                for (int i = 0; i < a.cg; ++i) v += (double)chan[t * a.cg + i];
-                group[t] = v / m;
-            }
-            __syncthreads();
-        };
-        A s[1][VEC] = {};
+        double v[1];
+        A p[1] = {0};
 #pragma unroll
         for (int i = 0; i < R; ++i)
             if (on && ty + i * step < L) {
                 const Pack<T, VEC> xv = unpacked<T>(x[i]);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s[0][e] += (A)xv.e[e];
+                for (int e = 0; e < VEC; ++e) p[0] += (A)xv.e[e];
             }
         pack_again();
-        reduce(s);
-        grouped();
-        const A mu = (A)group[g];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[0][e] = 0;
+        means(p, v);
+        const A mu = (A)v[0];
+        p[0] = 0;
 #pragma unroll
         for (int i = 0; i < R; ++i)
-            if (one_by_one(); on && ty + i * step < L) {
+            if (on && ty + i * step < L) {
                 const Pack<T, VEC> xv = unpacked<T>(x[i]);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const A d = (A)xv.e[e] - mu;
-                    s[0][e] += d * d;
+                    p[0] += d * d;
                 }
             }
         pack_again();
-        reduce(s);
-        grouped();
-        r = (A)(1.0 / sqrt(group[g] + a.eps));
+        means(p, v);
+        r = (A)(1.0 / sqrt(v[0] + a.eps));
         shift = -mu * r;
         if (on && at % a.cg == 0 && ty == 0) {
-            A* st = reinterpret_cast<A*>(a.stats) + (n * a.G + c / a.cg) * 2;
+            A* st = reinterpret_cast<A*>(a.stats) + (n * a.G + g) * 2;
             st[0] = mu;
             st[1] = r;
         }
@@ -661,30 +675,21 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
                 add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, r, shift, w[e], b[e]);
         }
         pack_again();
-        reduce(s);
-        for (int i = t; i < NG * groups; i += 64 * W) {
-            const int gi = i % groups, k = i / groups;
-            double v = 0;
-            for (int j = 0; j < a.cg; ++j) {
-                const int ch = gi * a.cg + j;
-                v += (double)chan[k * tc + ch] * (MODE == 1 || k >= 2 ? weight(ch) : 1.0);
-            }
-            group[i] = v / m;
-        }
-        __syncthreads();
-        A* share = reinterpret_cast<A*>(a.chan) + n * 2 * a.C + c0;
+        A p[NG] = {};
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+#pragma unroll
+            for (int k = 0; k < NG; ++k) p[k] += MODE == 1 || k >= 2 ? w[e] * s[k][e] : s[k][e];
+        double v[NG];
+        means(p, v);
         if constexpr (MODE == 1) {
-            if (a.chan)
-                for (int i = t; i < have; i += 64 * W) {
-                    share[i] = chan[tc + i];
-                    share[a.C + i] = chan[i];
-                }
-            const A k1 = (A)group[g], k2 = (A)group[groups + g];
+            if (a.chan) shares(s[1], s[0]);
+            const A k1 = (A)v[0], k2 = (A)v[1];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int l = ty + i * step;
                 one_by_one();
-            if (!on || l >= L) continue;
+                if (!on || l >= L) continue;
                 const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]);
                 Pack<T, VEC> o;
 #pragma unroll
@@ -697,48 +702,40 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
                 stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
             }
         } else {
-            for (int i = t; i < have; i += 64 * W) {
-                const int gi = i / a.cg;
-                double v[10] = {};
+            const double u1d = v[0], u2d = v[1], k1d = v[2], k2d = v[3], rd = (double)r;
+            const A u1 = (A)u1d, u2 = (A)u2d, k2 = (A)k2d, along = (A)(v[4] - k1d * u1d - u2d * k2d);
+            A uw[VEC], ub[VEC], gw[VEC], gb[VEC], q[2] = {0, 0};
+            params<A, VEC>(a.uw, c, (A)0, uw);
+            params<A, VEC>(a.ub, c, (A)0, ub);
 #pragma unroll
-                for (int k = 0; k < NS; ++k) v[k] = (double)chan[k * tc + i];
-                const double rg = (double)reinterpret_cast<const A*>(a.stats)[(n * a.G + c0 / a.cg + gi) * 2 + 1];
-                const Second o = second<ACT>(v, weight(i), (double)param<A>(a.uw, c0 + i, (A)0),
-                                             (double)param<A>(a.ub, c0 + i, (A)0), rg, group[gi], group[groups + gi]);
-                chan[NS * tc + i] = (A)o.v1;
-                chan[(NS + 1) * tc + i] = (A)o.v2;
-                if (a.chan) {
-                    share[i] = (A)o.gw;
-                    share[a.C + i] = (A)o.t;
+            for (int e = 0; e < VEC; ++e) {
+                A th = 0;
+                gb[e] = 0;
+                if constexpr (ACT != 0) {  // q = cu u + ch h + cc
+                    const A cu = w[e] * r, ch = uw[e] - cu * u2, cc = ub[e] - cu * u1;
+                    gb[e] = cu * s[8][e] + ch * s[6][e] + cc * s[5][e];
+                    th = cu * s[9][e] + ch * s[7][e] + cc * s[6][e];
                 }
+                q[0] += w[e] * gb[e] + uw[e] * s[2][e];
+                q[1] += w[e] * th + uw[e] * s[3][e];
+                gw[e] = r * (s[4][e] - u1 * s[2][e] - u2 * s[3][e]) + th;
             }
-            __syncthreads();
-            for (int i = t; i < 2 * groups; i += 64 * W) {
-                const int gi = i % groups, k = i / groups;
-                double v = 0;
-                for (int j = 0; j < a.cg; ++j) v += (double)chan[(NS + k) * tc + gi * a.cg + j];
-                group[5 * groups + i] = v / m;
-            }
-            __syncthreads();
-            const auto of = [&](int k) { return group[k * groups + g]; };
-            const double u1d = of(0), u2d = of(1), k1d = of(2), k2d = of(3), rd = (double)r;
-            const A u1 = (A)u1d, u2 = (A)u2d, k2 = (A)k2d, along = (A)(of(4) - k1d * u1d - u2d * k2d);
-            const A v1 = (A)(of(5) - rd * (u1d * k2d + k1d * u2d)), v2 = (A)(of(6) - 2.0 * rd * u2d * k2d);
-            A uw[VEC], ub[VEC];
-            params<A, VEC>(a.uw, on ? c : c0, (A)0, uw);
-            params<A, VEC>(a.ub, on ? c : c0, (A)0, ub);
+            double z[2];
+            means(q, z);
+            if (a.chan) shares(gw, gb);
+            const A v1 = (A)(z[0] - rd * (u1d * k2d + k1d * u2d)), v2 = (A)(z[1] - 2.0 * rd * u2d * k2d);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int l = ty + i * step;
                 one_by_one();
-            if (!on || l >= L) continue;
+                if (!on || l >= L) continue;
                 const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]), uv = unpacked<T>(u[i]);
                 Pack<T, VEC> o, o2;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     A gx, gdy;
-                    second_out<ACT, A>((A)xv.e[e], (A)dv.e[e], (A)uv.e[e], r, shift, w[e], b[e], uw[e], ub[e], u1, u2, k2,
-                                       v1, v2, along, gx, gdy);
+                    second_out<ACT, A>((A)xv.e[e], (A)dv.e[e], (A)uv.e[e], r, shift, w[e], b[e], uw[e], ub[e], u1, u2, k2, v1, v2,
+                                       along, gx, gdy);
                     o.e[e] = (T)gx;
                     o2.e[e] = (T)gdy;
                 }
@@ -829,6 +826,7 @@ struct Scratch {
 // Above their cells (256 of the second derivative, 1,024 of the others at 8 threads across) k_sums and k_apply read twice.
 struct Whole {
     int waves = 0, cells = 0, tx = 0, tile = 0, tiles = 0;
+    static constexpr int few(int mode) { return mode == 2 ? 3 : 4; }  // of the second derivative's three, a third wave fits
     Whole(int mode, int dtype, int64_t L, int C, int groups, bool vector) {
         const int vec = vector_of(dtype, C), cg = C / groups;
         if (!vector || dtype == EBR_DTYPE_F64 || vec == 1 || cg % vec || L > 4096) return;
@@ -842,7 +840,7 @@ struct Whole {
                 const int r = (int)((L + step - 1) / step);
                 if (r > 8 || (w == 4 && r > 4 && mode != 2)) continue;
                 waves = w;
-                cells = r <= 4 ? 4 : 8;
+                cells = r <= few(mode) ? few(mode) : 8;
                 tx = x;
                 tile = t < C ? t : C;
                 tiles = (C + tile - 1) / tile;
@@ -854,14 +852,14 @@ struct Whole {
 
 template <typename T, int MODE, int ACT> static void launch_whole(hipStream_t s, const Whole& h, const Args& a) {
     using A = typename Acc<T>::type;
-    constexpr int VEC = 16 / (int)sizeof(T), NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5;
-    const int tc = h.tx * VEC;
-    const size_t lds = ((size_t)h.waves * NS + NS + 2) * tc * sizeof(A) + (size_t)(NS + 7) * (h.tile / a.cg) * sizeof(double);
+    constexpr int VEC = 16 / (int)sizeof(T);
+    constexpr int FEW = Whole::few(MODE);
+    const size_t lds = ((size_t)h.waves * 2 * h.tx * VEC + 5 * h.tx) * sizeof(A);
     const dim3 grid((unsigned)(a.B * h.tiles)), block(64 * h.waves);
-    if (h.waves == 4 && h.cells == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 4, 4>), grid, block, lds, s, a);
+    if (h.waves == 4 && h.cells == FEW) hipLaunchKernelGGL((k_whole<T, MODE, ACT, FEW, 4>), grid, block, lds, s, a);
     else if (h.waves == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 8, 4>), grid, block, lds, s, a);
     else if constexpr (MODE != 2) {
-        if (h.cells == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 4, 16>), grid, block, lds, s, a);
+        if (h.cells == FEW) hipLaunchKernelGGL((k_whole<T, MODE, ACT, FEW, 16>), grid, block, lds, s, a);
         else hipLaunchKernelGGL((k_whole<T, MODE, ACT, 8, 16>), grid, block, lds, s, a);
     }
 }
