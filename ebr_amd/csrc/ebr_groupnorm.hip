@@ -510,13 +510,16 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
 
 // -- groups that a workgroup holds ---------------------------------------------------------------------------------------
 
-// 16 bytes of elements as they lie in memory: held as elements, each of 16 bits would have a register of its own.
-template <typename T> __device__ __forceinline__ Pack<T, 16 / (int)sizeof(T)> unpacked(uint4 w) {
-    Pack<T, 16 / (int)sizeof(T)> v;
-    __builtin_memcpy(&v, &w, 16);
+// Elements as they lie in memory: held as elements, each of 16 bits would have a register of its own.
+template <int BYTES> struct Words { using type = uint4; };
+template <> struct Words<8> { using type = uint2; };
+template <typename T, int VEC, typename W> __device__ __forceinline__ Pack<T, VEC> unpacked(W w) {
+    Pack<T, VEC> v;
+    __builtin_memcpy(&v, &w, sizeof(v));
     return v;
 }
 __device__ __forceinline__ void opaque(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+__device__ __forceinline__ void opaque(uint2& w) { asm volatile("" : "+v"(w.x), "+v"(w.y)); }
 
 // The next cell's arithmetic after this one's: side by side they take registers that hold other waves' elements.
 __device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0); }
@@ -528,9 +531,11 @@ __device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0)
 // means by itself, and what goes through shared memory is one number a thread for each mean (five and then two of the second
 // derivative, in place of ten for each channel), and for the parameters' gradients, where they are wanted, two a channel.
 // With every channel's sums reduced, the second derivative of 768 boards of 81 x 512 took 224 us, most of it that reduction.
-template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bounds__(64 * W) void k_whole(Args a) {
+template <typename T, int VEC, int MODE, int ACT, int R, int W>
+__global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(Args a) {
     using A = typename Acc<T>::type;
-    constexpr int VEC = 16 / (int)sizeof(T), NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5, NG = MODE == 2 ? 5 : NS;
+    using Raw = typename Words<VEC * (int)sizeof(T)>::type;
+    constexpr int NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5, NG = MODE == 2 ? 5 : NS;
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tc = a.tx * VEC;
     A* waves = reinterpret_cast<A*>(shared);  // [W][NG][tx], and [W][2][tc]
@@ -545,15 +550,16 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
     const int64_t base = n * a.L * a.C + c;
     const double m = (double)a.L * a.cg;
 
-    // every load unconditional: a thread without channels reads the tile's first, a row past the end the last
-    uint4 x[R], dy[MODE >= 1 ? R : 1], u[MODE == 2 ? R : 1];
+    // no load depends on the thread: one without channels reads the tile's first, and a cell past the end is the last
+    Raw x[R], dy[MODE >= 1 ? R : 1], u[MODE == 2 ? R : 1];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
+        if (MODE == 2 && i * step >= L) break;  // (in the others this costs registers)
         const int l = ty + i * step;
         const int64_t off = base + (int64_t)(l < L ? l : L - 1) * a.C;
-        x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + off);
-        if constexpr (MODE >= 1) dy[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.dy) + off);
-        if constexpr (MODE == 2) u[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.u) + off);
+        x[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.x) + off);
+        if constexpr (MODE >= 1) dy[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.dy) + off);
+        if constexpr (MODE == 2) u[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.u) + off);
     }
     A w[VEC], b[VEC], r = 0, shift = 0;
     params<A, VEC>(a.w, c, (A)1, w);
@@ -625,7 +631,7 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
 #pragma unroll
         for (int i = 0; i < R; ++i)
             if (on && ty + i * step < L) {
-                const Pack<T, VEC> xv = unpacked<T>(x[i]);
+                const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) p[0] += (A)xv.e[e];
             }
@@ -636,7 +642,7 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
 #pragma unroll
         for (int i = 0; i < R; ++i)
             if (on && ty + i * step < L) {
-                const Pack<T, VEC> xv = unpacked<T>(x[i]);
+                const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const A d = (A)xv.e[e] - mu;
@@ -657,7 +663,7 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
             const int l = ty + i * step;
             one_by_one();
             if (!on || l >= L) continue;
-            const Pack<T, VEC> xv = unpacked<T>(x[i]);
+            const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]);
             Pack<T, VEC> o;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) o.e[e] = (T)act<ACT, A>(w[e] * fused((A)xv.e[e], r, shift) + b[e]);
@@ -669,7 +675,7 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
         for (int i = 0; i < R; ++i) {
             one_by_one();
             if (!on || ty + i * step >= L) continue;
-            const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]), uv = unpacked<T>(u[MODE == 2 ? i : 0]);
+            const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]), uv = unpacked<T, VEC>(u[MODE == 2 ? i : 0]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, r, shift, w[e], b[e]);
@@ -690,7 +696,7 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
                 const int l = ty + i * step;
                 one_by_one();
                 if (!on || l >= L) continue;
-                const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]);
+                const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]);
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
@@ -729,7 +735,7 @@ template <typename T, int MODE, int ACT, int R, int W> __global__ __launch_bound
                 const int l = ty + i * step;
                 one_by_one();
                 if (!on || l >= L) continue;
-                const Pack<T, VEC> xv = unpacked<T>(x[i]), dv = unpacked<T>(dy[i]), uv = unpacked<T>(u[i]);
+                const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]), uv = unpacked<T, VEC>(u[i]);
                 Pack<T, VEC> o, o2;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
@@ -826,11 +832,14 @@ struct Scratch {
 // Above their cells (256 of the second derivative, 1,024 of the others at 8 threads across) k_sums and k_apply read twice.
 struct Whole {
     int waves = 0, cells = 0, tx = 0, tile = 0, tiles = 0;
-    static constexpr int few(int mode) { return mode == 2 ? 3 : 4; }  // of the second derivative's three, a third wave fits
+    // the two numbers of cells that there are kernels for
+    static constexpr int few(int mode, bool wide) { return mode != 2 ? 4 : wide ? 3 : 6; }
+    static constexpr int many(int mode, bool wide) { return mode != 2 || wide ? 8 : 16; }
     Whole(int mode, int dtype, int64_t L, int C, int groups, bool vector) {
-        const int vec = vector_of(dtype, C), cg = C / groups;
+        const int vec = mode == 2 ? 4 : vector_of(dtype, C), cg = C / groups;
         if (!vector || dtype == EBR_DTYPE_F64 || vec == 1 || cg % vec || L > 4096) return;
-        for (int x = 8; x <= (mode == 2 ? 32 : 64); x *= 2) {
+        const bool wide = dtype == EBR_DTYPE_F32;
+        for (int x = !wide && vec == 4 ? 16 : 8; x <= 64; x *= 2) {
             const int t = x * vec / cg * cg;
             if (t * 4 < x * vec * 3 && t < C) continue;
             if (t == 0) continue;
@@ -838,9 +847,9 @@ struct Whole {
                 if (w == 16 && (mode == 2 || x > 32)) continue;  // (shared memory)
                 const int64_t step = 64 * w / x;
                 const int r = (int)((L + step - 1) / step);
-                if (r > 8 || (w == 4 && r > 4 && mode != 2)) continue;
+                if (r > many(mode, wide) || (w == 4 && r > 4 && mode != 2)) continue;
                 waves = w;
-                cells = r <= few(mode) ? few(mode) : 8;
+                cells = r <= few(mode, wide) ? few(mode, wide) : many(mode, wide);
                 tx = x;
                 tile = t < C ? t : C;
                 tiles = (C + tile - 1) / tile;
@@ -852,15 +861,15 @@ struct Whole {
 
 template <typename T, int MODE, int ACT> static void launch_whole(hipStream_t s, const Whole& h, const Args& a) {
     using A = typename Acc<T>::type;
-    constexpr int VEC = 16 / (int)sizeof(T);
-    constexpr int FEW = Whole::few(MODE);
+    constexpr bool WIDE = sizeof(T) == 4;
+    constexpr int VEC = MODE == 2 ? 4 : 16 / (int)sizeof(T), FEW = Whole::few(MODE, WIDE), MANY = Whole::many(MODE, WIDE);
     const size_t lds = ((size_t)h.waves * 2 * h.tx * VEC + 5 * h.tx) * sizeof(A);
     const dim3 grid((unsigned)(a.B * h.tiles)), block(64 * h.waves);
-    if (h.waves == 4 && h.cells == FEW) hipLaunchKernelGGL((k_whole<T, MODE, ACT, FEW, 4>), grid, block, lds, s, a);
-    else if (h.waves == 4) hipLaunchKernelGGL((k_whole<T, MODE, ACT, 8, 4>), grid, block, lds, s, a);
+    if (h.waves == 4 && h.cells == FEW) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, FEW, 4>), grid, block, lds, s, a);
+    else if (h.waves == 4) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, MANY, 4>), grid, block, lds, s, a);
     else if constexpr (MODE != 2) {
-        if (h.cells == FEW) hipLaunchKernelGGL((k_whole<T, MODE, ACT, FEW, 16>), grid, block, lds, s, a);
-        else hipLaunchKernelGGL((k_whole<T, MODE, ACT, 8, 16>), grid, block, lds, s, a);
+        if (h.cells == FEW) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, FEW, 16>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, MANY, 16>), grid, block, lds, s, a);
     }
 }
 
