@@ -337,21 +337,21 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
     const auto cells = [&](int s) { return (double)(s + 1 < a.splits ? a.rows : a.L - s * a.rows); };
     A* stats = reinterpret_cast<A*>(a.stats) + (n * a.G + g) * 2;
     if constexpr (MODE == 0) {
-        double v[1] = {0};
+        // about the first part's first mean, in 64 bits: one pass over the parts
+        const double about = (double)part[c0];
+        double v[2] = {0, 0};
         for (int c = tc; c < a.cg; c += cols)
-            for (int s = ts; s < a.splits; s += lanes) v[0] += cells(s) * (double)part[(int64_t)s * 2 * a.C + c0 + c];
-        all_sums<1>(v, lds);
-        const double mu = v[0] / m;
-        v[0] = 0;
-        for (int c = tc; c < a.cg; c += cols)
+#pragma unroll 4
             for (int s = ts; s < a.splits; s += lanes) {
-                const double d = (double)part[(int64_t)s * 2 * a.C + c0 + c] - mu;
-                v[0] += (double)part[((int64_t)s * 2 + 1) * a.C + c0 + c] + cells(s) * d * d;
+                const double d = (double)part[(int64_t)s * 2 * a.C + c0 + c] - about;
+                v[0] += cells(s) * d;
+                v[1] += (double)part[((int64_t)s * 2 + 1) * a.C + c0 + c] + cells(s) * d * d;
             }
-        all_sums<1>(v, lds);
+        all_sums<2>(v, lds);
+        const double mu = about + v[0] / m, var = v[1] / m - (v[0] / m) * (v[0] / m);
         if (threadIdx.x == 0) {
             stats[0] = (A)mu;
-            stats[1] = (A)(1.0 / sqrt(v[0] / m + a.eps));
+            stats[1] = (A)(1.0 / sqrt((var > 0 ? var : var == var ? 0.0 : var) + a.eps));
         }
         return;
     }
@@ -770,7 +770,7 @@ static int vector_of(int dtype, int C) {
 }
 
 // How the work is laid out, from the sizes alone: 16 threads of 16 bytes take 256 bytes of each cell; parts of L as many
-// as give the card about eight workgroups for each of its 256 compute units, with at least 8 cells for each thread.
+// as give the card about four workgroups for each of its 256 compute units, with at least 8 cells for each thread.
 struct Plan {
     int vec, tx, tiles, splits;
     int64_t rows;
@@ -780,7 +780,7 @@ struct Plan {
         while (tx < (vec > 1 ? 16 : 64) && tx * vec < C) tx *= 2;
         tiles = (C + tx * vec - 1) / (tx * vec);
         const int64_t step = THREADS / tx, least = 8 * step;
-        int64_t s = 2048 / (B * tiles);
+        int64_t s = 1024 / (B * tiles);
         if (s > (L + least - 1) / least) s = (L + least - 1) / least;
         if (s < 1) s = 1;
         rows = (L + s - 1) / s;
