@@ -38,6 +38,7 @@ struct Args {
     int64_t N, row;  // row: elements from one row of x to the next
     int V, K, teacher_type, wide;
     double k;  // log2 e / T
+    float k_low;  // what k lacks in 32 bits
     double weight;  // forward: T^2 ln 2; backward: T
     int reduction;
     void *stats, *loss, *scale, *part;
@@ -48,9 +49,22 @@ struct Args {
     void* soft;         // [N][splits]: a part's maximum and sum
 };
 
-// What a row's softmaxes need: its largest logit and log2 of the sum above it, the teacher's alike. tm is -inf for a row
-// that is not counted.
-template <typename A> struct alignas(4 * sizeof(A)) Stats { A m, s2, tm, ts2; };
+// What a row's softmaxes need: its largest logit and the sum above it, the teacher's alike. ts is 0 for a row that is not
+// counted.
+template <typename A> struct alignas(4 * sizeof(A)) Stats { A m, s, tm, ts; };
+
+// The factor of exponents: d times it in base 2. At 32 bits its own rounding would be a relative error of every exponent,
+// 3e-8 of up to some 30 in a small probability; FINE adds what it lacks. 16-bit outputs do without.
+template <typename A, bool FINE> struct Base {
+    A k, low;
+    __device__ __forceinline__ explicit Base(const Args& a) : k((A)a.k), low((A)a.k_low) {}
+    __device__ __forceinline__ A times(A d) const {
+        if constexpr (FINE && sizeof(A) == 4) return __builtin_fmaf(d, k, fmaxf(d, -1e30f) * low);  // -inf stays -inf
+        return d * k;
+    }
+    __device__ __forceinline__ A power(A d) const { return pow2(times(d)); }
+};
+template <typename T> using BaseOf = Base<typename Acc<T>::type, sizeof(T) >= 4>;
 template <typename A> struct alignas(16) Partial { double loss, rows; };
 
 template <typename A> __device__ __forceinline__ A teacher_at(const Args& a, int64_t i) {
@@ -71,17 +85,17 @@ __device__ __forceinline__ int column(const Args& a, int64_t i) {
 // A maximum and the sum of 2^((x - m) k) above it, of parts of a row.
 template <typename A> struct Soft {
     A m, s;
-    __device__ __forceinline__ void add(A x, A k) {
+    template <typename B> __device__ __forceinline__ void add(A x, const B& k) {
         if (x > m) {
-            s *= pow2((m - x) * k);  // 0 from nothing: s is 0 then
+            s *= k.power(m - x);  // 0 from nothing: s is 0 then
             m = x;
         }
-        s += m == lowest<A>() ? (x == m ? (A)0 : x) : pow2((x - m) * k);  // nothing but -inf so far: 0, or a NaN
+        s += m == lowest<A>() ? (x == m ? (A)0 : x) : k.power(x - m);  // nothing but -inf so far: 0, or a NaN
     }
-    __device__ __forceinline__ void merge(A om, A os, A k) {
+    template <typename B> __device__ __forceinline__ void merge(A om, A os, const B& k) {
         const A top = larger(m, om);
         const A base = top == lowest<A>() ? (A)0 : top;
-        s = s * pow2((m - base) * k) + os * pow2((om - base) * k);
+        s = s * k.power(m - base) + os * k.power(om - base);
         m = top;
     }
 };
@@ -95,7 +109,7 @@ template <typename T> __device__ __forceinline__ int before_vectors(const T* p) 
 
 // Columns [from, to) of a row by TEAM threads, several vectors at a time: one step of the running maximum for all of them.
 template <typename T, int TEAM, typename A>
-__device__ __forceinline__ Soft<A> soft_row(const T* x, int from, int to, int t, A k) {
+__device__ __forceinline__ Soft<A> soft_row(const T* x, int from, int to, int t, const BaseOf<T>& k) {
     constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
     using V = Loose<T, VEC>;
     Soft<A> v = {lowest<A>(), 0};
@@ -109,8 +123,8 @@ __device__ __forceinline__ Soft<A> soft_row(const T* x, int from, int to, int t,
         const A base = top == lowest<A>() ? (A)0 : top;
         A sum = 0;
 #pragma unroll
-        for (int i = 0; i < n; ++i) sum += pow2((e[i] - base) * k);
-        v.s = v.s * pow2((v.m - base) * k) + sum;
+        for (int i = 0; i < n; ++i) sum += k.power(e[i] - base);
+        v.s = v.s * k.power(v.m - base) + sum;
         v.m = top;
     };
     for (; j + (AT_ONCE - 1) * TEAM * VEC + VEC <= to; j += AT_ONCE * TEAM * VEC) {
@@ -134,7 +148,7 @@ __device__ __forceinline__ Soft<A> soft_row(const T* x, int from, int to, int t,
 }
 
 // Over the TEAM threads of a row: aligned lanes of a wave, or the whole workgroup.
-template <int TEAM, typename A> __device__ __forceinline__ void soft_all(Soft<A>& v, A k, A* lds) {
+template <int TEAM, typename A, typename B> __device__ __forceinline__ void soft_all(Soft<A>& v, const B& k, A* lds) {
     constexpr int W = TEAM < 64 ? TEAM : 64;
 #pragma unroll
     for (int d = W / 2; d >= 1; d >>= 1) {
@@ -171,23 +185,24 @@ template <int TEAM, typename A> __device__ __forceinline__ A sum_all(A v, A* lds
 // weight.
 template <typename T, int TEAM, typename A>
 __device__ __forceinline__ A teach(const Args& a, int64_t n, Stats<A>& st, int t, bool on, A* lds) {
-    const A k = (A)a.k;
+    const Base<A, true> k(a);
     Soft<A> v = {lowest<A>(), 0};
     if (on)
         for (int i = t; i < a.K; i += TEAM)
             if (column(a, n * a.K + i) >= 0) v.add(teacher_at<A>(a, n * a.K + i), k);
     soft_all<TEAM, A>(v, k, lds);
     st.tm = v.m;
-    st.ts2 = lg2(v.s);
+    st.ts = v.s;
     A sum = 0;
-    if (on && !(v.m == lowest<A>() && v.s == (A)0)) {
+    if (on && v.s != (A)0) {
+        const A ts2 = lg2(v.s), s2 = lg2(st.s);
         const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
         for (int i = t; i < a.K; i += TEAM) {
             const int c = column(a, n * a.K + i);
             if (c < 0) continue;
-            const A lp = (teacher_at<A>(a, n * a.K + i) - v.m) * k - st.ts2, p = pow2(lp);
+            const A e = k.times(teacher_at<A>(a, n * a.K + i) - v.m), p = pow2(e) / v.s;
             if (p == (A)0) continue;
-            sum += p * (lp - (((A)x[c] - st.m) * k - st.s2));
+            sum += p * ((e - ts2) - (k.times((A)x[c] - st.m) - s2));
         }
     }
     return sum_all<TEAM, A>(sum, lds);
@@ -199,8 +214,8 @@ template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
     __shared__ A lds[16];
     const int64_t n = blockIdx.x / a.splits;
     const int part = (int)(blockIdx.x % a.splits), from = part * a.width, to = from + a.width < a.V ? from + a.width : a.V;
-    Soft<A> v = soft_row<T, 256, A>(reinterpret_cast<const T*>(a.x) + n * a.row, from, to, threadIdx.x, (A)a.k);
-    soft_all<256, A>(v, (A)a.k, lds);
+    Soft<A> v = soft_row<T, 256, A>(reinterpret_cast<const T*>(a.x) + n * a.row, from, to, threadIdx.x, BaseOf<T>(a));
+    soft_all<256, A>(v, BaseOf<T>(a), lds);
     if (threadIdx.x == 0) reinterpret_cast<Soft<A>*>(a.soft)[blockIdx.x] = v;
 }
 
@@ -212,7 +227,7 @@ template <typename T, int TEAM, bool JOIN> __global__ __launch_bounds__(256) voi
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + team;
     const bool on = n < a.N;
-    const A k = (A)a.k;
+    const BaseOf<T> k(a);
     Soft<A> v = {lowest<A>(), 0};
     if (on) {
         const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
@@ -228,10 +243,10 @@ template <typename T, int TEAM, bool JOIN> __global__ __launch_bounds__(256) voi
         }
     }
     soft_all<TEAM, A>(v, k, lds);
-    Stats<A> st = {v.m, lg2(v.s), 0, 0};
+    Stats<A> st = {v.m, v.s, 0, 0};
     const A sum = teach<T, TEAM, A>(a, n, st, t, on, lds);
     if (t == 0) {
-        const bool counted = on && !(st.tm == lowest<A>() && st.ts2 == lowest<A>());
+        const bool counted = on && st.ts != (A)0;
         const A loss = counted ? (A)a.weight * sum : (A)0;
         if (on) {
             reinterpret_cast<Stats<A>*>(a.stats)[n] = st;
@@ -284,16 +299,16 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_sh
     const int t = threadIdx.x % TEAM;
     const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
     if (n >= a.N || t >= a.V) return;
-    const A k = (A)a.k;
+    const BaseOf<T> k(a);
     const Stats<A> st = reinterpret_cast<const Stats<A>*>(a.stats)[n];
     A d = 0;
-    if (!(st.tm == lowest<A>() && st.ts2 == lowest<A>())) {
+    if (st.ts != (A)0) {
         A p = 0;
         for (int i = 0; i < a.K; ++i)
-            if (column(a, n * a.K + i) == t) p += pow2((teacher_at<A>(a, n * a.K + i) - st.tm) * k - st.ts2);
+            if (column(a, n * a.K + i) == t) p += k.power(teacher_at<A>(a, n * a.K + i) - st.tm);
         A c = reinterpret_cast<const A*>(a.grad)[n * a.grad_step] * (A)a.weight;
         if (a.scale) c *= *reinterpret_cast<const A*>(a.scale);
-        d = c * (pow2(((A)reinterpret_cast<const T*>(a.x)[n * a.row + t] - st.m) * k - st.s2) - p);
+        d = c * (k.power((A)reinterpret_cast<const T*>(a.x)[n * a.row + t] - st.m) / st.s - p / st.ts);
     }
     reinterpret_cast<T*>(a.dx)[n * a.V + t] = (T)d;
 }
@@ -312,26 +327,27 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
     const int64_t n = (int64_t)(blockIdx.x / a.splits) * (256 / TEAM) + team;
     const int from = (int)(blockIdx.x % a.splits) * a.width, to = from + a.width < a.V ? from + a.width : a.V;
     const bool on = n < a.N;
-    const A k = (A)a.k;
+    const BaseOf<T> k(a);
     Stats<A> st = {};
-    A c = 0;
+    A c = 0, share = 0;
     bool counted = false;
     const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
     T* dx = reinterpret_cast<T*>(a.dx) + n * a.V;
-    const auto q = [&](T v) { return pow2(((A)v - st.m) * k - st.s2); };
+    const auto q = [&](T v) { return k.power((A)v - st.m) * share; };  // c times the softmax
     if (on) {
         st = reinterpret_cast<const Stats<A>*>(a.stats)[n];
-        counted = !(st.tm == lowest<A>() && st.ts2 == lowest<A>());
+        counted = st.ts != (A)0;
         c = reinterpret_cast<const A*>(a.grad)[n * a.grad_step] * (A)a.weight;
         if (a.scale) c *= *reinterpret_cast<const A*>(a.scale);
+        share = c / st.s;
         for (int i = t; i < a.K; i += TEAM) {
             const int j = column(a, n * a.K + i);
             const bool mine = j >= from && j < to;
             col[i] = mine ? j : -1;
-            prob[i] = mine ? pow2((teacher_at<A>(a, n * a.K + i) - st.tm) * k - st.ts2) : (A)0;
+            prob[i] = mine ? k.power(teacher_at<A>(a, n * a.K + i) - st.tm) / st.ts : (A)0;
         }
         const int head = before_vectors(dx + from);
-        if (t < head && from + t < to) dx[from + t] = counted ? (T)(c * q(x[from + t])) : (T)0.f;
+        if (t < head && from + t < to) dx[from + t] = counted ? (T)q(x[from + t]) : (T)0.f;
         int j = from + head + t * VEC;
         if (counted) {
             for (; j + (AT_ONCE - 1) * TEAM * VEC + VEC <= to; j += AT_ONCE * TEAM * VEC) {
@@ -342,7 +358,7 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
                 for (int i = 0; i < AT_ONCE; ++i) {
                     V o;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) o.e[e] = (T)(c * q(p[i].e[e]));
+                    for (int e = 0; e < VEC; ++e) o.e[e] = (T)q(p[i].e[e]);
                     *reinterpret_cast<V*>(dx + j + i * TEAM * VEC) = o;
                 }
             }
@@ -350,10 +366,10 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
                 const V p = *reinterpret_cast<const V*>(x + j);
                 V o;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o.e[e] = (T)(c * q(p.e[e]));
+                for (int e = 0; e < VEC; ++e) o.e[e] = (T)q(p.e[e]);
                 *reinterpret_cast<V*>(dx + j) = o;
             }
-            for (; j < to; ++j) dx[j] = (T)(c * q(x[j]));
+            for (; j < to; ++j) dx[j] = (T)q(x[j]);
         } else {
             const V zero = {};
             for (; j + VEC <= to; j += TEAM * VEC) *reinterpret_cast<V*>(dx + j) = zero;
@@ -372,7 +388,7 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
                 first = first && o >= i;
                 p += prob[o];
             }
-        if (first) dx[j] = (T)(c * (q(x[j]) - p));
+        if (first) dx[j] = (T)(q(x[j]) - c * p);
     }
 }
 
@@ -395,6 +411,8 @@ static int splits_of(int64_t N, int64_t V) {
 static int width_of(int64_t V, int splits) { return (int)(((V + splits - 1) / splits + 7) / 8 * 8); }
 
 static int64_t groups(int64_t N, int team) { return (N + 256 / team - 1) / (256 / team); }
+
+static float low_of(double k) { return (float)(k - (double)(float)k); }
 
 static int check(int dtype, int tdtype, int64_t N, int64_t V, int K, int64_t row, double T) {
     for (const int d : {dtype, tdtype})
@@ -449,7 +467,7 @@ int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, in
     if (N > 0 && !scratch && (one || splits_of(N, V) > 1)) return EBR_ERR_SCRATCH;
     if (!aligned(stats, 16) || !aligned(scratch, 16)) return EBR_ERR_ALIGN;
     Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature,
-              temperature * temperature * LN2, reduction, stats, loss, scale, scratch};
+              low_of(LOG2E / temperature), temperature * temperature * LN2, reduction, stats, loss, scale, scratch};
     hipStream_t s = (hipStream_t)stream;
     return by_type(dtype, [&](auto v) {
         using T = decltype(v);
@@ -483,8 +501,8 @@ int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V
     if (N == 0) return EBR_OK;
     if (!logits || !teacher || !ids || !stats || !grad || !dx) return EBR_ERR_NULL;
     if (!aligned(stats, 16)) return EBR_ERR_ALIGN;
-    Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature, temperature,
-              EBR_REDUCE_NONE, const_cast<void*>(stats), nullptr, const_cast<void*>(scale), nullptr, grad, grad_stride, dx};
+    Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature,
+              low_of(LOG2E / temperature), temperature, EBR_REDUCE_NONE, const_cast<void*>(stats), nullptr, const_cast<void*>(scale), nullptr, grad, grad_stride, dx};
     return by_type(dtype, [&](auto v) {
         using T = decltype(v);
         using A = typename Acc<T>::type;
