@@ -46,6 +46,7 @@ struct Args {
     int64_t grad_step;
     void* dx;
     int splits, width;  // parts of a row where there are few, and their columns
+    int seen;           // words of k_grad's bits for a row's columns, a power of two
     void* soft;         // [N][splits]: a part's maximum and sum
 };
 
@@ -220,7 +221,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
 }
 
 // Rows' losses, from the logits, or with JOIN from the rows' parts.
-template <typename T, int TEAM, bool JOIN> __global__ __launch_bounds__(256) void k_loss(Args a) {
+template <typename T, int TEAM, bool SHORT, bool JOIN> __global__ __launch_bounds__(256) void k_loss(Args a) {
     using A = typename Acc<T>::type;
     __shared__ A lds[16];
     __shared__ double rows[256 / TEAM][2];
@@ -236,7 +237,7 @@ template <typename T, int TEAM, bool JOIN> __global__ __launch_bounds__(256) voi
                 const Soft<A> p = reinterpret_cast<const Soft<A>*>(a.soft)[n * a.splits + i];
                 v.merge(p.m, p.s, k);
             }
-        } else if constexpr (TEAM < 64) {
+        } else if constexpr (SHORT) {
             if (t < a.V) v.add((A)x[t], k);  // a column a thread
         } else {
             v = soft_row<T, TEAM, A>(x, 0, a.V, t, k);
@@ -320,10 +321,12 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
     using A = typename Acc<T>::type;
     constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
     using V = Loose<T, VEC>;
+    constexpr int TEAMS = 256 / TEAM;
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    A* prob = reinterpret_cast<A*>(shared) + (int64_t)team * a.K;
-    int* col = reinterpret_cast<int*>(reinterpret_cast<A*>(shared) + (int64_t)(256 / TEAM) * a.K) + (int64_t)team * a.K;
+    A* prob = reinterpret_cast<A*>(shared) + team * a.K;
+    int* col = reinterpret_cast<int*>(reinterpret_cast<A*>(shared) + TEAMS * a.K) + team * a.K;
+    uint32_t* seen = reinterpret_cast<uint32_t*>(shared + TEAMS * a.K * (int)(sizeof(A) + sizeof(int))) + team * (a.seen + 1);
     const int64_t n = (int64_t)(blockIdx.x / a.splits) * (256 / TEAM) + team;
     const int from = (int)(blockIdx.x % a.splits) * a.width, to = from + a.width < a.V ? from + a.width : a.V;
     const bool on = n < a.N;
@@ -334,6 +337,9 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
     const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
     T* dx = reinterpret_cast<T*>(a.dx) + n * a.V;
     const auto q = [&](T v) { return k.power((A)v - st.m) * share; };  // c times the softmax
+    // a bit for each column (or several, of a wide part) tells whether two entries may name the same: seen[a.seen] is set
+    for (int i = t; i <= a.seen; i += TEAM) seen[i] = 0;
+    __syncthreads();
     if (on) {
         st = reinterpret_cast<const Stats<A>*>(a.stats)[n];
         counted = st.ts != (A)0;
@@ -345,6 +351,9 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
             const bool mine = j >= from && j < to;
             col[i] = mine ? j : -1;
             prob[i] = mine ? k.power(teacher_at<A>(a, n * a.K + i) - st.tm) / st.ts : (A)0;
+            if (!mine) continue;
+            const uint32_t at = (uint32_t)(j - from) & (uint32_t)(a.seen * 32 - 1), bit = 1u << (at & 31);
+            if (atomicOr(&seen[at >> 5], bit) & bit) seen[a.seen] = 1;
         }
         const int head = before_vectors(dx + from);
         if (t < head && from + t < to) dx[from + t] = counted ? (T)q(x[from + t]) : (T)0.f;
@@ -381,29 +390,51 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
     for (int i = t; i < a.K; i += TEAM) {
         const int j = col[i];
         if (j < 0) continue;
-        A p = 0;
+        A p = prob[i];
         bool first = true;
-        for (int o = 0; o < a.K; ++o)
-            if (col[o] == j) {
-                first = first && o >= i;
-                p += prob[o];
-            }
+        if (seen[a.seen]) {
+            p = 0;
+            for (int o = 0; o < a.K; ++o)
+                if (col[o] == j) {
+                    first = first && o >= i;
+                    p += prob[o];
+                }
+        }
         if (first) dx[j] = (T)(q(x[j]) - c * p);
     }
 }
 
-// Threads of a row: as many lanes as it has columns, up to a wave, and a workgroup for long rows.
-static int team_of(int64_t V) {
+constexpr int SHORT_ROW = 32;  // columns of a row in which each has a thread
+
+// k_grad's bits for the columns of a part: exact up to 2^17.
+static int seen_of(int64_t width) {
+    int w = 1;
+    while (w < 4096 && (int64_t)w * 32 < width) w *= 2;
+    return w;
+}
+static int64_t shared_of(int team, int K, int64_t width, int es) {
+    return (int64_t)(256 / team) * (K * (int64_t)(es + 4) + 4 * (seen_of(width) + 1));
+}
+
+// Threads of a row: one a column for the shortest; then as many lanes as it has vectors, up to a wave, but not so few that
+// the rows of a workgroup take more than 32 KiB of shared memory in the gradient; a workgroup for long rows.
+static int team_of(int dtype, int64_t V, int K) {
     if (V > 2048) return 256;
     int t = 8;
-    while (t < 64 && t < V) t *= 2;
-    return t;
+    if (V <= SHORT_ROW) {
+        while (t < V) t *= 2;
+        return t;
+    }
+    const int es = dtype == EBR_DTYPE_F64 ? 8 : dtype == EBR_DTYPE_F32 ? 4 : 2, acc = es == 8 ? 8 : 4;
+    while (t < 64 && (int64_t)t * (16 / es) < V) t *= 2;
+    while (t < 64 && shared_of(t, K, V, acc) > 32768) t *= 2;
+    return t < 64 || shared_of(t, K, V, acc) <= 32768 ? t : 256;
 }
 
 // Parts of a row: where rows of a workgroup each leave compute units without any, as many as give each of the 256 about
 // four, with at least 4,096 columns (a round of loads) and at most 64 parts.
 static int splits_of(int64_t N, int64_t V) {
-    if (team_of(V) < 256 || N >= 512) return 1;
+    if (V <= 2048 || N >= 512) return 1;
     int64_t s = 1024 / (N > 0 ? N : 1);
     if (s > V / 4096) s = V / 4096;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -418,7 +449,7 @@ static int check(int dtype, int tdtype, int64_t N, int64_t V, int K, int64_t row
     for (const int d : {dtype, tdtype})
         if (d != EBR_DTYPE_F32 && d != EBR_DTYPE_BF16 && d != EBR_DTYPE_F16 && d != EBR_DTYPE_F64) return EBR_ERR_DTYPE;
     if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V >= ((int64_t)1 << 30) || K < 1 || K > K_MAX || row < V ||
-        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T > 0) || T > 1e30 || T < 1e-30 || groups(N, team_of(V)) > MAX_BLOCKS)
+        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T > 0) || T > 1e30 || T < 1e-30 || groups(N, team_of(dtype, V, K)) > MAX_BLOCKS)
         return EBR_ERR_SHAPE;
     return EBR_OK;
 }
@@ -432,13 +463,19 @@ template <typename F> static int by_type(int dtype, F f) {
     }
 }
 
-template <typename F> static void by_team(int team, F f) {
+template <typename F> static void by_team(int team, int64_t V, F f) {
+    const auto with = [&](auto t) {
+        constexpr int TEAM = decltype(t)::value;
+        if constexpr (TEAM <= SHORT_ROW)
+            if (V <= SHORT_ROW) return f(t, std::true_type());
+        f(t, std::false_type());
+    };
     switch (team) {
-        case 8: f(std::integral_constant<int, 8>()); break;
-        case 16: f(std::integral_constant<int, 16>()); break;
-        case 32: f(std::integral_constant<int, 32>()); break;
-        case 64: f(std::integral_constant<int, 64>()); break;
-        default: f(std::integral_constant<int, 256>()); break;
+        case 8: with(std::integral_constant<int, 8>()); break;
+        case 16: with(std::integral_constant<int, 16>()); break;
+        case 32: with(std::integral_constant<int, 32>()); break;
+        case 64: with(std::integral_constant<int, 64>()); break;
+        default: with(std::integral_constant<int, 256>()); break;
     }
 }
 
@@ -452,7 +489,7 @@ int64_t ebr_block_distill_scratch(int dtype, int64_t N, int64_t V, int K) {
     if (check(dtype, dtype, N, V, K, V, 1.0)) return -1;
     const int splits = splits_of(N, V);
     const int64_t soft = splits > 1 ? N * splits * 2 * (dtype == EBR_DTYPE_F64 ? 8 : 4) : 0;
-    return (soft + 15) / 16 * 16 + groups(N, splits > 1 ? 64 : team_of(V)) * (int64_t)sizeof(Partial<float>);
+    return (soft + 15) / 16 * 16 + groups(N, splits > 1 ? 64 : team_of(dtype, V, K)) * (int64_t)sizeof(Partial<float>);
 }
 
 int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, int K, int64_t row_stride, double temperature,
@@ -472,7 +509,7 @@ int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, in
     return by_type(dtype, [&](auto v) {
         using T = decltype(v);
         using A = typename Acc<T>::type;
-        const int splits = splits_of(N, V), team = splits > 1 ? 64 : team_of(V);
+        const int splits = splits_of(N, V), team = splits > 1 ? 64 : team_of(dtype, V, K);
         a.splits = splits;
         a.width = width_of(V, splits);
         if (splits > 1) {
@@ -480,11 +517,11 @@ int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, in
             const int64_t soft = N * splits * (int64_t)sizeof(Soft<A>);
             a.part = reinterpret_cast<char*>(scratch) + (soft + 15) / 16 * 16;
             hipLaunchKernelGGL((k_part<T>), dim3((unsigned)(N * splits)), dim3(256), 0, s, a);
-            hipLaunchKernelGGL((k_loss<T, 64, true>), dim3((unsigned)groups(N, 64)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_loss<T, 64, false, true>), dim3((unsigned)groups(N, 64)), dim3(256), 0, s, a);
         } else if (N > 0) {
-            by_team(team, [&](auto w) {
-                hipLaunchKernelGGL((k_loss<T, decltype(w)::value, false>), dim3((unsigned)groups(N, team)), dim3(256), 0, s,
-                                   a);
+            by_team(team, V, [&](auto w, auto is_short) {
+                hipLaunchKernelGGL((k_loss<T, decltype(w)::value, decltype(is_short)::value, false>),
+                                   dim3((unsigned)groups(N, team)), dim3(256), 0, s, a);
             });
         }
         if (one) hipLaunchKernelGGL((k_total<A>), dim3(1), dim3(1024), 0, s, a, groups(N, team));
@@ -506,18 +543,18 @@ int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V
     return by_type(dtype, [&](auto v) {
         using T = decltype(v);
         using A = typename Acc<T>::type;
-        const int team = team_of(V);
+        const int team = team_of(dtype, V, K);
         a.splits = splits_of(N, V);
         a.width = width_of(V, a.splits);
-        const size_t lds = (size_t)(256 / team) * K * (sizeof(A) + sizeof(int));
-        by_team(team, [&](auto w) {
+        a.seen = seen_of(a.width);
+        const size_t lds = (size_t)shared_of(team, K, a.width, sizeof(A));
+        by_team(team, V, [&](auto w, auto is_short) {
             constexpr int TEAM = decltype(w)::value;
-            if constexpr (TEAM < 64)
-                hipLaunchKernelGGL((k_grad_short<T, TEAM>), dim3((unsigned)groups(N, team)), dim3(256), 0,
-                                   (hipStream_t)stream, a);
+            const dim3 grid((unsigned)(groups(N, team) * a.splits));
+            if constexpr (decltype(is_short)::value)
+                hipLaunchKernelGGL((k_grad_short<T, TEAM>), grid, dim3(256), 0, (hipStream_t)stream, a);
             else
-                hipLaunchKernelGGL((k_grad<T, TEAM>), dim3((unsigned)(groups(N, team) * a.splits)), dim3(256), lds,
-                                   (hipStream_t)stream, a);
+                hipLaunchKernelGGL((k_grad<T, TEAM>), grid, dim3(256), lds, (hipStream_t)stream, a);
         });
         return launched();
     });

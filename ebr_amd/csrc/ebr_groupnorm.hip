@@ -538,8 +538,12 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
     constexpr int NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5, NG = MODE == 2 ? 5 : NS;
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, tc = a.tx * VEC;
-    A* waves = reinterpret_cast<A*>(shared);  // [W][NG][tx], and [W][2][tc]
-    A* cols = waves + W * 2 * tc;             // [NG][tx]
+    // what lanes of the same channels have not added up between them: rows of a wave's each, or of the threads of a cell
+    // where these are several waves
+    const int rows = a.tx < 64 ? W : 64 * W / a.tx, row = a.tx < 64 ? wave : t / a.tx;
+    const bool first = a.tx >= 64 || lane < a.tx;
+    A* waves = reinterpret_cast<A*>(shared);  // [rows][NG][tx], and [rows][2][tc]
+    A* cols = waves + rows * 2 * tc;          // [NG][tx]
     const int tile = (int)(blockIdx.x % a.tiles);
     const int64_t n = blockIdx.x / a.tiles;
     const int c0 = tile * a.tile, have = a.C - c0 < a.tile ? a.C - c0 : a.tile;
@@ -584,14 +588,13 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
         for (int d = a.tx; d < 64; d <<= 1)
 #pragma unroll
             for (int k = 0; k < K; ++k) p[k] += __shfl_xor(p[k], d, 64);
-        if (lane < a.tx)
+        if (first)
 #pragma unroll
-            for (int k = 0; k < K; ++k) waves[(wave * K + k) * a.tx + lane] = p[k];
+            for (int k = 0; k < K; ++k) waves[(row * K + k) * a.tx + t % a.tx] = p[k];
         __syncthreads();
         for (int i = t; i < K * a.tx; i += 64 * W) {
             A v = waves[i];
-#pragma unroll
-            for (int q = 1; q < W; ++q) v += waves[q * K * a.tx + i];
+            for (int q = 1; q < rows; ++q) v += waves[q * K * a.tx + i];
             cols[i] = v;
         }
         __syncthreads();
@@ -610,17 +613,16 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
                 pw[e] += __shfl_xor(pw[e], d, 64);
                 pb[e] += __shfl_xor(pb[e], d, 64);
             }
-        if (lane < a.tx) {
-            store_wide<A, VEC>(waves + wave * 2 * tc + lane * VEC, pw);
-            store_wide<A, VEC>(waves + (wave * 2 + 1) * tc + lane * VEC, pb);
+        if (first) {
+            store_wide<A, VEC>(waves + row * 2 * tc + at, pw);
+            store_wide<A, VEC>(waves + (row * 2 + 1) * tc + at, pb);
         }
         __syncthreads();
         A* share = reinterpret_cast<A*>(a.chan) + n * 2 * a.C + c0;
         for (int i = t; i < 2 * tc; i += 64 * W) {
             if (i % tc >= have) continue;
             A v = waves[i];
-#pragma unroll
-            for (int q = 1; q < W; ++q) v += waves[q * 2 * tc + i];
+            for (int q = 1; q < rows; ++q) v += waves[q * 2 * tc + i];
             share[i < tc ? i : a.C + i - tc] = v;
         }
     };
@@ -826,10 +828,12 @@ struct Scratch {
     int64_t all() const { return part + means + chan; }
 };
 
-// Whether a workgroup holds a sample's tile of groups, and how: W waves of R cells a thread, tx threads across the tile's
-// channels. A thread's vector has to lie in one group, and a tile of whole groups to fill three quarters of the threads
-// across; 8 threads are 128 bytes of a cell. The second derivative, with 80 sums and three tensors in registers, has 4 waves.
-// Above their cells (256 of the second derivative, 1,024 of the others at 8 threads across) k_sums and k_apply read twice.
+// Whether a workgroup holds a sample's tile of groups, and how: W waves of some cells a thread, tx threads across the tile's
+// channels. A thread's vector (16 bytes; 4 channels of the second derivative, whose sums and three tensors fill the
+// registers) has to lie in one group, and a tile of whole groups to fill three quarters of the threads across, which take
+// 128 bytes of a cell or more: more where a sample has fewer cells than the rest of the workgroup holds. Larger groups
+// (above 256 cells at 128 bytes for the second derivative, 1,024 for the others) go through k_sums and k_apply, which read
+// everything twice.
 struct Whole {
     int waves = 0, cells = 0, tx = 0, tile = 0, tiles = 0;
     // the two numbers of cells that there are kernels for
@@ -839,15 +843,16 @@ struct Whole {
         const int vec = mode == 2 ? 4 : vector_of(dtype, C), cg = C / groups;
         if (!vector || dtype == EBR_DTYPE_F64 || vec == 1 || cg % vec || L > 4096) return;
         const bool wide = dtype == EBR_DTYPE_F32;
-        for (int x = !wide && vec == 4 ? 16 : 8; x <= 64; x *= 2) {
+        for (int x = !wide && vec == 4 ? 16 : 8; x <= 256; x *= 2) {
             const int t = x * vec / cg * cg;
-            if (t * 4 < x * vec * 3 && t < C) continue;
-            if (t == 0) continue;
+            if (t == 0 || (t * 4 < x * vec * 3 && t < C)) continue;
+            const bool more = x < 256 && t < C && L * 2 * x <= 256;  // half of the cells of a workgroup would be none
+            if (more) continue;
             for (const int w : {4, 16}) {
-                if (w == 16 && (mode == 2 || x > 32)) continue;  // (shared memory)
+                if (w == 16 && (mode == 2 || x > 32)) continue;  // (registers; shared memory)
                 const int64_t step = 64 * w / x;
                 const int r = (int)((L + step - 1) / step);
-                if (r > many(mode, wide) || (w == 4 && r > 4 && mode != 2)) continue;
+                if (r > many(mode, wide) || (w == 4 && r > 4 && mode != 2 && x <= 32)) continue;
                 waves = w;
                 cells = r <= few(mode, wide) ? few(mode, wide) : many(mode, wide);
                 tx = x;
@@ -863,7 +868,8 @@ template <typename T, int MODE, int ACT> static void launch_whole(hipStream_t s,
     using A = typename Acc<T>::type;
     constexpr bool WIDE = sizeof(T) == 4;
     constexpr int VEC = MODE == 2 ? 4 : 16 / (int)sizeof(T), FEW = Whole::few(MODE, WIDE), MANY = Whole::many(MODE, WIDE);
-    const size_t lds = ((size_t)h.waves * 2 * h.tx * VEC + 5 * h.tx) * sizeof(A);
+    const int rows = h.tx < 64 ? h.waves : 64 * h.waves / h.tx;
+    const size_t lds = ((size_t)rows * 2 * h.tx * VEC + 5 * h.tx) * sizeof(A);
     const dim3 grid((unsigned)(a.B * h.tiles)), block(64 * h.waves);
     if (h.waves == 4 && h.cells == FEW) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, FEW, 4>), grid, block, lds, s, a);
     else if (h.waves == 4) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, MANY, 4>), grid, block, lds, s, a);

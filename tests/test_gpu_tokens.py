@@ -220,6 +220,20 @@ def test_distill(cuda, dtype, lead, V, K):
     _check_distill(x, t, ids, T=1.0 if K % 2 else 2.5)
 
 
+# every number of threads a row, rows that end inside a workgroup, and many entries for short rows
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("N,V,K", [(70, 32, 5), (70, 33, 33), (50, 97, 8), (37, 130, 100), (19, 300, 256), (9, 500, 500), (6, 1024, 1024),
+                                   (3, 2000, 1024), (700, 2100, 3), (2, 140000, 1024), (2, 300000, 700)])  # fmt: skip
+def test_distill_teams(cuda, dtype, N, V, K):
+    _say(f"distill teams {N} {V} {K} {dtype}")
+    g = torch.Generator(cuda).manual_seed(N)
+    x = (torch.randn(N, V, generator=g, device=cuda) * 2).to(dtype)
+    t, ids = _teacher(cuda, (N,), V, K, seed=K)
+    _check_distill(x, t, ids, T=1.5)
+    ids[::2] = torch.randint(0, V, ids[::2].shape, generator=g, device=cuda)  # with tokens named twice
+    _check_distill(x, t, ids, T=1.5)
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("V,K", [(11, 5), (700, 20), (5000, 70)])
 def test_distill_ragged_rows(cuda, reduction, V, K):
