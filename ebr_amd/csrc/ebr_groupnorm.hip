@@ -25,7 +25,7 @@ using namespace ebr_row;
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int SUMS[3] = {2, 2, 10};   // of a mode; mode 0: the mean and the squares about it
-constexpr int MEANS[3] = {2, 2, 6};   // kept of a group: mode 0: mu, r; 1: mean k, mean(k h); 2: see Group2
+constexpr int MEANS[3] = {2, 2, 6};   // kept of a group: mode 0: mu, r; 1: mean k, mean(k h); 2: u, u h, k h, v, v h, and Group2's along
 
 struct Args {
     const void *x, *dy, *u;
@@ -48,9 +48,6 @@ __device__ __forceinline__ float pow_e(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ double pow_e(double x) { return exp(x); }
 __device__ __forceinline__ float inverse(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
-
-__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
-__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 // The activation's value, or its first two derivatives. ACT 0: none, 1: silu.
 template <int ACT, typename A> __device__ __forceinline__ A act(A a) {
@@ -94,59 +91,80 @@ template <typename A, int VEC> __device__ __forceinline__ void params(const void
         for (int e = 0; e < VEC; ++e) v[e] = none;
 }
 
-// What a thread knows of its channels; h = x r + shift, shift = -mu r, rounded once (and shift no further than mu itself).
+// What a thread knows of its channels. Elements enter as d = x - mu, not through x r - mu r in one step: of a group of
+// (nearly) one value the difference is exact, where mu r would be rounded at the size of mu / sqrt(eps). The factor r of
+// h = d r goes into the weights and, after the last cell, into the sums.
 template <typename A, int VEC> struct Channels {
-    A shift[VEC], r[VEC], w[VEC], b[VEC];
+    A mu[VEC], r[VEC], w[VEC], b[VEC];
     __device__ __forceinline__ void load(const Args& a, int64_t n, int c) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const A* s = reinterpret_cast<const A*>(a.stats) + (n * a.G + (c + e) / a.cg) * 2;
+            mu[e] = s[0];
             r[e] = s[1];
-            shift[e] = -s[0] * s[1];
         }
         params<A, VEC>(a.w, c, (A)1, w);
         params<A, VEC>(a.b, c, (A)0, b);
     }
 };
 
-// An element's part of the sums of modes 1 and 2.
+// An element's part of the sums of modes 1 and 2, with d in h's place; wr = w r.
 template <int ACT, int MODE, typename A, int NS, int VEC>
-__device__ __forceinline__ void add_sums(A (&s)[NS][VEC], int e, A x, A dy, A u, A r, A shift, A w, A b) {
-    const A h = fused(x, r, shift);
+__device__ __forceinline__ void add_sums(A (&s)[NS][VEC], int e, A x, A dy, A u, A mu, A wr, A b) {
+    const A d = x - mu;
     A f1, f2;
-    slopes<ACT, A>(w * h + b, f1, f2);
+    slopes<ACT, A>(wr * d + b, f1, f2);
     const A da = dy * f1;
     if constexpr (MODE == 1) {
         s[0][e] += da;
-        s[1][e] += da * h;
+        s[1][e] += da * d;
     } else {
         s[0][e] += u;
-        s[1][e] += u * h;
+        s[1][e] += u * d;
         s[2][e] += da;
-        s[3][e] += da * h;
+        s[3][e] += da * d;
         s[4][e] += da * u;
         if constexpr (ACT != 0) {
-            const A t = dy * f2, th = t * h, tu = t * u;
+            const A t = dy * f2, td = t * d, tu = t * u;
             s[5][e] += t;
-            s[6][e] += th;
-            s[7][e] += th * h;
+            s[6][e] += td;
+            s[7][e] += td * d;
             s[8][e] += tu;
-            s[9][e] += tu * h;
+            s[9][e] += tu * d;
         }
     }
 }
 
-// An element's gx and gdy, from its group's means.
+// Their factors of r.
+template <int MODE, typename A, int NS, int VEC> __device__ __forceinline__ void scale_sums(A (&s)[NS][VEC], int e, A r) {
+    s[1][e] *= r;
+    if constexpr (MODE == 2) {
+        s[3][e] *= r;
+        if constexpr (NS > 5) {
+            s[6][e] *= r;
+            s[7][e] *= r * r;
+            s[9][e] *= r;
+        }
+    }
+}
+
+// A group's constants of gx = r (v - v1 - h (v2 + r along)) and gdy, the factor r in all that it takes: of the weights
+// wr = w r and uwr = uw r alone are left.
+template <typename A> struct Group2 {
+    A u1, ru2, rrk2, rv1, e2;
+    __device__ __forceinline__ Group2() {}
+    // from the means of u, u h, and r times those of k h, v, v h and along
+    __device__ __forceinline__ Group2(A r, A u1_, A u2, A rk2, A rv1_, A rv2, A ralong)
+        : u1(u1_), ru2(r * u2), rrk2(r * rk2), rv1(rv1_), e2(r * (rv2 + r * ralong)) {}
+};
 template <int ACT, typename A>
-__device__ __forceinline__ void second_out(A x, A dy, A u, A r, A shift, A w, A b, A uw, A ub, A u1, A u2, A k2, A v1, A v2,
-                                           A along, A& gx, A& gdy) {
-    const A h = fused(x, r, shift);
+__device__ __forceinline__ void second_out(const Group2<A>& g, A x, A dy, A u, A mu, A wr, A b, A uwr, A ub, A& gx, A& gdy) {
+    const A d = x - mu;
     A f1, f2;
-    slopes<ACT, A>(w * h + b, f1, f2);
-    const A da = dy * f1, k = w * da;
-    const A q = w * r * (u - u1 - h * u2) + uw * h + ub;
-    const A v = w * dy * f2 * q + uw * da - r * (u * k2 + k * u2);
-    gx = r * (v - v1 - h * v2) - r * r * h * along;
+    slopes<ACT, A>(wr * d + b, f1, f2);
+    const A da = dy * f1, rk = wr * da;
+    const A q = wr * (u - g.u1 - d * g.ru2) + uwr * d + ub;
+    gx = wr * (dy * f2 * q) + uwr * da - u * g.rrk2 - rk * g.ru2 - g.rv1 - d * g.e2;
     gdy = f1 * q;
 }
 
@@ -203,8 +221,8 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
                     A mean = 0, m2 = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (i < n) mean += (A)x[i].e[e];
-                    mean *= f;
+                        if (i < n) mean += (A)x[i].e[e] - (A)x[0].e[e];  // 0 of cells of one value
+                    mean = (A)x[0].e[e] + mean * f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (i < n) m2 += ((A)x[i].e[e] - mean) * ((A)x[i].e[e] - mean);
@@ -226,9 +244,11 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
                 if constexpr (MODE == 2) u = ldp<T, VEC>(reinterpret_cast<const T*>(a.u) + at);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e)
-                    add_sums<ACT, MODE, A>(s, e, (A)x.e[e], (A)dy.e[e], MODE == 2 ? (A)u.e[e] : (A)0, ch.r[e], ch.shift[e],
-                                           ch.w[e], ch.b[e]);
+                    add_sums<ACT, MODE, A>(s, e, (A)x.e[e], (A)dy.e[e], MODE == 2 ? (A)u.e[e] : (A)0, ch.mu[e],
+                                           ch.w[e] * ch.r[e], ch.b[e]);
             }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) scale_sums<MODE, A>(s, e, ch.r[e]);
         }
     }
     // over the threads of the same channels: in a wave, then over the waves
@@ -465,7 +485,8 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
     const int64_t base = p.n * a.L * a.C + p.c;
     Channels<A, VEC> ch;
     ch.load(a, p.n, p.c);
-    A g[6][VEC], uw[VEC], ub[VEC];
+    A g[2][VEC], uw[VEC], ub[VEC];
+    Group2<A> g2[MODE == 2 ? VEC : 1];
     if constexpr (MODE == 2) {
         params<A, VEC>(a.uw, p.c, (A)0, uw);
         params<A, VEC>(a.ub, p.c, (A)0, ub);
@@ -474,8 +495,14 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const A* s = reinterpret_cast<const A*>(a.means) + (p.n * a.G + (p.c + e) / a.cg) * MEANS[MODE];
-#pragma unroll
-            for (int i = 0; i < MEANS[MODE]; ++i) g[i][e] = s[i];
+            if constexpr (MODE == 1) {
+                g[0][e] = s[0] * ch.r[e];
+                g[1][e] = s[1] * ch.r[e] * ch.r[e];
+            } else {
+                const A r = ch.r[e];
+                g2[e] = Group2<A>(r, s[0], s[1], r * s[2], r * s[3], r * s[4], r * s[5]);
+                uw[e] *= r;
+            }
         }
     for (int64_t l = p.from + p.ty; l < p.to; l += p.step) {
         const int64_t at = base + l * a.C;
@@ -485,21 +512,20 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
         if constexpr (MODE == 2) u = ldp<T, VEC>(reinterpret_cast<const T*>(a.u) + at);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const A r = ch.r[e], w = ch.w[e];
+            const A wr = ch.w[e] * ch.r[e], b = ch.b[e];
             if constexpr (MODE == 2) {
                 A gx, gdy;
-                second_out<ACT, A>((A)x.e[e], (A)dy.e[e], (A)u.e[e], r, ch.shift[e], w, ch.b[e], uw[e], ub[e], g[0][e], g[1][e],
-                                   g[2][e], g[3][e], g[4][e], g[5][e], gx, gdy);
+                second_out<ACT, A>(g2[e], (A)x.e[e], (A)dy.e[e], (A)u.e[e], ch.mu[e], wr, b, uw[e], ub[e], gx, gdy);
                 o.e[e] = (T)gx;
                 o2.e[e] = (T)gdy;
             } else {
-                const A h = fused((A)x.e[e], r, ch.shift[e]), av = w * h + ch.b[e];
+                const A d = (A)x.e[e] - ch.mu[e], av = wr * d + b;
                 if constexpr (MODE == 0) {
                     o.e[e] = (T)act<ACT, A>(av);
                 } else {
                     A f1, f2;
                     slopes<ACT, A>(av, f1, f2);
-                    o.e[e] = (T)(r * (w * (A)dy.e[e] * f1 - g[0][e] - h * g[1][e]));
+                    o.e[e] = (T)(wr * ((A)dy.e[e] * f1) - g[0][e] - d * g[1][e]);
                 }
             }
         }
@@ -565,13 +591,13 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
         if constexpr (MODE >= 1) dy[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.dy) + off);
         if constexpr (MODE == 2) u[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.u) + off);
     }
-    A w[VEC], b[VEC], r = 0, shift = 0;
+    A w[VEC], b[VEC], mu = 0, r = 0;
     params<A, VEC>(a.w, c, (A)1, w);
     params<A, VEC>(a.b, c, (A)0, b);
     if constexpr (MODE >= 1) {
         const A* st = reinterpret_cast<const A*>(a.stats) + (n * a.G + g) * 2;
+        mu = st[0];
         r = st[1];
-        shift = -st[0] * st[1];
     }
     // Between the sums and the outputs the elements stay packed as they came, or they take twice the registers.
     const auto pack_again = [&]() {
@@ -628,8 +654,8 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
     };
 
     if constexpr (MODE == 0) {
-        double v[1];
-        A p[1] = {0};
+        double v[1], v2[2];
+        A p[1] = {0}, p2[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < R; ++i)
             if (on && ty + i * step < L) {
@@ -639,8 +665,8 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
             }
         pack_again();
         means(p, v);
-        const A mu = (A)v[0];
-        p[0] = 0;
+        // about that mean, which the sum's rounding has left a little off: the mean of what is left makes it up
+        mu = (A)v[0];
 #pragma unroll
         for (int i = 0; i < R; ++i)
             if (on && ty + i * step < L) {
@@ -648,13 +674,17 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const A d = (A)xv.e[e] - mu;
-                    p[0] += d * d;
+                    p2[0] += d;
+                    p2[1] += d * d;
                 }
             }
         pack_again();
-        means(p, v);
-        r = (A)(1.0 / sqrt(v[0] + a.eps));
-        shift = -mu * r;
+        means(p2, v2);
+        mu = (A)((double)mu + v2[0]);
+        const double var = v2[1] - v2[0] * v2[0];
+        r = (A)(1.0 / sqrt((var > 0 ? var : var == var ? 0.0 : var) + a.eps));
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] *= r;
         if (on && at % a.cg == 0 && ty == 0) {
             A* st = reinterpret_cast<A*>(a.stats) + (n * a.G + g) * 2;
             st[0] = mu;
@@ -668,11 +698,13 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
             const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]);
             Pack<T, VEC> o;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) o.e[e] = (T)act<ACT, A>(w[e] * fused((A)xv.e[e], r, shift) + b[e]);
+            for (int e = 0; e < VEC; ++e) o.e[e] = (T)act<ACT, A>(w[e] * ((A)xv.e[e] - mu) + b[e]);
             stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
         }
     } else {
         A s[NS][VEC] = {};
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] *= r;  // from here on
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             one_by_one();
@@ -680,9 +712,11 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
             const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]), uv = unpacked<T, VEC>(u[MODE == 2 ? i : 0]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
-                add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, r, shift, w[e], b[e]);
+                add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, mu, w[e], b[e]);
         }
         pack_again();
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) scale_sums<MODE, A>(s, e, r);
         A p[NG] = {};
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
@@ -692,7 +726,7 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
         means(p, v);
         if constexpr (MODE == 1) {
             if (a.chan) shares(s[1], s[0]);
-            const A k1 = (A)v[0], k2 = (A)v[1];
+            const A rk1 = (A)v[0], rrk2 = r * (A)v[1];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int l = ty + i * step;
@@ -702,16 +736,16 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const A h = fused((A)xv.e[e], r, shift);
+                    const A d = (A)xv.e[e] - mu;
                     A f1, f2;
-                    slopes<ACT, A>(w[e] * h + b[e], f1, f2);
-                    o.e[e] = (T)(r * (w[e] * (A)dv.e[e] * f1 - k1 - h * k2));
+                    slopes<ACT, A>(w[e] * d + b[e], f1, f2);
+                    o.e[e] = (T)(w[e] * ((A)dv.e[e] * f1) - rk1 - d * rrk2);
                 }
                 stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
             }
         } else {
-            const double u1d = v[0], u2d = v[1], k1d = v[2], k2d = v[3], rd = (double)r;
-            const A u1 = (A)u1d, u2 = (A)u2d, k2 = (A)k2d, along = (A)(v[4] - k1d * u1d - u2d * k2d);
+            const double u1d = v[0], u2d = v[1], rk1 = v[2], rk2 = v[3], rd = (double)r;
+            const A u1 = (A)u1d, u2 = (A)u2d;
             A uw[VEC], ub[VEC], gw[VEC], gb[VEC], q[2] = {0, 0};
             params<A, VEC>(a.uw, c, (A)0, uw);
             params<A, VEC>(a.ub, c, (A)0, ub);
@@ -720,18 +754,20 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
                 A th = 0;
                 gb[e] = 0;
                 if constexpr (ACT != 0) {  // q = cu u + ch h + cc
-                    const A cu = w[e] * r, ch = uw[e] - cu * u2, cc = ub[e] - cu * u1;
+                    const A cu = w[e], ch = uw[e] - cu * u2, cc = ub[e] - cu * u1;
                     gb[e] = cu * s[8][e] + ch * s[6][e] + cc * s[5][e];
                     th = cu * s[9][e] + ch * s[7][e] + cc * s[6][e];
                 }
+                gw[e] = r * (s[4][e] - u1 * s[2][e] - u2 * s[3][e]) + th;
+                uw[e] *= r;
                 q[0] += w[e] * gb[e] + uw[e] * s[2][e];
                 q[1] += w[e] * th + uw[e] * s[3][e];
-                gw[e] = r * (s[4][e] - u1 * s[2][e] - u2 * s[3][e]) + th;
             }
             double z[2];
             means(q, z);
             if (a.chan) shares(gw, gb);
-            const A v1 = (A)(z[0] - rd * (u1d * k2d + k1d * u2d)), v2 = (A)(z[1] - 2.0 * rd * u2d * k2d);
+            const Group2<A> gc(r, u1, u2, (A)rk2, (A)(z[0] - rd * (u1d * rk2 + rk1 * u2d)), (A)(z[1] - 2.0 * rd * u2d * rk2),
+                               (A)(v[4] - rk1 * u1d - u2d * rk2));
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int l = ty + i * step;
@@ -742,8 +778,7 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     A gx, gdy;
-                    second_out<ACT, A>((A)xv.e[e], (A)dv.e[e], (A)uv.e[e], r, shift, w[e], b[e], uw[e], ub[e], u1, u2, k2, v1, v2,
-                                       along, gx, gdy);
+                    second_out<ACT, A>(gc, (A)xv.e[e], (A)dv.e[e], (A)uv.e[e], mu, w[e], b[e], uw[e], ub[e], gx, gdy);
                     o.e[e] = (T)gx;
                     o2.e[e] = (T)gdy;
                 }
@@ -831,7 +866,9 @@ struct Scratch {
 // Whether a workgroup holds a sample's tile of groups, and how: W waves of some cells a thread, tx threads across the tile's
 // channels. A thread's vector (16 bytes; 4 channels of the second derivative, whose sums and three tensors fill the
 // registers) has to lie in one group, and a tile of whole groups to fill three quarters of the threads across, which take
-// 128 bytes of a cell or more: more where a sample has fewer cells than the rest of the workgroup holds. Larger groups
+// 128 bytes of a cell or more: more where a sample has fewer cells than the rest of the workgroup holds (a graded step of
+// 1,000 samples of 4 cells of 1,024 bf16 channels took 169 us with 28 of 32 threads idle, 119 across) or where a group is
+// wider (one group of 16 such cells: 427 us through the kernels above, 156 held). Larger groups
 // (above 256 cells at 128 bytes for the second derivative, 1,024 for the others) go through k_sums and k_apply, which read
 // everything twice.
 struct Whole {

@@ -176,6 +176,11 @@ def test_constant_groups_and_extremes(cuda):
     b = torch.linspace(-1, 1, 32, device=cuda)
     y = block.group_norm(torch.full((2, 20, 32), 3.0, device=cuda, dtype=torch.bfloat16), 4, None, b)
     assert torch.equal(y, b.to(torch.bfloat16).expand(2, 20, 32))
+    for shape in ((2, 20, 32), (1, 900, 512), (1, 3000, 12)):  # held by a workgroup, by 16 waves, read twice
+        b = torch.linspace(-1, 1, shape[-1], device=cuda)
+        for value in (1000.1, -3e4, 7e-3):
+            assert torch.equal(block.group_norm(torch.full(shape, value, device=cuda), 4, None, b), b.expand(shape))
+    b = torch.linspace(-1, 1, 32, device=cuda)
     x = torch.randn(3, 20, 32, generator=torch.Generator(cuda).manual_seed(1), device=cuda)
     good = block.group_norm(x, 4, None, b, EPS, "silu")
     for bad in (float("inf"), float("nan")):
@@ -278,6 +283,15 @@ def test_distilled_step_of_an_energy_with_group_norms(cuda, monkeypatch):
             assert p.grad is None, n
             continue
         assert float((p.grad - q.grad).norm()) <= 1e-4 * float(q.grad.norm().clamp(min=1e-6)), n
+
+
+def test_compiled_gradient_of_an_energy_with_group_norms(cuda):
+    """The energy's gradient under torch.compile agrees with eager to second order (the gate that training runs)."""
+    _say("compiled group norm")
+    model, _ = _model(cuda, block_impl="fused", embed_impl="fused")
+    x, z, _ = _batch(cuda)
+    errs = en.verify_compiled_energy_grad(model, en.compiled_energy_grad(model), z, model.puzzle_embedding(x, z.dtype))
+    assert max(errs.values()) < 1e-3
 
 
 def test_distilled_step_replays(cuda):

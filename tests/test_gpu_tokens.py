@@ -260,6 +260,10 @@ def test_distill_masked_logits(cuda, V):
     off = torch.ones(6, V, dtype=torch.bool, device=cuda).scatter_(1, ids, False) & (torch.arange(V, device=cuda) % 3 > 0)
     for low in (-math.inf, torch.finfo(torch.float32).min):
         _check_distill(x.masked_fill(off, low).to(torch.bfloat16), t, ids)
+    for dtype in (torch.float32, torch.bfloat16):  # a row whose mask leaves nothing: as if all were equal
+        y = x.to(dtype)
+        y[4] = torch.finfo(dtype).min
+        _check_distill(y, t, ids, T=0.9)
     t[0, 1:], t[1, 0], t[2] = -math.inf, -math.inf, -math.inf  # one entry left, one gone, a row without any
     _check_distill(x, t, ids)
     # the teacher wants what the student rules out: infinite, by the formula
