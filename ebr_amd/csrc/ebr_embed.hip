@@ -39,23 +39,24 @@ constexpr int ROWS = 4;
 template <typename TW, typename TY, int VEC>
 __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int team, double scale, const TW* w, TY* y) {
     using A = typename Acc<TW>::type;
+    using Raw = typename Words<VEC * (int)sizeof(TW)>::type;
     const int t = threadIdx.x & (team - 1), per = 256 / team;
     for (int64_t n0 = (int64_t)blockIdx.x * per * ROWS + threadIdx.x / team; n0 < N; n0 += (int64_t)gridDim.x * per * ROWS) {
         uint32_t v[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) v[r] = n0 + r * per < N ? token(ids, n0 + r * per) : (uint32_t)ids.V;
         for (int c = t * VEC; c < C; c += team * VEC) {
-            TW x[ROWS][VEC] = {};
+            Raw x[ROWS];  // (of row 0 where there is none)
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
-                if (v[r] < (uint32_t)ids.V) load_wide<TW, VEC>(w + (int64_t)v[r] * C + c, x[r]);
+                x[r] = *reinterpret_cast<const Raw*>(w + (int64_t)(v[r] < (uint32_t)ids.V ? v[r] : 0) * C + c);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (n0 + r * per >= N) break;
+                const Pack<TW, VEC> p = unpacked<TW, VEC>(x[r]);
                 Pack<TY, VEC> o;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)  // a row of zeros stays one, whatever the scale's sign
-                    o.e[e] = v[r] < (uint32_t)ids.V ? (TY)((A)x[r][e] * (A)scale) : (TY)0.f;
+                for (int e = 0; e < VEC; ++e) o.e[e] = v[r] < (uint32_t)ids.V ? (TY)((A)p.e[e] * (A)scale) : (TY)0.f;
                 stp<TY, VEC>(y + (n0 + r * per) * C + c, o);
             }
         }
@@ -144,6 +145,10 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(SortArgs a) {
     __shared__ uint32_t count[SORT_WAVES][SORT_DIGITS];
     __shared__ uint32_t start[SORT_DIGITS], waves[SORT_WAVES];
     const int t = threadIdx.x, wave = t >> 6, digits = 1 << a.bits;
+    const int64_t from = (int64_t)blockIdx.x * a.tiles * SORT_THREADS + t;
+    const auto key_at = [&](int64_t i) { return i < a.N ? (a.kin ? a.kin[i] : token(a.ids, i)) : 0; };
+    const auto pos_at = [&](int64_t i) { return i < a.N ? (a.kin ? a.pin[i] : (uint32_t)i) : 0; };
+    uint32_t next_key = key_at(from), next_pos = pos_at(from);  // on their way while the counts come
     uint32_t before = 0, total = 0;
     if (t < digits) {
 #pragma unroll 16
@@ -156,10 +161,13 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(SortArgs a) {
     const uint32_t base = digits_before(total, waves);
     if (t < digits) start[t] = base + before;
     for (int tile = 0; tile < a.tiles; ++tile) {
-        const int64_t i = ((int64_t)blockIdx.x * a.tiles + tile) * SORT_THREADS + t;
+        const int64_t i = from + (int64_t)tile * SORT_THREADS;
         const bool valid[1] = {i < a.N};
-        const uint32_t key[1] = {valid[0] ? (a.kin ? a.kin[i] : token(a.ids, i)) : 0};
-        const uint32_t pos = valid[0] ? (a.kin ? a.pin[i] : (uint32_t)i) : 0;
+        const uint32_t key[1] = {next_key}, pos = next_pos;
+        if (tile + 1 < a.tiles) {
+            next_key = key_at(i + SORT_THREADS);
+            next_pos = pos_at(i + SORT_THREADS);
+        }
         uint32_t rank[1];
         rank_tile<1>(key, valid, a.shift, a.bits, count, rank);
         if (t < digits) {
@@ -270,7 +278,7 @@ __device__ __forceinline__ int first_from(const uint32_t* key, int n, uint32_t v
     return lo;
 }
 
-constexpr int AHEAD = 8;  // rows whose loads are under way together
+constexpr int AHEAD = 8;  // rows whose loads are under way together (of 16 the sums take twice as long)
 
 // The first workgroups sum: a team of lanes, as many as there are columns for and a wave at most, takes a chunk of the
 // sorted positions and VEC columns a lane. A run of equal tokens inside the chunk is written to the table at once; a run
@@ -278,6 +286,7 @@ constexpr int AHEAD = 8;  // rows whose loads are under way together
 // search: these are most of the table for text, and their stores fill the time that the sums wait for their rows.
 template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_sum(SumArgs a) {
     using A = typename Acc<TW>::type;
+    using Raw = typename Words<VEC * (int)sizeof(TY)>::type;
     TW* dw = reinterpret_cast<TW*>(a.dw);
     if (blockIdx.x >= a.sum_blocks) {
         __shared__ uint8_t absent[256];
@@ -323,8 +332,9 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
     const auto fetch = [&](int i) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            key[j] = i + j < to ? a.key[i + j] : V;
-            pos[j] = i + j < to ? a.pos[i + j] : 0;
+            const int at = i + j < to ? i + j : to - 1;
+            key[j] = a.key[at];
+            pos[j] = a.pos[at];
         }
     };
     fetch(from);
@@ -338,13 +348,15 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
         if (opened || goes_on) store_wide<A, VEC>(part + (opened ? 0 : a.C), acc);
         else put_row<A, TW, VEC>(dw + (int64_t)cur * a.C + c, acc, a.scale);
     };
-    for (int i = from; i < to; i += AHEAD) {
-        Pack<TY, VEC> row[AHEAD];
+    for (int i = from; i < to && key[0] < V; i += AHEAD) {  // (positions without a token come last)
+        // no load depends on a condition (past the chunk's end it is the last row again), and rows stay as they lie in memory
+        // until their turn: as elements behind conditions, each of 16 bits would have a register of its own
+        Raw row[AHEAD];
         uint32_t k[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             k[j] = key[j];
-            if (k[j] < V) row[j] = ldp<TY, VEC>(dy + (int64_t)pos[j] * a.C);
+            row[j] = *reinterpret_cast<const Raw*>(dy + (int64_t)pos[j] * a.C);
         }
         if (i + AHEAD < to) fetch(i + AHEAD);
 #pragma unroll
@@ -357,9 +369,11 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] = 0;
             }
-            if (cur < V)
+            if (cur < V) {
+                const Pack<TY, VEC> v = unpacked<TY, VEC>(row[j]);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) acc[e] += (A)row[j].e[e];
+                for (int e = 0; e < VEC; ++e) acc[e] += (A)v.e[e];
+            }
         }
     }
     close(cur == after);
@@ -445,7 +459,7 @@ template <typename F> static int by_types(int wt, int yt, F f) {
 
 // Sorted positions that a team adds up: 64, or fewer (down to one round of loads) as far as that takes to have 768 waves,
 // three for each compute unit; more for very many positions, which bounds the parts that a run is in.
-constexpr int CHUNK = 64, MIN_CHUNK = AHEAD, MIN_WAVES = 768, MAX_CHUNKS = 4096;
+constexpr int CHUNK = 64, MIN_CHUNK = 8, MIN_WAVES = 768, MAX_CHUNKS = 4096;
 
 struct Plan {
     int passes, bits, groups, tiles, chunk, chunks;

@@ -536,14 +536,6 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
 
 // -- groups that a workgroup holds ---------------------------------------------------------------------------------------
 
-// Elements as they lie in memory: held as elements, each of 16 bits would have a register of its own.
-template <int BYTES> struct Words { using type = uint4; };
-template <> struct Words<8> { using type = uint2; };
-template <typename T, int VEC, typename W> __device__ __forceinline__ Pack<T, VEC> unpacked(W w) {
-    Pack<T, VEC> v;
-    __builtin_memcpy(&v, &w, sizeof(v));
-    return v;
-}
 __device__ __forceinline__ void opaque(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
 __device__ __forceinline__ void opaque(uint2& w) { asm volatile("" : "+v"(w.x), "+v"(w.y)); }
 

@@ -21,6 +21,18 @@ template <typename T, int N> __device__ __forceinline__ void stp(T* p, const Pac
     *reinterpret_cast<Pack<T, N>*>(p) = v;
 }
 
+// Elements as they lie in memory: held as elements, each of 16 bits would have a register of its own.
+template <int BYTES> struct Words { using type = uint4; };
+template <> struct Words<8> { using type = uint2; };
+template <> struct Words<4> { using type = uint32_t; };
+template <> struct Words<2> { using type = uint16_t; };
+template <typename T, int VEC, typename W> __device__ __forceinline__ Pack<T, VEC> unpacked(W w) {
+    Pack<T, VEC> v;
+    static_assert(sizeof(v) == sizeof(w), "the words of a pack");
+    __builtin_memcpy(&v, &w, sizeof(v));
+    return v;
+}
+
 // N elements of T from or to memory of which 16 bytes (or all of them, where fewer) are aligned, as whole vectors.
 template <typename T, int N, typename A> __device__ __forceinline__ void load_wide(const T* p, A (&x)[N]) {
     constexpr int V = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
