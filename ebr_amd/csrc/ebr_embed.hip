@@ -381,13 +381,13 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
 
 constexpr int JOIN_WAVES = 8;
 
-// Runs over chunks' borders: the workgroup of the chunk in which a run begins adds its parts, each wave every eighth, and
-// the waves' sums in order.
+// Runs over chunks' borders: the workgroup of the chunk in which a run begins adds its parts, its teams of lanes (as k_sum's)
+// in turn, and the teams' sums in order.
 template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_join(SumArgs a) {
     using A = typename Acc<TW>::type;
-    __shared__ A sums[JOIN_WAVES][64 * VEC];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int chunk = (int)blockIdx.x, c = (int)blockIdx.y * 64 * VEC + lane * VEC;
+    __shared__ A sums[JOIN_WAVES * 64 * VEC];
+    const int lane = threadIdx.x & 63, teams = 64 * JOIN_WAVES / a.team, team = threadIdx.x / a.team;
+    const int chunk = (int)blockIdx.x, at = (threadIdx.x & (a.team - 1)) * VEC, c = (int)blockIdx.y * a.team * VEC + at;
     const int from = chunk * a.chunk, next = from + a.chunk;
     const uint32_t k = a.key[next - 1];
     if (k >= (uint32_t)a.V || a.key[next] != k) return;                // nothing goes on (as for all that follow, of the
@@ -404,32 +404,33 @@ template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) vo
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0;
     if (c < a.C) {
-        if (wave == 0) load_wide<A, VEC>(part + ((int64_t)chunk * 2 + 1) * a.C, acc);
-        int j = chunk + 1 + wave;
-        for (; j + 3 * JOIN_WAVES < end; j += 4 * JOIN_WAVES) {
+        if (team == 0) load_wide<A, VEC>(part + ((int64_t)chunk * 2 + 1) * a.C, acc);
+        int j = chunk + 1 + team;
+        for (; j + 3 * teams < end; j += 4 * teams) {
             A x[4][VEC];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_wide<A, VEC>(part + (int64_t)(j + i * JOIN_WAVES) * 2 * a.C, x[i]);
+            for (int i = 0; i < 4; ++i) load_wide<A, VEC>(part + (int64_t)(j + i * teams) * 2 * a.C, x[i]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] += x[i][e];
         }
-        for (; j < end; j += JOIN_WAVES) {
+        for (; j < end; j += teams) {
             A x[VEC];
             load_wide<A, VEC>(part + (int64_t)j * 2 * a.C, x);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] += x[e];
         }
     }
+    const int width = a.team * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sums[wave][lane * VEC + e] = acc[e];
+    for (int e = 0; e < VEC; ++e) sums[team * width + at + e] = acc[e];
+    const int used = end - chunk - 1 < teams ? end - chunk - 1 : teams;  // teams that had a part
     __syncthreads();
-    if (wave || c >= a.C) return;
+    if (team || c >= a.C) return;
+    for (int w = 1; w < used; ++w)
 #pragma unroll
-    for (int w = 1; w < JOIN_WAVES; ++w)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += sums[w][lane * VEC + e];
+        for (int e = 0; e < VEC; ++e) acc[e] += sums[w * width + at + e];
     put_row<A, TW, VEC>(reinterpret_cast<TW*>(a.dw) + (int64_t)k * a.C + c, acc, a.scale);
 }
 
@@ -458,8 +459,9 @@ template <typename F> static int by_types(int wt, int yt, F f) {
 }
 
 // Sorted positions that a team adds up: 64, or fewer (down to one round of loads) as far as that takes to have 768 waves,
-// three for each compute unit; more for very many positions, which bounds the parts that a run is in.
-constexpr int CHUNK = 64, MIN_CHUNK = 8, MIN_WAVES = 768, MAX_CHUNKS = 4096;
+// three for each compute unit, of 512 columns each; more for very many positions, which bounds the parts that a run is in.
+constexpr int CHUNK = 64, MIN_CHUNK = 8, MAX_CHUNKS = 8192;
+constexpr int64_t MIN_COLUMNS = 768 * 512;
 
 struct Plan {
     int passes, bits, groups, tiles, chunk, chunks;
@@ -473,7 +475,7 @@ struct Plan {
         tiles = (int)((all + SORT_GROUPS - 1) / SORT_GROUPS);
         groups = tiles ? (int)((all + tiles - 1) / tiles) : 0;
         chunk = CHUNK;
-        while (chunk > MIN_CHUNK && (N + chunk - 1) / chunk * ((C + 511) / 512) < MIN_WAVES) chunk /= 2;
+        while (chunk > MIN_CHUNK && (N + chunk - 1) / chunk * C < MIN_COLUMNS) chunk /= 2;
         while ((N + chunk - 1) / chunk > MAX_CHUNKS) chunk *= 2;
         chunks = (int)((N + chunk - 1) / chunk);
         words = 4 * N + (int64_t)groups * SORT_DIGITS;
@@ -501,7 +503,8 @@ template <typename TW, typename TY, int VEC> static void launch_sums(hipStream_t
     hipLaunchKernelGGL((k_sum<TW, TY, VEC>), dim3((unsigned)(a.sum_blocks + zeros)), dim3(256), 0, s, a);
     if (a.chunks > 1) {
         constexpr int JV = VEC == 1 ? 1 : 16 / (int)sizeof(A);
-        const int64_t tiles = (a.C + 64 * JV - 1) / (64 * JV);
+        a.team = team_of(a.C, JV);
+        const int64_t tiles = (a.C + a.team * JV - 1) / (a.team * JV);
         hipLaunchKernelGGL((k_join<TW, JV>), dim3(a.chunks - 1, (unsigned)tiles), dim3(64 * JOIN_WAVES), 0, s, a);
     }
 }

@@ -193,6 +193,7 @@ template <int VEC> __device__ __forceinline__ Place place(const Args& a) {
 // Per-channel sums of a part of L.
 template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(THREADS) void k_sums(Args a) {
     using A = typename Acc<T>::type;
+    using Raw = typename Words<VEC * (int)sizeof(T)>::type;
     constexpr int NS = MODE == 0 ? 2 : MODE == 1 ? 2 : ACT ? 10 : 5, NL = MODE == 0 ? 3 : NS;
     __shared__ A lds[WAVES][64 * VEC];
     const Place p = place<VEC>(a);
@@ -205,27 +206,28 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
     if (p.on) {
         if constexpr (MODE == 0) {
             for (int64_t l = p.from + p.ty; l < p.to; l += 8 * (int64_t)p.step) {
-                Pack<T, VEC> x[8];
-                int n = 0;
+                Raw x[8];  // (past the end the last cell again)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int64_t row = l + (int64_t)i * p.step;
-                    if (row < p.to) {
-                        x[i] = ldp<T, VEC>(reinterpret_cast<const T*>(a.x) + base + row * a.C);
-                        ++n;
-                    }
+                    x[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.x) + base + (row < p.to ? row : p.to - 1) * a.C);
                 }
+                const int64_t left = (p.to - 1 - l) / p.step + 1;
+                const int n = left < 8 ? (int)left : 8;
                 const A f = (A)1 / (A)n;
+                Pack<T, VEC> xv[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) xv[i] = unpacked<T, VEC>(x[i]);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     A mean = 0, m2 = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (i < n) mean += (A)x[i].e[e] - (A)x[0].e[e];  // 0 of cells of one value
-                    mean = (A)x[0].e[e] + mean * f;
+                        if (i < n) mean += (A)xv[i].e[e] - (A)xv[0].e[e];  // 0 of cells of one value
+                    mean = (A)xv[0].e[e] + mean * f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (i < n) m2 += ((A)x[i].e[e] - mean) * ((A)x[i].e[e] - mean);
+                        if (i < n) m2 += ((A)xv[i].e[e] - mean) * ((A)xv[i].e[e] - mean);
                     Spread<A> v = {s[2][e], s[0][e], s[1][e]};
                     v.merge((A)n, mean, m2);
                     s[2][e] = v.n;
