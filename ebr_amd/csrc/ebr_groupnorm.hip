@@ -790,7 +790,7 @@ static int check(int dtype, int64_t B, int64_t L, int C, int groups, int act) {
         return EBR_ERR_DTYPE;
     if (B < 1 || L < 1 || C < 1 || C > (1 << 20) || groups < 1 || C % groups || B >= ((int64_t)1 << 31) ||
         L >= ((int64_t)1 << 40) || B * L >= ((int64_t)1 << 40) || B * L * C >= ((int64_t)1 << 40) ||
-        (act != EBR_ACT_NONE && act != EBR_ACT_SILU) || B * groups > MAX_BLOCKS)
+        (act != EBR_ACT_NONE && act != EBR_ACT_SILU))
         return EBR_ERR_SHAPE;
     return EBR_OK;
 }
@@ -925,7 +925,7 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
     a.rows = p.rows;
     const Whole h(MODE, dtype, a.L, a.C, a.G, vector);
     const int64_t blocks = h.waves ? a.B * h.tiles * (h.waves / 4) : a.B * p.splits * p.tiles;
-    if (blocks > MAX_BLOCKS) return EBR_ERR_SHAPE;
+    if (blocks > MAX_BLOCKS || (!h.waves && a.B * a.G > MAX_BLOCKS)) return EBR_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     by_kind(dtype, vector, act, [&](auto v, auto n, auto f) {
         using T = decltype(v);

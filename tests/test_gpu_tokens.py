@@ -110,6 +110,7 @@ def test_embedding_takes_what_users_hold(cuda):
     dy = torch.randn(961, generator=g, device=cuda)[1:].view(6, 10, 16)
     (dw,) = torch.autograd.grad(tokens.embedding(ids, leaf), leaf, dy)
     assert torch.equal(dw, torch.autograd.grad(tokens.embedding(ids, leaf), leaf, dy.clone())[0])
+    assert torch.equal(tokens.embedding(torch.tensor(3, device=cuda), leaf), leaf[3])  # one token, no batch
     for shape, V, C in (((0,), 5, 8), ((2, 0), 5, 8), ((3,), 5, 0), ((3,), 0, 8)):
         t = torch.zeros(V, C, device=cuda, requires_grad=True)
         y = tokens.embedding(torch.zeros(shape, dtype=torch.int64, device=cuda), t)
@@ -348,6 +349,44 @@ def _step_inputs(cuda, n=600, V=40, C=32):
     out_w = torch.randn(C, V, generator=g, device=cuda, requires_grad=True)
     t, tids = _teacher(cuda, (n,), V, 5, seed=1)
     return ids, w, out_w, t, tids
+
+
+def test_tokens_compiled(cuda):
+    """Under torch.compile (no Triton) the same ops run, with the eager call's bits."""
+    _say("tokens compiled")
+    a = _step_inputs(cuda)
+
+    def loss_of(ids, w, out_w, t, tids):
+        return tokens.distill_loss(tokens.embedding(ids, w, dtype=torch.bfloat16).float() @ out_w, t, tids, 2.0)
+
+    loss = torch.compile(loss_of, backend="aot_eager")(*a)
+    got = loss, *torch.autograd.grad(loss, (a[1], a[2]))
+    assert all(torch.equal(p, q) for p, q in zip(got, _step(*a)))
+
+
+def test_tokens_from_two_threads(cuda):
+    """Two programs' calls at once, each on a stream of its own."""
+    _say("tokens threads")
+    import threading
+
+    a = _step_inputs(cuda)
+    ref = _step(*a)
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            own = [p.detach().clone().requires_grad_(p.requires_grad) for p in a]
+            for _ in range(5):
+                got[i] = _step(*own)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(p, q) for i in range(2) for p, q in zip(ref, got[i]))
 
 
 def test_tokens_on_another_stream(cuda):

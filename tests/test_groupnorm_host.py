@@ -46,7 +46,7 @@ P = 0x100000  # a placeholder that no refused call reads
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dt=4), 1), (dict(act=2), 2), (dict(B=0), 2), (dict(L=0), 2), (dict(C=0), 2), (dict(G=0), 2), (dict(G=5), 2),
-    (dict(C=2**21, G=1), 2), (dict(B=2**30, L=2**30), 2), (dict(x=0), 4), (dict(stats=0), 4), (dict(y=0), 4),
+    (dict(C=2**21, G=1), 2), (dict(B=2**30, L=2**30), 2), (dict(B=2**25, L=1), 2), (dict(B=2**25, L=1, C=9, G=1), 2), (dict(x=0), 4), (dict(stats=0), 4), (dict(y=0), 4),
     (dict(scratch=0), 5), (dict(scratch=P + 4), 3),
 ])  # fmt: skip
 def test_entries_refuse(kw, code):
