@@ -103,6 +103,14 @@ template <typename A> struct Soft {
 
 template <typename T, int VEC> struct __attribute__((packed, aligned(sizeof(T)))) Loose { T e[VEC]; };
 
+template <typename T, int VEC> __device__ __forceinline__ void store_past(T* p, const Loose<T, VEC>& v) {
+    using W = uint32_t __attribute__((ext_vector_type(4)));
+    typedef W __attribute__((aligned(2))) LooseW;
+    W w;
+    __builtin_memcpy(&w, &v, 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<LooseW*>(p));
+}
+
 // Elements before the next 16-byte boundary.
 template <typename T> __device__ __forceinline__ int before_vectors(const T* p) {
     return (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T));
@@ -317,6 +325,10 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_sh
 // A row's columns, or a part of them, each from q alone; then the columns among them that the teacher names once more, each
 // by the first of its entries, which adds the others of the same column in their order. The second write comes after a
 // barrier, from the same workgroup.
+//
+// The stores go past the caches: otherwise what reads next waits for these lines to be written back. Of 4,096 rows of 50,021
+// bf16 logits a loss and its gradient took 271 us, and 252 so; of 2,600 rows 168 and 139 us, with a sum of the gradient
+// after it 253 and 224, and of 600 rows (60 MB, which the last-level cache would keep) 68 and 68.
 template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Args a) {
     using A = typename Acc<T>::type;
     constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
@@ -327,8 +339,10 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
     A* prob = reinterpret_cast<A*>(shared) + team * a.K;
     int* col = reinterpret_cast<int*>(reinterpret_cast<A*>(shared) + TEAMS * a.K) + team * a.K;
     uint32_t* seen = reinterpret_cast<uint32_t*>(shared + TEAMS * a.K * (int)(sizeof(A) + sizeof(int))) + team * (a.seen + 1);
-    const int64_t n = (int64_t)(blockIdx.x / a.splits) * (256 / TEAM) + team;
-    const int from = (int)(blockIdx.x % a.splits) * a.width, to = from + a.width < a.V ? from + a.width : a.V;
+    // the forward's last rows first: those that the last-level cache still has
+    const uint32_t block = gridDim.x - 1 - blockIdx.x;
+    const int64_t n = (int64_t)(block / a.splits) * (256 / TEAM) + team;
+    const int from = (int)(block % a.splits) * a.width, to = from + a.width < a.V ? from + a.width : a.V;
     const bool on = n < a.N;
     const BaseOf<T> k(a);
     Stats<A> st = {};
@@ -368,7 +382,7 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
                     V o;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) o.e[e] = (T)q(p[i].e[e]);
-                    *reinterpret_cast<V*>(dx + j + i * TEAM * VEC) = o;
+                    store_past<T, VEC>(dx + j + i * TEAM * VEC, o);
                 }
             }
             for (; j + VEC <= to; j += TEAM * VEC) {
@@ -376,7 +390,7 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
                 V o;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) o.e[e] = (T)q(p.e[e]);
-                *reinterpret_cast<V*>(dx + j) = o;
+                store_past<T, VEC>(dx + j, o);
             }
             for (; j < to; ++j) dx[j] = (T)q(x[j]);
         } else {

