@@ -217,6 +217,13 @@ __device__ __forceinline__ A teach(const Args& a, int64_t n, Stats<A>& st, int t
     return sum_all<TEAM, A>(sum, lds);
 }
 
+// The loss and the factor of its rows from their sum and number.
+template <typename A> __device__ __forceinline__ void finish(const Args& a, const Partial<A>& v) {
+    const double f = a.reduction == EBR_REDUCE_SUM ? 1.0 : 1.0 / (v.rows > 0 ? v.rows : 1.0);
+    *reinterpret_cast<A*>(a.loss) = (A)(v.loss * f);
+    *reinterpret_cast<A*>(a.scale) = (A)f;
+}
+
 // A part of a row, where there are too few rows to fill the card.
 template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
     using A = typename Acc<T>::type;
@@ -272,7 +279,8 @@ template <typename T, int TEAM, bool SHORT, bool JOIN> __global__ __launch_bound
             p.loss += rows[i][0];
             p.rows += rows[i][1];
         }
-        reinterpret_cast<Partial<A>*>(a.part)[blockIdx.x] = p;
+        if (gridDim.x == 1) finish<A>(a, p);
+        else reinterpret_cast<Partial<A>*>(a.part)[blockIdx.x] = p;
     }
 }
 
@@ -296,9 +304,7 @@ template <typename A> __global__ __launch_bounds__(1024) void k_total(Args a, in
             v.loss += lds[w].loss;
             v.rows += lds[w].rows;
         }
-        const double f = a.reduction == EBR_REDUCE_SUM ? 1.0 : 1.0 / (v.rows > 0 ? v.rows : 1.0);
-        *reinterpret_cast<A*>(a.loss) = (A)(v.loss * f);
-        *reinterpret_cast<A*>(a.scale) = (A)f;
+        finish<A>(a, v);
     }
 }
 
@@ -538,7 +544,7 @@ int ebr_block_distill(int dtype, int tdtype, int ids64, int64_t N, int64_t V, in
                                    dim3((unsigned)groups(N, team)), dim3(256), 0, s, a);
             });
         }
-        if (one) hipLaunchKernelGGL((k_total<A>), dim3(1), dim3(1024), 0, s, a, groups(N, team));
+        if (one && groups(N, team) != 1) hipLaunchKernelGGL((k_total<A>), dim3(1), dim3(1024), 0, s, a, groups(N, team));
         return launched();
     });
 }

@@ -639,12 +639,16 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
             store_wide<A, VEC>(waves + (row * 2 + 1) * tc + at, pb);
         }
         __syncthreads();
-        A* share = reinterpret_cast<A*>(a.chan) + n * 2 * a.C + c0;
+        // one sample's share is the gradient
+        A* share = reinterpret_cast<A*>(a.chan) + n * 2 * a.C;
+        A* of[2] = {a.B == 1 ? reinterpret_cast<A*>(a.dw) : share, a.B == 1 ? reinterpret_cast<A*>(a.db) : share + a.C};
         for (int i = t; i < 2 * tc; i += 64 * W) {
-            if (i % tc >= have) continue;
+            A* out = of[i >= tc];
+            const int at_ = i >= tc ? i - tc : i;
+            if (at_ >= have || !out) continue;
             A v = waves[i];
             for (int q = 1; q < rows; ++q) v += waves[q * 2 * tc + i];
-            share[i < tc ? i : a.C + i - tc] = v;
+            out[c0 + at_] = v;
         }
     };
 
@@ -939,7 +943,8 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
                 a.tiles = h.tiles;
                 launch_whole<T, MODE, ACT>(s, h, a);
             }
-            if (MODE != 0 && a.chan) hipLaunchKernelGGL((k_params<A>), dim3((a.C + 31) / 32, 2), dim3(1024), 0, s, a);
+            if (MODE != 0 && a.chan && a.B > 1)
+                hipLaunchKernelGGL((k_params<A>), dim3((a.C + 31) / 32, 2), dim3(1024), 0, s, a);
             return;
         }
         hipLaunchKernelGGL((k_sums<T, VEC, MODE, ACT>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a);
