@@ -108,9 +108,9 @@ template <typename A, int VEC> struct Channels {
     }
 };
 
-// An element's part of the sums of modes 1 and 2, with d in h's place; wr = w r.
+// An element's part of the sums of modes 1 and 2, with d in h's place; wr = w r. Returns da.
 template <int ACT, int MODE, typename A, int NS, int VEC>
-__device__ __forceinline__ void add_sums(A (&s)[NS][VEC], int e, A x, A dy, A u, A mu, A wr, A b) {
+__device__ __forceinline__ A add_sums(A (&s)[NS][VEC], int e, A x, A dy, A u, A mu, A wr, A b) {
     const A d = x - mu;
     A f1, f2;
     slopes<ACT, A>(wr * d + b, f1, f2);
@@ -133,6 +133,7 @@ __device__ __forceinline__ void add_sums(A (&s)[NS][VEC], int e, A x, A dy, A u,
             s[9][e] += tu * d;
         }
     }
+    return da;
 }
 
 // Their factors of r.
@@ -540,6 +541,7 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
 // -- groups that a workgroup holds ---------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void opaque(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+__device__ __forceinline__ void opaque(uint32_t& w) { asm volatile("" : "+v"(w)); }
 __device__ __forceinline__ void opaque(uint2& w) { asm volatile("" : "+v"(w.x), "+v"(w.y)); }
 
 // The next cell's arithmetic after this one's: side by side they take registers that hold other waves' elements.
@@ -553,7 +555,7 @@ __device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0)
 // derivative, in place of ten for each channel), and for the parameters' gradients, where they are wanted, two a channel.
 // With every channel's sums reduced, the second derivative of 768 boards of 81 x 512 took 224 us, most of it that reduction.
 template <typename T, int VEC, int MODE, int ACT, int R, int W>
-__global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(Args a) {
+__global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(Args a) {
     using A = typename Acc<T>::type;
     using Raw = typename Words<VEC * (int)sizeof(T)>::type;
     constexpr int NS = MODE == 0 ? 1 : MODE == 1 ? 2 : ACT ? 10 : 5, NG = MODE == 2 ? 5 : NS;
@@ -563,8 +565,9 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
     // where these are several waves
     const int rows = a.tx < 64 ? W : 64 * W / a.tx, row = a.tx < 64 ? wave : t / a.tx;
     const bool first = a.tx >= 64 || lane < a.tx;
+    constexpr int SLOTS = 2 * VEC > 5 ? 2 * VEC : 5;
     A* waves = reinterpret_cast<A*>(shared);  // [rows][NG][tx], and [rows][2][tc]
-    A* cols = waves + rows * 2 * tc;          // [NG][tx]
+    A* cols = waves + rows * SLOTS * a.tx;    // [NG][tx]
     const int tile = (int)(blockIdx.x % a.tiles);
     const int64_t n = blockIdx.x / a.tiles;
     const int c0 = tile * a.tile, have = a.C - c0 < a.tile ? a.C - c0 : a.tile;
@@ -635,8 +638,11 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
                 pb[e] += __shfl_xor(pb[e], d, 64);
             }
         if (first) {
-            store_wide<A, VEC>(waves + row * 2 * tc + at, pw);
-            store_wide<A, VEC>(waves + (row * 2 + 1) * tc + at, pb);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                waves[row * 2 * tc + at + e] = pw[e];
+                waves[(row * 2 + 1) * tc + at + e] = pb[e];
+            }
         }
         __syncthreads();
         // one sample's share is the gradient
@@ -701,6 +707,11 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
             stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
         }
     } else {
+        // The gradient of up to four cells keeps da, and its second half has neither dy nor the activation to take again: which
+        // is as long as the memory traffic otherwise (50 us for 768 boards of 81 x 512 bf16, 42 so). In the second derivative the
+        // same made no difference.
+        constexpr bool KEEP = MODE == 1 && ACT != 0 && R <= 4;
+        A kept[KEEP ? R : 1][KEEP ? VEC : 1];
         A s[NS][VEC] = {};
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[e] *= r;  // from here on
@@ -710,8 +721,10 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
             if (!on || ty + i * step >= L) continue;
             const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]), uv = unpacked<T, VEC>(u[MODE == 2 ? i : 0]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, mu, w[e], b[e]);
+            for (int e = 0; e < VEC; ++e) {
+                const A da = add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, mu, w[e], b[e]);
+                if constexpr (KEEP) kept[i][e] = da;
+            }
         }
         pack_again();
 #pragma unroll
@@ -736,9 +749,15 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 6 ? 4 : 1) void k_whole(A
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const A d = (A)xv.e[e] - mu;
-                    A f1, f2;
-                    slopes<ACT, A>(w[e] * d + b[e], f1, f2);
-                    o.e[e] = (T)(w[e] * ((A)dv.e[e] * f1) - rk1 - d * rrk2);
+                    A da;
+                    if constexpr (KEEP) {
+                        da = kept[i][e];
+                    } else {
+                        A f1, f2;
+                        slopes<ACT, A>(w[e] * d + b[e], f1, f2);
+                        da = (A)dv.e[e] * f1;
+                    }
+                    o.e[e] = (T)(w[e] * da - rk1 - d * rrk2);
                 }
                 stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
             }
@@ -863,55 +882,76 @@ struct Scratch {
 };
 
 // Whether a workgroup holds a sample's tile of groups, and how: W waves of some cells a thread, tx threads across the tile's
-// channels. A thread's vector (16 bytes; 4 channels of the second derivative, whose sums and three tensors fill the
-// registers) has to lie in one group, and a tile of whole groups to fill three quarters of the threads across, which take
-// 128 bytes of a cell or more: more where a sample has fewer cells than the rest of the workgroup holds (a graded step of
-// 1,000 samples of 4 cells of 1,024 bf16 channels took 169 us with 28 of 32 threads idle, 119 across) or where a group is
-// wider (one group of 16 such cells: 427 us through the kernels above, 156 held). Larger groups
-// (above 256 cells at 128 bytes for the second derivative, 1,024 for the others) go through k_sums and k_apply, which read
-// everything twice.
+// channels. A thread's vector has to lie in one group, and a tile of whole groups to fill three quarters of the threads
+// across, which take 128 bytes of a cell or more: more where a sample has fewer cells than the rest of the workgroup holds (a
+// graded step of 1,000 samples of 4 cells of 1,024 bf16 channels took 169 us with 28 of 32 threads idle, 119 across) or
+// where a group is wider (one group of 16 such cells: 427 us through k_sums and k_apply, 156 held). Above 256 cells at 128
+// bytes for the second derivative, 1,024 for the others, groups go through those, which read everything twice.
+//
+// The vector is 16 bytes, but 2 channels of 16 bits in the second derivative, whose ten sums a channel and three tensors
+// fill the registers: 768 boards of 81 x 512 bf16 took 113 us at 8 channels (three waves a SIMD), 102 at 4 (four), 94 at 2
+// (five). Of groups too wide for that, 4.
 struct Whole {
-    int waves = 0, cells = 0, tx = 0, tile = 0, tiles = 0;
+    int waves = 0, cells = 0, vec = 0, tx = 0, tile = 0, tiles = 0;
     // the two numbers of cells that there are kernels for
-    static constexpr int few(int mode, bool wide) { return mode != 2 ? 4 : wide ? 3 : 6; }
-    static constexpr int many(int mode, bool wide) { return mode != 2 || wide ? 8 : 16; }
+    static constexpr int few(int mode, bool wide, int vec) { return mode != 2 ? 4 : wide ? 3 : vec == 2 ? 12 : 16; }
+    static constexpr int many(int mode, bool wide, int vec) { return mode != 2 || wide ? 8 : vec == 2 ? 32 : 16; }
     Whole(int mode, int dtype, int64_t L, int C, int groups, bool vector) {
-        const int vec = mode == 2 ? 4 : vector_of(dtype, C), cg = C / groups;
-        if (!vector || dtype == EBR_DTYPE_F64 || vec == 1 || cg % vec || L > 4096) return;
+        const int full = vector_of(dtype, C);
         const bool wide = dtype == EBR_DTYPE_F32;
-        for (int x = !wide && vec == 4 ? 16 : 8; x <= 256; x *= 2) {
-            const int t = x * vec / cg * cg;
-            if (t == 0 || (t * 4 < x * vec * 3 && t < C)) continue;
-            const bool more = x < 256 && t < C && L * 2 * x <= 256;  // half of the cells of a workgroup would be none
-            if (more) continue;
+        if (!vector || dtype == EBR_DTYPE_F64 || full == 1 || L > 4096) return;
+        if (mode == 2 && !wide) {
+            if (!fit(mode, wide, 2, L, C, groups)) fit(mode, wide, 4, L, C, groups);
+        } else {
+            fit(mode, wide, full, L, C, groups);
+        }
+    }
+    bool fit(int mode, bool wide, int v, int64_t L, int C, int groups) {
+        const int cg = C / groups;
+        if (cg % v) return false;
+        for (int x = 128 / (v * (wide ? 4 : 2)); x <= 256; x *= 2) {
+            const int t = x * v / cg * cg;
+            if (t == 0 || (t * 4 < x * v * 3 && t < C)) continue;
+            if (x < 256 && t < C && L * 2 * x <= 256) continue;  // half of the cells of a workgroup would be none
             for (const int w : {4, 16}) {
                 if (w == 16 && (mode == 2 || x > 32)) continue;  // (registers; shared memory)
                 const int64_t step = 64 * w / x;
                 const int r = (int)((L + step - 1) / step);
-                if (r > many(mode, wide) || (w == 4 && r > 4 && mode != 2 && x <= 32)) continue;
+                if (r > many(mode, wide, v) || (w == 4 && r > 4 && mode != 2 && x <= 32)) continue;
                 waves = w;
-                cells = r <= few(mode, wide) ? few(mode, wide) : many(mode, wide);
+                cells = r <= few(mode, wide, v) ? few(mode, wide, v) : many(mode, wide, v);
+                vec = v;
                 tx = x;
                 tile = t < C ? t : C;
                 tiles = (C + tile - 1) / tile;
-                return;
+                return true;
             }
         }
+        return false;
     }
 };
 
-template <typename T, int MODE, int ACT> static void launch_whole(hipStream_t s, const Whole& h, const Args& a) {
+template <typename T, int VEC, int MODE, int ACT> static void launch_vec(hipStream_t s, const Whole& h, const Args& a) {
     using A = typename Acc<T>::type;
     constexpr bool WIDE = sizeof(T) == 4;
-    constexpr int VEC = MODE == 2 ? 4 : 16 / (int)sizeof(T), FEW = Whole::few(MODE, WIDE), MANY = Whole::many(MODE, WIDE);
+    constexpr int FEW = Whole::few(MODE, WIDE, VEC), MANY = Whole::many(MODE, WIDE, VEC);
     const int rows = h.tx < 64 ? h.waves : 64 * h.waves / h.tx;
-    const size_t lds = ((size_t)rows * 2 * h.tx * VEC + 5 * h.tx) * sizeof(A);
+    const size_t lds = ((size_t)rows * (2 * VEC > 5 ? 2 * VEC : 5) * h.tx + 5 * h.tx) * sizeof(A);
     const dim3 grid((unsigned)(a.B * h.tiles)), block(64 * h.waves);
     if (h.waves == 4 && h.cells == FEW) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, FEW, 4>), grid, block, lds, s, a);
     else if (h.waves == 4) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, MANY, 4>), grid, block, lds, s, a);
     else if constexpr (MODE != 2) {
         if (h.cells == FEW) hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, FEW, 16>), grid, block, lds, s, a);
         else hipLaunchKernelGGL((k_whole<T, VEC, MODE, ACT, MANY, 16>), grid, block, lds, s, a);
+    }
+}
+
+template <typename T, int MODE, int ACT> static void launch_whole(hipStream_t s, const Whole& h, const Args& a) {
+    if constexpr (MODE == 2 && sizeof(T) == 2) {
+        if (h.vec == 2) launch_vec<T, 2, MODE, ACT>(s, h, a);
+        else launch_vec<T, 4, MODE, ACT>(s, h, a);
+    } else {
+        launch_vec<T, 16 / (int)sizeof(T), MODE, ACT>(s, h, a);
     }
 }
 

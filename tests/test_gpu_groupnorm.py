@@ -138,7 +138,7 @@ def test_group_norm(cuda, dtype, act, shape, G):
 @pytest.mark.parametrize("shape,G", [
     ((2, 32, 64), 8), ((2, 33, 64), 4), ((3, 128, 96), 4), ((2, 129, 96), 4), ((2, 256, 64), 2), ((2, 257, 64), 2), ((2, 5, 512), 1),
     ((2, 130, 256), 2), ((1, 1024, 64), 8), ((1, 1025, 64), 8), ((2, 500, 128), 2), ((3, 17, 144), 3), ((1, 60, 2048), 4), ((700, 4, 64), 4),
-    ((3, 4, 1024), 32), ((2, 16, 1024), 1), ((2, 7, 2048), 1), ((2, 1, 512), 2), ((2, 3, 96), 2), ((5, 2, 264), 1), ((2, 9, 4096), 2),
+    ((3, 4, 1024), 32), ((2, 16, 1024), 1), ((2, 7, 2048), 1), ((2, 1, 512), 2), ((2, 3, 96), 2), ((5, 2, 264), 1), ((2, 9, 4096), 2), ((2, 30, 320), 32), ((1, 193, 60), 6), ((2, 256, 128), 64),
 ])  # fmt: skip
 def test_held_groups(cuda, dtype, shape, G):
     _say(f"group_norm held {shape} {G} {dtype}")
