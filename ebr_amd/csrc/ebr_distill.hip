@@ -224,7 +224,8 @@ template <typename A> __device__ __forceinline__ void finish(const Args& a, cons
     *reinterpret_cast<A*>(a.scale) = (A)f;
 }
 
-// A part of a row, where there are too few rows to fill the card.
+// A part of a row, where there are too few rows to fill the card: 24 rows of 131,072 fp32 logits took 95 us a workgroup each,
+// 5 us in 32 parts and 6 to join them (their gradient 108 and 6).
 template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
     using A = typename Acc<T>::type;
     __shared__ A lds[16];
@@ -235,7 +236,9 @@ template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
     if (threadIdx.x == 0) reinterpret_cast<Soft<A>*>(a.soft)[blockIdx.x] = v;
 }
 
-// Rows' losses, from the logits, or with JOIN from the rows' parts.
+// Rows' losses, from the logits, or with JOIN from the rows' parts. 4,096 rows of 50,021 bf16 logits take 87 us (4.7 TB/s;
+// loading the next round ahead of this one's arithmetic, or a maximum in fewer instructions, made no difference), 31,104 rows
+// of 11 8 us (latency: a row's entries, their logits).
 template <typename T, int TEAM, bool SHORT, bool JOIN> __global__ __launch_bounds__(256) void k_loss(Args a) {
     using A = typename Acc<T>::type;
     __shared__ A lds[16];
@@ -308,7 +311,7 @@ template <typename A> __global__ __launch_bounds__(1024) void k_total(Args a, in
     }
 }
 
-// Rows of at most TEAM columns: a thread has a column and goes through the row's entries.
+// Rows of at most TEAM columns: a thread has a column and goes through the row's entries. 31,104 rows of 11 take 6 us.
 template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_short(Args a) {
     using A = typename Acc<T>::type;
     const int t = threadIdx.x % TEAM;
@@ -334,7 +337,8 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_sh
 //
 // The stores go past the caches: otherwise what reads next waits for these lines to be written back. Of 4,096 rows of 50,021
 // bf16 logits a loss and its gradient took 271 us, and 252 so; of 2,600 rows 168 and 139 us, with a sum of the gradient
-// after it 253 and 224, and of 600 rows (60 MB, which the last-level cache would keep) 68 and 68.
+// after it 253 and 224, and of 600 rows (60 MB, which the last-level cache would keep) 68 and 68. The gradient alone takes
+// 148 us for the 4,096 rows (820 MB, 5.5 TB/s).
 template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Args a) {
     using A = typename Acc<T>::type;
     constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
@@ -426,7 +430,8 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
 
 constexpr int SHORT_ROW = 32;  // columns of a row in which each has a thread
 
-// k_grad's bits for the columns of a part: exact up to 2^17.
+// k_grad's bits for the columns of a part: exact up to 2^17. Without them each entry went through all the others: 20,000 rows
+// of 4,001 with 256 entries took 265 us with their loss, 178 with them.
 static int seen_of(int64_t width) {
     int w = 1;
     while (w < 4096 && (int64_t)w * 32 < width) w *= 2;
@@ -436,8 +441,9 @@ static int64_t shared_of(int team, int K, int64_t width, int es) {
     return (int64_t)(256 / team) * (K * (int64_t)(es + 4) + 4 * (seen_of(width) + 1));
 }
 
-// Threads of a row: one a column for the shortest; then as many lanes as it has vectors, up to a wave, but not so few that
-// the rows of a workgroup take more than 32 KiB of shared memory in the gradient; a workgroup for long rows.
+// Threads of a row: one a column for the shortest; then as many lanes as it has vectors, up to a wave (65,536 rows of 97
+// bf16 took 104 us a wave each, 62 with 16 lanes), but not so few that the rows of a workgroup take more than 32 KiB of shared
+// memory in the gradient; a workgroup for long rows.
 static int team_of(int dtype, int64_t V, int K) {
     if (V > 2048) return 256;
     int t = 8;

@@ -34,7 +34,8 @@ __device__ __forceinline__ uint32_t token(const Ids& ids, int64_t n) {
 // -- lookup ------------------------------------------------------------------------------------------------------------
 
 // A row's threads, at most a wave of them, go over its columns VEC at a time, ROWS rows side by side: a row's load waits
-// for its token's, and the next rows' fill that time.
+// for its token's, and the next rows' fill that time. 31,104 rows of 512 bf16 from an fp32 table of 11 take 11 us (2.8 TB/s
+// of writes; the chain token, row, store is half of it), 32,768 rows of 2,048 from one of 100,003 57 us (4.1 TB/s).
 constexpr int ROWS = 4;
 template <typename TW, typename TY, int VEC>
 __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int team, double scale, const TW* w, TY* y) {
@@ -67,7 +68,8 @@ __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int t
 
 // A workgroup ranks a tile of 1,024 positions a round, as many rounds as leave at most 128 workgroups (each reads all the
 // others' counts); up to 4,096 positions are one workgroup's. A tile of 4,096 left most of the card idle: 16,384 positions
-// took 9.9 us a pass, 5.5 in tiles of 1,024.
+// took 9.9 us a pass, 5.4 in tiles of 1,024 (and 2.9 the counts before it). Latency bounds it: launches, and what one kernel
+// wrote and the next reads on other XCDs. Nine bits a pass: one for boards, two up to a vocabulary of 262,143.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ONE = 4096;
 constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS;
 constexpr int SORT_GROUPS = 128;
@@ -283,7 +285,10 @@ constexpr int AHEAD = 8;  // rows whose loads are under way together (of 16 the 
 // The first workgroups sum: a team of lanes, as many as there are columns for and a wave at most, takes a chunk of the
 // sorted positions and VEC columns a lane. A run of equal tokens inside the chunk is written to the table at once; a run
 // over its border goes to part. The other workgroups write zeros to the rows of tokens that do not occur, found by
-// search: these are most of the table for text, and their stores fill the time that the sums wait for their rows.
+// search: these are most of the table for text, and their stores fill the time that the sums wait for their rows. They go
+// past the caches, in whole lines: 16,384 tokens of 50,021 x 1,024 bf16 took 81 us with their gradient, 61 so (but 32 bytes a
+// lane, which halves lines, cost the fp32 table of 100,003 x 2,048 150 us).
+// Bound by memory: 21 us for those tokens (132 MB, 6.3 TB/s), 188 us for 32,768 tokens of that table (953 MB, 5.1 TB/s).
 template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_sum(SumArgs a) {
     using A = typename Acc<TW>::type;
     using Raw = typename Words<VEC * (int)sizeof(TY)>::type;
@@ -382,7 +387,8 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
 constexpr int JOIN_WAVES = 8;
 
 // Runs over chunks' borders: the workgroup of the chunk in which a run begins adds its parts, its teams of lanes (as k_sum's)
-// in turn, and the teams' sums in order.
+// in turn, and the teams' sums in order. 4 to 7 us, most of it the launch: few runs are that long, but one wave for each took
+// 22 us where 11 tokens have 31,104 positions.
 template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_join(SumArgs a) {
     using A = typename Acc<TW>::type;
     __shared__ A sums[JOIN_WAVES * 64 * VEC];
