@@ -191,9 +191,10 @@ template <int TEAM, typename A> __device__ __forceinline__ A sum_all(A v, A* lds
 }
 
 // The teacher's part of a row, once its student statistics are known: its statistics and the row's loss in units of
-// weight.
+// weight. These few terms are taken in 64 bits: a logit that a mask has set to the type's lowest value has a logarithm
+// that 32 bits hold in the end, but not in base 2 nor below T = 1.
 template <typename T, int TEAM, typename A>
-__device__ __forceinline__ A teach(const Args& a, int64_t n, Stats<A>& st, int t, bool on, A* lds) {
+__device__ __forceinline__ double teach(const Args& a, int64_t n, Stats<A>& st, int t, bool on, A* lds, double* sums) {
     const Base<A, true> k(a);
     Soft<A> v = {lowest<A>(), 0};
     if (on)
@@ -202,19 +203,19 @@ __device__ __forceinline__ A teach(const Args& a, int64_t n, Stats<A>& st, int t
     soft_all<TEAM, A>(v, k, lds);
     st.tm = v.m;
     st.ts = v.s;
-    A sum = 0;
+    double sum = 0;
     if (on && v.s != (A)0) {
-        const A ts2 = lg2(v.s), s2 = lg2(st.s);
+        const double ts2 = lg2(v.s), s2 = lg2(st.s);
         const T* x = reinterpret_cast<const T*>(a.x) + n * a.row;
         for (int i = t; i < a.K; i += TEAM) {
             const int c = column(a, n * a.K + i);
             if (c < 0) continue;
             const A e = k.times(teacher_at<A>(a, n * a.K + i) - v.m), p = pow2(e) / v.s;
             if (p == (A)0) continue;
-            sum += p * ((e - ts2) - (k.times((A)x[c] - st.m) - s2));
+            sum += p * ((e - ts2) - (((double)x[c] - st.m) * a.k - s2));
         }
     }
-    return sum_all<TEAM, A>(sum, lds);
+    return sum_all<TEAM, double>(sum, sums);
 }
 
 // The loss and the factor of its rows from their sum and number.
@@ -242,7 +243,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
 template <typename T, int TEAM, bool SHORT, bool JOIN> __global__ __launch_bounds__(256) void k_loss(Args a) {
     using A = typename Acc<T>::type;
     __shared__ A lds[16];
-    __shared__ double rows[256 / TEAM][2];
+    __shared__ double rows[256 / TEAM][2], sums[4];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const int64_t n = (int64_t)blockIdx.x * (256 / TEAM) + team;
     const bool on = n < a.N;
@@ -263,15 +264,15 @@ template <typename T, int TEAM, bool SHORT, bool JOIN> __global__ __launch_bound
     }
     soft_all<TEAM, A>(v, k, lds);
     Stats<A> st = {v.m, v.s, 0, 0};
-    const A sum = teach<T, TEAM, A>(a, n, st, t, on, lds);
+    const double sum = teach<T, TEAM, A>(a, n, st, t, on, lds, sums);
     if (t == 0) {
         const bool counted = on && st.ts != (A)0;
-        const A loss = counted ? (A)a.weight * sum : (A)0;
+        const double loss = counted ? a.weight * sum : 0;
         if (on) {
             reinterpret_cast<Stats<A>*>(a.stats)[n] = st;
-            if (a.reduction == EBR_REDUCE_NONE) reinterpret_cast<A*>(a.loss)[n] = loss;
+            if (a.reduction == EBR_REDUCE_NONE) reinterpret_cast<A*>(a.loss)[n] = (A)loss;
         }
-        rows[team][0] = (double)loss;
+        rows[team][0] = loss;
         rows[team][1] = counted;
     }
     if (a.reduction == EBR_REDUCE_NONE) return;
@@ -474,8 +475,9 @@ static float low_of(double k) { return (float)(k - (double)(float)k); }
 static int check(int dtype, int tdtype, int64_t N, int64_t V, int K, int64_t row, double T) {
     for (const int d : {dtype, tdtype})
         if (d != EBR_DTYPE_F32 && d != EBR_DTYPE_BF16 && d != EBR_DTYPE_F16 && d != EBR_DTYPE_F64) return EBR_ERR_DTYPE;
+    // (T: so that its square, and what Base adds at 32 bits, are far from the largest float)
     if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V >= ((int64_t)1 << 30) || K < 1 || K > K_MAX || row < V ||
-        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T > 0) || T > 1e30 || T < 1e-30 || groups(N, team_of(dtype, V, K)) > MAX_BLOCKS)
+        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T >= 1e-15 && T <= 1e15) || groups(N, team_of(dtype, V, K)) > MAX_BLOCKS)
         return EBR_ERR_SHAPE;
     return EBR_OK;
 }

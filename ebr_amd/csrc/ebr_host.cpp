@@ -1438,8 +1438,8 @@ py::object distill_loss(const py::handle& hx, const py::handle& ht, const py::ha
         dtype_code(t.scalar_type()) < 0 || t.device() != x.device() || ids.device() != x.device() || recorded({t}))
         return py::none();
     const int64_t lead = x.dim() - 1;
-    if (x.sizes().slice(0, lead) != t.sizes().slice(0, lead) || t.size(lead) > 1024 || !(temperature >= 1e-30) ||
-        temperature > 1e30)
+    if (x.sizes().slice(0, lead) != t.sizes().slice(0, lead) || t.size(lead) > 1024 || !(temperature >= 1e-15) ||
+        temperature > 1e15)
         return py::none();
     if (ebr_block_distill_scratch(dtype_code(x.scalar_type()), x.numel() / x.size(lead), x.size(lead), (int)t.size(lead)) < 0)
         return py::none();

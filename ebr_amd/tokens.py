@@ -205,8 +205,8 @@ def _check_distill(logits: Tensor, teacher: Tensor, ids: Tensor, temperature: fl
     if teacher.device != logits.device or ids.device != logits.device:
         raise ValueError(f"tokens: logits are on {logits.device}, teacher_logits on {teacher.device}, teacher_ids on "
                          f"{ids.device}")
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"tokens: temperature must be positive and finite, got {temperature}")
+    if not 1e-15 <= temperature <= 1e15:
+        raise ValueError(f"tokens: temperature must be from 1e-15 to 1e15, got {temperature}")
 
 
 def _rows(logits: Tensor) -> Tuple[Tensor, int]:
@@ -340,7 +340,8 @@ def distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, te
 
     A row without an entry of positive probability has loss 0 and gradient 0. ``reduction``: "mean" over the other rows (0
     if there is none), "sum", or "none" for [...]. The loss is fp32 (fp64 for fp64 logits) whatever the logits' dtype. K is
-    at most 1024; a teacher entry of one token with any logit is the cross entropy to it. Only the logits get a gradient."""
+    at most 1024, T from 1e-15 to 1e15; a teacher entry of one token with any logit is the cross entropy to it. Only the
+    logits get a gradient."""
     host = _host.module()
     y = None if host is None or reduction not in REDUCTIONS else host.distill_loss(
         logits, teacher_logits, teacher_ids, temperature, REDUCTIONS[reduction])

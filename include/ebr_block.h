@@ -72,9 +72,10 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
 /* How rows' losses go together. */
 enum { EBR_REDUCE_NONE = 0, EBR_REDUCE_SUM = 1, EBR_REDUCE_MEAN = 2 };
 
-/* Distillation from the K (at most 1024) top logits of a teacher: with p the softmax of a row's teacher / T over the
- * entries whose ids lie in [0, V), and q the softmax of its logits / T, loss = T^2 sum_k p_k (log p_k - log q_id_k). A row
- * without an entry of positive probability has loss 0 and is not counted in the mean (0 if none is).
+/* Distillation from the K (at most 1024) top logits of a teacher at a temperature T from 1e-15 to 1e15: with p the softmax
+ * of a row's teacher / T over the entries whose ids lie in [0, V), and q the softmax of its logits / T, loss = T^2 sum_k p_k
+ * (log p_k - log q_id_k). A row without an entry of positive probability has loss 0 and is not counted in the mean (0 if
+ * none is).
  * logits: N rows of V, row_stride elements apart; teacher (of tdtype) and ids (int64 where ids64, else int32): contiguous
  * [N, K]. loss: fp32 (fp64 for fp64 logits), [N] for EBR_REDUCE_NONE, else one. stats: [N, 4] of loss's type, 16-byte
  * aligned, and scale: one of it (not for EBR_REDUCE_NONE), both for the backward. */

@@ -221,6 +221,30 @@ def test_distill(cuda, dtype, lead, V, K):
     _check_distill(x, t, ids, T=1.0 if K % 2 else 2.5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [5, 97, 5000, 20000])
+@pytest.mark.parametrize("T", [0.5, 1.0])
+def test_distill_entry_whose_logit_a_mask_has_set_to_the_lowest_value(cuda, dtype, V, T):
+    """The loss is p (max - lowest) T but for terms of order 1, half of the largest float at T = 1: finite in 32 bits, though
+    the logarithm in base 2, or at T = 0.5, is not. p = 1/2 exactly, and 16 steps are far more than the roundings of the
+    difference, the product and the result (half a step each)."""
+    _say(f"distill lowest logit {V} {dtype} {T}")
+    x = torch.randn(7, V, generator=torch.Generator().manual_seed(3)).to(cuda, dtype)
+    x[:, 1] = torch.finfo(dtype).min
+    ids = torch.tensor([[1, 2]], device=cuda).expand(7, 2)
+    t = torch.zeros(7, 2, device=cuda)
+    x.requires_grad_(True)
+    ref = 0.5 * T * (x.detach().double().amax(-1) - torch.finfo(dtype).min)
+    rows = tokens.distill_loss(x, t, ids, T, "none")
+    loss = tokens.distill_loss(x, t, ids, T)
+    assert bool(((rows.detach().double() - ref).abs() <= 16 * 2.0**-24 * ref).all())
+    assert abs(loss.item() - ref.mean().item()) <= 16 * 2.0**-24 * ref.mean().item()
+    (dx,) = torch.autograd.grad(loss, x)
+    assert bool(torch.isfinite(dx).all())
+    want = -T * 0.5 / 7  # no probability of its own
+    assert bool(((dx[:, 1].double() - want).abs() <= torch.finfo(dtype).eps * abs(want)).all())
+
+
 # every number of threads a row, rows that end inside a workgroup, and many entries for short rows
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
 @pytest.mark.parametrize("N,V,K", [(70, 32, 5), (70, 33, 33), (50, 97, 8), (37, 130, 100), (19, 300, 256), (9, 500, 500), (6, 1024, 1024),

@@ -123,3 +123,9 @@ def test_scratch_sizes():
     assert lib.ebr_block_embed_bwd_scratch(0, 5000, 0, 512) == -1
     assert lib.ebr_block_distill_scratch(1, 100, 11, 4) > 0
     assert lib.ebr_block_distill_scratch(1, 100, 11, 0) == -1
+
+
+@pytest.mark.parametrize("temperature", [9e-16, 1.1e15, float("inf"), -1.0])
+def test_distill_refuses_temperatures_whose_square_leaves_fp32(temperature):
+    with pytest.raises(ValueError, match="temperature"):
+        _distill(temperature=temperature)
