@@ -6,7 +6,7 @@
 // Both are bound by memory. The lookup reads the tokens' rows and writes y. The gradient has to read dy once and to write
 // the whole table, most of it zeros for text; what costs is bringing a token's rows together. Atomic sums would do that in
 // an order that changes from run to run, so the positions are sorted by token instead (a stable radix sort: equal tokens
-// keep their order), and a sum always adds the same rows in the same order, in 32 bits.
+// keep their order; few tokens need none), and a sum always adds the same rows in the same order, in 32 bits.
 #include <type_traits>
 
 #include "rowwise.hpp"
@@ -440,6 +440,57 @@ template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) vo
     put_row<A, TW, VEC>(reinterpret_cast<TW*>(a.dw) + (int64_t)k * a.C + c, acc, a.scale);
 }
 
+// -- few tokens --------------------------------------------------------------------------------------------------------
+
+// A workgroup for each row of the table and 64 vectors of its columns: its four waves look through a quarter of the positions
+// each, a position a lane, and add the rows of those that hold its token, AHEAD at a time; then the waves' sums go together in
+// order. One launch in place of three, no scratch, nothing waited for: 81 tokens of 11 x 512 take 2.8 us in a row of calls,
+// sorted 10.6, and of 16,000 x 2,048 29 and 33. 256 positions of one token, the slowest, 11 and 12; 32,768 rows of 64 columns,
+// each a workgroup's, about the same.
+constexpr int FEW = 256, FEW_ROWS = 32768;
+
+template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_few(Ids ids, int N, int C, double scale,
+                                                                                          const TY* dy, TW* dw) {
+    using A = typename Acc<TW>::type;
+    using Raw = typename Words<VEC * (int)sizeof(TY)>::type;
+    __shared__ A sums[4][64 * VEC];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane * VEC;
+    const int64_t c = (int64_t)blockIdx.y * 64 * VEC + at;
+    const int per = (N + 3) / 4, n = wave * per + lane;
+    const uint32_t v = blockIdx.x;
+    uint64_t mine = __ballot(lane < per && n < N && token(ids, n) == v);
+    const TY* from = dy + (int64_t)wave * per * C + (c < C ? c : 0);
+    A acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0;
+    while (mine) {
+        Raw row[AHEAD];
+        const int have = __popcll(mine);
+        int p = 0;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {  // past the last one it is that one again
+            if (mine) p = __ffsll((unsigned long long)mine) - 1;
+            mine &= mine - 1;
+            row[j] = *reinterpret_cast<const Raw*>(from + (int64_t)p * C);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (j >= have) break;
+            const Pack<TY, VEC> x = unpacked<TY, VEC>(row[j]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += (A)x.e[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sums[wave][at + e] = acc[e];
+    __syncthreads();
+    if (wave || c >= C) return;
+    for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += sums[w][at + e];
+    put_row<A, TW, VEC>(dw + (int64_t)v * C + c, acc, scale);
+}
+
 // -- launches ----------------------------------------------------------------------------------------------------------
 
 static bool types_ok(int wt, int yt) {
@@ -489,6 +540,8 @@ struct Plan {
         part = (int64_t)chunks * 2 * C;
     }
 };
+
+static bool few(int64_t N, int64_t V) { return N > 0 && N <= FEW && V <= FEW_ROWS; }
 
 // Lanes of a row of C / vec vectors: the next power of two, at most a wave.
 static int team_of(int C, int vec) {
@@ -558,6 +611,20 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
     if (N > 0 && !scratch) return EBR_ERR_SCRATCH;
     if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
     hipStream_t s = (hipStream_t)stream;
+    if (few(N, V))
+        return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
+            using TW = decltype(tw);
+            using TY = decltype(ty);
+            constexpr int VEC = 16 / (int)sizeof(TY);
+            const auto go = [&](auto vec) {
+                constexpr int VN = decltype(vec)::value;
+                hipLaunchKernelGGL((k_few<TW, TY, VN>), dim3((unsigned)V, (C + 64 * VN - 1) / (64 * VN)), dim3(256), 0, s,
+                                   Ids{ids, ids64 != 0, (int)V}, (int)N, C, scale, (const TY*)dy, (TW*)dw);
+            };
+            if (C % VEC == 0 && aligned(dy, 16) && aligned(dw, 16)) go(std::integral_constant<int, VEC>());
+            else go(std::integral_constant<int, 1>());
+            return launched();
+        });
     const Plan p(N, V, C);
     uint32_t* w32 = reinterpret_cast<uint32_t*>(scratch);
     uint32_t *k0 = w32, *p0 = w32 + N, *k1 = w32 + 2 * N, *p1 = w32 + 3 * N, *counts = w32 + 4 * N;

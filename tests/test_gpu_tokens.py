@@ -74,6 +74,29 @@ def test_embedding(cuda, wt, yt, N, V, C):
     _check_embed(ids, w, 1.0 if C % 2 else -1.7, yt)
 
 
+# the most tokens and rows that go without a sort, and one more of each; columns that end inside a tile and off the vectors
+@pytest.mark.parametrize("N,V,C", [(256, 11, 520), (257, 11, 520), (255, 32768, 8), (256, 32769, 8), (3, 32768, 9), (256, 2, 1537),
+                                   (64, 5, 513), (65, 1, 24)])  # fmt: skip
+@pytest.mark.parametrize("wt,yt", PAIRS[:4])
+def test_embedding_of_few_tokens(cuda, wt, yt, N, V, C):
+    _say(f"embedding of few {N} {V} {C} {wt} {yt}")
+    g = torch.Generator(cuda).manual_seed(N)
+    ids = (torch.rand(N, generator=g, device=cuda) ** 3 * V).long()
+    ids[N // 2 :: 9] = -1
+    ids[-1] = V - 1
+    _check_embed(ids.int() if C % 2 else ids, torch.randn(V, C, generator=g, device=cuda).to(wt), 2.5, yt)
+
+
+# as below, with more tokens than go without a sort
+@pytest.mark.parametrize("ids", [
+    [-1] * 290, [3] * 900, [0, 2**32 + 3, 2**40, -(2**32) + 1, 6] * 60, list(range(7)) * 50 + [7], [5] * 264 + [6] * 64, [5] * 63 + [6] * 630,
+])  # fmt: skip
+def test_embedding_of_special_tokens_sorted(cuda, ids):
+    _say(f"embedding of {len(ids)} {ids[:5]}..")
+    w = torch.randn(7, 16, generator=torch.Generator(cuda).manual_seed(1), device=cuda)
+    _check_embed(torch.tensor(ids, device=cuda), w, 1.0, torch.float32)
+
+
 # more than one workgroup's sort (4096), one, two and three passes of 9 bits, more than 256 sort groups of a tile (2^20), and
 # chunks of more than 64 positions (2^18)
 @pytest.mark.parametrize("N,V,C", [(4097, 11, 64), (20000, 50021, 40), (9000, 300001, 9), (300000, 5, 16), (1100000, 70000, 2)])
