@@ -6,7 +6,8 @@
 // Both are bound by memory. The lookup reads the tokens' rows and writes y. The gradient has to read dy once and to write
 // the whole table, most of it zeros for text; what costs is bringing a token's rows together. Atomic sums would do that in
 // an order that changes from run to run, so the positions are sorted by token instead (a stable radix sort: equal tokens
-// keep their order; few tokens need none), and a sum always adds the same rows in the same order, in 32 bits.
+// keep their order; few tokens, and small tables, need no sort), and a sum always adds the same rows in the same order, in 32
+// bits.
 #include <type_traits>
 
 #include "rowwise.hpp"
@@ -388,7 +389,7 @@ constexpr int JOIN_WAVES = 8;
 
 // Runs over chunks' borders: the workgroup of the chunk in which a run begins adds its parts, its teams of lanes (as k_sum's)
 // in turn, and the teams' sums in order. 4 to 7 us, most of it the launch: few runs are that long, but one wave for each took
-// 22 us where 11 tokens have 31,104 positions.
+// 22 us where 11 tokens had 31,104 positions.
 template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_join(SumArgs a) {
     using A = typename Acc<TW>::type;
     __shared__ A sums[JOIN_WAVES * 64 * VEC];
@@ -491,6 +492,89 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
     put_row<A, TW, VEC>(dw + (int64_t)v * C + c, acc, scale);
 }
 
+// -- small tables ------------------------------------------------------------------------------------------------------
+
+// A table of few rows has all its sums in shared memory, a set for each wave: rows of dy come in their order, TALLY of them
+// under way, and go to their tokens' sums. A workgroup has a chunk of the positions, its waves a part of it each, and 64 vectors
+// of the columns. Its sums together are its part of the gradient.
+//
+// 31,104 positions of 11 x 512 bf16 take 14 us with the join, where sorting and summing take 27 (32 MB, 6.7 us of them); with
+// 65,536 x 2,048 55 us and 64 (4.9 TB/s). From 17 rows on, four waves' sums fill the memory: 32 rows take 20 us and 26 in the
+// first case, 83 and 65 in the second, and more rows are slower than the sort in all. The next rows' loads ahead of the
+// sums made it 75 us there, and 59 of the 55.
+constexpr int TALLY = 16;
+static bool small(int64_t N, int64_t V, int64_t C) { return N > 0 && (V <= 16 || (V <= 32 && N * C <= 1 << 25)); }
+
+struct TallyArgs {
+    Ids ids;
+    const void* dy;
+    void *part, *dw;  // part: [chunks][V][C]
+    int N, C, per, chunks;  // per: positions of a wave
+    double scale;
+};
+
+template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(1024) void k_tally(TallyArgs a) {
+    using A = typename Acc<TW>::type;
+    using Raw = typename Words<VEC * (int)sizeof(TY)>::type;
+    constexpr int WIDTH = 64 * VEC;
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, V = a.ids.V, all = V * WIDTH;
+    A* sums = reinterpret_cast<A*>(shared);
+    A* mine = sums + wave * all + lane * VEC;
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) mine[v * WIDTH + e] = 0;
+    const int c0 = (int)blockIdx.y * WIDTH, c = c0 + lane * VEC;
+    const int64_t from = ((int64_t)blockIdx.x * waves + wave) * a.per, to = from + a.per < a.N ? from + a.per : a.N;
+    const TY* dy = reinterpret_cast<const TY*>(a.dy) + (c < a.C ? c : 0);
+    for (int64_t base = from; base < to; base += 64) {
+        const uint32_t k = base + lane < to ? token(a.ids, base + lane) : (uint32_t)V;
+        const int have = to - base < 64 ? (int)(to - base) : 64;
+        for (int i = 0; i < have; i += TALLY) {
+            Raw row[TALLY];
+#pragma unroll
+            for (int j = 0; j < TALLY; ++j)  // past the last position it is that one again
+                row[j] = *reinterpret_cast<const Raw*>(dy + (base + (i + j < have ? i + j : have - 1)) * a.C);
+#pragma unroll
+            for (int j = 0; j < TALLY; ++j) {
+                if (i + j >= have) break;
+                const int v = __builtin_amdgcn_readlane((int)k, i + j);
+                if (v >= V) continue;
+                const Pack<TY, VEC> x = unpacked<TY, VEC>(row[j]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) mine[v * WIDTH + e] += (A)x.e[e];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < all; i += blockDim.x) {
+        const int v = i / WIDTH, at = c0 + i % WIDTH;
+        if (at >= a.C) continue;
+        A s = sums[i];
+        for (int w = 1; w < waves; ++w) s += sums[w * all + i];
+        if (a.chunks > 1) reinterpret_cast<A*>(a.part)[((int64_t)blockIdx.x * V + v) * a.C + at] = s;
+        else reinterpret_cast<TW*>(a.dw)[(int64_t)v * a.C + at] = (TW)(s * (A)a.scale);
+    }
+}
+
+// The chunks' parts together: 64 sums a workgroup, its waves taking the chunks in turn, and then the waves' sums in order.
+template <typename TW> __global__ __launch_bounds__(1024) void k_tally_join(TallyArgs a) {
+    using A = typename Acc<TW>::type;
+    __shared__ A sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t all = (int64_t)a.ids.V * a.C, i = (int64_t)blockIdx.x * 64 + lane;
+    const A* part = reinterpret_cast<const A*>(a.part) + i;
+    A s = 0;
+    if (i < all)
+#pragma unroll 8
+        for (int k = wave; k < a.chunks; k += 16) s += part[k * all];
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || i >= all) return;
+    for (int w = 1; w < 16; ++w) s += sums[w][lane];
+    reinterpret_cast<TW*>(a.dw)[i] = (TW)(s * (A)a.scale);
+}
+
 // -- launches ----------------------------------------------------------------------------------------------------------
 
 static bool types_ok(int wt, int yt) {
@@ -542,6 +626,18 @@ struct Plan {
 };
 
 static bool few(int64_t N, int64_t V) { return N > 0 && N <= FEW && V <= FEW_ROWS; }
+
+// Of k_tally: waves whose sums fill 64 KiB, and chunks for two workgroups on each compute unit, of at least TALLY positions a
+// wave.
+struct Tally {
+    int waves = 16, per, chunks;
+    Tally(int64_t N, int64_t V, int64_t C) {
+        while (waves > 1 && waves * V * 512 > 65536) waves /= 2;
+        const int64_t tiles = (C + 127) / 128, each = (N * tiles + 512 * waves - 1) / (512 * waves);
+        per = (int)((each + TALLY - 1) / TALLY * TALLY);
+        chunks = (int)((N + (int64_t)waves * per - 1) / ((int64_t)waves * per));
+    }
+};
 
 // Lanes of a row of C / vec vectors: the next power of two, at most a wave.
 static int team_of(int C, int vec) {
@@ -599,6 +695,7 @@ int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int
 
 int64_t ebr_block_embed_bwd_scratch(int wdtype, int64_t N, int64_t V, int C) {
     if (check(wdtype, wdtype, N, V, C)) return -1;
+    if (small(N, V, C)) return Tally(N, V, C).chunks * V * C * (wdtype == EBR_DTYPE_F64 ? 8 : 4);
     const Plan p(N, V, C);
     return p.words * 4 + p.part * (wdtype == EBR_DTYPE_F64 ? 8 : 4);
 }
@@ -623,6 +720,25 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
             };
             if (C % VEC == 0 && aligned(dy, 16) && aligned(dw, 16)) go(std::integral_constant<int, VEC>());
             else go(std::integral_constant<int, 1>());
+            return launched();
+        });
+    if (small(N, V, C))
+        return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
+            using TW = decltype(tw);
+            using TY = decltype(ty);
+            constexpr int VEC = sizeof(TY) == 8 ? 1 : 2;
+            const Tally p(N, V, C);
+            const TallyArgs a = {{ids, ids64 != 0, (int)V}, dy, scratch, dw, (int)N, C, p.per, p.chunks, scale};
+            const auto go = [&](auto vec) {
+                constexpr int VN = decltype(vec)::value;
+                using A = typename Acc<TW>::type;
+                hipLaunchKernelGGL((k_tally<TW, TY, VN>), dim3(p.chunks, (C + 64 * VN - 1) / (64 * VN)), dim3(64 * p.waves),
+                                   (size_t)p.waves * V * 64 * VN * sizeof(A), s, a);
+            };
+            if (C % VEC == 0 && aligned(dy, VEC * sizeof(TY))) go(std::integral_constant<int, VEC>());
+            else go(std::integral_constant<int, 1>());
+            if (p.chunks > 1)
+                hipLaunchKernelGGL((k_tally_join<TW>), dim3((unsigned)((V * C + 63) / 64)), dim3(1024), 0, s, a);
             return launched();
         });
     const Plan p(N, V, C);

@@ -87,13 +87,27 @@ def test_embedding_of_few_tokens(cuda, wt, yt, N, V, C):
     _check_embed(ids.int() if C % 2 else ids, torch.randn(V, C, generator=g, device=cuda).to(wt), 2.5, yt)
 
 
-# as below, with more tokens than go without a sort
+# the largest tables whose sums a workgroup holds, with one chunk and many, and the first that do not fit
+@pytest.mark.parametrize("N,V,C", [(257, 16, 130), (700, 17, 64), (5000, 32, 129), (31104, 11, 512), (20000, 32, 1679), (20000, 32, 1677),
+                                   (70001, 2, 3), (300, 33, 8), (1025, 1, 66), (300000, 40, 16)])  # fmt: skip
+@pytest.mark.parametrize("wt,yt", [PAIRS[0], PAIRS[2], PAIRS[4], PAIRS[5]])
+def test_embedding_of_small_tables(cuda, wt, yt, N, V, C):
+    _say(f"embedding of a small table {N} {V} {C} {wt} {yt}")
+    g = torch.Generator(cuda).manual_seed(N)
+    ids = (torch.rand(N, generator=g, device=cuda) ** 3 * V).long()
+    ids[N // 3 :: 11] = -1
+    ids[-1] = V - 1
+    _check_embed(ids, torch.randn(V, C, generator=g, device=cuda).to(wt), 0.75, yt)
+
+
+# as below, with more tokens than go without a sort, of a small table and of one whose positions are sorted
+@pytest.mark.parametrize("V", [7, 40])
 @pytest.mark.parametrize("ids", [
     [-1] * 290, [3] * 900, [0, 2**32 + 3, 2**40, -(2**32) + 1, 6] * 60, list(range(7)) * 50 + [7], [5] * 264 + [6] * 64, [5] * 63 + [6] * 630,
 ])  # fmt: skip
-def test_embedding_of_special_tokens_sorted(cuda, ids):
-    _say(f"embedding of {len(ids)} {ids[:5]}..")
-    w = torch.randn(7, 16, generator=torch.Generator(cuda).manual_seed(1), device=cuda)
+def test_embedding_of_special_tokens_sorted(cuda, ids, V):
+    _say(f"embedding of {len(ids)} {ids[:5]}.. {V}")
+    w = torch.randn(V, 16, generator=torch.Generator(cuda).manual_seed(1), device=cuda)
     _check_embed(torch.tensor(ids, device=cuda), w, 1.0, torch.float32)
 
 
