@@ -8,6 +8,7 @@
 // an order that changes from run to run, so the positions are sorted by token instead (a stable radix sort: equal tokens
 // keep their order; few tokens, and small tables, need no sort), and a sum always adds the same rows in the same order, in 32
 // bits.
+#include <initializer_list>
 #include <type_traits>
 
 #include "rowwise.hpp"
@@ -34,37 +35,46 @@ __device__ __forceinline__ uint32_t token(const Ids& ids, int64_t n) {
 
 // -- lookup ------------------------------------------------------------------------------------------------------------
 
-// A row's threads, at most a wave of them, go over its columns VEC at a time, ROWS rows side by side: a row's load waits
-// for its token's, and the next rows' fill that time. 31,104 rows of 512 bf16 from an fp32 table of 11 take 11 us (2.8 TB/s
-// of writes; the chain token, row, store is half of it), 32,768 rows of 2,048 from one of 100,003 57 us (4.1 TB/s).
-constexpr int ROWS = 4;
+// A row's threads, at most a wave of them, go over its columns VEC at a time (16 bytes of y), some rows side by side: a row's
+// load waits for its token's, and the next rows' fill that time. 31,104 rows of 512 bf16 from an fp32 table of 11 take 9.5 us
+// (3.3 TB/s of writes; the chain token, row, store is half of it), 32,768 rows of 2,048 from one of 100,003 67 us in a row of
+// calls (4 TB/s). With 8 bytes of y a thread 10.2 and 71 us; with four rows of an fp32 table side by side 9.8 and 74, with two
+// of a 16-bit one 11.4 and 51.8 where four take 10.3 and 52.5.
+template <typename TW> constexpr int rows_of() { return sizeof(TW) == 2 ? 4 : 2; }
 template <typename TW, typename TY, int VEC>
 __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int team, double scale, const TW* w, TY* y) {
     using A = typename Acc<TW>::type;
-    using Raw = typename Words<VEC * (int)sizeof(TW)>::type;
+    constexpr int ROWS = rows_of<TW>();
+    constexpr int PIECE = VEC * (int)sizeof(TW) > 16 ? 16 / (int)sizeof(TW) : VEC, PIECES = VEC / PIECE;
+    using Raw = typename Words<PIECE * (int)sizeof(TW)>::type;
     const int t = threadIdx.x & (team - 1), per = 256 / team;
     for (int64_t n0 = (int64_t)blockIdx.x * per * ROWS + threadIdx.x / team; n0 < N; n0 += (int64_t)gridDim.x * per * ROWS) {
         uint32_t v[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) v[r] = n0 + r * per < N ? token(ids, n0 + r * per) : (uint32_t)ids.V;
         for (int c = t * VEC; c < C; c += team * VEC) {
-            Raw x[ROWS];  // (of row 0 where there is none)
+            Raw x[ROWS][PIECES];  // (of row 0 where there is none)
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
-                x[r] = *reinterpret_cast<const Raw*>(w + (int64_t)(v[r] < (uint32_t)ids.V ? v[r] : 0) * C + c);
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+                    x[r][i] = *reinterpret_cast<const Raw*>(w + (int64_t)(v[r] < (uint32_t)ids.V ? v[r] : 0) * C + c + i * PIECE);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (n0 + r * per >= N) break;
-                const Pack<TW, VEC> p = unpacked<TW, VEC>(x[r]);
                 Pack<TY, VEC> o;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o.e[e] = v[r] < (uint32_t)ids.V ? (TY)((A)p.e[e] * (A)scale) : (TY)0.f;
+                for (int i = 0; i < PIECES; ++i) {
+                    const Pack<TW, PIECE> p = unpacked<TW, PIECE>(x[r][i]);
+#pragma unroll
+                    for (int e = 0; e < PIECE; ++e)
+                        o.e[i * PIECE + e] = v[r] < (uint32_t)ids.V ? (TY)((A)p.e[e] * (A)scale) : (TY)0.f;
+                }
                 stp<TY, VEC>(y + (n0 + r * per) * C + c, o);
             }
         }
     }
 }
-
 // -- positions sorted by token -----------------------------------------------------------------------------------------
 
 // A workgroup ranks a tile of 1,024 positions a round, as many rounds as leave at most 128 workgroups (each reads all the
@@ -315,7 +325,7 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
             absent[threadIdx.x] = !(lo < ends[1] && a.key[lo] == v);
         }
         __syncthreads();
-        constexpr int ZV = VEC == 1 ? 1 : 16 / (int)sizeof(TW);  // a wave's store covers whole lines
+        constexpr int ZV = VEC < 16 / (int)sizeof(TW) ? VEC : 16 / (int)sizeof(TW);  // a wave's store covers whole lines
         const TW zero[ZV] = {};
         const int per = 256 / a.team, t = threadIdx.x & (a.team - 1);
         for (int r = threadIdx.x / a.team; r < rows; r += per) {
@@ -646,6 +656,16 @@ static int team_of(int C, int vec) {
     return t;
 }
 
+// Columns that a thread takes at once: 16 bytes of TY, half of that, or one element, as C and the pointers allow.
+template <typename TY, typename F> static void by_vector(int C, std::initializer_list<const void*> ps, F f) {
+    constexpr int VEC = 16 / (int)sizeof(TY), HALF = VEC / 2;
+    bool whole = true;
+    for (const void* p : ps) whole = whole && aligned(p, 16);
+    if (whole && C % VEC == 0) return f(std::integral_constant<int, VEC>());
+    if (whole && C % HALF == 0) return f(std::integral_constant<int, HALF>());
+    f(std::integral_constant<int, 1>());
+}
+
 template <typename TW, typename TY, int VEC> static void launch_sums(hipStream_t s, SumArgs a) {
     using A = typename Acc<TW>::type;
     a.team = team_of(a.C, VEC);
@@ -657,7 +677,7 @@ template <typename TW, typename TY, int VEC> static void launch_sums(hipStream_t
     const int64_t zeros = ((int64_t)a.V + a.zero_rows - 1) / a.zero_rows;
     hipLaunchKernelGGL((k_sum<TW, TY, VEC>), dim3((unsigned)(a.sum_blocks + zeros)), dim3(256), 0, s, a);
     if (a.chunks > 1) {
-        constexpr int JV = VEC == 1 ? 1 : 16 / (int)sizeof(A);
+        constexpr int JV = VEC < 16 / (int)sizeof(A) ? VEC : 16 / (int)sizeof(A);
         a.team = team_of(a.C, JV);
         const int64_t tiles = (a.C + a.team * JV - 1) / (a.team * JV);
         hipLaunchKernelGGL((k_join<TW, JV>), dim3(a.chunks - 1, (unsigned)tiles), dim3(64 * JOIN_WAVES), 0, s, a);
@@ -680,15 +700,13 @@ int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int
     return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
         using TW = decltype(tw);
         using TY = decltype(ty);
-        constexpr int VEC = 16 / (int)sizeof(TW);
         const auto go = [&](auto vec) {
             constexpr int VN = decltype(vec)::value;
             const int team = team_of(C, VN);
-            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, ROWS * (256 / team))), dim3(256), 0, (hipStream_t)stream, i,
+            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, rows_of<TW>() * (256 / team))), dim3(256), 0, (hipStream_t)stream, i,
                                N, C, team, scale, (const TW*)w, (TY*)y);
         };
-        if (C % VEC == 0 && aligned(w, 16) && aligned(y, 16)) go(std::integral_constant<int, VEC>());
-        else go(std::integral_constant<int, 1>());
+        by_vector<TY>(C, {w, y}, go);
         return launched();
     });
 }
@@ -712,14 +730,12 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
         return by_types(wdtype, ydtype, [&](auto tw, auto ty) {
             using TW = decltype(tw);
             using TY = decltype(ty);
-            constexpr int VEC = 16 / (int)sizeof(TY);
             const auto go = [&](auto vec) {
                 constexpr int VN = decltype(vec)::value;
                 hipLaunchKernelGGL((k_few<TW, TY, VN>), dim3((unsigned)V, (C + 64 * VN - 1) / (64 * VN)), dim3(256), 0, s,
                                    Ids{ids, ids64 != 0, (int)V}, (int)N, C, scale, (const TY*)dy, (TW*)dw);
             };
-            if (C % VEC == 0 && aligned(dy, 16) && aligned(dw, 16)) go(std::integral_constant<int, VEC>());
-            else go(std::integral_constant<int, 1>());
+            by_vector<TY>(C, {dy, dw}, go);
             return launched();
         });
     if (small(N, V, C))
@@ -764,9 +780,7 @@ int ebr_block_embed_bwd(int wdtype, int ydtype, int ids64, int64_t N, int64_t V,
         using TY = decltype(ty);
         SumArgs a = {swapped ? k1 : k0, swapped ? p1 : p0, dy, dw, w32 + p.words, (int)N, (int)V, C, p.chunk, p.chunks,
                      0, 0, 0, scale};
-        constexpr int VEC = 16 / (int)sizeof(TY);
-        if (C % VEC == 0 && aligned(dy, 16) && aligned(dw, 16)) launch_sums<TW, TY, VEC>(s, a);
-        else launch_sums<TW, TY, 1>(s, a);
+        by_vector<TY>(C, {dy, dw}, [&](auto vec) { launch_sums<TW, TY, decltype(vec)::value>(s, a); });
         return launched();
     });
 }

@@ -87,6 +87,16 @@ def test_embedding_of_few_tokens(cuda, wt, yt, N, V, C):
     _check_embed(ids.int() if C % 2 else ids, torch.randn(V, C, generator=g, device=cuda).to(wt), 2.5, yt)
 
 
+# columns that take half a vector each, or a quarter: few tokens, sorted ones in one workgroup and in many
+@pytest.mark.parametrize("N,V,C", [(200, 9, 12), (200, 9, 6), (300, 40, 12), (300, 40, 10), (5000, 700, 1500), (5000, 700, 6)])
+@pytest.mark.parametrize("wt,yt", PAIRS)
+def test_embedding_of_half_vectors(cuda, wt, yt, N, V, C):
+    _say(f"embedding of half vectors {N} {V} {C} {wt} {yt}")
+    g = torch.Generator(cuda).manual_seed(N + C)
+    ids = (torch.rand(N, generator=g, device=cuda) ** 3 * (V + 1)).long()
+    _check_embed(ids, torch.randn(V, C, generator=g, device=cuda).to(wt), 1.5, yt)
+
+
 # the largest tables whose sums a workgroup holds, with one chunk and many, and the first that do not fit
 @pytest.mark.parametrize("N,V,C", [(257, 16, 130), (700, 17, 64), (5000, 32, 129), (31104, 11, 512), (20000, 32, 1679), (20000, 32, 1677),
                                    (70001, 2, 3), (300, 33, 8), (1025, 1, 66), (300000, 40, 16)])  # fmt: skip
