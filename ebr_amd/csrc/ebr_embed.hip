@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int t
 // A workgroup ranks a tile of 1,024 positions a round, as many rounds as leave at most 128 workgroups (each reads all the
 // others' counts); up to 4,096 positions are one workgroup's. A tile of 4,096 left most of the card idle: 16,384 positions
 // took 9.9 us a pass, 5.4 in tiles of 1,024 (and 2.9 the counts before it). Latency bounds it: launches, and what one kernel
-// wrote and the next reads on other XCDs. Nine bits a pass: one for boards, two up to a vocabulary of 262,143.
+// wrote and the next reads on other XCDs. Nine bits a pass: one up to a vocabulary of 511, two up to 262,143.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ONE = 4096;
 constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS;
 constexpr int SORT_GROUPS = 128;

@@ -1374,7 +1374,7 @@ py::object embedding(const py::handle& hids, const py::handle& hw, double scale,
 
 // Rows of V columns with unit stride, and the stride from one to the next.
 Tensor logit_rows(const Tensor& logits, int64_t* stride) {
-    Tensor x = logits.reshape({-1, logits.size(-1)});
+    Tensor x = logits.dim() == 2 ? logits : logits.reshape({-1, logits.size(-1)});
     if ((x.size(1) > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < x.size(1))) x = x.contiguous();
     *stride = std::max(x.stride(0), x.size(1));
     return x;
@@ -1392,16 +1392,17 @@ struct Distill : Function<Distill> {
         const auto acc = x.options().dtype(acc_type(x));
         const bool none = reduction == EBR_REDUCE_NONE;
         const Tensor loss = at::empty(none ? logits.sizes().slice(0, logits.dim() - 1) : at::IntArrayRef(), acc);
-        const Tensor stats = at::empty({N, 4}, acc), scale = none ? Tensor() : at::empty({1}, acc);
-        const int64_t n = ebr_block_distill_scratch(code, N, V, (int)K);
+        const int64_t n = ebr_block_distill_scratch(code, N, V, (int)K), es = loss.element_size();
         TORCH_CHECK_VALUE(n >= 0, "ebr_block_distill: sizes out of range");
-        const Tensor s = at::empty({n}, x.options().dtype(at::kByte));
+        const Tensor kept = at::empty({4 * N + 4 + n / es}, acc);  // stats [N, 4], scale (in 4), scratch (16 bytes' multiple)
+        char* at = static_cast<char*>(kept.data_ptr());
         check(ebr_block_distill(code, dtype_code(teacher.scalar_type()), wide(ids), N, V, (int)K, row, temperature,
-                                (int)reduction, x.data_ptr(), teacher.data_ptr(), ids.data_ptr(), stats.data_ptr(),
-                                loss.data_ptr(), vptr(scale), s.data_ptr(), stream_of(x)),
+                                (int)reduction, x.data_ptr(), teacher.data_ptr(), ids.data_ptr(), at, loss.data_ptr(),
+                                none ? nullptr : at + 4 * N * es, at + (4 * N + 4) * es, stream_of(x)),
               "ebr_block_distill");
-        ctx->save_for_backward({logits, teacher_, ids_, stats, scale});
+        ctx->save_for_backward({logits, teacher_, ids_, kept});
         ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["none"] = none;
         ctx->set_materialize_grads(false);
         return {loss};
     }
@@ -1409,20 +1410,23 @@ struct Distill : Function<Distill> {
         variable_list out(5);
         if (!g[0].defined()) return out;
         const variable_list sv = ctx->get_saved_variables();
-        const Tensor &logits = sv[0], &stats = sv[3], &scale = sv[4];
+        const Tensor &logits = sv[0], &kept = sv[3];
         const double temperature = ctx->saved_data["temperature"].toDouble();
+        const bool none = ctx->saved_data["none"].toBool();
+        const int64_t N = logits.numel() / logits.size(-1);
         if (!native(g))
-            return python_grads("distill", 5, logits, sv[1], sv[2], stats,
-                                scale.defined() ? scale : at::empty({0}, stats.options()), temperature, g[0]);
+            return python_grads("distill", 5, logits, sv[1], sv[2], kept.narrow(0, 0, 4 * N).view({N, 4}),
+                                kept.narrow(0, 4 * N, none ? 0 : 1), temperature, g[0]);
         RECORD_FUNCTION("ebr_fused::distill_bwd", std::vector<c10::IValue>());
         const c10::DeviceGuard on(logits.device());
         int64_t row;
         const Tensor x = logit_rows(logits, &row), teacher = dense(sv[1]), ids = dense(sv[2]);
-        const Tensor grad = dense(g[0].to(stats.scalar_type())), dx = at::empty(logits.sizes(), logits.options());
-        check(ebr_block_distill_bwd(dtype_code(x.scalar_type()), dtype_code(teacher.scalar_type()), wide(ids), x.size(0),
-                                    x.size(1), (int)teacher.size(-1), row, temperature, x.data_ptr(), teacher.data_ptr(),
-                                    ids.data_ptr(), stats.data_ptr(), vptr(scale), grad.data_ptr(), !scale.defined(),
-                                    dx.data_ptr(), stream_of(x)),
+        const Tensor grad = dense(g[0].to(kept.scalar_type())), dx = at::empty(logits.sizes(), logits.options());
+        const char* at = static_cast<const char*>(kept.data_ptr());
+        check(ebr_block_distill_bwd(dtype_code(x.scalar_type()), dtype_code(teacher.scalar_type()), wide(ids), N, x.size(1),
+                                    (int)teacher.size(-1), row, temperature, x.data_ptr(), teacher.data_ptr(),
+                                    ids.data_ptr(), at, none ? nullptr : at + 4 * N * kept.element_size(), grad.data_ptr(),
+                                    none, dx.data_ptr(), stream_of(x)),
               "ebr_block_distill_bwd");
         out[0] = dx;
         if (recorded({logits, g[0]})) out[0] = last({dx})[0];
