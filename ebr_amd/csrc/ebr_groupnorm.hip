@@ -47,6 +47,7 @@ struct Args {
     int tile;               // channels of a workgroup that holds whole groups
     int64_t rows;           // of a part
     double eps;
+    double inv;  // 1 / (L cg)
 };
 
 __device__ __forceinline__ float pow_e(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896f); }
@@ -583,7 +584,6 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
     const int c = on ? c0 + at : c0, g = c / a.cg, gcols = a.cg / VEC, gfrom = (c - c0) / a.cg * gcols;
     const int L = (int)a.L;
     const int64_t base = n * a.L * a.C + c;
-    const double m = (double)a.L * a.cg;
 
     // no load depends on the thread: one without channels reads the tile's first, and a cell past the end is the last
     Raw x[R], dy[MODE >= 1 ? R : 1], u[MODE == 2 ? R : 1];
@@ -633,7 +633,7 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
         for (int k = 0; k < K; ++k) {
             double v = 0;
             for (int i = 0; i < gcols; ++i) v += (double)cols[k * a.tx + gfrom + i];
-            out[k] = v / m;
+            out[k] = v * a.inv;
         }
     };
     // the sample's share of the parameters' gradients
@@ -971,6 +971,7 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
     a.means = at + sc.part;
     a.chan = MODE != 0 && (a.dw || a.db) ? at + sc.part + sc.means : nullptr;
     a.cg = a.C / a.G;
+    a.inv = 1.0 / ((double)a.L * a.cg);
     a.tx = p.tx;
     a.tiles = p.tiles;
     a.splits = p.splits;
