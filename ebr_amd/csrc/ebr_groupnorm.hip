@@ -17,8 +17,8 @@
 // are about the mean, or of eight cells at a time about theirs, which go together by the rule for the variance of a union.
 //
 // Bound by memory as far as the arithmetic (some 20, 30 and 75 operations an element) leaves it. 768 boards of 81 x 512 bf16
-// (64 MB a tensor), groups of 16 channels: 30 us (4.2 TB/s), 42 (4.6), 94 (3.4) for the norm, its gradient and the second
-// derivative; 64 boards of 900 x 512: 36 and 56 us. Two grids of 128 x 128 x 320 fp32 (42 MB a tensor, read twice, the
+// (64 MB a tensor), groups of 16 channels: 28 us (4.5 TB/s), 41 (4.6), 87 (3.7) for the norm, its gradient and the second
+// derivative; 64 boards of 900 x 512: 34 and 55 us. Two grids of 128 x 128 x 320 fp32 (42 MB a tensor, read twice, the
 // second time from the last-level cache): 35, 48 and 79 us in three launches each.
 #include <type_traits>
 
@@ -613,7 +613,9 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
             if constexpr (MODE == 2) opaque(u[i]);
         }
     };
-    // p's means over this thread's group: over the wave's threads of the same channels, over the waves, over the channels
+    // p's means over this thread's group: over the wave's threads of the same channels, over the waves, over the channels. The
+    // sums stay in 32 bits, as the cells' are, and only the mean is taken in 64, by a product: with divisions, and the channels
+    // added in 64 bits, the three orders of 768 boards of 81 x 512 bf16 took 31, 43 and 95 us, 28, 41 and 87 so.
     const auto means = [&](auto& p, double* out) {
         constexpr int K = sizeof(p) / sizeof(p[0]);
         for (int d = a.tx; d < 64; d <<= 1)
@@ -631,9 +633,9 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            double v = 0;
-            for (int i = 0; i < gcols; ++i) v += (double)cols[k * a.tx + gfrom + i];
-            out[k] = v * a.inv;
+            A v = 0;
+            for (int i = 0; i < gcols; ++i) v += cols[k * a.tx + gfrom + i];
+            out[k] = (double)v * a.inv;
         }
     };
     // the sample's share of the parameters' gradients
@@ -716,7 +718,7 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
     } else {
         // The gradient of up to four cells keeps da, and its second half has neither dy nor the activation to take again: which
         // is as long as the memory traffic otherwise (50 us for 768 boards of 81 x 512 bf16, 42 so). In the second derivative the
-        // same made no difference.
+        // sigmoids kept took 85 us where it takes 87, in 116 registers.
         constexpr bool KEEP = MODE == 1 && ACT != 0 && R <= 4;
         A kept[KEEP ? R : 1][KEEP ? VEC : 1];
         A s[NS][VEC] = {};
@@ -897,7 +899,7 @@ struct Scratch {
 //
 // The vector is 16 bytes, but 2 channels of 16 bits in the second derivative, whose ten sums a channel and three tensors
 // fill the registers: 768 boards of 81 x 512 bf16 took 113 us at 8 channels (three waves a SIMD), 102 at 4 (four), 94 at 2
-// (five). Of groups too wide for that, 4.
+// (five), all with divisions in the means. Of groups too wide for that, 4.
 struct Whole {
     int waves = 0, cells = 0, vec = 0, tx = 0, tile = 0, tiles = 0;
     // the two numbers of cells that there are kernels for
