@@ -393,13 +393,18 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
             for (int p = ts; p < a.splits; p += lanes)
 #pragma unroll
                 for (int i = 0; i < NS; ++i) s[i] += (double)part[((int64_t)p * NS + i) * a.C + c0 + c];
-        if (lanes == 1) return;
-        __syncthreads();
+        for (int d = cols; d < 64; d <<= 1)
 #pragma unroll
-        for (int i = 0; i < NS; ++i) tot[i][threadIdx.x] = s[i];
+            for (int i = 0; i < NS; ++i) s[i] += __shfl_xor(s[i], d, 64);
+        const int wide = cols < 64 ? 64 : cols;  // threads that hold the same sums, or parts of others
+        if (wide == (int)blockDim.x) return;
+        __syncthreads();
+        if ((int)threadIdx.x % wide < cols)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) tot[i][threadIdx.x / wide * cols + tc] = s[i];
         __syncthreads();
         if (ts == 0)
-            for (int l = 1; l < lanes; ++l)
+            for (int l = 1; l < (int)blockDim.x / wide; ++l)
 #pragma unroll
                 for (int i = 0; i < NS; ++i) s[i] += tot[i][l * cols + tc];
     };
