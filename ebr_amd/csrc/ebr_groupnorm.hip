@@ -358,7 +358,7 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
     __shared__ double tot[NS][THREADS];
     const int64_t n = blockIdx.x / a.G;
     const int g = (int)(blockIdx.x % a.G), c0 = g * a.cg;
-    const double m = (double)a.L * a.cg;
+    const double inv = a.inv;
     int cols = 1;
     while (cols < a.cg && cols < (int)blockDim.x) cols *= 2;
     const int tc = threadIdx.x % cols, ts = threadIdx.x / cols, lanes = (int)blockDim.x / cols;
@@ -377,7 +377,7 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
                 v[1] += (double)part[((int64_t)s * 2 + 1) * a.C + c0 + c] + cells(s) * d * d;
             }
         all_sums<2>(v, lds);
-        const double mu = about + v[0] / m, var = v[1] / m - (v[0] / m) * (v[0] / m);
+        const double off = v[0] * inv, mu = about + off, var = v[1] * inv - off * off;
         if (threadIdx.x == 0) {
             stats[0] = (A)mu;
             stats[1] = (A)(1.0 / sqrt((var > 0 ? var : var == var ? 0.0 : var) + a.eps));
@@ -427,8 +427,8 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
         }
         all_sums<2>(k, lds);
         if (threadIdx.x == 0) {
-            out[0] = (A)(k[0] / m);
-            out[1] = (A)(k[1] / m);
+            out[0] = (A)(k[0] * inv);
+            out[1] = (A)(k[1] * inv);
         }
     }
     if constexpr (MODE == 2) {
@@ -446,7 +446,7 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
             k[4] += w * s[4];
         }
         all_sums<5>(k, lds);
-        const double u1 = k[0] / m, u2 = k[1] / m, k1 = k[2] / m, k2 = k[3] / m, ku = k[4] / m;
+        const double u1 = k[0] * inv, u2 = k[1] * inv, k1 = k[2] * inv, k2 = k[3] * inv, ku = k[4] * inv;
         double v[2] = {0, 0};
         for (int i = 0; i < rounds; ++i) {
             const int c = tc + i * cols;
@@ -466,8 +466,8 @@ template <typename A, int MODE, int ACT> __global__ __launch_bounds__(THREADS) v
             out[0] = (A)u1;
             out[1] = (A)u2;
             out[2] = (A)k2;
-            out[3] = (A)(v[0] / m - r * (u1 * k2 + k1 * u2));
-            out[4] = (A)(v[1] / m - 2.0 * r * u2 * k2);
+            out[3] = (A)(v[0] * inv - r * (u1 * k2 + k1 * u2));
+            out[4] = (A)(v[1] * inv - 2.0 * r * u2 * k2);
             out[5] = (A)(ku - k1 * u1 - u2 * k2);
         }
     }
