@@ -459,10 +459,11 @@ static int team_of(int dtype, int64_t V, int K) {
 }
 
 // Parts of a row: where rows of a workgroup each leave compute units without any, as many as give each of the 256 about
-// four, with at least 4,096 columns (a round of loads) and at most 64 parts.
+// four, with at least 4,096 columns (a round of loads) and at most 64 parts. An empty batch has no parts: nothing is launched
+// for its rows.
 static int splits_of(int64_t N, int64_t V) {
-    if (V <= 2048 || N >= 512) return 1;
-    int64_t s = 1024 / (N > 0 ? N : 1);
+    if (V <= 2048 || N < 1 || N >= 512) return 1;
+    int64_t s = 1024 / N;
     if (s > V / 4096) s = V / 4096;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }

@@ -404,6 +404,19 @@ def test_distill_gradients_by_differences(cuda):
         dx.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [8191, 8192, 50021, 300000])
+def test_distill_of_no_rows_of_a_long_vocabulary(cuda, dtype, V):
+    """Few long rows are split into parts; no rows have none: the sum and the mean are 0, the gradient is empty."""
+    _say(f"distill no rows {V} {dtype}")
+    t, ids = torch.zeros(0, 3, 4, device=cuda), torch.zeros(0, 3, 4, dtype=torch.int64, device=cuda)
+    for reduction, want in (("mean", ()), ("sum", ()), ("none", (0, 3))):
+        x = torch.zeros(0, 3, V, device=cuda, dtype=dtype, requires_grad=True)
+        loss = tokens.distill_loss(x, t, ids, 2.0, reduction)
+        assert loss.shape == want and bool((loss == 0).all())
+        assert torch.autograd.grad(loss.sum(), x)[0].shape == x.shape
+
+
 # -- streams and graphs ------------------------------------------------------------------------------------------------
 
 
