@@ -340,7 +340,7 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
     const int chunk = (int)(item / tiles), c = (int)(item % tiles) * per + (threadIdx.x & (a.team - 1)) * VEC;
     if (c >= a.C) return;
     const uint32_t V = (uint32_t)a.V;
-    const int from = chunk * a.chunk, to = from + a.chunk < a.N ? from + a.chunk : a.N;
+    const int from = chunk * a.chunk, to = a.N - from > a.chunk ? from + a.chunk : a.N;  // (from + chunk may pass 32 bits)
     const TY* dy = reinterpret_cast<const TY*>(a.dy) + c;
     A* part = reinterpret_cast<A*>(a.part) + (int64_t)chunk * 2 * a.C + c;
     const uint32_t before = from > 0 ? a.key[from - 1] : V, after = to < a.N ? a.key[to] : V;

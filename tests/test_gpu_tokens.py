@@ -187,6 +187,24 @@ def test_embedding_repeats_its_bits_and_differentiates_again(cuda):
     assert torch.equal(back, torch.where((few >= 0)[:, None], c[few.clamp(min=0)], torch.zeros_like(back)))
 
 
+def test_embedding_gradient_of_the_most_positions(cuda):
+    """The most tokens that a call takes, sorted: the last chunk's end passes 32 bits. Ones are counted: whole numbers below
+    2^24 exactly, the others by at most 8,192 additions of parts (2^-24 each)."""
+    _say("embedding of 2^31 - 4097 tokens")
+    N, V = 2**31 - 4097, 40
+    ids = torch.full((N,), 3, dtype=torch.int32, device=cuda)
+    ids[::7159] = V - 1
+    w = torch.randn(V, 1, generator=torch.Generator(cuda).manual_seed(1), device=cuda, requires_grad=True)
+    y = tokens.embedding(ids, w, dtype=torch.bfloat16)
+    last = -(-N // 7159)
+    assert y[7159 * (last - 1)] == w[V - 1].bfloat16() and y[N - 1] == w[3 if (N - 1) % 7159 else V - 1].bfloat16()
+    (dw,) = torch.autograd.grad(y, w, torch.ones(1, 1, device=cuda, dtype=torch.bfloat16).expand(N, 1))
+    assert dw[V - 1].item() == last
+    assert abs(dw[3].item() - (N - last)) <= 8192 * 2.0**-24 * N
+    dw[3], dw[V - 1] = 0, 0
+    assert bool((dw == 0).all())
+
+
 # -- distillation ------------------------------------------------------------------------------------------------------
 
 
