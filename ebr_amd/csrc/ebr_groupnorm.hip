@@ -79,7 +79,7 @@ template <typename A> struct Spread {
         if (all == (A)0) return;
         const A d = omean - mean, f = on / all;
         mean += d * f;
-        m2 += om2 + d * d * n * f;
+        m2 += om2 + d * (d * (n * f));  // n f is 0 where a side has nothing: d is the other's mean, its square perhaps infinite
         n = all;
     }
 };

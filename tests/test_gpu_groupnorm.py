@@ -192,6 +192,26 @@ def test_constant_groups_and_extremes(cuda):
         assert torch.equal(y, good)
 
 
+# read twice: threads and lanes without cells, one part and many, one channel a thread and vectors
+@pytest.mark.parametrize("shape,G", [((1, 3000, 12), 4), ((2, 9, 7), 7), ((3, 40, 9), 1), ((1, 5000, 512), 16), ((2, 4100, 16), 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_groups_of_one_large_value(cuda, dtype, shape, G):
+    """A group of one value has h = 0 whatever the value, whose square need not be a number of 32 bits; and cells around 1e20
+    with deviation 1e16: x loses 10^4 u against it, and h as in ``test_far_from_zero``."""
+    _say(f"group_norm large {shape} {dtype}")
+    b = torch.linspace(-1, 1, shape[-1], device=cuda)
+    for value in (1e20, torch.finfo(dtype).max, torch.finfo(dtype).min):
+        x = torch.full(shape, value, device=cuda, dtype=dtype).requires_grad_(True)
+        y = block.group_norm(x, G, None, b)
+        assert torch.equal(y, b.to(dtype).expand(shape)), value
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert bool(torch.isfinite(dx).all()), value
+    if dtype == torch.float32 and shape[1] * shape[2] // G > 1000:
+        x = 1e20 * (1 + 1e-4 * torch.randn(shape, generator=torch.Generator(cuda).manual_seed(1), device=cuda))
+        ref = _plain(x.double(), G, None, None, None)
+        assert float((block.group_norm(x, G, eps=EPS) - ref).abs().max()) <= 3 * 1e4 * 2.0**-24 * float(ref.abs().max())
+
+
 def test_views_and_empty_calls(cuda):
     _say("group_norm views")
     ts = _inputs(cuda, (4, 12, 48), torch.bfloat16, seed=3)
