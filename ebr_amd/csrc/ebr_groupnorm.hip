@@ -47,7 +47,8 @@ struct Args {
     int tile;               // channels of a workgroup that holds whole groups
     int64_t rows;           // of a part
     double eps;
-    double inv;  // 1 / (L cg)
+    double inv;          // 1 / (L cg)
+    double unit, units;  // the power of two that is 1 / (L cg) or the next below, and 1 / unit
 };
 
 __device__ __forceinline__ float pow_e(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896f); }
@@ -673,6 +674,8 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
     };
 
     if constexpr (MODE == 0) {
+        // in units in which the sum of the largest values does not overflow; a power of two: nothing else changes
+        const A unit = (A)a.unit;
         double v[1], v2[2];
         A p[1] = {0}, p2[2] = {0, 0};
 #pragma unroll
@@ -680,12 +683,13 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
             if (on && ty + i * step < L) {
                 const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) p[0] += (A)xv.e[e];
+                for (int e = 0; e < VEC; ++e) p[0] += (A)xv.e[e] * unit;
             }
         pack_again();
         means(p, v);
-        // about that mean, which the sum's rounding has left a little off: the mean of what is left makes it up
-        mu = (A)v[0];
+        // about that mean, which the sum's rounding has left a little off (and may have left past the largest value): the mean
+        // of what is left makes it up
+        mu = (A)fmin(fmax(v[0] * a.units, -(double)__FLT_MAX__), (double)__FLT_MAX__);
 #pragma unroll
         for (int i = 0; i < R; ++i)
             if (on && ty + i * step < L) {
@@ -979,6 +983,9 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
     a.chan = MODE != 0 && (a.dw || a.db) ? at + sc.part + sc.means : nullptr;
     a.cg = a.C / a.G;
     a.inv = 1.0 / ((double)a.L * a.cg);
+    a.units = 1.0;
+    while (a.units < (double)a.L * a.cg) a.units *= 2;
+    a.unit = 1.0 / a.units;
     a.tx = p.tx;
     a.tiles = p.tiles;
     a.splits = p.splits;

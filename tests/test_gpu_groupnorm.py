@@ -212,6 +212,22 @@ def test_long_groups_of_one_large_value(cuda, dtype, shape, G):
         assert float((block.group_norm(x, G, eps=EPS) - ref).abs().max()) <= 3 * 1e4 * 2.0**-24 * float(ref.abs().max())
 
 
+# a thread with few cells and many, one wave a SIMD's share and 16 waves, a tile of several groups and one of all channels
+@pytest.mark.parametrize("shape,G", [((2, 20, 32), 4), ((1, 900, 512), 16), ((2, 256, 64), 2), ((2, 5, 512), 1), ((1, 1024, 64), 8)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_held_groups_of_one_large_value(cuda, dtype, shape, G):
+    """As ``test_long_groups_of_one_large_value`` where a workgroup holds the group: its elements' sum need not be a number of
+    32 bits either."""
+    _say(f"group_norm held large {shape} {dtype}")
+    b = torch.linspace(-1, 1, shape[-1], device=cuda)
+    for value in (1e20, 1e36, torch.finfo(dtype).max, torch.finfo(dtype).min):
+        x = torch.full(shape, value, device=cuda, dtype=dtype).requires_grad_(True)
+        y = block.group_norm(x, G, None, b)
+        assert torch.equal(y, b.to(dtype).expand(shape)), value
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert bool(torch.isfinite(dx).all()), value
+
+
 def test_views_and_empty_calls(cuda):
     _say("group_norm views")
     ts = _inputs(cuda, (4, 12, 48), torch.bfloat16, seed=3)
