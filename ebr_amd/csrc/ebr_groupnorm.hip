@@ -831,7 +831,7 @@ static int check(int dtype, int64_t B, int64_t L, int C, int groups, int act) {
     if (dtype != EBR_DTYPE_F32 && dtype != EBR_DTYPE_BF16 && dtype != EBR_DTYPE_F16 && dtype != EBR_DTYPE_F64)
         return EBR_ERR_DTYPE;
     if (B < 1 || L < 1 || C < 1 || C > (1 << 20) || groups < 1 || C % groups || B >= ((int64_t)1 << 31) ||
-        L >= ((int64_t)1 << 40) || B * L >= ((int64_t)1 << 40) || B * L * C >= ((int64_t)1 << 40) ||
+        L >= ((int64_t)1 << 40) || B > (((int64_t)1 << 40) - 1) / L || B * L * C >= ((int64_t)1 << 40) ||  // (no product wraps)
         (act != EBR_ACT_NONE && act != EBR_ACT_SILU))
         return EBR_ERR_SHAPE;
     return EBR_OK;

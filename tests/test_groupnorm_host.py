@@ -66,6 +66,11 @@ def test_scratch_sizes():
     assert lib.ebr_block_groupnorm_scratch(1, 0, 2, 81, 512, 31) == -1
 
 
+@pytest.mark.parametrize("B,L,C", [(2**30, 2**34, 1), (2**26, 2**38, 16), (2**25, 2**39, 3), (2**30, 2**33, 8)])
+def test_scratch_refuses_sizes_whose_product_passes_64_bits(B, L, C):
+    assert [_capi.load().ebr_block_groupnorm_scratch(1, order, B, L, C, 1) for order in (0, 1, 2)] == [-1, -1, -1]
+
+
 def test_eager_group_norm_is_torch_s():
     x = torch.randn(3, 6, 7, 24, generator=torch.Generator().manual_seed(0), dtype=torch.float32)
     ref = torch.nn.functional.group_norm(x.double().permute(0, 3, 1, 2), 4, eps=1e-5).permute(0, 2, 3, 1)
