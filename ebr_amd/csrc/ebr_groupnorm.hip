@@ -949,6 +949,12 @@ struct Whole {
     }
 };
 
+// The workgroups of a mode, or -1 where a launch does not hold them (or one for each group of the samples).
+static int64_t blocks_of(const Plan& p, const Whole& h, int64_t B, int groups) {
+    const int64_t n = h.waves ? B * h.tiles * (h.waves / 4) : B * p.splits * p.tiles;
+    return n > MAX_BLOCKS || (!h.waves && B * groups > MAX_BLOCKS) ? -1 : n;
+}
+
 template <typename T, int VEC, int MODE, int ACT> static void launch_vec(hipStream_t s, const Whole& h, const Args& a) {
     using A = typename Acc<T>::type;
     constexpr bool WIDE = sizeof(T) == 4;
@@ -991,8 +997,8 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
     a.splits = p.splits;
     a.rows = p.rows;
     const Whole h(MODE, dtype, a.L, a.C, a.G, vector);
-    const int64_t blocks = h.waves ? a.B * h.tiles * (h.waves / 4) : a.B * p.splits * p.tiles;
-    if (blocks > MAX_BLOCKS || (!h.waves && a.B * a.G > MAX_BLOCKS)) return EBR_ERR_SHAPE;
+    const int64_t blocks = blocks_of(p, h, a.B, a.G);
+    if (blocks < 0) return EBR_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     by_kind(dtype, vector, act, [&](auto v, auto n, auto f) {
         using T = decltype(v);
@@ -1026,9 +1032,11 @@ extern "C" {
 
 int64_t ebr_block_groupnorm_scratch(int dtype, int order, int64_t B, int64_t L, int C, int groups) {
     if (check(dtype, B, L, C, groups, 0) || order < 0 || order > 2) return -1;
-    int64_t most = 0;
-    for (const bool vector : {true, false}) {  // tensors off 16-byte alignment take another plan
+    int64_t most = -1;
+    for (const bool aligned : {true, false}) {  // tensors off 16-byte alignment take another plan
+        const bool vector = aligned && vector_of(dtype, C) > 1;
         const Plan p(dtype, B, L, C, vector);
+        if (blocks_of(p, Whole(order, dtype, L, C, groups, vector), B, groups) < 0) continue;
         const int64_t n = Scratch(p, order, B, C, groups, acc_bytes(dtype)).all();
         most = n > most ? n : most;
     }

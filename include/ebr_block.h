@@ -113,7 +113,9 @@ int ebr_block_groupnorm_bwd2(int dtype, int act, int64_t B, int64_t L, int C, in
                              const void* b, const void* stats, const void* dy, const void* u, const void* uw, const void* ub,
                              void* gx, void* gdy, void* gw, void* gb, void* scratch, void* stream);
 
-/* Bytes of scratch of the group norm (order 0) and its derivatives (1, 2), -1 for sizes or types that they refuse. */
+/* Bytes of scratch of the group norm (order 0) and its derivatives (1, 2), for tensors of any alignment; -1 for sizes or types
+ * that they refuse: more than 2^40 - 1 elements, or 2^24 - 1 workgroups or, where these do not hold whole groups, groups of
+ * all samples. */
 int64_t ebr_block_groupnorm_scratch(int dtype, int order, int64_t B, int64_t L, int C, int groups);
 
 #ifdef __cplusplus

@@ -71,6 +71,17 @@ def test_scratch_refuses_sizes_whose_product_passes_64_bits(B, L, C):
     assert [_capi.load().ebr_block_groupnorm_scratch(1, order, B, L, C, 1) for order in (0, 1, 2)] == [-1, -1, -1]
 
 
+@pytest.mark.parametrize("order", [0, 1, 2])
+@pytest.mark.parametrize("dtype,B,L,C,G,fits", [
+    (1, 2**25, 1, 8, 1, False), (1, 2**24, 1, 64, 8, False), (1, 2**24 - 1, 1, 64, 8, True),  # a workgroup for each sample
+    (0, 2**23, 2, 5, 5, False), (0, 2**21, 2, 5, 5, True),                                    # one for each group
+    # several for each sample: 5 of vectors of 2 (21 million in all), 3 of single elements (12.6), which tensors off alignment take
+    (3, 2**22, 1, 130, 1, True), (3, 2**24, 1, 130, 1, False), (3, 2**21, 1, 130, 1, True),
+])  # fmt: skip
+def test_scratch_refuses_what_a_launch_does_not_hold(dtype, B, L, C, G, fits, order):
+    assert (_capi.load().ebr_block_groupnorm_scratch(dtype, order, B, L, C, G) >= 0) == fits
+
+
 def test_eager_group_norm_is_torch_s():
     x = torch.randn(3, 6, 7, 24, generator=torch.Generator().manual_seed(0), dtype=torch.float32)
     ref = torch.nn.functional.group_norm(x.double().permute(0, 3, 1, 2), 4, eps=1e-5).permute(0, 2, 3, 1)
