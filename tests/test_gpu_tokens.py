@@ -121,8 +121,8 @@ def test_embedding_of_special_tokens_sorted(cuda, ids, V):
     _check_embed(torch.tensor(ids, device=cuda), w, 1.0, torch.float32)
 
 
-# more than one workgroup's sort (4096), one, two and three passes of 9 bits, more than 256 sort groups of a tile (2^20), and
-# chunks of more than 64 positions (2^18)
+# more than one workgroup's sort (4096), two and three passes of 9 bits, more than a tile a sort group (from 2^17 on), and chunks
+# of more than 64 positions (from 2^19 on); the tables of 5 and 11 rows are summed without a sort
 @pytest.mark.parametrize("N,V,C", [(4097, 11, 64), (20000, 50021, 40), (9000, 300001, 9), (300000, 5, 16), (1100000, 70000, 2)])
 def test_embedding_sorts(cuda, N, V, C):
     _say(f"embedding sorts {N} {V} {C}")
@@ -185,6 +185,29 @@ def test_embedding_repeats_its_bits_and_differentiates_again(cuda):
     c = torch.randn(5, 3, generator=g, device=cuda)
     (back,) = torch.autograd.grad(dw, dy, c)
     assert torch.equal(back, torch.where((few >= 0)[:, None], c[few.clamp(min=0)], torch.zeros_like(back)))
+
+
+# sorted in many workgroups (more than 4,096 positions, and more than 16 rows or, of many, 32): one pass of 9 bits and two, a
+# tile of 1,024 a workgroup and more (from 2^17 positions on), chunks of 64 positions and more (from 2^19 on), sixteen bits
+# and 32, and half and single vectors; every other position the same token, whose run goes over most chunks' borders
+@pytest.mark.parametrize("wt,yt", [PAIRS[0], PAIRS[2], PAIRS[3]])
+@pytest.mark.parametrize("N,V,C", [(4097, 33, 64), (31104, 40, 512), (140000, 600, 12), (300000, 50021, 16), (530001, 37, 8), (70001, 300, 5)])
+def test_embedding_sorts_in_many_workgroups_and_repeats_its_bits(cuda, wt, yt, N, V, C):
+    _say(f"embedding sorts, again {N} {V} {C} {wt} {yt}")
+    g = torch.Generator(cuda).manual_seed(N)
+    ids = (torch.rand(N, generator=g, device=cuda) ** 2 * V).long()
+    ids[::2] = V // 2
+    ids[::5] = -1
+    w = torch.randn(V, C, generator=g, device=cuda).to(wt).requires_grad_(True)
+    dy = torch.randn(N, C, generator=g, device=cuda).to(yt)
+    dw = [torch.autograd.grad(tokens.embedding(ids, w, 0.5, yt), w, dy)[0] for _ in range(4)]
+    assert all(torch.equal(dw[0], d) for d in dw[1:])
+    flat, d = ids.cpu(), dy.cpu().double()  # (half of the rows to one: on the GPU that takes seconds)
+    keep = flat >= 0
+    ref, size = (torch.zeros(V, C, dtype=torch.float64).index_add_(0, flat[keep], v[keep]) * 0.5 for v in (d, d.abs()))
+    n = torch.bincount(flat[keep], minlength=V)[:, None]
+    got = dw[0].cpu()
+    _near(got, ref, _half_step(got, ref) * (ref != 0) + 1.01 * U[wt] * (n + 2) * size, "dw")  # the bound of _check_embed
 
 
 def test_embedding_gradient_of_the_most_positions(cuda):
