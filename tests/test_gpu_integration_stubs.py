@@ -95,3 +95,20 @@ def test_descent_stub_matches_the_ops_exactly(cuda):
     out, rms = stub["step_and_project"](v, g, alpha, z, active, eps)
     assert torch.equal(out, descent.step_and_project(v, g, alpha, z, active, eps))
     assert rms.shape == (B,) and torch.isfinite(rms).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("N,V,K", [(7, 11, 3), (3, 20000, 40)])
+def test_distill_stub_matches_the_op_exactly(cuda, dtype, N, V, K):
+    from ebr_amd import tokens
+
+    stub = _stub("# training/distill_hip.py")
+    _say(f"distill stub {N} {V} {K} {dtype}")
+    gen = torch.Generator(device=cuda).manual_seed(9)
+    x = torch.randn(N, V, generator=gen, device=cuda).to(dtype).requires_grad_(True)
+    t, ids = torch.randn(N, K, generator=gen, device=cuda), torch.randint(0, V, (N, K), generator=gen, device=cuda)
+    ref = tokens.distill_loss(x, t, ids, temperature=2.0)
+    loss, stats, scale = stub["distill"](x.detach(), t, ids, 2.0)
+    assert torch.equal(loss, ref.detach()) and stats.dtype == scale.dtype == loss.dtype == ref.dtype
+    grad = torch.full_like(loss, 0.7)
+    assert torch.equal(stub["distill_bwd"](x.detach(), t, ids, stats, scale, grad, 2.0), torch.autograd.grad(ref, x, grad)[0])

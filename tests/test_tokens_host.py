@@ -129,3 +129,17 @@ def test_scratch_sizes():
 def test_distill_refuses_temperatures_whose_square_leaves_fp32(temperature):
     with pytest.raises(ValueError, match="temperature"):
         _distill(temperature=temperature)
+
+
+def test_the_guide_s_loss_calls_the_entries_with_their_arguments():
+    """The launcher-level loss of the integration guide compiles, and passes as many arguments as the entry points take (its
+    GPU test runs it)."""
+    import ast
+    import re
+    from pathlib import Path
+
+    text = (Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    (src,) = (b for b in re.findall(r"```python\n(.*?)```", text, re.S) if b.startswith("# training/distill_hip.py"))
+    called = {n.func.attr: len(n.args) for n in ast.walk(ast.parse(src))
+              if isinstance(n, ast.Call) and isinstance(n.func, ast.Attribute) and n.func.attr.startswith("ebr_block")}
+    assert called == {n: len(_capi.SIGNATURES[n][1]) for n in ("ebr_block_distill_scratch", "ebr_block_distill", "ebr_block_distill_bwd")}
