@@ -529,8 +529,9 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
                activation: Optional[str] = None) -> Tensor:
     """f(weight * h + bias) for a channels-last tensor [B, ..., C]: h is x less its mean and over the square root of its
     variance plus ``eps``, both taken for each sample and each group of C / groups neighbouring channels, over all cells.
-    ``activation``: None, or "silu". ``weight`` and ``bias``: [C], or None (1 and 0). Statistics and sums are fp32 or wider,
-    outputs rounded once to x's dtype; differentiable twice, for x, weight and bias, and a third derivative raises."""
+    ``activation``: None, or "silu". ``weight`` and ``bias``: [C], or None (1 and 0). Statistics and sums are fp32 or wider
+    (a group's squares about its mean have to stay in that range), outputs rounded once to x's dtype; differentiable twice,
+    for x, weight and bias, and a third derivative raises."""
     host = _host.module()
     y = None if host is None or activation not in ACTIVATIONS else host.group_norm(x, groups, weight, bias, eps,
                                                                                    ACTIVATIONS[activation])

@@ -225,8 +225,8 @@ template <typename A> __device__ __forceinline__ void finish(const Args& a, cons
     *reinterpret_cast<A*>(a.scale) = (A)f;
 }
 
-// A part of a row, where there are too few rows to fill the card: 24 rows of 131,072 fp32 logits took 95 us a workgroup each,
-// 5 us in 32 parts and 6 to join them (their gradient 108 and 6).
+// A part of a row, where there are too few rows to fill the card: 24 rows of 131,072 fp32 logits take 95 us a workgroup each,
+// in 32 parts 5 us and 6 to join them (their gradient 108 and 6).
 template <typename T> __global__ __launch_bounds__(256) void k_part(Args a) {
     using A = typename Acc<T>::type;
     __shared__ A lds[16];
@@ -337,9 +337,9 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad_sh
 // barrier, from the same workgroup.
 //
 // The stores go past the caches: otherwise what reads next waits for these lines to be written back. Of 4,096 rows of 50,021
-// bf16 logits a loss and its gradient took 271 us, and 252 so; of 2,600 rows 168 and 139 us, with a sum of the gradient
-// after it 253 and 224, and of 600 rows (60 MB, which the last-level cache would keep) 68 and 68. The gradient alone takes
-// 148 us for the 4,096 rows (820 MB, 5.5 TB/s).
+// bf16 logits a loss and its gradient take 271 us through the caches and 251 past them; of 2,600 rows 168 and 139 us, with a
+// sum of the gradient after it 253 and 224, and of 600 rows (60 MB, which the last-level cache would keep) 68 and 68. The
+// gradient alone takes 148 us for the 4,096 rows (820 MB, 5.5 TB/s).
 template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Args a) {
     using A = typename Acc<T>::type;
     constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
@@ -431,8 +431,8 @@ template <typename T, int TEAM> __global__ __launch_bounds__(256) void k_grad(Ar
 
 constexpr int SHORT_ROW = 32;  // columns of a row in which each has a thread
 
-// k_grad's bits for the columns of a part: exact up to 2^17. Without them each entry went through all the others: 20,000 rows
-// of 4,001 with 256 entries took 265 us with their loss, 178 with them.
+// k_grad's bits for the columns of a part: exact up to 2^17. Without them each entry goes through all the others: 20,000 rows
+// of 4,001 bf16 logits with 256 entries take 312 us with their loss, 182 with them (fp32 361 and 303).
 static int seen_of(int64_t width) {
     int w = 1;
     while (w < 4096 && (int64_t)w * 32 < width) w *= 2;
@@ -443,7 +443,7 @@ static int64_t shared_of(int team, int K, int64_t width, int es) {
 }
 
 // Threads of a row: one a column for the shortest; then as many lanes as it has vectors, up to a wave (65,536 rows of 97
-// bf16 took 104 us a wave each, 62 with 16 lanes), but not so few that the rows of a workgroup take more than 32 KiB of shared
+// bf16 take 104 us a wave each, 57 with 16 lanes), but not so few that the rows of a workgroup take more than 32 KiB of shared
 // memory in the gradient; a workgroup for long rows.
 static int team_of(int dtype, int64_t V, int K) {
     if (V > 2048) return 256;
@@ -478,7 +478,8 @@ static int check(int dtype, int tdtype, int64_t N, int64_t V, int K, int64_t row
         if (d != EBR_DTYPE_F32 && d != EBR_DTYPE_BF16 && d != EBR_DTYPE_F16 && d != EBR_DTYPE_F64) return EBR_ERR_DTYPE;
     // (T: so that its square, and what Base adds at 32 bits, are far from the largest float)
     if (N < 0 || N >= ((int64_t)1 << 31) || V < 1 || V >= ((int64_t)1 << 30) || K < 1 || K > K_MAX || row < V ||
-        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T >= 1e-15 && T <= 1e15) || groups(N, team_of(dtype, V, K)) > MAX_BLOCKS)
+        N * V >= ((int64_t)1 << 40) || row >= ((int64_t)1 << 40) || !(T >= 1e-15 && T <= 1e15) ||
+        groups(N, team_of(dtype, V, K)) > MAX_BLOCKS)
         return EBR_ERR_SHAPE;
     return EBR_OK;
 }
@@ -568,7 +569,8 @@ int ebr_block_distill_bwd(int dtype, int tdtype, int ids64, int64_t N, int64_t V
     if (!logits || !teacher || !ids || !stats || !grad || !dx) return EBR_ERR_NULL;
     if (!aligned(stats, 16)) return EBR_ERR_ALIGN;
     Args a = {logits, teacher, ids, N, row_stride, (int)V, K, tdtype, ids64 != 0, LOG2E / temperature,
-              low_of(LOG2E / temperature), temperature, EBR_REDUCE_NONE, const_cast<void*>(stats), nullptr, const_cast<void*>(scale), nullptr, grad, grad_stride, dx};
+              low_of(LOG2E / temperature), temperature, EBR_REDUCE_NONE, const_cast<void*>(stats), nullptr,
+              const_cast<void*>(scale), nullptr, grad, grad_stride, dx};
     return by_type(dtype, [&](auto v) {
         using T = decltype(v);
         using A = typename Acc<T>::type;

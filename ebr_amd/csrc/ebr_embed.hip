@@ -58,7 +58,8 @@ __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int t
             for (int r = 0; r < ROWS; ++r)
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i)
-                    x[r][i] = *reinterpret_cast<const Raw*>(w + (int64_t)(v[r] < (uint32_t)ids.V ? v[r] : 0) * C + c + i * PIECE);
+                    x[r][i] =
+                        *reinterpret_cast<const Raw*>(w + (int64_t)(v[r] < (uint32_t)ids.V ? v[r] : 0) * C + c + i * PIECE);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (n0 + r * per >= N) break;
@@ -75,12 +76,13 @@ __global__ __launch_bounds__(256) void k_lookup(Ids ids, int64_t N, int C, int t
         }
     }
 }
+
 // -- positions sorted by token -----------------------------------------------------------------------------------------
 
 // A workgroup ranks a tile of 1,024 positions a round, as many rounds as leave at most 128 workgroups (each reads all the
-// others' counts); up to 4,096 positions are one workgroup's. A tile of 4,096 left most of the card idle: 16,384 positions
-// took 9.9 us a pass, 5.4 in tiles of 1,024 (and 2.9 the counts before it). Latency bounds it: launches, and what one kernel
-// wrote and the next reads on other XCDs. Nine bits a pass: one up to a vocabulary of 511, two up to 262,143.
+// others' counts); up to 4,096 positions are one workgroup's. 16,384 positions take 5.4 us a pass (and 3 the counts before it);
+// in tiles of 4,096, which leave most of the card idle, 9.9. Latency bounds it: launches, and what one kernel wrote and the
+// next reads on other XCDs. Nine bits a pass: one up to a vocabulary of 511, two up to 262,143.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ONE = 4096;
 constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS;
 constexpr int SORT_GROUPS = 128;
@@ -297,9 +299,9 @@ constexpr int AHEAD = 8;  // rows whose loads are under way together (of 16 the 
 // sorted positions and VEC columns a lane. A run of equal tokens inside the chunk is written to the table at once; a run
 // over its border goes to part. The other workgroups write zeros to the rows of tokens that do not occur, found by
 // search: these are most of the table for text, and their stores fill the time that the sums wait for their rows. They go
-// past the caches, in whole lines: 16,384 tokens of 50,021 x 1,024 bf16 took 81 us with their gradient, 61 so (but 32 bytes a
-// lane, which halves lines, cost the fp32 table of 100,003 x 2,048 150 us).
-// Bound by memory: 21 us for those tokens (132 MB, 6.3 TB/s), 188 us for 32,768 tokens of that table (953 MB, 5.1 TB/s).
+// past the caches, in whole lines: 16,384 tokens of 50,021 x 1,024 bf16 take 61 us with their gradient, through the caches 81
+// (32 bytes a lane, which halves lines, cost the fp32 table of 100,003 x 2,048 150 us).
+// Bound by memory: 21 us for those tokens (132 MB, 6.3 TB/s), 186 us for 32,768 tokens of that table (953 MB, 5.1 TB/s).
 template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_sum(SumArgs a) {
     using A = typename Acc<TW>::type;
     using Raw = typename Words<VEC * (int)sizeof(TY)>::type;
@@ -398,8 +400,8 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
 constexpr int JOIN_WAVES = 8;
 
 // Runs over chunks' borders: the workgroup of the chunk in which a run begins adds its parts, its teams of lanes (as k_sum's)
-// in turn, and the teams' sums in order. 4 to 7 us, most of it the launch: few runs are that long, but one wave for each took
-// 22 us where 11 tokens had 31,104 positions.
+// in turn, and the teams' sums in order. 4 to 10 us, most of it the launch. Few runs are that long; one wave for each takes
+// 22 us where 11 tokens have 31,104 positions.
 template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_join(SumArgs a) {
     using A = typename Acc<TW>::type;
     __shared__ A sums[JOIN_WAVES * 64 * VEC];
@@ -460,8 +462,8 @@ template <typename TW, int VEC> __global__ __launch_bounds__(64 * JOIN_WAVES) vo
 // each a workgroup's, about the same.
 constexpr int FEW = 256, FEW_ROWS = 32768;
 
-template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) void k_few(Ids ids, int N, int C, double scale,
-                                                                                          const TY* dy, TW* dw) {
+template <typename TW, typename TY, int VEC>
+__global__ __launch_bounds__(256) void k_few(Ids ids, int N, int C, double scale, const TY* dy, TW* dw) {
     using A = typename Acc<TW>::type;
     using Raw = typename Words<VEC * (int)sizeof(TY)>::type;
     __shared__ A sums[4][64 * VEC];
@@ -508,10 +510,11 @@ template <typename TW, typename TY, int VEC> __global__ __launch_bounds__(256) v
 // under way, and go to their tokens' sums. A workgroup has a chunk of the positions, its waves a part of it each, and 64 vectors
 // of the columns. Its sums together are its part of the gradient.
 //
-// 31,104 positions of 11 x 512 bf16 take 14 us with the join, where sorting and summing take 27 (32 MB, 6.7 us of them); with
-// 65,536 x 2,048 55 us and 64 (4.9 TB/s). From 17 rows on, four waves' sums fill the memory: 32 rows take 20 us and 26 in the
-// first case, 83 and 65 in the second, and more rows are slower than the sort in all. The next rows' loads ahead of the
-// sums made it 75 us there, and 59 of the 55.
+// 31,104 positions of 11 x 512 bf16 take 16 us with the join, where sorting and summing take 27 (32 MB, 6.7 us of them); the
+// whole gradient of 65,536 x 2,048 (268 MB, 56 us) 62 us and 66 in a row of calls, where the last-level cache keeps part of dy,
+// and 96 and 110 after other work. From 17 rows on, four waves' sums fill the memory: 32 rows take 20 us and 26 in the first
+// case, 83 and 65 in the second, and more rows are slower than the sort in all. With the next rows' loads ahead of the sums,
+// 11 rows take 59 us in place of 55 of the second case's kernel.
 constexpr int TALLY = 16;
 static bool small(int64_t N, int64_t V, int64_t C) { return N > 0 && (V <= 16 || (V <= 32 && N * C <= 1 << 25)); }
 
@@ -703,8 +706,8 @@ int ebr_block_embed(int wdtype, int ydtype, int ids64, int64_t N, int64_t V, int
         const auto go = [&](auto vec) {
             constexpr int VN = decltype(vec)::value;
             const int team = team_of(C, VN);
-            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, rows_of<TW>() * (256 / team))), dim3(256), 0, (hipStream_t)stream, i,
-                               N, C, team, scale, (const TW*)w, (TY*)y);
+            hipLaunchKernelGGL((k_lookup<TW, TY, VN>), dim3(blocks_for(N, rows_of<TW>() * (256 / team))), dim3(256), 0,
+                               (hipStream_t)stream, i, N, C, team, scale, (const TW*)w, (TY*)y);
         };
         by_vector<TY>(C, {w, y}, go);
         return launched();

@@ -17,9 +17,10 @@
 // are about the mean, or of eight cells at a time about theirs, which go together by the rule for the variance of a union.
 //
 // Bound by memory as far as the arithmetic (some 20, 30 and 75 operations an element) leaves it. 768 boards of 81 x 512 bf16
-// (64 MB a tensor), groups of 16 channels: 28 us (4.5 TB/s), 41 (4.6), 87 (3.7) for the norm, its gradient and the second
-// derivative; 64 boards of 900 x 512: 34 and 55 us. Two grids of 128 x 128 x 320 fp32 (42 MB a tensor, read twice, the
-// second time from the last-level cache): 35, 48 and 79 us in three launches each.
+// (64 MB a tensor), groups of 16 channels: 29 us (4.4 TB/s), 42 (4.5), 88 (3.6) for the norm, its gradient and the second
+// derivative; 64 boards of 900 x 512 (59 MB): 34 and 50 to 57 us, and 134 for the second derivative, read twice and at one
+// wave a SIMD in k_sums. Two grids of 128 x 128 x 320 fp32 (42 MB a tensor, read twice, the second time from the last-level
+// cache): 35, 47 and 77 us in three launches each.
 #include <type_traits>
 
 #include "rowwise.hpp"
@@ -30,7 +31,8 @@ using namespace ebr_row;
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int SUMS[3] = {2, 2, 10};   // of a mode; mode 0: the mean and the squares about it
-constexpr int MEANS[3] = {2, 2, 6};   // kept of a group: mode 0: mu, r; 1: mean k, mean(k h); 2: u, u h, k h, v, v h, and Group2's along
+// kept of a group: mode 0: mu, r; 1: mean k, mean(k h); 2: u, u h, k h, v, v h, and Group2's along
+constexpr int MEANS[3] = {2, 2, 6};
 
 struct Args {
     const void *x, *dy, *u;
@@ -80,7 +82,7 @@ template <typename A> struct Spread {
         if (all == (A)0) return;
         const A d = omean - mean, f = on / all;
         mean += d * f;
-        m2 += om2 + d * (d * (n * f));  // n f is 0 where a side has nothing: d is the other's mean, its square perhaps infinite
+        m2 += om2 + d * (d * (n * f));  // n f is 0 where a side has nothing: d is a mean then, its square perhaps infinite
         n = all;
     }
 };
@@ -218,7 +220,8 @@ template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(T
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int64_t row = l + (int64_t)i * p.step;
-                    x[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.x) + base + (row < p.to ? row : p.to - 1) * a.C);
+                    x[i] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.x) + base +
+                                                         (row < p.to ? row : p.to - 1) * a.C);
                 }
                 const int64_t left = (p.to - 1 - l) / p.step + 1;
                 const int n = left < 8 ? (int)left : 8;
@@ -493,7 +496,8 @@ template <typename A> __global__ __launch_bounds__(1024) void k_params(Args a) {
 }
 
 // The outputs of a part of L, past the caches, which hold what is read here for the second time: a graded step of 64 boards
-// of 900 x 512 bf16 took 231 us, and 206 so (with a reader of each output 314 and 298).
+// of 900 x 512 bf16, whose second derivative comes here, takes 224 us through the caches and 214 past them, of 16 of 4,400 x
+// 512, which comes here in all three orders, 289 and 264 (with a reader of each output 314 and 305, 397 and 381).
 template <typename T, int VEC, int MODE, int ACT> __global__ __launch_bounds__(THREADS) void k_apply(Args a) {
     using A = typename Acc<T>::type;
     const Place p = place<VEC>(a);
@@ -565,9 +569,9 @@ __device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0)
 // A thread sums its own cells by channel. All that follows is linear in these sums, so a thread takes them to its group's
 // means by itself, and what goes through shared memory is one number a thread for each mean (five and then two of the second
 // derivative, in place of ten for each channel), and for the parameters' gradients, where they are wanted, two a channel.
-// With every channel's sums reduced, the second derivative of 768 boards of 81 x 512 took 224 us, most of it that reduction;
-// 113 so. A wave for each group, without barriers, was slower (32 bytes of a cell at a time: 134 against 102), and so were
-// wider cells (256 bytes, eight waves: 107).
+// Every channel's sums through shared memory doubled the second derivative (224 and 113 us for 768 boards of 81 x 512). A wave
+// for each group, without barriers, is slower (32 bytes of a cell at a time: 134 and 102 us), and so are wider cells (256
+// bytes, eight waves: 107 and 102).
 template <typename T, int VEC, int MODE, int ACT, int R, int W>
 __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(Args a) {
     using A = typename Acc<T>::type;
@@ -621,7 +625,7 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
     };
     // p's means over this thread's group: over the wave's threads of the same channels, over the waves, over the channels. The
     // sums stay in 32 bits, as the cells' are, and only the mean is taken in 64, by a product: with divisions, and the channels
-    // added in 64 bits, the three orders of 768 boards of 81 x 512 bf16 took 31, 43 and 95 us, 28, 41 and 87 so.
+    // added in 64 bits, the three orders of 768 boards of 81 x 512 bf16 take 31, 43 and 95 us in place of 28, 41 and 87.
     const auto means = [&](auto& p, double* out) {
         constexpr int K = sizeof(p) / sizeof(p[0]);
         for (int d = a.tx; d < 64; d <<= 1)
@@ -725,9 +729,9 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
             stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + (int64_t)l * a.C, o);
         }
     } else {
-        // The gradient of up to four cells keeps da, and its second half has neither dy nor the activation to take again: which
-        // is as long as the memory traffic otherwise (50 us for 768 boards of 81 x 512 bf16, 42 so). In the second derivative the
-        // sigmoids kept took 85 us where it takes 87, in 116 registers.
+        // The gradient of up to four cells keeps da, and its second half has neither dy nor the activation to take again, which
+        // is as long as the memory traffic (768 boards of 81 x 512 bf16 take 42 us, and 50 with both taken again). In the second
+        // derivative, sigmoids that are kept would gain 2 us of 87 there, for 116 registers and a wave less on each SIMD.
         constexpr bool KEEP = MODE == 1 && ACT != 0 && R <= 4;
         A kept[KEEP ? R : 1][KEEP ? VEC : 1];
         A s[NS][VEC] = {};
@@ -737,10 +741,12 @@ __global__ __launch_bounds__(64 * W, MODE == 2 && R == 12 ? 5 : 1) void k_whole(
         for (int i = 0; i < R; ++i) {
             one_by_one();
             if (!on || ty + i * step >= L) continue;
-            const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]), uv = unpacked<T, VEC>(u[MODE == 2 ? i : 0]);
+            const Pack<T, VEC> xv = unpacked<T, VEC>(x[i]), dv = unpacked<T, VEC>(dy[i]);
+            const Pack<T, VEC> uv = unpacked<T, VEC>(u[MODE == 2 ? i : 0]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const A da = add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, mu, w[e], b[e]);
+                const A da =
+                    add_sums<ACT, MODE, A>(s, e, (A)xv.e[e], (A)dv.e[e], MODE == 2 ? (A)uv.e[e] : (A)0, mu, w[e], b[e]);
                 if constexpr (KEEP) kept[i][e] = da;
             }
         }
@@ -902,13 +908,14 @@ struct Scratch {
 // Whether a workgroup holds a sample's tile of groups, and how: W waves of some cells a thread, tx threads across the tile's
 // channels. A thread's vector has to lie in one group, and a tile of whole groups to fill three quarters of the threads
 // across, which take 128 bytes of a cell or more: more where a sample has fewer cells than the rest of the workgroup holds (a
-// graded step of 1,000 samples of 4 cells of 1,024 bf16 channels took 169 us with 28 of 32 threads idle, 119 across) or
-// where a group is wider (one group of 16 such cells: 427 us through k_sums and k_apply, 156 held). Above 256 cells at 128
+// graded step of 1,000 samples of 4 cells of 1,024 bf16 channels takes 169 us with 28 of 32 threads idle, 118 across) or
+// where a group is wider (one group of 16 such cells: 427 us through k_sums and k_apply, 132 held). Above 256 cells at 128
 // bytes for the second derivative, 1,024 for the others, groups go through those, which read everything twice.
 //
 // The vector is 16 bytes, but 2 channels of 16 bits in the second derivative, whose ten sums a channel and three tensors
-// fill the registers: 768 boards of 81 x 512 bf16 took 113 us at 8 channels (three waves a SIMD), 102 at 4 (four), 94 at 2
-// (five), all with divisions in the means. Of groups too wide for that, 4.
+// fill the registers: 768 boards of 81 x 512 bf16 take 88 us so (five waves a SIMD), 132 at 4 channels. Of groups too wide for
+// 2, 4. Kernels hold 12 or 32 cells a thread then: boards of 81 cells need 11, and of 100 13, which take 119 us at 768 boards
+// (three waves a SIMD).
 struct Whole {
     int waves = 0, cells = 0, vec = 0, tx = 0, tile = 0, tiles = 0;
     // the two numbers of cells that there are kernels for
@@ -1016,8 +1023,8 @@ template <int MODE> static int run(int dtype, int act, Args a, void* scratch, vo
             return;
         }
         hipLaunchKernelGGL((k_sums<T, VEC, MODE, ACT>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a);
-        hipLaunchKernelGGL((k_means<A, MODE, ACT>), dim3((unsigned)(a.B * a.G)), dim3(a.cg * (int64_t)a.splits > 64 ? THREADS : 64),
-                           0, s, a);
+        hipLaunchKernelGGL((k_means<A, MODE, ACT>), dim3((unsigned)(a.B * a.G)),
+                           dim3(a.cg * (int64_t)a.splits > 64 ? THREADS : 64), 0, s, a);
         hipLaunchKernelGGL((k_apply<T, VEC, MODE, ACT>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a);
         if (MODE != 0 && a.chan) hipLaunchKernelGGL((k_params<A>), dim3((a.C + 31) / 32, 2), dim3(1024), 0, s, a);
     });

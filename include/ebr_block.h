@@ -1,7 +1,7 @@
 /* C ABI of the energy network's fused pointwise blocks in libebr_attn.so (gfx950): rms_norm over the last dimension
  * and the SwiGLU activation, each with its backward and the backward of that backward, as the graded latent descent
- * differentiates the energy twice; the group norm with an activation, likewise; and the ends of a training step, the embedding of tokens with its table's gradient and
- * the distillation loss with its gradient.
+ * differentiates the energy twice; the group norm with an activation, likewise; and the ends of a training step, the
+ * embedding of tokens with its table's gradient and the distillation loss with its gradient.
  *
  * Tensors are contiguous rows of one dtype (EBR_DTYPE_F32, _BF16, _F16 or _F64). Arithmetic is fp32 (fp64 for fp64);
  * outputs are rounded once to the dtype. Conventions otherwise as in ebr_attn.h (error codes, streams, ownership).
