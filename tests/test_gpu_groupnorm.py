@@ -212,7 +212,7 @@ def test_long_groups_of_one_large_value(cuda, dtype, shape, G):
         assert float((block.group_norm(x, G, eps=EPS) - ref).abs().max()) <= 3 * 1e4 * 2.0**-24 * float(ref.abs().max())
 
 
-# a thread with few cells and many, one wave a SIMD's share and 16 waves, a tile of several groups and one of all channels
+# few cells a thread and many, 4 waves and 16, a tile of several groups and one of all channels
 @pytest.mark.parametrize("shape,G", [((2, 20, 32), 4), ((1, 900, 512), 16), ((2, 256, 64), 2), ((2, 5, 512), 1), ((1, 1024, 64), 8)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_held_groups_of_one_large_value(cuda, dtype, shape, G):
