@@ -1,5 +1,5 @@
 """ctypes binding of ``libebr_attn.so`` (declared in ``include/ebr_attn.h``, ``include/ebr_rope.h``,
-``include/ebr_descent.h`` and ``include/ebr_block.h``).
+``include/ebr_descent.h``, ``include/ebr_block.h`` and ``include/ebr_optim.h``).
 
 The library is built in-tree by ``ebr_amd.build`` into ``ebr_amd/_lib/``. Loading needs only the HIP runtime, so the
 symbols can be checked on a machine without a GPU; every compute entry point needs a gfx950 device.
@@ -167,6 +167,26 @@ SIGNATURES = {
         ctypes.c_int64,
         [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 2,
     ),
+    "ebr_block_layernorm": (
+        ctypes.c_int,
+        [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int, ctypes.c_double] + [_P] * 6,
+    ),
+    "ebr_block_layernorm_bwd": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int] + [_P] * 9),
+    "ebr_block_layernorm_bwd2": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int] + [_P] * 12),
+    "ebr_block_layernorm_scratch": (ctypes.c_int64, [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int]),
+    "ebr_block_swiglu_linear": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 4),
+    "ebr_block_swiglu_linear_bwd": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 7),
+    "ebr_block_swiglu_linear_bwd2": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 9),
+    "ebr_block_swiglu_linear_scratch": (ctypes.c_int64, [ctypes.c_int] * 2 + [ctypes.c_int64] * 3),
+    # include/ebr_optim.h
+    "ebr_block_grad_norm": (ctypes.c_int, [ctypes.c_int64] + [_P] * 5),
+    "ebr_block_grad_norm_scratch": (ctypes.c_int64, [ctypes.c_int64, _P]),
+    "ebr_block_adamw": (
+        ctypes.c_int,
+        [ctypes.c_int] * 3 + [ctypes.c_int64, _P, ctypes.c_double, _P] + [ctypes.c_double] * 4
+        + [_P, ctypes.c_double, _P, _P],
+    ),
+    "ebr_block_adamw_scratch": (ctypes.c_int64, [ctypes.c_int64]),
     "ebr_attn_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ebr_attn_abi_version": (ctypes.c_int, []),
     "ebr_attn_arch": (ctypes.c_char_p, []),
@@ -201,6 +221,14 @@ def load(path: Optional[Path] = None) -> ctypes.CDLL:
         if path is None:
             _LIB, _ERROR = lib, None
         return lib
+
+
+class OptimGrad(ctypes.Structure):  # ebr_optim_grad
+    _fields_ = [("g", _P), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class OptimTensor(ctypes.Structure):  # ebr_optim_tensor
+    _fields_ = [("p", _P), ("g", _P), ("m", _P), ("v", _P), ("ms", _P), ("vs", _P), ("step", _P), ("n", ctypes.c_int64)]
 
 
 def load_error() -> Optional[str]:

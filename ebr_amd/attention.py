@@ -27,6 +27,7 @@ from torch import nn
 from ebr_amd.layers import (
     RMS_NORM_EPS,
     CastedLinear,
+    LayerNorm,
     RopeFused,
     RotaryTable2D,
     SwiGLU,
@@ -397,7 +398,8 @@ class EnergyAttention(nn.Module):
 
 class EnergyReasoningBlock(nn.Module):
     """Post-norm block: h <- rms_norm(h + sublayer(h)) for the attention, then for the SwiGLU MLP. ``norm="group"`` takes a
-    group norm over the board's cells (``norm_groups`` groups of channels) in rms_norm's place."""
+    group norm over the board's cells (``norm_groups`` groups of channels) in rms_norm's place, ``norm="layer"`` a layer norm
+    with a learned weight and bias. ``mlp_impl``: the MLP's, ``block_impl`` if not given."""
 
     norm = "rms"  # on the class: a whole module unpickled from before it existed has no such attribute
 
@@ -408,15 +410,21 @@ class EnergyReasoningBlock(nn.Module):
             raise ValueError(f"hidden_size {hidden} does not split into {heads} heads")
         self.block_impl = getattr(config, "block_impl", "eager")
         self.norm, self.norm_groups = getattr(config, "norm", "rms"), getattr(config, "norm_groups", 1)
-        if self.norm not in ("rms", "group"):
-            raise ValueError(f"norm must be 'rms' or 'group', got {self.norm!r}")
+        if self.norm not in ("rms", "group", "layer"):
+            raise ValueError(f"norm must be 'rms', 'group' or 'layer', got {self.norm!r}")
         if self.norm == "group" and (self.norm_groups < 1 or hidden % self.norm_groups):
             raise ValueError(f"hidden_size {hidden} does not split into {self.norm_groups} norm groups")
         self.self_attn = EnergyAttention(hidden, hidden // heads, heads, backend=config.attn_backend,
                                          nograd_backend=config.attn_nograd_backend)
-        self.mlp = SwiGLU(hidden_size=hidden, expansion=config.expansion, impl=self.block_impl)
+        mlp_impl = getattr(config, "mlp_impl", None)
+        self.mlp = SwiGLU(hidden_size=hidden, expansion=config.expansion, impl=mlp_impl or self.block_impl)
+        if self.norm == "layer":
+            impl = "fused" if self.block_impl == "fused" else "eager"
+            self.layer_norms = nn.ModuleList(LayerNorm(hidden, RMS_NORM_EPS, impl) for _ in range(2))
 
-    def _add_norm(self, h: Tensor, r: Tensor) -> Tensor:
+    def _add_norm(self, h: Tensor, r: Tensor, at: int = 0) -> Tensor:
+        if self.norm == "layer":
+            return self.layer_norms[at](h + r)
         if self.norm == "group":
             if self.block_impl == "fused":
                 from ebr_amd import block
@@ -434,8 +442,8 @@ class EnergyReasoningBlock(nn.Module):
 
     def forward(self, cos_sin: Any, hidden_states: Tensor) -> Tensor:
         h = hidden_states
-        for sublayer in self._sublayers(cos_sin):
-            h = self._add_norm(h, sublayer(h))
+        for at, sublayer in enumerate(self._sublayers(cos_sin)):
+            h = self._add_norm(h, sublayer(h), at)
         return h
 
 

@@ -7,22 +7,25 @@ training loss differentiates it again).
 - ``swiglu(gate_up)``       reference models/layers.py:74-84 (``gate, up = gate_up.chunk(2, -1)``; ``silu(gate) * up``)
 - ``group_norm(x, groups, weight, bias, eps, activation)``   over a board's cells, channels last, with its activation
   (kernels ``ebr_amd/csrc/ebr_groupnorm.hip``)
+- ``layer_norm(x, weight, bias, eps)``   over the last dimension (kernels ``ebr_amd/csrc/ebr_layernorm.hip``)
+- ``swiglu_linear(x, weight)``   ``swiglu`` of x's projection by the stacked gate and up weights, the products on the matrix
+  cores with the activation in their epilogue (kernels ``ebr_amd/csrc/ebr_glu.hip``)
 
 Ops (``torch.ops.ebr_fused.*``, HIP device only; a missing library raises): ``block_rmsnorm``, ``block_rmsnorm_bwd``,
 ``block_rmsnorm_bwd2``, ``block_swiglu``, ``block_swiglu_bwd``, ``block_swiglu_bwd2``, ``block_groupnorm``,
-``block_groupnorm_bwd``, ``block_groupnorm_bwd2``. Autograd: each op's backward
-is the next op, so the functions are differentiable to second order; the second backward is not itself
+``block_groupnorm_bwd``, ``block_groupnorm_bwd2``, ``block_layernorm``, ``block_layernorm_bwd``, ``block_layernorm_bwd2``,
+``block_swiglu_linear``, ``block_swiglu_linear_bwd``, ``block_swiglu_linear_bwd2``. Autograd: each op's backward is the next op, so the functions are differentiable to second order; the second backward is not itself
 differentiable. The arithmetic is fp32 (fp64 for fp64 tensors), each output rounded once to the dtype where eager
 autograd chains several rounded kernels, so 16-bit results differ from eager by rounding only.
 """
 
 # No ``from __future__ import annotations``: custom_op schema inference needs real type objects.
-from typing import Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from ebr_amd import _capi, _host
+from ebr_amd import _capi, _host, linear
 from ebr_amd.fused_attn.loader import hip_library
 from ebr_amd.fused_attn.ops import _DTYPE_CODE, _stream
 
@@ -441,7 +444,7 @@ def _wants_params(ctx, w: Optional[Tensor], b: Optional[Tensor]) -> bool:
         node, at = ctx.next_functions[at][0], at + 1
         if not ctx.needs_input_grad[i] or node is None:
             continue
-        if node.name().endswith("AccumulateGrad") or torch._C._will_engine_execute_node(node):
+        if linear._will_run(node):
             return True
     return False
 
@@ -548,6 +551,420 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     return _GroupNorm.apply(x, weight, bias, groups, float(eps), ACTIVATIONS[activation])[0]
 
 
+# ---------------------------------------------------------------------------------------------------------------------
+# Layer norm
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _last(x: Tensor) -> Tuple[int, int]:
+    """Rows and C of a tensor [..., C]."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"fused block: layer_norm needs [..., C], got {tuple(x.shape)}")
+    return x.numel() // x.shape[-1], x.shape[-1]
+
+
+def _norm_params(x: Tensor, ps: Sequence[Tuple[str, Optional[Tensor]]]) -> Tuple[torch.dtype, List[Optional[Tensor]]]:
+    """The weights and biases [C] as the kernels read them, contiguous and of one dtype: their own where they share one, else
+    the accumulation type."""
+    for name, p in ps:
+        if p is None:
+            continue
+        if tuple(p.shape) != (x.shape[-1],) or p.device != x.device:
+            raise ValueError(f"fused block: {name} is {tuple(p.shape)} on {p.device}, expected ({x.shape[-1]},) on {x.device}")
+        if p.dtype not in _DTYPE_CODE:
+            raise TypeError(f"fused block: unsupported dtype {p.dtype} of {name}")
+    types = {p.dtype for _, p in ps if p is not None}
+    dtype = types.pop() if len(types) == 1 else _acc(x)
+    return dtype, [None if p is None else _c(p.to(dtype)) for _, p in ps]
+
+
+def _layer_scratch(x: Tensor, order: int, rows: int, C: int) -> Tensor:
+    n = hip_library().ebr_block_layernorm_scratch(_code(x), order, rows, C)
+    if n < 0:
+        _capi.check(2, "ebr_block_layernorm")
+    return torch.empty((n,), device=x.device, dtype=torch.uint8)
+
+
+@torch.library.custom_op("ebr_fused::block_layernorm", mutates_args=(), device_types="cuda")
+def layernorm_op(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor]:
+    """(y, stats [rows, 4]: each row's rounded mean, what that lacks, 1 / sqrt(variance + eps), 0)."""
+    lib = hip_library()
+    code, (rows, C) = _code(x), _last(x)
+    x = _c(x)
+    wt, (w, b) = _norm_params(x, (("weight", weight), ("bias", bias)))
+    y = torch.empty_like(x)
+    stats = torch.empty((rows, 4), device=x.device, dtype=_acc(x))
+    if rows == 0:
+        return y, stats
+    with torch.cuda.device(x.device):
+        rc = lib.ebr_block_layernorm(code, _DTYPE_CODE[wt], rows, C, eps, x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(),
+                                     stats.data_ptr(), _stream(x))
+    _capi.check(rc, "ebr_block_layernorm")
+    return y, stats
+
+
+@layernorm_op.register_fake
+def _(x, weight, bias, eps):
+    return (torch.empty_like(x, memory_format=torch.contiguous_format),
+            x.new_empty((x.numel() // x.shape[-1], 4), dtype=_acc(x)))
+
+
+def _check_row_stats(stats: Tensor, x: Tensor, rows: int) -> Tensor:
+    _like(stats, (rows, 4), x, "stats")
+    if stats.dtype != _acc(x):
+        raise TypeError(f"fused block: stats are {stats.dtype}, expected {_acc(x)}")
+    return _c(stats)
+
+
+@torch.library.custom_op("ebr_fused::block_layernorm_bwd", mutates_args=(), device_types="cuda")
+def layernorm_bwd_op(x: Tensor, weight: Optional[Tensor], stats: Tensor, dy: Tensor, ptype: torch.dtype,
+                     params: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx, dw, db); the latter of ``ptype``, and empty without ``params``."""
+    lib = hip_library()
+    code, (rows, C) = _code(x), _last(x)
+    _like(dy, x.shape, x, "dy")
+    stats = _check_row_stats(stats, x, rows)
+    x, dy = _c(x), _c(dy.to(x.dtype))
+    _, (w,) = _norm_params(x, (("weight", weight),))
+    w = None if w is None else _c(w.to(ptype))
+    dx = torch.empty_like(x)
+    dw, db = (torch.empty((C if params else 0,), device=x.device, dtype=ptype) for _ in range(2))
+    if rows == 0:
+        return dx, dw.zero_(), db.zero_()
+    scratch = _layer_scratch(x, 1, rows, C)
+    with torch.cuda.device(x.device):
+        rc = lib.ebr_block_layernorm_bwd(
+            code, _DTYPE_CODE[ptype], rows, C, x.data_ptr(), _ptr(w), stats.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+            dw.data_ptr() if params else 0, db.data_ptr() if params else 0, scratch.data_ptr(), _stream(x),
+        )  # fmt: skip
+    _capi.check(rc, "ebr_block_layernorm_bwd")
+    return dx, dw, db
+
+
+@layernorm_bwd_op.register_fake
+def _(x, weight, stats, dy, ptype, params):
+    dw = x.new_empty((x.shape[-1] if params else 0,), dtype=ptype)
+    return torch.empty_like(x, memory_format=torch.contiguous_format), dw, torch.empty_like(dw)
+
+
+@torch.library.custom_op("ebr_fused::block_layernorm_bwd2", mutates_args=(), device_types="cuda")
+def layernorm_bwd2_op(x: Tensor, weight: Optional[Tensor], stats: Tensor, dy: Tensor, u: Tensor, uw: Optional[Tensor],
+                      ub: Optional[Tensor], ptype: torch.dtype, params: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(gx, gdy, gw): the gradients of <u, dx> + <uw, dw> + <ub, db>; gw of ``ptype``, and empty without ``params``."""
+    lib = hip_library()
+    code, (rows, C) = _code(x), _last(x)
+    _like(dy, x.shape, x, "dy")
+    _like(u, x.shape, x, "u")
+    stats = _check_row_stats(stats, x, rows)
+    x, dy, u = _c(x), _c(dy.to(x.dtype)), _c(u.to(x.dtype))
+    ps = [_norm_params(x, ((n, p),))[1][0] for n, p in (("weight", weight), ("uw", uw), ("ub", ub))]
+    w, uw, ub = (None if p is None else _c(p.to(ptype)) for p in ps)
+    gx, gdy = torch.empty_like(x), torch.empty_like(x)
+    gw = torch.empty((C if params else 0,), device=x.device, dtype=ptype)
+    if rows == 0:
+        return gx, gdy, gw.zero_()
+    scratch = _layer_scratch(x, 2, rows, C)
+    with torch.cuda.device(x.device):
+        rc = lib.ebr_block_layernorm_bwd2(
+            code, _DTYPE_CODE[ptype], rows, C, x.data_ptr(), _ptr(w), stats.data_ptr(), dy.data_ptr(), u.data_ptr(),
+            _ptr(uw), _ptr(ub), gx.data_ptr(), gdy.data_ptr(), gw.data_ptr() if params else 0, scratch.data_ptr(), _stream(x),
+        )  # fmt: skip
+    _capi.check(rc, "ebr_block_layernorm_bwd2")
+    return gx, gdy, gw
+
+
+@layernorm_bwd2_op.register_fake
+def _(x, weight, stats, dy, u, uw, ub, ptype, params):
+    gx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    return gx, torch.empty_like(gx), x.new_empty((x.shape[-1] if params else 0,), dtype=ptype)
+
+
+def _ptype(x: Tensor, w: Optional[Tensor], b: Optional[Tensor]) -> torch.dtype:
+    """The dtype that the parameters' gradients leave the kernels in."""
+    types = {p.dtype for p in (w, b) if p is not None}
+    return types.pop() if len(types) == 1 else _acc(x)
+
+
+class _LayerNormBwd2(torch.autograd.Function):
+    """A node of its own, so that a third derivative is an error: without it the gradients would pass for constants."""
+
+    @staticmethod
+    def forward(x, w, stats, dy, u, uw, ub, ptype, params):
+        gx, gdy, gw = torch.ops.ebr_fused.block_layernorm_bwd2(x, w, stats, dy, u, uw, ub, ptype, params)
+        return gx, gdy, _as(gw, w) if params else None
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("trying to differentiate twice a function that was marked with @once_differentiable: "
+                           "layer_norm has no third derivative")
+
+
+class _LayerNormBwd(torch.autograd.Function):
+    @staticmethod
+    def forward(x, w, b, stats, dy, params):
+        ptype = _ptype(x, w, b)
+        dx, dw, db = torch.ops.ebr_fused.block_layernorm_bwd(x, w, stats, dy, ptype, params)
+        return dx, _as(dw, w) if params else None, _as(db, b) if params else None
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, b, stats, dy, _ = inputs
+        ctx.ptype = _ptype(x, w, b)
+        ctx.save_for_backward(x, w, stats, dy)
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def backward(ctx, u, uw, ub):
+        x, w, stats, dy = ctx.saved_tensors
+        if u is None and uw is None and ub is None:
+            return (None,) * 6
+        params = _wants_params(ctx, w, None)
+        u = torch.zeros_like(x) if u is None else u
+        gx, gdy, gw = _LayerNormBwd2.apply(x, w, stats, dy, u, uw, ub, ctx.ptype, params)
+        return gx, gw, None, None, gdy, None
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(x, w, b, eps):
+        return torch.ops.ebr_fused.block_layernorm(x, w, b, eps)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, b, _ = inputs
+        ctx.mark_non_differentiable(output[1])
+        ctx.save_for_backward(x, w, b, output[1])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def backward(ctx, dy, _stats):
+        x, w, b, stats = ctx.saved_tensors
+        if dy is None:
+            return (None,) * 4
+        dx, dw, db = _LayerNormBwd.apply(x, w, b, stats, dy, _wants_params(ctx, w, b))
+        return dx, dw, db, None
+
+
+@_host.gradient("layer_norm")
+def _layer_norm_grads(x, w, b, stats, params, dy):
+    return _LayerNormBwd.apply(x, w, b, stats, dy, params)
+
+
+@_host.gradient("layer_norm_bwd")
+def _layer_norm_bwd_grads(x, w, stats, dy, ptype, params, u, uw, ub):
+    u = torch.zeros_like(x) if u is None else u
+    gx, gdy, gw = _LayerNormBwd2.apply(x, w, stats, dy, u, uw, ub, _CODE_DTYPE[ptype], params)
+    return gx, gw, None, None, gdy
+
+
+_CODE_DTYPE = {code: dtype for dtype, code in _DTYPE_CODE.items()}
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """weight * h + bias over the last dimension of x [..., C]: h is x less its row's mean and over the square root of the
+    row's variance plus ``eps``. ``weight`` and ``bias``: [C], or None (1 and 0). Statistics and sums are fp32 or wider (the
+    squares about a row's mean have to stay in that range), outputs rounded once; differentiable twice, for x,
+    weight and bias, and a third derivative raises."""
+    host = _host.module()
+    y = None if host is None else host.layer_norm(x, weight, bias, eps)
+    if y is not None:
+        return y
+    _code(x), _last(x), _norm_params(x.detach(), (("weight", weight), ("bias", bias)))
+    if not eps >= 0:
+        raise ValueError(f"fused block: eps must not be negative, got {eps}")
+    return _LayerNorm.apply(x, weight, bias, float(eps))[0]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Gated projection
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _projection(x: Tensor, w: Tensor) -> Tuple[int, int, int]:
+    """N, C and I of x [..., C] and a weight [2 I, C]."""
+    if w.dim() != 2 or w.shape[0] % 2 or w.shape[0] < 2:
+        raise ValueError(f"fused block: swiglu_linear's weight must be [2 I, C], got {tuple(w.shape)}")
+    if x.dim() < 1 or x.shape[-1] != w.shape[1] or x.shape[-1] < 1:
+        raise ValueError(f"fused block: x is {tuple(x.shape)}, expected [..., {w.shape[1]}]")
+    if x.device != w.device:
+        raise ValueError(f"fused block: x is on {x.device}, weight on {w.device}")
+    if x.dtype != w.dtype:
+        raise TypeError(f"fused block: x is {x.dtype}, weight {w.dtype}")
+    return x.numel() // x.shape[-1], x.shape[-1], w.shape[0] // 2
+
+
+def _projection_scratch(x: Tensor, order: int, N: int, C: int, I: int) -> Tensor:
+    n = hip_library().ebr_block_swiglu_linear_scratch(_code(x), order, N, C, I)
+    if n < 0:
+        _capi.check(2, "ebr_block_swiglu_linear")
+    return torch.empty((n,), device=x.device, dtype=torch.uint8)
+
+
+@torch.library.custom_op("ebr_fused::block_swiglu_linear", mutates_args=(), device_types="cuda")
+def swiglu_linear_op(x: Tensor, weight: Tensor) -> Tensor:
+    lib = hip_library()
+    code, (N, C, I) = _code(x), _projection(x, weight)
+    x, weight = _c(x), _c(weight)
+    y = x.new_empty((*x.shape[:-1], I))
+    if N == 0:
+        return y
+    with torch.cuda.device(x.device):
+        rc = lib.ebr_block_swiglu_linear(code, N, C, I, x.data_ptr(), weight.data_ptr(), y.data_ptr(), _stream(x))
+    _capi.check(rc, "ebr_block_swiglu_linear")
+    return y
+
+
+@swiglu_linear_op.register_fake
+def _(x, weight):
+    return x.new_empty((*x.shape[:-1], weight.shape[0] // 2))
+
+
+@torch.library.custom_op("ebr_fused::block_swiglu_linear_bwd", mutates_args=(), device_types="cuda")
+def swiglu_linear_bwd_op(x: Tensor, weight: Tensor, dy: Tensor, want_x: bool, want_w: bool) -> Tuple[Tensor, Tensor]:
+    """(dx, dw), each empty where not wanted."""
+    lib = hip_library()
+    code, (N, C, I) = _code(x), _projection(x, weight)
+    _like(dy, (*x.shape[:-1], I), x, "dy")
+    x, weight, dy = _c(x), _c(weight), _c(dy.to(x.dtype))
+    dx = x.new_empty(x.shape if want_x else (0,))
+    dw = x.new_empty(weight.shape if want_w else (0,))
+    if N == 0:
+        return dx, dw.zero_()
+    scratch = _projection_scratch(x, 1, N, C, I)
+    with torch.cuda.device(x.device):
+        rc = lib.ebr_block_swiglu_linear_bwd(
+            code, N, C, I, x.data_ptr(), weight.data_ptr(), dy.data_ptr(), dx.data_ptr() if want_x else 0,
+            dw.data_ptr() if want_w else 0, scratch.data_ptr(), _stream(x),
+        )  # fmt: skip
+    _capi.check(rc, "ebr_block_swiglu_linear_bwd")
+    return dx, dw
+
+
+@swiglu_linear_bwd_op.register_fake
+def _(x, weight, dy, want_x, want_w):
+    return x.new_empty(x.shape if want_x else (0,)), x.new_empty(weight.shape if want_w else (0,))
+
+
+@torch.library.custom_op("ebr_fused::block_swiglu_linear_bwd2", mutates_args=(), device_types="cuda")
+def swiglu_linear_bwd2_op(x: Tensor, weight: Tensor, dy: Tensor, c: Tensor, want_x: bool,
+                          want_w: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(gx, gdy, gw) of <c, dx>; gx and gw empty where not wanted."""
+    lib = hip_library()
+    code, (N, C, I) = _code(x), _projection(x, weight)
+    _like(dy, (*x.shape[:-1], I), x, "dy")
+    _like(c, x.shape, x, "c")
+    x, weight, dy, c = _c(x), _c(weight), _c(dy.to(x.dtype)), _c(c.to(x.dtype))
+    gx = x.new_empty(x.shape if want_x else (0,))
+    gw = x.new_empty(weight.shape if want_w else (0,))
+    gdy = torch.empty_like(dy)
+    if N == 0:
+        return gx, gdy, gw.zero_()
+    scratch = _projection_scratch(x, 2, N, C, I)
+    with torch.cuda.device(x.device):
+        rc = lib.ebr_block_swiglu_linear_bwd2(
+            code, N, C, I, x.data_ptr(), weight.data_ptr(), dy.data_ptr(), c.data_ptr(), gx.data_ptr() if want_x else 0,
+            gdy.data_ptr(), gw.data_ptr() if want_w else 0, scratch.data_ptr(), _stream(x),
+        )  # fmt: skip
+    _capi.check(rc, "ebr_block_swiglu_linear_bwd2")
+    return gx, gdy, gw
+
+
+@swiglu_linear_bwd2_op.register_fake
+def _(x, weight, dy, c, want_x, want_w):
+    return (x.new_empty(x.shape if want_x else (0,)), torch.empty_like(dy, memory_format=torch.contiguous_format),
+            x.new_empty(weight.shape if want_w else (0,)))
+
+
+class _SwiGLULinearBwd2(torch.autograd.Function):
+    """A node of its own, so that a third derivative is an error: without it the gradients would pass for constants."""
+
+    @staticmethod
+    def forward(x, w, dy, c, want_x, want_w):
+        gx, gdy, gw = torch.ops.ebr_fused.block_swiglu_linear_bwd2(x, w, dy, c, want_x, want_w)
+        return gx if want_x else None, gdy, gw if want_w else None
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("trying to differentiate twice a function that was marked with @once_differentiable: "
+                           "swiglu_linear has no third derivative")
+
+
+class _SwiGLULinearDx(torch.autograd.Function):
+    """dx alone, as a node of its own."""
+
+    @staticmethod
+    def forward(x, w, dy):
+        return torch.ops.ebr_fused.block_swiglu_linear_bwd(x, w, dy, True, False)[0]
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(*inputs)
+
+    @staticmethod
+    def backward(ctx, c):
+        x, w, dy = ctx.saved_tensors
+        gx, gdy, gw = _SwiGLULinearBwd2.apply(x, w, dy, c, linear._needed(ctx, 0), linear._needed(ctx, 1))
+        return gx, gw, gdy
+
+
+def _projection_grads(x, w, dy, want_x, want_w):
+    """(dx, dw). Under create_graph the weight's gradient, and the input's beside it, are taken of the parts, each with
+    derivatives of its own: the weight's own derivatives are then theirs."""
+    if torch.is_grad_enabled() and want_w:
+        dgu = _SwiGLUBwd.apply(linear._Linear.apply(x, w), dy)
+        return linear._Dgrad.apply(dgu, w) if want_x else None, linear.weight_grad(dgu, x)
+    if torch.is_grad_enabled() and want_x:
+        return _SwiGLULinearDx.apply(x, w, dy), None
+    dx, dw = torch.ops.ebr_fused.block_swiglu_linear_bwd(x, w, dy, want_x, want_w)
+    return dx if want_x else None, dw if want_w else None
+
+
+class _SwiGLULinear(torch.autograd.Function):
+    @staticmethod
+    def forward(x, w):
+        return torch.ops.ebr_fused.block_swiglu_linear(x, w)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(*inputs)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        return _projection_grads(x, w, dy, linear._needed(ctx, 0), linear._needed(ctx, 1))
+
+
+@_host.gradient("swiglu_linear")
+def _swiglu_linear_grads(x, w, dy, want_x, want_w):
+    return _projection_grads(x, w, dy, want_x, want_w)
+
+
+@_host.gradient("swiglu_linear_dx")
+def _swiglu_linear_dx_grads(x, w, dy, c, want_x, want_w):
+    gx, gdy, gw = _SwiGLULinearBwd2.apply(x, w, dy, c, want_x, want_w)
+    return gx, gw, gdy
+
+
+def swiglu_linear(x: Tensor, weight: Tensor) -> Tensor:
+    """``swiglu(x @ weight.T)`` for x [..., C] and a weight [2 I, C] of its dtype, the gate's rows first: both projections,
+    the activation and the product in one kernel, [..., I]. The projections are summed in fp32 (fp64 for fp64) and never
+    rounded or kept: the derivatives take them again from x. Differentiable twice."""
+    host = None if torch.compiler.is_compiling() else _host.module()
+    y = None if host is None else host.swiglu_linear(x, weight)
+    if y is not None:
+        return y
+    _code(x), _projection(x, weight)
+    return _SwiGLULinear.apply(x, weight)
+
+
 def rms_norm(x: Tensor, eps: float) -> Tensor:
     """Unit RMS over the last dim (statistics in fp32), differentiable twice."""
     host = _host.module()
@@ -577,5 +994,7 @@ def swiglu(gate_up: Tensor) -> Tensor:
 rms_norm = torch._dynamo.allow_in_graph(rms_norm)
 swiglu = torch._dynamo.allow_in_graph(swiglu)
 group_norm = torch._dynamo.allow_in_graph(group_norm)
+layer_norm = torch._dynamo.allow_in_graph(layer_norm)
+swiglu_linear = torch._dynamo.allow_in_graph(swiglu_linear)
 
-__all__ = ["add_rms_norm", "group_norm", "rms_norm", "swiglu"]
+__all__ = ["add_rms_norm", "group_norm", "layer_norm", "rms_norm", "swiglu", "swiglu_linear"]

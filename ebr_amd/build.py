@@ -26,7 +26,7 @@ ARCH = "gfx950"
 
 SOURCES = [CSRC / "ebr_attn.hip", CSRC / "ebr_rope.hip", CSRC / "ebr_descent.hip", CSRC / "ebr_block.hip",
            CSRC / "ebr_embed.hip", CSRC / "ebr_distill.hip", CSRC / "ebr_groupnorm.hip",
-           CSRC / "ebr_noalloc.hip"]
+           CSRC / "ebr_layernorm.hip", CSRC / "ebr_glu.hip", CSRC / "ebr_optim.hip", CSRC / "ebr_noalloc.hip"]
 HEADERS = [
     CSRC / "attn_tiles.hpp",
     CSRC / "attn_resident.hpp",
@@ -35,6 +35,7 @@ HEADERS = [
     ROOT / "include" / "ebr_rope.h",
     ROOT / "include" / "ebr_descent.h",
     ROOT / "include" / "ebr_block.h",
+    ROOT / "include" / "ebr_optim.h",
     CSRC / "attn_f64.hpp",
     CSRC / "rowwise.hpp",
 ]

@@ -1,0 +1,703 @@
+// The gated projection y = silu(x Wg^T) * (x Wu^T) on gfx950, with its first and second derivatives (C ABI and formulas:
+// include/ebr_block.h): products on the matrix cores with the activation, or its second derivative, in their epilogues.
+//
+// Every product is D[j][i] = sum over k of A(i, k) B(j, k), i being the direction in which D lies in memory. An operand lies
+// with its rows' k side by side (K), or with its rows side by side for each k (M):
+//   [g|u] = x W^T     A = W (K), rows of gate and up in turns of 32, so that a lane holds both at the same place; B = x (K).
+//                     With B = rows of x and of c in turns of 32, a lane holds [cg|cu] = c W^T there as well
+//   dx = [dg|du] W    A = W (M), B = [dg|du] (K)
+//   dW = [dg|du]^T x  A = x (M), B = [dg|du] (M), the rows split among workgroups, partial sums added up in a fixed order
+//
+// The derivatives take g and u again: kept rounded they would double the gradients' errors, and of C below about a thousand
+// the product costs less than moving them.
+//
+// A workgroup's tile of TI x TJ steps through k in stages of 128 bytes an operand row, each stage loaded straight into shared
+// memory while the one before is multiplied. The two buffers are separate arrays: the compiler then knows that the loads
+// under way do not concern the reads, and does not wait for them. Rows' 16-byte chunks (64-byte chunks for operands of the
+// second kind, which are read transposed) are exchanged by a function of the row, so that lanes meet no bank conflicts.
+// Whatever lies outside the tensors is read as zero by the buffer loads' bounds.
+#include <type_traits>
+#include <utility>
+
+#include "../../include/ebr_block.h"
+#include "rowwise.hpp"
+
+namespace ebr_glu {
+
+using namespace ebr_row;
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+#define EBR_LDS __attribute__((address_space(3)))
+
+enum { K_ROWS = 0, M_ROWS = 1 };                                  // how an operand lies
+enum { EP_OUT = 0, EP_PART = 1, EP_FWD = 2, EP_BWD = 3, EP_BWD2 = 4 };  // what becomes of D: y, [dg|du], or all of bwd2's
+constexpr int STAGE = 128;                                        // bytes of k a stage
+constexpr uint32_t OUTSIDE = 0x40000000;                          // an offset past a buffer's end
+
+struct Args {
+    const void *a[4], *b[4];  // pairs: the sum goes over the k of all of them, one after the other
+    int64_t lda, ldb;         // elements between rows (of k, for M)
+    int64_t ni, nj, nk;       // rows of A (gated: of the gate), of B, and k of one pair
+    int pairs, splits;
+    int64_t steps;            // stages of a split
+    int ti, tj;               // tiles
+    void *out, *dgu, *ggu;    // D, y or gdy; [dg|du]; [gg|gu]
+    void *dgu2, *ggu2;        // what these lack of their values before rounding, or null
+    const void *dy, *c;
+    int64_t ldo;
+};
+
+template <typename T> struct Mma;
+template <> struct Mma<__bf16> {
+    static __device__ __forceinline__ f32x16 step(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<_Float16> {
+    static __device__ __forceinline__ f32x16 step(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<float> {  // four values of k a lane, one a step
+    static __device__ __forceinline__ f32x16 step(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, (uint32_t)a[e]),
+                                                     __builtin_bit_cast(float, (uint32_t)b[e]), c, 0, 0, 0);
+        return c;
+    }
+};
+
+// One operand's part of a workgroup: ROWS rows, of which WAVES waves load their share.
+template <typename T, int LIES, int ROWS, int WAVES, bool PAIRED> struct Side {
+    static constexpr int ES = (int)sizeof(T), EPC = 16 / ES, KS = STAGE / ES;  // elements of a chunk, k of a stage
+    static constexpr int BYTES = ROWS * STAGE, LOADS = BYTES / 1024 / WAVES;
+    static constexpr int ROWB = LIES == K_ROWS ? STAGE : ROWS * ES;  // bytes of a row in shared memory
+    static constexpr int MASK = ROWB / 64 >= 4 ? 3 : ROWB / 64 - 1;
+    static_assert(BYTES % (1024 * WAVES) == 0, "whole loads a wave");
+
+    // The chunk (16 bytes) that lies at place p of a stage: its row (K) or k (M), and its first element there.
+    static __device__ __forceinline__ void chunk(int p, int& row, int& at) {
+        row = p * 16 / ROWB;
+        const int c = p - row * (ROWB / 16);
+        if constexpr (LIES == K_ROWS) at = (c ^ ((row >> 1) & 7)) * EPC;
+        else at = ((((c >> 2) ^ (row & MASK)) << 2) | (c & 3)) * EPC;
+    }
+    // Row r of the tile that begins at row ``first``, in the operand, or -1 where there is none. PAIRED: rows of the two
+    // operands of a pair in turns of 32, the same ones of each.
+    static __device__ __forceinline__ int64_t source(int r, int64_t first, int64_t n) {
+        const int64_t i = PAIRED ? first / 2 + (r >> 6) * 32 + (r & 31) : first + r;
+        return i < n ? i : -1;
+    }
+    static __device__ __forceinline__ bool other(int r) { return PAIRED && ((r >> 5) & 1); }
+
+    // This lane's byte offsets from the tile's place at the stage's k, past the end where a row is missing.
+    uint32_t off[LOADS];
+    int kat[LOADS];  // the k of its first element in a stage
+    __device__ __forceinline__ void offsets(int64_t first, int64_t n, int64_t ld, int wave, int lane) {
+#pragma unroll
+        for (int q = 0; q < LOADS; ++q) {
+            int row, at;
+            chunk((wave * LOADS + q) * 64 + lane, row, at);
+            if constexpr (LIES == K_ROWS) {
+                const int64_t s = source(row, first, n);
+                off[q] = s < 0 ? OUTSIDE : (uint32_t)(((s - (PAIRED ? first / 2 : first)) * ld + at) * ES);
+                kat[q] = at;
+            } else {
+                off[q] = first + at < n ? (uint32_t)((row * ld + at) * ES) : OUTSIDE;
+                kat[q] = row;
+            }
+        }
+    }
+    // Loads the stage at k0, of which ``rest`` k are left, into ``to``.
+    __device__ __forceinline__ void load(const T* base, const T* base2, int64_t first, int64_t ld, int64_t k0, int64_t rest,
+                                         unsigned char* to, int wave) const {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass has no buffers)
+        constexpr int RAW = 0x00020000;  // dwords as they are
+        const int64_t skip = LIES == K_ROWS ? (PAIRED ? first / 2 : first) * ld + k0 : first + k0 * ld;
+        const int left = rest < KS ? (int)rest : KS;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + skip), 0, (int)OUTSIDE, RAW);
+        __amdgpu_buffer_rsrc_t r2 = r;
+        if constexpr (PAIRED) r2 = __builtin_amdgcn_make_buffer_rsrc((void*)(base2 + skip), 0, (int)OUTSIDE, RAW);
+#pragma unroll
+        for (int q = 0; q < LOADS; ++q) {
+            const int at = wave * LOADS + q;  // (a load's 8 rows are of one operand)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(other(at * 8) ? r2 : r, (EBR_LDS void*)(to + at * 1024), 16,
+                                                     kat[q] < left ? off[q] : OUTSIDE, 0, 0, 0);
+        }
+#endif
+    }
+    // The same for operands of any alignment and width, through registers.
+    static __device__ __forceinline__ void load_any(const T* base, const T* base2, int64_t first, int64_t n, int64_t ld,
+                                                    int64_t k0, int64_t nk, unsigned char* to) {
+        for (int p = threadIdx.x; p < BYTES / 16; p += WAVES * 64) {
+            int row, at;
+            chunk(p, row, at);
+            T v[EPC];
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) {
+                v[e] = (T)0.f;
+                if constexpr (LIES == K_ROWS) {
+                    const int64_t s = source(row, first, n);
+                    if (s >= 0 && k0 + at + e < nk) v[e] = (other(row) ? base2 : base)[s * ld + k0 + at + e];
+                } else {
+                    if (k0 + row < nk && first + at + e < n) v[e] = base[(k0 + row) * ld + first + at + e];
+                }
+            }
+            __builtin_memcpy(to + p * 16, v, 16);
+        }
+    }
+    // The 32 rows from r0 (a multiple of 32) at step s of a stage: lane (row l % 32, half l / 32) gets EPC values of k.
+    static __device__ __forceinline__ u32x4 read(const unsigned char* from, int r0, int s, int lane) {
+        const int l32 = lane & 31, half = lane >> 5;
+        if constexpr (LIES == K_ROWS) {
+            const int row = r0 + l32;
+            return *reinterpret_cast<const u32x4*>(from + row * ROWB + (((2 * s + half) ^ ((row >> 1) & 7)) << 4));
+        } else if constexpr (ES == 2) {
+            const int l16 = lane & 15, k = 16 * s + 8 * half + (l16 >> 2), col = (r0 + (lane & 16) + 4 * (l16 & 3)) * ES;
+            const unsigned char* p = from + k * ROWB + ((((col >> 6) ^ (k & MASK)) << 6) | (col & 63));
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((EBR_LDS s16x4*)p));
+            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((EBR_LDS s16x4*)(p + 4 * ROWB)));
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        } else {
+            u32x4 v;
+            const int col = (r0 + l32) * ES;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = 8 * s + 4 * half + e;
+                v[e] = *reinterpret_cast<const uint32_t*>(from + k * ROWB + ((((col >> 6) ^ (k & MASK)) << 6) | (col & 63)));
+            }
+            return v;
+        }
+    }
+};
+
+template <typename A> __device__ __forceinline__ A sigmoid(A g);
+template <> __device__ __forceinline__ float sigmoid(float g) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896f * g));
+}
+template <> __device__ __forceinline__ double sigmoid(double g) { return 1.0 / (1.0 + exp(-g)); }
+
+template <typename A> __device__ __forceinline__ A gated(A g, A u) { return g * sigmoid(g) * u; }
+// Its gradients for g and u, and those of <c, (dg, du)> for g, u and dy.
+template <typename A> __device__ __forceinline__ void first_of(A g, A u, A dy, A& dg, A& du) {
+    const A s = sigmoid(g);
+    dg = dy * u * (s * ((A)1 + g * ((A)1 - s)));
+    du = dy * (g * s);
+}
+template <typename A>
+__device__ __forceinline__ void second_of(A g, A u, A dy, A cg, A cu, A& gg, A& gu, A& gdy) {
+    const A s = sigmoid(g), f1 = s * ((A)1 + g * ((A)1 - s)), f2 = s * ((A)1 - s) * ((A)2 + g * ((A)1 - (A)2 * s));
+    gg = dy * (cg * u * f2 + cu * f1);
+    gu = cg * dy * f1;
+    gdy = cg * u * f1 + cu * (g * s);
+}
+
+// Four neighbours at p, of which ``n`` exist.
+template <typename T> __device__ __forceinline__ void put4(T* p, const float (&v)[4], int64_t n, bool whole) {
+    if (whole && n >= 4) {
+        Pack<T, 4> x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.e[e] = (T)v[e];
+        stp<T, 4>(p, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < n) p[e] = (T)v[e];
+    }
+}
+// What two fours lack of their values once rounded.
+template <typename T>
+__device__ __forceinline__ void put_rest(T* p, const float (&g)[4], const float (&u)[4], int64_t next, int64_t n, bool whole) {
+    float rg[4], ru[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        rg[e] = g[e] - (float)(T)g[e];
+        ru[e] = u[e] - (float)(T)u[e];
+        if (!__builtin_isfinite(rg[e])) rg[e] = 0.f;  // (of a value past the type's range)
+        if (!__builtin_isfinite(ru[e])) ru[e] = 0.f;
+    }
+    put4(p, rg, n, whole);
+    put4(p + next, ru, n, whole);
+}
+template <typename T> __device__ __forceinline__ void get4(const T* p, float (&v)[4], int64_t n, bool whole) {
+    if (whole && n >= 4) {
+        const Pack<T, 4> x = ldp<T, 4>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)x.e[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+    }
+}
+
+// All of a wave's memory operations done, and every wave there.
+__device__ __forceinline__ void stage_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The tile of a workgroup: each of the 8 XCDs, which take workgroups in turns, gets neighbouring tiles, and of those a block
+// of GROUP tiles of j goes with all i before the next.
+__device__ __forceinline__ void tile_of(const Args& a, int& ti, int& tj, int& split) {
+    constexpr int GROUP = 8;
+    const unsigned tiles = (unsigned)a.ti * a.tj, all = tiles * a.splits, b = blockIdx.x;
+    const unsigned per = all / 8, more = all % 8, x = b % 8;
+    const unsigned at = x * per + (x < more ? x : more) + b / 8;
+    split = (int)(at / tiles);
+    const unsigned t = at % tiles, block = t / (GROUP * a.ti), first = block * GROUP;
+    const unsigned rows = a.tj - first < GROUP ? a.tj - first : GROUP, in = t - block * GROUP * a.ti;
+    tj = (int)(first + in % rows);
+    ti = (int)(in / rows);
+}
+
+template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int WJ, bool ANY>
+__global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
+    constexpr int WAVES = WI * WJ, FI = TI / WI / 32, FJ = TJ / WJ / 32;
+    constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
+    static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
+    using SA = Side<T, ALIES, TI, WAVES, GATED>;
+    using SB = Side<T, BLIES, TJ, WAVES, TWO>;
+    __shared__ __attribute__((aligned(16))) unsigned char a0[SA::BYTES], b0[SB::BYTES];
+    __shared__ __attribute__((aligned(16))) unsigned char a1[ANY ? 16 : SA::BYTES], b1[ANY ? 16 : SB::BYTES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave % WI, wj = wave / WI;
+    int ti, tj, split;
+    tile_of(a, ti, tj, split);
+    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
+    f32x16 acc[FI][FJ];
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    const int64_t one = (a.nk + SA::KS - 1) / SA::KS, all = one * a.pairs;  // stages of a pair
+    int64_t step = split * a.steps;
+    const int64_t end = step + a.steps < all ? step + a.steps : all;
+    const auto multiply = [&](const unsigned char* pa, const unsigned char* pb) {
+        u32x4 fa[2][FI], fb[2][FJ];
+        const auto fragments = [&](int s) {
+#pragma unroll
+            for (int i = 0; i < FI; ++i) fa[s & 1][i] = SA::read(pa, (wi * FI + i) * 32, s, lane);
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) fb[s & 1][j] = SB::read(pb, (wj * FJ + j) * 32, s, lane);
+        };
+        fragments(0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s < 3) fragments(s + 1);
+#pragma unroll
+            for (int i = 0; i < FI; ++i)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j) acc[i][j] = Mma<T>::step(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);  // (all fragments of a stage at once would not fit the registers)
+        }
+    };
+    if constexpr (ANY) {
+        for (; step < end; ++step) {
+            const int pair = (int)(step / one);
+            const int64_t k0 = (step - pair * one) * SA::KS;
+            __syncthreads();
+            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
+            SA::load_any(pa, pa + a.ni * a.lda, i0, a.ni, a.lda, k0, a.nk, a0);
+            SB::load_any(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.nj, a.ldb, k0, a.nk, b0);
+            __syncthreads();
+            multiply(a0, b0);
+        }
+    } else {
+        SA sa;
+        SB sb;
+        sa.offsets(i0, a.ni, a.lda, wave, lane);
+        sb.offsets(j0, a.nj, a.ldb, wave, lane);
+        // Stages in twos, the last one of an odd number with one of zeros (which costs a stage's products, but a branch out of
+        // the loop's middle would cost a second copy of all sums).
+        const auto load = [&](unsigned char* la, unsigned char* lb) {
+            const bool in = step < end;
+            const int64_t at = in ? step : end - 1;
+            const int pair = (at >= one) + (at >= 2 * one) + (at >= 3 * one);
+            const int64_t k0 = (at - pair * one) * SA::KS, left = in ? a.nk - k0 : 0;
+            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
+            sa.load(pa, pa + a.ni * a.lda, i0, a.lda, k0, left, la, wave);
+            sb.load(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.ldb, k0, left, lb, wave);
+            ++step;
+        };
+        const int64_t n = end - step;
+        load(a0, b0);
+        stage_barrier();
+        for (int64_t s = 0; s < n; s += 2) {
+            load(a1, b1);
+            multiply(a0, b0);
+            stage_barrier();
+            load(a0, b0);
+            multiply(a1, b1);
+            stage_barrier();
+        }
+    }
+
+    const int64_t jl = j0 + wj * FJ * 32 + (lane & 31);
+    const int il = 4 * (lane >> 5);
+    if constexpr (!GATED) {
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) {
+            const int64_t row = jl + j * 32;
+            if (row >= a.nj) continue;
+#pragma unroll
+            for (int i = 0; i < FI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int64_t col = i0 + (wi * FI + i) * 32 + 8 * q + il;
+                    const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    if (col >= a.ni) continue;
+                    if constexpr (EP == EP_OUT) {
+                        put4(reinterpret_cast<T*>(a.out) + row * a.ldo + col, v, a.ni - col, !ANY);
+                    } else {
+                        float* p = reinterpret_cast<float*>(a.out) + (split * a.nj + row) * a.ni + col;
+                        put4(p, v, a.ni - col, !ANY);
+                    }
+                }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < FJ; j += TWO ? 2 : 1) {
+            const int64_t row = TWO ? j0 / 2 + (wj * FJ + j) * 16 + (lane & 31) : jl + j * 32;
+            if (row >= a.nj) continue;
+#pragma unroll
+            for (int i = 0; i < FI; i += 2)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int64_t col = i0 / 2 + (wi * FI + i) * 16 + 8 * q + il;
+                    if (col >= a.ni) continue;
+                    const int64_t n = a.ni - col, at = row * a.ni + col, two = row * 2 * a.ni + col;
+                    T* const dgu = reinterpret_cast<T*>(a.dgu) + two;
+                    T* const ggu = reinterpret_cast<T*>(a.ggu) + two;
+                    float dy[4], og[4], ou[4], o[4];
+                    if constexpr (EP != EP_FWD) get4(reinterpret_cast<const T*>(a.dy) + at, dy, n, !ANY);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float g = acc[i][j][4 * q + e], u = acc[i + 1][j][4 * q + e];
+                        if constexpr (EP == EP_FWD) o[e] = gated(g, u);
+                        else first_of(g, u, dy[e], og[e], ou[e]);
+                    }
+                    if constexpr (EP == EP_FWD) put4(reinterpret_cast<T*>(a.out) + at, o, n, !ANY);
+                    if (EP == EP_BWD || (TWO && a.dgu)) {
+                        put4(dgu, og, n, !ANY);
+                        put4(dgu + a.ni, ou, n, !ANY);
+                        if (a.dgu2) put_rest(reinterpret_cast<T*>(a.dgu2) + two, og, ou, a.ni, n, !ANY);
+                    }
+                    if constexpr (TWO) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            second_of(acc[i][j][4 * q + e], acc[i + 1][j][4 * q + e], dy[e], acc[i][j + 1][4 * q + e],
+                                      acc[i + 1][j + 1][4 * q + e], og[e], ou[e], o[e]);
+                        put4(reinterpret_cast<T*>(a.out) + at, o, n, !ANY);
+                        if (a.ggu) {
+                            put4(ggu, og, n, !ANY);
+                            put4(ggu + a.ni, ou, n, !ANY);
+                            if (a.ggu2) put_rest(reinterpret_cast<T*>(a.ggu2) + two, og, ou, a.ni, n, !ANY);
+                        }
+                    }
+                }
+        }
+    }
+}
+
+// fp64, for gradient checks: 64 x 64 of D (gated: of each half, and of both right operands) a workgroup, 4 x 4 a thread.
+template <int ALIES, int BLIES, int EP> __global__ __launch_bounds__(256) void k_product64(Args a) {
+    constexpr int NA = EP >= EP_FWD ? 2 : 1, NB = EP == EP_BWD2 ? 2 : 1;
+    __shared__ double la[NA][16][65], lb[NB][16][65];
+    const int ti = blockIdx.x % a.ti, tj = blockIdx.x / a.ti;
+    const int64_t i0 = (int64_t)ti * 64, j0 = (int64_t)tj * 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    double acc[NB][NA][4][4] = {};
+    for (int pair = 0; pair < a.pairs; ++pair) {
+        const double* pa = reinterpret_cast<const double*>(a.a[pair]);
+        const double* pb[2] = {reinterpret_cast<const double*>(a.b[pair]), reinterpret_cast<const double*>(a.c)};
+        for (int64_t k0 = 0; k0 < a.nk; k0 += 16) {
+            __syncthreads();
+            for (int p = threadIdx.x; p < 1024; p += 256) {
+                const int r = p & 63, k = p >> 6;
+                const bool in = k0 + k < a.nk;
+                for (int h = 0; h < NA; ++h) {
+                    const int64_t row = i0 + r + h * a.ni;
+                    la[h][k][r] = in && i0 + r < a.ni ? pa[ALIES == K_ROWS ? row * a.lda + k0 + k : (k0 + k) * a.lda + row] : 0.0;
+                }
+                const int64_t row = j0 + r;
+                for (int h = 0; h < NB; ++h)
+                    lb[h][k][r] = in && row < a.nj ? pb[h][BLIES == K_ROWS ? row * a.ldb + k0 + k : (k0 + k) * a.ldb + row] : 0.0;
+            }
+            __syncthreads();
+            for (int k = 0; k < 16; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        for (int f = 0; f < NB; ++f)
+                            for (int h = 0; h < NA; ++h) acc[f][h][i][j] += la[h][k][tx + 16 * i] * lb[f][k][ty + 16 * j];
+        }
+    }
+    double *const out = reinterpret_cast<double*>(a.out), *const dgu = reinterpret_cast<double*>(a.dgu);
+    double* const ggu = reinterpret_cast<double*>(a.ggu);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t row = j0 + ty + 16 * j, col = i0 + tx + 16 * i;
+            if (row >= a.nj || col >= a.ni) continue;
+            const int64_t at = row * a.ni + col, two = row * 2 * a.ni + col;
+            const double g = acc[0][0][i][j], u = acc[0][NA - 1][i][j];
+            if constexpr (EP < EP_FWD) out[row * a.ldo + col] = g;
+            if constexpr (EP == EP_FWD) out[at] = gated(g, u);
+            if constexpr (EP > EP_FWD) {
+                const double dy = reinterpret_cast<const double*>(a.dy)[at];
+                double og, ou, o;
+                if (a.dgu) first_of(g, u, dy, dgu[two], dgu[two + a.ni]);
+                if constexpr (EP == EP_BWD2) {
+                    second_of(g, u, dy, acc[NB - 1][0][i][j], acc[NB - 1][1][i][j], og, ou, o);
+                    out[at] = o;
+                    if (a.ggu) {
+                        ggu[two] = og;
+                        ggu[two + a.ni] = ou;
+                    }
+                }
+            }
+        }
+}
+
+// The splits' partial sums added up, in their order.
+template <typename T> __global__ __launch_bounds__(256) void k_join(const float* part, int splits, int64_t n, T* out) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+        float s[4] = {0, 0, 0, 0}, v[4];
+        for (int k = 0; k < splits; ++k) {
+            const float* p = part + k * n + i;
+            get4(p, v, n - i, n % 4 == 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += v[e];
+        }
+        put4(out + i, s, n - i, n % 4 == 0);
+    }
+}
+
+// -- launches ----------------------------------------------------------------------------------------------------------
+
+static int size_of(int dtype) { return dtype == EBR_DTYPE_F64 ? 8 : dtype == EBR_DTYPE_F32 ? 4 : 2; }
+static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
+
+static int check(int dtype, int64_t N, int64_t C, int64_t I) {
+    if (!known(dtype)) return EBR_ERR_DTYPE;
+    if (N < 1 || C < 1 || I < 1 || N >= ((int64_t)1 << 31) || C >= (1 << 20) || I >= (1 << 20)) return EBR_ERR_SHAPE;
+    const auto tiles = [](int64_t n) { return (n + 63) / 64; };  // (a launch holds fewer than 2^32 threads)
+    const int64_t most = tiles(2 * I) > tiles(C) ? tiles(2 * I) : tiles(C);
+    return tiles(2 * N) * most > MAX_BLOCKS || tiles(2 * I) * tiles(C) > MAX_BLOCKS ? EBR_ERR_SHAPE : EBR_OK;
+}
+
+// The tiles that a product is cut into, from its sizes alone.
+struct Cut {
+    int tile;            // 256, 128 or 64
+    int64_t ti, tj;
+    int splits = 1;
+    int64_t steps;
+    Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, bool split, bool any) {  // gated: 0, 1, or 2 for TWO
+        const auto up = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
+        const int64_t wide = gated ? 2 * ni : ni, high = gated == 2 ? 2 * nj : nj, all = up(nk, STAGE / size_of(dtype)) * pairs;
+        tile = 256;
+        if (dtype == EBR_DTYPE_F64) tile = 64;
+        else if (dtype == EBR_DTYPE_F32 || any) tile = 128;
+        const auto tiles = [&](int t) { return up(wide, t) * up(high, t); };
+        if (dtype != EBR_DTYPE_F64) {
+            if (tile == 256 && tiles(256) < (split ? 4 : 200)) tile = 128;
+            if (tile == 128 && tiles(128) < (split ? 8 : 200)) tile = 64;
+        }
+        ti = dtype == EBR_DTYPE_F64 ? up(ni, 64) : up(wide, tile);
+        tj = dtype == EBR_DTYPE_F64 ? up(nj, 64) : up(high, tile);
+        steps = all;
+        if (split && dtype != EBR_DTYPE_F64) {
+            const int64_t want = up(tile == 256 ? 256 : 512, ti * tj), most = up(all, 4);
+            splits = (int)(want < most ? want : most);
+            if (splits < 1) splits = 1;
+            steps = up(all, splits);
+            splits = (int)up(all, steps);
+        }
+    }
+};
+
+template <typename T, int ALIES, int BLIES, int EP, bool ANY> static void launch(hipStream_t s, const Cut& c, const Args& a) {
+    const dim3 grid((unsigned)(c.ti * c.tj * c.splits));
+    if constexpr (std::is_same_v<T, double>) {
+        hipLaunchKernelGGL((k_product64<ALIES, BLIES, EP>), grid, dim3(256), 0, s, a);
+    } else {
+        if constexpr (!ANY && sizeof(T) == 2) {
+            if (c.tile == 256) {
+                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 4, 2, ANY>), grid, dim3(512), 0, s, a);
+                return;
+            }
+        }
+        if (c.tile == 128) hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 128, 128, 2, 2, ANY>), grid, dim3(256), 0, s, a);
+        else if constexpr (EP == EP_BWD2)
+            hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 1, ANY>), grid, dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 2, ANY>), grid, dim3(128), 0, s, a);
+    }
+}
+
+// One product, whose operands, strides, sizes and outputs ``a`` holds.
+template <int ALIES, int BLIES, int EP> static void product(int dtype, bool any, const Cut& c, Args a, hipStream_t s) {
+    a.ti = (int)c.ti, a.tj = (int)c.tj, a.splits = c.splits, a.steps = c.steps;
+    const auto with = [&](auto v) {
+        using T = decltype(v);
+        if (any) launch<T, ALIES, BLIES, EP, true>(s, c, a);
+        else launch<T, ALIES, BLIES, EP, false>(s, c, a);
+    };
+    switch (dtype) {
+        case EBR_DTYPE_F32: with(float()); break;
+        case EBR_DTYPE_BF16: with(__bf16()); break;
+        case EBR_DTYPE_F16: with(_Float16()); break;
+        default: launch<double, ALIES, BLIES, EP, true>(s, c, a); break;
+    }
+}
+
+// Whether tensors of these widths (elements of a row) go by the whole 16-byte chunk.
+static bool whole(int dtype, std::initializer_list<int64_t> widths, std::initializer_list<const void*> ps) {
+    const int per = 16 / size_of(dtype);
+    for (const int64_t w : widths)
+        if (w % per || w >= (1 << 20)) return false;
+    for (const void* p : ps)
+        if (!aligned(p, 16)) return false;
+    return true;
+}
+
+// [dg|du] or [gg|gu], rounded, and what they lack where the products take that as well: of few rows a weight's gradient adds up
+// few products, and shows their roundings.
+struct Grads {
+    const void *g, *rest;
+};
+static bool with_rest(int dtype, int64_t N) { return size_of(dtype) == 2 && N <= 64; }
+
+// dx of dgu, and dw of (x, dgu) and, where there is one, a second pair.
+static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w, Grads dgu, void* dx, hipStream_t s) {
+    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, 2 * I}, {w, dgu.g, dgu.rest, dx});
+    Args a = {};
+    a.a[0] = a.a[1] = w, a.b[0] = dgu.g, a.b[1] = dgu.rest, a.pairs = dgu.rest ? 2 : 1;
+    a.lda = C, a.ldb = 2 * I, a.ni = C, a.nj = N, a.nk = 2 * I, a.out = dx, a.ldo = C;
+    product<M_ROWS, K_ROWS, EP_OUT>(dtype, any, Cut(dtype, C, N, 2 * I, a.pairs, 0, false, any), a, s);
+}
+
+static Cut weight_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs, bool any) {
+    return Cut(dtype, C, 2 * I, N, pairs, 0, true, any);
+}
+static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* x, Grads dgu, const void* x2, Grads dgu2, void* dw,
+                        float* part, hipStream_t s) {
+    Args a = {};
+    bool fit = true;
+    for (const auto& [of, grads] : {std::pair<const void*, Grads>(x, dgu), std::pair<const void*, Grads>(x2, dgu2)})
+        for (const void* g : {grads.g, grads.rest})
+            if (g) {
+                fit = fit && whole(dtype, {}, {of, g});
+                a.a[a.pairs] = of, a.b[a.pairs++] = g;
+            }
+    const bool any = dtype == EBR_DTYPE_F64 || !fit || !whole(dtype, {C, 2 * I}, {dw});
+    const Cut c = weight_cut(dtype, N, C, I, a.pairs, any);
+    a.lda = C, a.ldb = 2 * I, a.ni = C, a.nj = 2 * I, a.nk = N, a.out = dw, a.ldo = C;
+    if (c.splits == 1) {
+        product<M_ROWS, M_ROWS, EP_OUT>(dtype, any, c, a, s);
+        return;
+    }
+    a.out = part;
+    product<M_ROWS, M_ROWS, EP_PART>(dtype, any, c, a, s);
+    const int64_t n = 2 * I * C;
+    const dim3 grid(blocks_for(n, 1024));
+    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, part, c.splits, n, (__bf16*)dw);
+    else if (dtype == EBR_DTYPE_F16)
+        hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, part, c.splits, n, (_Float16*)dw);
+    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, part, c.splits, n, (float*)dw);
+}
+
+static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace ebr_glu
+
+using namespace ebr_glu;
+
+extern "C" {
+
+int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I) {
+    if (check(dtype, N, C, I) || order < 0 || order > 2) return -1;
+    if (order == 0) return 16;
+    int64_t part = 0;
+    const int64_t each = with_rest(dtype, N) ? 2 : 1;
+    for (const bool any : {false, true}) {
+        const Cut c = weight_cut(dtype, N, C, I, (int)(order * each), any);
+        const int64_t n = c.splits > 1 ? c.splits * 2 * I * C * 4 : 0;
+        part = n > part ? n : part;
+    }
+    // [dg|du], for order 2 [gg|gu] too, and the weight gradient's partial sums
+    return order * each * up16(N * 2 * I * size_of(dtype)) + part + 16;
+}
+
+int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* stream) {
+    const int rc = check(dtype, N, C, I);
+    if (rc) return rc;
+    if (!x || !w || !y) return EBR_ERR_NULL;
+    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, y});
+    Args a = {};
+    a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = y;
+    product<K_ROWS, K_ROWS, EP_FWD>(dtype, any, Cut(dtype, I, N, C, 1, 1, false, any), a, (hipStream_t)stream);
+    return launched();
+}
+
+int ebr_block_swiglu_linear_bwd(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
+                                void* dx, void* dw, void* scratch, void* stream) {
+    const int rc = check(dtype, N, C, I);
+    if (rc) return rc;
+    if (!x || !w || !dy) return EBR_ERR_NULL;
+    if (!scratch) return EBR_ERR_SCRATCH;
+    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    if (!dx && !dw) return EBR_OK;
+    hipStream_t s = (hipStream_t)stream;
+    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, dy});
+    Args a = {};
+    a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.dy = dy;
+    const int64_t rows = up16(N * 2 * I * size_of(dtype));
+    char* at = reinterpret_cast<char*>(scratch);
+    a.dgu = at, at += rows;
+    if (with_rest(dtype, N)) a.dgu2 = at, at += rows;
+    product<K_ROWS, K_ROWS, EP_BWD>(dtype, any, Cut(dtype, I, N, C, 1, 1, false, any), a, s);
+    const Grads dgu = {a.dgu, a.dgu2};
+    if (dx) input_grad(dtype, N, C, I, w, dgu, dx, s);
+    if (dw) weight_grad(dtype, N, C, I, x, dgu, nullptr, {}, dw, reinterpret_cast<float*>(at), s);
+    return launched();
+}
+
+int ebr_block_swiglu_linear_bwd2(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
+                                 const void* c, void* gx, void* gdy, void* gw, void* scratch, void* stream) {
+    const int rc = check(dtype, N, C, I);
+    if (rc) return rc;
+    if (!x || !w || !dy || !c || !gdy) return EBR_ERR_NULL;
+    if (!scratch) return EBR_ERR_SCRATCH;
+    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, dy, c, gdy});
+    Args a = {};
+    a.a[0] = w, a.b[0] = x, a.c = c, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = gdy, a.dy = dy;
+    const int64_t rows = up16(N * 2 * I * size_of(dtype));
+    char* at = reinterpret_cast<char*>(scratch);
+    for (void** to : {gx || gw ? &a.ggu : nullptr, gw ? &a.dgu : nullptr}) {
+        if (to) *to = at, at += rows;
+        if (to && with_rest(dtype, N)) *(to == &a.ggu ? &a.ggu2 : &a.dgu2) = at, at += rows;
+    }
+    product<K_ROWS, K_ROWS, EP_BWD2>(dtype, any, Cut(dtype, I, N, C, 1, 2, false, any), a, s);
+    const Grads dgu = {a.dgu, a.dgu2}, ggu = {a.ggu, a.ggu2};
+    if (gx) input_grad(dtype, N, C, I, w, ggu, gx, s);
+    if (gw) weight_grad(dtype, N, C, I, x, ggu, c, dgu, gw, reinterpret_cast<float*>(at), s);
+    return launched();
+}
+
+}  // extern "C"

@@ -1,8 +1,8 @@
 // Native host path of the GPU ops: argument checks, output allocation, autograd nodes and the launches of
 // libebr_attn.so (include/ebr_*.h) in C++, for calls on plain GPU tensors.
 //
-// The Python layer (ebr_amd/fused_attn/ops.py, rope_split.py, block.py, descent.py, linear.py, tokens.py) defines the ops, their
-// fakes and their autograd Functions, and stays the path of every call this file does not take: tensor subclasses and
+// The Python layer (ebr_amd/fused_attn/ops.py, rope_split.py, block.py, descent.py, linear.py, tokens.py, optim.py) defines the ops,
+// their fakes and their autograd Functions, and stays the path of every call this file does not take: tensor subclasses and
 // fake tensors, torch.func transforms, dispatch and function modes, tracing, forward-mode duals, saved-tensor hooks,
 // tensors off the GPU, and every argument the Python layer would refuse or pad. Each entry point below returns None for
 // those, and the caller goes on in Python. A node asks again when it runs: a backward under a transform (batched
@@ -31,11 +31,13 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 
 #include "ebr_attn.h"
 #include "ebr_block.h"
 #include "ebr_descent.h"
+#include "ebr_optim.h"
 #include "ebr_rope.h"
 
 namespace {
@@ -107,6 +109,11 @@ int dtype_code(at::ScalarType t) {
         case at::kDouble: return EBR_DTYPE_F64;
         default: return -1;
     }
+}
+
+at::ScalarType type_of(int64_t code) {
+    return code == EBR_DTYPE_F32 ? at::kFloat : code == EBR_DTYPE_BF16 ? at::kBFloat16
+         : code == EBR_DTYPE_F16 ? at::kHalf : at::kDouble;
 }
 
 bool same_kind(const Tensor& a, const Tensor& b) {
@@ -1273,14 +1280,391 @@ py::object group_norm(const py::handle& hx, int64_t groups, const py::handle& hw
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// Layer norm, differentiable twice (ebr_amd/block.py)
+// ---------------------------------------------------------------------------------------------------------------------
+
+// The dtype that a layer norm's parameters go into the kernels in, and their gradients come out: their own where they share
+// one.
+at::ScalarType param_type(const Tensor& x, const Tensor& w, const Tensor& b) {
+    if (w.defined() && b.defined()) return w.scalar_type() == b.scalar_type() ? w.scalar_type() : acc_type(x);
+    return w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : acc_type(x);
+}
+Tensor param_as(const Tensor& p, at::ScalarType t) { return p.defined() ? dense(p.to(t)) : Tensor(); }
+
+Tensor layer_scratch(const Tensor& x, int order, const RowsOf& r) {
+    const int64_t n = ebr_block_layernorm_scratch(dtype_code(x.scalar_type()), order, r.rows, (int)r.width);
+    TORCH_CHECK_VALUE(n >= 0, "ebr_block_layernorm: sizes out of range");
+    return at::empty({n}, x.options().dtype(at::kByte));
+}
+
+variable_list layernorm(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps) {
+    RECORD_FUNCTION("ebr_fused::block_layernorm", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(x_.device());
+    const auto pt = param_type(x_, w_, b_);
+    const Tensor x = dense(x_), w = param_as(w_, pt), b = param_as(b_, pt), y = at::empty(x.sizes(), x.options());
+    const RowsOf r(x);
+    const Tensor stats = at::empty({r.rows, 4}, x.options().dtype(acc_type(x)));
+    check(ebr_block_layernorm(dtype_code(x.scalar_type()), dtype_code(pt), r.rows, (int)r.width, eps, x.data_ptr(), vptr(w),
+                              vptr(b), y.data_ptr(), stats.data_ptr(), stream_of(x)),
+          "ebr_block_layernorm");
+    return {y, stats};
+}
+
+// {dx, dw, db}: the latter, of the type pt, with want_w and want_b.
+variable_list layernorm_bwd(const Tensor& x_, const Tensor& w_, const Tensor& stats, const Tensor& dy_, at::ScalarType pt,
+                            bool want_w, bool want_b) {
+    RECORD_FUNCTION("ebr_fused::block_layernorm_bwd", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(x_.device());
+    const Tensor x = dense(x_), dy = dense(dy_.to(x_.scalar_type())), w = param_as(w_, pt);
+    const RowsOf r(x);
+    const auto p = x.options().dtype(pt);
+    const Tensor dx = at::empty(x.sizes(), x.options()), s = layer_scratch(x, 1, r);
+    const Tensor dw = want_w ? at::empty({r.width}, p) : Tensor(), db = want_b ? at::empty({r.width}, p) : Tensor();
+    check(ebr_block_layernorm_bwd(dtype_code(x.scalar_type()), dtype_code(pt), r.rows, (int)r.width, x.data_ptr(), vptr(w),
+                                  stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), vptr(dw), vptr(db), s.data_ptr(),
+                                  stream_of(x)),
+          "ebr_block_layernorm_bwd");
+    return {dx, dw, db};
+}
+
+Tensor to_type(const Tensor& t, const Tensor& like) { return t.defined() ? t.to(like.scalar_type()) : t; }
+
+struct LayerNormBwd : Function<LayerNormBwd> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w_,
+                                 const std::optional<Tensor>& b_, const Tensor& stats, const Tensor& dy, bool want_w,
+                                 bool want_b) {
+        const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
+        const auto pt = param_type(x, w, b);
+        ctx->save_for_backward({x, w, stats, dy});
+        ctx->saved_data["type"] = (int64_t)dtype_code(pt);
+        ctx->saved_data["has_b"] = b.defined();
+        ctx->saved_data["want_w"] = want_w;
+        ctx->saved_data["want_b"] = want_b;
+        ctx->set_materialize_grads(false);
+        const variable_list d = layernorm_bwd(x, w, stats, dy, pt, want_w, want_b);
+        variable_list out = {d[0]};  // dx, and what is wanted of dw and db
+        if (want_w) out.push_back(to_type(d[1], w));
+        if (want_b) out.push_back(to_type(d[2], b));
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(7);
+        const bool had_w = ctx->saved_data["want_w"].toBool(), had_b = ctx->saved_data["want_b"].toBool();
+        const Tensor u_ = g[0], uw_ = had_w ? g[1] : Tensor(), ub_ = had_b ? g[1 + had_w] : Tensor();
+        if (!u_.defined() && !uw_.defined() && !ub_.defined()) return out;
+        const variable_list sv = ctx->get_saved_variables();
+        const Tensor &x_ = sv[0], &w_ = sv[1], &stats = sv[2], &dy_ = sv[3];
+        const int64_t code = ctx->saved_data["type"].toInt();
+        const bool want_w = w_.defined() && ctx->needs_input_grad(1);
+        if (!native(g))
+            return python_grads("layer_norm_bwd", 7, x_, maybe(w_), stats, dy_, code, want_w, maybe(u_), maybe(uw_), maybe(ub_));
+        RECORD_FUNCTION("ebr_fused::block_layernorm_bwd2", std::vector<c10::IValue>());
+        const c10::DeviceGuard on(x_.device());
+        const auto pt = type_of(code);
+        const Tensor x = dense(x_), dy = dense(dy_.to(x_.scalar_type())), w = param_as(w_, pt);
+        const Tensor u = u_.defined() ? dense(u_.to(x_.scalar_type())) : at::zeros_like(x);
+        const Tensor uw = param_as(uw_, pt), ub = param_as(ub_, pt);
+        const RowsOf r(x);
+        const Tensor gx = at::empty(x.sizes(), x.options()), gdy = at::empty(x.sizes(), x.options());
+        const Tensor gw = want_w ? at::empty({r.width}, x.options().dtype(pt)) : Tensor(), s = layer_scratch(x, 2, r);
+        check(ebr_block_layernorm_bwd2(dtype_code(x.scalar_type()), (int)code, r.rows, (int)r.width, x.data_ptr(), vptr(w),
+                                       stats.data_ptr(), dy.data_ptr(), u.data_ptr(), vptr(uw), vptr(ub), gx.data_ptr(),
+                                       gdy.data_ptr(), vptr(gw), s.data_ptr(), stream_of(x)),
+              "ebr_block_layernorm_bwd2");
+        variable_list d = {gx, want_w ? to_type(gw, w_) : Tensor(), gdy.to(dy_.scalar_type())};
+        if (recorded({x_, w_, dy_, u_, uw_, ub_})) d = last(std::move(d));
+        out[0] = d[0];
+        out[1] = d[1];
+        out[4] = d[2];
+        return out;
+    }
+};
+
+struct LayerNorm : Function<LayerNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w_,
+                                 const std::optional<Tensor>& b_, double eps) {
+        const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
+        const variable_list out = layernorm(x, w, b, eps);
+        ctx->save_for_backward({x, w, b, out[1]});
+        ctx->set_materialize_grads(false);
+        return {out[0]};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(4);
+        if (!g[0].defined()) return out;
+        const variable_list s = ctx->get_saved_variables();
+        const auto [want_w, want_b] = wanted(ctx, s[1], s[2]);
+        if (!native(g)) return python_grads("layer_norm", 4, s[0], maybe(s[1]), maybe(s[2]), s[3], want_w || want_b, g[0]);
+        if (!at::GradMode::is_enabled()) {
+            const variable_list d =
+                layernorm_bwd(s[0], s[1], s[3], g[0], param_type(s[0], s[1], s[2]), want_w, want_b);
+            return {d[0], want_w ? to_type(d[1], s[1]) : Tensor(), want_b ? to_type(d[2], s[2]) : Tensor(), Tensor()};
+        }
+        const variable_list d = LayerNormBwd::apply(s[0], maybe(s[1]), maybe(s[2]), s[3], g[0], want_w, want_b);
+        out[0] = d[0];
+        if (want_w) out[1] = d[1];
+        if (want_b) out[2] = d[1 + want_w];
+        return out;
+    }
+};
+
+py::object layer_norm(const py::handle& hx, const py::handle& hw, const py::handle& hb, double eps) {
+    const Tensor x = plain(hx);
+    if (!block_takes(x) || !(eps >= 0)) return py::none();
+    Tensor p[2];
+    const py::handle given[2] = {hw, hb};
+    for (int i = 0; i < 2; ++i) {
+        if (given[i].is_none()) continue;
+        p[i] = plain(given[i]);
+        if (!p[i].defined() || p[i].dim() != 1 || p[i].size(0) != x.size(-1) || p[i].device() != x.device() ||
+            dtype_code(p[i].scalar_type()) < 0)
+            return py::none();
+    }
+    const RowsOf r(x);
+    if (ebr_block_layernorm_scratch(dtype_code(x.scalar_type()), 2, r.rows, (int)r.width) < 0) return py::none();
+    if (!recorded({x, p[0], p[1]})) return py::cast(layernorm(x, p[0], p[1], eps)[0]);
+    return py::cast(LayerNorm::apply(x, maybe(p[0]), maybe(p[1]), eps)[0]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The gated projection, differentiable twice (ebr_amd/block.py)
+// ---------------------------------------------------------------------------------------------------------------------
+
+struct ProjectionShape {
+    int code;
+    int64_t N, C, I;
+    ProjectionShape(const Tensor& x, const Tensor& w)
+        : code(dtype_code(x.scalar_type())), N(x.numel() / x.size(-1)), C(x.size(-1)), I(w.size(0) / 2) {}
+    Tensor scratch(const Tensor& x, int order) const {
+        const int64_t n = ebr_block_swiglu_linear_scratch(code, order, N, C, I);
+        TORCH_CHECK_VALUE(n >= 0, "ebr_block_swiglu_linear: sizes out of range");
+        return at::empty({n}, x.options().dtype(at::kByte));
+    }
+};
+
+Tensor projected(const Tensor& x_, const Tensor& w_) {
+    RECORD_FUNCTION("ebr_fused::block_swiglu_linear", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(x_.device());
+    const Tensor x = dense(x_), w = dense(w_);
+    const ProjectionShape n(x, w);
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = n.I;
+    const Tensor y = at::empty(shape, x.options());
+    check(ebr_block_swiglu_linear(n.code, n.N, n.C, n.I, x.data_ptr(), w.data_ptr(), y.data_ptr(), stream_of(x)),
+          "ebr_block_swiglu_linear");
+    return y;
+}
+
+variable_list projected_bwd(const Tensor& x_, const Tensor& w_, const Tensor& dy_, bool want_x, bool want_w) {
+    RECORD_FUNCTION("ebr_fused::block_swiglu_linear_bwd", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(x_.device());
+    const Tensor x = dense(x_), w = dense(w_), dy = dense(dy_.to(x_.scalar_type()));
+    const ProjectionShape n(x, w);
+    const Tensor dx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
+    const Tensor dw = want_w ? at::empty(w.sizes(), w.options()) : Tensor(), s = n.scratch(x, 1);
+    check(ebr_block_swiglu_linear_bwd(n.code, n.N, n.C, n.I, x.data_ptr(), w.data_ptr(), dy.data_ptr(), vptr(dx), vptr(dw),
+                                      s.data_ptr(), stream_of(x)),
+          "ebr_block_swiglu_linear_bwd");
+    return {dx, dw};
+}
+
+// dx as a node of its own.
+struct SwiGLULinearDx : Function<SwiGLULinearDx> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& dy) {
+        ctx->save_for_backward({x, w, dy});
+        ctx->set_materialize_grads(false);
+        return {projected_bwd(x, w, dy, true, false)[0]};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        if (!g[0].defined()) return variable_list(3);
+        const variable_list sv = ctx->get_saved_variables();
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        if (!native(g)) return python_grads("swiglu_linear_dx", 3, sv[0], sv[1], sv[2], g[0], want_x, want_w);
+        RECORD_FUNCTION("ebr_fused::block_swiglu_linear_bwd2", std::vector<c10::IValue>());
+        const c10::DeviceGuard on(sv[0].device());
+        const auto st = sv[0].scalar_type();
+        const Tensor x = dense(sv[0]), w = dense(sv[1]), dy = dense(sv[2].to(st)), c = dense(g[0].to(st));
+        const ProjectionShape n(x, w);
+        const Tensor gx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
+        const Tensor gw = want_w ? at::empty(w.sizes(), w.options()) : Tensor();
+        const Tensor gdy = at::empty(dy.sizes(), dy.options()), s = n.scratch(x, 2);
+        check(ebr_block_swiglu_linear_bwd2(n.code, n.N, n.C, n.I, x.data_ptr(), w.data_ptr(), dy.data_ptr(), c.data_ptr(),
+                                           vptr(gx), gdy.data_ptr(), vptr(gw), s.data_ptr(), stream_of(x)),
+              "ebr_block_swiglu_linear_bwd2");
+        variable_list d = {gx, gw, gdy.to(sv[2].scalar_type())};
+        return recorded({sv[0], sv[1], sv[2], g[0]}) ? last(std::move(d)) : d;
+    }
+};
+
+struct SwiGLULinear : Function<SwiGLULinear> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+        ctx->save_for_backward({x, w});
+        ctx->set_materialize_grads(false);
+        return {projected(x, w)};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        variable_list out(2);
+        if (!g[0].defined()) return out;
+        const variable_list s = ctx->get_saved_variables();
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        if (!native(g)) return python_grads("swiglu_linear", 2, s[0], s[1], g[0], want_x, want_w);
+        if (!at::GradMode::is_enabled()) return projected_bwd(s[0], s[1], g[0], want_x, want_w);
+        if (want_w) {  // recorded: of the parts, which have derivatives of their own (ebr_amd/block.py)
+            const Tensor dgu = SwiGLUBwd::apply(Linear::apply(s[0], s[1])[0], g[0])[0];
+            if (want_x) out[0] = Dgrad::apply(dgu, s[1])[0];
+            out[1] = weight_grad(dgu, s[0]);
+        } else if (want_x) {
+            out[0] = SwiGLULinearDx::apply(s[0], s[1], g[0])[0];
+        }
+        return out;
+    }
+};
+
+py::object swiglu_linear(const py::handle& hx, const py::handle& hw) {
+    const Tensor x = plain(hx), w = plain(hw);
+    if (!block_takes(x) || !w.defined() || w.dim() != 2 || w.size(0) < 2 || w.size(0) % 2 || w.size(1) != x.size(-1) ||
+        !same_kind(x, w))
+        return py::none();
+    const ProjectionShape n(x, w);
+    if (ebr_block_swiglu_linear_scratch(n.code, 2, n.N, n.C, n.I) < 0) return py::none();
+    return py::cast(recorded({x, w}) ? SwiGLULinear::apply(x, w)[0] : projected(x, w));
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The optimizer's step (ebr_amd/optim.py, which has checked the tensors)
+// ---------------------------------------------------------------------------------------------------------------------
+
+// The tensors of a list, or nothing where one of them is not an ordinary dense GPU tensor on that device, contiguous where it
+// is not to be ``strided``.
+std::optional<variable_list> plain_list(const py::sequence& ts, const c10::Device& on, bool strided) {
+    variable_list out;
+    out.reserve(ts.size());
+    for (const auto& h : ts) {
+        out.push_back(plain(h));
+        if (!out.back().defined() || out.back().device() != on || !(strided || out.back().is_contiguous())) return std::nullopt;
+    }
+    return out;
+}
+
+// {norm in fp64, norm in fp32} of gradients.
+std::pair<Tensor, Tensor> norm_of(variable_list grads) {
+    RECORD_FUNCTION("ebr_fused::grad_norm", std::vector<c10::IValue>());
+    for (Tensor& g : grads) g = dense(g);
+    std::vector<ebr_optim_grad> t(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i)
+        t[i] = {grads[i].data_ptr(), grads[i].numel(), dtype_code(grads[i].scalar_type()), 0};
+    const int64_t n = ebr_block_grad_norm_scratch((int64_t)t.size(), t.data());
+    TORCH_CHECK_VALUE(n >= 0, "ebr_block_grad_norm: sizes out of range");
+    const auto o = grads[0].options().requires_grad(false);
+    const Tensor norm = at::empty({}, o.dtype(at::kDouble)), single = at::empty({}, o.dtype(at::kFloat));
+    const Tensor s = at::empty({n}, o.dtype(at::kByte));
+    check(ebr_block_grad_norm((int64_t)t.size(), t.data(), static_cast<double*>(norm.data_ptr()), fptr(single), s.data_ptr(),
+                              stream_of(norm)),
+          "ebr_block_grad_norm");
+    return {norm, single};
+}
+
+// One step, or False for tensors that the Python layer has to refuse or to take itself. ``scales``: a pair for each tensor, or
+// None. ``norm``: the clipped gradients' norm in fp64, or None.
+bool adamw(const py::sequence& hp, const py::sequence& hg, const py::sequence& hm, const py::sequence& hv,
+           const py::sequence& hs, const py::object& hscales, double lr, const py::handle& hlr, double beta1, double beta2,
+           double eps, double decay, const py::handle& hnorm, double max_norm) {
+    const size_t n = hp.size();
+    if (!plain_context() || n == 0) return false;
+    const Tensor first = plain(hp[0]);
+    if (!first.defined()) return false;
+    const bool eight = !hscales.is_none();
+    py::list hms, hvs;
+    if (eight)
+        for (const auto& pair : hscales.cast<py::sequence>()) {
+            const auto two = pair.cast<py::sequence>();
+            if (two.size() != 2) return false;
+            hms.append(two[0]);
+            hvs.append(two[1]);
+        }
+    std::optional<variable_list> l[7];
+    const py::sequence given[7] = {hp, hg, hm, hv, hs, hms, hvs};
+    for (int i = 0; i < (eight ? 7 : 5); ++i) {
+        l[i] = plain_list(given[i], first.device(), i == 1);
+        if (!l[i] || l[i]->size() != n) return false;
+    }
+    const variable_list &p = *l[0], &m = *l[2], &v = *l[3], &step = *l[4];
+    variable_list g = *l[1];
+    std::vector<ebr_optim_tensor> all(n);
+    std::vector<std::pair<int, int>> kinds;  // of parameter and gradient
+    std::vector<size_t> kind(n);
+    for (size_t i = 0; i < n; ++i) {
+        const int pc = dtype_code(p[i].scalar_type()), gc = dtype_code(g[i].scalar_type());
+        const bool half = gc == EBR_DTYPE_BF16 || gc == EBR_DTYPE_F16, wide = pc == EBR_DTYPE_F64;
+        const auto held = eight ? at::kFloat8_e4m3fn : wide ? at::kDouble : at::kFloat;
+        const int64_t len = p[i].numel(), blocks = (len + 255) / 256;
+        if (pc < 0 || gc < 0 || (gc != pc && !(pc == EBR_DTYPE_F32 && half)) || (eight && wide) ||
+            g[i].sizes() != p[i].sizes() || m[i].scalar_type() != held || v[i].scalar_type() != held || m[i].numel() != len ||
+            v[i].numel() != len || step[i].scalar_type() != at::kLong || step[i].numel() != 1)
+            return false;
+        if (eight)
+            for (const Tensor& s : {(*l[5])[i], (*l[6])[i]})
+                if (s.scalar_type() != at::kFloat || s.numel() != blocks) return false;
+        g[i] = dense(g[i]);
+        all[i] = {p[i].data_ptr(), g[i].data_ptr(), m[i].data_ptr(), v[i].data_ptr(), eight ? fptr((*l[5])[i]) : nullptr,
+                  eight ? fptr((*l[6])[i]) : nullptr, static_cast<int64_t*>(step[i].data_ptr()), len};
+        const std::pair<int, int> k = {pc, gc};
+        kind[i] = std::find(kinds.begin(), kinds.end(), k) - kinds.begin();
+        if (kind[i] == kinds.size()) kinds.push_back(k);
+    }
+    for (const bool steps : {false, true}) {
+        std::vector<const void*> at_;
+        for (const ebr_optim_tensor& t : all)
+            if (steps || t.n > 0) at_.push_back(steps ? t.step : t.p);
+        std::sort(at_.begin(), at_.end());
+        if (std::adjacent_find(at_.begin(), at_.end()) != at_.end()) return false;  // the same one twice
+    }
+    Tensor lr_dev, norm;
+    if (!hlr.is_none()) {
+        lr_dev = plain(hlr);
+        if (!lr_dev.defined()) return false;
+    }
+    if (!hnorm.is_none()) {
+        norm = plain(hnorm);
+        if (!norm.defined() || norm.device() != first.device()) return false;
+    }
+    RECORD_FUNCTION("ebr_fused::adamw", std::vector<c10::IValue>());
+    const c10::DeviceGuard on(first.device());
+    const auto bytes = first.options().dtype(at::kByte).requires_grad(false);
+    for (size_t k = 0; k < kinds.size(); ++k) {
+        std::vector<ebr_optim_tensor> t;
+        for (size_t i = 0; i < n; ++i)
+            if (kind[i] == k) t.push_back(all[i]);
+        const Tensor s = at::empty({ebr_block_adamw_scratch((int64_t)t.size())}, bytes);
+        check(ebr_block_adamw(kinds[k].first, kinds[k].second, eight ? 8 : 32, (int64_t)t.size(), t.data(), lr, fptr(lr_dev),
+                              beta1, beta2, eps, decay, static_cast<const double*>(vptr(norm)), max_norm, s.data_ptr(),
+                              stream_of(first)),
+              "ebr_block_adamw");
+    }
+    for (const int i : {0, 2, 3, 4, 5, 6})  // written in place
+        if (l[i])
+            for (const Tensor& x : *l[i]) x.unsafeGetTensorImpl()->bump_version();
+    return true;
+}
+
+// The gradients' norm in fp64 and in fp32, or None.
+py::object grad_norms(const py::sequence& hgrads) {
+    if (!plain_context() || hgrads.size() == 0) return py::none();
+    const Tensor first = plain(hgrads[0]);
+    if (!first.defined()) return py::none();
+    const auto grads = plain_list(hgrads, first.device(), true);
+    if (!grads) return py::none();
+    for (const Tensor& g : *grads)
+        if (dtype_code(g.scalar_type()) < 0) return py::none();
+    const c10::DeviceGuard on(first.device());
+    const auto [norm, single] = norm_of(*grads);
+    return py::make_tuple(norm, single);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // Token ends of a training step (ebr_amd/tokens.py): the embedding, linear and differentiable to any order, and the
 // distillation loss, differentiable once
 // ---------------------------------------------------------------------------------------------------------------------
-
-at::ScalarType type_of(int64_t code) {
-    return code == EBR_DTYPE_F32 ? at::kFloat : code == EBR_DTYPE_BF16 ? at::kBFloat16
-         : code == EBR_DTYPE_F16 ? at::kHalf : at::kDouble;
-}
 
 bool token_type(const Tensor& ids) { return ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt; }
 int wide(const Tensor& ids) { return ids.scalar_type() == at::kLong; }
@@ -1465,6 +1849,10 @@ PYBIND11_MODULE(ebr_host, m) {
     m.def("step_and_project", &step_and_project);
     m.def("linear", &linear);
     m.def("group_norm", &group_norm);
+    m.def("layer_norm", &layer_norm);
+    m.def("swiglu_linear", &swiglu_linear);
+    m.def("grad_norms", &grad_norms);
+    m.def("adamw", &adamw);
     m.def("embedding", &embedding);
     m.def("distill_loss", &distill_loss);
 }

@@ -1,0 +1,434 @@
+// AdamW over many tensors and the global norm of their gradients on gfx950 (C ABI and the formulas: include/ebr_optim.h).
+//
+// The tensors' addresses travel in the kernels' arguments, up to TENSORS (GRADS) a launch, so nothing is copied to the device
+// and nothing kept: a workgroup finds its tensor by its own number in a table of the tensors' first workgroups.
+//
+// Bound by memory: 28 bytes an element with fp32 parameters, gradients and moments, 16 with moments in 8 bits, and the
+// gradients once more for the norm. The step's factors (powers of the betas, the clipping) are taken once a tensor by
+// k_factors, which also counts the step.
+//
+// Moments in 8 bits are taken in fp64: a moment next to the border between two numbers goes to the same side in any order of
+// operations, and the arithmetic (some 70 operations an element) still fits under the loads. A wave takes the 256 elements of
+// one scale, four a lane, so that the block's largest needs no shared memory.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "../../include/ebr_optim.h"
+#include "rowwise.hpp"
+
+namespace ebr_opt {
+
+using namespace ebr_row;
+
+constexpr int THREADS = 256, BLOCK = 256, TENSORS = 48, GRADS = 144;
+constexpr int64_t LEAST = 4096, MOST = 65536;  // elements of a workgroup
+
+// What a step multiplies by, for one tensor.
+struct alignas(16) Factors {
+    double clip, step, root, decay;  // of the gradient; lr / (1 - beta1^t); 1 / sqrt(1 - beta2^t); 1 - lr decay
+    uint32_t dither, zero[3];        // t * 0x9E3779B1
+};
+
+struct Table {
+    ebr_optim_tensor t[TENSORS];
+    int first[TENSORS + 1];  // the first workgroup of each, and of what would be next
+    int count, per;          // per: elements of a workgroup
+    const Factors* factors;
+    double beta1, beta2, rest1, rest2, eps;
+};
+
+struct Prepare {
+    int64_t* step[TENSORS];
+    int count;
+    Factors* factors;
+    const float* lr_dev;
+    const double* norm;
+    double lr, beta1, beta2, decay, max_norm;
+};
+
+struct Sums {
+    const void* g[GRADS];
+    int64_t n[GRADS];
+    int first[GRADS + 1], dtype[GRADS];
+    int count, per;
+    double* part;
+};
+
+__global__ __launch_bounds__(64) void k_factors(Prepare a) {
+    const int i = threadIdx.x;
+    if (i >= a.count) return;
+    const int64_t t = *a.step[i] + 1;
+    *a.step[i] = t;
+    const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+    Factors f = {};
+    f.clip = 1.0;
+    if (a.norm) {
+        const double c = a.max_norm / (*a.norm + 1e-6);
+        f.clip = c > 1.0 ? 1.0 : c;  // (a norm that is NaN gives NaN)
+    }
+    f.step = lr / (1.0 - pow(a.beta1, (double)t));
+    f.root = 1.0 / sqrt(1.0 - pow(a.beta2, (double)t));
+    f.decay = 1.0 - lr * a.decay;
+    f.dither = (uint32_t)t * 0x9E3779B1u;
+    a.factors[i] = f;
+}
+
+// The tensor of this workgroup: the last one that begins at or before it.
+template <typename Tab> __device__ __forceinline__ int tensor_of(const Tab& a) {
+    int lo = 0, hi = a.count;
+    const int b = blockIdx.x;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.first[mid] <= b) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Four elements from i on, of which n - i exist; whole where they may be (``wide``: their address allows it).
+template <typename T, typename A> __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool wide, A (&v)[4]) {
+    if (wide && i + 4 <= n) {
+        const Pack<T, 4> x = ldp<T, 4>(p + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (A)x.e[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = i + e < n ? (A)p[i + e] : (A)0;
+    }
+}
+template <typename T, typename A> __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool wide, const A (&v)[4]) {
+    if (wide && i + 4 <= n) {
+        Pack<T, 4> x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.e[e] = (T)v[e];
+        stp<T, 4>(p + i, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) p[i + e] = (T)v[e];
+    }
+}
+// A pack of four is an aligned vector of at most 16 bytes; four fp64 go as two.
+template <typename T> __device__ __forceinline__ bool wide4(const void* p) {
+    return sizeof(T) <= 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
+}
+
+template <typename A> __device__ __forceinline__ A root(A x);
+template <> __device__ __forceinline__ float root(float x) { return __builtin_sqrtf(x); }
+template <> __device__ __forceinline__ double root(double x) { return sqrt(x); }
+
+template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_adamw(Table a) {
+    using A = typename Acc<P>::type;
+    const int which = tensor_of(a);
+    const ebr_optim_tensor t = a.t[which];
+    const Factors f = a.factors[which];
+    const A clip = (A)f.clip, step = (A)f.step, rt = (A)f.root, decay = (A)f.decay, eps = (A)a.eps;
+    const A b1 = (A)a.beta1, b2 = (A)a.beta2, c1 = (A)a.rest1, c2 = (A)a.rest2;
+    P* const p = reinterpret_cast<P*>(t.p);
+    const G* const g = reinterpret_cast<const G*>(t.g);
+    A *const m = reinterpret_cast<A*>(t.m), *const v = reinterpret_cast<A*>(t.v);
+    const bool wp = wide4<P>(p), wg = wide4<G>(g), wm = wide4<A>(m), wv = wide4<A>(v);
+    const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
+    const int64_t to = from + a.per < t.n ? from + a.per : t.n;
+    for (int64_t i = from + threadIdx.x * 4; i < to; i += THREADS * 4) {
+        A pv[4], gv[4], mv[4], vv[4];
+        load4(p, i, to, wp, pv);
+        load4(g, i, to, wg, gv);
+        load4(m, i, to, wm, mv);
+        load4(v, i, to, wv, vv);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const A ge = gv[e] * clip;
+            mv[e] = b1 * mv[e] + c1 * ge;
+            vv[e] = b2 * vv[e] + c2 * (ge * ge);
+            pv[e] = pv[e] * decay - step * mv[e] / (root(vv[e]) * rt + eps);
+        }
+        store4(p, i, to, wp, pv);
+        store4(m, i, to, wm, mv);
+        store4(v, i, to, wv, vv);
+    }
+}
+
+// The e4m3 number of y = |moment| / scale, as its seven bits: floor(y / s + t) steps s of its binade.
+__device__ __forceinline__ uint32_t e4m3(double y, double t) {
+    int e = __builtin_amdgcn_frexp_exp(y) - 1;
+    if (e < -6 || y == 0.0) e = -6;
+    const int code = ((e + 6) << 3) + (int)(__builtin_ldexp(y, 3 - e) + t);
+    return y != y ? 0x7Fu : (uint32_t)(code > 0x7E ? 0x7E : code);
+}
+
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v = fmax(v, __shfl_xor(v, m, 64));
+    return v;
+}
+
+template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_adamw8(Table a) {
+    const int which = tensor_of(a);
+    const ebr_optim_tensor t = a.t[which];
+    const Factors f = a.factors[which];
+    const float step = (float)f.step, rt = (float)f.root, decay = (float)f.decay, eps = (float)a.eps;
+    P* const p = reinterpret_cast<P*>(t.p);
+    const G* const g = reinterpret_cast<const G*>(t.g);
+    uint8_t *const m = reinterpret_cast<uint8_t*>(t.m), *const v = reinterpret_cast<uint8_t*>(t.v);
+    const bool wp = wide4<P>(p), wg = wide4<G>(g), wm = wide4<uint8_t>(m), wv = wide4<uint8_t>(v);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
+    const int64_t to = from + a.per < t.n ? from + a.per : t.n;
+    for (int64_t b = from + wave * BLOCK; b < to; b += THREADS / 64 * BLOCK) {
+        const int64_t i = b + lane * 4;
+        float pv[4], gv[4];
+        uint32_t mq[4], vq[4];
+        load4(p, i, to, wp, pv);
+        load4(g, i, to, wg, gv);
+        load4(m, i, to, wm, mq);
+        load4(v, i, to, wv, vq);
+        const double ms = (double)t.ms[b / BLOCK], vs = (double)t.vs[b / BLOCK];
+        double mv[4], rv[4];
+        double mt = 0, vt = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double ge = (double)gv[e] * f.clip;
+            const double r = (double)__builtin_amdgcn_cvt_f32_fp8((int)vq[e], 0) * vs;
+            mv[e] = a.beta1 * ((double)__builtin_amdgcn_cvt_f32_fp8((int)mq[e], 0) * ms) + a.rest1 * ge;
+            rv[e] = sqrt(a.beta2 * (r * r) + a.rest2 * (ge * ge));
+            mt = fmax(mt, fabs(mv[e]));
+            vt = fmax(vt, rv[e]);
+            pv[e] = pv[e] * decay - step * (float)mv[e] / ((float)rv[e] * rt + eps);
+        }
+        store4(p, i, to, wp, pv);
+        mt = wave_max(mt) / 448.0;
+        vt = wave_max(vt) / 448.0;
+        const bool some_m = !(mt < 0x1p-126), some_v = !(vt < 0x1p-126);
+        const double im = some_m ? 1.0 / mt : 0.0, iv = some_v ? 1.0 / vt : 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t w = (uint32_t)(i + e) * 0x85EBCA77u + f.dither;
+            mq[e] = e4m3(fabs(mv[e]) * im, (double)(w >> 8) * 0x1p-24) | (mv[e] < 0 ? 0x80u : 0u);
+            vq[e] = e4m3(rv[e] * iv, (double)((w + 0x80000000u) >> 8) * 0x1p-24);
+            if (some_v && rv[e] > 0 && vq[e] == 0) vq[e] = 1;
+        }
+        store4(m, i, to, wm, mq);
+        store4(v, i, to, wv, vq);
+        if (lane == 0) {
+            t.ms[b / BLOCK] = some_m ? (float)mt : 0.f;
+            t.vs[b / BLOCK] = some_v ? (float)vt : 0.f;
+        }
+    }
+}
+
+template <typename G> __device__ __forceinline__ double squares(const void* g_, int64_t from, int64_t to) {
+    const G* const g = reinterpret_cast<const G*>(g_);
+    constexpr int N = 16 / (int)sizeof(G);
+    double s = 0;
+    if (((uintptr_t)g & 15) == 0) {  // from is a multiple of a vector
+        for (int64_t i = from + threadIdx.x * N; i < to; i += THREADS * N) {
+            if (i + N <= to) {
+                const Pack<G, N> v = ldp<G, N>(g + i);
+#pragma unroll
+                for (int e = 0; e < N; ++e) s += (double)v.e[e] * (double)v.e[e];
+            } else {
+                for (int64_t j = i; j < to; ++j) s += (double)g[j] * (double)g[j];
+            }
+        }
+    } else {
+        for (int64_t i = from + threadIdx.x; i < to; i += THREADS) s += (double)g[i] * (double)g[i];
+    }
+    return s;
+}
+
+__device__ __forceinline__ double block_sum(double s, double* lds) {
+    s = lanes_sum<64>(s);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    double all = 0;
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) all += lds[w];
+    return all;
+}
+
+__global__ __launch_bounds__(THREADS) void k_squares(Sums a) {
+    __shared__ double lds[THREADS / 64];
+    const int which = tensor_of(a);
+    const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
+    const int64_t to = from + a.per < a.n[which] ? from + a.per : a.n[which];
+    double s;
+    switch (a.dtype[which]) {
+        case EBR_DTYPE_F32: s = squares<float>(a.g[which], from, to); break;
+        case EBR_DTYPE_BF16: s = squares<__bf16>(a.g[which], from, to); break;
+        case EBR_DTYPE_F16: s = squares<_Float16>(a.g[which], from, to); break;
+        default: s = squares<double>(a.g[which], from, to); break;
+    }
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(1024) void k_norm(const double* part, int64_t parts, double* norm, float* single) {
+    __shared__ double lds[16];
+    double s = 0;
+    for (int64_t i = threadIdx.x; i < parts; i += 1024) s += part[i];
+    s = sqrt(block_sum(s, lds));
+    if (threadIdx.x != 0) return;
+    *norm = s;
+    if (single) *single = (float)s;
+}
+
+// -- launches ----------------------------------------------------------------------------------------------------------
+
+static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
+
+// Elements of a workgroup, a multiple of LEAST: four workgroups for each of the 256 compute units where there is enough.
+static int64_t per_group(int64_t total) {
+    const int64_t want = (total / 2048 + LEAST - 1) / LEAST * LEAST;
+    return std::min(std::max(want, LEAST), MOST);
+}
+static int64_t groups(int64_t n, int64_t per) { return (n + per - 1) / per; }
+
+constexpr int64_t TOO_MANY = (int64_t)1 << 40;  // elements
+
+static int64_t total_of(int64_t count, const ebr_optim_grad* g) {
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (g[i].n < 0 || g[i].n >= TOO_MANY || (total += g[i].n) >= TOO_MANY) return -1;
+    }
+    return total;
+}
+
+template <typename P, typename G> static void step(hipStream_t s, int bits, unsigned blocks, const Table& a) {
+    if constexpr (sizeof(P) < 8) {
+        if (bits == 8) {
+            hipLaunchKernelGGL((k_adamw8<P, G>), dim3(blocks), dim3(THREADS), 0, s, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_adamw<P, G>), dim3(blocks), dim3(THREADS), 0, s, a);
+}
+
+// Whether two tensors share a parameter or a step.
+static bool twice(int64_t count, const ebr_optim_tensor* t) {
+    std::vector<const void*> ps, steps;
+    for (int64_t i = 0; i < count; ++i) {
+        if (t[i].n > 0) ps.push_back(t[i].p);
+        steps.push_back(t[i].step);
+    }
+    for (auto* v : {&ps, &steps}) {
+        std::sort(v->begin(), v->end());
+        if (std::adjacent_find(v->begin(), v->end()) != v->end()) return true;
+    }
+    return false;
+}
+
+}  // namespace ebr_opt
+
+using namespace ebr_opt;
+
+extern "C" {
+
+int64_t ebr_block_grad_norm_scratch(int64_t count, const ebr_optim_grad* grads) {
+    if (count < 1 || !grads) return -1;
+    const int64_t total = total_of(count, grads);
+    if (total < 0) return -1;
+    const int64_t per = per_group(total);
+    int64_t parts = 0;
+    for (int64_t i = 0; i < count; ++i) parts += ebr_opt::groups(grads[i].n, per);
+    return parts > MAX_BLOCKS ? -1 : 8 * parts + 16;
+}
+
+int ebr_block_grad_norm(int64_t count, const ebr_optim_grad* grads, double* norm, float* single, void* scratch,
+                        void* stream) {
+    if (count < 1) return EBR_ERR_SHAPE;
+    if (!grads || !norm) return EBR_ERR_NULL;
+    for (int64_t i = 0; i < count; ++i) {
+        if (!known(grads[i].dtype)) return EBR_ERR_DTYPE;
+        if (grads[i].n > 0 && !grads[i].g) return EBR_ERR_NULL;
+    }
+    if (ebr_block_grad_norm_scratch(count, grads) < 0) return EBR_ERR_SHAPE;
+    if (!scratch) return EBR_ERR_SCRATCH;
+    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    const int64_t per = per_group(total_of(count, grads));
+    int64_t parts = 0;
+    for (int64_t i = 0; i < count;) {
+        Sums a;
+        int blocks = 0;
+        for (a.count = 0; i < count && a.count < GRADS; ++i) {
+            if (grads[i].n == 0) continue;
+            a.g[a.count] = grads[i].g;
+            a.n[a.count] = grads[i].n;
+            a.dtype[a.count] = grads[i].dtype;
+            a.first[a.count++] = blocks;
+            blocks += (int)ebr_opt::groups(grads[i].n, per);
+        }
+        if (blocks == 0) break;
+        a.first[a.count] = blocks;
+        a.per = (int)per;
+        a.part = reinterpret_cast<double*>(scratch) + parts;
+        hipLaunchKernelGGL(k_squares, dim3(blocks), dim3(THREADS), 0, s, a);
+        parts += blocks;
+    }
+    hipLaunchKernelGGL(k_norm, dim3(1), dim3(1024), 0, s, reinterpret_cast<const double*>(scratch), parts, norm, single);
+    return launched();
+}
+
+int64_t ebr_block_adamw_scratch(int64_t count) {
+    return count < 0 || count >= ((int64_t)1 << 31) ? -1 : count * (int64_t)sizeof(Factors) + 16;
+}
+
+int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_optim_tensor* tensors, double lr,
+                    const float* lr_dev, double beta1, double beta2, double eps, double decay, const double* norm,
+                    double max_norm, void* scratch, void* stream) {
+    const bool half = gtype == EBR_DTYPE_BF16 || gtype == EBR_DTYPE_F16;
+    if (!known(ptype) || !known(gtype) || (gtype != ptype && !(ptype == EBR_DTYPE_F32 && half)) ||
+        (bits != 32 && bits != 8) || (bits == 8 && ptype == EBR_DTYPE_F64))
+        return EBR_ERR_DTYPE;
+    if (ebr_block_adamw_scratch(count) < 0 || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0))
+        return EBR_ERR_SHAPE;
+    if (count == 0) return EBR_OK;
+    if (!tensors) return EBR_ERR_NULL;
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        const ebr_optim_tensor& t = tensors[i];
+        if (t.n < 0 || t.n >= TOO_MANY || (total += t.n) >= TOO_MANY) return EBR_ERR_SHAPE;
+        if (!t.step || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || (bits == 8 && (!t.ms || !t.vs))))) return EBR_ERR_NULL;
+    }
+    const int64_t per = per_group(total);
+    if (total / per + count > MAX_BLOCKS) return EBR_ERR_SHAPE;
+    try {
+        if (twice(count, tensors)) return EBR_ERR_SHAPE;
+    } catch (const std::bad_alloc&) {
+        return EBR_ERR_HIP_BASE + (int)hipErrorOutOfMemory;
+    }
+    if (!scratch) return EBR_ERR_SCRATCH;
+    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    Factors* factors = reinterpret_cast<Factors*>(scratch);
+    for (int64_t i = 0; i < count; i += TENSORS, factors += TENSORS) {
+        Table a = {};
+        Prepare pre = {};
+        a.count = pre.count = (int)std::min<int64_t>(TENSORS, count - i);
+        a.factors = pre.factors = factors;
+        a.per = (int)per;
+        a.beta1 = pre.beta1 = beta1, a.beta2 = pre.beta2 = beta2;
+        a.rest1 = 1.0 - beta1, a.rest2 = 1.0 - beta2, a.eps = eps;
+        pre.lr = lr, pre.lr_dev = lr_dev, pre.decay = decay, pre.norm = norm, pre.max_norm = max_norm;
+        int blocks = 0;
+        for (int k = 0; k < a.count; ++k) {
+            a.t[k] = tensors[i + k];
+            pre.step[k] = a.t[k].step;
+            a.first[k] = blocks;
+            blocks += (int)ebr_opt::groups(a.t[k].n, per);
+        }
+        a.first[a.count] = blocks;
+        hipLaunchKernelGGL(k_factors, dim3(1), dim3(64), 0, s, pre);
+        if (blocks == 0) continue;
+        if (ptype == EBR_DTYPE_F64) step<double, double>(s, bits, blocks, a);
+        else if (ptype == EBR_DTYPE_BF16) step<__bf16, __bf16>(s, bits, blocks, a);
+        else if (ptype == EBR_DTYPE_F16) step<_Float16, _Float16>(s, bits, blocks, a);
+        else if (gtype == EBR_DTYPE_BF16) step<float, __bf16>(s, bits, blocks, a);
+        else if (gtype == EBR_DTYPE_F16) step<float, _Float16>(s, bits, blocks, a);
+        else step<float, float>(s, bits, blocks, a);
+    }
+    return launched();
+}
+
+}  // extern "C"

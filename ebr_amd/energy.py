@@ -56,7 +56,8 @@ class EnergyConfig:
     block_impl: str = "eager"  # "fused": rms_norm and the SwiGLU activation as HIP kernels (ebr_amd.block)
     linear_impl: str = "eager"  # "splitk": projection weight gradients as split-K GEMMs (ebr_amd.linear)
     embed_impl: str = "eager"  # "fused": token lookup and table gradient as HIP kernels (ebr_amd.tokens)
-    norm: str = "rms"  # "group": the blocks' norms over the board's cells, in norm_groups groups of channels
+    mlp_impl: Optional[str] = None  # None: as block_impl; "projected": SwiGLU's projection and activation as one HIP kernel
+    norm: str = "rms"  # "group": the blocks' norms over the board's cells, in norm_groups groups of channels; "layer"
     norm_groups: int = 8
 
 
@@ -292,11 +293,12 @@ def teacher_logits(model, decoder, x, z0, k: int, steps: int = 64, alpha=0.1):
 
 def train_step(model, decoder, x, z0, targets, steps: int = 16, alpha=0.1, compiled=None,
                wrapper: Optional[str] = None, sigma=None, noises=None, active=None, teacher=None,
-               temperature: float = 1.0) -> torch.Tensor:
+               temperature: float = 1.0, optimizer=None) -> torch.Tensor:
     """One config-3 training step: graded descent (create_graph), CE to ``targets``, backward. Returns the loss.
     ``wrapper`` and the rest select the reference microstep (``descend``). With ``teacher``, (values, ids) as
     ``teacher_logits`` gives them, the loss is the distillation from them at ``temperature`` (``tokens.distill_loss``, GPU
-    only) in the cross entropy's place, and ``targets`` is not read."""
+    only) in the cross entropy's place, and ``targets`` is not read. ``optimizer`` (such as ``ebr_amd.optim.AdamW``): its step
+    on the gradients follows, and they are cleared."""
     x_emb = model.puzzle_embedding(x, z0.dtype)
     z = z0.detach().requires_grad_(True)
     v = descend(model, z, x_emb, steps, alpha, create_graph=True, compiled=compiled, wrapper=wrapper, sigma=sigma,
@@ -305,21 +307,25 @@ def train_step(model, decoder, x, z0, targets, steps: int = 16, alpha=0.1, compi
         from ebr_amd import tokens
 
         loss = tokens.distill_loss(decoder.lm_head(v), *teacher, temperature=temperature)
-        loss.backward()
-        return loss.detach()
-    logits = decoder(v)
-    loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
+    else:
+        logits = decoder(v)
+        loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
     loss.backward()
+    if optimizer is not None:
+        optimizer.step()
+        optimizer.zero_grad(set_to_none=True)
     return loss.detach()
 
 
-def graph_train_step(model, decoder, x, z0, targets, steps: int = 16, alpha=0.1, warmup: int = 2):
+def graph_train_step(model, decoder, x, z0, targets, steps: int = 16, alpha=0.1, warmup: int = 2, optimizer=None):
     """``train_step`` captured in a HIP graph over static inputs ``x``, ``z0``, ``targets`` (config 3 with the fused
     kernels: every launch goes to torch's current stream, nothing synchronises with the host, no allocation outside
     torch's allocator). Returns ``(graph, loss)``: ``graph.replay()`` re-runs the whole step (graded descent, CE,
     backward) on the inputs' current contents and writes ``loss`` and every parameter's ``.grad`` in place (the
     gradients are assigned, not accumulated: they are allocated by the captured backward). Warm-up steps run on a side
-    stream first, as capture needs (the attention self-test and the allocator's pools settle there)."""
+    stream first, as capture needs (the attention self-test and the allocator's pools settle there). ``optimizer``
+    (``ebr_amd.optim.AdamW``): its step on these gradients is captured too, so that every replay takes one; the warm-up steps
+    take none."""
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -328,9 +334,13 @@ def graph_train_step(model, decoder, x, z0, targets, steps: int = 16, alpha=0.1,
             model.zero_grad(set_to_none=True)
             decoder.zero_grad(set_to_none=True)
     torch.cuda.current_stream().wait_stream(side)
+    if optimizer is not None:
+        optimizer.init_state()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         loss = train_step(model, decoder, x, z0, targets, steps, alpha)
+        if optimizer is not None:
+            optimizer.step()
     return graph, loss
 
 

@@ -53,6 +53,33 @@ def group_norm(x: torch.Tensor, groups: int, eps: float) -> torch.Tensor:
     return (c * torch.rsqrt(c.square().mean(dim=(1, 3), keepdim=True) + eps)).reshape(x.shape).to(x.dtype)
 
 
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float) -> torch.Tensor:
+    """Zero mean and unit variance over the last dim, times weight, plus bias, in fp32, result in the input dtype."""
+    xf = x.float()
+    c = xf - xf.mean(dim=-1, keepdim=True)
+    return (c * torch.rsqrt(c.square().mean(dim=-1, keepdim=True) + eps) * weight.float() + bias.float()).to(x.dtype)
+
+
+class LayerNorm(nn.Module):
+    """``layer_norm`` with a learned fp32 weight and bias; ``impl="fused"`` runs it and its first and second derivatives as HIP
+    kernels (``ebr_amd.block.layer_norm``)."""
+
+    def __init__(self, hidden_size: int, eps: float = RMS_NORM_EPS, impl: str = "eager") -> None:
+        super().__init__()
+        if impl not in ("eager", "fused"):
+            raise ValueError(f"LayerNorm impl must be 'eager' or 'fused', got {impl!r}")
+        self.weight = nn.Parameter(torch.ones(hidden_size))
+        self.bias = nn.Parameter(torch.zeros(hidden_size))
+        self.eps, self.impl = eps, impl
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.impl == "fused":
+            from ebr_amd import block
+
+            return block.layer_norm(x, self.weight, self.bias, self.eps)
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
 class CastedLinear(nn.Module):
     """y = x W^T (+ b) with fp32 parameters cast to x.dtype at every call. ``impl="splitk"`` takes the weight
     gradients as split-K GEMMs with fp32 partials (``ebr_amd.linear``); the values are those of ``F.linear``."""
@@ -86,12 +113,13 @@ def swiglu_intermediate(hidden_size: int, expansion: float) -> int:
 
 class SwiGLU(nn.Module):
     """down(silu(gate) * up) with gate, up the halves of one projection; ``impl="fused"`` runs the activation (and its
-    first and second derivatives) as one HIP kernel each (``ebr_amd.block.swiglu``)."""
+    first and second derivatives) as one HIP kernel each (``ebr_amd.block.swiglu``), ``impl="projected"`` the projection
+    with the activation in it (``ebr_amd.block.swiglu_linear``)."""
 
     def __init__(self, hidden_size: int, expansion: float, impl: str = "eager") -> None:
         super().__init__()
-        if impl not in ("eager", "fused"):
-            raise ValueError(f"SwiGLU impl must be 'eager' or 'fused', got {impl!r}")
+        if impl not in ("eager", "fused", "projected"):
+            raise ValueError(f"SwiGLU impl must be 'eager', 'fused' or 'projected', got {impl!r}")
         inter = swiglu_intermediate(hidden_size, expansion)
         self.gate_up_proj = CastedLinear(hidden_size, 2 * inter, bias=False)
         self.down_proj = CastedLinear(inter, hidden_size, bias=False)
@@ -102,6 +130,10 @@ class SwiGLU(nn.Module):
             from ebr_amd import block
 
             return self.down_proj(block.swiglu(self.gate_up_proj(x)))
+        if self.impl == "projected":
+            from ebr_amd import block
+
+            return self.down_proj(block.swiglu_linear(x, self.gate_up_proj.weight.to(x.dtype)))
         gate, up = self.gate_up_proj(x).chunk(2, dim=-1)
         return self.down_proj(F.silu(gate) * up)
 
@@ -186,6 +218,7 @@ class RotaryTable2D(nn.Module):
 __all__ = [
     "RMS_NORM_EPS",
     "CastedLinear",
+    "LayerNorm",
     "RopeFused",
     "RotaryEmbedding2D",
     "RotaryTable2D",

@@ -54,11 +54,16 @@ def weight_grad(a: Tensor, b: Tensor) -> Tensor:
 
 def _needed(ctx, i: int) -> bool:
     node = ctx.next_functions[i][0]
-    if not ctx.needs_input_grad[i] or node is None:
-        return False
+    return ctx.needs_input_grad[i] and node is not None and _will_run(node)
+
+
+def _will_run(node) -> bool:
     if node.name().endswith("AccumulateGrad"):  # a leaf: the engine cannot say under autograd.grad, so compute it
         return True
-    return torch._C._will_engine_execute_node(node)
+    try:
+        return torch._C._will_engine_execute_node(node)
+    except RuntimeError:  # a leaf of a transform's
+        return True
 
 
 class _Dgrad(torch.autograd.Function):

@@ -1,7 +1,8 @@
 /* C ABI of the energy network's fused pointwise blocks in libebr_attn.so (gfx950): rms_norm over the last dimension
  * and the SwiGLU activation, each with its backward and the backward of that backward, as the graded latent descent
  * differentiates the energy twice; the group norm with an activation, likewise; and the ends of a training step, the
- * embedding of tokens with its table's gradient and the distillation loss with its gradient.
+ * embedding of tokens with its table's gradient and the distillation loss with its gradient; a layer norm with learned weight
+ * and bias, and the gated projection of the feed-forward block, each to second order.
  *
  * Tensors are contiguous rows of one dtype (EBR_DTYPE_F32, _BF16, _F16 or _F64). Arithmetic is fp32 (fp64 for fp64);
  * outputs are rounded once to the dtype. Conventions otherwise as in ebr_attn.h (error codes, streams, ownership).
@@ -117,6 +118,44 @@ int ebr_block_groupnorm_bwd2(int dtype, int act, int64_t B, int64_t L, int C, in
  * that they refuse: more than 2^40 - 1 elements, or 2^24 - 1 workgroups or, where these do not hold whole groups, groups of
  * all samples. */
 int64_t ebr_block_groupnorm_scratch(int dtype, int order, int64_t B, int64_t L, int C, int groups);
+
+/* y = w h + b, h = (x - mean) / sqrt(variance + eps), per row of C (at most 2^24) elements. w and b: [C] of wdtype, or NULL (1
+ * and 0). stats: [rows, 4] of fp32 (fp64 for fp64), for the derivatives: the rounded mean, what it lacks, and the factor. */
+int ebr_block_layernorm(int dtype, int wdtype, int64_t rows, int C, double eps, const void* x, const void* w, const void* b,
+                        void* y, void* stats, void* stream);
+
+/* dx, and dw and db (of wdtype; NULL where not wanted), of y given dy. Scratch of order 1, 16-byte aligned. */
+int ebr_block_layernorm_bwd(int dtype, int wdtype, int64_t rows, int C, const void* x, const void* w, const void* stats,
+                            const void* dy, void* dx, void* dw, void* db, void* scratch, void* stream);
+
+/* Gradients of <u, dx> + <uw, dw> + <ub, db> (uw, ub: of wdtype, NULL for zero) with respect to x (gx), dy (gdy) and w (gw,
+ * NULL where not wanted; b has none). Scratch of order 2. */
+int ebr_block_layernorm_bwd2(int dtype, int wdtype, int64_t rows, int C, const void* x, const void* w, const void* stats,
+                             const void* dy, const void* u, const void* uw, const void* ub, void* gx, void* gdy, void* gw,
+                             void* scratch, void* stream);
+
+/* Bytes of scratch of the layer norm's derivatives (order 1, 2), for tensors of any alignment; -1 for sizes or types that they
+ * refuse. */
+int64_t ebr_block_layernorm_scratch(int dtype, int order, int64_t rows, int C);
+
+/* y = silu(g) u for x [N, C] and w [2 I, C], gate rows first: g = x w[:I]^T, u = x w[I:]^T, summed in fp32 (fp64 for fp64) and
+ * not rounded before y [N, I]; N below 2^31, C and I below 2^20. */
+int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* stream);
+
+/* dx [N, C] and dw [2 I, C] (NULL where not wanted) of y given dy [N, I]: g and u are taken again, [dg | du] is their gradient
+ * as of ebr_block_swiglu_bwd, rounded, dx = [dg | du] w and dw = [dg | du]^T x. Scratch of order 1, 16-byte aligned. */
+int ebr_block_swiglu_linear_bwd(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
+                                void* dx, void* dw, void* scratch, void* stream);
+
+/* Gradients of <c, dx> with respect to x (gx), dy (gdy) and w (gw), c [N, C]: with [cg | cu] = c w^T in fp32, [gg | gu] (rounded)
+ * and gdy are as of ebr_block_swiglu_bwd2, gx = [gg | gu] w, gw = [gg | gu]^T x + [dg | du]^T c. gx and gw: NULL where not
+ * wanted. Scratch of order 2. */
+int ebr_block_swiglu_linear_bwd2(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
+                                 const void* c, void* gx, void* gdy, void* gw, void* scratch, void* stream);
+
+/* Bytes of scratch of the gated projection's derivatives (order 1, 2), for tensors of any alignment; -1 for sizes or types that
+ * they refuse. */
+int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I);
 
 #ifdef __cplusplus
 }
