@@ -259,91 +259,145 @@ __device__ __forceinline__ void tile_of(const Args& a, int& ti, int& tj, int& sp
     ti = (int)(in / rows);
 }
 
-template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int WJ, bool ANY>
-__global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
-    constexpr int WAVES = WI * WJ, FI = TI / WI / 32, FJ = TJ / WJ / 32;
-    constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
-    static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
-    using SA = Side<T, ALIES, TI, WAVES, GATED>;
-    using SB = Side<T, BLIES, TJ, WAVES, TWO>;
-    __shared__ __attribute__((aligned(16))) unsigned char a0[SA::BYTES], b0[SB::BYTES];
-    __shared__ __attribute__((aligned(16))) unsigned char a1[ANY ? 16 : SA::BYTES], b1[ANY ? 16 : SB::BYTES];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wi = wave % WI, wj = wave / WI;
-    int ti, tj, split;
-    tile_of(a, ti, tj, split);
-    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
-    f32x16 acc[FI][FJ];
+// A wave's way from its sums to rows of memory: planes of 32 rows of COLS values in shared memory, in chunks of 16 bytes exchanged
+// by a function of the row. A lane holds four neighbours of one row; memory gets (and gives) whole chunks, a row's side by side.
+template <typename O, int COLS> struct Plane {
+    static constexpr int PER = 16 / (int)sizeof(O), ROWB = COLS * (int)sizeof(O), CHUNKS = ROWB / 16, BYTES = 32 * ROWB;
+    static constexpr int SHIFT = ROWB == 256 ? 0 : ROWB == 128 ? 1 : 2, MOVES = BYTES / 1024;
+    static_assert(ROWB == 64 || ROWB == 128 || ROWB == 256, "rows of whole banks");
+    static __device__ __forceinline__ int place(int row, int chunk) {
+        return row * ROWB + ((chunk ^ ((row >> SHIFT) & (CHUNKS - 1))) << 4);
+    }
+    // four values of ``row`` from column ``col`` (a multiple of 4) on
+    static __device__ __forceinline__ unsigned char* four(unsigned char* at, int row, int col) {
+        return at + place(row, col / PER) + col % PER * (int)sizeof(O);
+    }
+    static __device__ __forceinline__ void put(unsigned char* at, int row, int col, const float (&v)[4]) {
+        Pack<O, 4> x;
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
+        for (int e = 0; e < 4; ++e) x.e[e] = (O)v[e];
+        stp<O, 4>(reinterpret_cast<O*>(four(at, row, col)), x);
+    }
+    static __device__ __forceinline__ void get(unsigned char* at, int row, int col, float (&v)[4]) {
+        const Pack<O, 4> x = ldp<O, 4>(reinterpret_cast<const O*>(four(at, row, col)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)x.e[e];
+    }
+    // all of it to rows of memory ``ld`` elements apart, of which ``rows`` and ``cols`` exist
+    static __device__ __forceinline__ void store(const unsigned char* at, O* to, int64_t ld, int64_t rows, int64_t cols, int lane) {
+        u32x4 v[MOVES];
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m) {
+            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
+            v[m] = *reinterpret_cast<const u32x4*>(at + place(row, chunk));
+        }
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m) {
+            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
+            if (row < rows && chunk * PER < cols) *reinterpret_cast<u32x4*>(to + row * ld + chunk * PER) = v[m];
+        }
+    }
+    static __device__ __forceinline__ void load(unsigned char* at, const O* from, int64_t ld, int64_t rows, int64_t cols, int lane) {
+        u32x4 v[MOVES];
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m) {
+            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
+            v[m] = row < rows && chunk * PER < cols ? *reinterpret_cast<const u32x4*>(from + row * ld + chunk * PER) : u32x4{};
+        }
+#pragma unroll
+        for (int m = 0; m < MOVES; ++m) {
+            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
+            *reinterpret_cast<u32x4*>(at + place(row, chunk)) = v[m];
+        }
+    }
+};
+
+// What becomes of a wave's sums, 32 rows at a time through ``at``, shared memory of its own.
+template <typename T, int EP, int FI, int FJ>
+__device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t ifrom, int64_t jfrom, int split,
+                                       unsigned char* at, int lane) {
+    constexpr bool TWO = EP == EP_BWD2;
+    const int l32 = lane & 31, il = 4 * (lane >> 5);
+    if constexpr (EP < EP_FWD) {
+        using O = std::conditional_t<EP == EP_PART, float, T>;
+        constexpr int COLS = 128 / (int)sizeof(O), EACH = COLS / 32;  // a plane's tiles of 32
+        using P = Plane<O, COLS>;
+        O* const out = reinterpret_cast<O*>(a.out) + (EP == EP_PART ? (int64_t)split * a.nj * a.ni : 0);
 #pragma unroll
         for (int j = 0; j < FJ; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-    const int64_t one = (a.nk + SA::KS - 1) / SA::KS, all = one * a.pairs;  // stages of a pair
-    int64_t step = split * a.steps;
-    const int64_t end = step + a.steps < all ? step + a.steps : all;
-    const auto multiply = [&](const unsigned char* pa, const unsigned char* pb) {
-        u32x4 fa[2][FI], fb[2][FJ];
-        const auto fragments = [&](int s) {
+            for (int i = 0; i < FI; i += EACH) {
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < FI; ++i) fa[s & 1][i] = SA::read(pa, (wi * FI + i) * 32, s, lane);
+                for (int e = 0; e < EACH; ++e)
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) fb[s & 1][j] = SB::read(pb, (wj * FJ + j) * 32, s, lane);
-        };
-        fragments(0);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (s < 3) fragments(s + 1);
-#pragma unroll
-            for (int i = 0; i < FI; ++i)
-#pragma unroll
-                for (int j = 0; j < FJ; ++j) acc[i][j] = Mma<T>::step(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
-            __builtin_amdgcn_sched_barrier(0);  // (all fragments of a stage at once would not fit the registers)
-        }
-    };
-    if constexpr (ANY) {
-        for (; step < end; ++step) {
-            const int pair = (int)(step / one);
-            const int64_t k0 = (step - pair * one) * SA::KS;
-            __syncthreads();
-            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
-            SA::load_any(pa, pa + a.ni * a.lda, i0, a.ni, a.lda, k0, a.nk, a0);
-            SB::load_any(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.nj, a.ldb, k0, a.nk, b0);
-            __syncthreads();
-            multiply(a0, b0);
-        }
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x16& s = acc[i + e][j];
+                        const float v[4] = {s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+                        P::put(at + i / EACH * P::BYTES, l32, e * 32 + 8 * q + il, v);
+                    }
+                __builtin_amdgcn_wave_barrier();
+                const int64_t row = jfrom + j * 32, col = ifrom + i * 32;
+                P::store(at + i / EACH * P::BYTES, out + row * a.ldo + col, a.ldo, a.nj - row, a.ni - col, lane);
+            }
     } else {
-        SA sa;
-        SB sb;
-        sa.offsets(i0, a.ni, a.lda, wave, lane);
-        sb.offsets(j0, a.nj, a.ldb, wave, lane);
-        // Stages in twos, the last one of an odd number with one of zeros (which costs a stage's products, but a branch out of
-        // the loop's middle would cost a second copy of all sums).
-        const auto load = [&](unsigned char* la, unsigned char* lb) {
-            const bool in = step < end;
-            const int64_t at = in ? step : end - 1;
-            const int pair = (at >= one) + (at >= 2 * one) + (at >= 3 * one);
-            const int64_t k0 = (at - pair * one) * SA::KS, left = in ? a.nk - k0 : 0;
-            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
-            sa.load(pa, pa + a.ni * a.lda, i0, a.lda, k0, left, la, wave);
-            sb.load(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.ldb, k0, left, lb, wave);
-            ++step;
-        };
-        const int64_t n = end - step;
-        load(a0, b0);
-        stage_barrier();
-        for (int64_t s = 0; s < n; s += 2) {
-            load(a1, b1);
-            multiply(a0, b0);
-            stage_barrier();
-            load(a0, b0);
-            multiply(a1, b1);
-            stage_barrier();
+        using P = Plane<T, FI * 16>;  // of gate or up, each half of the wave's rows of A
+        enum { DY = 0, Y = 0, DG = 1, DU = 2, GG = 3, GU = 4 };
+        const int64_t col = ifrom / 2, cols = a.ni - col;
+        T* const y = reinterpret_cast<T*>(a.out);
+        T *const dgu = reinterpret_cast<T*>(a.dgu), *const ggu = reinterpret_cast<T*>(a.ggu);
+#pragma unroll
+        for (int j = 0; j < FJ; j += TWO ? 2 : 1) {
+            const int64_t row = TWO ? jfrom / 2 + j * 16 : jfrom + j * 32, rows = a.nj - row;
+            const int64_t one = row * a.ni + col, two = row * 2 * a.ni + col;
+            __builtin_amdgcn_wave_barrier();
+            if constexpr (EP != EP_FWD) P::load(at + DY * P::BYTES, reinterpret_cast<const T*>(a.dy) + one, a.ni, rows, cols, lane);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < FI; i += 2)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = i * 16 + 8 * q + il;
+                    float dy[4], o[4], og[4], ou[4], rg[4], ru[4];
+                    if constexpr (EP != EP_FWD) P::get(at + DY * P::BYTES, l32, c, dy);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float g = acc[i][j][4 * q + e], u = acc[i + 1][j][4 * q + e];
+                        if constexpr (EP == EP_FWD) o[e] = gated(g, u);
+                        else first_of(g, u, dy[e], og[e], ou[e]);
+                        if constexpr (TWO)
+                            second_of(g, u, dy[e], acc[i][j + 1][4 * q + e], acc[i + 1][j + 1][4 * q + e], rg[e], ru[e], o[e]);
+                    }
+                    if constexpr (EP != EP_BWD) P::put(at + Y * P::BYTES, l32, c, o);
+                    if constexpr (EP != EP_FWD) {
+                        P::put(at + DG * P::BYTES, l32, c, og);
+                        P::put(at + DU * P::BYTES, l32, c, ou);
+                    }
+                    if constexpr (TWO) {
+                        P::put(at + GG * P::BYTES, l32, c, rg);
+                        P::put(at + GU * P::BYTES, l32, c, ru);
+                    }
+                }
+            __builtin_amdgcn_wave_barrier();
+            if constexpr (EP != EP_BWD) P::store(at + Y * P::BYTES, y + one, a.ni, rows, cols, lane);
+            if (EP == EP_BWD || (TWO && dgu)) {
+                P::store(at + DG * P::BYTES, dgu + two, 2 * a.ni, rows, cols, lane);
+                P::store(at + DU * P::BYTES, dgu + two + a.ni, 2 * a.ni, rows, cols, lane);
+            }
+            if (TWO && ggu) {
+                P::store(at + GG * P::BYTES, ggu + two, 2 * a.ni, rows, cols, lane);
+                P::store(at + GU * P::BYTES, ggu + two + a.ni, 2 * a.ni, rows, cols, lane);
+            }
         }
     }
+}
 
+// The same straight from the registers, for tensors of any width and alignment and for few rows (what [dg|du] lacks of its
+// values before rounding is written here alone).
+template <typename T, int EP, int FI, int FJ, bool ANY>
+__device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t i0, int64_t j0, int wi, int wj,
+                                           int split, int lane) {
+    constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
     const int64_t jl = j0 + wj * FJ * 32 + (lane & 31);
     const int il = 4 * (lane >> 5);
     if constexpr (!GATED) {
@@ -408,6 +462,114 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
                     }
                 }
         }
+    }
+}
+
+template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int WJ, bool ANY>
+__global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
+    constexpr int WAVES = WI * WJ, FI = TI / WI / 32, FJ = TJ / WJ / 32;
+    constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
+    constexpr bool STAGED = !ANY && sizeof(T) == 2 && TI >= 128;  // four waves, an array each
+    static_assert(!STAGED || WAVES == 4, "an array a wave");
+    static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
+    using SA = Side<T, ALIES, TI, WAVES, GATED>;
+    using SB = Side<T, BLIES, TJ, WAVES, TWO>;
+    __shared__ __attribute__((aligned(16))) unsigned char a0[SA::BYTES], b0[SB::BYTES];
+    __shared__ __attribute__((aligned(16))) unsigned char a1[ANY ? 16 : SA::BYTES], b1[ANY ? 16 : SB::BYTES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave % WI, wj = wave / WI;
+    int ti, tj, split;
+    tile_of(a, ti, tj, split);
+    const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
+    f32x16 acc[FI][FJ];
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    const int64_t one = (a.nk + SA::KS - 1) / SA::KS, all = one * a.pairs;  // stages of a pair
+    int64_t step = split * a.steps;
+    const int64_t end = step + a.steps < all ? step + a.steps : all;
+    u32x4 fa[2][FI], fb[2][FJ];
+    const auto read = [&](const unsigned char* pa, const unsigned char* pb, int s) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i) fa[s & 1][i] = SA::read(pa, (wi * FI + i) * 32, s, lane);
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) fb[s & 1][j] = SB::read(pb, (wj * FJ + j) * 32, s, lane);
+    };
+    const auto multiply = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) acc[i][j] = Mma<T>::step(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);  // (all fragments of a stage at once would not fit the registers)
+    };
+    if constexpr (ANY) {
+        for (; step < end; ++step) {
+            const int pair = (int)(step / one);
+            const int64_t k0 = (step - pair * one) * SA::KS;
+            __syncthreads();
+            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
+            SA::load_any(pa, pa + a.ni * a.lda, i0, a.ni, a.lda, k0, a.nk, a0);
+            SB::load_any(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.nj, a.ldb, k0, a.nk, b0);
+            __syncthreads();
+            read(a0, b0, 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (q < 3) read(a0, b0, q + 1);
+                multiply(q);
+            }
+        }
+    } else {
+        SA sa;
+        SB sb;
+        sa.offsets(i0, a.ni, a.lda, wave, lane);
+        sb.offsets(j0, a.nj, a.ldb, wave, lane);
+        // Stages in twos, the last one of an odd number with one of zeros (which costs a stage's products, but a branch out of
+        // the loop's middle would cost a second copy of all sums).
+        const auto load = [&](unsigned char* la, unsigned char* lb) {
+            const bool in = step < end;
+            const int64_t at = in ? step : end - 1;
+            const int pair = (at >= one) + (at >= 2 * one) + (at >= 3 * one);
+            const int64_t k0 = (at - pair * one) * SA::KS, left = in ? a.nk - k0 : 0;
+            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
+            sa.load(pa, pa + a.ni * a.lda, i0, a.lda, k0, left, la, wave);
+            sb.load(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.ldb, k0, left, lb, wave);
+            ++step;
+        };
+        // A stage's last products run while the next one's first fragments are read, after the barrier that says that its loads
+        // are there and that nobody reads this stage's buffer any more, which the loads after next go to.
+        const int64_t n = end - step;
+        const auto stage = [&](unsigned char* pa, unsigned char* pb, const unsigned char* na, const unsigned char* nb) {
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                read(pa, pb, q + 1);
+                multiply(q);
+            }
+            stage_barrier();
+            load(pa, pb);
+            read(na, nb, 0);
+            multiply(3);
+        };
+        load(a0, b0);
+        stage_barrier();
+        load(a1, b1);
+        read(a0, b0, 0);
+        for (int64_t s = 0; s < n; s += 2) {
+            stage(a0, b0, a1, b1);
+            stage(a1, b1, a0, b0);
+        }
+        stage_barrier();  // (the loads past the end, of zeros, are done with the buffers)
+    }
+
+    if constexpr (STAGED) {
+        // (every wave is past its last read of the buffers: the last stage's barrier)
+        unsigned char* const own = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1;
+        finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, split, own, lane);
+    } else {
+        finish_any<T, EP, FI, FJ, ANY>(a, acc, i0, j0, wi, wj, split, lane);
     }
 }
 
@@ -537,7 +699,7 @@ template <typename T, int ALIES, int BLIES, int EP, bool ANY> static void launch
     } else {
         if constexpr (!ANY && sizeof(T) == 2) {
             if (c.tile == 256) {
-                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 4, 2, ANY>), grid, dim3(512), 0, s, a);
+                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 2, 2, ANY>), grid, dim3(256), 0, s, a);
                 return;
             }
         }
