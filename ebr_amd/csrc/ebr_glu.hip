@@ -115,16 +115,17 @@ template <typename T, int LIES, int ROWS, int WAVES, bool PAIRED> struct Side {
             }
         }
     }
-    // Loads the stage at k0, of which ``rest`` k are left, into ``to``.
-    __device__ __forceinline__ void load(const T* base, const T* base2, int64_t first, int64_t ld, int64_t k0, int64_t rest,
-                                         unsigned char* to, int wave) const {
+    // How far the tile's place at k0 lies from the operand's.
+    static __device__ __forceinline__ int64_t skip(int64_t first, int64_t ld, int64_t k0) {
+        return LIES == K_ROWS ? (PAIRED ? first / 2 : first) * ld + k0 : first + k0 * ld;
+    }
+    // Loads the stage at p (and, of a pair's other operand, p2), of which ``left`` k exist, into ``to``.
+    __device__ __forceinline__ void load(const T* p, const T* p2, int left, unsigned char* to, int wave) const {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass has no buffers)
         constexpr int RAW = 0x00020000;  // dwords as they are
-        const int64_t skip = LIES == K_ROWS ? (PAIRED ? first / 2 : first) * ld + k0 : first + k0 * ld;
-        const int left = rest < KS ? (int)rest : KS;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + skip), 0, (int)OUTSIDE, RAW);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)OUTSIDE, RAW);
         __amdgpu_buffer_rsrc_t r2 = r;
-        if constexpr (PAIRED) r2 = __builtin_amdgcn_make_buffer_rsrc((void*)(base2 + skip), 0, (int)OUTSIDE, RAW);
+        if constexpr (PAIRED) r2 = __builtin_amdgcn_make_buffer_rsrc((void*)p2, 0, (int)OUTSIDE, RAW);
 #pragma unroll
         for (int q = 0; q < LOADS; ++q) {
             const int at = wave * LOADS + q;  // (a load's 8 rows are of one operand)
@@ -504,6 +505,14 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
         for (int i = 0; i < FI; ++i)
 #pragma unroll
             for (int j = 0; j < FJ; ++j) acc[i][j] = Mma<T>::step(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+        // the next fragments' reads between the first products, so that they are there after the last ones
+        constexpr int READS = FI * (ALIES == K_ROWS ? 1 : sizeof(T) == 2 ? 2 : 4) + FJ * (BLIES == K_ROWS ? 1 : sizeof(T) == 2 ? 2 : 4);
+        constexpr int MM = FI * FJ * (sizeof(T) == 2 ? 1 : 4), EACH = (READS + MM / 2 - 1) / (MM / 2 > 0 ? MM / 2 : 1);
+#pragma unroll
+        for (int g = 0; g < MM / 2; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);  // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // a product
+        }
         __builtin_amdgcn_sched_barrier(0);  // (all fragments of a stage at once would not fit the registers)
     };
     if constexpr (ANY) {
@@ -529,31 +538,52 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
         sb.offsets(j0, a.nj, a.ldb, wave, lane);
         // Stages in twos, the last one of an odd number with one of zeros (which costs a stage's products, but a branch out of
         // the loop's middle would cost a second copy of all sums).
-        const auto load = [&](unsigned char* la, unsigned char* lb) {
-            const bool in = step < end;
-            const int64_t at = in ? step : end - 1;
-            const int pair = (at >= one) + (at >= 2 * one) + (at >= 3 * one);
-            const int64_t k0 = (at - pair * one) * SA::KS, left = in ? a.nk - k0 : 0;
-            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
-            sa.load(pa, pa + a.ni * a.lda, i0, a.lda, k0, left, la, wave);
-            sb.load(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.ldb, k0, left, lb, wave);
+        const T *pa = nullptr, *pb = nullptr, *pa2 = nullptr, *pb2 = nullptr;  // of the stage to be loaded next
+        int64_t rest = 0;  // its k and those after it in its pair
+        const auto begin = [&]() {
+            const int pair = (int)(step / one);
+            const int64_t k0 = (step - pair * one) * SA::KS;
+            const int64_t ia = SA::skip(i0, a.lda, k0), ib = SB::skip(j0, a.ldb, k0);
+            pa = reinterpret_cast<const T*>(a.a[pair]) + ia;
+            pb = reinterpret_cast<const T*>(a.b[pair]) + ib;
+            if (GATED) pa2 = pa + a.ni * a.lda;
+            if (TWO) pb2 = reinterpret_cast<const T*>(a.c) + ib;
+            rest = a.nk - k0;
+        };
+        const int64_t sa_step = ALIES == K_ROWS ? SA::KS : SA::KS * a.lda, sb_step = BLIES == K_ROWS ? SB::KS : SB::KS * a.ldb;
+        const auto advance = [&]() {
             ++step;
+            rest -= SA::KS;
+            pa += sa_step;
+            pb += sb_step;
+            if (GATED) pa2 += sa_step;
+            if (TWO) pb2 += sb_step;
+            if (step >= end) rest = 0;
+            else if (rest <= 0) begin();
+        };
+        const auto load = [&](unsigned char* la, unsigned char* lb) {
+            const int left = rest < SA::KS ? (int)rest : SA::KS;
+            sa.load(pa, pa2, left, la, wave);
+            sb.load(pb, pb2, left, lb, wave);
         };
         // A stage's last products run while the next one's first fragments are read, after the barrier that says that its loads
         // are there and that nobody reads this stage's buffer any more, which the loads after next go to.
         const int64_t n = end - step;
-        const auto stage = [&](unsigned char* pa, unsigned char* pb, const unsigned char* na, const unsigned char* nb) {
+        const auto stage = [&](unsigned char* la, unsigned char* lb, const unsigned char* na, const unsigned char* nb) {
 #pragma unroll
             for (int q = 0; q < 3; ++q) {
-                read(pa, pb, q + 1);
+                read(la, lb, q + 1);
+                if (q == 2) advance();
                 multiply(q);
             }
             stage_barrier();
-            load(pa, pb);
+            load(la, lb);
             read(na, nb, 0);
             multiply(3);
         };
+        begin();
         load(a0, b0);
+        advance();
         stage_barrier();
         load(a1, b1);
         read(a0, b0, 0);
