@@ -11,9 +11,9 @@
 // The derivatives take g and u again: kept rounded they would double the gradients' errors, and of C below about a thousand
 // the product costs less than moving them.
 //
-// A workgroup's tile of TI x TJ steps through k in stages of 128 bytes an operand row, each stage loaded straight into shared
-// memory while the one before is multiplied. The two buffers are separate arrays: the compiler then knows that the loads
-// under way do not concern the reads, and does not wait for them. Rows' 16-byte chunks (64-byte chunks for operands of the
+// A workgroup's tile of TI x TJ steps through k in stages of 64 bytes an operand row, loaded straight into shared memory three
+// stages ahead. The four buffers are separate arrays: the compiler then knows that the loads under way do not concern the
+// reads, and does not wait for them. Rows' 16-byte chunks (64-byte chunks for operands of the
 // second kind, which are read transposed) are exchanged by a function of the row, so that lanes meet no bank conflicts.
 // Whatever lies outside the tensors is read as zero by the buffer loads' bounds.
 #include <type_traits>
@@ -37,7 +37,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 enum { K_ROWS = 0, M_ROWS = 1 };                                  // how an operand lies
 enum { EP_OUT = 0, EP_PART = 1, EP_FWD = 2, EP_BWD = 3, EP_BWD2 = 4 };  // what becomes of D: y, [dg|du], or all of bwd2's
-constexpr int STAGE = 128;                                        // bytes of k a stage
+constexpr int STAGE = 64;                                         // bytes of k a stage
 constexpr uint32_t OUTSIDE = 0x40000000;                          // an offset past a buffer's end
 
 struct Args {
@@ -86,7 +86,7 @@ template <typename T, int LIES, int ROWS, int WAVES, bool PAIRED> struct Side {
     static __device__ __forceinline__ void chunk(int p, int& row, int& at) {
         row = p * 16 / ROWB;
         const int c = p - row * (ROWB / 16);
-        if constexpr (LIES == K_ROWS) at = (c ^ ((row >> 1) & 7)) * EPC;
+        if constexpr (LIES == K_ROWS) at = (c ^ ((row >> 2) & 3)) * EPC;
         else at = ((((c >> 2) ^ (row & MASK)) << 2) | (c & 3)) * EPC;
     }
     // Row r of the tile that begins at row ``first``, in the operand, or -1 where there is none. PAIRED: rows of the two
@@ -128,8 +128,8 @@ template <typename T, int LIES, int ROWS, int WAVES, bool PAIRED> struct Side {
         if constexpr (PAIRED) r2 = __builtin_amdgcn_make_buffer_rsrc((void*)p2, 0, (int)OUTSIDE, RAW);
 #pragma unroll
         for (int q = 0; q < LOADS; ++q) {
-            const int at = wave * LOADS + q;  // (a load's 8 rows are of one operand)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(other(at * 8) ? r2 : r, (EBR_LDS void*)(to + at * 1024), 16,
+            const int at = wave * LOADS + q;  // (a load's 16 rows are of one operand)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(other(at * 16) ? r2 : r, (EBR_LDS void*)(to + at * 1024), 16,
                                                      kat[q] < left ? off[q] : OUTSIDE, 0, 0, 0);
         }
 #endif
@@ -159,7 +159,7 @@ template <typename T, int LIES, int ROWS, int WAVES, bool PAIRED> struct Side {
         const int l32 = lane & 31, half = lane >> 5;
         if constexpr (LIES == K_ROWS) {
             const int row = r0 + l32;
-            return *reinterpret_cast<const u32x4*>(from + row * ROWB + (((2 * s + half) ^ ((row >> 1) & 7)) << 4));
+            return *reinterpret_cast<const u32x4*>(from + row * ROWB + (((2 * s + half) ^ ((row >> 2) & 3)) << 4));
         } else if constexpr (ES == 2) {
             const int l16 = lane & 15, k = 16 * s + 8 * half + (l16 >> 2), col = (r0 + (lane & 16) + 4 * (l16 & 3)) * ES;
             const unsigned char* p = from + k * ROWB + ((((col >> 6) ^ (k & MASK)) << 6) | (col & 63));
@@ -238,10 +238,11 @@ template <typename T> __device__ __forceinline__ void get4(const T* p, float (&v
     }
 }
 
-// All of a wave's memory operations done, and every wave there.
-__device__ __forceinline__ void stage_barrier() {
+// All of a wave's reads of shared memory done, and all but its last N loads; and every wave there.
+template <int N> __device__ __forceinline__ void stage_barrier() {
+    static_assert(N < 64, "vmcnt");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -475,8 +476,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
     using SA = Side<T, ALIES, TI, WAVES, GATED>;
     using SB = Side<T, BLIES, TJ, WAVES, TWO>;
-    __shared__ __attribute__((aligned(16))) unsigned char a0[SA::BYTES], b0[SB::BYTES];
-    __shared__ __attribute__((aligned(16))) unsigned char a1[ANY ? 16 : SA::BYTES], b1[ANY ? 16 : SB::BYTES];
+    constexpr int BUFFER = SA::BYTES + SB::BYTES, MORE = ANY ? 16 : BUFFER;
+    __shared__ __attribute__((aligned(16))) unsigned char s0[BUFFER], s1[MORE], s2[MORE], s3[MORE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave % WI, wj = wave / WI;
     int ti, tj, split;
@@ -494,24 +495,27 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     int64_t step = split * a.steps;
     const int64_t end = step + a.steps < all ? step + a.steps : all;
     u32x4 fa[2][FI], fb[2][FJ];
-    const auto read = [&](const unsigned char* pa, const unsigned char* pb, int s) {
+    const auto read = [&](const unsigned char* from, int s) {
 #pragma unroll
-        for (int i = 0; i < FI; ++i) fa[s & 1][i] = SA::read(pa, (wi * FI + i) * 32, s, lane);
+        for (int i = 0; i < FI; ++i) fa[s][i] = SA::read(from, (wi * FI + i) * 32, s, lane);
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) fb[s & 1][j] = SB::read(pb, (wj * FJ + j) * 32, s, lane);
+        for (int j = 0; j < FJ; ++j) fb[s][j] = SB::read(from + SA::BYTES, (wj * FJ + j) * 32, s, lane);
     };
     const auto multiply = [&](int s) {
 #pragma unroll
         for (int i = 0; i < FI; ++i)
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) acc[i][j] = Mma<T>::step(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
-        // the next fragments' reads between the first products, so that they are there after the last ones
+            for (int j = 0; j < FJ; ++j) acc[i][j] = Mma<T>::step(fa[s][i], fb[s][j], acc[i][j]);
+        // the next fragments' reads (and the next stage's loads) between the first products, so that they are there after the
+        // last ones
         constexpr int READS = FI * (ALIES == K_ROWS ? 1 : sizeof(T) == 2 ? 2 : 4) + FJ * (BLIES == K_ROWS ? 1 : sizeof(T) == 2 ? 2 : 4);
         constexpr int MM = FI * FJ * (sizeof(T) == 2 ? 1 : 4), EACH = (READS + MM / 2 - 1) / (MM / 2 > 0 ? MM / 2 : 1);
+        constexpr int GO = (SA::LOADS + SB::LOADS + MM / 2 - 1) / (MM / 2 > 0 ? MM / 2 : 1);
 #pragma unroll
         for (int g = 0; g < MM / 2; ++g) {
-            __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);  // LDS reads
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // a product
+            __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);             // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                // a product
+            if (s == 1) __builtin_amdgcn_sched_group_barrier(0x020, GO, 0);  // loads
         }
         __builtin_amdgcn_sched_barrier(0);  // (all fragments of a stage at once would not fit the registers)
     };
@@ -521,82 +525,84 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
             const int64_t k0 = (step - pair * one) * SA::KS;
             __syncthreads();
             const T* pa = reinterpret_cast<const T*>(a.a[pair]);
-            SA::load_any(pa, pa + a.ni * a.lda, i0, a.ni, a.lda, k0, a.nk, a0);
-            SB::load_any(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.nj, a.ldb, k0, a.nk, b0);
+            SA::load_any(pa, pa + a.ni * a.lda, i0, a.ni, a.lda, k0, a.nk, s0);
+            SB::load_any(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.nj, a.ldb, k0, a.nk,
+                         s0 + SA::BYTES);
             __syncthreads();
-            read(a0, b0, 0);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (q < 3) read(a0, b0, q + 1);
-                multiply(q);
-            }
+            read(s0, 0);
+            read(s0, 1);
+            multiply(0);
+            multiply(1);
         }
     } else {
         SA sa;
         SB sb;
         sa.offsets(i0, a.ni, a.lda, wave, lane);
         sb.offsets(j0, a.nj, a.ldb, wave, lane);
-        // Stages in twos, the last one of an odd number with one of zeros (which costs a stage's products, but a branch out of
-        // the loop's middle would cost a second copy of all sums).
-        const T *pa = nullptr, *pb = nullptr, *pa2 = nullptr, *pb2 = nullptr;  // of the stage to be loaded next
-        int64_t rest = 0;  // its k and those after it in its pair
-        const auto begin = [&]() {
-            const int pair = (int)(step / one);
-            const int64_t k0 = (step - pair * one) * SA::KS;
-            const int64_t ia = SA::skip(i0, a.lda, k0), ib = SB::skip(j0, a.ldb, k0);
-            pa = reinterpret_cast<const T*>(a.a[pair]) + ia;
-            pb = reinterpret_cast<const T*>(a.b[pair]) + ib;
-            if (GATED) pa2 = pa + a.ni * a.lda;
-            if (TWO) pb2 = reinterpret_cast<const T*>(a.c) + ib;
-            rest = a.nk - k0;
-        };
+        const T *pa, *pb, *pa2 = nullptr, *pb2 = nullptr;  // of the stage to be loaded next
+        int rest;                                          // its k and those after it
         const int64_t sa_step = ALIES == K_ROWS ? SA::KS : SA::KS * a.lda, sb_step = BLIES == K_ROWS ? SB::KS : SB::KS * a.ldb;
         const auto advance = [&]() {
-            ++step;
             rest -= SA::KS;
             pa += sa_step;
             pb += sb_step;
             if (GATED) pa2 += sa_step;
             if (TWO) pb2 += sb_step;
-            if (step >= end) rest = 0;
-            else if (rest <= 0) begin();
         };
-        const auto load = [&](unsigned char* la, unsigned char* lb) {
-            const int left = rest < SA::KS ? (int)rest : SA::KS;
-            sa.load(pa, pa2, left, la, wave);
-            sb.load(pb, pb2, left, lb, wave);
+        const auto load = [&](unsigned char* to) {
+            const int left = rest < SA::KS ? rest : SA::KS;  // (none past the end: the loads read nothing and write zeros)
+            sa.load(pa, pa2, left, to, wave);
+            sb.load(pb, pb2, left, to + SA::BYTES, wave);
         };
         // A stage's last products run while the next one's first fragments are read, after the barrier that says that its loads
-        // are there and that nobody reads this stage's buffer any more, which the loads after next go to.
-        const int64_t n = end - step;
-        const auto stage = [&](unsigned char* la, unsigned char* lb, const unsigned char* na, const unsigned char* nb) {
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-                read(la, lb, q + 1);
-                if (q == 2) advance();
-                multiply(q);
-            }
-            stage_barrier();
-            load(la, lb);
-            read(na, nb, 0);
-            multiply(3);
+        // are there and that nobody reads this stage's buffer any more, which the loads of the fourth stage from here go to:
+        // loads have three stages' time.
+        constexpr int AHEAD = 2 * (SA::LOADS + SB::LOADS);  // of a wave, of the two stages after the next
+        const auto stage = [&](unsigned char* here, const unsigned char* next) {
+            read(here, 1);
+            multiply(0);
+            advance();
+            stage_barrier<AHEAD>();
+            load(here);
+            read(next, 0);
+            multiply(1);
         };
-        begin();
-        load(a0, b0);
-        advance();
-        stage_barrier();
-        load(a1, b1);
-        read(a0, b0, 0);
-        for (int64_t s = 0; s < n; s += 2) {
-            stage(a0, b0, a1, b1);
-            stage(a1, b1, a0, b0);
+        for (int pair = 0; pair < a.pairs; ++pair) {
+            // this split's stages of the pair: in fours, what lacks of them with zeros (which costs their products, but a branch
+            // out of the loop's middle would cost a second copy of all sums)
+            const int64_t from = step > pair * one ? step - pair * one : 0, to = end < (pair + 1) * one ? end - pair * one : one;
+            if (from >= to) continue;
+            const int64_t k0 = from * SA::KS, k1 = to * SA::KS < a.nk ? to * SA::KS : a.nk;
+            const int64_t ia = SA::skip(i0, a.lda, k0), ib = SB::skip(j0, a.ldb, k0);
+            pa = reinterpret_cast<const T*>(a.a[pair]) + ia;
+            pb = reinterpret_cast<const T*>(a.b[pair]) + ib;
+            if (GATED) pa2 = pa + a.ni * a.lda;
+            if (TWO) pb2 = reinterpret_cast<const T*>(a.c) + ib;
+            rest = (int)(k1 - k0);
+            const int n = (int)(to - from);
+            if (pair > 0) stage_barrier<0>();  // (the loads past the last pair's end are done with the buffers)
+            load(s0);
+            advance();
+            load(s1);
+            advance();
+            load(s2);
+            stage_barrier<AHEAD>();
+            advance();
+            load(s3);
+            read(s0, 0);
+            for (int s = 0; s < n; s += 4) {
+                stage(s0, s1);
+                stage(s1, s2);
+                stage(s2, s3);
+                stage(s3, s0);
+            }
         }
-        stage_barrier();  // (the loads past the end, of zeros, are done with the buffers)
+        stage_barrier<0>();  // (the loads past the end, of zeros, are done with the buffers)
     }
 
     if constexpr (STAGED) {
         // (every wave is past its last read of the buffers: the last stage's barrier)
-        unsigned char* const own = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1;
+        unsigned char* const own = wave == 0 ? s0 : wave == 1 ? s1 : wave == 2 ? s2 : s3;
         finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, split, own, lane);
     } else {
         finish_any<T, EP, FI, FJ, ANY>(a, acc, i0, j0, wi, wj, split, lane);
