@@ -285,34 +285,44 @@ template <typename O, int COLS> struct Plane {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (float)x.e[e];
     }
-    // all of it to rows of memory ``ld`` elements apart, of which ``rows`` and ``cols`` exist
-    static __device__ __forceinline__ void store(const unsigned char* at, O* to, int64_t ld, int64_t rows, int64_t cols, int lane) {
+    // all of it to (from) rows of memory ``ld`` elements apart, of which ``rows`` and ``cols`` exist: a move takes STEP rows
+    static constexpr int STEP = 64 / CHUNKS;
+    static __device__ __forceinline__ uint32_t offset(int64_t ld, int lane) {
+        return (uint32_t)(lane / CHUNKS * (int)ld + lane % CHUNKS * PER) * (uint32_t)sizeof(O);
+    }
+    static __device__ __forceinline__ bool there(int m, int rows, int cols, int lane) {
+        return m * STEP + lane / CHUNKS < rows && lane % CHUNKS * PER < cols;
+    }
+    static __device__ __forceinline__ void store(const unsigned char* at, O* to, int64_t ld, int rows, int cols, int lane) {
         u32x4 v[MOVES];
 #pragma unroll
-        for (int m = 0; m < MOVES; ++m) {
-            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
-            v[m] = *reinterpret_cast<const u32x4*>(at + place(row, chunk));
-        }
+        for (int m = 0; m < MOVES; ++m)
+            v[m] = *reinterpret_cast<const u32x4*>(at + place(m * STEP + lane / CHUNKS, lane % CHUNKS));
+        char* base = reinterpret_cast<char*>(to);
+        const uint32_t off = offset(ld, lane);
 #pragma unroll
         for (int m = 0; m < MOVES; ++m) {
-            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
-            if (row < rows && chunk * PER < cols) *reinterpret_cast<u32x4*>(to + row * ld + chunk * PER) = v[m];
+            if (there(m, rows, cols, lane)) *reinterpret_cast<u32x4*>(base + off) = v[m];
+            base += STEP * ld * (int64_t)sizeof(O);
         }
     }
-    static __device__ __forceinline__ void load(unsigned char* at, const O* from, int64_t ld, int64_t rows, int64_t cols, int lane) {
+    static __device__ __forceinline__ void load(unsigned char* at, const O* from, int64_t ld, int rows, int cols, int lane) {
         u32x4 v[MOVES];
+        const char* base = reinterpret_cast<const char*>(from);
+        const uint32_t off = offset(ld, lane);
 #pragma unroll
         for (int m = 0; m < MOVES; ++m) {
-            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
-            v[m] = row < rows && chunk * PER < cols ? *reinterpret_cast<const u32x4*>(from + row * ld + chunk * PER) : u32x4{};
+            v[m] = there(m, rows, cols, lane) ? *reinterpret_cast<const u32x4*>(base + off) : u32x4{};
+            base += STEP * ld * (int64_t)sizeof(O);
         }
 #pragma unroll
-        for (int m = 0; m < MOVES; ++m) {
-            const int p = m * 64 + lane, row = p / CHUNKS, chunk = p % CHUNKS;
-            *reinterpret_cast<u32x4*>(at + place(row, chunk)) = v[m];
-        }
+        for (int m = 0; m < MOVES; ++m)
+            *reinterpret_cast<u32x4*>(at + place(m * STEP + lane / CHUNKS, lane % CHUNKS)) = v[m];
     }
 };
+
+// How many of a plane's rows or columns there are: none where it lies outside.
+__device__ __forceinline__ int left(int64_t n) { return n > 256 ? 256 : (int)n; }
 
 // What becomes of a wave's sums, 32 rows at a time through ``at``, shared memory of its own.
 template <typename T, int EP, int FI, int FJ>
@@ -340,17 +350,19 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
                     }
                 __builtin_amdgcn_wave_barrier();
                 const int64_t row = jfrom + j * 32, col = ifrom + i * 32;
-                P::store(at + i / EACH * P::BYTES, out + row * a.ldo + col, a.ldo, a.nj - row, a.ni - col, lane);
+                P::store(at + i / EACH * P::BYTES, out + row * a.ldo + col, a.ldo, left(a.nj - row), left(a.ni - col), lane);
             }
     } else {
         using P = Plane<T, FI * 16>;  // of gate or up, each half of the wave's rows of A
         enum { DY = 0, Y = 0, DG = 1, DU = 2, GG = 3, GU = 4 };
-        const int64_t col = ifrom / 2, cols = a.ni - col;
+        const int64_t col = ifrom / 2;
+        const int cols = left(a.ni - col);
         T* const y = reinterpret_cast<T*>(a.out);
         T *const dgu = reinterpret_cast<T*>(a.dgu), *const ggu = reinterpret_cast<T*>(a.ggu);
 #pragma unroll
         for (int j = 0; j < FJ; j += TWO ? 2 : 1) {
-            const int64_t row = TWO ? jfrom / 2 + j * 16 : jfrom + j * 32, rows = a.nj - row;
+            const int64_t row = TWO ? jfrom / 2 + j * 16 : jfrom + j * 32;
+            const int rows = left(a.nj - row);
             const int64_t one = row * a.ni + col, two = row * 2 * a.ni + col;
             __builtin_amdgcn_wave_barrier();
             if constexpr (EP != EP_FWD) P::load(at + DY * P::BYTES, reinterpret_cast<const T*>(a.dy) + one, a.ni, rows, cols, lane);
@@ -379,6 +391,7 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
                         P::put(at + GG * P::BYTES, l32, c, rg);
                         P::put(at + GU * P::BYTES, l32, c, ru);
                     }
+                    if constexpr (EP != EP_FWD) __builtin_amdgcn_sched_barrier(0);  // (several at once would not fit the registers)
                 }
             __builtin_amdgcn_wave_barrier();
             if constexpr (EP != EP_BWD) P::store(at + Y * P::BYTES, y + one, a.ni, rows, cols, lane);
@@ -567,7 +580,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
             read(next, 0);
             multiply(1);
         };
-        for (int pair = 0; pair < a.pairs; ++pair) {
+        for (int pair = 0; pair < (GATED ? 1 : a.pairs); ++pair) {
             // this split's stages of the pair: in fours, what lacks of them with zeros (which costs their products, but a branch
             // out of the loop's middle would cost a second copy of all sums)
             const int64_t from = step > pair * one ? step - pair * one : 0, to = end < (pair + 1) * one ? end - pair * one : one;

@@ -7,9 +7,9 @@
 // gradients once more for the norm. The step's factors (powers of the betas, the clipping) are taken once a tensor by
 // k_factors, which also counts the step.
 //
-// Moments in 8 bits are taken in fp64: a moment next to the border between two numbers goes to the same side in any order of
-// operations, and the arithmetic (some 70 operations an element) still fits under the loads. A wave takes the 256 elements of
-// one scale, four a lane, so that the block's largest needs no shared memory.
+// Moments in 8 bits are what fp64 makes of them: a moment next to the border between two numbers goes to the same side in any
+// order of operations. A wave takes the 256 elements of one scale, four a lane, in fp32, with a bound on how far each is off,
+// and again in fp64 where that reaches over a border.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -22,7 +22,8 @@ namespace ebr_opt {
 using namespace ebr_row;
 
 constexpr int THREADS = 256, BLOCK = 256, TENSORS = 48, GRADS = 144;
-constexpr int64_t LEAST = 4096, MOST = 65536;  // elements of a workgroup
+constexpr int AT_ONCE = 4;                         // vectors under way in the norm
+constexpr int64_t STEP = 1024, LEAST = 4096, MOST = 65536;  // elements of a workgroup: of a step, and of the norm
 
 // What a step multiplies by, for one tensor.
 struct alignas(16) Factors {
@@ -52,6 +53,7 @@ struct Sums {
     int64_t n[GRADS];
     int first[GRADS + 1], dtype[GRADS];
     int count, per;
+    int wide;  // an fp64 gradient is among them: all sums in fp64
     double* part;
 };
 
@@ -164,76 +166,223 @@ __device__ __forceinline__ double wave_max(double v) {
     return v;
 }
 
+// What a wave knows of its 256 elements: four a lane.
+struct Eight {
+    float p[4], g[4];
+    uint32_t m[4], v[4];
+    float ms, vs;
+    uint32_t at;  // the first one's number, times the dither's factor, plus the step's part
+};
+__device__ __forceinline__ double dither(uint32_t w) { return (double)(w >> 8) * 0x1p-24; }
+__device__ __forceinline__ float number(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
+
+// The step in fp64; the parameters of ``done`` (a bit each) have theirs.
+__device__ __forceinline__ void step64(Eight& x, const Table& a, const Factors& f, int done) {
+    const float step = (float)f.step, rt = (float)f.root, decay = (float)f.decay, eps = (float)a.eps;
+    double mv[4], rv[4], mt = 0, vt = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const double ge = (double)x.g[e] * f.clip, r = (double)number(x.v[e]) * (double)x.vs;
+        mv[e] = a.beta1 * ((double)number(x.m[e]) * (double)x.ms) + a.rest1 * ge;
+        rv[e] = sqrt(a.beta2 * (r * r) + a.rest2 * (ge * ge));
+        mt = fmax(mt, fabs(mv[e]));
+        vt = fmax(vt, rv[e]);
+        if (!(done >> e & 1)) x.p[e] = x.p[e] * decay - step * (float)mv[e] / ((float)rv[e] * rt + eps);
+    }
+    mt = wave_max(mt) / 448.0;
+    vt = wave_max(vt) / 448.0;
+    const bool some_m = !(mt < 0x1p-126), some_v = !(vt < 0x1p-126);
+    const double im = some_m ? 1.0 / mt : 0.0, iv = some_v ? 1.0 / vt : 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t w = x.at + (uint32_t)e * 0x85EBCA77u;
+        x.m[e] = e4m3(fabs(mv[e]) * im, dither(w)) | (mv[e] < 0 ? 0x80u : 0u);
+        x.v[e] = e4m3(rv[e] * iv, dither(w + 0x80000000u));
+        if (some_v && rv[e] > 0 && x.v[e] == 0) x.v[e] = 1;
+    }
+    x.ms = some_m ? (float)mt : 0.f;
+    x.vs = some_v ? (float)vt : 0.f;
+}
+
+// The largest of a wave's values, none of them below 0, for all lanes: by rotations of rows of 16 lanes, then swaps of rows.
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int u = __float_as_int(v);
+        int w = u;
+        if (i == 0) w = __builtin_amdgcn_update_dpp(u, u, 0x128, 0xF, 0xF, false);  // row_ror:8
+        if (i == 1) w = __builtin_amdgcn_update_dpp(u, u, 0x124, 0xF, 0xF, false);
+        if (i == 2) w = __builtin_amdgcn_update_dpp(u, u, 0x122, 0xF, 0xF, false);
+        if (i == 3) w = __builtin_amdgcn_update_dpp(u, u, 0x121, 0xF, 0xF, false);
+        v = fmaxf(v, __int_as_float(w));
+    }
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// The number of a moment y in fp32, where that is sure: y * 2^(3 - e) = A is off by no more than ``off`` A + ``more`` (and half a
+// step of fp32 at 16 where t is added), so that nothing changes if floor(A + t) has that much room on both sides. ``unsure`` is
+// set where it has not, also for what is not finite.
+__device__ __forceinline__ uint32_t e4m3(float y, uint32_t w, float off, float more, bool& unsure) {
+    int e = __builtin_amdgcn_frexp_expf(y) - 1;
+    if (e < -6 || y == 0.f) e = -6;
+    const float A = __builtin_ldexpf(y, 3 - e), F = A + (float)(w >> 8) * 0x1p-24f, fl = floorf(F), d = F - fl;
+    const float room = A * off + __builtin_ldexpf(more, 3 - e) + 0x1p-20f;
+    if (!(d > room && d < 1.f - room)) unsure = true;
+    const int code = ((e + 6) << 3) + (int)fl;
+    return (uint32_t)(code > 0x7E ? 0x7E : code);
+}
+
+// The same in fp32, where it comes to the same numbers; where that is not sure, false, and ``done``'s parameters alone are new (so
+// that a parameter does not depend on its neighbours). With u = 2^-24: a
+// first moment is the sum of two terms that are off by 3.5 u each, so 4.5 u of their size S; a root is off by 6 u. The scales
+// are taken in fp64 of the element with the largest fp32 value; one that fp32 does not tell from it may be larger by 9 u of its
+// S, at most 9 u (1 + 2 beta1 old largest / largest), and 12 u for the root. About one wave in fifty has to go to fp64.
+// Roots are taken of values scaled by a power of two near the old largest, so that squares stay in range.
+__device__ __forceinline__ bool step32(Eight& x, const Table& a, const Factors& f, int& done) {
+    constexpr float U = 0x1p-24f;
+    const float clip = (float)f.clip, b1 = (float)a.beta1, c1 = (float)a.rest1, b2 = (float)a.beta2, c2 = (float)a.rest2;
+    const bool had = x.vs > 0.f;
+    const float unit = had ? __builtin_ldexpf(1.f, -__builtin_amdgcn_frexp_expf(x.vs) - 9) : 1.f, vs = x.vs * unit;
+    done = 0;
+    if (!(unit >= 0x1p-100f)) return false;
+    const float step = (float)f.step, rt = (float)f.root / unit, decay = (float)f.decay, eps = (float)a.eps;
+    float mv[4], rv[4], size[4], mt = 0, vt = 0, mg = 0, mq = 0, vg = 0, vq = 0;
+    bool some_m = false, some_v = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float ge = x.g[e] * clip, gs = ge * unit, qm = number(x.m[e]), qv = number(x.v[e]), r = qv * vs;
+        const float t1 = b1 * (qm * x.ms), t2 = c1 * ge;
+        mv[e] = t1 + t2;
+        size[e] = fabsf(t1) + fabsf(t2);
+        rv[e] = __builtin_sqrtf(b2 * (r * r) + c2 * (gs * gs));
+        const bool there = x.g[e] != 0.f || qv != 0.f;
+        some_m = some_m || x.g[e] != 0.f || qm != 0.f;
+        some_v = some_v || there;
+        if ((rv[e] >= 0x1p-55f || !there) && rv[e] <= 0x1p60f && fabsf(mv[e]) <= 0x1p100f) {  // (squares in range)
+            x.p[e] = x.p[e] * decay - step * mv[e] / (rv[e] * rt + eps);
+            done |= 1 << e;
+        }
+        if (!(fabsf(mv[e]) <= mt)) mt = fabsf(mv[e]), mg = x.g[e], mq = qm;  // (a NaN stays, and is unsure below)
+        if (!(rv[e] <= vt)) vt = rv[e], vg = x.g[e], vq = qv;
+    }
+    const float mtop = wave_max(mt), vtop = wave_max(vt);
+    if (__ballot(done != 15) != 0) return false;
+    // where all are 0 so are their numbers; else the largest have to be well inside fp32's range
+    const bool any_m = __ballot(some_m) != 0, any_v = __ballot(some_v) != 0;
+    if (any_m && !(mtop >= 0x1p-90f && mtop <= 0x1p100f)) return false;
+    if (any_v && !(vtop >= 0x1p-30f && vtop <= 0x1p60f)) return false;
+    float im = 0, iv = 0, ms = 0, vs_new = 0;
+    if (any_m) {
+        const int at = __builtin_ctzll(__ballot(mt == mtop) | 1ull << 63);
+        const double g = (double)__shfl(mg, at, 64) * f.clip, q = (double)__shfl(mq, at, 64);
+        ms = (float)(fabs(a.beta1 * (q * (double)x.ms) + a.rest1 * g) / 448.0);
+        if (!(ms >= 0x1p-100f)) return false;
+        im = 1.f / ms;
+    }
+    if (any_v) {
+        const int at = __builtin_ctzll(__ballot(vt == vtop) | 1ull << 63);
+        const double g = (double)__shfl(vg, at, 64) * f.clip, r = (double)__shfl(vq, at, 64) * (double)x.vs;
+        vs_new = (float)(sqrt(a.beta2 * (r * r) + a.rest2 * (g * g)) / 448.0);
+        if (!(vs_new >= 0x1p-100f)) return false;
+        iv = 1.f / (vs_new * unit);
+    }
+    const float off_m = U * (13.f + 18.f * b1 * x.ms * im), off_v = 22.f * U;  // (with 4 u of the scale and the product)
+    uint32_t qm[4], qv[4];
+    bool unsure = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t w = x.at + (uint32_t)e * 0x85EBCA77u;
+        qm[e] = e4m3(fabsf(mv[e]) * im, w, off_m, 4.5f * U * size[e] * im, unsure) | (mv[e] < 0.f ? 0x80u : 0u);
+        qv[e] = e4m3(rv[e] * iv, w + 0x80000000u, off_v, 0.f, unsure);
+        if (qv[e] == 0 && (x.g[e] != 0.f || x.v[e] != 0)) qv[e] = 1;
+    }
+    if (__ballot(unsure) != 0) return false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x.m[e] = qm[e];
+        x.v[e] = qv[e];
+    }
+    x.ms = ms;
+    x.vs = vs_new;
+    return true;
+}
+
 template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_adamw8(Table a) {
     const int which = tensor_of(a);
     const ebr_optim_tensor t = a.t[which];
     const Factors f = a.factors[which];
-    const float step = (float)f.step, rt = (float)f.root, decay = (float)f.decay, eps = (float)a.eps;
     P* const p = reinterpret_cast<P*>(t.p);
     const G* const g = reinterpret_cast<const G*>(t.g);
     uint8_t *const m = reinterpret_cast<uint8_t*>(t.m), *const v = reinterpret_cast<uint8_t*>(t.v);
     const bool wp = wide4<P>(p), wg = wide4<G>(g), wm = wide4<uint8_t>(m), wv = wide4<uint8_t>(v);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
     const int64_t to = from + a.per < t.n ? from + a.per : t.n;
     for (int64_t b = from + wave * BLOCK; b < to; b += THREADS / 64 * BLOCK) {
         const int64_t i = b + lane * 4;
-        float pv[4], gv[4];
-        uint32_t mq[4], vq[4];
-        load4(p, i, to, wp, pv);
-        load4(g, i, to, wg, gv);
-        load4(m, i, to, wm, mq);
-        load4(v, i, to, wv, vq);
-        const double ms = (double)t.ms[b / BLOCK], vs = (double)t.vs[b / BLOCK];
-        double mv[4], rv[4];
-        double mt = 0, vt = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const double ge = (double)gv[e] * f.clip;
-            const double r = (double)__builtin_amdgcn_cvt_f32_fp8((int)vq[e], 0) * vs;
-            mv[e] = a.beta1 * ((double)__builtin_amdgcn_cvt_f32_fp8((int)mq[e], 0) * ms) + a.rest1 * ge;
-            rv[e] = sqrt(a.beta2 * (r * r) + a.rest2 * (ge * ge));
-            mt = fmax(mt, fabs(mv[e]));
-            vt = fmax(vt, rv[e]);
-            pv[e] = pv[e] * decay - step * (float)mv[e] / ((float)rv[e] * rt + eps);
-        }
-        store4(p, i, to, wp, pv);
-        mt = wave_max(mt) / 448.0;
-        vt = wave_max(vt) / 448.0;
-        const bool some_m = !(mt < 0x1p-126), some_v = !(vt < 0x1p-126);
-        const double im = some_m ? 1.0 / mt : 0.0, iv = some_v ? 1.0 / vt : 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t w = (uint32_t)(i + e) * 0x85EBCA77u + f.dither;
-            mq[e] = e4m3(fabs(mv[e]) * im, (double)(w >> 8) * 0x1p-24) | (mv[e] < 0 ? 0x80u : 0u);
-            vq[e] = e4m3(rv[e] * iv, (double)((w + 0x80000000u) >> 8) * 0x1p-24);
-            if (some_v && rv[e] > 0 && vq[e] == 0) vq[e] = 1;
-        }
-        store4(m, i, to, wm, mq);
-        store4(v, i, to, wv, vq);
+        Eight x;
+        load4(p, i, to, wp, x.p);
+        load4(g, i, to, wg, x.g);
+        load4(m, i, to, wm, x.m);
+        load4(v, i, to, wv, x.v);
+        x.ms = t.ms[b / BLOCK];
+        x.vs = t.vs[b / BLOCK];
+        x.at = (uint32_t)i * 0x85EBCA77u + f.dither;
+        int done;
+        if (!step32(x, a, f, done)) step64(x, a, f, done);
+        store4(p, i, to, wp, x.p);
+        store4(m, i, to, wm, x.m);
+        store4(v, i, to, wv, x.v);
         if (lane == 0) {
-            t.ms[b / BLOCK] = some_m ? (float)mt : 0.f;
-            t.vs[b / BLOCK] = some_v ? (float)vt : 0.f;
+            t.ms[b / BLOCK] = x.ms;
+            t.vs[b / BLOCK] = x.vs;
         }
     }
 }
 
-template <typename G> __device__ __forceinline__ double squares(const void* g_, int64_t from, int64_t to) {
+// The sum of squares of g[from, to), a thread's share of it. FAST: in fp32, each square and the sum with what their rounding
+// leaves (a conversion to fp64 and a product there take four times as long: 160 million elements 165 us whatever their type).
+template <typename G, bool FAST> __device__ __forceinline__ double squares(const void* g_, int64_t from, int64_t to) {
     const G* const g = reinterpret_cast<const G*>(g_);
     constexpr int N = 16 / (int)sizeof(G);
+    using Raw = typename Words<16>::type;
     double s = 0;
+    float top[AT_ONCE] = {}, rest[AT_ONCE] = {};
+    const auto add = [&](int k, G x) {
+        if constexpr (FAST) {
+            const float v = (float)x, q = v * v, t = top[k] + q, was = t - top[k];
+            rest[k] += ((top[k] - (t - was)) + (q - was)) + (sizeof(G) == 2 ? 0.f : __builtin_fmaf(v, v, -q));
+            top[k] = t;
+        } else {
+            s += (double)x * (double)x;
+        }
+    };
+    int64_t i = from + threadIdx.x * N;
     if (((uintptr_t)g & 15) == 0) {  // from is a multiple of a vector
-        for (int64_t i = from + threadIdx.x * N; i < to; i += THREADS * N) {
-            if (i + N <= to) {
-                const Pack<G, N> v = ldp<G, N>(g + i);
+        for (; i + ((AT_ONCE - 1) * THREADS + 1) * N <= to; i += AT_ONCE * THREADS * N) {
+            Raw raw[AT_ONCE];
 #pragma unroll
-                for (int e = 0; e < N; ++e) s += (double)v.e[e] * (double)v.e[e];
-            } else {
-                for (int64_t j = i; j < to; ++j) s += (double)g[j] * (double)g[j];
+            for (int k = 0; k < AT_ONCE; ++k) raw[k] = *reinterpret_cast<const Raw*>(g + i + k * THREADS * N);
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const Pack<G, N> v = unpacked<G, N>(raw[k]);
+#pragma unroll
+                for (int e = 0; e < N; ++e) add(k, v.e[e]);
             }
         }
+        for (; i + N <= to; i += THREADS * N) {
+            const Pack<G, N> v = ldp<G, N>(g + i);
+#pragma unroll
+            for (int e = 0; e < N; ++e) add(0, v.e[e]);
+        }
+        for (; i < to; ++i) add(0, g[i]);  // (the last thread's: less than a vector)
     } else {
-        for (int64_t i = from + threadIdx.x; i < to; i += THREADS) s += (double)g[i] * (double)g[i];
+        for (i = from + threadIdx.x; i < to; i += THREADS) add(0, g[i]);
+    }
+    if constexpr (FAST) {
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) s += (double)top[k] + (double)rest[k];
     }
     return s;
 }
@@ -252,14 +401,23 @@ __global__ __launch_bounds__(THREADS) void k_squares(Sums a) {
     const int which = tensor_of(a);
     const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
     const int64_t to = from + a.per < a.n[which] ? from + a.per : a.n[which];
-    double s;
-    switch (a.dtype[which]) {
-        case EBR_DTYPE_F32: s = squares<float>(a.g[which], from, to); break;
-        case EBR_DTYPE_BF16: s = squares<__bf16>(a.g[which], from, to); break;
-        case EBR_DTYPE_F16: s = squares<_Float16>(a.g[which], from, to); break;
-        default: s = squares<double>(a.g[which], from, to); break;
-    }
+    const void* g = a.g[which];
+    const int dtype = a.dtype[which];
+    double s = 0;
+    if (a.wide) s = 0;
+    else if (dtype == EBR_DTYPE_F32) s = squares<float, true>(g, from, to);
+    else if (dtype == EBR_DTYPE_BF16) s = squares<__bf16, true>(g, from, to);
+    else if (dtype == EBR_DTYPE_F16) s = squares<_Float16, true>(g, from, to);
     s = block_sum(s, lds);
+    // an fp64 gradient, and squares that fp32 does not hold: below 2^-60 in all some may be missing (of one above it, less than 2^-40 is)
+    if (!(s >= 0x1p-60 && s <= 0x1p120)) {
+        if (dtype == EBR_DTYPE_F32) s = squares<float, false>(g, from, to);
+        else if (dtype == EBR_DTYPE_BF16) s = squares<__bf16, false>(g, from, to);
+        else if (dtype == EBR_DTYPE_F16) s = squares<_Float16, false>(g, from, to);
+        else s = squares<double, false>(g, from, to);
+        __syncthreads();
+        s = block_sum(s, lds);
+    }
     if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
@@ -277,7 +435,9 @@ __global__ __launch_bounds__(1024) void k_norm(const double* part, int64_t parts
 
 static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
 
-// Elements of a workgroup, a multiple of LEAST: four workgroups for each of the 256 compute units where there is enough.
+// Elements of a workgroup of the norm, a multiple of LEAST: eight workgroups for each of the 256 compute units where there is
+// enough. A step's workgroups take one vector a thread, whatever the number of elements: of 160 million fp32 ones it takes 1,046
+// us so, 1,130 with 8 and 1,322 with 64 (every workgroup a stream of its own through four arrays).
 static int64_t per_group(int64_t total) {
     const int64_t want = (total / 2048 + LEAST - 1) / LEAST * LEAST;
     return std::min(std::max(want, LEAST), MOST);
@@ -348,8 +508,11 @@ int ebr_block_grad_norm(int64_t count, const ebr_optim_grad* grads, double* norm
     hipStream_t s = (hipStream_t)stream;
     const int64_t per = per_group(total_of(count, grads));
     int64_t parts = 0;
+    bool wide = false;
+    for (int64_t i = 0; i < count; ++i) wide = wide || grads[i].dtype == EBR_DTYPE_F64;
     for (int64_t i = 0; i < count;) {
         Sums a;
+        a.wide = wide;
         int blocks = 0;
         for (a.count = 0; i < count && a.count < GRADS; ++i) {
             if (grads[i].n == 0) continue;
@@ -391,8 +554,6 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
         if (t.n < 0 || t.n >= TOO_MANY || (total += t.n) >= TOO_MANY) return EBR_ERR_SHAPE;
         if (!t.step || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || (bits == 8 && (!t.ms || !t.vs))))) return EBR_ERR_NULL;
     }
-    const int64_t per = per_group(total);
-    if (total / per + count > MAX_BLOCKS) return EBR_ERR_SHAPE;
     try {
         if (twice(count, tensors)) return EBR_ERR_SHAPE;
     } catch (const std::bad_alloc&) {
@@ -402,6 +563,8 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
     if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     Factors* factors = reinterpret_cast<Factors*>(scratch);
+    int64_t per = STEP;
+    while (total / per + count > MAX_BLOCKS) per *= 2;
     for (int64_t i = 0; i < count; i += TENSORS, factors += TENSORS) {
         Table a = {};
         Prepare pre = {};

@@ -165,7 +165,7 @@ def _norms(grads: Sequence[Tensor]) -> Tuple[Tensor, Tensor]:
 
 
 def grad_norm(grads: Sequence[Tensor]) -> Tensor:
-    """The 2-norm of all the gradients together, summed in fp64 in a fixed order: one fp32 number on their device. The
+    """The 2-norm of all the gradients together, summed to 47 bits in a fixed order: one fp32 number on their device. The
     gradients may be of different dtypes."""
     return _norms(grads)[1]
 
