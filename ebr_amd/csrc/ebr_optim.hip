@@ -22,8 +22,8 @@ namespace ebr_opt {
 using namespace ebr_row;
 
 constexpr int THREADS = 256, BLOCK = 256, TENSORS = 48, GRADS = 144;
-constexpr int AT_ONCE = 4;                         // vectors under way in the norm
-constexpr int64_t STEP = 1024, LEAST = 4096, MOST = 65536;  // elements of a workgroup: of a step, and of the norm
+constexpr int AT_ONCE = 4;                                                 // vectors under way in the norm
+constexpr int64_t STEP = 1024, STEP8 = 4096, LEAST = 4096, MOST = 16384;   // elements of a workgroup: of a step, and of the norm
 
 // What a step multiplies by, for one tensor.
 struct alignas(16) Factors {
@@ -88,32 +88,30 @@ template <typename Tab> __device__ __forceinline__ int tensor_of(const Tab& a) {
     return lo;
 }
 
-// Four elements from i on, of which n - i exist; whole where they may be (``wide``: their address allows it).
-template <typename T, typename A> __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool wide, A (&v)[4]) {
-    if (wide && i + 4 <= n) {
-        const Pack<T, 4> x = ldp<T, 4>(p + i);
+// Four elements from i on: ``full`` (for a whole wave) in one access whatever their alignment (which the hardware takes: the lanes'
+// elements lie side by side, so most lines are whole all the same), else those of them that are below n.
+template <typename T, typename A> __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool full, A (&v)[4]) {
+    if (full) {
+        T x[4];
+        __builtin_memcpy(x, p + i, sizeof(x));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (A)x.e[e];
+        for (int e = 0; e < 4; ++e) v[e] = (A)x[e];
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = i + e < n ? (A)p[i + e] : (A)0;
     }
 }
-template <typename T, typename A> __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool wide, const A (&v)[4]) {
-    if (wide && i + 4 <= n) {
-        Pack<T, 4> x;
+template <typename T, typename A> __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool full, const A (&v)[4]) {
+    if (full) {
+        T x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.e[e] = (T)v[e];
-        stp<T, 4>(p + i, x);
+        for (int e = 0; e < 4; ++e) x[e] = (T)v[e];
+        __builtin_memcpy(p + i, x, sizeof(x));
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (i + e < n) p[i + e] = (T)v[e];
     }
-}
-// A pack of four is an aligned vector of at most 16 bytes; four fp64 go as two.
-template <typename T> __device__ __forceinline__ bool wide4(const void* p) {
-    return sizeof(T) <= 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
 
 template <typename A> __device__ __forceinline__ A root(A x);
@@ -130,15 +128,16 @@ template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_a
     P* const p = reinterpret_cast<P*>(t.p);
     const G* const g = reinterpret_cast<const G*>(t.g);
     A *const m = reinterpret_cast<A*>(t.m), *const v = reinterpret_cast<A*>(t.v);
-    const bool wp = wide4<P>(p), wg = wide4<G>(g), wm = wide4<A>(m), wv = wide4<A>(v);
     const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
     const int64_t to = from + a.per < t.n ? from + a.per : t.n;
-    for (int64_t i = from + threadIdx.x * 4; i < to; i += THREADS * 4) {
+    for (int64_t at = from; at < to; at += THREADS * 4) {
+        const int64_t i = at + threadIdx.x * 4;
+        const bool full = at + THREADS * 4 <= to;
         A pv[4], gv[4], mv[4], vv[4];
-        load4(p, i, to, wp, pv);
-        load4(g, i, to, wg, gv);
-        load4(m, i, to, wm, mv);
-        load4(v, i, to, wv, vv);
+        load4(p, i, to, full, pv);
+        load4(g, i, to, full, gv);
+        load4(m, i, to, full, mv);
+        load4(v, i, to, full, vv);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const A ge = gv[e] * clip;
@@ -146,9 +145,9 @@ template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_a
             vv[e] = b2 * vv[e] + c2 * (ge * ge);
             pv[e] = pv[e] * decay - step * mv[e] / (root(vv[e]) * rt + eps);
         }
-        store4(p, i, to, wp, pv);
-        store4(m, i, to, wm, mv);
-        store4(v, i, to, wv, vv);
+        store4(p, i, to, full, pv);
+        store4(m, i, to, full, mv);
+        store4(v, i, to, full, vv);
     }
 }
 
@@ -223,31 +222,33 @@ __device__ __forceinline__ float wave_max(float v) {
 // The number of a moment y in fp32, where that is sure: y * 2^(3 - e) = A is off by no more than ``off`` A + ``more`` (and half a
 // step of fp32 at 16 where t is added), so that nothing changes if floor(A + t) has that much room on both sides. ``unsure`` is
 // set where it has not, also for what is not finite.
-__device__ __forceinline__ uint32_t e4m3(float y, uint32_t w, float off, float more, bool& unsure) {
+template <bool MORE> __device__ __forceinline__ uint32_t e4m3(float y, uint32_t w, float off, float more, bool& unsure) {
     int e = __builtin_amdgcn_frexp_expf(y) - 1;
     if (e < -6 || y == 0.f) e = -6;
     const float A = __builtin_ldexpf(y, 3 - e), F = A + (float)(w >> 8) * 0x1p-24f, fl = floorf(F), d = F - fl;
-    const float room = A * off + __builtin_ldexpf(more, 3 - e) + 0x1p-20f;
+    float room = A * off + 0x1p-20f;
+    if constexpr (MORE) room += __builtin_ldexpf(more, 3 - e);
     if (!(d > room && d < 1.f - room)) unsure = true;
     const int code = ((e + 6) << 3) + (int)fl;
     return (uint32_t)(code > 0x7E ? 0x7E : code);
 }
 
 // The same in fp32, where it comes to the same numbers; where that is not sure, false, and ``done``'s parameters alone are new (so
-// that a parameter does not depend on its neighbours). With u = 2^-24: a
-// first moment is the sum of two terms that are off by 3.5 u each, so 4.5 u of their size S; a root is off by 6 u. The scales
-// are taken in fp64 of the element with the largest fp32 value; one that fp32 does not tell from it may be larger by 9 u of its
-// S, at most 9 u (1 + 2 beta1 old largest / largest), and 12 u for the root. About one wave in fifty has to go to fp64.
-// Roots are taken of values scaled by a power of two near the old largest, so that squares stay in range.
+// that a parameter does not depend on its neighbours). With u = 2^-24: a first moment is the sum of two terms that are off by 3.5
+// u each, so 4.5 u of their size S; the largest, and with it the scale, by no more than that of any S, at most 4.5 u (1 + 2 beta1
+// old largest / largest); a root and the largest root are off by 6 u each. The scale, its inverse and the product with it add 6 u.
+// About one wave in sixty has to go to fp64. Roots are taken of values scaled by a power of two near the old largest, so that
+// squares stay in range.
 __device__ __forceinline__ bool step32(Eight& x, const Table& a, const Factors& f, int& done) {
     constexpr float U = 0x1p-24f;
     const float clip = (float)f.clip, b1 = (float)a.beta1, c1 = (float)a.rest1, b2 = (float)a.beta2, c2 = (float)a.rest2;
     const bool had = x.vs > 0.f;
-    const float unit = had ? __builtin_ldexpf(1.f, -__builtin_amdgcn_frexp_expf(x.vs) - 9) : 1.f, vs = x.vs * unit;
+    const int shift = had ? __builtin_amdgcn_frexp_expf(x.vs) + 9 : 0;
+    const float unit = __builtin_ldexpf(1.f, -shift), back = __builtin_ldexpf(1.f, shift), vs = x.vs * unit;
     done = 0;
-    if (!(unit >= 0x1p-100f)) return false;
-    const float step = (float)f.step, rt = (float)f.root / unit, decay = (float)f.decay, eps = (float)a.eps;
-    float mv[4], rv[4], size[4], mt = 0, vt = 0, mg = 0, mq = 0, vg = 0, vq = 0;
+    if (shift > 100) return false;
+    const float step = (float)f.step, rt = (float)f.root * back, decay = (float)f.decay, eps = (float)a.eps;
+    float mv[4], rv[4], size[4], mt = 0, vt = 0;
     bool some_m = false, some_v = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -255,46 +256,36 @@ __device__ __forceinline__ bool step32(Eight& x, const Table& a, const Factors& 
         const float t1 = b1 * (qm * x.ms), t2 = c1 * ge;
         mv[e] = t1 + t2;
         size[e] = fabsf(t1) + fabsf(t2);
-        rv[e] = __builtin_sqrtf(b2 * (r * r) + c2 * (gs * gs));
+        rv[e] = __builtin_amdgcn_sqrtf(b2 * (r * r) + c2 * (gs * gs));
         const bool there = x.g[e] != 0.f || qv != 0.f;
         some_m = some_m || x.g[e] != 0.f || qm != 0.f;
         some_v = some_v || there;
-        if ((rv[e] >= 0x1p-55f || !there) && rv[e] <= 0x1p60f && fabsf(mv[e]) <= 0x1p100f) {  // (squares in range)
-            x.p[e] = x.p[e] * decay - step * mv[e] / (rv[e] * rt + eps);
+        const float den = rv[e] * rt + eps;  // (squares and reciprocals in range)
+        if ((rv[e] >= 0x1p-55f || !there) && rv[e] <= 0x1p60f && fabsf(mv[e]) <= 0x1p100f && den >= 0x1p-120f && den <= 0x1p120f) {
+            x.p[e] = x.p[e] * decay - step * mv[e] * __builtin_amdgcn_rcpf(den);
             done |= 1 << e;
         }
-        if (!(fabsf(mv[e]) <= mt)) mt = fabsf(mv[e]), mg = x.g[e], mq = qm;  // (a NaN stays, and is unsure below)
-        if (!(rv[e] <= vt)) vt = rv[e], vg = x.g[e], vq = qv;
+        mt = fmaxf(mt, fabsf(mv[e]));
+        vt = fmaxf(vt, rv[e]);
     }
-    const float mtop = wave_max(mt), vtop = wave_max(vt);
     if (__ballot(done != 15) != 0) return false;
     // where all are 0 so are their numbers; else the largest have to be well inside fp32's range
     const bool any_m = __ballot(some_m) != 0, any_v = __ballot(some_v) != 0;
-    if (any_m && !(mtop >= 0x1p-90f && mtop <= 0x1p100f)) return false;
-    if (any_v && !(vtop >= 0x1p-30f && vtop <= 0x1p60f)) return false;
-    float im = 0, iv = 0, ms = 0, vs_new = 0;
-    if (any_m) {
-        const int at = __builtin_ctzll(__ballot(mt == mtop) | 1ull << 63);
-        const double g = (double)__shfl(mg, at, 64) * f.clip, q = (double)__shfl(mq, at, 64);
-        ms = (float)(fabs(a.beta1 * (q * (double)x.ms) + a.rest1 * g) / 448.0);
-        if (!(ms >= 0x1p-100f)) return false;
-        im = 1.f / ms;
-    }
-    if (any_v) {
-        const int at = __builtin_ctzll(__ballot(vt == vtop) | 1ull << 63);
-        const double g = (double)__shfl(vg, at, 64) * f.clip, r = (double)__shfl(vq, at, 64) * (double)x.vs;
-        vs_new = (float)(sqrt(a.beta2 * (r * r) + a.rest2 * (g * g)) / 448.0);
-        if (!(vs_new >= 0x1p-100f)) return false;
-        iv = 1.f / (vs_new * unit);
-    }
-    const float off_m = U * (13.f + 18.f * b1 * x.ms * im), off_v = 22.f * U;  // (with 4 u of the scale and the product)
+    mt = wave_max(mt);
+    vt = wave_max(vt);
+    if (any_m && !(mt >= 0x1p-90f)) return false;
+    if (any_v && !(vt >= 0x1p-30f)) return false;
+    const float im = any_m ? 448.f * __builtin_amdgcn_rcpf(mt) : 0.f, iv = any_v ? 448.f * __builtin_amdgcn_rcpf(vt) : 0.f;
+    const float ms = mt * (1.f / 448.f), vs_new = vt * (1.f / 448.f) * back;
+    if (any_v && !(vs_new >= 0x1p-100f)) return false;
+    const float off_m = U * (10.5f + 9.f * b1 * x.ms * im), off_v = 18.f * U;
     uint32_t qm[4], qv[4];
     bool unsure = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const uint32_t w = x.at + (uint32_t)e * 0x85EBCA77u;
-        qm[e] = e4m3(fabsf(mv[e]) * im, w, off_m, 4.5f * U * size[e] * im, unsure) | (mv[e] < 0.f ? 0x80u : 0u);
-        qv[e] = e4m3(rv[e] * iv, w + 0x80000000u, off_v, 0.f, unsure);
+        qm[e] = e4m3<true>(fabsf(mv[e]) * im, w, off_m, 4.5f * U * size[e] * im, unsure) | (mv[e] < 0.f ? 0x80u : 0u);
+        qv[e] = e4m3<false>(rv[e] * iv, w + 0x80000000u, off_v, 0.f, unsure);
         if (qv[e] == 0 && (x.g[e] != 0.f || x.v[e] != 0)) qv[e] = 1;
     }
     if (__ballot(unsure) != 0) return false;
@@ -315,25 +306,25 @@ template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_a
     P* const p = reinterpret_cast<P*>(t.p);
     const G* const g = reinterpret_cast<const G*>(t.g);
     uint8_t *const m = reinterpret_cast<uint8_t*>(t.m), *const v = reinterpret_cast<uint8_t*>(t.v);
-    const bool wp = wide4<P>(p), wg = wide4<G>(g), wm = wide4<uint8_t>(m), wv = wide4<uint8_t>(v);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t from = (int64_t)(blockIdx.x - a.first[which]) * a.per;
     const int64_t to = from + a.per < t.n ? from + a.per : t.n;
     for (int64_t b = from + wave * BLOCK; b < to; b += THREADS / 64 * BLOCK) {
         const int64_t i = b + lane * 4;
+        const bool full = b + BLOCK <= to;
         Eight x;
-        load4(p, i, to, wp, x.p);
-        load4(g, i, to, wg, x.g);
-        load4(m, i, to, wm, x.m);
-        load4(v, i, to, wv, x.v);
+        load4(p, i, to, full, x.p);
+        load4(g, i, to, full, x.g);
+        load4(m, i, to, full, x.m);
+        load4(v, i, to, full, x.v);
         x.ms = t.ms[b / BLOCK];
         x.vs = t.vs[b / BLOCK];
         x.at = (uint32_t)i * 0x85EBCA77u + f.dither;
         int done;
         if (!step32(x, a, f, done)) step64(x, a, f, done);
-        store4(p, i, to, wp, x.p);
-        store4(m, i, to, wm, x.m);
-        store4(v, i, to, wv, x.v);
+        store4(p, i, to, full, x.p);
+        store4(m, i, to, full, x.m);
+        store4(v, i, to, full, x.v);
         if (lane == 0) {
             t.ms[b / BLOCK] = x.ms;
             t.vs[b / BLOCK] = x.vs;
@@ -436,11 +427,19 @@ __global__ __launch_bounds__(1024) void k_norm(const double* part, int64_t parts
 static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
 
 // Elements of a workgroup of the norm, a multiple of LEAST: eight workgroups for each of the 256 compute units where there is
-// enough. A step's workgroups take one vector a thread, whatever the number of elements: of 160 million fp32 ones it takes 1,046
-// us so, 1,130 with 8 and 1,322 with 64 (every workgroup a stream of its own through four arrays).
+// enough, and no more than MOST (160 million bf16 elements take 165 us with 8,192 and 16,384, 206 with 65,536).
 static int64_t per_group(int64_t total) {
     const int64_t want = (total / 2048 + LEAST - 1) / LEAST * LEAST;
     return std::min(std::max(want, LEAST), MOST);
+}
+
+// Elements of a workgroup of a step. With 32-bit moments one vector a thread (80 million fp32 elements: 412 us, 417 with 4; a
+// workgroup of 64 vectors a thread is a stream of its own through four arrays, and took a quarter longer). With 8-bit ones, where
+// a workgroup's start counts against few bytes, up to four where that leaves eight workgroups for every compute unit: 80 million
+// elements 343 us (one vector: 372), 900,001 in 60 tensors 7.9 us with one (four: 13.8).
+static int64_t per_step(int64_t total, int bits) {
+    const int64_t want = total / 2048 / STEP * STEP;
+    return bits == 8 ? std::min(std::max(want, STEP), STEP8) : STEP;
 }
 static int64_t groups(int64_t n, int64_t per) { return (n + per - 1) / per; }
 
@@ -563,7 +562,7 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
     if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     Factors* factors = reinterpret_cast<Factors*>(scratch);
-    int64_t per = STEP;
+    int64_t per = per_step(total, bits);
     while (total / per + count > MAX_BLOCKS) per *= 2;
     for (int64_t i = 0; i < count; i += TENSORS, factors += TENSORS) {
         Table a = {};
