@@ -11,6 +11,7 @@
 // order of operations. A wave takes the 256 elements of one scale, four a lane, in fp32, with a bound on how far each is off,
 // and again in fp64 where that reaches over a border.
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <vector>
 
@@ -36,7 +37,7 @@ struct Table {
     int first[TENSORS + 1];  // the first workgroup of each, and of what would be next
     int count, per;          // per: elements of a workgroup
     const Factors* factors;
-    double beta1, beta2, rest1, rest2, eps;
+    double beta1, beta2, rest1, rest2, root2, eps;  // 1 - beta, and the second one's root
 };
 
 struct Prepare {
@@ -165,24 +166,37 @@ __device__ __forceinline__ double wave_max(double v) {
     return v;
 }
 
-// What a wave knows of its 256 elements: four a lane.
+// What a wave knows of its 256 elements: four a lane, the moments' numbers a byte each.
 struct Eight {
     float p[4], g[4];
-    uint32_t m[4], v[4];
+    uint32_t m, v;
     float ms, vs;
     uint32_t at;  // the first one's number, times the dither's factor, plus the step's part
 };
 __device__ __forceinline__ double dither(uint32_t w) { return (double)(w >> 8) * 0x1p-24; }
-__device__ __forceinline__ float number(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
+template <int E> __device__ __forceinline__ float number(uint32_t codes) { return __builtin_amdgcn_cvt_f32_fp8((int)codes, E); }
+__device__ __forceinline__ void numbers(uint32_t codes, float (&x)[4]) {
+    x[0] = number<0>(codes), x[1] = number<1>(codes), x[2] = number<2>(codes), x[3] = number<3>(codes);
+}
+// The low bytes of four words, and their high bytes.
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&x)[4]) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(x[3], x[2], 0x0C0C0400), __builtin_amdgcn_perm(x[1], x[0], 0x0C0C0400), 0x05040100);
+}
+__device__ __forceinline__ uint32_t high_bytes(const uint32_t (&x)[4]) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(x[3], x[2], 0x0C0C0703), __builtin_amdgcn_perm(x[1], x[0], 0x0C0C0703), 0x05040100);
+}
 
 // The step in fp64; the parameters of ``done`` (a bit each) have theirs.
 __device__ __forceinline__ void step64(Eight& x, const Table& a, const Factors& f, int done) {
     const float step = (float)f.step, rt = (float)f.root, decay = (float)f.decay, eps = (float)a.eps;
     double mv[4], rv[4], mt = 0, vt = 0;
+    float qm[4], qv[4];
+    numbers(x.m, qm);
+    numbers(x.v, qv);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const double ge = (double)x.g[e] * f.clip, r = (double)number(x.v[e]) * (double)x.vs;
-        mv[e] = a.beta1 * ((double)number(x.m[e]) * (double)x.ms) + a.rest1 * ge;
+        const double ge = (double)x.g[e] * f.clip, r = (double)qv[e] * (double)x.vs;
+        mv[e] = a.beta1 * ((double)qm[e] * (double)x.ms) + a.rest1 * ge;
         rv[e] = sqrt(a.beta2 * (r * r) + a.rest2 * (ge * ge));
         mt = fmax(mt, fabs(mv[e]));
         vt = fmax(vt, rv[e]);
@@ -192,111 +206,154 @@ __device__ __forceinline__ void step64(Eight& x, const Table& a, const Factors& 
     vt = wave_max(vt) / 448.0;
     const bool some_m = !(mt < 0x1p-126), some_v = !(vt < 0x1p-126);
     const double im = some_m ? 1.0 / mt : 0.0, iv = some_v ? 1.0 / vt : 0.0;
+    uint32_t cm[4], cv[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const uint32_t w = x.at + (uint32_t)e * 0x85EBCA77u;
-        x.m[e] = e4m3(fabs(mv[e]) * im, dither(w)) | (mv[e] < 0 ? 0x80u : 0u);
-        x.v[e] = e4m3(rv[e] * iv, dither(w + 0x80000000u));
-        if (some_v && rv[e] > 0 && x.v[e] == 0) x.v[e] = 1;
+        cm[e] = e4m3(fabs(mv[e]) * im, dither(w)) | (__builtin_signbit(mv[e]) ? 0x80u : 0u);
+        cv[e] = e4m3(rv[e] * iv, dither(w + 0x80000000u));
+        if (some_v && rv[e] > 0 && cv[e] == 0) cv[e] = 1;
     }
+    x.m = low_bytes(cm);
+    x.v = low_bytes(cv);
     x.ms = some_m ? (float)mt : 0.f;
     x.vs = some_v ? (float)vt : 0.f;
 }
 
-// The largest of a wave's values, none of them below 0, for all lanes: by rotations of rows of 16 lanes, then swaps of rows.
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int u = __float_as_int(v);
-        int w = u;
-        if (i == 0) w = __builtin_amdgcn_update_dpp(u, u, 0x128, 0xF, 0xF, false);  // row_ror:8
-        if (i == 1) w = __builtin_amdgcn_update_dpp(u, u, 0x124, 0xF, 0xF, false);
-        if (i == 2) w = __builtin_amdgcn_update_dpp(u, u, 0x122, 0xF, 0xF, false);
-        if (i == 3) w = __builtin_amdgcn_update_dpp(u, u, 0x121, 0xF, 0xF, false);
-        v = fmaxf(v, __int_as_float(w));
-    }
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
+__device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+
+// The largest of a wave's numbers, for all lanes: by rotations of rows of 16 lanes, then swaps of rows.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = umax(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x128, 0xF, 0xF, false));  // row_ror:8
+    v = umax(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x124, 0xF, 0xF, false));
+    v = umax(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x122, 0xF, 0xF, false));
+    v = umax(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x121, 0xF, 0xF, false));
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = umax(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane(umax(r[0], r[1]));
 }
 
-// The number of a moment y in fp32, where that is sure: y * 2^(3 - e) = A is off by no more than ``off`` A + ``more`` (and half a
-// step of fp32 at 16 where t is added), so that nothing changes if floor(A + t) has that much room on both sides. ``unsure`` is
-// set where it has not, also for what is not finite.
-template <bool MORE> __device__ __forceinline__ uint32_t e4m3(float y, uint32_t w, float off, float more, bool& unsure) {
-    int e = __builtin_amdgcn_frexp_expf(y) - 1;
-    if (e < -6 || y == 0.f) e = -6;
-    const float A = __builtin_ldexpf(y, 3 - e), F = A + (float)(w >> 8) * 0x1p-24f, fl = floorf(F), d = F - fl;
-    float room = A * off + 0x1p-20f;
-    if constexpr (MORE) room += __builtin_ldexpf(more, 3 - e);
-    if (!(d > room && d < 1.f - room)) unsure = true;
-    const int code = ((e + 6) << 3) + (int)fl;
-    return (uint32_t)(code > 0x7E ? 0x7E : code);
-}
+// The e4m3 number of y >= 0, in fp32 and integers. fp32's bits of y, read as a number of steps of 2^-20, are 8 (e + 127) + 8 f for
+// y = 2^e (1 + f): an e4m3 number's code, and its 20 bits of fraction. Below 2^-6, where e4m3's steps stay 2^-9, they are those of
+// y + 2^-6 less 8; the larger of the two is the right one on each side. The sum with t, of as many bits, is exact; what its
+// fraction lacks to 0 or 1 is what y may be off by. ``line``: the bits, ``sum``: with t, and 64 for bytes to begin at 1024.
+struct Code {
+    uint32_t line, sum;
+    __device__ __forceinline__ Code(float y, uint32_t t) : line(umax(bits(y), bits(y + 0x1p-6f) - (8u << 20))), sum(line + t + (64u << 20)) {}
+    // in the low byte
+    __device__ __forceinline__ uint32_t value(uint32_t least) const { return umax(umin(sum >> 20, 1024 + 0x7E), 1024 + least); }
+    // below 2^19 where y is off by less than ``room``
+    __device__ __forceinline__ uint32_t doubt(uint32_t room) const {
+        const uint32_t d = sum & 0xFFFFF, mid = 1u << 19;
+        return (d > mid ? d - mid : mid - d) + room;
+    }
+};
 
 // The same in fp32, where it comes to the same numbers; where that is not sure, false, and ``done``'s parameters alone are new (so
-// that a parameter does not depend on its neighbours). With u = 2^-24: a first moment is the sum of two terms that are off by 3.5
-// u each, so 4.5 u of their size S; the largest, and with it the scale, by no more than that of any S, at most 4.5 u (1 + 2 beta1
-// old largest / largest); a root and the largest root are off by 6 u each. The scale, its inverse and the product with it add 6 u.
-// About one wave in sixty has to go to fp64. Roots are taken of values scaled by a power of two near the old largest, so that
-// squares stay in range.
+// that a parameter does not depend on its neighbours).
+//
+// With u = 2^-24, the uniform factors being rounded once: a first moment's terms are off by 2 u each, so it by 3 u of their size S;
+// the largest, and with it the scale, by no more than that of any S, at most 3 u (1 + 2 beta1 old largest / largest). A number of
+// e4m3 is exact when squared; a root, and the largest root, are off by 4.5 u (a sum by 5 u, then the root's own 2 u). A scale's
+// inverse and the products with it add 4 u. In steps of 2^-20 of the code, whose binade is 8 to 16 steps of e4m3, u of a number is
+// 1 at most: 13 for a root, 7 + 6 beta1 old / new scale + 3 u S 2^(3 - e) / scale for a first moment, and 2 for what y + 2^-6 and t
+// were cut by. About one wave in sixty has to go to fp64. Roots are taken of values scaled by a power of two near the old largest,
+// so that squares stay in range. The largest numbers are compared as bits, where infinities and NaN are above all others.
 __device__ __forceinline__ bool step32(Eight& x, const Table& a, const Factors& f, int& done) {
-    constexpr float U = 0x1p-24f;
-    const float clip = (float)f.clip, b1 = (float)a.beta1, c1 = (float)a.rest1, b2 = (float)a.beta2, c2 = (float)a.rest2;
-    const bool had = x.vs > 0.f;
-    const int shift = had ? __builtin_amdgcn_frexp_expf(x.vs) + 9 : 0;
-    const float unit = __builtin_ldexpf(1.f, -shift), back = __builtin_ldexpf(1.f, shift), vs = x.vs * unit;
     done = 0;
-    if (shift > 100) return false;
+    const int shift = x.vs > 0.f ? __builtin_amdgcn_frexp_expf(x.vs) + 9 : 0;
+    const float unit = __builtin_ldexpf(1.f, -shift), back = __builtin_ldexpf(1.f, shift), vs = x.vs * unit;
+    const float b1 = (float)(a.beta1 * x.ms), c1 = (float)(a.rest1 * f.clip), b2 = (float)(a.beta2 * ((double)vs * vs)),
+                c2 = (float)(a.root2 * f.clip) * unit;
     const float step = (float)f.step, rt = (float)f.root * back, decay = (float)f.decay, eps = (float)a.eps;
-    float mv[4], rv[4], size[4], mt = 0, vt = 0;
-    bool some_m = false, some_v = false;
+    // what makes reciprocals and small squares safe: with it, a root of at least LEAST has both, and one of 0 has no part in it
+    constexpr float LEAST_ROOT = 0x1p-55f, MOST_ROOT = 0x1p60f, MOST_MOMENT = 0x1p100f;
+    if (!(rt >= 0x1p-60f && rt <= 0x1p55f && eps >= 0x1p-120f && eps <= 0x1p60f && (b2 == 0.f ? a.beta2 == 0.0 || x.vs == 0.f : b2 >= 0x1p-60f)))
+        return false;
+    float qm[4], qv[4], mv[4], rv[4], size[4], p[4];
+    numbers(x.m, qm);
+    numbers(x.v, qv);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float ge = x.g[e] * clip, gs = ge * unit, qm = number(x.m[e]), qv = number(x.v[e]), r = qv * vs;
-        const float t1 = b1 * (qm * x.ms), t2 = c1 * ge;
+        const float t1 = b1 * qm[e], t2 = c1 * x.g[e], gs = c2 * x.g[e];
         mv[e] = t1 + t2;
         size[e] = fabsf(t1) + fabsf(t2);
-        rv[e] = __builtin_amdgcn_sqrtf(b2 * (r * r) + c2 * (gs * gs));
-        const bool there = x.g[e] != 0.f || qv != 0.f;
-        some_m = some_m || x.g[e] != 0.f || qm != 0.f;
-        some_v = some_v || there;
-        const float den = rv[e] * rt + eps;  // (squares and reciprocals in range)
-        if ((rv[e] >= 0x1p-55f || !there) && rv[e] <= 0x1p60f && fabsf(mv[e]) <= 0x1p100f && den >= 0x1p-120f && den <= 0x1p120f) {
-            x.p[e] = x.p[e] * decay - step * mv[e] * __builtin_amdgcn_rcpf(den);
-            done |= 1 << e;
+        rv[e] = __builtin_amdgcn_sqrtf(__builtin_fmaf(gs, gs, qv[e] * qv[e] * b2));
+        p[e] = x.p[e] * decay - step * mv[e] * __builtin_amdgcn_rcpf(rv[e] * rt + eps);
+    }
+    const uint32_t mt = wave_max(umax(umax(bits(fabsf(mv[0])), bits(fabsf(mv[1]))), umax(bits(fabsf(mv[2])), bits(fabsf(mv[3])))));
+    const uint32_t vt = wave_max(umax(umax(bits(rv[0]), bits(rv[1])), umax(bits(rv[2]), bits(rv[3]))));
+    const bool small = __ballot(fminf(fminf(rv[0], rv[1]), fminf(rv[2], rv[3])) < LEAST_ROOT) != 0;
+    bool sure = mt <= bits(MOST_MOMENT) && vt <= bits(MOST_ROOT);
+    bool any_m = true, any_v = true;
+    if (!sure || small || mt < bits(0x1p-90f) || vt < bits(0x1p-30f)) {
+        // a root below LEAST_ROOT is one of zeros alone, or not done here; the largest are of zeros alone, or well inside fp32's range
+        bool some_m = false, some_v = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool there = x.g[e] != 0.f || (qv[e] != 0.f && b2 != 0.f);
+            some_m = some_m || x.g[e] != 0.f || qm[e] != 0.f;
+            some_v = some_v || there;
+            if ((rv[e] >= LEAST_ROOT || !there) && rv[e] <= MOST_ROOT && fabsf(mv[e]) <= MOST_MOMENT) {
+                x.p[e] = p[e];
+                done |= 1 << e;
+            }
         }
-        mt = fmaxf(mt, fabsf(mv[e]));
-        vt = fmaxf(vt, rv[e]);
+        any_m = __ballot(some_m) != 0, any_v = __ballot(some_v) != 0;
+        if (__ballot(done != 15) != 0 || (any_m && mt < bits(0x1p-90f)) || (any_v && vt < bits(0x1p-30f))) return false;
+    } else {
+        done = 15;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.p[e] = p[e];
     }
-    if (__ballot(done != 15) != 0) return false;
-    // where all are 0 so are their numbers; else the largest have to be well inside fp32's range
-    const bool any_m = __ballot(some_m) != 0, any_v = __ballot(some_v) != 0;
-    mt = wave_max(mt);
-    vt = wave_max(vt);
-    if (any_m && !(mt >= 0x1p-90f)) return false;
-    if (any_v && !(vt >= 0x1p-30f)) return false;
-    const float im = any_m ? 448.f * __builtin_amdgcn_rcpf(mt) : 0.f, iv = any_v ? 448.f * __builtin_amdgcn_rcpf(vt) : 0.f;
-    const float ms = mt * (1.f / 448.f), vs_new = vt * (1.f / 448.f) * back;
-    if (any_v && !(vs_new >= 0x1p-100f)) return false;
-    const float off_m = U * (10.5f + 9.f * b1 * x.ms * im), off_v = 18.f * U;
-    uint32_t qm[4], qv[4];
-    bool unsure = false;
+    const float top_m = __uint_as_float(mt), top_v = __uint_as_float(vt);
+    const float im = any_m ? 448.f * __builtin_amdgcn_rcpf(top_m) : 0.f, iv = any_v ? 448.f * __builtin_amdgcn_rcpf(top_v) : 0.f;
+    const float ms = top_m * (1.f / 448.f), vs_new = top_v * (1.f / 448.f) * back;
+    if ((any_v && !(vs_new >= 0x1p-100f)) || !(b1 * im <= 0x1p10f)) return false;  // (a room fits an integer)
+    constexpr uint32_t room_v = 15;
+    const float room_m = 10.f + 6.1f * b1 * im, more = 1.55f * im;  // 3.1 u 2^(3 + 20) / scale, to be times S 2^-e
+    uint32_t cm[4], cv[4], doubt = 0, signs[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t w = x.at + (uint32_t)e * 0x85EBCA77u;
-        qm[e] = e4m3<true>(fabsf(mv[e]) * im, w, off_m, 4.5f * U * size[e] * im, unsure) | (mv[e] < 0.f ? 0x80u : 0u);
-        qv[e] = e4m3<false>(rv[e] * iv, w + 0x80000000u, off_v, 0.f, unsure);
-        if (qv[e] == 0 && (x.g[e] != 0.f || x.v[e] != 0)) qv[e] = 1;
+        const uint32_t t = (x.at + (uint32_t)e * 0x85EBCA77u) >> 12;
+        const Code m(fabsf(mv[e]) * im, t), v(rv[e] * iv, t ^ 0x80000u);
+        const float scale = __uint_as_float(0x7F000000u - (m.line & 0x7F800000u));  // 2^-e, or twice 2^6
+        doubt = umax(doubt, umax(m.doubt((uint32_t)__builtin_fmaf(size[e] * more, scale, room_m)), v.doubt(room_v)));
+        cm[e] = m.value(0);
+        cv[e] = v.value(umin(bits(rv[e]), 1));
+        signs[e] = bits(mv[e]);
     }
-    if (__ballot(unsure) != 0) return false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x.m[e] = qm[e];
-        x.v[e] = qv[e];
-    }
+    if (__ballot(doubt >= 1u << 19) != 0) return false;
+    x.m = low_bytes(cm) | (high_bytes(signs) & 0x80808080u);
+    x.v = low_bytes(cv);
     x.ms = ms;
     x.vs = vs_new;
     return true;
+}
+
+// A word of four bytes, from i on.
+__device__ __forceinline__ uint32_t load_word(const uint8_t* p, int64_t i, int64_t n, bool full) {
+    uint32_t x = 0;
+    if (full) {
+        __builtin_memcpy(&x, p + i, 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) x |= (uint32_t)p[i + e] << 8 * e;
+    }
+    return x;
+}
+__device__ __forceinline__ void store_word(uint8_t* p, int64_t i, int64_t n, bool full, uint32_t x) {
+    if (full) {
+        __builtin_memcpy(p + i, &x, 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) p[i + e] = (uint8_t)(x >> 8 * e);
+    }
 }
 
 template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_adamw8(Table a) {
@@ -315,16 +372,16 @@ template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_a
         Eight x;
         load4(p, i, to, full, x.p);
         load4(g, i, to, full, x.g);
-        load4(m, i, to, full, x.m);
-        load4(v, i, to, full, x.v);
+        x.m = load_word(m, i, to, full);
+        x.v = load_word(v, i, to, full);
         x.ms = t.ms[b / BLOCK];
         x.vs = t.vs[b / BLOCK];
         x.at = (uint32_t)i * 0x85EBCA77u + f.dither;
         int done;
         if (!step32(x, a, f, done)) step64(x, a, f, done);
         store4(p, i, to, full, x.p);
-        store4(m, i, to, full, x.m);
-        store4(v, i, to, full, x.v);
+        store_word(m, i, to, full, x.m);
+        store_word(v, i, to, full, x.v);
         if (lane == 0) {
             t.ms[b / BLOCK] = x.ms;
             t.vs[b / BLOCK] = x.vs;
@@ -571,7 +628,7 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
         a.factors = pre.factors = factors;
         a.per = (int)per;
         a.beta1 = pre.beta1 = beta1, a.beta2 = pre.beta2 = beta2;
-        a.rest1 = 1.0 - beta1, a.rest2 = 1.0 - beta2, a.eps = eps;
+        a.rest1 = 1.0 - beta1, a.rest2 = 1.0 - beta2, a.root2 = std::sqrt(a.rest2), a.eps = eps;
         pre.lr = lr, pre.lr_dev = lr_dev, pre.decay = decay, pre.norm = norm, pre.max_norm = max_norm;
         int blocks = 0;
         for (int k = 0; k < a.count; ++k) {
