@@ -54,7 +54,6 @@ struct Sums {
     int64_t n[GRADS];
     int first[GRADS + 1], dtype[GRADS];
     int count, per;
-    int wide;  // an fp64 gradient is among them: all sums in fp64
     double* part;
 };
 
@@ -389,50 +388,48 @@ template <typename P, typename G> __global__ __launch_bounds__(THREADS) void k_a
     }
 }
 
-// The sum of squares of g[from, to), a thread's share of it. FAST: in fp32, each square and the sum with what their rounding
-// leaves (a conversion to fp64 and a product there take four times as long: 160 million elements 165 us whatever their type).
+// The size of x in fp64, from its bits: fp32's fraction and exponent, moved (the conversion takes four times a sum's time). What is
+// 0 or below the normal numbers comes out between 2^-127 and 2^-126, what is not finite above all that is.
+__device__ __forceinline__ double moved(uint32_t hi, uint32_t lo) { return __hiloint2double((int)(hi + (896u << 20)), (int)lo); }
+__device__ __forceinline__ double size_of(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+    return moved(b >> 3, b << 29);
+}
+__device__ __forceinline__ double size_of(_Float16 x) { return size_of((float)x); }
+__device__ __forceinline__ double size_of(__bf16 x) {
+    uint16_t b;
+    __builtin_memcpy(&b, &x, 2);
+    return moved((uint32_t)(b & 0x7FFF) << 13, 0);
+}
+
+// The sum of squares of g[from, to), a thread's share of it, in fp64. FAST: of sizes as above.
 template <typename G, bool FAST> __device__ __forceinline__ double squares(const void* g_, int64_t from, int64_t to) {
     const G* const g = reinterpret_cast<const G*>(g_);
     constexpr int N = 16 / (int)sizeof(G);
-    using Raw = typename Words<16>::type;
-    double s = 0;
-    float top[AT_ONCE] = {}, rest[AT_ONCE] = {};
+    double sum[AT_ONCE] = {};
     const auto add = [&](int k, G x) {
-        if constexpr (FAST) {
-            const float v = (float)x, q = v * v, t = top[k] + q, was = t - top[k];
-            rest[k] += ((top[k] - (t - was)) + (q - was)) + (sizeof(G) == 2 ? 0.f : __builtin_fmaf(v, v, -q));
-            top[k] = t;
-        } else {
-            s += (double)x * (double)x;
-        }
+        double v;
+        if constexpr (FAST) v = size_of(x);
+        else v = (double)x;
+        sum[k] = __builtin_fma(v, v, sum[k]);
     };
     int64_t i = from + threadIdx.x * N;
-    if (((uintptr_t)g & 15) == 0) {  // from is a multiple of a vector
-        for (; i + ((AT_ONCE - 1) * THREADS + 1) * N <= to; i += AT_ONCE * THREADS * N) {
-            Raw raw[AT_ONCE];
+    G x[AT_ONCE][N];
+    for (; i + ((AT_ONCE - 1) * THREADS + 1) * N <= to; i += AT_ONCE * THREADS * N) {
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) raw[k] = *reinterpret_cast<const Raw*>(g + i + k * THREADS * N);
+        for (int k = 0; k < AT_ONCE; ++k) __builtin_memcpy(x[k], g + i + k * THREADS * N, 16);  // whatever their alignment
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) {
-                const Pack<G, N> v = unpacked<G, N>(raw[k]);
+        for (int k = 0; k < AT_ONCE; ++k)
 #pragma unroll
-                for (int e = 0; e < N; ++e) add(k, v.e[e]);
-            }
-        }
-        for (; i + N <= to; i += THREADS * N) {
-            const Pack<G, N> v = ldp<G, N>(g + i);
-#pragma unroll
-            for (int e = 0; e < N; ++e) add(0, v.e[e]);
-        }
-        for (; i < to; ++i) add(0, g[i]);  // (the last thread's: less than a vector)
-    } else {
-        for (i = from + threadIdx.x; i < to; i += THREADS) add(0, g[i]);
+            for (int e = 0; e < N; ++e) add(k, x[k][e]);
     }
-    if constexpr (FAST) {
+    for (; i + N <= to; i += THREADS * N) {
+        __builtin_memcpy(x[0], g + i, 16);
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) s += (double)top[k] + (double)rest[k];
+        for (int e = 0; e < N; ++e) add(0, x[0][e]);
     }
-    return s;
+    for (; i < to; ++i) add(0, g[i]);  // (the last thread's: less than a vector)
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 __device__ __forceinline__ double block_sum(double s, double* lds) {
@@ -452,13 +449,12 @@ __global__ __launch_bounds__(THREADS) void k_squares(Sums a) {
     const void* g = a.g[which];
     const int dtype = a.dtype[which];
     double s = 0;
-    if (a.wide) s = 0;
-    else if (dtype == EBR_DTYPE_F32) s = squares<float, true>(g, from, to);
+    if (dtype == EBR_DTYPE_F32) s = squares<float, true>(g, from, to);
     else if (dtype == EBR_DTYPE_BF16) s = squares<__bf16, true>(g, from, to);
     else if (dtype == EBR_DTYPE_F16) s = squares<_Float16, true>(g, from, to);
     s = block_sum(s, lds);
-    // an fp64 gradient, and squares that fp32 does not hold: below 2^-60 in all some may be missing (of one above it, less than 2^-40 is)
-    if (!(s >= 0x1p-60 && s <= 0x1p120)) {
+    // an fp64 gradient, one that is not finite, and sums that a size's 2^-126 counts in
+    if (!(s >= 0x1p-120 && s <= 0x1p255)) {
         if (dtype == EBR_DTYPE_F32) s = squares<float, false>(g, from, to);
         else if (dtype == EBR_DTYPE_BF16) s = squares<__bf16, false>(g, from, to);
         else if (dtype == EBR_DTYPE_F16) s = squares<_Float16, false>(g, from, to);
@@ -484,7 +480,7 @@ __global__ __launch_bounds__(1024) void k_norm(const double* part, int64_t parts
 static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
 
 // Elements of a workgroup of the norm, a multiple of LEAST: eight workgroups for each of the 256 compute units where there is
-// enough, and no more than MOST (160 million bf16 elements take 165 us with 8,192 and 16,384, 206 with 65,536).
+// enough, and no more than MOST (with 65,536 the last workgroups leave the card half empty: a quarter longer at 160 million).
 static int64_t per_group(int64_t total) {
     const int64_t want = (total / 2048 + LEAST - 1) / LEAST * LEAST;
     return std::min(std::max(want, LEAST), MOST);
@@ -564,11 +560,8 @@ int ebr_block_grad_norm(int64_t count, const ebr_optim_grad* grads, double* norm
     hipStream_t s = (hipStream_t)stream;
     const int64_t per = per_group(total_of(count, grads));
     int64_t parts = 0;
-    bool wide = false;
-    for (int64_t i = 0; i < count; ++i) wide = wide || grads[i].dtype == EBR_DTYPE_F64;
     for (int64_t i = 0; i < count;) {
         Sums a;
-        a.wide = wide;
         int blocks = 0;
         for (a.count = 0; i < count && a.count < GRADS; ++i) {
             if (grads[i].n == 0) continue;

@@ -40,7 +40,7 @@ typedef struct {
     int64_t n;
 } ebr_optim_tensor;
 
-/* norm[0] = sqrt(sum of g^2 over all gradients), summed to 47 bits (in fp64 where one of them is) in a fixed order; single[0], where not NULL, the same in
+/* norm[0] = sqrt(sum of g^2 over all gradients), summed in fp64 in a fixed order; single[0], where not NULL, the same in
  * fp32. At least one gradient; n may be 0. scratch: ebr_block_grad_norm_scratch bytes, 16-byte aligned. */
 int ebr_block_grad_norm(int64_t count, const ebr_optim_grad* grads, double* norm, float* single, void* scratch,
                         void* stream);
