@@ -11,10 +11,11 @@
 // one value far from zero keeps what there is of its differences. Both come out of two sums over the row, the second of which
 // gives the squares as well. Backwards read m, c and r back.
 //
-// Bound by memory. A row stays in the registers of TPR threads between its sums and its outputs, so every tensor is read once;
-// rows too wide for a workgroup, and fp64, go through k_rows and k_apply, which read them twice. The parameters' sums stay in
-// the registers of the threads that hold the columns, over all rows of a workgroup, then go through one partial a workgroup to
-// k_params: always in the same order.
+// Bound by memory: 62,208 rows of 256 in bf16 take 13.3 us forward, 17.8 backward and 31 in the second (4.8, 5.4 and 5.1 TB/s),
+// 16,384 of 2048 23.5 and 42 (5.7 and 4.8 TB/s; a copy of this size goes at 5 to 7). A row stays in the registers of TPR threads
+// between its sums and its outputs, so every tensor is read once; rows too wide for a workgroup, and fp64, go through k_rows and
+// k_apply, which read them twice. The parameters' sums stay in the registers of the threads that hold the columns, over all rows
+// of a workgroup, then go through one partial a workgroup to k_params: always in the same order.
 #include <type_traits>
 
 #include "rowwise.hpp"
@@ -54,22 +55,75 @@ template <typename A> __device__ __forceinline__ A variance(A square, A c) {
     return square == (A)INFINITY ? square : v < (A)0 ? (A)0 : v;
 }
 
-// Consecutive parameters of any type.
-template <typename A, int VEC> __device__ __forceinline__ void params(const void* p, int type, int c, A none, A (&v)[VEC]) {
+// A row's vectors: where its width is no multiple of VEC, the last one ends with the row and shares its first ``skip`` elements
+// with the one before, which alone counts them in sums (both write them, the same). VEC and more: a vector past the row.
+template <int VEC> __device__ __forceinline__ int place(int col, int C) { return col < C - VEC ? col : C - VEC; }
+template <int VEC, typename F> __device__ __forceinline__ void each(int skip, F f) {
+    if (skip <= 0) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        if (!p) v[e] = none;
-        else if (type == EBR_DTYPE_F32) v[e] = (A) reinterpret_cast<const float*>(p)[c + e];
-        else if (type == EBR_DTYPE_BF16) v[e] = (A) reinterpret_cast<const __bf16*>(p)[c + e];
-        else if (type == EBR_DTYPE_F16) v[e] = (A) reinterpret_cast<const _Float16*>(p)[c + e];
-        else v[e] = (A) reinterpret_cast<const double*>(p)[c + e];
+        for (int e = 0; e < VEC; ++e) f(e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e >= skip) f(e);
     }
 }
+// In one access, whatever the alignment.
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> fetch(const T* p) {
+    Pack<T, VEC> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+template <typename T, int VEC> __device__ __forceinline__ void put(T* p, const Pack<T, VEC>& v) { __builtin_memcpy(p, &v, sizeof(v)); }
+
+// Consecutive parameters of any type.
+template <typename A, int VEC> __device__ __forceinline__ void params(const void* p, int type, int c, A none, A (&v)[VEC]) {
+    const auto take = [&](auto zero) {
+        using W = decltype(zero);
+        W x[VEC];
+        __builtin_memcpy(x, reinterpret_cast<const W*>(p) + c, sizeof(x));
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = (A)x[e];
+    };
+    if (!p) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = none;
+    } else if (type == EBR_DTYPE_F32) take(float());
+    else if (type == EBR_DTYPE_BF16) take(__bf16());
+    else if (type == EBR_DTYPE_F16) take(_Float16());
+    else take(double());
+}
+
+// The sum over aligned parts of W lanes, the same in all of them: in fp32 by rotations of rows of 16 lanes and swaps of rows.
+template <int W> __device__ __forceinline__ float total(float v) {
+    if constexpr (W < 16) {
+        return lanes_sum<W>(v);
+    } else {
+        const auto turned = [](float x, auto how) {
+            const int u = __float_as_int(x);
+            return __int_as_float(__builtin_amdgcn_update_dpp(u, u, decltype(how)::value, 0xF, 0xF, false));
+        };
+        v += turned(v, std::integral_constant<int, 0x128>());
+        v += turned(v, std::integral_constant<int, 0x124>());
+        v += turned(v, std::integral_constant<int, 0x122>());
+        v += turned(v, std::integral_constant<int, 0x121>());
+        if constexpr (W >= 32) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        if constexpr (W == 64) {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        return v;
+    }
+}
+template <int W> __device__ __forceinline__ double total(double v) { return lanes_sum<W>(v); }
 
 // Sums over the TPR threads of a row, for all of them.
 template <int TPR, int K, typename A> __device__ __forceinline__ void row_sums(A (&v)[K], A* lds) {
 #pragma unroll
-    for (int i = 0; i < K; ++i) v[i] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[i]);
+    for (int i = 0; i < K; ++i) v[i] = total<(TPR < 64 ? TPR : 64)>(v[i]);
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -103,7 +157,8 @@ template <typename A> struct Row {
 };
 
 template <typename A> __device__ __forceinline__ void load_stats(const Args& a, int64_t row, Row<A>& q) {
-    const A* s = reinterpret_cast<const A*>(a.stats) + row * 4;
+    A s[4];
+    __builtin_memcpy(s, reinterpret_cast<const A*>(a.stats) + row * 4, sizeof(s));
     q.m = s[0];
     q.c = s[1];
     q.r = s[2];
@@ -140,6 +195,7 @@ template <typename T, int VEC, int MODE, int TPR, int NV>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
     using A = typename Acc<T>::type;
     using Raw = typename Words<VEC * (int)sizeof(T)>::type;
+    static_assert(sizeof(Raw) == VEC * sizeof(T), "the words of a pack");
     constexpr int THREADS = TPR > 256 ? TPR : 256, SLOTS = THREADS / TPR, K = MODE == 2 ? 7 : 2;
     __shared__ A lds[THREADS * VEC];
     const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
@@ -147,14 +203,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
     A w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int col = (j * TPR + lane) * VEC;
-        if (col < a.C) params<A, VEC>(a.w, a.wtype, col, (A)1, w[j]);
+        const int col = place<VEC>((j * TPR + lane) * VEC, a.C);
+        params<A, VEC>(a.w, a.wtype, col, (A)1, w[j]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            if (col >= a.C) w[j][e] = 0;
-            sw[j][e] = sb[j][e] = 0;
-        }
-        if (MODE == 0 && col < a.C) params<A, VEC>(a.b, a.wtype, col, (A)0, sb[j]);
+        for (int e = 0; e < VEC; ++e) sw[j][e] = sb[j][e] = 0;
+        if (MODE == 0) params<A, VEC>(a.b, a.wtype, col, (A)0, sb[j]);
     }
     for (int64_t first = (int64_t)blockIdx.x * SLOTS; first < a.rows; first += (int64_t)gridDim.x * SLOTS) {
         const int64_t row = first + slot;
@@ -163,20 +216,22 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
         Raw rx[NV], rd[NV], ru[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (j * TPR + lane) * VEC;
-            const int64_t at = base + (col < a.C ? col : 0);
-            rx[j] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.x) + at);
-            if constexpr (MODE != 0) rd[j] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.dy) + at);
-            if constexpr (MODE == 2) ru[j] = *reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.u) + at);
+            const int64_t at = base + place<VEC>((j * TPR + lane) * VEC, a.C);
+            const auto words = [&](const void* p) {
+                Raw r;
+                __builtin_memcpy(&r, reinterpret_cast<const T*>(p) + at, sizeof(r));
+                return r;
+            };
+            rx[j] = words(a.x);
+            if constexpr (MODE != 0) rd[j] = words(a.dy);
+            if constexpr (MODE == 2) ru[j] = words(a.u);
         }
         if constexpr (MODE == 0) {
             A s1[1] = {0};
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const Pack<T, VEC> x = unpacked<T, VEC>(rx[j]);
-                if ((j * TPR + lane) * VEC < a.C)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) s1[0] += (A)x.e[e] * unit;
+                each<VEC>((j * TPR + lane) * VEC - (a.C - VEC), [&](int e) { s1[0] += (A)x.e[e] * unit; });
             }
             row_sums<TPR>(s1, lds);
             const A m = within(s1[0] * (A)a.mean);
@@ -184,13 +239,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const Pack<T, VEC> x = unpacked<T, VEC>(rx[j]);
-                if ((j * TPR + lane) * VEC < a.C)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const A d = (A)x.e[e] - m;
-                        s2[0] += d;
-                        s2[1] += d * d;
-                    }
+                each<VEC>((j * TPR + lane) * VEC - (a.C - VEC), [&](int e) {
+                    const A d = (A)x.e[e] - m;
+                    s2[0] += d;
+                    s2[1] += d * d;
+                });
             }
             row_sums<TPR>(s2, lds);
             const A c = s2[0] * inv;
@@ -210,7 +263,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) o.e[e] = (T)((((A)x.e[e] - m) - c) * r * w[j][e] + sb[j][e]);
-                stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + col, o);
+                put<T, VEC>(reinterpret_cast<T*>(a.y) + base + place<VEC>(col, a.C), o);
             }
         } else {
             Row<A> q;
@@ -226,11 +279,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
                 Pack<T, VEC> u = x;
                 if constexpr (MODE == 2) u = unpacked<T, VEC>(ru[j]);
                 A uw[VEC];
-                if (MODE == 2 && a.uw) params<A, VEC>(a.uw, a.wtype, col, (A)0, uw);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
+                if (MODE == 2 && a.uw) params<A, VEC>(a.uw, a.wtype, place<VEC>(col, a.C), (A)0, uw);
+                each<VEC>(col - (a.C - VEC), [&](int e) {
                     add_row<MODE>(s, q.h((A)x.e[e]), w[j][e] * (A)d.e[e], (A)u.e[e],
                                   MODE == 2 && a.uw ? uw[e] * (A)d.e[e] : (A)0);
+                });
             }
             row_sums<TPR>(s, lds);
             take_row<MODE>(q, s, inv);
@@ -242,8 +295,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
                 Pack<T, VEC> u = x, o, o2;
                 if constexpr (MODE == 2) u = unpacked<T, VEC>(ru[j]);
                 A uw[VEC], ub[VEC];
-                if (MODE == 2 && a.uw) params<A, VEC>(a.uw, a.wtype, col, (A)0, uw);
-                if (MODE == 2 && a.ub) params<A, VEC>(a.ub, a.wtype, col, (A)0, ub);
+                if (MODE == 2 && a.uw) params<A, VEC>(a.uw, a.wtype, place<VEC>(col, a.C), (A)0, uw);
+                if (MODE == 2 && a.ub) params<A, VEC>(a.ub, a.wtype, place<VEC>(col, a.C), (A)0, ub);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const A h = q.h((A)x.e[e]), dv = (A)d.e[e], k = w[j][e] * dv;
@@ -264,8 +317,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
                         sw[j][e] += dv * pu;
                     }
                 }
-                stp<T, VEC>(reinterpret_cast<T*>(a.y) + base + col, o);
-                if constexpr (MODE == 2) stp<T, VEC>(reinterpret_cast<T*>(a.gdy) + base + col, o2);
+                put<T, VEC>(reinterpret_cast<T*>(a.y) + base + place<VEC>(col, a.C), o);
+                if constexpr (MODE == 2) put<T, VEC>(reinterpret_cast<T*>(a.gdy) + base + place<VEC>(col, a.C), o2);
             }
         }
     }
@@ -292,7 +345,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_held(Args a) {
             }
             if (slot == 0 && col < a.C)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) part[(int64_t)i * a.C + col + e] = v[e];
+                for (int e = 0; e < VEC; ++e) part[(int64_t)i * a.C + place<VEC>(col, a.C) + e] = v[e];
         }
     }
 }
@@ -309,22 +362,22 @@ template <typename T, int VEC, int MODE> __global__ __launch_bounds__(WIDE) void
         const T* x = reinterpret_cast<const T*>(a.x) + row * a.C;
         if constexpr (MODE == 0) {
             A s1[1] = {0};
-            for (int c = threadIdx.x * VEC; c < a.C; c += WIDE * VEC) {
-                const Pack<T, VEC> v = ldp<T, VEC>(x + c);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) s1[0] += (A)v.e[e] * unit;
+            for (int col = threadIdx.x * VEC; col < a.C; col += WIDE * VEC) {
+                const int c = place<VEC>(col, a.C);
+                const Pack<T, VEC> v = fetch<T, VEC>(x + c);
+                each<VEC>(col - c, [&](int e) { s1[0] += (A)v.e[e] * unit; });
             }
             row_sums<WIDE>(s1, lds);
             const A m = within(s1[0] * (A)a.mean);
             A s2[2] = {0, 0};
-            for (int c = threadIdx.x * VEC; c < a.C; c += WIDE * VEC) {
-                const Pack<T, VEC> v = ldp<T, VEC>(x + c);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
+            for (int col = threadIdx.x * VEC; col < a.C; col += WIDE * VEC) {
+                const int c = place<VEC>(col, a.C);
+                const Pack<T, VEC> v = fetch<T, VEC>(x + c);
+                each<VEC>(col - c, [&](int e) {
                     const A d = (A)v.e[e] - m;
                     s2[0] += d;
                     s2[1] += d * d;
-                }
+                });
             }
             row_sums<WIDE>(s2, lds);
             const A c = s2[0] * inv;
@@ -343,16 +396,17 @@ template <typename T, int VEC, int MODE> __global__ __launch_bounds__(WIDE) void
             A s[K];
 #pragma unroll
             for (int i = 0; i < K; ++i) s[i] = 0;
-            for (int c = threadIdx.x * VEC; c < a.C; c += WIDE * VEC) {
-                const Pack<T, VEC> xv = ldp<T, VEC>(x + c), dv = ldp<T, VEC>(dy + c);
+            for (int col = threadIdx.x * VEC; col < a.C; col += WIDE * VEC) {
+                const int c = place<VEC>(col, a.C);
+                const Pack<T, VEC> xv = fetch<T, VEC>(x + c), dv = fetch<T, VEC>(dy + c);
                 Pack<T, VEC> uv = xv;
-                if constexpr (MODE == 2) uv = ldp<T, VEC>(u + c);
+                if constexpr (MODE == 2) uv = fetch<T, VEC>(u + c);
                 A w[VEC], uw[VEC];
                 params<A, VEC>(a.w, a.wtype, c, (A)1, w);
                 params<A, VEC>(MODE == 2 ? a.uw : nullptr, a.wtype, c, (A)0, uw);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
+                each<VEC>(col - c, [&](int e) {
                     add_row<MODE>(s, q.h((A)xv.e[e]), w[e] * (A)dv.e[e], (A)uv.e[e], uw[e] * (A)dv.e[e]);
+                });
             }
             row_sums<WIDE>(s, lds);
             if (threadIdx.x == 0)
@@ -367,10 +421,10 @@ template <typename T, int VEC, int MODE> __global__ __launch_bounds__(256) void 
     using A = typename Acc<T>::type;
     constexpr int K = MODE == 2 ? 7 : 2;
     const int tiles = (a.C + 256 * VEC - 1) / (256 * VEC);
-    const int col = ((int)(blockIdx.x % tiles) * 256 + threadIdx.x) * VEC;
+    const int from_col = ((int)(blockIdx.x % tiles) * 256 + threadIdx.x) * VEC, col = place<VEC>(from_col, a.C);
     const int64_t chunk = blockIdx.x / tiles, from = chunk * a.chunk;
     const int64_t to = from + a.chunk < a.rows ? from + a.chunk : a.rows;
-    if (col >= a.C) return;
+    if (from_col >= a.C) return;
     const A inv = (A)a.inv;
     A w[VEC], b[VEC], uw[VEC], ub[VEC], sw[VEC], sb[VEC];
     params<A, VEC>(a.w, a.wtype, col, (A)1, w);
@@ -381,10 +435,10 @@ template <typename T, int VEC, int MODE> __global__ __launch_bounds__(256) void 
     for (int e = 0; e < VEC; ++e) sw[e] = sb[e] = 0;
     for (int64_t row = from; row < to; ++row) {
         const int64_t at = row * a.C + col;
-        const Pack<T, VEC> x = ldp<T, VEC>(reinterpret_cast<const T*>(a.x) + at);
+        const Pack<T, VEC> x = fetch<T, VEC>(reinterpret_cast<const T*>(a.x) + at);
         Pack<T, VEC> d = x, u = x, o, o2;
-        if constexpr (MODE != 0) d = ldp<T, VEC>(reinterpret_cast<const T*>(a.dy) + at);
-        if constexpr (MODE == 2) u = ldp<T, VEC>(reinterpret_cast<const T*>(a.u) + at);
+        if constexpr (MODE != 0) d = fetch<T, VEC>(reinterpret_cast<const T*>(a.dy) + at);
+        if constexpr (MODE == 2) u = fetch<T, VEC>(reinterpret_cast<const T*>(a.u) + at);
         Row<A> q;
         load_stats(a, row, q);
         if constexpr (MODE != 0) {
@@ -411,8 +465,8 @@ template <typename T, int VEC, int MODE> __global__ __launch_bounds__(256) void 
                 sw[e] += dv * pu;
             }
         }
-        stp<T, VEC>(reinterpret_cast<T*>(a.y) + at, o);
-        if constexpr (MODE == 2) stp<T, VEC>(reinterpret_cast<T*>(a.gdy) + at, o2);
+        put<T, VEC>(reinterpret_cast<T*>(a.y) + at, o);
+        if constexpr (MODE == 2) put<T, VEC>(reinterpret_cast<T*>(a.gdy) + at, o2);
     }
     if (MODE == 0 || !a.part) return;
     A* part = reinterpret_cast<A*>(a.part) + chunk * 2 * a.C + col;
@@ -423,9 +477,8 @@ template <typename T, int VEC, int MODE> __global__ __launch_bounds__(256) void 
     }
 }
 
-// The workgroups' sums added up: 16 columns a workgroup, 64 threads for each.
-constexpr int PCOLS = 16, PROWS = 64;
-template <typename A>
+// The workgroups' sums added up, PCOLS columns a workgroup.
+template <typename A, int PCOLS, int PROWS = 1024 / PCOLS>
 __global__ __launch_bounds__(PCOLS * PROWS) void k_params(const void* part_, int64_t parts, int C, int wtype, void* dw, void* db) {
     __shared__ A lds[PROWS][PCOLS + 1];
     void* const out = blockIdx.y == 0 ? dw : db;
@@ -471,28 +524,26 @@ static int check(int dtype, int wtype, int64_t rows, int C) {
 
 static int64_t acc_bytes(int dtype) { return dtype == EBR_DTYPE_F64 ? 8 : 4; }
 
-// How rows are laid out over threads, from the sizes alone.
+// How rows are laid out over threads, from the sizes alone: 8 to 32 elements a thread. A wave takes rows of up to 2048, without a
+// barrier (16384 x 2048 bf16: forward 23.5 us; 26.8 by four waves of 8 elements a thread, backward the same 42), a workgroup of 256
+// threads rows of up to 8192 (1000 x 5003 fp32: forward 10.0 us, backward 16.3; 12.5 and 18.2 with 1024 threads), one of 1024
+// rows of up to 16384, as more elements a thread would not fit its registers.
 struct Plan {
-    int vec, tpr = 0, nv = 0;  // tpr 0: through k_rows and k_apply
+    int vec, tpr = 0, each = 0;  // tpr 0: through k_rows and k_apply
     int64_t parts, chunk = 0;
-    Plan(int dtype, int64_t rows, int C, bool aligned) {
-        const int full = dtype == EBR_DTYPE_F64 ? 2 : dtype == EBR_DTYPE_F32 ? 4 : 8;
-        vec = aligned && C % full == 0 ? full : 1;
+    Plan(int mode, int dtype, int64_t rows, int C) {
+        vec = dtype == EBR_DTYPE_F64 ? 2 : dtype == EBR_DTYPE_F32 ? 4 : 8;
+        if (C < vec) vec = 1;
         if (dtype != EBR_DTYPE_F64) {
-            if (vec > 1) {
-                for (const int t : {16, 32, 64, 256, 1024})
-                    if (tpr == 0 && C <= (t < 64 ? 1 : 4) * t * vec) tpr = t;
-                if (tpr) nv = (C + tpr * vec - 1) / (tpr * vec);
-                if (tpr > 64 && nv < 2) nv = 2;
-            } else {
-                if (C <= 256) tpr = 64, nv = 4;
-                else if (C <= 1024) tpr = 256, nv = 4;
-                else if (C <= 8192) tpr = 1024, nv = C <= 4096 ? 4 : 8;
-            }
+            for (const int t : {16, 32, 64, 256, 1024})
+                if (tpr == 0 && C <= (t < 64 ? 8 : t < 1024 ? 32 : 16) * t) tpr = t;
+            if (tpr) each = vec == 1 ? 1 : (C + tpr * 8 - 1) / (tpr * 8) * 8;
         }
         if (tpr) {
             const int slots = tpr < 256 ? 256 / tpr : 1;
-            const int64_t groups = (rows + slots - 1) / slots, most = tpr == 1024 ? 512 : 1024;
+            // as many as the card holds at once where they keep sums (16384 x 2048 bf16 backward: 42 us with 512, 49 with 1024)
+            const int64_t groups = (rows + slots - 1) / slots;
+            const int64_t most = (mode == 0 ? 2048 : each > 16 ? 512 : 1024) / (tpr == 1024 ? 2 : 1);
             parts = groups < most ? groups : most;
         } else {
             const int64_t tiles = (C + 256 * vec - 1) / (256 * vec);
@@ -515,26 +566,18 @@ struct Scratch {
     int64_t all() const { return part + rowc + 16; }
 };
 
-static bool all_aligned(std::initializer_list<const void*> ps) {
-    for (const void* p : ps)
-        if (!aligned(p, 16)) return false;
-    return true;
-}
-
 template <typename T, int VEC, int MODE> static void launch(hipStream_t s, const Plan& p, const Args& a) {
     const dim3 grid((unsigned)p.parts);
-#define EBR_HELD(TPR, NV)                                                                                        \
-    if (p.tpr == TPR && p.nv == NV) {                                                                            \
-        hipLaunchKernelGGL((k_held<T, VEC, MODE, TPR, NV>), grid, dim3(TPR > 256 ? TPR : 256), 0, s, a);         \
-        return;                                                                                                  \
+#define EBR_HELD(TPR, EACH)                                                                                          \
+    if (p.tpr == TPR && p.each == EACH) {                                                                            \
+        hipLaunchKernelGGL((k_held<T, VEC, MODE, TPR, EACH / VEC>), grid, dim3(TPR > 256 ? TPR : 256), 0, s, a);     \
+        return;                                                                                                      \
     }
-    if constexpr (sizeof(T) < 8) {
-        if constexpr (VEC > 1) {
-            EBR_HELD(16, 1) EBR_HELD(32, 1) EBR_HELD(64, 1) EBR_HELD(64, 2) EBR_HELD(64, 3) EBR_HELD(64, 4)
-            EBR_HELD(256, 2) EBR_HELD(256, 3) EBR_HELD(256, 4) EBR_HELD(1024, 2) EBR_HELD(1024, 3) EBR_HELD(1024, 4)
-        } else {
-            EBR_HELD(64, 4) EBR_HELD(256, 4) EBR_HELD(1024, 4) EBR_HELD(1024, 8)
-        }
+    if constexpr (sizeof(T) < 8 && VEC == 1) {
+        EBR_HELD(16, 1)
+    } else if constexpr (sizeof(T) < 8) {
+        EBR_HELD(16, 8) EBR_HELD(32, 8) EBR_HELD(64, 8) EBR_HELD(64, 16) EBR_HELD(64, 24) EBR_HELD(64, 32)
+        EBR_HELD(256, 8) EBR_HELD(256, 16) EBR_HELD(256, 24) EBR_HELD(256, 32) EBR_HELD(1024, 8) EBR_HELD(1024, 16)
     }
 #undef EBR_HELD
     const int64_t tiles = (a.C + 256 * VEC - 1) / (256 * VEC);
@@ -543,7 +586,7 @@ template <typename T, int VEC, int MODE> static void launch(hipStream_t s, const
 }
 
 template <int MODE> static int run(int dtype, Args a, void* dw, void* db, void* scratch, void* stream) {
-    const Plan p(dtype, a.rows, a.C, all_aligned({a.x, a.dy, a.u, a.y, a.gdy}));
+    const Plan p(MODE, dtype, a.rows, a.C);
     const Scratch sc(p, MODE, dtype, a.rows, a.C);
     a.part = dw || db ? scratch : nullptr;
     a.rowc = reinterpret_cast<char*>(scratch) + sc.part;
@@ -554,12 +597,15 @@ template <int MODE> static int run(int dtype, Args a, void* dw, void* db, void* 
     hipStream_t s = (hipStream_t)stream;
     const auto with = [&](auto v) {
         using T = decltype(v);
-        constexpr int FULL = 16 / (int)sizeof(T);
-        if (p.vec > 1) launch<T, FULL, MODE>(s, p, a);
+        if (p.vec > 1) launch<T, 16 / (int)sizeof(T), MODE>(s, p, a);
         else launch<T, 1, MODE>(s, p, a);
-        if (MODE != 0 && a.part)
-            hipLaunchKernelGGL((k_params<typename Acc<T>::type>), dim3((a.C + PCOLS - 1) / PCOLS, MODE == 1 ? 2 : 1),
-                               dim3(PCOLS * PROWS), 0, s, a.part, p.parts, a.C, a.wtype, dw, db);
+        if (MODE == 0 || !a.part) return;
+        using A = typename Acc<T>::type;
+        const int pcols = a.C >= 4096 ? 64 : 16;  // (500 sums of 5003 in 64 columns each: 6.0 us, in 16: 10.0)
+        const dim3 grid((a.C + pcols - 1) / pcols, MODE == 1 ? 2 : 1);
+        const auto add = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(1024), 0, s, a.part, p.parts, a.C, a.wtype, dw, db); };
+        if (pcols == 64) add(k_params<A, 64>);
+        else add(k_params<A, 16>);
     };
     switch (dtype) {
         case EBR_DTYPE_F32: with(float()); break;
@@ -578,12 +624,7 @@ extern "C" {
 
 int64_t ebr_block_layernorm_scratch(int dtype, int order, int64_t rows, int C) {
     if (check(dtype, dtype, rows, C) || order < 0 || order > 2) return -1;
-    int64_t most = 0;
-    for (const bool aligned : {true, false}) {  // tensors off 16-byte alignment take another plan
-        const int64_t n = Scratch(Plan(dtype, rows, C, aligned), order, dtype, rows, C).all();
-        most = n > most ? n : most;
-    }
-    return most;
+    return Scratch(Plan(order, dtype, rows, C), order, dtype, rows, C).all();
 }
 
 int ebr_block_layernorm(int dtype, int wtype, int64_t rows, int C, double eps, const void* x, const void* w, const void* b,
