@@ -622,6 +622,86 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     }
 }
 
+// Few rows of x: the weight, once, straight into registers, bound by its bytes. A workgroup's waves take 16 rows of gate and of
+// up, and of their k 128 bytes in turns; the order of k within a product is the lanes' own (each brings 16 bytes of its row of
+// either operand), so that a wave's loads take whole lines. The waves' sums are added up through shared memory.
+//
+// Against tiles of 64, weights from memory, us: bf16 C 2048 I 5632 14.5 : 18.7 for one row (3.2 TB/s), 19.4 : 18.8 for 17, 24.7 :
+// 19.1 for 33; C 4096 I 11008 40 : 46 (4.5 TB/s), 53 : 53, 65 : 55; C 256 I 768 2.7 : 4.1, 3.2 : 4.1, 3.6 : 4.2; fp32 C 2048 I 5632
+// 31 : 68, 45 : 68, 66 : 68. So for up to 32 rows.
+template <typename T> struct Mma16;
+template <> struct Mma16<__bf16> {
+    static __device__ __forceinline__ f32x4 step(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma16<_Float16> {
+    static __device__ __forceinline__ f32x4 step(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma16<float> {
+    static __device__ __forceinline__ f32x4 step(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)a[e]),
+                                                     __builtin_bit_cast(float, (uint32_t)b[e]), c, 0, 0, 0);
+        return c;
+    }
+};
+constexpr int FEW = 32, FEW_WAVES = 8;
+template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void k_few(Args a) {
+    constexpr int EPC = 16 / (int)sizeof(T), TURN = 8 * EPC, AT_ONCE = 4;  // k of a wave's turn; turns under way
+    __shared__ f32x4 sums[FEW_WAVES][2][FJ][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, part = lane >> 4;
+    const int64_t i0 = (int64_t)blockIdx.x * 16, row = i0 + l16 < a.ni ? i0 + l16 : a.ni - 1;  // (the last one again past the end)
+    const T* const gate = reinterpret_cast<const T*>(a.a[0]) + row * a.lda;
+    const T* const up = gate + a.ni * a.lda;
+    const T* const x = reinterpret_cast<const T*>(a.b[0]);
+    f32x4 acc[2][FJ] = {};
+    for (int64_t k0 = wave * TURN; k0 < a.nk; k0 += FEW_WAVES * TURN * AT_ONCE) {
+        u32x4 g[AT_ONCE][2], u[AT_ONCE][2], b[AT_ONCE][2][FJ];
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t k = k0 + t * FEW_WAVES * TURN + (part * 2 + h) * EPC;
+                const bool in = k < a.nk;
+                g[t][h] = in ? *reinterpret_cast<const u32x4*>(gate + k) : u32x4{};
+                u[t][h] = in ? *reinterpret_cast<const u32x4*>(up + k) : u32x4{};
+#pragma unroll
+                for (int j = 0; j < FJ; ++j)
+                    b[t][h][j] = in && j * 16 + l16 < a.nj ? *reinterpret_cast<const u32x4*>(x + (j * 16 + l16) * a.ldb + k) : u32x4{};
+            }
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j) {
+                    acc[0][j] = Mma16<T>::step(g[t][h], b[t][h][j], acc[0][j]);
+                    acc[1][j] = Mma16<T>::step(u[t][h], b[t][h][j], acc[1][j]);
+                }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) sums[wave][h][j][lane] = acc[h][j];
+    __syncthreads();
+    if (wave >= FJ) return;
+    f32x4 g = {}, u = {};
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w) {
+        g += sums[w][0][wave][lane];
+        u += sums[w][1][wave][lane];
+    }
+    const int64_t n = wave * 16 + l16, i = i0 + 4 * part;
+    if (n >= a.nj || i >= a.ni) return;
+    const float v[4] = {gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3])};
+    put4(reinterpret_cast<T*>(a.out) + n * a.ni + i, v, 4, true);
+}
+
 // fp64, for gradient checks: 64 x 64 of D (gated: of each half, and of both right operands) a workgroup, 4 x 4 a thread.
 template <int ALIES, int BLIES, int EP> __global__ __launch_bounds__(256) void k_product64(Args a) {
     constexpr int NA = EP >= EP_FWD ? 2 : 1, NB = EP == EP_BWD2 ? 2 : 1;
@@ -831,6 +911,12 @@ static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* 
     else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, part, c.splits, n, (float*)dw);
 }
 
+template <typename T> static void few(hipStream_t s, const Args& a) {
+    const dim3 grid((unsigned)((a.ni + 15) / 16)), threads(64 * FEW_WAVES);
+    if (a.nj <= 16) hipLaunchKernelGGL((k_few<T, 1>), grid, threads, 0, s, a);
+    else hipLaunchKernelGGL((k_few<T, 2>), grid, threads, 0, s, a);
+}
+
 static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 }  // namespace ebr_glu
@@ -860,6 +946,12 @@ int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const vo
     const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, y});
     Args a = {};
     a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = y;
+    if (!any && N <= FEW) {
+        if (dtype == EBR_DTYPE_F32) few<float>((hipStream_t)stream, a);
+        else if (dtype == EBR_DTYPE_BF16) few<__bf16>((hipStream_t)stream, a);
+        else few<_Float16>((hipStream_t)stream, a);
+        return launched();
+    }
     product<K_ROWS, K_ROWS, EP_FWD>(dtype, any, Cut(dtype, I, N, C, 1, 1, false, any), a, (hipStream_t)stream);
     return launched();
 }

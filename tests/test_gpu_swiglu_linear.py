@@ -127,6 +127,20 @@ def test_sizes(cuda, N, C, I, dtype):
     _check(*_inputs(cuda, N, C, I, dtype, seed=N).values())
 
 
+# up to 32 rows, whose forward reads the weight by itself: rows off 16, a last turn that is not full, many turns, widths off 16
+@pytest.mark.parametrize("N", [1, 3, 15, 16, 17, 31, 32])
+@pytest.mark.parametrize("C,I", [(8, 8), (72, 24), (520, 16), (2056, 40), (5000, 1000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_few_rows(cuda, N, C, I, dtype):
+    _say(f"swiglu_linear few rows {N} {C} {I} {dtype}")
+    ts = _inputs(cuda, N, C, I, dtype, seed=N + C)
+    y = block.swiglu_linear(ts["x"], ts["w"])
+    (want, *_), (tol, *_) = _forms(*ts.values())
+    assert y.dtype == dtype and y.shape == (N, I) and bool(((y.double() - want).abs() <= tol).all())
+    one = block.swiglu_linear(ts["x"][N - 1], ts["w"])  # a row alone, of one dimension: the same sums
+    assert N > 16 or torch.equal(one, y[N - 1])
+
+
 @pytest.mark.parametrize("N,C,I", [(1, 5, 3), (70, 65, 66), (129, 31, 40)])
 def test_fp64(cuda, N, C, I):
     _say(f"swiglu_linear fp64 {N} {C} {I}")
