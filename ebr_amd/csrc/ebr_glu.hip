@@ -327,7 +327,7 @@ __device__ __forceinline__ int left(int64_t n) { return n > 256 ? 256 : (int)n; 
 // What becomes of a wave's sums, 32 rows at a time through ``at``, shared memory of its own.
 template <typename T, int EP, int FI, int FJ>
 __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t ifrom, int64_t jfrom, int split,
-                                       unsigned char* at, int lane) {
+                                       unsigned char* at, unsigned char* at4, int lane) {
     constexpr bool TWO = EP == EP_BWD2;
     const int l32 = lane & 31, il = 4 * (lane >> 5);
     if constexpr (EP < EP_FWD) {
@@ -354,7 +354,7 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
             }
     } else {
         using P = Plane<T, FI * 16>;  // of gate or up, each half of the wave's rows of A
-        enum { DY = 0, Y = 0, DG = 1, DU = 2, GG = 3, GU = 4 };
+        enum { DY = 0, Y = 0, DG = 1, DU = 2, GG = 3 };  // and GU at ``at4``
         const int64_t col = ifrom / 2;
         const int cols = left(a.ni - col);
         T* const y = reinterpret_cast<T*>(a.out);
@@ -389,7 +389,7 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
                     }
                     if constexpr (TWO) {
                         P::put(at + GG * P::BYTES, l32, c, rg);
-                        P::put(at + GU * P::BYTES, l32, c, ru);
+                        P::put(at4, l32, c, ru);
                     }
                     if constexpr (EP != EP_FWD) __builtin_amdgcn_sched_barrier(0);  // (several at once would not fit the registers)
                 }
@@ -401,7 +401,7 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
             }
             if (TWO && ggu) {
                 P::store(at + GG * P::BYTES, ggu + two, 2 * a.ni, rows, cols, lane);
-                P::store(at + GU * P::BYTES, ggu + two + a.ni, 2 * a.ni, rows, cols, lane);
+                P::store(at4, ggu + two + a.ni, 2 * a.ni, rows, cols, lane);
             }
         }
     }
@@ -484,13 +484,14 @@ template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int 
 __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     constexpr int WAVES = WI * WJ, FI = TI / WI / 32, FJ = TJ / WJ / 32;
     constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
-    constexpr bool STAGED = !ANY && sizeof(T) == 2 && TI >= 128;  // four waves, an array each
-    static_assert(!STAGED || WAVES == 4, "an array a wave");
+    constexpr bool STAGED = !ANY && sizeof(T) == 2 && TI >= 128;  // four waves, an array each, or eight, half of one
+    static_assert(!STAGED || WAVES == 4 || WAVES == 8, "an array a wave");
     static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
     using SA = Side<T, ALIES, TI, WAVES, GATED>;
     using SB = Side<T, BLIES, TJ, WAVES, TWO>;
     constexpr int BUFFER = SA::BYTES + SB::BYTES, MORE = ANY ? 16 : BUFFER;
-    __shared__ __attribute__((aligned(16))) unsigned char s0[BUFFER], s1[MORE], s2[MORE], s3[MORE];
+    constexpr int FIFTH = TWO && WAVES == 8 ? BUFFER / 8 : 0;  // a wave's fifth plane, where half a buffer holds four
+    __shared__ __attribute__((aligned(16))) unsigned char s0[BUFFER], s1[MORE], s2[MORE], s3[MORE], s4[FIFTH ? WAVES * FIFTH : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave % WI, wj = wave / WI;
     int ti, tj, split;
@@ -615,8 +616,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
 
     if constexpr (STAGED) {
         // (every wave is past its last read of the buffers: the last stage's barrier)
-        unsigned char* const own = wave == 0 ? s0 : wave == 1 ? s1 : wave == 2 ? s2 : s3;
-        finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, split, own, lane);
+        constexpr int PER = WAVES / 4, MINE = BUFFER / PER;
+        unsigned char* const own = (wave / PER == 0 ? s0 : wave / PER == 1 ? s1 : wave / PER == 2 ? s2 : s3) + wave % PER * MINE;
+        constexpr int FOUR = 4 * 32 * FI * 16 * (int)sizeof(T);  // planes
+        static_assert(!TWO || (FIFTH ? FOUR <= MINE && FOUR / 4 <= FIFTH : FOUR / 4 * 5 <= MINE), "a wave's planes");
+        finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, split, own, FIFTH ? s4 + wave * FIFTH : own + FOUR, lane);
     } else {
         finish_any<T, EP, FI, FJ, ANY>(a, acc, i0, j0, wi, wj, split, lane);
     }
@@ -812,7 +816,8 @@ struct Cut {
         tj = dtype == EBR_DTYPE_F64 ? up(nj, 64) : up(high, tile);
         steps = all;
         if (split && dtype != EBR_DTYPE_F64) {
-            const int64_t want = up(tile == 256 ? 256 : 512, ti * tj), most = up(all, 4);
+            // as many workgroups as the card holds at once, and not one more: 258 of 62208 x 256 -> 1536 took 165 us, 252 113
+            const int64_t want = (tile == 256 ? 256 : 512) / (ti * tj), most = up(all, 4);
             splits = (int)(want < most ? want : most);
             if (splits < 1) splits = 1;
             steps = up(all, splits);
@@ -828,7 +833,8 @@ template <typename T, int ALIES, int BLIES, int EP, bool ANY> static void launch
     } else {
         if constexpr (!ANY && sizeof(T) == 2) {
             if (c.tile == 256) {
-                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 2, 2, ANY>), grid, dim3(256), 0, s, a);
+                constexpr int WJ = EP >= EP_FWD ? 4 : 2;
+                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 2, WJ, ANY>), grid, dim3(128 * WJ), 0, s, a);
                 return;
             }
         }
