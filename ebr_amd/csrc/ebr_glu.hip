@@ -16,6 +16,7 @@
 // reads, and does not wait for them. Rows' 16-byte chunks (64-byte chunks for operands of the
 // second kind, which are read transposed) are exchanged by a function of the row, so that lanes meet no bank conflicts.
 // Whatever lies outside the tensors is read as zero by the buffer loads' bounds.
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -47,6 +48,7 @@ struct Args {
     int pairs, splits;
     int64_t steps;            // stages of a split
     int ti, tj;               // tiles
+    int tile0, count;         // those of this launch
     void *out, *dgu, *ggu;    // D, y or gdy; [dg|du]; [gg|gu]
     void *dgu2, *ggu2;        // what these lack of their values before rounding, or null
     const void *dy, *c;
@@ -247,18 +249,22 @@ template <int N> __device__ __forceinline__ void stage_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// The tile of a workgroup: each of the 8 XCDs, which take workgroups in turns, gets neighbouring tiles, and of those a block
-// of GROUP tiles of j goes with all i before the next.
-__device__ __forceinline__ void tile_of(const Args& a, int& ti, int& tj, int& split) {
+// Tile t: a block of GROUP tiles of j goes with all i before the next.
+__device__ __forceinline__ void place_of(const Args& a, unsigned t, int& ti, int& tj) {
     constexpr int GROUP = 8;
-    const unsigned tiles = (unsigned)a.ti * a.tj, all = tiles * a.splits, b = blockIdx.x;
-    const unsigned per = all / 8, more = all % 8, x = b % 8;
-    const unsigned at = x * per + (x < more ? x : more) + b / 8;
-    split = (int)(at / tiles);
-    const unsigned t = at % tiles, block = t / (GROUP * a.ti), first = block * GROUP;
+    const unsigned block = t / (GROUP * a.ti), first = block * GROUP;
     const unsigned rows = a.tj - first < GROUP ? a.tj - first : GROUP, in = t - block * GROUP * a.ti;
     tj = (int)(first + in % rows);
     ti = (int)(in / rows);
+}
+// The tile of a workgroup: each of the 8 XCDs, which take workgroups in turns, gets neighbouring tiles.
+__device__ __forceinline__ void tile_of(const Args& a, int& ti, int& tj, int& split, int& local) {
+    const unsigned tiles = (unsigned)a.count, all = tiles * a.splits, b = blockIdx.x;
+    const unsigned per = all / 8, more = all % 8, x = b % 8;
+    const unsigned at = x * per + (x < more ? x : more) + b / 8;
+    split = (int)(at / tiles);
+    local = (int)(at % tiles);
+    place_of(a, a.tile0 + local, ti, tj);
 }
 
 // A wave's way from its sums to rows of memory: planes of 32 rows of COLS values in shared memory, in chunks of 16 bytes exchanged
@@ -326,7 +332,7 @@ __device__ __forceinline__ int left(int64_t n) { return n > 256 ? 256 : (int)n; 
 
 // What becomes of a wave's sums, 32 rows at a time through ``at``, shared memory of its own.
 template <typename T, int EP, int FI, int FJ>
-__device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t ifrom, int64_t jfrom, int split,
+__device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t ifrom, int64_t jfrom, float* part, int ldp,
                                        unsigned char* at, unsigned char* at4, int lane) {
     constexpr bool TWO = EP == EP_BWD2;
     const int l32 = lane & 31, il = 4 * (lane >> 5);
@@ -334,7 +340,10 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
         using O = std::conditional_t<EP == EP_PART, float, T>;
         constexpr int COLS = 128 / (int)sizeof(O), EACH = COLS / 32;  // a plane's tiles of 32
         using P = Plane<O, COLS>;
-        O* const out = reinterpret_cast<O*>(a.out) + (EP == EP_PART ? (int64_t)split * a.nj * a.ni : 0);
+        O* out;  // at the wave's first place
+        int64_t ldo = ldp;
+        if constexpr (EP == EP_PART) out = part;
+        else out = reinterpret_cast<O*>(a.out) + jfrom * a.ldo + ifrom, ldo = a.ldo;
 #pragma unroll
         for (int j = 0; j < FJ; ++j)
 #pragma unroll
@@ -350,7 +359,7 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
                     }
                 __builtin_amdgcn_wave_barrier();
                 const int64_t row = jfrom + j * 32, col = ifrom + i * 32;
-                P::store(at + i / EACH * P::BYTES, out + row * a.ldo + col, a.ldo, left(a.nj - row), left(a.ni - col), lane);
+                P::store(at + i / EACH * P::BYTES, out + j * 32 * ldo + i * 32, ldo, left(a.nj - row), left(a.ni - col), lane);
             }
     } else {
         using P = Plane<T, FI * 16>;  // of gate or up, each half of the wave's rows of A
@@ -411,7 +420,7 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
 // values before rounding is written here alone).
 template <typename T, int EP, int FI, int FJ, bool ANY>
 __device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t i0, int64_t j0, int wi, int wj,
-                                           int split, int lane) {
+                                           float* part, int ldp, int lane) {
     constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
     const int64_t jl = j0 + wj * FJ * 32 + (lane & 31);
     const int il = 4 * (lane >> 5);
@@ -430,8 +439,7 @@ __device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI
                     if constexpr (EP == EP_OUT) {
                         put4(reinterpret_cast<T*>(a.out) + row * a.ldo + col, v, a.ni - col, !ANY);
                     } else {
-                        float* p = reinterpret_cast<float*>(a.out) + (split * a.nj + row) * a.ni + col;
-                        put4(p, v, a.ni - col, !ANY);
+                        put4(part + (row - j0) * ldp + (col - i0), v, a.ni - col, true);
                     }
                 }
         }
@@ -494,8 +502,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     __shared__ __attribute__((aligned(16))) unsigned char s0[BUFFER], s1[MORE], s2[MORE], s3[MORE], s4[FIFTH ? WAVES * FIFTH : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave % WI, wj = wave / WI;
-    int ti, tj, split;
-    tile_of(a, ti, tj, split);
+    int ti, tj, split, local;
+    tile_of(a, ti, tj, split, local);
     const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
     f32x16 acc[FI][FJ];
 #pragma unroll
@@ -614,15 +622,18 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
         stage_barrier<0>();  // (the loads past the end, of zeros, are done with the buffers)
     }
 
+    // the sums of a split: tile by tile
+    float* const part = EP == EP_PART ? reinterpret_cast<float*>(a.out) + ((int64_t)split * a.count + local) * (TI * TJ) : nullptr;
     if constexpr (STAGED) {
         // (every wave is past its last read of the buffers: the last stage's barrier)
         constexpr int PER = WAVES / 4, MINE = BUFFER / PER;
         unsigned char* const own = (wave / PER == 0 ? s0 : wave / PER == 1 ? s1 : wave / PER == 2 ? s2 : s3) + wave % PER * MINE;
         constexpr int FOUR = 4 * 32 * FI * 16 * (int)sizeof(T);  // planes
         static_assert(!TWO || (FIFTH ? FOUR <= MINE && FOUR / 4 <= FIFTH : FOUR / 4 * 5 <= MINE), "a wave's planes");
-        finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, split, own, FIFTH ? s4 + wave * FIFTH : own + FOUR, lane);
+        finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, EP == EP_PART ? part + wj * FJ * 32 * TI + wi * FI * 32 : part,
+                              TI, own, FIFTH ? s4 + wave * FIFTH : own + FOUR, lane);
     } else {
-        finish_any<T, EP, FI, FJ, ANY>(a, acc, i0, j0, wi, wj, split, lane);
+        finish_any<T, EP, FI, FJ, ANY>(a, acc, i0, j0, wi, wj, part, TI, lane);
     }
 }
 
@@ -768,18 +779,22 @@ template <int ALIES, int BLIES, int EP> __global__ __launch_bounds__(256) void k
         }
 }
 
-// The splits' partial sums added up, in their order.
-template <typename T> __global__ __launch_bounds__(256) void k_join(const float* part, int splits, int64_t n, T* out) {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-        float s[4] = {0, 0, 0, 0}, v[4];
-        for (int k = 0; k < splits; ++k) {
-            const float* p = part + k * n + i;
-            get4(p, v, n - i, n % 4 == 0);
+// The splits' partial sums of the tiles from tile0 on added up, in their order.
+template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int tile, const float* part, T* out, bool wide) {
+    const int per = tile * tile / 1024;  // workgroups of a tile
+    int ti, tj;
+    place_of(a, a.tile0 + blockIdx.x / per, ti, tj);
+    const int at = (blockIdx.x % per * 256 + threadIdx.x) * 4;
+    const int64_t row = (int64_t)tj * tile + at / tile, col = (int64_t)ti * tile + at % tile;
+    if (row >= a.nj || col >= a.ni) return;
+    float s[4] = {0, 0, 0, 0}, v[4];
+    const float* p = part + (int64_t)(blockIdx.x / per) * tile * tile + at;
+    for (int k = 0; k < a.splits; ++k, p += (int64_t)a.count * tile * tile) {
+        get4(p, v, 4, true);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] += v[e];
-        }
-        put4(out + i, s, n - i, n % 4 == 0);
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
     }
+    put4(out + row * a.ldo + col, s, a.ni - col, wide);
 }
 
 // -- launches ----------------------------------------------------------------------------------------------------------
@@ -799,8 +814,10 @@ static int check(int dtype, int64_t N, int64_t C, int64_t I) {
 struct Cut {
     int tile;            // 256, 128 or 64
     int64_t ti, tj;
-    int splits = 1;
-    int64_t steps;
+    int splits = 1;      // of the tiles from ``whole`` on
+    int64_t steps, whole;
+    int64_t tiles() const { return ti * tj; }
+    int64_t part_bytes() const { return splits > 1 ? splits * (tiles() - whole) * tile * tile * 4 : 0; }
     Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, bool split, bool any) {  // gated: 0, 1, or 2 for TWO
         const auto up = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
         const int64_t wide = gated ? 2 * ni : ni, high = gated == 2 ? 2 * nj : nj, all = up(nk, STAGE / size_of(dtype)) * pairs;
@@ -815,19 +832,24 @@ struct Cut {
         ti = dtype == EBR_DTYPE_F64 ? up(ni, 64) : up(wide, tile);
         tj = dtype == EBR_DTYPE_F64 ? up(nj, 64) : up(high, tile);
         steps = all;
+        whole = ti * tj;
         if (split && dtype != EBR_DTYPE_F64) {
-            // as many workgroups as the card holds at once, and not one more: 258 of 62208 x 256 -> 1536 took 165 us, 252 113
-            const int64_t want = (tile == 256 ? 256 : 512) / (ti * tj), most = up(all, 4);
-            splits = (int)(want < most ? want : most);
-            if (splits < 1) splits = 1;
-            steps = up(all, splits);
-            splits = (int)up(all, steps);
+            // As many workgroups as the card holds at once, and not one more: 258 of 62208 x 256 -> 1536 took 165 us, 252 113. Where
+            // there are more tiles than that, those of the last round alone are split: 352 of 8192 x 2048 -> 11264 take 357 us, 410 unsplit.
+            const int64_t held = tile == 256 ? 256 : 512, last = whole <= held ? whole : tile == 256 ? whole % held : 0;
+            const int64_t most = whole <= held ? up(all, 4) : all / 64;
+            const int64_t want = last ? std::min(held / last, most) : 1;
+            if (want > 1) {
+                steps = up(all, want);
+                splits = (int)up(all, steps);
+                if (splits > 1) whole -= last;
+            }
         }
     }
 };
 
 template <typename T, int ALIES, int BLIES, int EP, bool ANY> static void launch(hipStream_t s, const Cut& c, const Args& a) {
-    const dim3 grid((unsigned)(c.ti * c.tj * c.splits));
+    const dim3 grid((unsigned)(a.count * a.splits));
     if constexpr (std::is_same_v<T, double>) {
         hipLaunchKernelGGL((k_product64<ALIES, BLIES, EP>), grid, dim3(256), 0, s, a);
     } else {
@@ -846,8 +868,11 @@ template <typename T, int ALIES, int BLIES, int EP, bool ANY> static void launch
 }
 
 // One product, whose operands, strides, sizes and outputs ``a`` holds.
-template <int ALIES, int BLIES, int EP> static void product(int dtype, bool any, const Cut& c, Args a, hipStream_t s) {
-    a.ti = (int)c.ti, a.tj = (int)c.tj, a.splits = c.splits, a.steps = c.steps;
+template <int ALIES, int BLIES, int EP> static void product(int dtype, bool any, const Cut& c, Args& a, hipStream_t s) {
+    constexpr bool PART = EP == EP_PART;  // its tiles that are split, else those that are not
+    a.ti = (int)c.ti, a.tj = (int)c.tj, a.tile0 = PART ? (int)c.whole : 0, a.count = (int)(PART ? c.tiles() - c.whole : c.whole);
+    a.splits = PART ? c.splits : 1;
+    a.steps = PART ? c.steps : INT64_MAX / 4;
     const auto with = [&](auto v) {
         using T = decltype(v);
         if (any) launch<T, ALIES, BLIES, EP, true>(s, c, a);
@@ -903,18 +928,15 @@ static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* 
     const bool any = dtype == EBR_DTYPE_F64 || !fit || !whole(dtype, {C, 2 * I}, {dw});
     const Cut c = weight_cut(dtype, N, C, I, a.pairs, any);
     a.lda = C, a.ldb = 2 * I, a.ni = C, a.nj = 2 * I, a.nk = N, a.out = dw, a.ldo = C;
-    if (c.splits == 1) {
-        product<M_ROWS, M_ROWS, EP_OUT>(dtype, any, c, a, s);
-        return;
-    }
+    if (c.whole) product<M_ROWS, M_ROWS, EP_OUT>(dtype, any, c, a, s);
+    if (c.splits == 1) return;
     a.out = part;
     product<M_ROWS, M_ROWS, EP_PART>(dtype, any, c, a, s);
-    const int64_t n = 2 * I * C;
-    const dim3 grid(blocks_for(n, 1024));
-    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, part, c.splits, n, (__bf16*)dw);
-    else if (dtype == EBR_DTYPE_F16)
-        hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, part, c.splits, n, (_Float16*)dw);
-    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, part, c.splits, n, (float*)dw);
+    const dim3 grid((unsigned)(a.count * (c.tile * c.tile / 1024)));
+    const bool wide = C % 4 == 0 && aligned(dw, 16);
+    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, a, c.tile, part, (__bf16*)dw, wide);
+    else if (dtype == EBR_DTYPE_F16) hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, a, c.tile, part, (_Float16*)dw, wide);
+    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, a, c.tile, part, (float*)dw, wide);
 }
 
 template <typename T> static void few(hipStream_t s, const Args& a) {
@@ -937,9 +959,7 @@ int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t
     int64_t part = 0;
     const int64_t each = with_rest(dtype, N) ? 2 : 1;
     for (const bool any : {false, true}) {
-        const Cut c = weight_cut(dtype, N, C, I, (int)(order * each), any);
-        const int64_t n = c.splits > 1 ? c.splits * 2 * I * C * 4 : 0;
-        part = n > part ? n : part;
+        part = std::max(part, weight_cut(dtype, N, C, I, (int)(order * each), any).part_bytes());
     }
     // [dg|du], for order 2 [gg|gu] too, and the weight gradient's partial sums
     return order * each * up16(N * 2 * I * size_of(dtype)) + part + 16;

@@ -154,6 +154,14 @@ def test_the_large_tiles(cuda):
         _check(*_inputs(cuda, N, C, I, torch.bfloat16, seed=C).values())
 
 
+def test_more_tiles_than_a_round(cuda):
+    """The weight's gradient in 288 tiles of 256, the last 32 of which split their rows, some with an edge."""
+    _say("swiglu_linear more tiles than a round")
+    a = _check(*_inputs(cuda, 4100, 4096, 2184, torch.bfloat16, seed=6).values())
+    b = _run(*_inputs(cuda, 4100, 4096, 2184, torch.bfloat16, seed=6).values())
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_large_gates(cuda):
     """Gates of some hundreds, whose exponentials leave the range on either side."""
     _say("swiglu_linear large gates")
