@@ -174,7 +174,7 @@ SIGNATURES = {
     "ebr_block_layernorm_bwd": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int] + [_P] * 9),
     "ebr_block_layernorm_bwd2": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int] + [_P] * 12),
     "ebr_block_layernorm_scratch": (ctypes.c_int64, [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_int]),
-    "ebr_block_swiglu_linear": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 4),
+    "ebr_block_swiglu_linear": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 5),
     "ebr_block_swiglu_linear_bwd": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 7),
     "ebr_block_swiglu_linear_bwd2": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 3 + [_P] * 9),
     "ebr_block_swiglu_linear_scratch": (ctypes.c_int64, [ctypes.c_int] * 2 + [ctypes.c_int64] * 3),

@@ -797,6 +797,12 @@ def _projection(x: Tensor, w: Tensor) -> Tuple[int, int, int]:
     return x.numel() // x.shape[-1], x.shape[-1], w.shape[0] // 2
 
 
+def _whole(t: Tensor) -> Tensor:
+    """t contiguous and 16-byte aligned."""
+    t = _c(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _projection_scratch(x: Tensor, order: int, N: int, C: int, I: int) -> Tensor:
     n = hip_library().ebr_block_swiglu_linear_scratch(_code(x), order, N, C, I)
     if n < 0:
@@ -808,12 +814,15 @@ def _projection_scratch(x: Tensor, order: int, N: int, C: int, I: int) -> Tensor
 def swiglu_linear_op(x: Tensor, weight: Tensor) -> Tensor:
     lib = hip_library()
     code, (N, C, I) = _code(x), _projection(x, weight)
-    x, weight = _c(x), _c(weight)
+    x, weight = _whole(x), _whole(weight)
     y = x.new_empty((*x.shape[:-1], I))
     if N == 0:
         return y
+    scratch = _projection_scratch(x, 0, N, C, I)
     with torch.cuda.device(x.device):
-        rc = lib.ebr_block_swiglu_linear(code, N, C, I, x.data_ptr(), weight.data_ptr(), y.data_ptr(), _stream(x))
+        rc = lib.ebr_block_swiglu_linear(
+            code, N, C, I, x.data_ptr(), weight.data_ptr(), y.data_ptr(), scratch.data_ptr(), _stream(x)
+        )
     _capi.check(rc, "ebr_block_swiglu_linear")
     return y
 
@@ -829,7 +838,7 @@ def swiglu_linear_bwd_op(x: Tensor, weight: Tensor, dy: Tensor, want_x: bool, wa
     lib = hip_library()
     code, (N, C, I) = _code(x), _projection(x, weight)
     _like(dy, (*x.shape[:-1], I), x, "dy")
-    x, weight, dy = _c(x), _c(weight), _c(dy.to(x.dtype))
+    x, weight, dy = _whole(x), _whole(weight), _whole(dy.to(x.dtype))
     dx = x.new_empty(x.shape if want_x else (0,))
     dw = x.new_empty(weight.shape if want_w else (0,))
     if N == 0:
@@ -857,7 +866,7 @@ def swiglu_linear_bwd2_op(x: Tensor, weight: Tensor, dy: Tensor, c: Tensor, want
     code, (N, C, I) = _code(x), _projection(x, weight)
     _like(dy, (*x.shape[:-1], I), x, "dy")
     _like(c, x.shape, x, "c")
-    x, weight, dy, c = _c(x), _c(weight), _c(dy.to(x.dtype)), _c(c.to(x.dtype))
+    x, weight, dy, c = _whole(x), _whole(weight), _whole(dy.to(x.dtype)), _whole(c.to(x.dtype))
     gx = x.new_empty(x.shape if want_x else (0,))
     gw = x.new_empty(weight.shape if want_w else (0,))
     gdy = torch.empty_like(dy)

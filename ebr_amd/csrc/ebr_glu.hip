@@ -136,26 +136,6 @@ template <typename T, int LIES, int ROWS, int WAVES, bool PAIRED> struct Side {
         }
 #endif
     }
-    // The same for operands of any alignment and width, through registers.
-    static __device__ __forceinline__ void load_any(const T* base, const T* base2, int64_t first, int64_t n, int64_t ld,
-                                                    int64_t k0, int64_t nk, unsigned char* to) {
-        for (int p = threadIdx.x; p < BYTES / 16; p += WAVES * 64) {
-            int row, at;
-            chunk(p, row, at);
-            T v[EPC];
-#pragma unroll
-            for (int e = 0; e < EPC; ++e) {
-                v[e] = (T)0.f;
-                if constexpr (LIES == K_ROWS) {
-                    const int64_t s = source(row, first, n);
-                    if (s >= 0 && k0 + at + e < nk) v[e] = (other(row) ? base2 : base)[s * ld + k0 + at + e];
-                } else {
-                    if (k0 + row < nk && first + at + e < n) v[e] = base[(k0 + row) * ld + first + at + e];
-                }
-            }
-            __builtin_memcpy(to + p * 16, v, 16);
-        }
-    }
     // The 32 rows from r0 (a multiple of 32) at step s of a stage: lane (row l % 32, half l / 32) gets EPC values of k.
     static __device__ __forceinline__ u32x4 read(const unsigned char* from, int r0, int s, int lane) {
         const int l32 = lane & 31, half = lane >> 5;
@@ -416,10 +396,10 @@ __device__ __forceinline__ void finish(const Args& a, const f32x16 (&acc)[FI][FJ
     }
 }
 
-// The same straight from the registers, for tensors of any width and alignment and for few rows (what [dg|du] lacks of its
+// The same straight from the registers, for fp32 and for few rows (what [dg|du] lacks of its
 // values before rounding is written here alone).
-template <typename T, int EP, int FI, int FJ, bool ANY>
-__device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t i0, int64_t j0, int wi, int wj,
+template <typename T, int EP, int FI, int FJ>
+__device__ __forceinline__ void finish_few(const Args& a, const f32x16 (&acc)[FI][FJ], int64_t i0, int64_t j0, int wi, int wj,
                                            float* part, int ldp, int lane) {
     constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
     const int64_t jl = j0 + wj * FJ * 32 + (lane & 31);
@@ -437,7 +417,7 @@ __device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI
                     const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                     if (col >= a.ni) continue;
                     if constexpr (EP == EP_OUT) {
-                        put4(reinterpret_cast<T*>(a.out) + row * a.ldo + col, v, a.ni - col, !ANY);
+                        put4(reinterpret_cast<T*>(a.out) + row * a.ldo + col, v, a.ni - col, true);
                     } else {
                         put4(part + (row - j0) * ldp + (col - i0), v, a.ni - col, true);
                     }
@@ -458,29 +438,29 @@ __device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI
                     T* const dgu = reinterpret_cast<T*>(a.dgu) + two;
                     T* const ggu = reinterpret_cast<T*>(a.ggu) + two;
                     float dy[4], og[4], ou[4], o[4];
-                    if constexpr (EP != EP_FWD) get4(reinterpret_cast<const T*>(a.dy) + at, dy, n, !ANY);
+                    if constexpr (EP != EP_FWD) get4(reinterpret_cast<const T*>(a.dy) + at, dy, n, true);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float g = acc[i][j][4 * q + e], u = acc[i + 1][j][4 * q + e];
                         if constexpr (EP == EP_FWD) o[e] = gated(g, u);
                         else first_of(g, u, dy[e], og[e], ou[e]);
                     }
-                    if constexpr (EP == EP_FWD) put4(reinterpret_cast<T*>(a.out) + at, o, n, !ANY);
+                    if constexpr (EP == EP_FWD) put4(reinterpret_cast<T*>(a.out) + at, o, n, true);
                     if (EP == EP_BWD || (TWO && a.dgu)) {
-                        put4(dgu, og, n, !ANY);
-                        put4(dgu + a.ni, ou, n, !ANY);
-                        if (a.dgu2) put_rest(reinterpret_cast<T*>(a.dgu2) + two, og, ou, a.ni, n, !ANY);
+                        put4(dgu, og, n, true);
+                        put4(dgu + a.ni, ou, n, true);
+                        if (a.dgu2) put_rest(reinterpret_cast<T*>(a.dgu2) + two, og, ou, a.ni, n, true);
                     }
                     if constexpr (TWO) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             second_of(acc[i][j][4 * q + e], acc[i + 1][j][4 * q + e], dy[e], acc[i][j + 1][4 * q + e],
                                       acc[i + 1][j + 1][4 * q + e], og[e], ou[e], o[e]);
-                        put4(reinterpret_cast<T*>(a.out) + at, o, n, !ANY);
+                        put4(reinterpret_cast<T*>(a.out) + at, o, n, true);
                         if (a.ggu) {
-                            put4(ggu, og, n, !ANY);
-                            put4(ggu + a.ni, ou, n, !ANY);
-                            if (a.ggu2) put_rest(reinterpret_cast<T*>(a.ggu2) + two, og, ou, a.ni, n, !ANY);
+                            put4(ggu, og, n, true);
+                            put4(ggu + a.ni, ou, n, true);
+                            if (a.ggu2) put_rest(reinterpret_cast<T*>(a.ggu2) + two, og, ou, a.ni, n, true);
                         }
                     }
                 }
@@ -488,18 +468,18 @@ __device__ __forceinline__ void finish_any(const Args& a, const f32x16 (&acc)[FI
     }
 }
 
-template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int WJ, bool ANY>
+template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int WJ>
 __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     constexpr int WAVES = WI * WJ, FI = TI / WI / 32, FJ = TJ / WJ / 32;
     constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
-    constexpr bool STAGED = !ANY && sizeof(T) == 2 && TI >= 128;  // four waves, an array each, or eight, half of one
+    constexpr bool STAGED = sizeof(T) == 2 && TI >= 128;  // four waves, an array each, or eight, half of one
     static_assert(!STAGED || WAVES == 4 || WAVES == 8, "an array a wave");
     static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
     using SA = Side<T, ALIES, TI, WAVES, GATED>;
     using SB = Side<T, BLIES, TJ, WAVES, TWO>;
-    constexpr int BUFFER = SA::BYTES + SB::BYTES, MORE = ANY ? 16 : BUFFER;
+    constexpr int BUFFER = SA::BYTES + SB::BYTES;
     constexpr int FIFTH = TWO && WAVES == 8 ? BUFFER / 8 : 0;  // a wave's fifth plane, where half a buffer holds four
-    __shared__ __attribute__((aligned(16))) unsigned char s0[BUFFER], s1[MORE], s2[MORE], s3[MORE], s4[FIFTH ? WAVES * FIFTH : 16];
+    __shared__ __attribute__((aligned(16))) unsigned char s0[BUFFER], s1[BUFFER], s2[BUFFER], s3[BUFFER], s4[FIFTH ? WAVES * FIFTH : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave % WI, wj = wave / WI;
     int ti, tj, split, local;
@@ -541,86 +521,69 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
         }
         __builtin_amdgcn_sched_barrier(0);  // (all fragments of a stage at once would not fit the registers)
     };
-    if constexpr (ANY) {
-        for (; step < end; ++step) {
-            const int pair = (int)(step / one);
-            const int64_t k0 = (step - pair * one) * SA::KS;
-            __syncthreads();
-            const T* pa = reinterpret_cast<const T*>(a.a[pair]);
-            SA::load_any(pa, pa + a.ni * a.lda, i0, a.ni, a.lda, k0, a.nk, s0);
-            SB::load_any(reinterpret_cast<const T*>(a.b[pair]), reinterpret_cast<const T*>(a.c), j0, a.nj, a.ldb, k0, a.nk,
-                         s0 + SA::BYTES);
-            __syncthreads();
-            read(s0, 0);
-            read(s0, 1);
-            multiply(0);
-            multiply(1);
+    SA sa;
+    SB sb;
+    sa.offsets(i0, a.ni, a.lda, wave, lane);
+    sb.offsets(j0, a.nj, a.ldb, wave, lane);
+    const T *pa, *pb, *pa2 = nullptr, *pb2 = nullptr;  // of the stage to be loaded next
+    int rest;                                          // its k and those after it
+    const int64_t sa_step = ALIES == K_ROWS ? SA::KS : SA::KS * a.lda, sb_step = BLIES == K_ROWS ? SB::KS : SB::KS * a.ldb;
+    const auto advance = [&]() {
+        rest -= SA::KS;
+        pa += sa_step;
+        pb += sb_step;
+        if (GATED) pa2 += sa_step;
+        if (TWO) pb2 += sb_step;
+    };
+    const auto load = [&](unsigned char* to) {
+        const int left = rest < SA::KS ? rest : SA::KS;  // (none past the end: the loads read nothing and write zeros)
+        sa.load(pa, pa2, left, to, wave);
+        sb.load(pb, pb2, left, to + SA::BYTES, wave);
+    };
+    // A stage's last products run while the next one's first fragments are read, after the barrier that says that its loads
+    // are there and that nobody reads this stage's buffer any more, which the loads of the fourth stage from here go to:
+    // loads have three stages' time.
+    constexpr int AHEAD = 2 * (SA::LOADS + SB::LOADS);  // of a wave, of the two stages after the next
+    const auto stage = [&](unsigned char* here, const unsigned char* next) {
+        read(here, 1);
+        multiply(0);
+        advance();
+        stage_barrier<AHEAD>();
+        load(here);
+        read(next, 0);
+        multiply(1);
+    };
+    for (int pair = 0; pair < (GATED ? 1 : a.pairs); ++pair) {
+        // this split's stages of the pair: in fours, what lacks of them with zeros (which costs their products, but a branch
+        // out of the loop's middle would cost a second copy of all sums)
+        const int64_t from = step > pair * one ? step - pair * one : 0, to = end < (pair + 1) * one ? end - pair * one : one;
+        if (from >= to) continue;
+        const int64_t k0 = from * SA::KS, k1 = to * SA::KS < a.nk ? to * SA::KS : a.nk;
+        const int64_t ia = SA::skip(i0, a.lda, k0), ib = SB::skip(j0, a.ldb, k0);
+        pa = reinterpret_cast<const T*>(a.a[pair]) + ia;
+        pb = reinterpret_cast<const T*>(a.b[pair]) + ib;
+        if (GATED) pa2 = pa + a.ni * a.lda;
+        if (TWO) pb2 = reinterpret_cast<const T*>(a.c) + ib;
+        rest = (int)(k1 - k0);
+        const int n = (int)(to - from);
+        if (pair > 0) stage_barrier<0>();  // (the loads past the last pair's end are done with the buffers)
+        load(s0);
+        advance();
+        load(s1);
+        advance();
+        load(s2);
+        stage_barrier<AHEAD>();
+        advance();
+        load(s3);
+        read(s0, 0);
+        for (int s = 0; s < n; s += 4) {
+            stage(s0, s1);
+            stage(s1, s2);
+            stage(s2, s3);
+            stage(s3, s0);
         }
-    } else {
-        SA sa;
-        SB sb;
-        sa.offsets(i0, a.ni, a.lda, wave, lane);
-        sb.offsets(j0, a.nj, a.ldb, wave, lane);
-        const T *pa, *pb, *pa2 = nullptr, *pb2 = nullptr;  // of the stage to be loaded next
-        int rest;                                          // its k and those after it
-        const int64_t sa_step = ALIES == K_ROWS ? SA::KS : SA::KS * a.lda, sb_step = BLIES == K_ROWS ? SB::KS : SB::KS * a.ldb;
-        const auto advance = [&]() {
-            rest -= SA::KS;
-            pa += sa_step;
-            pb += sb_step;
-            if (GATED) pa2 += sa_step;
-            if (TWO) pb2 += sb_step;
-        };
-        const auto load = [&](unsigned char* to) {
-            const int left = rest < SA::KS ? rest : SA::KS;  // (none past the end: the loads read nothing and write zeros)
-            sa.load(pa, pa2, left, to, wave);
-            sb.load(pb, pb2, left, to + SA::BYTES, wave);
-        };
-        // A stage's last products run while the next one's first fragments are read, after the barrier that says that its loads
-        // are there and that nobody reads this stage's buffer any more, which the loads of the fourth stage from here go to:
-        // loads have three stages' time.
-        constexpr int AHEAD = 2 * (SA::LOADS + SB::LOADS);  // of a wave, of the two stages after the next
-        const auto stage = [&](unsigned char* here, const unsigned char* next) {
-            read(here, 1);
-            multiply(0);
-            advance();
-            stage_barrier<AHEAD>();
-            load(here);
-            read(next, 0);
-            multiply(1);
-        };
-        for (int pair = 0; pair < (GATED ? 1 : a.pairs); ++pair) {
-            // this split's stages of the pair: in fours, what lacks of them with zeros (which costs their products, but a branch
-            // out of the loop's middle would cost a second copy of all sums)
-            const int64_t from = step > pair * one ? step - pair * one : 0, to = end < (pair + 1) * one ? end - pair * one : one;
-            if (from >= to) continue;
-            const int64_t k0 = from * SA::KS, k1 = to * SA::KS < a.nk ? to * SA::KS : a.nk;
-            const int64_t ia = SA::skip(i0, a.lda, k0), ib = SB::skip(j0, a.ldb, k0);
-            pa = reinterpret_cast<const T*>(a.a[pair]) + ia;
-            pb = reinterpret_cast<const T*>(a.b[pair]) + ib;
-            if (GATED) pa2 = pa + a.ni * a.lda;
-            if (TWO) pb2 = reinterpret_cast<const T*>(a.c) + ib;
-            rest = (int)(k1 - k0);
-            const int n = (int)(to - from);
-            if (pair > 0) stage_barrier<0>();  // (the loads past the last pair's end are done with the buffers)
-            load(s0);
-            advance();
-            load(s1);
-            advance();
-            load(s2);
-            stage_barrier<AHEAD>();
-            advance();
-            load(s3);
-            read(s0, 0);
-            for (int s = 0; s < n; s += 4) {
-                stage(s0, s1);
-                stage(s1, s2);
-                stage(s2, s3);
-                stage(s3, s0);
-            }
-        }
-        stage_barrier<0>();  // (the loads past the end, of zeros, are done with the buffers)
     }
+    stage_barrier<0>();  // (the loads past the end, of zeros, are done with the buffers)
 
     // the sums of a split: tile by tile
     float* const part = EP == EP_PART ? reinterpret_cast<float*>(a.out) + ((int64_t)split * a.count + local) * (TI * TJ) : nullptr;
@@ -633,7 +596,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
         finish<T, EP, FI, FJ>(a, acc, i0 + wi * FI * 32, j0 + wj * FJ * 32, EP == EP_PART ? part + wj * FJ * 32 * TI + wi * FI * 32 : part,
                               TI, own, FIFTH ? s4 + wave * FIFTH : own + FOUR, lane);
     } else {
-        finish_any<T, EP, FI, FJ, ANY>(a, acc, i0, j0, wi, wj, part, TI, lane);
+        finish_few<T, EP, FI, FJ>(a, acc, i0, j0, wi, wj, part, TI, lane);
     }
 }
 
@@ -670,6 +633,19 @@ template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void 
     __shared__ f32x4 sums[FEW_WAVES][2][FJ][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, part = lane >> 4;
+    // 16 bytes of a row from k on, or what it has of them; at the row's end the bytes before, taken out
+    const auto chunk = [&](const T* p, int64_t k) {
+        const int64_t at = k < a.nk - EPC ? k : a.nk - EPC, cut = (k - at) * 8 * (int)sizeof(T);
+        u32x4 v;
+        __builtin_memcpy(&v, p + at, 16);
+        if (cut > 0)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int64_t n = cut - 32 * w;
+                v[w] = n <= 0 ? v[w] : n < 32 ? v[w] & (~0u << n) : 0;
+            }
+        return v;
+    };
     const int64_t i0 = (int64_t)blockIdx.x * 16, row = i0 + l16 < a.ni ? i0 + l16 : a.ni - 1;  // (the last one again past the end)
     const T* const gate = reinterpret_cast<const T*>(a.a[0]) + row * a.lda;
     const T* const up = gate + a.ni * a.lda;
@@ -683,11 +659,10 @@ template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void 
             for (int h = 0; h < 2; ++h) {
                 const int64_t k = k0 + t * FEW_WAVES * TURN + (part * 2 + h) * EPC;
                 const bool in = k < a.nk;
-                g[t][h] = in ? *reinterpret_cast<const u32x4*>(gate + k) : u32x4{};
-                u[t][h] = in ? *reinterpret_cast<const u32x4*>(up + k) : u32x4{};
+                g[t][h] = in ? chunk(gate, k) : u32x4{};
+                u[t][h] = in ? chunk(up, k) : u32x4{};
 #pragma unroll
-                for (int j = 0; j < FJ; ++j)
-                    b[t][h][j] = in && j * 16 + l16 < a.nj ? *reinterpret_cast<const u32x4*>(x + (j * 16 + l16) * a.ldb + k) : u32x4{};
+                for (int j = 0; j < FJ; ++j) b[t][h][j] = in && j * 16 + l16 < a.nj ? chunk(x + (j * 16 + l16) * a.ldb, k) : u32x4{};
             }
 #pragma unroll
         for (int t = 0; t < AT_ONCE; ++t)
@@ -714,7 +689,7 @@ template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void 
     const int64_t n = wave * 16 + l16, i = i0 + 4 * part;
     if (n >= a.nj || i >= a.ni) return;
     const float v[4] = {gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3])};
-    put4(reinterpret_cast<T*>(a.out) + n * a.ni + i, v, 4, true);
+    put4(reinterpret_cast<T*>(a.out) + n * a.ni + i, v, a.ni - i, a.ni % 4 == 0);
 }
 
 // fp64, for gradient checks: 64 x 64 of D (gated: of each half, and of both right operands) a workgroup, 4 x 4 a thread.
@@ -780,7 +755,7 @@ template <int ALIES, int BLIES, int EP> __global__ __launch_bounds__(256) void k
 }
 
 // The splits' partial sums of the tiles from tile0 on added up, in their order.
-template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int tile, const float* part, T* out, bool wide) {
+template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int tile, const float* part, T* out) {
     const int per = tile * tile / 1024;  // workgroups of a tile
     int ti, tj;
     place_of(a, a.tile0 + blockIdx.x / per, ti, tj);
@@ -794,7 +769,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int 
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[e] += v[e];
     }
-    put4(out + row * a.ldo + col, s, a.ni - col, wide);
+    put4(out + row * a.ldo + col, s, a.ni - col, true);
 }
 
 // -- launches ----------------------------------------------------------------------------------------------------------
@@ -804,7 +779,7 @@ static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d
 
 static int check(int dtype, int64_t N, int64_t C, int64_t I) {
     if (!known(dtype)) return EBR_ERR_DTYPE;
-    if (N < 1 || C < 1 || I < 1 || N >= ((int64_t)1 << 31) || C >= (1 << 20) || I >= (1 << 20)) return EBR_ERR_SHAPE;
+    if (N < 1 || C < 1 || I < 1 || N >= ((int64_t)1 << 31) || C > (1 << 20) - 8 || I > (1 << 19) - 8) return EBR_ERR_SHAPE;
     const auto tiles = [](int64_t n) { return (n + 63) / 64; };  // (a launch holds fewer than 2^32 threads)
     const int64_t most = tiles(2 * I) > tiles(C) ? tiles(2 * I) : tiles(C);
     return tiles(2 * N) * most > MAX_BLOCKS || tiles(2 * I) * tiles(C) > MAX_BLOCKS ? EBR_ERR_SHAPE : EBR_OK;
@@ -818,12 +793,12 @@ struct Cut {
     int64_t steps, whole;
     int64_t tiles() const { return ti * tj; }
     int64_t part_bytes() const { return splits > 1 ? splits * (tiles() - whole) * tile * tile * 4 : 0; }
-    Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, bool split, bool any) {  // gated: 0, 1, or 2 for TWO
+    Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, bool split) {  // gated: 0, 1, or 2 for TWO
         const auto up = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
         const int64_t wide = gated ? 2 * ni : ni, high = gated == 2 ? 2 * nj : nj, all = up(nk, STAGE / size_of(dtype)) * pairs;
         tile = 256;
         if (dtype == EBR_DTYPE_F64) tile = 64;
-        else if (dtype == EBR_DTYPE_F32 || any) tile = 128;
+        else if (dtype == EBR_DTYPE_F32) tile = 128;
         const auto tiles = [&](int t) { return up(wide, t) * up(high, t); };
         if (dtype != EBR_DTYPE_F64) {
             if (tile == 256 && tiles(256) < (split ? 4 : 200)) tile = 128;
@@ -848,52 +823,41 @@ struct Cut {
     }
 };
 
-template <typename T, int ALIES, int BLIES, int EP, bool ANY> static void launch(hipStream_t s, const Cut& c, const Args& a) {
+template <typename T, int ALIES, int BLIES, int EP> static void launch(hipStream_t s, const Cut& c, const Args& a) {
     const dim3 grid((unsigned)(a.count * a.splits));
     if constexpr (std::is_same_v<T, double>) {
         hipLaunchKernelGGL((k_product64<ALIES, BLIES, EP>), grid, dim3(256), 0, s, a);
     } else {
-        if constexpr (!ANY && sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2) {
             if (c.tile == 256) {
                 constexpr int WJ = EP >= EP_FWD ? 4 : 2;
-                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 2, WJ, ANY>), grid, dim3(128 * WJ), 0, s, a);
+                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 2, WJ>), grid, dim3(128 * WJ), 0, s, a);
                 return;
             }
         }
-        if (c.tile == 128) hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 128, 128, 2, 2, ANY>), grid, dim3(256), 0, s, a);
+        if (c.tile == 128) hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 128, 128, 2, 2>), grid, dim3(256), 0, s, a);
         else if constexpr (EP == EP_BWD2)
-            hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 1, ANY>), grid, dim3(64), 0, s, a);
-        else hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 2, ANY>), grid, dim3(128), 0, s, a);
+            hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 1>), grid, dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 2>), grid, dim3(128), 0, s, a);
     }
 }
 
 // One product, whose operands, strides, sizes and outputs ``a`` holds.
-template <int ALIES, int BLIES, int EP> static void product(int dtype, bool any, const Cut& c, Args& a, hipStream_t s) {
+template <int ALIES, int BLIES, int EP> static void product(int dtype, const Cut& c, Args& a, hipStream_t s) {
     constexpr bool PART = EP == EP_PART;  // its tiles that are split, else those that are not
     a.ti = (int)c.ti, a.tj = (int)c.tj, a.tile0 = PART ? (int)c.whole : 0, a.count = (int)(PART ? c.tiles() - c.whole : c.whole);
     a.splits = PART ? c.splits : 1;
     a.steps = PART ? c.steps : INT64_MAX / 4;
     const auto with = [&](auto v) {
         using T = decltype(v);
-        if (any) launch<T, ALIES, BLIES, EP, true>(s, c, a);
-        else launch<T, ALIES, BLIES, EP, false>(s, c, a);
+        launch<T, ALIES, BLIES, EP>(s, c, a);
     };
     switch (dtype) {
         case EBR_DTYPE_F32: with(float()); break;
         case EBR_DTYPE_BF16: with(__bf16()); break;
         case EBR_DTYPE_F16: with(_Float16()); break;
-        default: launch<double, ALIES, BLIES, EP, true>(s, c, a); break;
+        default: with(double()); break;
     }
-}
-
-// Whether tensors of these widths (elements of a row) go by the whole 16-byte chunk.
-static bool whole(int dtype, std::initializer_list<int64_t> widths, std::initializer_list<const void*> ps) {
-    const int per = 16 / size_of(dtype);
-    for (const int64_t w : widths)
-        if (w % per || w >= (1 << 20)) return false;
-    for (const void* p : ps)
-        if (!aligned(p, 16)) return false;
-    return true;
 }
 
 // [dg|du] or [gg|gu], rounded, and what they lack where the products take that as well: of few rows a weight's gradient adds up
@@ -905,38 +869,31 @@ static bool with_rest(int dtype, int64_t N) { return size_of(dtype) == 2 && N <=
 
 // dx of dgu, and dw of (x, dgu) and, where there is one, a second pair.
 static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w, Grads dgu, void* dx, hipStream_t s) {
-    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, 2 * I}, {w, dgu.g, dgu.rest, dx});
     Args a = {};
     a.a[0] = a.a[1] = w, a.b[0] = dgu.g, a.b[1] = dgu.rest, a.pairs = dgu.rest ? 2 : 1;
     a.lda = C, a.ldb = 2 * I, a.ni = C, a.nj = N, a.nk = 2 * I, a.out = dx, a.ldo = C;
-    product<M_ROWS, K_ROWS, EP_OUT>(dtype, any, Cut(dtype, C, N, 2 * I, a.pairs, 0, false, any), a, s);
+    product<M_ROWS, K_ROWS, EP_OUT>(dtype, Cut(dtype, C, N, 2 * I, a.pairs, 0, false), a, s);
 }
 
-static Cut weight_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs, bool any) {
-    return Cut(dtype, C, 2 * I, N, pairs, 0, true, any);
+static Cut weight_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) {
+    return Cut(dtype, C, 2 * I, N, pairs, 0, true);
 }
 static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* x, Grads dgu, const void* x2, Grads dgu2, void* dw,
                         float* part, hipStream_t s) {
     Args a = {};
-    bool fit = true;
     for (const auto& [of, grads] : {std::pair<const void*, Grads>(x, dgu), std::pair<const void*, Grads>(x2, dgu2)})
         for (const void* g : {grads.g, grads.rest})
-            if (g) {
-                fit = fit && whole(dtype, {}, {of, g});
-                a.a[a.pairs] = of, a.b[a.pairs++] = g;
-            }
-    const bool any = dtype == EBR_DTYPE_F64 || !fit || !whole(dtype, {C, 2 * I}, {dw});
-    const Cut c = weight_cut(dtype, N, C, I, a.pairs, any);
+            if (g) a.a[a.pairs] = of, a.b[a.pairs++] = g;
+    const Cut c = weight_cut(dtype, N, C, I, a.pairs);
     a.lda = C, a.ldb = 2 * I, a.ni = C, a.nj = 2 * I, a.nk = N, a.out = dw, a.ldo = C;
-    if (c.whole) product<M_ROWS, M_ROWS, EP_OUT>(dtype, any, c, a, s);
+    if (c.whole) product<M_ROWS, M_ROWS, EP_OUT>(dtype, c, a, s);
     if (c.splits == 1) return;
     a.out = part;
-    product<M_ROWS, M_ROWS, EP_PART>(dtype, any, c, a, s);
+    product<M_ROWS, M_ROWS, EP_PART>(dtype, c, a, s);
     const dim3 grid((unsigned)(a.count * (c.tile * c.tile / 1024)));
-    const bool wide = C % 4 == 0 && aligned(dw, 16);
-    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, a, c.tile, part, (__bf16*)dw, wide);
-    else if (dtype == EBR_DTYPE_F16) hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, a, c.tile, part, (_Float16*)dw, wide);
-    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, a, c.tile, part, (float*)dw, wide);
+    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, a, c.tile, part, (__bf16*)dw);
+    else if (dtype == EBR_DTYPE_F16) hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, a, c.tile, part, (_Float16*)dw);
+    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, a, c.tile, part, (float*)dw);
 }
 
 template <typename T> static void few(hipStream_t s, const Args& a) {
@@ -947,6 +904,160 @@ template <typename T> static void few(hipStream_t s, const Args& a) {
 
 static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
+// Widths that are no whole 16-byte chunks: the products run on copies with zeros up to the next chunk, which add nothing, and
+// their outputs are copied back. (Reading such rows element by element took ten times as long: 8192 x 2048 -> 5631 bf16 with its
+// gradients 15.8 ms, 1.7 so, 1.3 with 5632.)
+struct Move {
+    const void* from;
+    void* to;
+    int64_t rows, have_rows, ldf, ldt;
+    int cols, have;  // written, and there to be read: zeros beyond
+};
+struct Moves {
+    Move m[5];
+    int first[6], count;
+};
+template <typename T> __global__ __launch_bounds__(256) void k_move(Moves a) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    int j = 0;
+    while (j + 1 < a.count && (int)blockIdx.x >= a.first[j + 1]) ++j;
+    const Move m = a.m[j];
+    const int64_t skip = (int64_t)(a.first[j + 1] - a.first[j]) * 4;
+    for (int64_t row = (int64_t)(blockIdx.x - a.first[j]) * 4 + threadIdx.x / 64; row < m.rows; row += skip) {
+        const T* from = reinterpret_cast<const T*>(m.from) + row * m.ldf;
+        T* to = reinterpret_cast<T*>(m.to) + row * m.ldt;
+        for (int c = threadIdx.x % 64 * VEC; c < m.cols; c += 64 * VEC) {
+            T v[VEC] = {};
+            if (row < m.have_rows) {
+                if (c + VEC <= m.have) __builtin_memcpy(v, from + c, 16);
+                else
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (c + e < m.have) v[e] = from[c + e];
+            }
+            if (c + VEC <= m.cols) __builtin_memcpy(to + c, v, 16);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (c + e < m.cols) to[c + e] = v[e];
+        }
+    }
+}
+
+struct Padded {
+    int dtype;
+    int64_t N, C, I, Cp, Ip;
+    char* at = nullptr;
+    Moves in = {}, out = {};
+    Padded(int dtype, int64_t N, int64_t C, int64_t I) : dtype(dtype), N(N), C(C), I(I) {
+        const int64_t per = dtype == EBR_DTYPE_F64 ? 1 : 16 / size_of(dtype);
+        Cp = (C + per - 1) / per * per, Ip = (I + per - 1) / per * per;
+    }
+    bool needed() const { return Cp != C || Ip != I; }
+    int64_t bytes(int64_t rows, int64_t cols) const { return up16(rows * cols * size_of(dtype)); }
+    // of x, w and y; of x, w, dy, dx and dw; of x, w, dy, c, gx, gdy and gw
+    int64_t all(int order) const {
+        if (!needed()) return 0;
+        return (order == 0 ? 1 : order + 1) * bytes(N, Cp) + (order < 2 ? 1 : 2) * bytes(N, Ip) + (order == 0 ? 1 : 2) * bytes(2 * Ip, Cp);
+    }
+    void add(Moves& to, const Move& m) {
+        to.m[to.count] = m;
+        const int64_t want = (m.rows + 3) / 4;
+        to.first[to.count + 1] = to.first[to.count] + (int)(want < 4096 ? want : 4096);
+        ++to.count;
+    }
+    char* take(int64_t rows, int64_t cols) {
+        char* p = at;
+        at += bytes(rows, cols);
+        return p;
+    }
+    const void* rows(const void* p, int64_t have, int64_t cols) {
+        char* to = take(N, cols);
+        add(in, {p, to, N, N, have, cols, (int)cols, (int)have});
+        return to;
+    }
+    const void* weight(const void* w) {
+        char* to = take(2 * Ip, Cp);
+        for (int h = 0; h < 2; ++h)
+            add(in, {(const char*)w + h * I * C * size_of(dtype), to + h * Ip * Cp * size_of(dtype), Ip, I, C, Cp, (int)Cp, (int)C});
+        return to;
+    }
+    void* rows_out(void* p, int64_t have, int64_t cols) {
+        if (!p) return nullptr;
+        char* from = take(N, cols);
+        add(out, {from, p, N, N, cols, have, (int)have, (int)have});
+        return from;
+    }
+    void* weight_out(void* w) {
+        if (!w) return nullptr;
+        char* from = take(2 * Ip, Cp);
+        for (int h = 0; h < 2; ++h)
+            add(out, {from + h * Ip * Cp * size_of(dtype), (char*)w + h * I * C * size_of(dtype), I, I, Cp, C, (int)C, (int)C});
+        return from;
+    }
+    void run(const Moves& m, hipStream_t s) const {
+        const dim3 grid((unsigned)m.first[m.count]);
+        if (m.count == 0) return;
+        if (size_of(dtype) == 2) hipLaunchKernelGGL((k_move<uint16_t>), grid, dim3(256), 0, s, m);
+        else hipLaunchKernelGGL((k_move<uint32_t>), grid, dim3(256), 0, s, m);
+    }
+};
+
+static bool all_aligned(std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if (!aligned(p, 16)) return false;
+    return true;
+}
+
+static void forward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, hipStream_t s) {
+    Args a = {};
+    a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = y;
+    if (dtype != EBR_DTYPE_F64 && N <= FEW && C * size_of(dtype) >= 16) {
+        if (dtype == EBR_DTYPE_F32) few<float>(s, a);
+        else if (dtype == EBR_DTYPE_BF16) few<__bf16>(s, a);
+        else few<_Float16>(s, a);
+        return;
+    }
+    product<K_ROWS, K_ROWS, EP_FWD>(dtype, Cut(dtype, I, N, C, 1, 1, false), a, s);
+}
+// Whether it takes rows of any width and alignment as they are.
+static bool as_they_are(int dtype, int64_t N, int64_t C) { return dtype == EBR_DTYPE_F64 || (N <= FEW && C * size_of(dtype) >= 16); }
+
+static int64_t own_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I) {
+    if (order == 0) return 0;
+    const int64_t each = with_rest(dtype, N) ? 2 : 1;
+    // [dg|du], for order 2 [gg|gu] too, and the weight gradient's partial sums
+    return order * each * up16(N * 2 * I * size_of(dtype)) + weight_cut(dtype, N, C, I, (int)(order * each)).part_bytes() + 16;
+}
+
+static void backward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy, void* dx, void* dw,
+                     char* at, hipStream_t s) {
+    Args a = {};
+    a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.dy = dy;
+    const int64_t rows = up16(N * 2 * I * size_of(dtype));
+    a.dgu = at, at += rows;
+    if (with_rest(dtype, N)) a.dgu2 = at, at += rows;
+    product<K_ROWS, K_ROWS, EP_BWD>(dtype, Cut(dtype, I, N, C, 1, 1, false), a, s);
+    const Grads dgu = {a.dgu, a.dgu2};
+    if (dx) input_grad(dtype, N, C, I, w, dgu, dx, s);
+    if (dw) weight_grad(dtype, N, C, I, x, dgu, nullptr, {}, dw, reinterpret_cast<float*>(at), s);
+}
+
+static void backward2(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy, const void* c,
+                      void* gx, void* gdy, void* gw, char* at, hipStream_t s) {
+    Args a = {};
+    a.a[0] = w, a.b[0] = x, a.c = c, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = gdy, a.dy = dy;
+    const int64_t rows = up16(N * 2 * I * size_of(dtype));
+    for (void** to : {gx || gw ? &a.ggu : nullptr, gw ? &a.dgu : nullptr}) {
+        if (to) *to = at, at += rows;
+        if (to && with_rest(dtype, N)) *(to == &a.ggu ? &a.ggu2 : &a.dgu2) = at, at += rows;
+    }
+    product<K_ROWS, K_ROWS, EP_BWD2>(dtype, Cut(dtype, I, N, C, 1, 2, false), a, s);
+    const Grads dgu = {a.dgu, a.dgu2}, ggu = {a.ggu, a.ggu2};
+    if (gx) input_grad(dtype, N, C, I, w, ggu, gx, s);
+    if (gw) weight_grad(dtype, N, C, I, x, ggu, c, dgu, gw, reinterpret_cast<float*>(at), s);
+}
+
 }  // namespace ebr_glu
 
 using namespace ebr_glu;
@@ -955,30 +1066,32 @@ extern "C" {
 
 int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I) {
     if (check(dtype, N, C, I) || order < 0 || order > 2) return -1;
-    if (order == 0) return 16;
-    int64_t part = 0;
-    const int64_t each = with_rest(dtype, N) ? 2 : 1;
-    for (const bool any : {false, true}) {
-        part = std::max(part, weight_cut(dtype, N, C, I, (int)(order * each), any).part_bytes());
-    }
-    // [dg|du], for order 2 [gg|gu] too, and the weight gradient's partial sums
-    return order * each * up16(N * 2 * I * size_of(dtype)) + part + 16;
+    if (order == 0 && as_they_are(dtype, N, C)) return 0;
+    const Padded p(dtype, N, C, I);
+    return own_scratch(dtype, order, N, p.Cp, p.Ip) + p.all(order);
 }
 
-int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* stream) {
+int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* scratch,
+                            void* stream) {
     const int rc = check(dtype, N, C, I);
     if (rc) return rc;
     if (!x || !w || !y) return EBR_ERR_NULL;
-    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, y});
-    Args a = {};
-    a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = y;
-    if (!any && N <= FEW) {
-        if (dtype == EBR_DTYPE_F32) few<float>((hipStream_t)stream, a);
-        else if (dtype == EBR_DTYPE_BF16) few<__bf16>((hipStream_t)stream, a);
-        else few<_Float16>((hipStream_t)stream, a);
-        return launched();
+    hipStream_t s = (hipStream_t)stream;
+    Padded p(dtype, N, C, I);
+    if (as_they_are(dtype, N, C)) {
+        forward(dtype, N, C, I, x, w, y, s);
+    } else if (p.needed()) {
+        if (!scratch) return EBR_ERR_SCRATCH;
+        if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+        p.at = reinterpret_cast<char*>(scratch);
+        x = p.rows(x, C, p.Cp), w = p.weight(w), y = p.rows_out(y, I, p.Ip);
+        p.run(p.in, s);
+        forward(dtype, N, p.Cp, p.Ip, x, w, y, s);
+        p.run(p.out, s);
+    } else {
+        if (!all_aligned({x, w, y})) return EBR_ERR_ALIGN;
+        forward(dtype, N, C, I, x, w, y, s);
     }
-    product<K_ROWS, K_ROWS, EP_FWD>(dtype, any, Cut(dtype, I, N, C, 1, 1, false, any), a, (hipStream_t)stream);
     return launched();
 }
 
@@ -988,20 +1101,19 @@ int ebr_block_swiglu_linear_bwd(int dtype, int64_t N, int64_t C, int64_t I, cons
     if (rc) return rc;
     if (!x || !w || !dy) return EBR_ERR_NULL;
     if (!scratch) return EBR_ERR_SCRATCH;
-    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    Padded p(dtype, N, C, I);
+    if (!aligned(scratch, 16) || (!p.needed() && dtype != EBR_DTYPE_F64 && !all_aligned({x, w, dy, dx, dw}))) return EBR_ERR_ALIGN;
     if (!dx && !dw) return EBR_OK;
     hipStream_t s = (hipStream_t)stream;
-    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, dy});
-    Args a = {};
-    a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.dy = dy;
-    const int64_t rows = up16(N * 2 * I * size_of(dtype));
-    char* at = reinterpret_cast<char*>(scratch);
-    a.dgu = at, at += rows;
-    if (with_rest(dtype, N)) a.dgu2 = at, at += rows;
-    product<K_ROWS, K_ROWS, EP_BWD>(dtype, any, Cut(dtype, I, N, C, 1, 1, false, any), a, s);
-    const Grads dgu = {a.dgu, a.dgu2};
-    if (dx) input_grad(dtype, N, C, I, w, dgu, dx, s);
-    if (dw) weight_grad(dtype, N, C, I, x, dgu, nullptr, {}, dw, reinterpret_cast<float*>(at), s);
+    char* const own = reinterpret_cast<char*>(scratch) + p.all(1);
+    if (p.needed()) {
+        p.at = reinterpret_cast<char*>(scratch);
+        x = p.rows(x, C, p.Cp), w = p.weight(w), dy = p.rows(dy, I, p.Ip);
+        dx = p.rows_out(dx, C, p.Cp), dw = p.weight_out(dw);
+    }
+    p.run(p.in, s);
+    backward(dtype, N, p.Cp, p.Ip, x, w, dy, dx, dw, own, s);
+    p.run(p.out, s);
     return launched();
 }
 
@@ -1011,21 +1123,19 @@ int ebr_block_swiglu_linear_bwd2(int dtype, int64_t N, int64_t C, int64_t I, con
     if (rc) return rc;
     if (!x || !w || !dy || !c || !gdy) return EBR_ERR_NULL;
     if (!scratch) return EBR_ERR_SCRATCH;
-    if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    Padded p(dtype, N, C, I);
+    if (!aligned(scratch, 16) || (!p.needed() && dtype != EBR_DTYPE_F64 && !all_aligned({x, w, dy, c, gx, gdy, gw})))
+        return EBR_ERR_ALIGN;
     hipStream_t s = (hipStream_t)stream;
-    const bool any = dtype == EBR_DTYPE_F64 || !whole(dtype, {C, I}, {x, w, dy, c, gdy});
-    Args a = {};
-    a.a[0] = w, a.b[0] = x, a.c = c, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = gdy, a.dy = dy;
-    const int64_t rows = up16(N * 2 * I * size_of(dtype));
-    char* at = reinterpret_cast<char*>(scratch);
-    for (void** to : {gx || gw ? &a.ggu : nullptr, gw ? &a.dgu : nullptr}) {
-        if (to) *to = at, at += rows;
-        if (to && with_rest(dtype, N)) *(to == &a.ggu ? &a.ggu2 : &a.dgu2) = at, at += rows;
+    char* const own = reinterpret_cast<char*>(scratch) + p.all(2);
+    if (p.needed()) {
+        p.at = reinterpret_cast<char*>(scratch);
+        x = p.rows(x, C, p.Cp), w = p.weight(w), dy = p.rows(dy, I, p.Ip), c = p.rows(c, C, p.Cp);
+        gx = p.rows_out(gx, C, p.Cp), gdy = p.rows_out(gdy, I, p.Ip), gw = p.weight_out(gw);
     }
-    product<K_ROWS, K_ROWS, EP_BWD2>(dtype, any, Cut(dtype, I, N, C, 1, 2, false, any), a, s);
-    const Grads dgu = {a.dgu, a.dgu2}, ggu = {a.ggu, a.ggu2};
-    if (gx) input_grad(dtype, N, C, I, w, ggu, gx, s);
-    if (gw) weight_grad(dtype, N, C, I, x, ggu, c, dgu, gw, reinterpret_cast<float*>(at), s);
+    p.run(p.in, s);
+    backward2(dtype, N, p.Cp, p.Ip, x, w, dy, c, gx, gdy, gw, own, s);
+    p.run(p.out, s);
     return launched();
 }
 

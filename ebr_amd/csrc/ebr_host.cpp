@@ -1438,19 +1438,26 @@ struct ProjectionShape {
     Tensor scratch(const Tensor& x, int order) const {
         const int64_t n = ebr_block_swiglu_linear_scratch(code, order, N, C, I);
         TORCH_CHECK_VALUE(n >= 0, "ebr_block_swiglu_linear: sizes out of range");
+        if (n == 0) return Tensor();
         return at::empty({n}, x.options().dtype(at::kByte));
     }
 };
 
+// t contiguous and 16-byte aligned.
+Tensor whole(const Tensor& t) {
+    const Tensor d = dense(t);
+    return reinterpret_cast<uintptr_t>(d.data_ptr()) % 16 == 0 ? d : d.clone();
+}
+
 Tensor projected(const Tensor& x_, const Tensor& w_) {
     RECORD_FUNCTION("ebr_fused::block_swiglu_linear", std::vector<c10::IValue>());
     const c10::DeviceGuard on(x_.device());
-    const Tensor x = dense(x_), w = dense(w_);
+    const Tensor x = whole(x_), w = whole(w_);
     const ProjectionShape n(x, w);
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = n.I;
-    const Tensor y = at::empty(shape, x.options());
-    check(ebr_block_swiglu_linear(n.code, n.N, n.C, n.I, x.data_ptr(), w.data_ptr(), y.data_ptr(), stream_of(x)),
+    const Tensor y = at::empty(shape, x.options()), s = n.scratch(x, 0);
+    check(ebr_block_swiglu_linear(n.code, n.N, n.C, n.I, x.data_ptr(), w.data_ptr(), y.data_ptr(), vptr(s), stream_of(x)),
           "ebr_block_swiglu_linear");
     return y;
 }
@@ -1458,7 +1465,7 @@ Tensor projected(const Tensor& x_, const Tensor& w_) {
 variable_list projected_bwd(const Tensor& x_, const Tensor& w_, const Tensor& dy_, bool want_x, bool want_w) {
     RECORD_FUNCTION("ebr_fused::block_swiglu_linear_bwd", std::vector<c10::IValue>());
     const c10::DeviceGuard on(x_.device());
-    const Tensor x = dense(x_), w = dense(w_), dy = dense(dy_.to(x_.scalar_type()));
+    const Tensor x = whole(x_), w = whole(w_), dy = whole(dy_.to(x_.scalar_type()));
     const ProjectionShape n(x, w);
     const Tensor dx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
     const Tensor dw = want_w ? at::empty(w.sizes(), w.options()) : Tensor(), s = n.scratch(x, 1);
@@ -1483,7 +1490,7 @@ struct SwiGLULinearDx : Function<SwiGLULinearDx> {
         RECORD_FUNCTION("ebr_fused::block_swiglu_linear_bwd2", std::vector<c10::IValue>());
         const c10::DeviceGuard on(sv[0].device());
         const auto st = sv[0].scalar_type();
-        const Tensor x = dense(sv[0]), w = dense(sv[1]), dy = dense(sv[2].to(st)), c = dense(g[0].to(st));
+        const Tensor x = whole(sv[0]), w = whole(sv[1]), dy = whole(sv[2].to(st)), c = whole(g[0].to(st));
         const ProjectionShape n(x, w);
         const Tensor gx = want_x ? at::empty(x.sizes(), x.options()) : Tensor();
         const Tensor gw = want_w ? at::empty(w.sizes(), w.options()) : Tensor();

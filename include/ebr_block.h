@@ -139,8 +139,11 @@ int ebr_block_layernorm_bwd2(int dtype, int wdtype, int64_t rows, int C, const v
 int64_t ebr_block_layernorm_scratch(int dtype, int order, int64_t rows, int C);
 
 /* y = silu(g) u for x [N, C] and w [2 I, C], gate rows first: g = x w[:I]^T, u = x w[I:]^T, summed in fp32 (fp64 for fp64) and
- * not rounded before y [N, I]; N below 2^31, C and I below 2^20. */
-int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* stream);
+ * not rounded before y [N, I]; N below 2^31, C up to 2^20 - 8, I up to 2^19 - 8. Tensors (here and below) of any alignment where
+ * C or I is no multiple of 16 bytes, or N at most 32 (y alone), else 16-byte aligned. Scratch of order 0, which may be 0 bytes
+ * (and NULL). */
+int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* scratch,
+                            void* stream);
 
 /* dx [N, C] and dw [2 I, C] (NULL where not wanted) of y given dy [N, I]: g and u are taken again, [dg | du] is their gradient
  * as of ebr_block_swiglu_bwd, rounded, dx = [dg | du] w and dw = [dg | du]^T x. Scratch of order 1, 16-byte aligned. */
@@ -153,8 +156,7 @@ int ebr_block_swiglu_linear_bwd(int dtype, int64_t N, int64_t C, int64_t I, cons
 int ebr_block_swiglu_linear_bwd2(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
                                  const void* c, void* gx, void* gdy, void* gw, void* scratch, void* stream);
 
-/* Bytes of scratch of the gated projection's derivatives (order 1, 2), for tensors of any alignment; -1 for sizes or types that
- * they refuse. */
+/* Bytes of scratch of the gated projection (order 0) and its derivatives (1, 2); -1 for sizes or types that they refuse. */
 int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I);
 
 #ifdef __cplusplus

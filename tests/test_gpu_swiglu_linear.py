@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from ebr_amd import block, linear
+from ebr_amd.fused_attn.loader import hip_library
 
 pytestmark = pytest.mark.gpu
 
@@ -127,9 +128,10 @@ def test_sizes(cuda, N, C, I, dtype):
     _check(*_inputs(cuda, N, C, I, dtype, seed=N).values())
 
 
-# up to 32 rows, whose forward reads the weight by itself: rows off 16, a last turn that is not full, many turns, widths off 16
+# up to 32 rows, whose forward reads the weight by itself: rows off 16, a last turn that is not full, many turns, widths off
+# 16 and off the vectors
 @pytest.mark.parametrize("N", [1, 3, 15, 16, 17, 31, 32])
-@pytest.mark.parametrize("C,I", [(8, 8), (72, 24), (520, 16), (2056, 40), (5000, 1000)])
+@pytest.mark.parametrize("C,I", [(8, 8), (72, 24), (520, 16), (2056, 40), (5000, 1000), (9, 33), (1031, 15), (2047, 1)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_few_rows(cuda, N, C, I, dtype):
     _say(f"swiglu_linear few rows {N} {C} {I} {dtype}")
@@ -160,6 +162,30 @@ def test_more_tiles_than_a_round(cuda):
     a = _check(*_inputs(cuda, 4100, 4096, 2184, torch.bfloat16, seed=6).values())
     b = _run(*_inputs(cuda, 4100, 4096, 2184, torch.bfloat16, seed=6).values())
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("N,C,I", [(40, 1, 1), (33, 9, 8), (700, 1031, 8), (3000, 264, 521), (5000, 263, 1025)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_widths_off_the_vectors(cuda, N, C, I, dtype):
+    """Copies with zeros up to whole chunks, of either width and of both; nothing of them is left in the outputs."""
+    _say(f"swiglu_linear off the vectors {N} {C} {I} {dtype}")
+    ts = _inputs(cuda, N, C, I, dtype, seed=I)
+    a = _check(**ts)
+    off = {n: torch.empty(t.numel() + 1, device=cuda, dtype=dtype)[1:].view(t.shape).copy_(t) for n, t in ts.items()}
+    assert all(torch.equal(x, y) for x, y in zip(a, _run(**off)))
+
+
+def test_refused_alignment(cuda):
+    """Tensors off 16 bytes where the widths are whole, and a scratch that is missing, at the C entry."""
+    lib = hip_library()
+    x, w, y = (torch.zeros(n + 8, device=cuda, dtype=torch.bfloat16) for n in (40 * 16, 48 * 16, 40 * 24))
+    p = [t.data_ptr() for t in (x, w, y)]
+    call = lambda *a: lib.ebr_block_swiglu_linear(1, 40, 16, 24, *a, 0, torch.cuda.current_stream().cuda_stream)  # noqa: E731
+    codes = {call(p[0] + 2, p[1], p[2]), call(p[0], p[1] + 2, p[2]), call(p[0], p[1], p[2] + 8)}
+    assert len(codes) == 1 and 0 not in codes and call(*p) == 0
+    assert lib.ebr_block_swiglu_linear(1, 40, 15, 24, *p, 0, 0) != 0  # padded rows want scratch
+    assert lib.ebr_block_swiglu_linear_scratch(1, 0, 40, 16, 24) == 0 < lib.ebr_block_swiglu_linear_scratch(1, 0, 40, 15, 24)
+    torch.cuda.synchronize()
 
 
 def test_large_gates(cuda):
