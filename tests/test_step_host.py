@@ -134,13 +134,18 @@ def test_entries_refuse():
     assert ln2(1, 0, 3, 8, P, P, P, P, P, P, P, P, P, P, 0, None) == 5
 
     f, b1, b2 = lib.ebr_block_swiglu_linear, lib.ebr_block_swiglu_linear_bwd, lib.ebr_block_swiglu_linear_bwd2
-    assert f(4, 3, 8, 8, P, P, P, None) == 1
-    for N, C, I in ((0, 8, 8), (3, 0, 8), (3, 8, 0), (1 << 31, 8, 8), (3, 1 << 20, 8), (3, 8, 1 << 20), ((1 << 31) - 1, 8, 1 << 19)):
-        assert f(1, N, C, I, P, P, P, None) == 2
+    assert f(4, 3, 8, 8, P, P, P, P, None) == 1
+    for N, C, I in ((0, 8, 8), (3, 0, 8), (3, 8, 0), (1 << 31, 8, 8), (3, (1 << 20) - 7, 8), (3, 8, (1 << 19) - 7),
+                    ((1 << 31) - 1, 8, 1 << 18)):
+        assert f(1, N, C, I, P, P, P, P, None) == 2
         assert b1(1, N, C, I, P, P, P, P, P, P, None) == 2
         assert b2(1, N, C, I, P, P, P, P, P, P, P, P, None) == 2
         assert lib.ebr_block_swiglu_linear_scratch(1, 1, N, C, I) == -1
-    assert f(1, 3, 8, 8, P, P, 0, None) == 4 and b1(1, 3, 8, 8, P, 0, P, P, P, P, None) == 4
+    assert f(1, 40, 8, 9, P, P, P, 0, None) == 5 and f(1, 40, 8, 9, P, P, P, P + 8, None) == 3  # copies want scratch
+    assert f(1, 40, 8, 8, P + 2, P, P, 0, None) == 3 and f(1, 40, 8, 8, P, P, P + 8, 0, None) == 3
+    assert b1(1, 3, 8, 8, P, P + 2, P, P, P, P, None) == 3 and b2(1, 3, 8, 8, P, P, P, P + 4, P, P, P, P, None) == 3
+    assert lib.ebr_block_swiglu_linear_scratch(1, 0, 40, 8, 8) == lib.ebr_block_swiglu_linear_scratch(1, 0, 3, 9, 9) == 0
+    assert f(1, 3, 8, 8, P, P, 0, P, None) == 4 and b1(1, 3, 8, 8, P, 0, P, P, P, P, None) == 4
     assert b1(1, 3, 8, 8, P, P, P, P, P, 0, None) == 5 and b1(1, 3, 8, 8, P, P, P, P, P, P + 4, None) == 3
     assert b1(1, 3, 8, 8, P, P, P, 0, 0, P, None) == 0  # nothing wanted, nothing done
     assert b2(1, 3, 8, 8, P, P, P, P, P, 0, P, P, None) == 4
