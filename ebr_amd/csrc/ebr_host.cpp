@@ -1619,13 +1619,17 @@ bool adamw(const py::sequence& hp, const py::sequence& hg, const py::sequence& h
         kind[i] = std::find(kinds.begin(), kinds.end(), k) - kinds.begin();
         if (kind[i] == kinds.size()) kinds.push_back(k);
     }
-    for (const bool steps : {false, true}) {
-        std::vector<const void*> at_;
-        for (const ebr_optim_tensor& t : all)
-            if (steps || t.n > 0) at_.push_back(steps ? t.step : t.p);
-        std::sort(at_.begin(), at_.end());
-        if (std::adjacent_find(at_.begin(), at_.end()) != at_.end()) return false;  // the same one twice
-    }
+    std::vector<std::pair<const char*, const char*>> written;
+    written.reserve(6 * n);
+    for (const int i : {0, 2, 3, 4, 5, 6})
+        if (l[i])
+            for (const Tensor& x : *l[i]) {
+                const char* const from = static_cast<const char*>(x.data_ptr());
+                if (x.numel() > 0) written.emplace_back(from, from + x.nbytes());
+            }
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].first < written[i - 1].second) return false;  // two that share memory
     Tensor lr_dev, norm;
     if (!hlr.is_none()) {
         lr_dev = plain(hlr);

@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "../../include/ebr_optim.h"
@@ -516,17 +517,20 @@ template <typename P, typename G> static void step(hipStream_t s, int bits, unsi
     hipLaunchKernelGGL((k_adamw<P, G>), dim3(blocks), dim3(THREADS), 0, s, a);
 }
 
-// Whether two tensors share a parameter or a step.
-static bool twice(int64_t count, const ebr_optim_tensor* t) {
-    std::vector<const void*> ps, steps;
+// Whether any two of the tensors that are written share memory.
+static bool twice(int64_t count, const ebr_optim_tensor* t, int64_t pbytes, int bits) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> at;
+    at.reserve(count * (bits == 8 ? 6 : 4));
+    const auto add = [&](const void* p, int64_t bytes) {
+        if (bytes > 0) at.emplace_back((uintptr_t)p, (uintptr_t)p + bytes);
+    };
     for (int64_t i = 0; i < count; ++i) {
-        if (t[i].n > 0) ps.push_back(t[i].p);
-        steps.push_back(t[i].step);
+        const int64_t n = t[i].n, held = bits == 8 ? n : n * (pbytes == 8 ? 8 : 4), scales = bits == 8 ? (n + BLOCK - 1) / BLOCK * 4 : 0;
+        add(t[i].p, n * pbytes), add(t[i].m, held), add(t[i].v, held), add(t[i].ms, scales), add(t[i].vs, scales), add(t[i].step, 8);
     }
-    for (auto* v : {&ps, &steps}) {
-        std::sort(v->begin(), v->end());
-        if (std::adjacent_find(v->begin(), v->end()) != v->end()) return true;
-    }
+    std::sort(at.begin(), at.end());
+    for (size_t i = 1; i < at.size(); ++i)
+        if (at[i].first < at[i - 1].second) return true;
     return false;
 }
 
@@ -604,7 +608,7 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
         if (!t.step || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || (bits == 8 && (!t.ms || !t.vs))))) return EBR_ERR_NULL;
     }
     try {
-        if (twice(count, tensors)) return EBR_ERR_SHAPE;
+        if (twice(count, tensors, ptype == EBR_DTYPE_F64 ? 8 : ptype == EBR_DTYPE_F32 ? 4 : 2, bits)) return EBR_ERR_SHAPE;
     } catch (const std::bad_alloc&) {
         return EBR_ERR_HIP_BASE + (int)hipErrorOutOfMemory;
     }

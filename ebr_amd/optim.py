@@ -135,6 +135,10 @@ def _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, scales) -> None:
         at = [x.data_ptr() for x in ts if x.numel() > 0]
         if len(set(at)) < len(at):
             raise ValueError(f"optim: the same {name} twice in one step")
+    written = [x for ts in (params, exp_avgs, exp_avg_sqs, steps, *(scales or ())) for x in ts if x.numel() > 0]
+    ends = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in written)
+    if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
+        raise ValueError("optim: two of the tensors that a step writes share memory")
 
 
 def _check_numbers(lr, betas, eps, weight_decay, max_norm, device=None) -> None:
@@ -165,7 +169,7 @@ def _norms(grads: Sequence[Tensor]) -> Tuple[Tensor, Tensor]:
 
 
 def grad_norm(grads: Sequence[Tensor]) -> Tensor:
-    """The 2-norm of all the gradients together, summed to 47 bits in a fixed order: one fp32 number on their device. The
+    """The 2-norm of all the gradients together, summed in fp64 in a fixed order: one fp32 number on their device. The
     gradients may be of different dtypes."""
     return _norms(grads)[1]
 

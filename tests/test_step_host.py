@@ -119,6 +119,14 @@ def test_the_same_tensor_twice():
         _step(steps=[s, s])
 
 
+def test_tensors_that_share_memory():
+    m = torch.zeros(10)
+    with pytest.raises(ValueError, match="share memory"):
+        _step(exp_avgs=[m[:4], m[4:8]], exp_avg_sqs=[m[6:], torch.zeros(4)])
+    with pytest.raises(NotImplementedError):  # side by side: no kernel off the GPU
+        _step(exp_avgs=[m[:4], m[4:8]])
+
+
 def test_entries_refuse():
     lib = _capi.load()
     ln, ln1, ln2 = lib.ebr_block_layernorm, lib.ebr_block_layernorm_bwd, lib.ebr_block_layernorm_bwd2
@@ -152,14 +160,15 @@ def test_entries_refuse():
 
 
 def _table(rows=2, **kw):
-    table = [dict(p=P + 4096 * k, g=P, m=P, v=P, ms=P, vs=P, step=P + 8 * k, n=100) | kw for k in range(rows)]
+    table = [dict(p=P + 4096 * k, g=P, m=P + 4096 * (k + 16), v=P + 4096 * (k + 32), ms=P + 4096 * (k + 48), vs=P + 4096 * (k + 64),
+                  step=P + 4096 * 80 + 8 * k, n=100) | kw for k in range(rows)]
     return (_capi.OptimTensor * rows)(*(tuple(r[f] for f, _ in _capi.OptimTensor._fields_) for r in table))
 
 
 @pytest.mark.parametrize("code,kw", [
     (1, dict(pt=4)), (1, dict(gt=-1)), (1, dict(pt=1, gt=0)), (1, dict(pt=0, gt=3)), (1, dict(bits=16)), (1, dict(pt=3, gt=3, bits=8)),
     (2, dict(count=-1)), (2, dict(b1=1.0)), (2, dict(b2=float("nan"))), (2, dict(eps=-1.0)), (2, dict(row=dict(n=-1))),
-    (2, dict(row=dict(n=1 << 40))), (2, dict(row=dict(p=P))), (2, dict(row=dict(step=P))),
+    (2, dict(row=dict(n=1 << 40))), (2, dict(row=dict(m=P + 4096 * 32 + 396))), (2, dict(bits=8, row=dict(vs=P + 4096 * 16 + 96))), (2, dict(row=dict(p=P))), (2, dict(row=dict(step=P))),
     (4, dict(row=dict(g=0))), (4, dict(row=dict(step=0))), (4, dict(bits=8, row=dict(vs=0))), (4, dict(table=0)),
     (5, dict(scratch=0)), (3, dict(scratch=P + 8)), (0, dict(count=0)),
 ])  # fmt: skip
