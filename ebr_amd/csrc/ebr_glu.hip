@@ -503,6 +503,20 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
 #pragma unroll
         for (int j = 0; j < FJ; ++j) fb[s][j] = SB::read(from + SA::BYTES, (wj * FJ + j) * 32, s, lane);
     };
+    // fp32: the sums of 64 k each, added up apart (one chain over all k is off by three times as much)
+    constexpr bool IN_PARTS = sizeof(T) == 4;
+    f32x16 sums[IN_PARTS ? FI : 1][IN_PARTS ? FJ : 1] = {};
+    const auto take = [&]() {
+        if constexpr (IN_PARTS) {
+#pragma unroll
+            for (int i = 0; i < FI; ++i)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j) {
+                    sums[i][j] += acc[i][j];
+                    acc[i][j] = f32x16{};
+                }
+        }
+    };
     const auto multiply = [&](int s) {
 #pragma unroll
         for (int i = 0; i < FI; ++i)
@@ -581,10 +595,16 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
             stage(s1, s2);
             stage(s2, s3);
             stage(s3, s0);
+            if constexpr (IN_PARTS) take();
         }
     }
     stage_barrier<0>();  // (the loads past the end, of zeros, are done with the buffers)
 
+    if constexpr (IN_PARTS)
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) acc[i][j] = sums[i][j];
     // the sums of a split: tile by tile
     float* const part = EP == EP_PART ? reinterpret_cast<float*>(a.out) + ((int64_t)split * a.count + local) * (TI * TJ) : nullptr;
     if constexpr (STAGED) {
@@ -785,6 +805,8 @@ static int check(int dtype, int64_t N, int64_t C, int64_t I) {
     return tiles(2 * N) * most > MAX_BLOCKS || tiles(2 * I) * tiles(C) > MAX_BLOCKS ? EBR_ERR_SHAPE : EBR_OK;
 }
 
+enum { UNSPLIT = 0, MANY_K = 1, FEW_TILES = 2 };
+
 // The tiles that a product is cut into, from its sizes alone.
 struct Cut {
     int tile;            // 256, 128 or 64
@@ -793,7 +815,8 @@ struct Cut {
     int64_t steps, whole;
     int64_t tiles() const { return ti * tj; }
     int64_t part_bytes() const { return splits > 1 ? splits * (tiles() - whole) * tile * tile * 4 : 0; }
-    Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, bool split) {  // gated: 0, 1, or 2 for TWO
+    // gated: 0, 1, or 2 for TWO; split: of many k by plan, or FEW_TILES, where the tiles of an unsplit product are few
+    Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, int split) {
         const auto up = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
         const int64_t wide = gated ? 2 * ni : ni, high = gated == 2 ? 2 * nj : nj, all = up(nk, STAGE / size_of(dtype)) * pairs;
         tile = 256;
@@ -801,8 +824,8 @@ struct Cut {
         else if (dtype == EBR_DTYPE_F32) tile = 128;
         const auto tiles = [&](int t) { return up(wide, t) * up(high, t); };
         if (dtype != EBR_DTYPE_F64) {
-            if (tile == 256 && tiles(256) < (split ? 4 : 200)) tile = 128;
-            if (tile == 128 && tiles(128) < (split ? 8 : 200)) tile = 64;
+            if (tile == 256 && tiles(256) < (split == MANY_K ? 4 : 200)) tile = 128;
+            if (tile == 128 && tiles(128) < (split == MANY_K ? 8 : 200)) tile = 64;
         }
         ti = dtype == EBR_DTYPE_F64 ? up(ni, 64) : up(wide, tile);
         tj = dtype == EBR_DTYPE_F64 ? up(nj, 64) : up(high, tile);
@@ -812,8 +835,8 @@ struct Cut {
             // As many workgroups as the card holds at once, and not one more: 258 of 62208 x 256 -> 1536 took 165 us, 252 113. Where
             // there are more tiles than that, those of the last round alone are split: 352 of 8192 x 2048 -> 11264 take 357 us, 410 unsplit.
             const int64_t held = tile == 256 ? 256 : 512, last = whole <= held ? whole : tile == 256 ? whole % held : 0;
-            const int64_t most = whole <= held ? up(all, 4) : all / 64;
-            const int64_t want = last ? std::min(held / last, most) : 1;
+            const int64_t most = split == FEW_TILES ? all / 8 : whole <= held ? up(all, 4) : all / 64;
+            const int64_t want = last && !(split == FEW_TILES && whole >= 128) ? std::min(held / last, most) : 1;
             if (want > 1) {
                 steps = up(all, want);
                 splits = (int)up(all, steps);
@@ -867,16 +890,33 @@ struct Grads {
 };
 static bool with_rest(int dtype, int64_t N) { return size_of(dtype) == 2 && N <= 64; }
 
-// dx of dgu, and dw of (x, dgu) and, where there is one, a second pair.
-static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w, Grads dgu, void* dx, hipStream_t s) {
+static void join(int dtype, const Cut& c, const Args& a, const float* part, void* out, hipStream_t s) {
+    const dim3 grid((unsigned)(a.count * (c.tile * c.tile / 1024)));
+    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, a, c.tile, part, (__bf16*)out);
+    else if (dtype == EBR_DTYPE_F16) hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, a, c.tile, part, (_Float16*)out);
+    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, a, c.tile, part, (float*)out);
+}
+
+// dx of dgu, and dw of (x, dgu) and, where there is one, a second pair. Of few rows dx has few tiles, and many k: split among
+// workgroups and joined it takes 9.0 us of 81 x 1536 -> 256 (10.8 unsplit); 4 x 1649 -> 2240 in fp32 to second order, which has
+// two of them, 325 us (545).
+static Cut input_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) { return Cut(dtype, C, N, 2 * I, pairs, 0, FEW_TILES); }
+static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w, Grads dgu, void* dx, float* part, hipStream_t s) {
     Args a = {};
     a.a[0] = a.a[1] = w, a.b[0] = dgu.g, a.b[1] = dgu.rest, a.pairs = dgu.rest ? 2 : 1;
     a.lda = C, a.ldb = 2 * I, a.ni = C, a.nj = N, a.nk = 2 * I, a.out = dx, a.ldo = C;
-    product<M_ROWS, K_ROWS, EP_OUT>(dtype, Cut(dtype, C, N, 2 * I, a.pairs, 0, false), a, s);
+    const Cut c = input_cut(dtype, N, C, I, a.pairs);
+    if (c.splits == 1) {
+        product<M_ROWS, K_ROWS, EP_OUT>(dtype, c, a, s);
+        return;
+    }
+    a.out = part;
+    product<M_ROWS, K_ROWS, EP_PART>(dtype, c, a, s);
+    join(dtype, c, a, part, dx, s);
 }
 
 static Cut weight_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) {
-    return Cut(dtype, C, 2 * I, N, pairs, 0, true);
+    return Cut(dtype, C, 2 * I, N, pairs, 0, MANY_K);
 }
 static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* x, Grads dgu, const void* x2, Grads dgu2, void* dw,
                         float* part, hipStream_t s) {
@@ -890,10 +930,7 @@ static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* 
     if (c.splits == 1) return;
     a.out = part;
     product<M_ROWS, M_ROWS, EP_PART>(dtype, c, a, s);
-    const dim3 grid((unsigned)(a.count * (c.tile * c.tile / 1024)));
-    if (dtype == EBR_DTYPE_BF16) hipLaunchKernelGGL((k_join<__bf16>), grid, dim3(256), 0, s, a, c.tile, part, (__bf16*)dw);
-    else if (dtype == EBR_DTYPE_F16) hipLaunchKernelGGL((k_join<_Float16>), grid, dim3(256), 0, s, a, c.tile, part, (_Float16*)dw);
-    else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, a, c.tile, part, (float*)dw);
+    join(dtype, c, a, part, dw, s);
 }
 
 template <typename T> static void few(hipStream_t s, const Args& a) {
@@ -1018,7 +1055,7 @@ static void forward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, c
         else few<_Float16>(s, a);
         return;
     }
-    product<K_ROWS, K_ROWS, EP_FWD>(dtype, Cut(dtype, I, N, C, 1, 1, false), a, s);
+    product<K_ROWS, K_ROWS, EP_FWD>(dtype, Cut(dtype, I, N, C, 1, 1, UNSPLIT), a, s);
 }
 // Whether it takes rows of any width and alignment as they are.
 static bool as_they_are(int dtype, int64_t N, int64_t C) { return dtype == EBR_DTYPE_F64 || (N <= FEW && C * size_of(dtype) >= 16); }
@@ -1026,8 +1063,9 @@ static bool as_they_are(int dtype, int64_t N, int64_t C) { return dtype == EBR_D
 static int64_t own_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I) {
     if (order == 0) return 0;
     const int64_t each = with_rest(dtype, N) ? 2 : 1;
-    // [dg|du], for order 2 [gg|gu] too, and the weight gradient's partial sums
-    return order * each * up16(N * 2 * I * size_of(dtype)) + weight_cut(dtype, N, C, I, (int)(order * each)).part_bytes() + 16;
+    // [dg|du], for order 2 [gg|gu] too, and a gradient's partial sums
+    const int64_t part = std::max(weight_cut(dtype, N, C, I, (int)(order * each)).part_bytes(), input_cut(dtype, N, C, I, (int)each).part_bytes());
+    return order * each * up16(N * 2 * I * size_of(dtype)) + part + 16;
 }
 
 static void backward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy, void* dx, void* dw,
@@ -1037,9 +1075,9 @@ static void backward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, 
     const int64_t rows = up16(N * 2 * I * size_of(dtype));
     a.dgu = at, at += rows;
     if (with_rest(dtype, N)) a.dgu2 = at, at += rows;
-    product<K_ROWS, K_ROWS, EP_BWD>(dtype, Cut(dtype, I, N, C, 1, 1, false), a, s);
+    product<K_ROWS, K_ROWS, EP_BWD>(dtype, Cut(dtype, I, N, C, 1, 1, UNSPLIT), a, s);
     const Grads dgu = {a.dgu, a.dgu2};
-    if (dx) input_grad(dtype, N, C, I, w, dgu, dx, s);
+    if (dx) input_grad(dtype, N, C, I, w, dgu, dx, reinterpret_cast<float*>(at), s);
     if (dw) weight_grad(dtype, N, C, I, x, dgu, nullptr, {}, dw, reinterpret_cast<float*>(at), s);
 }
 
@@ -1052,9 +1090,9 @@ static void backward2(int dtype, int64_t N, int64_t C, int64_t I, const void* x,
         if (to) *to = at, at += rows;
         if (to && with_rest(dtype, N)) *(to == &a.ggu ? &a.ggu2 : &a.dgu2) = at, at += rows;
     }
-    product<K_ROWS, K_ROWS, EP_BWD2>(dtype, Cut(dtype, I, N, C, 1, 2, false), a, s);
+    product<K_ROWS, K_ROWS, EP_BWD2>(dtype, Cut(dtype, I, N, C, 1, 2, UNSPLIT), a, s);
     const Grads dgu = {a.dgu, a.dgu2}, ggu = {a.ggu, a.ggu2};
-    if (gx) input_grad(dtype, N, C, I, w, ggu, gx, s);
+    if (gx) input_grad(dtype, N, C, I, w, ggu, gx, reinterpret_cast<float*>(at), s);
     if (gw) weight_grad(dtype, N, C, I, x, ggu, c, dgu, gw, reinterpret_cast<float*>(at), s);
 }
 
