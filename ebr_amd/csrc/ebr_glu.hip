@@ -16,6 +16,12 @@
 // reads, and does not wait for them. Rows' 16-byte chunks (64-byte chunks for operands of the
 // second kind, which are read transposed) are exchanged by a function of the row, so that lanes meet no bank conflicts.
 // Whatever lies outside the tensors is read as zero by the buffer loads' bounds.
+//
+// Tiles of 256 x 256 in 16 bits where there are enough of them: four waves of 128 x 128 (fewest bytes of shared memory a product),
+// eight of 128 x 64 where the activation follows, whose arithmetic two waves a SIMD overlap (62208 x 256 -> 768: forward 88 us, 99
+// with four; backward 118, 145; second 237, 275). Bound by the matrix cores at long k (8192 x 2048 -> 5632: forward 380 us, 995
+// TFLOP/s, the library's product without the activation 396; backward's product 403; dx 320, 1,180; dw 357, 1,060), at k of some
+// hundreds by prologue and epilogue. fp32 goes in tiles of 128, at the fp32 instructions' rate.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
