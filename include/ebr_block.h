@@ -134,8 +134,8 @@ int ebr_block_layernorm_bwd2(int dtype, int wdtype, int64_t rows, int C, const v
                              const void* dy, const void* u, const void* uw, const void* ub, void* gx, void* gdy, void* gw,
                              void* scratch, void* stream);
 
-/* Bytes of scratch of the layer norm's derivatives (order 1, 2), for tensors of any alignment; -1 for sizes or types that they
- * refuse. */
+/* Bytes of scratch of the layer norm's derivatives (order 1, 2), for tensors of any alignment, outputs apart from inputs; -1 for
+ * sizes or types that they refuse. */
 int64_t ebr_block_layernorm_scratch(int dtype, int order, int64_t rows, int C);
 
 /* y = silu(g) u for x [N, C] and w [2 I, C], gate rows first: g = x w[:I]^T, u = x w[I:]^T, summed in fp32 (fp64 for fp64) and
