@@ -654,8 +654,10 @@ template <> struct Mma16<float> {
     }
 };
 constexpr int FEW = 32, FEW_WAVES = 8;
-template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void k_few(Args a) {
-    constexpr int EPC = 16 / (int)sizeof(T), TURN = 8 * EPC, AT_ONCE = 4;  // k of a wave's turn; turns under way
+template <typename T, int EP, int ROWS> __global__ __launch_bounds__(64 * FEW_WAVES) void k_few(Args a) {
+    constexpr bool TWO = EP == EP_BWD2;
+    constexpr int FJ = ROWS * (TWO ? 2 : 1);  // sixteens of x, then of c
+    constexpr int EPC = 16 / (int)sizeof(T), TURN = 8 * EPC, AT_ONCE = FJ == 4 ? 2 : 4;  // k of a wave's turn; turns under way
     __shared__ f32x4 sums[FEW_WAVES][2][FJ][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, part = lane >> 4;
@@ -688,7 +690,11 @@ template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void 
                 g[t][h] = in ? chunk(gate, k) : u32x4{};
                 u[t][h] = in ? chunk(up, k) : u32x4{};
 #pragma unroll
-                for (int j = 0; j < FJ; ++j) b[t][h][j] = in && j * 16 + l16 < a.nj ? chunk(x + (j * 16 + l16) * a.ldb, k) : u32x4{};
+                for (int j = 0; j < FJ; ++j) {
+                    const int64_t n = j % ROWS * 16 + l16;
+                    const T* const from = j < ROWS ? x : reinterpret_cast<const T*>(a.c);
+                    b[t][h][j] = in && n < a.nj ? chunk(from + n * a.ldb, k) : u32x4{};
+                }
             }
 #pragma unroll
         for (int t = 0; t < AT_ONCE; ++t)
@@ -705,17 +711,39 @@ template <typename T, int FJ> __global__ __launch_bounds__(64 * FEW_WAVES) void 
 #pragma unroll
         for (int j = 0; j < FJ; ++j) sums[wave][h][j][lane] = acc[h][j];
     __syncthreads();
-    if (wave >= FJ) return;
-    f32x4 g = {}, u = {};
+    if (wave >= ROWS) return;
+    const auto total = [&](int h, int j) {
+        f32x4 v = {};
 #pragma unroll
-    for (int w = 0; w < FEW_WAVES; ++w) {
-        g += sums[w][0][wave][lane];
-        u += sums[w][1][wave][lane];
-    }
+        for (int w = 0; w < FEW_WAVES; ++w) v += sums[w][h][j][lane];
+        return v;
+    };
+    const f32x4 g = total(0, wave), u = total(1, wave);
+    f32x4 cg = {}, cu = {};
+    if constexpr (TWO) cg = total(0, wave + ROWS), cu = total(1, wave + ROWS);
     const int64_t n = wave * 16 + l16, i = i0 + 4 * part;
     if (n >= a.nj || i >= a.ni) return;
-    const float v[4] = {gated(g[0], u[0]), gated(g[1], u[1]), gated(g[2], u[2]), gated(g[3], u[3])};
-    put4(reinterpret_cast<T*>(a.out) + n * a.ni + i, v, a.ni - i, a.ni % 4 == 0);
+    const int64_t some = a.ni - i, at = n * a.ni + i, two = n * 2 * a.ni + i;
+    const bool whole = a.ni % 4 == 0;
+    T* const y = reinterpret_cast<T*>(a.out);
+    float dy[4], o[4], og[4], ou[4], rg[4], ru[4];
+    if constexpr (EP != EP_FWD) get4(reinterpret_cast<const T*>(a.dy) + at, dy, some, whole);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (EP == EP_FWD) o[e] = gated(g[e], u[e]);
+        else first_of(g[e], u[e], dy[e], og[e], ou[e]);
+        if constexpr (TWO) second_of(g[e], u[e], dy[e], cg[e], cu[e], rg[e], ru[e], o[e]);
+    }
+    if constexpr (EP != EP_BWD) put4(y + at, o, some, whole);
+    const auto both = [&](void* first, void* rest, const float (&vg)[4], const float (&vu)[4]) {
+        if (!first) return;
+        T* const p = reinterpret_cast<T*>(first) + two;
+        put4(p, vg, some, whole);
+        put4(p + a.ni, vu, some, whole);
+        if (rest) put_rest(reinterpret_cast<T*>(rest) + two, vg, vu, a.ni, some, whole);
+    };
+    if constexpr (EP != EP_FWD) both(a.dgu, a.dgu2, og, ou);
+    if constexpr (TWO) both(a.ggu, a.ggu2, rg, ru);
 }
 
 // fp64, for gradient checks: 64 x 64 of D (gated: of each half, and of both right operands) a workgroup, 4 x 4 a thread.
@@ -904,8 +932,8 @@ static void join(int dtype, const Cut& c, const Args& a, const float* part, void
 }
 
 // dx of dgu, and dw of (x, dgu) and, where there is one, a second pair. Of few rows dx has few tiles, and many k: split among
-// workgroups and joined it takes 9.0 us of 81 x 1536 -> 256 (10.8 unsplit); 4 x 1649 -> 2240 in fp32 to second order, which has
-// two of them, 325 us (545).
+// workgroups and joined it takes 9.0 us of 81 x 1536 -> 256 (10.8 unsplit); a pass of 4 x 1649 -> 2240 in fp32 to second order, which
+// has two of them, went from 545 us to 325 by it.
 static Cut input_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) { return Cut(dtype, C, N, 2 * I, pairs, 0, FEW_TILES); }
 static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w, Grads dgu, void* dx, float* part, hipStream_t s) {
     Args a = {};
@@ -939,10 +967,22 @@ static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* 
     join(dtype, c, a, part, dw, s);
 }
 
-template <typename T> static void few(hipStream_t s, const Args& a) {
-    const dim3 grid((unsigned)((a.ni + 15) / 16)), threads(64 * FEW_WAVES);
-    if (a.nj <= 16) hipLaunchKernelGGL((k_few<T, 1>), grid, threads, 0, s, a);
-    else hipLaunchKernelGGL((k_few<T, 2>), grid, threads, 0, s, a);
+// The products of gate and up: of few rows, or of many.
+static bool is_few(int dtype, int64_t N, int64_t C) { return dtype != EBR_DTYPE_F64 && N <= FEW && C * size_of(dtype) >= 16; }
+template <int EP> static void gates(int dtype, Args& a, hipStream_t s) {
+    if (!is_few(dtype, a.nj, a.nk)) {
+        product<K_ROWS, K_ROWS, EP>(dtype, Cut(dtype, a.ni, a.nj, a.nk, 1, EP == EP_BWD2 ? 2 : 1, UNSPLIT), a, s);
+        return;
+    }
+    const auto with = [&](auto v) {
+        using T = decltype(v);
+        const dim3 grid((unsigned)((a.ni + 15) / 16)), threads(64 * FEW_WAVES);
+        if (a.nj <= 16) hipLaunchKernelGGL((k_few<T, EP, 1>), grid, threads, 0, s, a);
+        else hipLaunchKernelGGL((k_few<T, EP, 2>), grid, threads, 0, s, a);
+    };
+    if (dtype == EBR_DTYPE_F32) with(float());
+    else if (dtype == EBR_DTYPE_BF16) with(__bf16());
+    else with(_Float16());
 }
 
 static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -1055,16 +1095,10 @@ static bool all_aligned(std::initializer_list<const void*> ps) {
 static void forward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, hipStream_t s) {
     Args a = {};
     a.a[0] = w, a.b[0] = x, a.lda = a.ldb = C, a.ni = I, a.nj = N, a.nk = C, a.pairs = 1, a.out = y;
-    if (dtype != EBR_DTYPE_F64 && N <= FEW && C * size_of(dtype) >= 16) {
-        if (dtype == EBR_DTYPE_F32) few<float>(s, a);
-        else if (dtype == EBR_DTYPE_BF16) few<__bf16>(s, a);
-        else few<_Float16>(s, a);
-        return;
-    }
-    product<K_ROWS, K_ROWS, EP_FWD>(dtype, Cut(dtype, I, N, C, 1, 1, UNSPLIT), a, s);
+    gates<EP_FWD>(dtype, a, s);
 }
 // Whether it takes rows of any width and alignment as they are.
-static bool as_they_are(int dtype, int64_t N, int64_t C) { return dtype == EBR_DTYPE_F64 || (N <= FEW && C * size_of(dtype) >= 16); }
+static bool as_they_are(int dtype, int64_t N, int64_t C) { return dtype == EBR_DTYPE_F64 || is_few(dtype, N, C); }
 
 static int64_t own_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I) {
     if (order == 0) return 0;
@@ -1081,7 +1115,7 @@ static void backward(int dtype, int64_t N, int64_t C, int64_t I, const void* x, 
     const int64_t rows = up16(N * 2 * I * size_of(dtype));
     a.dgu = at, at += rows;
     if (with_rest(dtype, N)) a.dgu2 = at, at += rows;
-    product<K_ROWS, K_ROWS, EP_BWD>(dtype, Cut(dtype, I, N, C, 1, 1, UNSPLIT), a, s);
+    gates<EP_BWD>(dtype, a, s);
     const Grads dgu = {a.dgu, a.dgu2};
     if (dx) input_grad(dtype, N, C, I, w, dgu, dx, reinterpret_cast<float*>(at), s);
     if (dw) weight_grad(dtype, N, C, I, x, dgu, nullptr, {}, dw, reinterpret_cast<float*>(at), s);
@@ -1096,7 +1130,7 @@ static void backward2(int dtype, int64_t N, int64_t C, int64_t I, const void* x,
         if (to) *to = at, at += rows;
         if (to && with_rest(dtype, N)) *(to == &a.ggu ? &a.ggu2 : &a.dgu2) = at, at += rows;
     }
-    product<K_ROWS, K_ROWS, EP_BWD2>(dtype, Cut(dtype, I, N, C, 1, 2, UNSPLIT), a, s);
+    gates<EP_BWD2>(dtype, a, s);
     const Grads dgu = {a.dgu, a.dgu2}, ggu = {a.ggu, a.ggu2};
     if (gx) input_grad(dtype, N, C, I, w, ggu, gx, reinterpret_cast<float*>(at), s);
     if (gw) weight_grad(dtype, N, C, I, x, ggu, c, dgu, gw, reinterpret_cast<float*>(at), s);

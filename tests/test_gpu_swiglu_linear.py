@@ -128,7 +128,7 @@ def test_sizes(cuda, N, C, I, dtype):
     _check(*_inputs(cuda, N, C, I, dtype, seed=N).values())
 
 
-# up to 32 rows, whose forward reads the weight by itself: rows off 16, a last turn that is not full, many turns, widths off
+# up to 32 rows, whose gates read the weight straight into registers: rows off 16, a last turn that is not full, many turns, widths off
 # 16 and off the vectors
 @pytest.mark.parametrize("N", [1, 3, 15, 16, 17, 31, 32])
 @pytest.mark.parametrize("C,I", [(8, 8), (72, 24), (520, 16), (2056, 40), (5000, 1000), (9, 33), (1031, 15), (2047, 1)])
@@ -136,9 +136,7 @@ def test_sizes(cuda, N, C, I, dtype):
 def test_few_rows(cuda, N, C, I, dtype):
     _say(f"swiglu_linear few rows {N} {C} {I} {dtype}")
     ts = _inputs(cuda, N, C, I, dtype, seed=N + C)
-    y = block.swiglu_linear(ts["x"], ts["w"])
-    (want, *_), (tol, *_) = _forms(*ts.values())
-    assert y.dtype == dtype and y.shape == (N, I) and bool(((y.double() - want).abs() <= tol).all())
+    y = _check(**ts)[0]
     one = block.swiglu_linear(ts["x"][N - 1], ts["w"])  # a row alone, of one dimension: the same sums
     assert N > 16 or torch.equal(one, y[N - 1])
 
