@@ -38,6 +38,7 @@ HEADERS = [
     ROOT / "include" / "ebr_optim.h",
     CSRC / "attn_f64.hpp",
     CSRC / "rowwise.hpp",
+    CSRC / "glu_plan.hpp",
 ]
 
 

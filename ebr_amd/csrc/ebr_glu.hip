@@ -27,6 +27,7 @@
 #include <utility>
 
 #include "../../include/ebr_block.h"
+#include "glu_plan.hpp"
 #include "rowwise.hpp"
 
 namespace ebr_glu {
@@ -44,7 +45,6 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 enum { K_ROWS = 0, M_ROWS = 1 };                                  // how an operand lies
 enum { EP_OUT = 0, EP_PART = 1, EP_FWD = 2, EP_BWD = 3, EP_BWD2 = 4 };  // what becomes of D: y, [dg|du], or all of bwd2's
-constexpr int STAGE = 64;                                         // bytes of k a stage
 constexpr uint32_t OUTSIDE = 0x40000000;                          // an offset past a buffer's end
 
 struct Args {
@@ -478,7 +478,7 @@ template <typename T, int ALIES, int BLIES, int EP, int TI, int TJ, int WI, int 
 __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     constexpr int WAVES = WI * WJ, FI = TI / WI / 32, FJ = TJ / WJ / 32;
     constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
-    constexpr bool STAGED = sizeof(T) == 2 && TI >= 128;  // four waves, an array each, or eight, half of one
+    constexpr bool STAGED = staged(sizeof(T), TI);  // four waves, an array each, or eight, half of one
     static_assert(!STAGED || WAVES == 4 || WAVES == 8, "an array a wave");
     static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
     using SA = Side<T, ALIES, TI, WAVES, GATED>;
@@ -653,7 +653,7 @@ template <> struct Mma16<float> {
         return c;
     }
 };
-constexpr int FEW = 32, FEW_WAVES = 8;
+constexpr int FEW_WAVES = 8;
 template <typename T, int EP, int ROWS> __global__ __launch_bounds__(64 * FEW_WAVES) void k_few(Args a) {
     constexpr bool TWO = EP == EP_BWD2;
     constexpr int FJ = ROWS * (TWO ? 2 : 1);  // sixteens of x, then of c
@@ -828,7 +828,6 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int 
 
 // -- launches ----------------------------------------------------------------------------------------------------------
 
-static int size_of(int dtype) { return dtype == EBR_DTYPE_F64 ? 8 : dtype == EBR_DTYPE_F32 ? 4 : 2; }
 static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
 
 static int check(int dtype, int64_t N, int64_t C, int64_t I) {
@@ -838,47 +837,6 @@ static int check(int dtype, int64_t N, int64_t C, int64_t I) {
     const int64_t most = tiles(2 * I) > tiles(C) ? tiles(2 * I) : tiles(C);
     return tiles(2 * N) * most > MAX_BLOCKS || tiles(2 * I) * tiles(C) > MAX_BLOCKS ? EBR_ERR_SHAPE : EBR_OK;
 }
-
-enum { UNSPLIT = 0, MANY_K = 1, FEW_TILES = 2 };
-
-// The tiles that a product is cut into, from its sizes alone.
-struct Cut {
-    int tile;            // 256, 128 or 64
-    int64_t ti, tj;
-    int splits = 1;      // of the tiles from ``whole`` on
-    int64_t steps, whole;
-    int64_t tiles() const { return ti * tj; }
-    int64_t part_bytes() const { return splits > 1 ? splits * (tiles() - whole) * tile * tile * 4 : 0; }
-    // gated: 0, 1, or 2 for TWO; split: of many k by plan, or FEW_TILES, where the tiles of an unsplit product are few
-    Cut(int dtype, int64_t ni, int64_t nj, int64_t nk, int pairs, int gated, int split) {
-        const auto up = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
-        const int64_t wide = gated ? 2 * ni : ni, high = gated == 2 ? 2 * nj : nj, all = up(nk, STAGE / size_of(dtype)) * pairs;
-        tile = 256;
-        if (dtype == EBR_DTYPE_F64) tile = 64;
-        else if (dtype == EBR_DTYPE_F32) tile = 128;
-        const auto tiles = [&](int t) { return up(wide, t) * up(high, t); };
-        if (dtype != EBR_DTYPE_F64) {
-            if (tile == 256 && tiles(256) < (split == MANY_K ? 4 : 200)) tile = 128;
-            if (tile == 128 && tiles(128) < (split == MANY_K ? 8 : 200)) tile = 64;
-        }
-        ti = dtype == EBR_DTYPE_F64 ? up(ni, 64) : up(wide, tile);
-        tj = dtype == EBR_DTYPE_F64 ? up(nj, 64) : up(high, tile);
-        steps = all;
-        whole = ti * tj;
-        if (split && dtype != EBR_DTYPE_F64) {
-            // As many workgroups as the card holds at once, and not one more: 258 of 62208 x 256 -> 1536 took 165 us, 252 113. Where
-            // there are more tiles than that, those of the last round alone are split: 352 of 8192 x 2048 -> 11264 take 357 us, 410 unsplit.
-            const int64_t held = tile == 256 ? 256 : 512, last = whole <= held ? whole : tile == 256 ? whole % held : 0;
-            const int64_t most = split == FEW_TILES ? all / 8 : whole <= held ? up(all, 4) : all / 64;
-            const int64_t want = last && !(split == FEW_TILES && whole >= 128) ? std::min(held / last, most) : 1;
-            if (want > 1) {
-                steps = up(all, want);
-                splits = (int)up(all, steps);
-                if (splits > 1) whole -= last;
-            }
-        }
-    }
-};
 
 template <typename T, int ALIES, int BLIES, int EP> static void launch(hipStream_t s, const Cut& c, const Args& a) {
     const dim3 grid((unsigned)(a.count * a.splits));
@@ -917,12 +875,10 @@ template <int ALIES, int BLIES, int EP> static void product(int dtype, const Cut
     }
 }
 
-// [dg|du] or [gg|gu], rounded, and what they lack where the products take that as well: of few rows a weight's gradient adds up
-// few products, and shows their roundings.
+// [dg|du] or [gg|gu], rounded, and what they lack where the products take that as well (with_rest).
 struct Grads {
     const void *g, *rest;
 };
-static bool with_rest(int dtype, int64_t N) { return size_of(dtype) == 2 && N <= 64; }
 
 static void join(int dtype, const Cut& c, const Args& a, const float* part, void* out, hipStream_t s) {
     const dim3 grid((unsigned)(a.count * (c.tile * c.tile / 1024)));
@@ -968,10 +924,9 @@ static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* 
 }
 
 // The products of gate and up: of few rows, or of many.
-static bool is_few(int dtype, int64_t N, int64_t C) { return dtype != EBR_DTYPE_F64 && N <= FEW && C * size_of(dtype) >= 16; }
 template <int EP> static void gates(int dtype, Args& a, hipStream_t s) {
     if (!is_few(dtype, a.nj, a.nk)) {
-        product<K_ROWS, K_ROWS, EP>(dtype, Cut(dtype, a.ni, a.nj, a.nk, 1, EP == EP_BWD2 ? 2 : 1, UNSPLIT), a, s);
+        product<K_ROWS, K_ROWS, EP>(dtype, gates_cut(dtype, EP - EP_FWD, a.nj, a.nk, a.ni), a, s);
         return;
     }
     const auto with = [&](auto v) {

@@ -1,0 +1,55 @@
+"""GPU parity of the layer norm, the gated projection and the optimizer's step next to the borders of their plans and arguments.
+
+Tolerances of the gated projection are those of ``tests/test_gpu_swiglu_linear.py``, whose closed forms in 64 bits are used."""
+
+import pytest
+import torch
+from test_gpu_swiglu_linear import _check, _forms, _inputs, _say
+
+from ebr_amd.fused_attn.loader import hip_library
+
+pytestmark = pytest.mark.gpu
+
+CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
+
+
+@pytest.fixture
+def cuda():
+    return torch.device("cuda", 0)
+
+
+# on both sides of where gate and up would go in tiles of 128 (I above 12,736) and of 256 (from 25,600 on) for these rows, and of
+# 64 rows, up to which the products take what [dg|du] and [gg|gu] lack of their values before rounding
+@pytest.mark.parametrize("N", [33, 48, 64, 65])
+@pytest.mark.parametrize("C,I", [(72, 12736), (72, 12744), (264, 14336), (40, 25608), (71, 12745)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gated_projection_of_some_rows_against_a_wide_weight(cuda, N, C, I, dtype):
+    _say(f"swiglu_linear wide weight {N} {C} {I} {dtype}")
+    ts = _inputs(cuda, N, C, I, dtype, seed=N + I)
+    got = _check(*ts.values())
+    lib, code, stream = hip_library(), CODE[dtype], torch.cuda.current_stream().cuda_stream
+    for order in (1, 2):  # scratch of NaN: whatever of it is read has been written
+        scratch = torch.full((lib.ebr_block_swiglu_linear_scratch(code, order, N, C, I),), 255, device=cuda, dtype=torch.uint8)
+        gx, gdy, gw = (torch.empty_like(ts[n]) for n in ("x", "dy", "w"))
+        p = [ts[n].data_ptr() for n in ("x", "w", "dy", "c")[: order + 2]]
+        if order == 1:
+            rc = lib.ebr_block_swiglu_linear_bwd(code, N, C, I, *p, gx.data_ptr(), gw.data_ptr(), scratch.data_ptr(), stream)
+        else:
+            rc = lib.ebr_block_swiglu_linear_bwd2(code, N, C, I, *p, gx.data_ptr(), gdy.data_ptr(), gw.data_ptr(),
+                                                  scratch.data_ptr(), stream)
+        assert rc == 0
+        assert torch.equal(gx, got[1 if order == 1 else 3]) and torch.equal(gw, got[2 if order == 1 else 5])
+        assert order == 1 or torch.equal(gdy, got[4])
+
+
+def test_gated_projection_carries_both_parts_up_to_64_rows(cuda):
+    """Of a wide weight as of a narrow one. A rounding to bf16 is off by 2^-8 / sqrt(3) of a number's binade in the mean square,
+    and a number is sqrt(1.5 / ln 2) of its binade (evenly spread over its logarithm): 1.54e-3. Values rounded once stay near that,
+    those of sums whose operands were rounded too are sqrt(2) of it off, 2.2e-3; 1.9e-3 lies between."""
+    _say("swiglu_linear both parts")
+    for I in (520, 14336):
+        ts = _inputs(cuda, 48, 136, I, torch.bfloat16, seed=I)
+        got = _check(*ts.values())
+        want, _ = _forms(**ts)
+        for k in (1, 2, 3, 5):
+            assert float((got[k].double() - want[k]).norm() / want[k].norm()) < 1.9e-3, (I, k)

@@ -1,0 +1,52 @@
+"""Host-side checks, no GPU, of what the layer norm, the gated projection and the optimizer's step do next to the borders of their
+plans and arguments. Parity of the kernels there is in ``tests/test_gpu_step_edges.py``."""
+
+import os
+import subprocess
+from pathlib import Path
+
+from ebr_amd import block
+
+PLAN = r"""
+#include "glu_plan.hpp"
+#include <cstdio>
+using namespace ebr_glu;
+int main() {
+    long seen = 0, wrong = 0;
+    const int64_t widths[] = {1, 8, 24, 64, 1000, 5632, 6400, 6408, 12736, 12744, 14336, 25600, 25608, 28672, (1 << 19) - 8};
+    for (int dtype = 0; dtype < 4; ++dtype)
+        for (int order = 1; order <= 2; ++order)
+            for (const int64_t C : {8, 72, 4096, (1 << 20) - 8})
+                for (const int64_t I : widths)
+                    for (int64_t N = 1; N <= 130; ++N) {
+                        const bool rest = with_rest(dtype, N);
+                        if (rest != (N <= 64 && (dtype == EBR_DTYPE_BF16 || dtype == EBR_DTYPE_F16))) ++wrong;
+                        if (is_few(dtype, N, C)) continue;
+                        const int tile = gates_cut(dtype, order, N, C, I).tile;
+                        if (tile != 64 && tile != 128 && tile != 256) ++wrong;
+                        if (rest && staged(size_of(dtype), tile)) {
+                            ++wrong;
+                            std::printf("%d %d %lld %lld %d\n", dtype, order, (long long)N, (long long)I, tile);
+                        }
+                        if (!rest) seen += staged(size_of(dtype), tile);
+                    }
+    return wrong ? 1 : seen ? 0 : 2;
+}
+"""
+
+
+def _host_program(tmp_path, source):
+    """A program of plain C++ beside the library's sources, run; its exit status and output."""
+    csrc = Path(block.__file__).parent / "csrc"
+    (tmp_path / "t.cpp").write_text(source)
+    cc = [os.environ.get("CXX", "g++"), "-std=c++17", "-O1", f"-I{csrc}", str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")]
+    subprocess.run(cc, check=True, capture_output=True)
+    run = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, timeout=60)
+    return run.returncode, run.stdout
+
+
+def test_gated_projection_of_few_rows_writes_what_its_products_read(tmp_path):
+    """What [dg|du] lacks of its values before rounding enters the derivatives' products of up to 64 rows in 16 bits: no tile
+    that leaves it unwritten stands before them."""
+    rc, out = _host_program(tmp_path, PLAN)
+    assert rc == 0, out
