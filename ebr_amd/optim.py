@@ -158,6 +158,23 @@ def _check_numbers(lr, betas, eps, weight_decay, max_norm, device=None) -> None:
         raise ValueError(f"optim: max_norm must be above 0, got {max_norm}")
 
 
+def _check_options(group: Dict[str, Any]) -> None:
+    """Refuses options of a group that make AdamW another step than this one."""
+    for name in ("amsgrad", "maximize"):
+        if group.get(name):
+            raise ValueError(f"optim: AdamW has no {name}")
+    if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+        raise ValueError("optim: AdamW's weight decay is decoupled from the gradients")
+
+
+def _check_saved(group: Dict[str, Any]) -> None:
+    """Refuses the saved group of another optimizer than this one, ``torch.optim.AdamW``, or an Adam that takes the same steps."""
+    missing = {"lr", "betas", "eps", "weight_decay"} - set(group)
+    if missing or ("maximize" in group and "amsgrad" not in group):
+        raise ValueError(f"optim: a group of another optimizer, with {sorted(group)}")
+    _check_options(group)
+
+
 def _norms(grads: Sequence[Tensor]) -> Tuple[Tensor, Tensor]:
     host = _host.module()
     out = None if host is None else host.grad_norms(grads)
@@ -237,7 +254,8 @@ class AdamW(torch.optim.Optimizer):
     groups together are clipped to this norm, on one device; ``grad_norm`` then is their norm before that in the last step.
     ``lr`` may be a number or, for steps captured into a graph, one fp32 number on the device. For a capture, allocate the
     state before it with ``init_state``. ``load_state_dict`` takes the moments as they were saved; with 32 bits also those of
-    ``torch.optim.AdamW``."""
+    ``torch.optim.AdamW``. ``amsgrad``, ``maximize`` and a weight decay that is part of the gradients, in a group or in a saved
+    one, are refused, as is the state of another optimizer."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, max_norm: Optional[float] = None, state_bits: int = 32) -> None:
@@ -247,6 +265,10 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm, self.state_bits = max_norm, state_bits
         self.grad_norm: Optional[Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, param_group: Dict[str, Any]) -> None:
+        _check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -340,6 +362,8 @@ class AdamW(torch.optim.Optimizer):
         for st in state_dict["state"].values():
             if set(st) != names:
                 raise ValueError(f"optim: the state of a parameter has {sorted(st)}, expected {sorted(names)}")
+        for group in state_dict["param_groups"]:
+            _check_saved(group)
         super().load_state_dict(state_dict)
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         ps = [p for group in self.param_groups for p in group["params"]]

@@ -5,7 +5,10 @@ import os
 import subprocess
 from pathlib import Path
 
-from ebr_amd import block
+import pytest
+import torch
+
+from ebr_amd import block, optim
 
 PLAN = r"""
 #include "glu_plan.hpp"
@@ -50,3 +53,46 @@ def test_gated_projection_of_few_rows_writes_what_its_products_read(tmp_path):
     that leaves it unwritten stands before them."""
     rc, out = _host_program(tmp_path, PLAN)
     assert rc == 0, out
+
+
+def _saved(cls, steps=1, **kw):
+    p = torch.nn.Parameter(torch.ones(6))
+    opt = cls([p], **kw)
+    for _ in range(steps):
+        p.grad = torch.ones(6)
+        opt.step()
+    return opt.state_dict()
+
+
+@pytest.mark.parametrize("steps", [0, 1])
+@pytest.mark.parametrize("cls,kw", [
+    (torch.optim.AdamW, dict(maximize=True)), (torch.optim.AdamW, dict(amsgrad=True)), (torch.optim.Adam, dict(weight_decay=0.1)),
+    (torch.optim.RAdam, {}), (torch.optim.NAdam, {}), (torch.optim.Adamax, {}), (torch.optim.SGD, dict(lr=0.1)),
+])  # fmt: skip
+def test_states_of_other_steps_are_refused(cls, kw, steps):
+    ours = optim.AdamW([torch.nn.Parameter(torch.zeros(6))], lr=3e-4)
+    with pytest.raises(ValueError, match="optim:"):
+        ours.load_state_dict(_saved(cls, steps, **kw))
+    assert ours.param_groups[0]["lr"] == 3e-4 and len(ours.state) == 0
+
+
+@pytest.mark.parametrize("cls,kw", [(torch.optim.AdamW, dict(weight_decay=0.1)), (torch.optim.Adam, {}), (torch.optim.AdamW, dict(foreach=False))])
+def test_states_of_the_same_steps_are_taken(cls, kw):
+    p = torch.nn.Parameter(torch.zeros(6))
+    ours, saved = optim.AdamW([p]), _saved(cls, 2, **kw)
+    for again in (False, True):  # theirs, then ours as it is after that
+        ours.load_state_dict(ours.state_dict() if again else saved)
+        assert int(ours.state[p]["step"]) == 2 and torch.equal(ours.state[p]["exp_avg_sq"], saved["state"][0]["exp_avg_sq"])
+        assert ours.param_groups[0]["weight_decay"] == saved["param_groups"][0]["weight_decay"]
+
+
+def test_groups_of_other_steps_are_refused():
+    p, q = (torch.nn.Parameter(torch.zeros(6)) for _ in range(2))
+    for kw in (dict(maximize=True), dict(amsgrad=True), dict(decoupled_weight_decay=False)):
+        with pytest.raises(ValueError, match="AdamW"):
+            optim.AdamW([dict(params=[p], **kw)])
+        ours = optim.AdamW([p])
+        with pytest.raises(ValueError, match="AdamW"):
+            ours.add_param_group(dict(params=[q], **kw))
+        assert len(ours.param_groups) == 1
+    assert len(optim.AdamW([dict(params=[p], maximize=False), dict(params=[q], lr=1e-4)]).param_groups) == 2
