@@ -364,24 +364,26 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"optim: the state of a parameter has {sorted(st)}, expected {sorted(names)}")
         for group in state_dict["param_groups"]:
             _check_saved(group)
-        super().load_state_dict(state_dict)
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         ps = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, ps):
-            if i not in state_dict["state"]:
-                continue
+        pairs = [(state_dict["state"][i], p) for i, p in zip(ids, ps) if i in state_dict["state"]]
+        for st, p in pairs:
+            for name in names:
+                given = torch.as_tensor(st[name])
+                shape = () if name == "step" else (-(-p.numel() // BLOCK),) if name.endswith("_scale") else p.shape
+                if given.shape != shape and not (name == "step" and given.numel() == 1):
+                    raise ValueError(f"optim: {name} is {tuple(given.shape)}, expected {tuple(shape)}")
+                if name in ("exp_avg", "exp_avg_root") and self.state_bits == 8 and given.dtype != STATE8:
+                    raise TypeError(f"optim: {name} is {given.dtype}, expected {STATE8}")
+        super().load_state_dict(state_dict)
+        for st, p in pairs:
             own = self.state[p]  # torch casts what it loads to the parameter's dtype: the moments have their own
             own.clear()
             for name, fresh in self._state_of(p).items():
-                given = torch.as_tensor(state_dict["state"][i][name])
-                if given.numel() != fresh.numel():
-                    raise ValueError(f"optim: {name} has {given.numel()} elements, expected {fresh.numel()}")
+                given = torch.as_tensor(st[name])
                 if fresh.dtype == STATE8:
-                    if given.dtype != STATE8:
-                        raise TypeError(f"optim: {name} is {given.dtype}, expected {STATE8}")
-                    fresh.view(torch.uint8).copy_(given.view(torch.uint8).reshape(fresh.shape))
-                else:
-                    fresh.copy_(given.reshape(fresh.shape))
+                    fresh, given = fresh.view(torch.uint8), given.view(torch.uint8)
+                fresh.copy_(given.reshape(fresh.shape))
 
 
 __all__ = ["AdamW", "adamw_", "grad_norm"]

@@ -96,3 +96,24 @@ def test_groups_of_other_steps_are_refused():
             ours.add_param_group(dict(params=[q], **kw))
         assert len(ours.param_groups) == 1
     assert len(optim.AdamW([dict(params=[p], maximize=False), dict(params=[q], lr=1e-4)]).param_groups) == 2
+
+
+@pytest.mark.parametrize("error,name,value", [
+    (ValueError, "exp_avg", torch.zeros(3, 2, dtype=torch.uint8).view(optim.STATE8)), (ValueError, "exp_avg_root_scale", torch.zeros(2)), (ValueError, "step", torch.zeros(2)),
+    (TypeError, "exp_avg_root", torch.zeros(2, 3)),
+])  # fmt: skip
+def test_a_refused_state_leaves_the_optimizer_as_it_was(error, name, value):
+    ps = [torch.nn.Parameter(torch.zeros(2, 3)) for _ in range(2)]
+    ours, other = (optim.AdamW(ps, lr=lr, state_bits=8) for lr in (3e-4, 1e-3))
+    for opt, t in ((ours, 5), (other, 7)):
+        opt.init_state()
+        for p in ps:
+            opt.state[p]["step"].fill_(t)
+    saved = other.state_dict()
+    saved["state"][1][name] = value
+    with pytest.raises(error, match="optim:"):
+        ours.load_state_dict(saved)
+    assert ours.param_groups[0]["lr"] == 3e-4 and [int(ours.state[p]["step"]) for p in ps] == [5, 5]
+    saved["state"][1] = saved["state"][0]
+    ours.load_state_dict(saved)
+    assert ours.param_groups[0]["lr"] == 1e-3 and [int(ours.state[p]["step"]) for p in ps] == [7, 7]
