@@ -581,7 +581,8 @@ template <typename T, int VEC, int MODE> static void launch(hipStream_t s, const
     }
 #undef EBR_HELD
     const int64_t tiles = (a.C + 256 * VEC - 1) / (256 * VEC);
-    hipLaunchKernelGGL((k_rows<T, VEC, MODE>), dim3(blocks_for(a.rows, 1)), dim3(WIDE), 0, s, a);
+    const int64_t most = MAX_BLOCKS / (WIDE / 256);  // (it goes on to the rows beyond)
+    hipLaunchKernelGGL((k_rows<T, VEC, MODE>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(WIDE), 0, s, a);
     hipLaunchKernelGGL((k_apply<T, VEC, MODE>), dim3((unsigned)(tiles * p.parts)), dim3(256), 0, s, a);
 }
 

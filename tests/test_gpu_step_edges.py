@@ -6,6 +6,7 @@ import pytest
 import torch
 from test_gpu_swiglu_linear import _check, _forms, _inputs, _say
 
+from ebr_amd import block
 from ebr_amd.fused_attn.loader import hip_library
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,35 @@ def test_gated_projection_carries_both_parts_up_to_64_rows(cuda):
         want, _ = _forms(**ts)
         for k in (1, 2, 3, 5):
             assert float((got[k].double() - want[k]).norm() / want[k].norm()) < 1.9e-3, (I, k)
+
+
+@pytest.mark.parametrize("rows,C,dtype", [((1 << 22) + 5, 6, torch.float64), ((1 << 24) + 5, 2, torch.float64)])
+def test_layer_norm_of_more_rows_than_a_launch_has_workgroups(cuda, rows, C, dtype):
+    """fp64 rows go through workgroups of 1,024 threads, of which a launch holds fewer than 2^22: the same rows again and again give
+    the same bits as once (differences there are off by at most 8 u, times r of at most 317 and a weight below 6). The parameters'
+    sums are off by at most a rounding a row, and 20 of a term's own, of their terms without their signs."""
+    _say(f"layer norm {rows} rows of {C}")
+    g = torch.Generator(cuda).manual_seed(3)
+    few, turns = 4096, -(-rows // 4096)
+    base = {n: torch.randn(few, C, generator=g, device=cuda, dtype=dtype).clamp(-4, 4) for n in ("x", "dy", "u")}
+    w, b = (torch.randn(C, generator=g, device=cuda, dtype=dtype).clamp(-4, 4) for _ in range(2))
+    full = {n: t.repeat(turns, 1)[:rows] for n, t in base.items()}
+    out = []
+    for ts in (base, full):
+        x, p, q = ts["x"].clone().requires_grad_(True), w.clone().requires_grad_(True), b.clone().requires_grad_(True)
+        y = block.layer_norm(x, p, q)
+        dy = ts["dy"].clone().requires_grad_(True)
+        dx, dw, db = torch.autograd.grad(y, (x, p, q), dy, create_graph=True)
+        out.append([t.detach() for t in (y, dx, dw, db, *torch.autograd.grad(dx, (x, dy), ts["u"]))])
+    h = base["x"] - base["x"].mean(1, keepdim=True)
+    h = h / (h.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    assert float((out[0][0] - (w * h + b)).abs().max()) <= 2.0**-53 * 8 * 317 * 6
+    rest = rows - (turns - 1) * few
+    for one, all_ in zip(*out):
+        if one.dim() == 2:
+            assert torch.equal(all_[: (turns - 1) * few].view(-1, few, C), one.expand(turns - 1, few, C))
+            assert torch.equal(all_[-rest:], one[:rest])
+    times = torch.full((few, 1), turns - 1, device=cuda, dtype=dtype)
+    times[:rest] += 1
+    for got, term in ((out[1][2], base["dy"] * h), (out[1][3], base["dy"])):
+        assert bool(((got - (times * term).sum(0)).abs() <= (rows + few + 20) * 2.0**-53 * (times * term.abs()).sum(0)).all())
