@@ -201,6 +201,19 @@ template <typename T> __device__ __forceinline__ void put4(T* p, const float (&v
             if (e < n) p[e] = (T)v[e];
     }
 }
+// The same whatever the alignment, in one access where there are four.
+template <typename T> __device__ __forceinline__ void put4_anywhere(T* p, const float (&v)[4], int64_t n) {
+    T x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (T)v[e];
+    if (n >= 4) {
+        __builtin_memcpy(p, x, sizeof(x));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < n) p[e] = x[e];
+    }
+}
 // What two fours lack of their values once rounded.
 template <typename T>
 __device__ __forceinline__ void put_rest(T* p, const float (&g)[4], const float (&u)[4], int64_t next, int64_t n, bool whole) {
@@ -626,7 +639,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     }
 }
 
-// Few rows of x: the weight, once, straight into registers, bound by its bytes. A workgroup's waves take 16 rows of gate and of
+// Few rows of x: the weight, once, straight into registers, bound by its bytes. x, w and y may have any alignment. A workgroup's waves take 16 rows of gate and of
 // up, and of their k 128 bytes in turns; the order of k within a product is the lanes' own (each brings 16 bytes of its row of
 // either operand), so that a wave's loads take whole lines. The waves' sums are added up through shared memory.
 //
@@ -734,7 +747,8 @@ template <typename T, int EP, int ROWS> __global__ __launch_bounds__(64 * FEW_WA
         else first_of(g[e], u[e], dy[e], og[e], ou[e]);
         if constexpr (TWO) second_of(g[e], u[e], dy[e], cg[e], cu[e], rg[e], ru[e], o[e]);
     }
-    if constexpr (EP != EP_BWD) put4(y + at, o, some, whole);
+    if constexpr (EP == EP_FWD) put4_anywhere(y + at, o, some);
+    if constexpr (EP == EP_BWD2) put4(y + at, o, some, whole);
     const auto both = [&](void* first, void* rest, const float (&vg)[4], const float (&vu)[4]) {
         if (!first) return;
         T* const p = reinterpret_cast<T*>(first) + two;

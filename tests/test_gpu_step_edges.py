@@ -86,3 +86,19 @@ def test_layer_norm_of_more_rows_than_a_launch_has_workgroups(cuda, rows, C, dty
     times[:rest] += 1
     for got, term in ((out[1][2], base["dy"] * h), (out[1][3], base["dy"])):
         assert bool(((got - (times * term).sum(0)).abs() <= (rows + few + 20) * 2.0**-53 * (times * term.abs()).sum(0)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("N,C,I", [(1, 64, 32), (3, 72, 20), (17, 520, 40), (32, 71, 36), (2, 64, 6)])
+def test_gated_projection_of_few_rows_at_any_address(cuda, N, C, I, dtype):
+    """The C entry, whose x, w and y lie off the vectors by one to seven elements: the bits of aligned ones, and nothing beside y."""
+    _say(f"swiglu_linear unaligned {N} {C} {I} {dtype}")
+    ts = _inputs(cuda, N, C, I, dtype, seed=I)
+    y = block.swiglu_linear(ts["x"], ts["w"])
+    for off in (1, 2, 3, 7):
+        x, w = (torch.empty(ts[n].numel() + off, device=cuda, dtype=dtype)[off:].copy_(ts[n].view(-1)) for n in ("x", "w"))
+        out = torch.full((N * I + 16,), -7.0, device=cuda, dtype=dtype)
+        rc = hip_library().ebr_block_swiglu_linear(CODE[dtype], N, C, I, x.data_ptr(), w.data_ptr(), out[off:].data_ptr(), None,
+                                                   torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(out[off : off + N * I].view(N, I), y)
+        assert bool((out[:off] == -7).all()) and bool((out[off + N * I :] == -7).all())
