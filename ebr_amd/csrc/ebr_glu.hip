@@ -493,6 +493,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_product(Args a) {
     constexpr bool GATED = EP >= EP_FWD, TWO = EP == EP_BWD2;
     constexpr bool STAGED = staged(sizeof(T), TI);  // four waves, an array each, or eight, half of one
     static_assert(!STAGED || WAVES == 4 || WAVES == 8, "an array a wave");
+    static_assert(64 * WAVES == product_threads(sizeof(T), TI, TWO ? 2 : GATED), "the threads that sizes are checked for");
     static_assert((!GATED || FI % 2 == 0) && (!TWO || FJ % 2 == 0), "a wave's tile holds both of a pair");
     using SA = Side<T, ALIES, TI, WAVES, GATED>;
     using SB = Side<T, BLIES, TJ, WAVES, TWO>;
@@ -666,7 +667,6 @@ template <> struct Mma16<float> {
         return c;
     }
 };
-constexpr int FEW_WAVES = 8;
 template <typename T, int EP, int ROWS> __global__ __launch_bounds__(64 * FEW_WAVES) void k_few(Args a) {
     constexpr bool TWO = EP == EP_BWD2;
     constexpr int FJ = ROWS * (TWO ? 2 : 1);  // sixteens of x, then of c
@@ -842,16 +842,6 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int 
 
 // -- launches ----------------------------------------------------------------------------------------------------------
 
-static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
-
-static int check(int dtype, int64_t N, int64_t C, int64_t I) {
-    if (!known(dtype)) return EBR_ERR_DTYPE;
-    if (N < 1 || C < 1 || I < 1 || N >= ((int64_t)1 << 31) || C > (1 << 20) - 8 || I > (1 << 19) - 8) return EBR_ERR_SHAPE;
-    const auto tiles = [](int64_t n) { return (n + 63) / 64; };  // (a launch holds fewer than 2^32 threads)
-    const int64_t most = tiles(2 * I) > tiles(C) ? tiles(2 * I) : tiles(C);
-    return tiles(2 * N) * most > MAX_BLOCKS || tiles(2 * I) * tiles(C) > MAX_BLOCKS ? EBR_ERR_SHAPE : EBR_OK;
-}
-
 template <typename T, int ALIES, int BLIES, int EP> static void launch(hipStream_t s, const Cut& c, const Args& a) {
     const dim3 grid((unsigned)(a.count * a.splits));
     if constexpr (std::is_same_v<T, double>) {
@@ -901,10 +891,7 @@ static void join(int dtype, const Cut& c, const Args& a, const float* part, void
     else hipLaunchKernelGGL((k_join<float>), grid, dim3(256), 0, s, a, c.tile, part, (float*)out);
 }
 
-// dx of dgu, and dw of (x, dgu) and, where there is one, a second pair. Of few rows dx has few tiles, and many k: split among
-// workgroups and joined it takes 9.0 us of 81 x 1536 -> 256 (10.8 unsplit); a pass of 4 x 1649 -> 2240 in fp32 to second order, which
-// has two of them, went from 545 us to 325 by it.
-static Cut input_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) { return Cut(dtype, C, N, 2 * I, pairs, 0, FEW_TILES); }
+// dx of dgu, and dw of (x, dgu) and, where there is one, a second pair.
 static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w, Grads dgu, void* dx, float* part, hipStream_t s) {
     Args a = {};
     a.a[0] = a.a[1] = w, a.b[0] = dgu.g, a.b[1] = dgu.rest, a.pairs = dgu.rest ? 2 : 1;
@@ -919,9 +906,6 @@ static void input_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* w
     join(dtype, c, a, part, dx, s);
 }
 
-static Cut weight_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) {
-    return Cut(dtype, C, 2 * I, N, pairs, 0, MANY_K);
-}
 static void weight_grad(int dtype, int64_t N, int64_t C, int64_t I, const void* x, Grads dgu, const void* x2, Grads dgu2, void* dw,
                         float* part, hipStream_t s) {
     Args a = {};
@@ -1002,8 +986,7 @@ struct Padded {
     char* at = nullptr;
     Moves in = {}, out = {};
     Padded(int dtype, int64_t N, int64_t C, int64_t I) : dtype(dtype), N(N), C(C), I(I) {
-        const int64_t per = dtype == EBR_DTYPE_F64 ? 1 : 16 / size_of(dtype);
-        Cp = (C + per - 1) / per * per, Ip = (I + per - 1) / per * per;
+        Cp = padded(dtype, C), Ip = padded(dtype, I);
     }
     bool needed() const { return Cp != C || Ip != I; }
     int64_t bytes(int64_t rows, int64_t cols) const { return up16(rows * cols * size_of(dtype)); }
@@ -1112,7 +1095,7 @@ using namespace ebr_glu;
 extern "C" {
 
 int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t C, int64_t I) {
-    if (check(dtype, N, C, I) || order < 0 || order > 2) return -1;
+    if (order < 0 || order > 2 || check(dtype, order, N, C, I)) return -1;
     if (order == 0 && as_they_are(dtype, N, C)) return 0;
     const Padded p(dtype, N, C, I);
     return own_scratch(dtype, order, N, p.Cp, p.Ip) + p.all(order);
@@ -1120,7 +1103,7 @@ int64_t ebr_block_swiglu_linear_scratch(int dtype, int order, int64_t N, int64_t
 
 int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* scratch,
                             void* stream) {
-    const int rc = check(dtype, N, C, I);
+    const int rc = check(dtype, 0, N, C, I);
     if (rc) return rc;
     if (!x || !w || !y) return EBR_ERR_NULL;
     hipStream_t s = (hipStream_t)stream;
@@ -1144,7 +1127,7 @@ int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const vo
 
 int ebr_block_swiglu_linear_bwd(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
                                 void* dx, void* dw, void* scratch, void* stream) {
-    const int rc = check(dtype, N, C, I);
+    const int rc = check(dtype, 1, N, C, I);
     if (rc) return rc;
     if (!x || !w || !dy) return EBR_ERR_NULL;
     if (!scratch) return EBR_ERR_SCRATCH;
@@ -1166,7 +1149,7 @@ int ebr_block_swiglu_linear_bwd(int dtype, int64_t N, int64_t C, int64_t I, cons
 
 int ebr_block_swiglu_linear_bwd2(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, const void* dy,
                                  const void* c, void* gx, void* gdy, void* gw, void* scratch, void* stream) {
-    const int rc = check(dtype, N, C, I);
+    const int rc = check(dtype, 2, N, C, I);
     if (rc) return rc;
     if (!x || !w || !dy || !c || !gdy) return EBR_ERR_NULL;
     if (!scratch) return EBR_ERR_SCRATCH;

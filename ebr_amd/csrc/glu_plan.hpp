@@ -74,4 +74,47 @@ static Cut gates_cut(int dtype, int order, int64_t N, int64_t C, int64_t I) {
     return Cut(dtype, I, N, C, 1, order == 2 ? 2 : 1, UNSPLIT, order > 0 && with_rest(dtype, N) ? 64 : 256);
 }
 
+// dx of [dg|du]. Of few rows it has few tiles, and many k: split among workgroups and joined it takes 9.0 us of 81 x 1536 -> 256
+// (10.8 unsplit); a pass of 4 x 1649 -> 2240 in fp32 to second order, which has two of them, went from 545 us to 325 by it.
+static Cut input_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) { return Cut(dtype, C, N, 2 * I, pairs, 0, FEW_TILES); }
+
+// dw of the rows of all pairs.
+static Cut weight_cut(int dtype, int64_t N, int64_t C, int64_t I, int pairs) {
+    return Cut(dtype, C, 2 * I, N, pairs, 0, MANY_K);
+}
+
+// Widths up to whole 16-byte chunks, in which the products run.
+static int64_t padded(int dtype, int64_t width) {
+    const int64_t per = dtype == EBR_DTYPE_F64 ? 1 : 16 / size_of(dtype);
+    return (width + per - 1) / per * per;
+}
+
+// Threads of a workgroup of a product's kernel, gated as in Cut.
+constexpr int product_threads(int bytes, int tile, int gated) {
+    return bytes == 8 || tile == 128 ? 256 : tile == 256 ? (gated ? 512 : 256) : gated == 2 ? 64 : 128;
+}
+constexpr int FEW_WAVES = 8;
+
+// Whether every launch of the forward (order 0) or a derivative holds fewer than 2^32 threads, as it has to.
+static bool fits(int dtype, int order, int64_t N, int64_t C, int64_t I) {
+    const auto holds = [](int64_t groups, int threads) { return groups < ((int64_t)1 << 32) / threads; };
+    const auto both = [&](const Cut& c, int gated) {
+        const int threads = product_threads(size_of(dtype), c.tile, gated);
+        const int64_t split = c.tiles() - c.whole;
+        return holds(c.whole, threads) && holds(split * c.splits, threads) && holds(split * (c.tile * c.tile / 1024), 256);
+    };
+    C = padded(dtype, C), I = padded(dtype, I);
+    if (is_few(dtype, N, C) ? !holds((I + 15) / 16, 64 * FEW_WAVES) : !both(gates_cut(dtype, order, N, C, I), order == 2 ? 2 : 1)) return false;
+    const int each = with_rest(dtype, N) ? 2 : 1;
+    return order == 0 || (both(input_cut(dtype, N, C, I, each), 0) && both(weight_cut(dtype, N, C, I, order * each), 0));
+}
+
+static bool known(int d) { return d == EBR_DTYPE_F32 || d == EBR_DTYPE_BF16 || d == EBR_DTYPE_F16 || d == EBR_DTYPE_F64; }
+
+static int check(int dtype, int order, int64_t N, int64_t C, int64_t I) {
+    if (!known(dtype)) return EBR_ERR_DTYPE;
+    if (N < 1 || C < 1 || I < 1 || N >= ((int64_t)1 << 31) || C > (1 << 20) - 8 || I > (1 << 19) - 8) return EBR_ERR_SHAPE;
+    return fits(dtype, order, N, C, I) ? EBR_OK : EBR_ERR_SHAPE;
+}
+
 }  // namespace ebr_glu

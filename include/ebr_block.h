@@ -139,7 +139,8 @@ int ebr_block_layernorm_bwd2(int dtype, int wdtype, int64_t rows, int C, const v
 int64_t ebr_block_layernorm_scratch(int dtype, int order, int64_t rows, int C);
 
 /* y = silu(g) u for x [N, C] and w [2 I, C], gate rows first: g = x w[:I]^T, u = x w[I:]^T, summed in fp32 (fp64 for fp64) and
- * not rounded before y [N, I]; N below 2^31, C up to 2^20 - 8, I up to 2^19 - 8. Tensors (here and below) of any alignment where
+ * not rounded before y [N, I]; N below 2^31, C up to 2^20 - 8, I up to 2^19 - 8, and launches (here and below) of fewer than 2^32
+ * threads: N below 2^30, and N C, N I and 2 C I below 2^36 with each size rounded up to 256, are always within them. Tensors (here and below) of any alignment where
  * C or I is no multiple of 16 bytes, or N at most 32 (y alone), else 16-byte aligned. Scratch of order 0, which may be 0 bytes
  * (and NULL). */
 int ebr_block_swiglu_linear(int dtype, int64_t N, int64_t C, int64_t I, const void* x, const void* w, void* y, void* scratch,

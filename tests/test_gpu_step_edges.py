@@ -102,3 +102,20 @@ def test_gated_projection_of_few_rows_at_any_address(cuda, N, C, I, dtype):
                                                    torch.cuda.current_stream().cuda_stream)
         assert rc == 0 and torch.equal(out[off : off + N * I].view(N, I), y)
         assert bool((out[:off] == -7).all()) and bool((out[off + N * I :] == -7).all())
+
+
+def test_gated_projection_of_more_rows_than_tiles_of_64_fit_a_launch(cuda):
+    """2^29 rows and some, whose tiles of 64 would be too many and whose tiles of 256 are not: the same rows again and again give the
+    same bits as once."""
+    N, few, C, I = (1 << 29) + 64, 4096, 8, 8
+    _say(f"swiglu_linear {N} rows")
+    ts = _inputs(cuda, few, C, I, torch.bfloat16, seed=1)
+    once = _check(*ts.values())
+    x = ts["x"].repeat(N // few + 1, 1)[:N].requires_grad_(True)
+    y = block.swiglu_linear(x, ts["w"])
+    dy = ts["dy"].repeat(N // few + 1, 1)[:N]
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for got, one in ((y.detach(), once[0]), (dx, once[1])):
+        for part in got[: N // few * few].view(8, -1, few, 8):
+            assert torch.equal(part, one.expand(part.shape))
+        assert torch.equal(got[N // few * few :], one[: N % few])

@@ -2,13 +2,14 @@
 plans and arguments. Parity of the kernels there is in ``tests/test_gpu_step_edges.py``."""
 
 import os
+import random
 import subprocess
 from pathlib import Path
 
 import pytest
 import torch
 
-from ebr_amd import block, optim
+from ebr_amd import _capi, block, optim
 
 PLAN = r"""
 #include "glu_plan.hpp"
@@ -117,3 +118,25 @@ def test_a_refused_state_leaves_the_optimizer_as_it_was(error, name, value):
     saved["state"][1] = saved["state"][0]
     ours.load_state_dict(saved)
     assert ours.param_groups[0]["lr"] == 1e-3 and [int(ours.state[p]["step"]) for p in ps] == [7, 7]
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2, 3])
+def test_sizes_that_the_gated_projection_takes(dtype):
+    """What the header says is always taken is, and what would be a launch of 2^32 threads and more is not."""
+    lib, rng = _capi.load(), random.Random(dtype)
+
+    def up(n):
+        return (n + 255) // 256 * 256
+
+    seen = 0
+    for _ in range(20000):
+        N, C, I = (int(2 ** rng.uniform(0, bits)) for bits in (30, 20, 19))
+        C, I = min(C, (1 << 20) - 8), min(I, (1 << 19) - 8)
+        if N < 1 << 30 and max(up(N) * up(C), up(N) * up(I), 2 * up(C) * up(I)) < 1 << 36:
+            seen += 1
+            assert all(lib.ebr_block_swiglu_linear_scratch(dtype, order, N, C, I) >= 0 for order in range(3)), (N, C, I)
+    assert seen > 1000
+    for N, C, I in ((2_000_000, 2048, 11008), ((1 << 29) + 64, 8, 8), (33, 16384, 1 << 16)):
+        assert all(lib.ebr_block_swiglu_linear_scratch(dtype, order, N, C, I) >= 0 for order in range(3)), (N, C, I)
+    for N, C, I in (((1 << 31) - 1, 8, 1 << 18), ((1 << 31) - 1, 8, 512), ((1 << 30) + 1, (1 << 20) - 8, (1 << 19) - 8)):
+        assert all(lib.ebr_block_swiglu_linear_scratch(dtype, order, N, C, I) == -1 for order in range(3)), (N, C, I)
