@@ -1577,7 +1577,7 @@ bool adamw(const py::sequence& hp, const py::sequence& hg, const py::sequence& h
            const py::sequence& hs, const py::object& hscales, double lr, const py::handle& hlr, double beta1, double beta2,
            double eps, double decay, const py::handle& hnorm, double max_norm) {
     const size_t n = hp.size();
-    if (!plain_context() || n == 0) return false;
+    if (!plain_context() || n == 0 || ebr_block_adamw_scratch((int64_t)n) < 0) return false;
     const Tensor first = plain(hp[0]);
     if (!first.defined()) return false;
     const bool eight = !hscales.is_none();

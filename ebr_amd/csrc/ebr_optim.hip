@@ -587,7 +587,7 @@ int ebr_block_grad_norm(int64_t count, const ebr_optim_grad* grads, double* norm
 }
 
 int64_t ebr_block_adamw_scratch(int64_t count) {
-    return count < 0 || count >= ((int64_t)1 << 31) ? -1 : count * (int64_t)sizeof(Factors) + 16;
+    return count < 0 || count > MAX_BLOCKS ? -1 : count * (int64_t)sizeof(Factors) + 16;
 }
 
 int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_optim_tensor* tensors, double lr,
@@ -617,7 +617,7 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
     hipStream_t s = (hipStream_t)stream;
     Factors* factors = reinterpret_cast<Factors*>(scratch);
     int64_t per = per_step(total, bits);
-    while (total / per + count > MAX_BLOCKS) per *= 2;
+    while (total / per + TENSORS > MAX_BLOCKS) per *= 2;  // (of a launch)
     for (int64_t i = 0; i < count; i += TENSORS, factors += TENSORS) {
         Table a = {};
         Prepare pre = {};

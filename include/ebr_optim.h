@@ -46,7 +46,7 @@ int ebr_block_grad_norm(int64_t count, const ebr_optim_grad* grads, double* norm
                         void* stream);
 int64_t ebr_block_grad_norm_scratch(int64_t count, const ebr_optim_grad* grads);
 
-/* One AdamW step of count tensors, whose parameters are of ptype and gradients of gtype (ptype, or a 16-bit type with fp32
+/* One AdamW step of count tensors (fewer than 2^24, and 2^40 elements), whose parameters are of ptype and gradients of gtype (ptype, or a 16-bit type with fp32
  * parameters), bits 32 or 8 (fp64: 32). With t the step's number, counted from 1:
  *   g <- g min(1, max_norm / (norm[0] + 1e-6))   where norm is not NULL: of all the gradients, as the call above leaves it
  *   m <- beta1 m + (1 - beta1) g,   v <- beta2 v + (1 - beta2) g^2

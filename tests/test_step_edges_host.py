@@ -140,3 +140,11 @@ def test_sizes_that_the_gated_projection_takes(dtype):
         assert all(lib.ebr_block_swiglu_linear_scratch(dtype, order, N, C, I) >= 0 for order in range(3)), (N, C, I)
     for N, C, I in (((1 << 31) - 1, 8, 1 << 18), ((1 << 31) - 1, 8, 512), ((1 << 30) + 1, (1 << 20) - 8, (1 << 19) - 8)):
         assert all(lib.ebr_block_swiglu_linear_scratch(dtype, order, N, C, I) == -1 for order in range(3)), (N, C, I)
+
+
+def test_more_tensors_than_a_step_takes():
+    lib = _capi.load()
+    assert lib.ebr_block_adamw_scratch((1 << 24) - 1) > 0
+    for count in (1 << 24, (1 << 31) - 1, 1 << 40):
+        assert lib.ebr_block_adamw_scratch(count) == -1
+        assert lib.ebr_block_adamw(0, 0, 32, count, None, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, None, 0.0, None, None) == 2
