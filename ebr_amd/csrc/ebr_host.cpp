@@ -1630,10 +1630,17 @@ bool adamw(const py::sequence& hp, const py::sequence& hg, const py::sequence& h
     std::sort(written.begin(), written.end());
     for (size_t i = 1; i < written.size(); ++i)
         if (written[i].first < written[i - 1].second) return false;  // two that share memory
+    const auto meets = [&](const Tensor& x) {
+        const char* const from = static_cast<const char*>(x.data_ptr());
+        const auto next = std::lower_bound(written.begin(), written.end(), std::pair<const char*, const char*>(from + x.nbytes(), nullptr));
+        return x.numel() > 0 && next != written.begin() && (next - 1)->second > from;
+    };
+    for (size_t i = 0; i < n; ++i)  // (as a step on its own parameter's elements it reads before it writes)
+        if (meets(g[i]) && !(g[i].data_ptr() == p[i].data_ptr() && g[i].scalar_type() == p[i].scalar_type())) return false;
     Tensor lr_dev, norm;
     if (!hlr.is_none()) {
         lr_dev = plain(hlr);
-        if (!lr_dev.defined()) return false;
+        if (!lr_dev.defined() || meets(lr_dev)) return false;
     }
     if (!hnorm.is_none()) {
         norm = plain(hnorm);

@@ -517,9 +517,11 @@ template <typename P, typename G> static void step(hipStream_t s, int bits, unsi
     hipLaunchKernelGGL((k_adamw<P, G>), dim3(blocks), dim3(THREADS), 0, s, a);
 }
 
-// Whether any two of the tensors that are written share memory.
-static bool twice(int64_t count, const ebr_optim_tensor* t, int64_t pbytes, int bits) {
-    std::vector<std::pair<uintptr_t, uintptr_t>> at;
+using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;  // of addresses, the end past the last
+
+// The memory that a step writes, in order of address.
+static Ranges written(int64_t count, const ebr_optim_tensor* t, int64_t pbytes, int bits) {
+    Ranges at;
     at.reserve(count * (bits == 8 ? 6 : 4));
     const auto add = [&](const void* p, int64_t bytes) {
         if (bytes > 0) at.emplace_back((uintptr_t)p, (uintptr_t)p + bytes);
@@ -529,10 +531,21 @@ static bool twice(int64_t count, const ebr_optim_tensor* t, int64_t pbytes, int 
         add(t[i].p, n * pbytes), add(t[i].m, held), add(t[i].v, held), add(t[i].ms, scales), add(t[i].vs, scales), add(t[i].step, 8);
     }
     std::sort(at.begin(), at.end());
+    return at;
+}
+// Whether any two of them share memory.
+static bool twice(const Ranges& at) {
     for (size_t i = 1; i < at.size(); ++i)
         if (at[i].first < at[i - 1].second) return true;
     return false;
 }
+// Whether ``bytes`` from p on do with one of them, no two of which do.
+static bool meets(const Ranges& at, const void* p, int64_t bytes) {
+    const auto next = std::lower_bound(at.begin(), at.end(), std::pair<uintptr_t, uintptr_t>((uintptr_t)p + bytes, 0));
+    return p && bytes > 0 && next != at.begin() && (next - 1)->second > (uintptr_t)p;
+}
+
+static int64_t bytes_of(int dtype) { return dtype == EBR_DTYPE_F64 ? 8 : dtype == EBR_DTYPE_F32 ? 4 : 2; }
 
 }  // namespace ebr_opt
 
@@ -607,13 +620,20 @@ int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_opt
         if (t.n < 0 || t.n >= TOO_MANY || (total += t.n) >= TOO_MANY) return EBR_ERR_SHAPE;
         if (!t.step || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || (bits == 8 && (!t.ms || !t.vs))))) return EBR_ERR_NULL;
     }
+    Ranges at;
     try {
-        if (twice(count, tensors, ptype == EBR_DTYPE_F64 ? 8 : ptype == EBR_DTYPE_F32 ? 4 : 2, bits)) return EBR_ERR_SHAPE;
+        at = written(count, tensors, bytes_of(ptype), bits);
     } catch (const std::bad_alloc&) {
         return EBR_ERR_HIP_BASE + (int)hipErrorOutOfMemory;
     }
+    if (twice(at)) return EBR_ERR_SHAPE;
     if (!scratch) return EBR_ERR_SCRATCH;
     if (!aligned(scratch, 16)) return EBR_ERR_ALIGN;
+    // what is read: a gradient may be its parameter, element by element
+    bool met = meets(at, lr_dev, 4) || meets(at, norm, 8) || meets(at, scratch, ebr_block_adamw_scratch(count));
+    for (int64_t i = 0; i < count && !met; ++i)
+        met = !(tensors[i].g == tensors[i].p && gtype == ptype) && meets(at, tensors[i].g, tensors[i].n * bytes_of(gtype));
+    if (met) return EBR_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     Factors* factors = reinterpret_cast<Factors*>(scratch);
     int64_t per = per_step(total, bits);

@@ -12,6 +12,7 @@ Ops (``torch.ops.ebr_fused.*``, HIP device only; a missing library raises): ``gr
 """
 
 # No ``from __future__ import annotations``: custom_op schema inference needs real type objects.
+import bisect
 import ctypes
 import math
 from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
@@ -64,7 +65,7 @@ def adamw_op(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequen
              beta2: float, eps: float, weight_decay: float, norm: Optional[Tensor], max_norm: float) -> None:
     """A step; scales: the first moments' and then the roots' in turn for each parameter, or none."""
     lib = hip_library()
-    _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, list(zip(scales[::2], scales[1::2])) or None)
+    _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, list(zip(scales[::2], scales[1::2])) or None, lr_dev)
     grads = [g.contiguous() for g in grads]
     kinds: Dict[Any, List[int]] = {}
     for i, (p, g) in enumerate(zip(params, grads)):
@@ -97,7 +98,7 @@ def _check_grads(grads: Sequence[Tensor]) -> None:
             raise ValueError(f"optim: gradients are on {grads[0].device} and {g.device}: one device a step")
 
 
-def _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, scales) -> None:
+def _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, scales, lr) -> None:
     n = len(params)
     lists = (("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs), ("steps", steps), ("scales", scales))
     for name, ts in lists:
@@ -136,9 +137,20 @@ def _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, scales) -> None:
         if len(set(at)) < len(at):
             raise ValueError(f"optim: the same {name} twice in one step")
     written = [x for ts in (params, exp_avgs, exp_avg_sqs, steps, *(scales or ())) for x in ts if x.numel() > 0]
-    ends = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in written)
+    ends = sorted(_range(x) for x in written)
     if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
         raise ValueError("optim: two of the tensors that a step writes share memory")
+    read = [g for p, g in zip(params, grads) if g.numel() > 0 and g.is_contiguous() and _range(g) != _range(p)]
+    for x in read + ([lr] if isinstance(lr, Tensor) else []):
+        start, end = _range(x)
+        at = bisect.bisect_left(ends, (end,))
+        if at > 0 and ends[at - 1][1] > start:
+            raise ValueError("optim: a step writes to a gradient or to its lr")
+
+
+def _range(x: Tensor) -> Tuple[int, int]:
+    """The addresses of a contiguous tensor, the end past its last."""
+    return x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()
 
 
 def _check_numbers(lr, betas, eps, weight_decay, max_norm, device=None) -> None:
@@ -199,7 +211,7 @@ def _launch(params, grads, exp_avgs, exp_avg_sqs, steps, scales, lr, betas, eps,
     if host is not None and host.adamw(params, grads, exp_avgs, exp_avg_sqs, steps, scales, number, lr_dev, betas[0], betas[1],
                                        eps, weight_decay, norm, clip):
         return
-    _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, scales)
+    _check_step(params, grads, exp_avgs, exp_avg_sqs, steps, scales, lr)
     with torch.no_grad():
         torch.ops.ebr_fused.adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps),
                                   [s for pair in scales or () for s in pair], number, lr_dev, betas[0], betas[1], eps,
@@ -218,10 +230,12 @@ def adamw_(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence
 
     Parameters are fp32, bfloat16, float16 or fp64; gradients of the same dtype, or 16-bit with fp32 parameters. ``exp_avgs``
     and ``exp_avg_sqs`` (m and v) are fp32 (fp64 for fp64), ``steps`` one int64 each. ``lr`` is a number or one fp32 number on
-    the device. With ``scales``, moments are in 8 bits: ``exp_avgs`` holds m and ``exp_avg_sqs`` the root of v as
-    float8_e4m3fn, and scales[k] is a pair of fp32 vectors, a scale for each 256 consecutive elements, that the numbers are
-    multiplied with. They are rounded up or down in turn over the steps, in proportion to what lies on either side
-    (``include/ebr_optim.h`` states the rule), so that small changes add up."""
+    the device. What a step writes shares no memory with anything else of it, but a gradient may be its own parameter.
+
+    With ``scales``, moments are in 8 bits: ``exp_avgs`` holds m and ``exp_avg_sqs`` the root of v as float8_e4m3fn, and scales[k]
+    is a pair of fp32 vectors, a scale for each 256 consecutive elements, that the numbers are multiplied with. They are rounded
+    up or down in turn over the steps, in proportion to what lies on either side (``include/ebr_optim.h`` states the rule), so
+    that small changes add up."""
     _check_numbers(lr, betas, eps, weight_decay, max_norm, params[0].device if len(params) else None)
     norm, single = (None, None) if max_norm is None else _norms(grads)
     _launch(params, grads, exp_avgs, exp_avg_sqs, steps, scales, lr, betas, eps, weight_decay, norm, max_norm)

@@ -57,7 +57,8 @@ int64_t ebr_block_grad_norm_scratch(int64_t count, const ebr_optim_grad* grads);
  * number y = moment / scale between two neighbours k s and (k + 1) s becomes floor(y / s + t) s, with t in [0, 1) the 24 upper
  * bits of (i * 0x85EBCA77 + step * 0x9E3779B1) mod 2^32 for the first moment, and of that plus 2^31 for the root: over the
  * steps t takes its values evenly, so that nothing is lost on average and no number stays where it is for good. A root above
- * 0 never becomes 0. scratch: ebr_block_adamw_scratch bytes, 16-byte aligned. No two tensors share a parameter or a step. */
+ * 0 never becomes 0. scratch: ebr_block_adamw_scratch bytes, 16-byte aligned. No two of the
+ * tensors that are written share memory, nor does what is read with them (but a gradient may be its own parameter). */
 int ebr_block_adamw(int ptype, int gtype, int bits, int64_t count, const ebr_optim_tensor* tensors, double lr,
                     const float* lr_dev, double beta1, double beta2, double eps, double decay, const double* norm,
                     double max_norm, void* scratch, void* stream);

@@ -6,7 +6,7 @@ import pytest
 import torch
 from test_gpu_swiglu_linear import _check, _forms, _inputs, _say
 
-from ebr_amd import block
+from ebr_amd import block, optim
 from ebr_amd.fused_attn.loader import hip_library
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +119,28 @@ def test_gated_projection_of_more_rows_than_tiles_of_64_fit_a_launch(cuda):
         for part in got[: N // few * few].view(8, -1, few, 8):
             assert torch.equal(part, one.expand(part.shape))
         assert torch.equal(got[N // few * few :], one[: N % few])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_gradient_that_is_its_parameter(cuda, bits):
+    """The bits of a step on a copy; a gradient in another's parameter is refused before anything is written."""
+    _say(f"adamw on its own parameter {bits}")
+    g = torch.Generator(cuda).manual_seed(1)
+    start = [torch.randn(n, generator=g, device=cuda) for n in (5, 3001)]
+    out = []
+    for copied in (False, True):
+        p = [t.clone() for t in start]
+        kind = optim.STATE8 if bits == 8 else torch.float32
+        m, v = ([torch.zeros(t.numel() * kind.itemsize, device=cuda, dtype=torch.uint8).view(kind) for t in p] for _ in range(2))
+        s = [torch.zeros((), device=cuda, dtype=torch.int64) for _ in p]
+        scales = [tuple(torch.zeros(-(-t.numel() // 256), device=cuda) for _ in range(2)) for t in p] if bits == 8 else None
+        for _ in range(3):
+            optim.adamw_(p, [t.clone() for t in p] if copied else p, m, v, s, lr=0.1, max_norm=1.0, scales=scales)
+        out.append([*p, *m, *v, *s])
+    held = [t.clone() for t in out[0][:2]]
+    for grads, lr in (([p[0], p[1].clone()], p[1][7]), ([p[1][:5], p[1].clone()], 0.1)):
+        with pytest.raises(ValueError, match="writes to a gradient"):
+            optim.adamw_(p, grads, m, v, s, lr=lr, scales=scales)
+    assert all(torch.equal(a, b) for a, b in zip(p, held))
+    for a, b in zip(*out):
+        assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)

@@ -1,6 +1,7 @@
 """Host-side checks, no GPU, of what the layer norm, the gated projection and the optimizer's step do next to the borders of their
 plans and arguments. Parity of the kernels there is in ``tests/test_gpu_step_edges.py``."""
 
+import ctypes
 import os
 import random
 import subprocess
@@ -148,3 +149,34 @@ def test_more_tensors_than_a_step_takes():
     for count in (1 << 24, (1 << 31) - 1, 1 << 40):
         assert lib.ebr_block_adamw_scratch(count) == -1
         assert lib.ebr_block_adamw(0, 0, 32, count, None, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, None, 0.0, None, None) == 2
+
+
+def _step(params, grads, lr=1e-3, **kw):
+    zeros = [[torch.zeros(p.shape) for p in params] for _ in range(2)]
+    steps = [torch.zeros((), dtype=torch.int64) for _ in params]
+    return optim.adamw_(params, grads, *zeros, steps, lr=lr, **kw)
+
+
+def test_a_step_that_writes_to_what_it_reads():
+    """A gradient in another's parameter, or a place further on in its own, would be read before or after it is written, as it comes."""
+    both = torch.zeros(12)
+    p, q, r = both[:4], both[4:8], torch.zeros(4)
+    for params, grads in (((p, q), (r, p)), ((p, q), (both[2:6], r)), ((p, q), (both[1:5], r)), ((p, q), (r, both[7:11]))):
+        with pytest.raises(ValueError, match="writes to a gradient"):
+            _step(params, grads)
+    with pytest.raises(ValueError, match="its lr"):
+        _step((p, q), (r, r), lr=both[5])
+    for grads in ((p, r), (r, both[8:]), (both.view(4, 3)[:, 0], r)):  # its own, one beside, and one that is copied: no kernel off the GPU
+        with pytest.raises(NotImplementedError):
+            _step((p, q), grads)
+
+
+@pytest.mark.parametrize("kw", [dict(g=0x101000), dict(g=0x100004), dict(lr=0x100018), dict(norm=0x102010), dict(scratch=0x101FF0)])
+def test_adamw_entry_refuses_to_write_to_what_it_reads(kw):
+    at = 0x100000
+    rows = [(at + 4096 * k, kw.get("g", 0x200000), at + 4096 * (2 + k), at + 4096 * (4 + k), 0, 0, at + 4096 * 6 + 8 * k, 1000)
+            for k in range(2)]
+    table = (_capi.OptimTensor * 2)(*rows)
+    rc = _capi.load().ebr_block_adamw(0, 0, 32, 2, ctypes.addressof(table), 1e-3, kw.get("lr"), 0.9, 0.99, 1e-8, 0.0, kw.get("norm"),
+                                      1.0, kw.get("scratch", 0x300000), None)
+    assert rc == 2
