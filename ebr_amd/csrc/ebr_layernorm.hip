@@ -574,16 +574,18 @@ template <typename T, int VEC, int MODE> static void launch(hipStream_t s, const
         return;                                                                                                      \
     }
     if constexpr (sizeof(T) < 8 && VEC == 1) {
-        EBR_HELD(16, 1)
-    } else if constexpr (sizeof(T) < 8) {
-        EBR_HELD(16, 8) EBR_HELD(32, 8) EBR_HELD(64, 8) EBR_HELD(64, 16) EBR_HELD(64, 24) EBR_HELD(64, 32)
-        EBR_HELD(256, 8) EBR_HELD(256, 16) EBR_HELD(256, 24) EBR_HELD(256, 32) EBR_HELD(1024, 8) EBR_HELD(1024, 16)
+        EBR_HELD(16, 1)  // (rows of fewer elements than a vector)
+    } else {
+        if constexpr (sizeof(T) < 8) {
+            EBR_HELD(16, 8) EBR_HELD(32, 8) EBR_HELD(64, 8) EBR_HELD(64, 16) EBR_HELD(64, 24) EBR_HELD(64, 32)
+            EBR_HELD(256, 16) EBR_HELD(256, 24) EBR_HELD(256, 32) EBR_HELD(1024, 16)
+        }
+        const int64_t tiles = (a.C + 256 * VEC - 1) / (256 * VEC);
+        const int64_t most = MAX_BLOCKS / (WIDE / 256);  // (it goes on to the rows beyond)
+        hipLaunchKernelGGL((k_rows<T, VEC, MODE>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(WIDE), 0, s, a);
+        hipLaunchKernelGGL((k_apply<T, VEC, MODE>), dim3((unsigned)(tiles * p.parts)), dim3(256), 0, s, a);
     }
 #undef EBR_HELD
-    const int64_t tiles = (a.C + 256 * VEC - 1) / (256 * VEC);
-    const int64_t most = MAX_BLOCKS / (WIDE / 256);  // (it goes on to the rows beyond)
-    hipLaunchKernelGGL((k_rows<T, VEC, MODE>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(WIDE), 0, s, a);
-    hipLaunchKernelGGL((k_apply<T, VEC, MODE>), dim3((unsigned)(tiles * p.parts)), dim3(256), 0, s, a);
 }
 
 template <int MODE> static int run(int dtype, Args a, void* dw, void* db, void* scratch, void* stream) {
