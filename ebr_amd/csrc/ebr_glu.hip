@@ -844,19 +844,25 @@ template <typename T> __global__ __launch_bounds__(256) void k_join(Args a, int 
 
 template <typename T, int ALIES, int BLIES, int EP> static void launch(hipStream_t s, const Cut& c, const Args& a) {
     const dim3 grid((unsigned)(a.count * a.splits));
+    // (fp64 is not split; of few tiles alone dx is: of 64)
+    constexpr bool SMALL = EP == EP_PART && ALIES == M_ROWS && BLIES == K_ROWS;
     if constexpr (std::is_same_v<T, double>) {
-        hipLaunchKernelGGL((k_product64<ALIES, BLIES, EP>), grid, dim3(256), 0, s, a);
+        if constexpr (EP != EP_PART) hipLaunchKernelGGL((k_product64<ALIES, BLIES, EP>), grid, dim3(256), 0, s, a);
     } else {
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2 && !SMALL) {
             if (c.tile == 256) {
                 constexpr int WJ = EP >= EP_FWD ? 4 : 2;
                 hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 256, 256, 2, WJ>), grid, dim3(128 * WJ), 0, s, a);
                 return;
             }
         }
-        if (c.tile == 128) hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 128, 128, 2, 2>), grid, dim3(256), 0, s, a);
-        else if constexpr (EP == EP_BWD2)
-            hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 1>), grid, dim3(64), 0, s, a);
+        if constexpr (!SMALL) {
+            if (c.tile == 128) {
+                hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 128, 128, 2, 2>), grid, dim3(256), 0, s, a);
+                return;
+            }
+        }
+        if constexpr (EP == EP_BWD2) hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 1>), grid, dim3(64), 0, s, a);
         else hipLaunchKernelGGL((k_product<T, ALIES, BLIES, EP, 64, 64, 1, 2>), grid, dim3(128), 0, s, a);
     }
 }

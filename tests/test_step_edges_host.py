@@ -180,3 +180,42 @@ def test_adamw_entry_refuses_to_write_to_what_it_reads(kw):
     rc = _capi.load().ebr_block_adamw(0, 0, 32, 2, ctypes.addressof(table), 1e-3, kw.get("lr"), 0.9, 0.99, 1e-8, 0.0, kw.get("norm"),
                                       1.0, kw.get("scratch", 0x300000), None)
     assert rc == 2
+
+
+CUTS = r"""
+#include "glu_plan.hpp"
+#include <cmath>
+#include <cstdio>
+#include <random>
+#include <set>
+#include <string>
+using namespace ebr_glu;
+int main() {
+    std::mt19937_64 rng(1);
+    const auto size = [&](double bits) { return (int64_t)std::exp2(std::uniform_real_distribution<double>(0, bits)(rng)); };
+    std::set<std::string> seen;
+    for (int k = 0; k < 3000000; ++k) {
+        const int dtype = k % 4, order = 1 + k / 4 % 2;
+        const int64_t N = size(22), C = padded(dtype, size(14)), I = padded(dtype, size(15));
+        const int each = with_rest(dtype, N) ? 2 : 1, bytes = size_of(dtype);
+        const Cut in = input_cut(dtype, N, C, I, each), w = weight_cut(dtype, N, C, I, order * each);
+        const auto say = [&](const char* what, int tile) { seen.insert(std::to_string(bytes) + what + std::to_string(tile)); };
+        for (int o = 0; o < 3; ++o)
+            if (!is_few(dtype, N, C)) say(o == 0 ? " forward " : o == 1 ? " first " : " second ", gates_cut(dtype, o, N, C, I).tile);
+        if (in.whole) say(" dx ", in.tile);
+        if (in.splits > 1) say(" dx split ", in.tile);
+        if (w.whole) say(" dw ", w.tile);
+        if (w.splits > 1) say(" dw split ", w.tile);
+    }
+    for (const std::string& s : seen) std::puts(s.c_str());
+}
+"""
+
+
+def test_the_gated_projection_s_kernels_are_all_taken(tmp_path):
+    """Every tile of every product is some size's, and no size takes another."""
+    rc, out = _host_program(tmp_path, CUTS)
+    want = {"8 forward 64", "8 first 64", "8 second 64", "8 dx 64", "8 dw 64", "4 dx split 64", "2 dx split 64"}
+    for bytes, tiles in ((4, (64, 128)), (2, (64, 128, 256))):
+        want |= {f"{bytes} {p} {t}" for t in tiles for p in ("forward", "first", "second", "dx", "dw", "dw split")}
+    assert rc == 0 and set(out.splitlines()) == want
