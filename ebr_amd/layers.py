@@ -114,7 +114,8 @@ def swiglu_intermediate(hidden_size: int, expansion: float) -> int:
 class SwiGLU(nn.Module):
     """down(silu(gate) * up) with gate, up the halves of one projection; ``impl="fused"`` runs the activation (and its
     first and second derivatives) as one HIP kernel each (``ebr_amd.block.swiglu``), ``impl="projected"`` the projection
-    with the activation in it (``ebr_amd.block.swiglu_linear``)."""
+    with the activation in it (``ebr_amd.block.swiglu_linear``, with weight gradients of its own: ``gate_up_proj`` gives its weight
+    and is not called, unless it has hooks, for which the projection and the activation are taken apart)."""
 
     def __init__(self, hidden_size: int, expansion: float, impl: str = "eager") -> None:
         super().__init__()
@@ -133,7 +134,10 @@ class SwiGLU(nn.Module):
         if self.impl == "projected":
             from ebr_amd import block
 
-            return self.down_proj(block.swiglu_linear(x, self.gate_up_proj.weight.to(x.dtype)))
+            at = self.gate_up_proj
+            if at._forward_hooks or at._forward_pre_hooks or at._backward_hooks or at._backward_pre_hooks:  # they want its call
+                return self.down_proj(block.swiglu(at(x)))
+            return self.down_proj(block.swiglu_linear(x, at.weight.to(x.dtype)))
         gate, up = self.gate_up_proj(x).chunk(2, dim=-1)
         return self.down_proj(F.silu(gate) * up)
 

@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from ebr_amd import _capi, block, optim
+from ebr_amd import _capi, block, layers, optim
 
 PLAN = r"""
 #include "glu_plan.hpp"
@@ -219,3 +219,28 @@ def test_the_gated_projection_s_kernels_are_all_taken(tmp_path):
     for bytes, tiles in ((4, (64, 128)), (2, (64, 128, 256))):
         want |= {f"{bytes} {p} {t}" for t in tiles for p in ("forward", "first", "second", "dx", "dw", "dw split")}
     assert rc == 0 and set(out.splitlines()) == want
+
+
+def test_hooks_of_the_projection_run(monkeypatch):
+    """``impl="projected"`` takes the projection's weight alone, but where the module has hooks it is called."""
+
+    def plain(gu):
+        gate, up = gu.chunk(2, -1)
+        return torch.nn.functional.silu(gate) * up
+
+    monkeypatch.setattr(block, "swiglu", plain)
+    monkeypatch.setattr(block, "swiglu_linear", lambda x, w: plain(x @ w.t()))
+    net, x, seen = layers.SwiGLU(8, 2.0, impl="projected"), torch.randn(3, 8), []
+    want = net(x)
+    at = net.gate_up_proj
+    for put in (lambda: at.register_forward_hook(lambda m, i, o: seen.append("after")),
+                lambda: at.register_forward_pre_hook(lambda m, i: seen.append("before")),
+                lambda: at.register_full_backward_hook(lambda m, i, o: seen.append("backward")),
+                lambda: at.register_full_backward_pre_hook(lambda m, o: seen.append("before backward"))):
+        handle = put()
+        y = net(x.clone().requires_grad_(True))
+        y.sum().backward()
+        assert torch.allclose(y, want)
+        handle.remove()
+        assert torch.allclose(net(x), want)
+    assert seen == ["after", "before", "backward", "before backward"]
