@@ -1337,7 +1337,6 @@ struct LayerNormBwd : Function<LayerNormBwd> {
         const auto pt = param_type(x, w, b);
         ctx->save_for_backward({x, w, stats, dy});
         ctx->saved_data["type"] = (int64_t)dtype_code(pt);
-        ctx->saved_data["has_b"] = b.defined();
         ctx->saved_data["want_w"] = want_w;
         ctx->saved_data["want_b"] = want_b;
         ctx->set_materialize_grads(false);
