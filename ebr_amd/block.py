@@ -14,8 +14,8 @@ training loss differentiates it again).
 Ops (``torch.ops.ebr_fused.*``, HIP device only; a missing library raises): ``block_rmsnorm``, ``block_rmsnorm_bwd``,
 ``block_rmsnorm_bwd2``, ``block_swiglu``, ``block_swiglu_bwd``, ``block_swiglu_bwd2``, ``block_groupnorm``,
 ``block_groupnorm_bwd``, ``block_groupnorm_bwd2``, ``block_layernorm``, ``block_layernorm_bwd``, ``block_layernorm_bwd2``,
-``block_swiglu_linear``, ``block_swiglu_linear_bwd``, ``block_swiglu_linear_bwd2``. Autograd: each op's backward is the next op, so the functions are differentiable to second order; the second backward is not itself
-differentiable. The arithmetic is fp32 (fp64 for fp64 tensors), each output rounded once to the dtype where eager
+``block_swiglu_linear``, ``block_swiglu_linear_bwd``, ``block_swiglu_linear_bwd2``. Autograd: each op's backward is the next
+op, so the functions are differentiable to second order; the second backward is not itself differentiable. The arithmetic is fp32 (fp64 for fp64 tensors), each output rounded once to the dtype where eager
 autograd chains several rounded kernels, so 16-bit results differ from eager by rounding only.
 """
 
@@ -964,8 +964,11 @@ def _swiglu_linear_dx_grads(x, w, dy, c, want_x, want_w):
 
 def swiglu_linear(x: Tensor, weight: Tensor) -> Tensor:
     """``swiglu(x @ weight.T)`` for x [..., C] and a weight [2 I, C] of its dtype, the gate's rows first: both projections,
-    the activation and the product in one kernel, [..., I]. The projections are summed in fp32 (fp64 for fp64) and never
-    rounded or kept: the derivatives take them again from x. Differentiable twice."""
+    the activation and the product in one kernel, [..., I]. The projections are summed in fp32 (fp64 for fp64) and not rounded
+    or kept: the derivatives take them again from x. Differentiable twice. In 16 bits the projections' gradients are rounded as
+    operands of the products that follow (of up to 64 rows what they lack goes with them). Under ``create_graph`` with the
+    weight's gradient wanted, the gradients are those of ``linear`` and ``swiglu``, which have derivatives for the weight too and
+    round the projections to x's dtype."""
     host = None if torch.compiler.is_compiling() else _host.module()
     y = None if host is None else host.swiglu_linear(x, weight)
     if y is not None:

@@ -8,8 +8,13 @@
 //   dx = [dg|du] W    A = W (M), B = [dg|du] (K)
 //   dW = [dg|du]^T x  A = x (M), B = [dg|du] (M), the rows split among workgroups, partial sums added up in a fixed order
 //
-// The derivatives take g and u again: kept rounded they would double the gradients' errors, and of C below about a thousand
-// the product costs less than moving them.
+// The derivatives take g and u again: kept rounded they would double the gradients' errors, and kept in fp32 their product costs
+// less than moving them for C below about a thousand (above it, 8192 x 2048 -> 5632, 403 us against some 145 for 369 MB written and
+// read, but nothing has to be held from the forward to the backward).
+//
+// [dg|du] and [gg|gu] are rounded to the type, as the matrix instructions take them: in 16 bits the gradients are 2.3e-3 off in
+// the mean square, where the rounding of the outputs alone makes 1.7e-3. Of up to 64 rows, whose products wait for the weight's bytes
+// in any case, what the rounding leaves goes in as a second operand; of more, it would double dx's and dw's products.
 //
 // A workgroup's tile of TI x TJ steps through k in stages of 64 bytes an operand row, loaded straight into shared memory three
 // stages ahead. The four buffers are separate arrays: the compiler then knows that the loads under way do not concern the

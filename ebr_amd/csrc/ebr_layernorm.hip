@@ -14,7 +14,7 @@
 // Bound by memory: 62,208 rows of 256 in bf16 take 13.3 us forward, 17.8 backward and 31 in the second (4.8, 5.4 and 5.1 TB/s),
 // 16,384 of 2048 23.5 and 42 (5.7 and 4.8 TB/s; a copy of this size goes at 5 to 7). A row stays in the registers of TPR threads
 // between its sums and its outputs, so every tensor is read once; rows too wide for a workgroup, and fp64, go through k_rows and
-// k_apply, which read them twice. The parameters' sums stay in the registers of the threads that hold the columns, over all rows
+// k_apply, which read them twice (1000 x 40000: 68 us forward and 84 backward in bf16, 102 and 167 in fp32). The parameters' sums stay in the registers of the threads that hold the columns, over all rows
 // of a workgroup, then go through one partial a workgroup to k_params: always in the same order.
 #include <type_traits>
 
