@@ -15,6 +15,7 @@ Ops (``torch.ops.ebr_fused.*``, HIP device only; a missing library raises): ``gr
 import bisect
 import ctypes
 import math
+from collections import OrderedDict
 from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -370,6 +371,12 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
+        # hooks run here: torch's turn would be between its copies and the moments as they are kept
+        before, after = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        state_dict = state_dict.copy()
+        for hook in before.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         names = {"step", "exp_avg", "exp_avg_sq"}
         if self.state_bits == 8:
             names = {"step", "exp_avg", "exp_avg_root", "exp_avg_scale", "exp_avg_root_scale"}
@@ -389,7 +396,11 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"optim: {name} is {tuple(given.shape)}, expected {tuple(shape)}")
                 if name in ("exp_avg", "exp_avg_root") and self.state_bits == 8 and given.dtype != STATE8:
                     raise TypeError(f"optim: {name} is {given.dtype}, expected {STATE8}")
-        super().load_state_dict(state_dict)
+        self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = OrderedDict(), OrderedDict()
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = before, after
         for st, p in pairs:
             own = self.state[p]  # torch casts what it loads to the parameter's dtype: the moments have their own
             own.clear()
@@ -398,6 +409,8 @@ class AdamW(torch.optim.Optimizer):
                 if fresh.dtype == STATE8:
                     fresh, given = fresh.view(torch.uint8), given.view(torch.uint8)
                 fresh.copy_(given.reshape(fresh.shape))
+        for hook in after.values():
+            hook(self)
 
 
 __all__ = ["AdamW", "adamw_", "grad_norm"]

@@ -244,3 +244,22 @@ def test_hooks_of_the_projection_run(monkeypatch):
         handle.remove()
         assert torch.allclose(net(x), want)
     assert seen == ["after", "before", "backward", "before backward"]
+
+
+def test_hooks_of_a_load_see_and_change_what_is_loaded():
+    """What a hook gives in a saved state's place is what is loaded, once; a hook that follows finds the moments as they are kept."""
+    p = torch.nn.Parameter(torch.zeros(6, dtype=torch.bfloat16))
+    ours, saved, seen = optim.AdamW([p]), _saved(torch.optim.AdamW, 2), []
+
+    def wider(opt, state_dict):
+        state = {k: dict(st, exp_avg=st["exp_avg"] + 2.0**-20) for k, st in state_dict["state"].items()}
+        seen.append("before")
+        return dict(state_dict, state=state)
+
+    ours.register_load_state_dict_pre_hook(wider)
+    ours.register_load_state_dict_post_hook(lambda opt: seen.append(opt.state[p]["exp_avg"].clone()))
+    for _ in range(2):
+        ours.load_state_dict(saved)
+    want = saved["state"][0]["exp_avg"] + 2.0**-20
+    assert seen[0] == seen[2] == "before" and len(seen) == 4
+    assert torch.equal(seen[1], want) and torch.equal(seen[3], want) and torch.equal(ours.state[p]["exp_avg"], want)
