@@ -144,3 +144,21 @@ def test_a_gradient_that_is_its_parameter(cuda, bits):
     assert all(torch.equal(a, b) for a, b in zip(p, held))
     for a, b in zip(*out):
         assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+
+@pytest.mark.parametrize("N,C,I", [(5, 72, 40), (6, 71, 41), (48, 72, 12744), (48, 264, 40), (200, 136, 264), (700, 264, 1032), (9000, 520, 1032)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gated_projection_s_gradients_alone(cuda, N, C, I, dtype):
+    """What is wanted alone has the bits that it has beside the rest."""
+    _say(f"swiglu_linear wanted alone {N} {C} {I} {dtype}")
+    x, w, dy, c = _inputs(cuda, N, C, I, dtype, seed=N).values()
+    ops = torch.ops.ebr_fused
+    dx, dw = ops.block_swiglu_linear_bwd(x, w, dy, True, True)
+    assert torch.equal(ops.block_swiglu_linear_bwd(x, w, dy, True, False)[0], dx)
+    assert torch.equal(ops.block_swiglu_linear_bwd(x, w, dy, False, True)[1], dw)
+    gx, gdy, gw = ops.block_swiglu_linear_bwd2(x, w, dy, c, True, True)
+    for want_x, want_w in ((True, False), (False, True), (False, False)):
+        a = ops.block_swiglu_linear_bwd2(x, w, dy, c, want_x, want_w)
+        assert torch.equal(a[1], gdy)
+        assert torch.equal(a[0], gx) if want_x else a[0].numel() == 0
+        assert torch.equal(a[2], gw) if want_w else a[2].numel() == 0
